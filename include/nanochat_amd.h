@@ -171,6 +171,18 @@ int nc_qk_norm_rope_append_fp8(const void *qkv, long long token_stride, int B, i
                                const int32_t *block_table, int max_pages, void *k_pages, void *v_pages,
                                float *kv_scale, int num_pages, void *stream);
 
+/*
+ * nc_qk_norm_rope_append_fp8 for packed rows, any number a sequence: row n of qkv (bf16 [rows][(Hq + 2 Hkv) 128] at
+ * token_stride elements) is the token at position positions[n] and its K and V go to cache slot slot_map[n] = 16 page +
+ * position % 16 (int32 [rows]; nc_pages_extend makes both), with the same bits; q goes to q_out (bf16 [rows][Hq][128]). A
+ * row whose slot lies outside [0, 16 num_pages) or whose position lies outside [0, rope_len) is skipped: its q_out row
+ * stays as it was. The slots of one call must differ. rows < 2^28, num_pages <= (2^31 - 1) / 16; no rows launch nothing.
+ */
+int nc_qk_norm_rope_append_rows_fp8(const void *qkv, long long token_stride, long long rows, int Hq, int Hkv,
+                                    const int32_t *positions, const int32_t *slot_map, const float *q_gain,
+                                    const float *k_gain, const float *cos, const float *sin, int rope_len, void *q_out,
+                                    void *k_pages, void *v_pages, float *kv_scale, int num_pages, void *stream);
+
 /* Workspace bytes nc_decode_attn_fp8 and nc_decode_step_fp8 need for these sizes (0 for unsupported sizes): fp32
  * partial results from its start and, in its last 1/256, one int32 arrival count per (sequence, KV head). The
  * workspace must be zero-filled before its first call and passed with the same workspace_bytes to every call: the
@@ -248,6 +260,29 @@ int nc_prefill_attn_fp8(const void *q, const void *k_pages, const void *v_pages,
                         const int32_t *block_table, int max_pages, int num_pages,
                         const int32_t *start_pos, int B, int T, int Hq, int Hkv, int window, float sm_scale,
                         void *out, void *stream);
+
+/*
+ * The page bookkeeping of `slots` (<= 4096) sequences over one pool, kept on the device; no counterpart in the reference
+ * (its slots own fixed caches, model/kernels/decode.cu:740-763). State: lengths int32 [slots], table int32
+ * [slots][max_pages] (-1: no page), free_pages int32 [num_pages] whose first free_count[0] entries are free. arrived: one
+ * int32, zero before the first call and left zero by every call. Calls on one state must be ordered. num_pages and
+ * max_pages are at most (2^31 - 1) / 16.
+ *
+ * nc_pages_extend: slot b asks for new_tokens[b] tokens, all or nothing (negative, or past max_pages * 16: none). In slot
+ * order, slots get pages while the pool has enough (a slot that needs no page is not refused for pages), then rows while
+ * `rows` suffice. The j-th page granted is free_pages[free_count - 1 - j]. Slot b's tokens become rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 (cu_seqlens int32 [slots + 1]) at positions lengths[b] ..; positions, slot_map int32 [rows]: a
+ * row's position and its cache slot 16 page + position % 16, both -1 past the last row; granted int32 [slots]. lengths,
+ * table and free_count are updated.
+ *
+ * nc_pages_trim: slot b longer than keep[b] >= 0 falls back to keep[b] tokens; the pages past them leave the table (-1)
+ * and join the free list, the first of them (in slot, then page order) topmost.
+ */
+int nc_pages_extend(const int32_t *new_tokens, int slots, int32_t *lengths, int32_t *table, int max_pages,
+                    const int32_t *free_pages, int32_t *free_count, int num_pages, int rows, int32_t *cu_seqlens,
+                    int32_t *positions, int32_t *slot_map, int32_t *granted, int32_t *arrived, void *stream);
+int nc_pages_trim(const int32_t *keep, int slots, int32_t *lengths, int32_t *table, int max_pages, int32_t *free_pages,
+                  int32_t *free_count, int num_pages, int32_t *arrived, void *stream);
 
 /*
  * Measurement only; no counterpart in the reference. Reads n pages of 2 KiB (one (page, head) of K or V codes) from

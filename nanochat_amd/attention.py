@@ -18,7 +18,7 @@ import torch
 
 from .config import HEAD_DIM
 from .kv_cache import PagedKVCache, _require
-from .native import check, hip_library, pointer, stream
+from .native import check, device_guard, hip_library, pointer, stream
 
 
 def qk_norm_rope_append(qkv: torch.Tensor, num_q_heads: int, cache: PagedKVCache, block_table: torch.Tensor,
@@ -52,6 +52,55 @@ def qk_norm_rope_append(qkv: torch.Tensor, num_q_heads: int, cache: PagedKVCache
         pointer(num_new) if num_new is not None else None, pointer(q_gain), pointer(k_gain), pointer(cos),
         pointer(sin), cos.size(0), pointer(q_out), pointer(block_table), block_table.size(1),
         pointer(cache.k_pages), pointer(cache.v_pages), pointer(cache.kv_scale), cache.num_pages, stream()))
+    return q_out
+
+
+def _same_device(device: torch.device, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def qk_norm_rope_append_packed(qkv: torch.Tensor, num_q_heads: int, cache: PagedKVCache, positions: torch.Tensor,
+                               slot_map: torch.Tensor, q_gain: torch.Tensor, k_gain: torch.Tensor, cos: torch.Tensor,
+                               sin: torch.Tensor, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """qk_norm_rope_append for packed rows, any number a sequence: qkv bf16 [rows, (Hq + 2 Hkv) * 128] (rows contiguous,
+    any row stride) -> q bf16 [rows, Hq, 128] normed and rotated; k (normed, rotated) and v are quantized into cache slot
+    slot_map[n] = 16 page + position % 16 of the token at positions[n] (int32 [rows], as paging.BlockTables.extend makes
+    them). A row whose slot lies outside the cache or whose position lies outside the rotary table (padding: -1) is
+    skipped, its row of q left as it was. The slots of one call must differ."""
+    if qkv.dim() != 2:
+        raise ValueError("qkv must be [rows, (Hq + 2 Hkv) * 128]")
+    rows, W = qkv.shape
+    Hkv = cache.num_kv_heads
+    if num_q_heads < 1 or W != (num_q_heads + 2 * Hkv) * HEAD_DIM:
+        raise ValueError(f"qkv width {W} != (Hq + 2 Hkv) * {HEAD_DIM} = {(num_q_heads + 2 * Hkv) * HEAD_DIM}")
+    if qkv.dtype != torch.bfloat16 or not qkv.is_cuda or qkv.stride(1) != 1 or (rows > 1 and qkv.stride(0) < W):
+        raise ValueError("qkv must be a bf16 device tensor with contiguous rows that do not overlap")
+    for name, t in (("q_gain", q_gain), ("k_gain", k_gain), ("cos", cos), ("sin", sin)):
+        _require(t, name, torch.float32)
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.size(0) < 1 or cos.size(1) != HEAD_DIM // 2:
+        raise ValueError("cos, sin must be [positions, 64]")
+    if q_gain.numel() != HEAD_DIM or k_gain.numel() != HEAD_DIM:
+        raise ValueError(f"q_gain, k_gain must be [{HEAD_DIM}]")
+    for name, t in (("positions", positions), ("slot_map", slot_map)):
+        _require(t, name, torch.int32)
+        if t.shape != (rows,):
+            raise ValueError(f"{name} must be [{rows}], got {tuple(t.shape)}")
+    if q_out is None:
+        q_out = torch.empty(rows, num_q_heads, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device)
+    _require(q_out, "q_out", torch.bfloat16)
+    if q_out.shape != (rows, num_q_heads, HEAD_DIM):
+        raise ValueError(f"q_out must be [{rows}, {num_q_heads}, {HEAD_DIM}]")
+    _same_device(qkv.device, cache=cache.k_pages, positions=positions, slot_map=slot_map, q_gain=q_gain, k_gain=k_gain,
+                 cos=cos, sin=sin, q_out=q_out)
+    if rows == 0:
+        return q_out
+    with device_guard(qkv):
+        check(hip_library().nc_qk_norm_rope_append_rows_fp8(
+            pointer(qkv), qkv.stride(0) if rows > 1 else W, rows, num_q_heads, Hkv, pointer(positions), pointer(slot_map),
+            pointer(q_gain), pointer(k_gain), pointer(cos), pointer(sin), cos.size(0), pointer(q_out),
+            pointer(cache.k_pages), pointer(cache.v_pages), pointer(cache.kv_scale), cache.num_pages, stream()))
     return q_out
 
 

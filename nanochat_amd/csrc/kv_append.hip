@@ -164,6 +164,133 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
     }
 }
 
+/* The fused append of packed rows by slot map: row n (of `rows`) is one token at position positions[n], its K and V go
+ * to cache slot slot_map[n] = 16 page + slot; a row whose slot lies outside the pool or whose position lies outside
+ * [0, rope_len) is skipped. Row math and bits are append_kernel's.
+ *
+ * Grid x = blocks of 16 consecutive rows, 16 lanes a row; y < Hkv: KV head y; y >= Hkv: q heads 4 (y - Hkv) .. + 3. A K
+ * row's codes are eight 16-byte blocks of its page, stored whole. A V block holds four slots of 16 dims: rows r .. r + 3 of
+ * the block of rows that sit in slots 4 g .. 4 g + 3 of one page (a quad, found from the slot map alone) store whole
+ * blocks, other rows their single bytes: the rows of different sequences in a decoding step, and up to three rows at
+ * either end of a block of rows whose position is not its row modulo 4. */
+struct AppendRowsArgs {
+    const uint16_t *qkv;       /* [rows][(Hq + 2 Hkv) 128] at token_stride */
+    long long token_stride;
+    int rows, Hq, Hkv;
+    const int32_t *positions, *slot_map;
+    const float *q_gain, *k_gain, *cos, *sin;
+    int rope_len;
+    uint16_t *q_out;           /* [rows][Hq][128] */
+    uint8_t *k_pages, *v_pages;
+    float *kv_scale;
+    int num_slots;             /* 16 num_pages */
+};
+
+constexpr int VROW_PITCH = 20;   /* bytes between dims of the V image: 16 rows and a spare dword, so two aligned dwords
+                                    hold any four consecutive rows */
+
+__global__ void __launch_bounds__(256) append_rows_kernel(AppendRowsArgs a) {
+    __shared__ __align__(16) uint8_t kimg[PAGE][HEAD_DIM];
+    __shared__ __align__(16) uint8_t vimg[HEAD_DIM][VROW_PITCH];
+    __shared__ float img_scale[2][PAGE];
+    __shared__ int slots[PAGE];
+    const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x >> 6;
+    const int i = lane & 15, r = 4 * wave + (lane >> 4);   /* the lane's place in its row, its row of the 16 */
+    const long long n = (long long)blockIdx.x * PAGE + r, tok = min(n, (long long)a.rows - 1);
+    int slot = a.slot_map[tok], p = a.positions[tok];
+    const bool live = n < a.rows && (unsigned)slot < (unsigned)a.num_slots && (unsigned)p < (unsigned)a.rope_len;
+    if (!live) p = 0, slot = -1;
+
+    if ((int)blockIdx.y >= a.Hkv) {
+        const int h0 = Q_GROUP * ((int)blockIdx.y - a.Hkv);
+        const uint16_t *row = a.qkv + tok * a.token_stride + h0 * HEAD_DIM;
+        uint4 raw[Q_GROUP];
+        float g[8], c[4], s[4];
+#pragma unroll
+        for (int j = 0; j < Q_GROUP; j++)
+            if (h0 + j < a.Hq) raw[j] = load_row16(row + j * HEAD_DIM, i);
+        load4_f32(a.cos + (long long)p * HALF + 4 * i, c);
+        load4_f32(a.sin + (long long)p * HALF + 4 * i, s);
+        load_gain16(a.q_gain, i, g);
+        uint16_t *q = a.q_out + (tok * a.Hq + h0) * HEAD_DIM;
+#pragma unroll
+        for (int j = 0; j < Q_GROUP; j++) {
+            if (h0 + j >= a.Hq) break;
+            float x[8], y[8];
+            unpack8(raw[j], x);
+            norm_rope16(x, g, c, s, y);
+            if (live) store_row16(q + j * HEAD_DIM, i, y);
+        }
+        return;
+    }
+
+    const int kvh = blockIdx.y;
+    const uint16_t *kx = a.qkv + tok * a.token_stride + (a.Hq + kvh) * HEAD_DIM;
+    const uint4 kraw = load_row16(kx, i), vraw = load_row16(kx + a.Hkv * HEAD_DIM, i);
+    float x[8], y[8], g[8], c[4], s[4];
+    load4_f32(a.cos + (long long)p * HALF + 4 * i, c);
+    load4_f32(a.sin + (long long)p * HALF + 4 * i, s);
+    load_gain16(a.k_gain, i, g);
+    unpack8(kraw, x);
+    norm_rope16(x, g, c, s, y);
+    unpack8(pack8(y), x);
+    uint32_t code[2];
+    float scale = quantize16(x, code);
+    *reinterpret_cast<uint32_t *>(&kimg[r][4 * i]) = code[0];
+    *reinterpret_cast<uint32_t *>(&kimg[r][HALF + 4 * i]) = code[1];
+    if (i == 0) {
+        img_scale[0][r] = scale;
+        slots[r] = slot;
+    }
+    unpack8(vraw, x);
+    scale = quantize16(x, code);
+#pragma unroll
+    for (int e = 0; e < 8; e++) vimg[(e < 4 ? 4 * i : HALF + 4 * i) + (e & 3)][r] = (uint8_t)(code[e >> 2] >> (8 * (e & 3)));
+    if (i == 0) img_scale[1][r] = scale;
+    __syncthreads();
+
+    /* the block's quads: bit r of `lead` where rows r .. r + 3 fill slots 4 g .. 4 g + 3 of a page */
+    const int mine = slots[lane & 15];
+    bool quad = mine >= 0 && (mine & 3) == 0 && (lane & 15) + 3 < PAGE;
+#pragma unroll
+    for (int k = 1; k < 4; k++) quad = quad && slots[min((lane & 15) + k, PAGE - 1)] == mine + k;
+    const uint32_t lead = (uint32_t)__ballot(quad) & 0xFFFFu;
+    const uint32_t live_rows = (uint32_t)__ballot(mine >= 0) & 0xFFFFu;
+    const int t = threadIdx.x & 127;
+    if (threadIdx.x < 128) {   /* K: row t / 8, its 16 bytes of dims 16 (t % 8) .. + 15 */
+        const int kr = t >> 3, d0 = 16 * (t & 7), sl = slots[kr];
+        if (sl >= 0) {
+            uint8_t *dst = a.k_pages + ((long long)(sl / PAGE) * a.Hkv + kvh) * PAGE_BYTES + k_page_offset(sl % PAGE, d0);
+            *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(&kimg[kr][d0]);
+        }
+    } else {                   /* V: 32 threads a quad, block t % 32 of it */
+        uint32_t left = lead;
+        for (int k = t >> 5; k > 0 && left; k--) left &= left - 1;
+        if (left) {
+            const int r0 = __ffs(left) - 1, sl = slots[r0], half = (t & 31) >> 4, d0 = 64 * half + (t & 15);
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {   /* dims d0 + 16 k: rows r0 .. r0 + 3, at any byte of two aligned dwords */
+                const uint32_t *v = reinterpret_cast<const uint32_t *>(&vimg[d0 + 16 * k][r0 & ~3]);
+                w[k] = __builtin_amdgcn_alignbyte(v[1], v[0], r0 & 3);
+            }
+            uint8_t *dst = a.v_pages + ((long long)(sl / PAGE) * a.Hkv + kvh) * PAGE_BYTES + v_page_offset(sl % PAGE, d0);
+            *reinterpret_cast<uint4 *>(dst) = uint4{w[0], w[1], w[2], w[3]};
+        }
+    }
+    uint32_t single = live_rows & ~(lead | lead << 1 | lead << 2 | lead << 3);
+    for (; single; single &= single - 1) {
+        const int vr = __ffs(single) - 1, sl = slots[vr];
+        if (threadIdx.x >= 128)
+            a.v_pages[((long long)(sl / PAGE) * a.Hkv + kvh) * PAGE_BYTES + v_page_offset(sl % PAGE, t)] = vimg[t][vr];
+    }
+    if (threadIdx.x < 2 * PAGE) {
+        const int kv = threadIdx.x >> 4, sl = slots[threadIdx.x & 15];
+        if (sl >= 0)
+            a.kv_scale[(((long long)(sl / PAGE) * a.Hkv + kvh) * 2 + kv) * PAGE + sl % PAGE] = img_scale[kv][threadIdx.x & 15];
+    }
+}
+
 /* The training-form prologue (reference model/kernels/qk_prologue.cu:8-32) of q's and k's [tokens][H] rows: input
  * token stride 3 H 128, output contiguous, position p % T for token p.
  *
@@ -391,6 +518,31 @@ extern "C" int nc_qk_norm_rope_append_fp8(const void *qkv, long long token_strid
     a.k_pages = (uint8_t *)k_pages; a.v_pages = (uint8_t *)v_pages;
     a.kv_scale = kv_scale; a.num_pages = num_pages;
     return launch_append(a, true, (hipStream_t)stream);
+}
+
+extern "C" int nc_qk_norm_rope_append_rows_fp8(const void *qkv, long long token_stride, long long rows, int Hq, int Hkv,
+                                               const int32_t *positions, const int32_t *slot_map, const float *q_gain,
+                                               const float *k_gain, const float *cos, const float *sin, int rope_len,
+                                               void *q_out, void *k_pages, void *v_pages, float *kv_scale, int num_pages,
+                                               void *stream) {
+    if (!qkv || !positions || !slot_map || !q_gain || !k_gain || !cos || !sin || !q_out || !k_pages || !v_pages || !kv_scale)
+        return NC_ERR_NULL;
+    if (rows < 0 || rows >= 1LL << 28 || Hq <= 0 || Hkv <= 0 || Hq > 32768 || Hkv > 32768 || num_pages <= 0 ||
+        num_pages > 0x7FFFFFFF / PAGE || rope_len <= 0 || token_stride < (long long)(Hq + 2 * Hkv) * HEAD_DIM)
+        return NC_ERR_SHAPE;
+    if (rows == 0) return NC_OK;
+    AppendRowsArgs a = {};
+    a.qkv = (const uint16_t *)qkv;
+    a.token_stride = token_stride;
+    a.rows = (int)rows; a.Hq = Hq; a.Hkv = Hkv;
+    a.positions = positions; a.slot_map = slot_map;
+    a.q_gain = q_gain; a.k_gain = k_gain; a.cos = cos; a.sin = sin; a.rope_len = rope_len;
+    a.q_out = (uint16_t *)q_out;
+    a.k_pages = (uint8_t *)k_pages; a.v_pages = (uint8_t *)v_pages; a.kv_scale = kv_scale;
+    a.num_slots = num_pages * PAGE;
+    const dim3 grid((unsigned)((rows + PAGE - 1) / PAGE), (unsigned)(Hkv + (Hq + Q_GROUP - 1) / Q_GROUP));
+    hipLaunchKernelGGL(append_rows_kernel, grid, dim3(256), 0, (hipStream_t)stream, a);
+    return (int)hipGetLastError();
 }
 
 extern "C" int qkp_backward_blocks() { return QKB_BLOCKS; }

@@ -1,0 +1,247 @@
+/*
+ * The page bookkeeping of a server's slots on the GPU: a step's tokens get pages, positions and cache slots from the
+ * requests' lengths, and pages go back to the free list when a slot shrinks. The block tables, lengths and free list live
+ * in device memory and no call reads them back, so a step that uses them can be captured into a graph. (The reference's
+ * slots own fixed contiguous caches, model/kernels/decode.cu:740-763, and need none of this.)
+ *
+ * Both kernels are one launch and bound by latency: a chain of the slots' loads, two prefix sums over the slots, and one
+ * round of loads and stores for the rows. Every workgroup computes the prefix sums for itself in LDS (4,096 slots at
+ * most), then takes its share of the rows (or freed pages). The state itself is written by the workgroup that arrives
+ * last: by then every other one has read it.
+ */
+#include "nc_device.h"
+#include "nanochat_amd.h"
+
+namespace nc {
+
+constexpr int PG_THREADS = 256;
+constexpr int PG_WAVES = PG_THREADS / WAVE;
+constexpr int PG_MAX_SLOTS = 4096;
+
+__device__ __forceinline__ int pages_of(int length) { return (int)(((unsigned)length + PAGE - 1) / PAGE); }
+
+/* Exclusive prefix sum of one value a thread over the workgroup. Every thread must call it. */
+__device__ __forceinline__ long long block_exclusive(long long v, long long (&part)[PG_WAVES]) {
+    const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x >> 6;
+    long long s = v;
+#pragma unroll
+    for (int o = 1; o < WAVE; o <<= 1) {
+        const long long t = __shfl_up(s, o, WAVE);
+        if (lane >= o) s += t;
+    }
+    __syncthreads();   /* the sums of the call before this one are read */
+    if (lane == WAVE - 1) part[wave] = s;
+    __syncthreads();
+    long long before = 0;
+#pragma unroll
+    for (int w = 0; w < PG_WAVES; w++) before += w < wave ? part[w] : 0;
+    return before + s - v;
+}
+
+/* The last b in [0, n) with cum[b] <= k; cum is non-decreasing and cum[0] = 0 <= k. */
+__device__ __forceinline__ int last_at_most(const int *cum, int n, int k) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cum[mid] <= k) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+/* Whether this workgroup is the last of the launch to arrive; the count returns to zero. Every thread must call it. What
+ * the workgroup loaded before it arrived has been used by then, so the last one may overwrite it: relaxed order is enough
+ * (nothing that one workgroup stores is read by another). */
+__device__ __forceinline__ bool last_block(int *arrived) {
+    __shared__ int last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+        if (last) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return last;
+}
+
+struct PagesArgs {
+    const int32_t *asked;      /* extend: new tokens; trim: lengths to keep */
+    int slots;
+    int32_t *lengths, *table;
+    int max_pages;
+    int32_t *free_pages, *free_count;
+    int num_pages, rows;
+    int32_t *cu_seqlens, *positions, *slot_map, *granted;
+    int *arrived;
+};
+
+/* LDS: cu [slots + 1], first [slots + 1] (granted rows and pages of the slots before), old [slots]. */
+__global__ void __launch_bounds__(PG_THREADS) pages_extend_kernel(PagesArgs a) {
+    extern __shared__ int pg_lds[];
+    __shared__ long long part[PG_WAVES];
+    int *cu = pg_lds, *first = cu + a.slots + 1, *old = first + a.slots + 1;
+    const int per = (a.slots + PG_THREADS - 1) / PG_THREADS;
+    const int b0 = min((int)threadIdx.x * per, a.slots), b1 = min(b0 + per, a.slots);
+    const int count = min(max(*a.free_count, 0), a.num_pages);
+    const long long cap = min((long long)a.max_pages * PAGE, 0x7FFFFFFFLL);
+
+    /* what each slot asks: its tokens (0 where its length would pass the table's row) and the pages they need */
+    long long pages = 0;
+    for (int b = b0; b < b1; b++) {
+        const int len = a.lengths[b];
+        long long n = max(a.asked[b], 0);
+        if (len < 0 || len + n > cap) n = 0;
+        old[b] = len;
+        cu[b] = (int)n;
+        pages += n > 0 ? pages_of(len + (int)n) - pages_of(len) : 0;
+    }
+    long long at = block_exclusive(pages, part);
+    /* pages in slot order, as long as they last; a slot that needs none is not refused */
+    long long tokens = 0;
+    for (int b = b0; b < b1; b++) {
+        const int n = cu[b], need = n > 0 ? pages_of(old[b] + n) - pages_of(old[b]) : 0;
+        at += need;
+        if (need > 0 && at > count) cu[b] = 0;
+        tokens += cu[b];
+    }
+    /* then rows in slot order, as long as they last. What is granted before a slot is a prefix of what was asked, so
+     * its sums have no gaps; a refused slot's own entries are never looked up */
+    long long row = block_exclusive(tokens, part);
+    int given = 0, need_given = 0;
+    for (int b = b0; b < b1; b++) {
+        const int n = cu[b];
+        row += n;
+        if (row > a.rows) cu[b] = 0;
+        given += cu[b];
+        need_given += cu[b] ? pages_of(old[b] + cu[b]) - pages_of(old[b]) : 0;
+    }
+    int cu_at = (int)block_exclusive(given, part), page_at = (int)block_exclusive(need_given, part);
+    for (int b = b0; b < b1; b++) {
+        const int n = cu[b], need = n ? pages_of(old[b] + n) - pages_of(old[b]) : 0;
+        cu[b] = cu_at;
+        first[b] = page_at;
+        cu_at += n;
+        page_at += need;
+        if (blockIdx.x == 0) a.granted[b] = n;
+    }
+    if (b1 == a.slots && b0 < b1) {   /* the thread of the last slot */
+        cu[a.slots] = cu_at;
+        first[a.slots] = page_at;
+    }
+    __syncthreads();
+    const int total = cu[a.slots];
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= a.slots; b += PG_THREADS) a.cu_seqlens[b] = cu[b];
+
+    for (long long r64 = (long long)blockIdx.x * PG_THREADS + threadIdx.x; r64 < a.rows;
+         r64 += (long long)gridDim.x * PG_THREADS) {
+        const int r = (int)r64;
+        int p = -1, slot = -1;
+        if (r < total) {
+            const int b = last_at_most(cu, a.slots, r);
+            p = old[b] + r - cu[b];
+            const int lp = p / PAGE, fresh = lp - pages_of(old[b]);
+            int32_t *entry = a.table + (long long)b * a.max_pages + lp;
+            int page;
+            if (fresh >= 0) {
+                page = a.free_pages[count - 1 - first[b] - fresh];
+                if (p % PAGE == 0) *entry = page;   /* a granted page's first position is a new row */
+            } else {
+                page = *entry;
+            }
+            slot = (unsigned)page < (unsigned)a.num_pages ? page * PAGE + p % PAGE : -1;
+        }
+        a.positions[r] = p;
+        a.slot_map[r] = slot;
+    }
+    if (!last_block(a.arrived)) return;
+    for (int b = threadIdx.x; b < a.slots; b += PG_THREADS)
+        if (cu[b + 1] != cu[b]) a.lengths[b] = old[b] + cu[b + 1] - cu[b];
+    if (threadIdx.x == 0) *a.free_count = count - first[a.slots];
+}
+
+/* LDS: gone [slots + 1] (freed pages of the slots before), from [slots] (each slot's first freed page). The pages join
+ * the free list so that the first one freed ends up topmost: a trim that undoes an extend restores the list. */
+__global__ void __launch_bounds__(PG_THREADS) pages_trim_kernel(PagesArgs a) {
+    extern __shared__ int pg_lds[];
+    __shared__ long long part[PG_WAVES];
+    int *gone = pg_lds, *from = gone + a.slots + 1;
+    const int per = (a.slots + PG_THREADS - 1) / PG_THREADS;
+    const int b0 = min((int)threadIdx.x * per, a.slots), b1 = min(b0 + per, a.slots);
+    const int count = min(max(*a.free_count, 0), a.num_pages);
+    long long freed = 0;
+    for (int b = b0; b < b1; b++) {
+        const int len = a.lengths[b], keep = a.asked[b];
+        const int held = min(pages_of(max(len, 0)), a.max_pages);
+        const int kept = keep >= 0 && keep < len ? min(pages_of(keep), held) : held;
+        from[b] = kept;
+        gone[b] = held - kept;
+        freed += held - kept;
+    }
+    /* more pages than the pool holds cannot be held by consistent tables; what would pass the list's end is dropped */
+    long long at = block_exclusive(freed, part);
+    for (int b = b0; b < b1; b++) {
+        const int n = gone[b];
+        gone[b] = (int)min(at, (long long)a.num_pages);
+        at += n;
+    }
+    if (b1 == a.slots && b0 < b1) gone[a.slots] = (int)min(at, (long long)a.num_pages);
+    __syncthreads();
+    const int total = min(gone[a.slots], a.num_pages - count);
+    for (long long j64 = (long long)blockIdx.x * PG_THREADS + threadIdx.x; j64 < total;
+         j64 += (long long)gridDim.x * PG_THREADS) {
+        const int j = (int)j64, b = last_at_most(gone, a.slots, j);
+        int32_t *entry = a.table + (long long)b * a.max_pages + from[b] + j - gone[b];
+        a.free_pages[count + total - 1 - j] = *entry;
+        *entry = -1;
+    }
+    if (!last_block(a.arrived)) return;
+    for (int b = threadIdx.x; b < a.slots; b += PG_THREADS) {
+        const int keep = a.asked[b];
+        if (keep >= 0 && keep < a.lengths[b]) a.lengths[b] = keep;
+    }
+    if (threadIdx.x == 0) *a.free_count = count + total;
+}
+
+static int pages_check(int slots, int max_pages, int num_pages) {
+    /* a cache slot (16 num_pages of them) and a position fit an int32 */
+    if (slots <= 0 || slots > PG_MAX_SLOTS || max_pages <= 0 || num_pages <= 0 || num_pages > 0x7FFFFFFF / PAGE ||
+        max_pages > 0x7FFFFFFF / PAGE)
+        return NC_ERR_SHAPE;
+    return NC_OK;
+}
+
+}  // namespace nc
+
+using namespace nc;
+
+extern "C" int nc_pages_extend(const int32_t *new_tokens, int slots, int32_t *lengths, int32_t *table, int max_pages,
+                               const int32_t *free_pages, int32_t *free_count, int num_pages, int rows,
+                               int32_t *cu_seqlens, int32_t *positions, int32_t *slot_map, int32_t *granted,
+                               int32_t *arrived, void *stream) {
+    if (!new_tokens || !lengths || !table || !free_pages || !free_count || !cu_seqlens || !positions || !slot_map ||
+        !granted || !arrived)
+        return NC_ERR_NULL;
+    if (rows <= 0) return NC_ERR_SHAPE;
+    if (const int e = pages_check(slots, max_pages, num_pages)) return e;
+    PagesArgs a = {};
+    a.asked = new_tokens; a.slots = slots; a.lengths = lengths; a.table = table; a.max_pages = max_pages;
+    a.free_pages = const_cast<int32_t *>(free_pages); a.free_count = free_count; a.num_pages = num_pages; a.rows = rows;
+    a.cu_seqlens = cu_seqlens; a.positions = positions; a.slot_map = slot_map; a.granted = granted; a.arrived = arrived;
+    const int grid = min((rows - 1) / PG_THREADS + 1, 128);
+    hipLaunchKernelGGL(pages_extend_kernel, dim3(grid), dim3(PG_THREADS), (3 * slots + 2) * sizeof(int),
+                       (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}
+
+extern "C" int nc_pages_trim(const int32_t *keep, int slots, int32_t *lengths, int32_t *table, int max_pages,
+                             int32_t *free_pages, int32_t *free_count, int num_pages, int32_t *arrived, void *stream) {
+    if (!keep || !lengths || !table || !free_pages || !free_count || !arrived) return NC_ERR_NULL;
+    if (const int e = pages_check(slots, max_pages, num_pages)) return e;
+    PagesArgs a = {};
+    a.asked = keep; a.slots = slots; a.lengths = lengths; a.table = table; a.max_pages = max_pages;
+    a.free_pages = free_pages; a.free_count = free_count; a.num_pages = num_pages; a.arrived = arrived;
+    const long long entries = min((long long)slots * max_pages, (long long)num_pages);
+    const int grid = (int)min((entries - 1) / (4 * PG_THREADS) + 1, 64LL);
+    hipLaunchKernelGGL(pages_trim_kernel, dim3(grid), dim3(PG_THREADS), (2 * slots + 1) * sizeof(int),
+                       (hipStream_t)stream, a);
+    return (int)hipGetLastError();
+}

@@ -12,6 +12,7 @@ missing library builds both once.
                            loads decode.cu
 """
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -27,7 +28,7 @@ LIB_DIR = PACKAGE / "lib"
 LIBRARY = LIB_DIR / "libnanochat_kv.so"
 DECODE_LIBRARY = LIB_DIR / "libnanochat_decode.so"
 KERNEL_SOURCES = [CSRC / "kv_append.hip", CSRC / "attention.hip", CSRC / "ve_gate.hip", CSRC / "flash_attn.hip",
-                  CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip"]
+                  CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip", CSRC / "paging.hip"]
 DECODE_SOURCES = [CSRC / "decoder.hip", CSRC / "slot_gemm.hip"]
 SOURCES = KERNEL_SOURCES + DECODE_SOURCES
 HEADERS = [CSRC / "nc_device.h", CSRC / "nc_internal.h", INCLUDE / "nanochat_amd.h", INCLUDE / "nanochat_decode.h"]
@@ -115,6 +116,11 @@ SIGNATURES = {
     "nc_weight_grad": ([c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_longlong, c_void_p], c_int),
     "nc_flash_attn_bwd_rows": ([c_void_p, c_longlong, c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_void_p],
                                c_int),
+    "nc_qk_norm_rope_append_rows_fp8": ([c_void_p, c_longlong, c_longlong, c_int, c_int] + [c_void_p] * 6 +
+                                        [c_int] + [c_void_p] * 4 + [c_int, c_void_p], c_int),
+    "nc_pages_extend": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int] + [c_void_p] * 6,
+                        c_int),
+    "nc_pages_trim": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p], c_int),
 }
 
 
@@ -206,6 +212,15 @@ def stream() -> int:
         return torch.cuda.current_stream().cuda_stream
     torch.cuda._lazy_init()
     return raw(torch._C._cuda_getDevice())
+
+
+def device_guard(t):
+    """A context in which t's device is the current one, whose stream and code a launch uses."""
+    import torch
+
+    if t.device.index == torch._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 if __name__ == "__main__":
