@@ -285,6 +285,24 @@ int nc_pages_trim(const int32_t *keep, int slots, int32_t *lengths, int32_t *tab
                   int32_t *free_count, int num_pages, int32_t *arrived, void *stream);
 
 /*
+ * A token a row from its logits and one given uniform number: the token choice of a decoding step (reference
+ * model/kernels/decode.cu:170-229, 361-411) for callers with logits of their own. logits: fp32, or bf16 (is_bf16), `rows`
+ * rows of `vocab` (<= 2^24) at row_stride elements. Per row: temperature fp32 (not above 0: the largest logit, the lowest
+ * index among equals); top_k int32, top_p and min_p fp32 (each may be NULL: off); mask (NULL, or uint32 words at
+ * mask_stride words a row: token t is allowed where bit t % 32 of word t / 32 is set). With w_i = exp((z_i - max z) /
+ * temperature) over the allowed tokens whose logit is neither NaN nor -inf (with a +inf logit only those weigh anything):
+ * the top_k largest stay (the lower index first among equals; top_k <= 0: all), of those the tokens with less than top_p
+ * of their weight strictly above them (at least the largest; top_p >= 1 or NaN: all), of those the ones with w_i >= min_p
+ * (taken into [0, 1]); tokens[row] is the first, in index order, whose running weight exceeds uniform[row] (in [0, 1),
+ * else the nearer end; NaN: 0) times the weight of all that are left; -1 where no token is allowed. Weights are held to
+ * 2^-46 of the largest (2^(ceil(log2 vocab) - 62) from 65,537 tokens on): smaller ones are never drawn. The result is
+ * reproducible and does not depend on the other rows. rows <= 2^22; no rows launch nothing.
+ */
+int nc_sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
+                     const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
+                     const float *min_p, const uint32_t *mask, long long mask_stride, int32_t *tokens, void *stream);
+
+/*
  * Measurement only; no counterpart in the reference. Reads n pages of 2 KiB (one (page, head) of K or V codes) from
  * src (src_bytes, a multiple of 2,048), page order[i] as the i-th (order NULL: page i; an entry outside the buffer
  * reads page 0), with `grid` workgroups of 256 threads, and writes one checksum word per thread to sink

@@ -28,7 +28,7 @@ LIB_DIR = PACKAGE / "lib"
 LIBRARY = LIB_DIR / "libnanochat_kv.so"
 DECODE_LIBRARY = LIB_DIR / "libnanochat_decode.so"
 KERNEL_SOURCES = [CSRC / "kv_append.hip", CSRC / "attention.hip", CSRC / "ve_gate.hip", CSRC / "flash_attn.hip",
-                  CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip", CSRC / "paging.hip"]
+                  CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip", CSRC / "paging.hip", CSRC / "sample.hip"]
 DECODE_SOURCES = [CSRC / "decoder.hip", CSRC / "slot_gemm.hip"]
 SOURCES = KERNEL_SOURCES + DECODE_SOURCES
 HEADERS = [CSRC / "nc_device.h", CSRC / "nc_internal.h", INCLUDE / "nanochat_amd.h", INCLUDE / "nanochat_decode.h"]
@@ -118,6 +118,8 @@ SIGNATURES = {
                                c_int),
     "nc_qk_norm_rope_append_rows_fp8": ([c_void_p, c_longlong, c_longlong, c_int, c_int] + [c_void_p] * 6 +
                                         [c_int] + [c_void_p] * 4 + [c_int, c_void_p], c_int),
+    "nc_sample_tokens": ([c_void_p, c_int, c_longlong, c_longlong, c_int] + [c_void_p] * 6 +
+                         [c_longlong, c_void_p, c_void_p], c_int),
     "nc_pages_extend": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int] + [c_void_p] * 6,
                         c_int),
     "nc_pages_trim": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p], c_int),

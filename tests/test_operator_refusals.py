@@ -57,6 +57,21 @@ def test_append_rows_rejects(lib):
     assert lib.nc_qk_norm_rope_append_rows_fp8(*append_args(rows=0)) == 0
 
 
+def sample_args(**over):
+    args = dict(logits=DUMMY, is_bf16=0, row_stride=100, rows=4, vocab=100, uniform=DUMMY, temperature=DUMMY, top_k=None,
+                top_p=None, min_p=None, mask=None, mask_stride=0, tokens=DUMMY, stream=None)
+    return list((args | over).values())
+
+
+def test_sample_rejects(lib):
+    for name in ("logits", "uniform", "temperature", "tokens"):
+        assert lib.nc_sample_tokens(*sample_args(**{name: None})) == -1, name
+    for over in (dict(rows=-1), dict(rows=2 ** 22 + 1), dict(vocab=0), dict(vocab=2 ** 24 + 1, row_stride=2 ** 25),
+                 dict(row_stride=99), dict(mask=DUMMY, mask_stride=3)):
+        assert lib.nc_sample_tokens(*sample_args(**over)) == -2, over
+    assert lib.nc_sample_tokens(*sample_args(rows=0)) == 0
+
+
 @pytest.mark.parametrize("sizes", [(0, 4, 8), (4097, 4, 8), (4, 0, 8), (4, 4, 0), (4, 2 ** 27, 8), (4, 4, 2 ** 27)])
 def test_block_tables_reject_sizes(sizes):
     with pytest.raises(ValueError):
