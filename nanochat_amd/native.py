@@ -31,7 +31,7 @@ KERNEL_SOURCES = [CSRC / "kv_append.hip", CSRC / "attention.hip", CSRC / "ve_gat
                   CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip", CSRC / "paging.hip", CSRC / "sample.hip"]
 DECODE_SOURCES = [CSRC / "decoder.hip", CSRC / "slot_gemm.hip"]
 SOURCES = KERNEL_SOURCES + DECODE_SOURCES
-HEADERS = [CSRC / "nc_device.h", CSRC / "nc_internal.h", INCLUDE / "nanochat_amd.h", INCLUDE / "nanochat_decode.h"]
+HEADERS = [CSRC / "nc_device.h", CSRC / "nc_internal.h", CSRC / "nc_row.h", CSRC / "nc_attend.h", INCLUDE / "nanochat_amd.h", INCLUDE / "nanochat_decode.h"]
 HEAD_DIM = 128
 
 # -ffp-contract=off: the append's fp32 order is part of its bit-exact contract (no implicit FMAs).
