@@ -261,6 +261,27 @@ int nc_prefill_attn_fp8(const void *q, const void *k_pages, const void *v_pages,
                         const int32_t *start_pos, int B, int T, int Hq, int Hkv, int window, float sm_scale,
                         void *out, void *stream);
 
+/* Workspace bytes nc_packed_attn_fp8 needs for these sizes, whatever the lengths on the device (0 for unsupported sizes):
+ * partial results, and counts in its last 1/256. As nc_decode_workspace_bytes's: zero-filled before its first call and
+ * passed with the same workspace_bytes to every call, by calls ordered on one stream; one workspace may serve both. */
+size_t nc_packed_workspace_bytes(long long rows, int B, int Hq, int Hkv, int max_seq_len, int window);
+
+/*
+ * Attention of packed rows over the paged fp8 cache: sequences with any numbers of new tokens in one launch (the reference
+ * runs one-token and prompt rows apart, model/kernels/decode.cu:567-675, 1041-1051). Sequence b's new tokens are rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q and out (bf16 [rows][Hq][128]; cu_seqlens int32 [B + 1], as
+ * nc_pages_extend makes it), the last of its seq_lens[b] tokens, all already in the cache; the row at position p attends
+ * keys [max(p - window, 0), p] (window < 0: all), scores (q . k) * sm_scale, fp32 softmax, out bf16. A sequence longer than
+ * max_seq_len (<= max_pages * 16) or shorter than its new tokens gets NaN, and so do the rows of a (row, KV head) that
+ * reaches a block-table entry outside [0, num_pages); rows outside every sequence are left as they are. Row offsets are
+ * taken into [0, rows]; if they overlap so that the workspace could not hold the launch, every row gets NaN. A sequence's
+ * output bits depend on its own numbers alone, not on the rest of the launch. rows <= 2^24, B <= 1024, Hq / Hkv <= 16.
+ */
+int nc_packed_attn_fp8(const void *q, const void *k_pages, const void *v_pages, const float *kv_scale,
+                       const int32_t *block_table, int max_pages, int num_pages, const int32_t *cu_seqlens,
+                       const int32_t *seq_lens, long long rows, int B, int Hq, int Hkv, int max_seq_len, int window,
+                       float sm_scale, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
 /*
  * The page bookkeeping of `slots` (<= 4096) sequences over one pool, kept on the device; no counterpart in the reference
  * (its slots own fixed caches, model/kernels/decode.cu:740-763). State: lengths int32 [slots], table int32

@@ -6,6 +6,8 @@
 - decode_attention: split-K flash-decode over the paged cache, replacing k_attn (decode.cu:567-675).
 - decode_step: the two in one launch (k_prologue + k_attn of a decode step, decode.cu:551-675, 861-863), with the
   same bits as qk_norm_rope_append followed by decode_attention.
+- qk_norm_rope_append_packed, packed_attention: the append and the attention of a step whose sequences bring any
+  numbers of new tokens, by the slot maps and row offsets of paging.BlockTables.
 - prefill_attention: MFMA chunked prefill, replacing the prefill rows of dec_prefill
   (decode.cu:1041-1051, append-then-attend order 859-863).
 
@@ -16,7 +18,7 @@ from collections import OrderedDict
 
 import torch
 
-from .config import HEAD_DIM
+from .config import HEAD_DIM, PAGE_SIZE
 from .kv_cache import PagedKVCache, _require
 from .native import check, device_guard, hip_library, pointer, stream
 
@@ -270,4 +272,67 @@ def prefill_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.T
         pointer(q), pointer(cache.k_pages), pointer(cache.v_pages), pointer(cache.kv_scale),
         pointer(block_table), block_table.size(1), cache.num_pages, pointer(start_pos), B, T, Hq, cache.num_kv_heads,
         window, sm_scale, pointer(out), stream()))
+    return out
+
+
+@functools.lru_cache(maxsize=256)
+def packed_workspace_bytes(rows: int, batch: int, num_q_heads: int, num_kv_heads: int, max_seq_len: int,
+                           window: int = -1) -> int:
+    """nc_packed_workspace_bytes (0: an unsupported shape), kept per shape."""
+    return hip_library().nc_packed_workspace_bytes(rows, batch, num_q_heads, num_kv_heads, max_seq_len, window)
+
+
+def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                     seq_lens: torch.Tensor, max_seq_len: int, window: int = -1, sm_scale: float | None = None,
+                     out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """q bf16 [rows, Hq, 128], the packed rows of sequences with any numbers of new tokens (decoding rows beside prompt
+    chunks and draft tokens), already appended -> out bf16 [rows, Hq, 128].
+
+    Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1]) and the last of its seq_lens[b]
+    tokens (int32 [B]); its row at position p attends keys [max(p - window, 0), p] through block_table[b]. max_seq_len
+    bounds seq_lens: a longer sequence's rows are NaN, as are those of one shorter than its new tokens. Rows outside every
+    sequence are not written. A sequence's output bits depend on nothing but its own numbers. A workspace passed in must
+    have been zero-filled before its first use (torch.zeros, at least packed_workspace_bytes) and only used by these and
+    decode_attention's calls since, one stream at a time. Without one, calls on a stream share a cached workspace; a call
+    that is being captured into a graph gets one of the graph's own."""
+    _require(q, "q", torch.bfloat16)
+    if q.dim() != 3 or q.size(2) != HEAD_DIM or q.size(1) < 1:
+        raise ValueError(f"q must be [rows, Hq, {HEAD_DIM}], got {tuple(q.shape)}")
+    rows, Hq, _ = q.shape
+    cache.check_table(block_table)
+    B = block_table.size(0)
+    for name, t, n in (("cu_seqlens", cu_seqlens, B + 1), ("seq_lens", seq_lens, B)):
+        _require(t, name, torch.int32)
+        if t.shape != (n,):
+            raise ValueError(f"{name} must be [{n}] for a block table of {B} sequences, got {tuple(t.shape)}")
+    if not 0 < max_seq_len <= block_table.size(1) * PAGE_SIZE:
+        raise ValueError(f"max_seq_len {max_seq_len} must be in [1, {block_table.size(1) * PAGE_SIZE}] (the block table)")
+    if sm_scale is None:
+        sm_scale = HEAD_DIM ** -0.5
+    if out is None:
+        out = torch.empty_like(q)
+    _require(out, "out", torch.bfloat16)
+    if out.shape != q.shape:
+        raise ValueError(f"out must be {tuple(q.shape)}")
+    _same_device(q.device, cache=cache.k_pages, block_table=block_table, cu_seqlens=cu_seqlens, seq_lens=seq_lens, out=out)
+    if rows == 0:
+        return out
+    window = max(window, -1)
+    need = packed_workspace_bytes(rows, B, Hq, cache.num_kv_heads, max_seq_len, window)
+    if need == 0:
+        raise ValueError(f"unsupported shape: rows={rows}, B={B}, Hq={Hq}, Hkv={cache.num_kv_heads}")
+    with device_guard(q):
+        if workspace is None:
+            if torch.cuda.is_current_stream_capturing():
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+                workspace[need - need // 256 - 8:].zero_()   # its counts, on every replay
+            else:
+                workspace = _workspace(q.device, need)
+        nbytes = workspace.numel() * workspace.element_size()
+        if nbytes < need or not workspace.is_contiguous() or workspace.device != q.device or workspace.data_ptr() % 16:
+            raise ValueError(f"workspace must be a contiguous 16-byte aligned tensor of at least {need} bytes on {q.device}")
+        check(hip_library().nc_packed_attn_fp8(
+            pointer(q), pointer(cache.k_pages), pointer(cache.v_pages), pointer(cache.kv_scale), pointer(block_table),
+            block_table.size(1), cache.num_pages, pointer(cu_seqlens), pointer(seq_lens), rows, B, Hq, cache.num_kv_heads,
+            max_seq_len, window, sm_scale, pointer(out), pointer(workspace), nbytes, stream()))
     return out

@@ -1,0 +1,800 @@
+/*
+ * Attention of packed query rows over the paged fp8 cache on gfx950: each sequence brings any number of new tokens (one to
+ * decode, a few drafts to verify, a chunk of a prompt), all already in the cache, and its row t attends the keys
+ * [max(p - window, 0), p] of its own sequence, p = seq_len - n + t. One launch serves the whole mix; lengths and row
+ * offsets stay on the device. (The reference runs such rows as separate kernels, model/kernels/decode.cu:567-675 and
+ * 1041-1051; the padded forms are attention.hip's.)
+ *
+ *   o = sum_j exp2(s_j - m) v_j / sum_j exp2(s_j - m),  s_j = (q . k_j) sm_scale log2(e),  m a running maximum
+ *
+ * The step over two pages (scores, softmax, PV) is nc_attend.h's. What bounds a sequence depends on its rows: a page of a
+ * KV head is 2 KiB of K, 2 KiB of V and 128 bytes of scales for 16 keys, and each query column costs 512 flops a key, so
+ * below about 80 columns (rows times the heads of a KV head) the pages' bytes take longer than the products. Hence two
+ * kinds of work items, each one workgroup of four waves, both streaming pages into LDS by asynchronous copies:
+ *
+ *   narrow  at most 32 columns: the four waves take the chunk's page pairs in turn, each through a ring of its own with two
+ *           pairs in flight and no barrier, and merge their four softmax states through LDS at the end
+ *   wide    a tile of up to 128 columns, 32 a wave: all waves walk the same pairs, each pair fetched once (PK_AHEAD ahead)
+ *
+ * A sequence's keys are cut into chunks (pk_plan), so that few rows over many keys still fill the chip; a (tile, KV head)
+ * of several chunks leaves one partial (O, max, sum) in fp32 a chunk, and the workgroup that finishes its last chunk merges
+ * them in order. The cuts depend on nothing but the sequence's own numbers, so its output bits do not depend on the rest
+ * of the launch. Items are taken in the order wide, narrow: the first by workgroup index, later ones from eight queues
+ * (an XCD's workgroups take every eighth item, which keeps a KV head's pages in that XCD's L2), so that unequal items even
+ * out.
+ */
+#include <limits.h>
+
+#include "nc_attend.h"
+#include "nanochat_amd.h"
+
+namespace nc {
+
+constexpr int PK_NT = 2;                       /* 16-column tiles a wave */
+constexpr int PK_NARROW_COLS = 16 * PK_NT;
+constexpr int PK_WIDE_COLS = WAVES * 16 * PK_NT;
+constexpr int PK_MAX_BATCH = 1024;
+constexpr int PK_QUEUES = 8;                   /* XCDs */
+constexpr int PK_NARROW_SPLIT = 128;           /* pages of a narrow chunk */
+constexpr int PK_WIDE_MIN = 128;               /* least and most pages of a wide chunk */
+constexpr int PK_WIDE_MAX = 1024;
+constexpr int PK_WIDE_ITEMS = 256;             /* items a wide sequence is cut into at most, if its chunks stay that long */
+constexpr int PK_AHEAD = 3;                    /* wide: pairs in flight */
+static_assert(PK_NARROW_SPLIT <= 256, "a wave's block-table entries of a narrow chunk: one a lane");
+
+/* One stage: the pair's K (2 x 2 KiB), V (2 x 2 KiB) and scales (per page 16 of K, then 16 of V; wide: a copy a wave). */
+constexpr int PK_SCALE_AT = 4 * PAGE_BYTES, PK_SCALE_BYTES = 256;
+constexpr int PK_WIDE_STAGE = PK_SCALE_AT + WAVES * PK_SCALE_BYTES, PK_WIDE_BUFS = PK_AHEAD + 1;
+constexpr int PK_NARROW_STAGE = PK_SCALE_AT + PK_SCALE_BYTES, PK_NARROW_BUFS = 2;
+constexpr int PK_STAGES = WAVES * PK_NARROW_BUFS * PK_NARROW_STAGE;   /* bytes of LDS */
+static_assert(PK_WIDE_BUFS * PK_WIDE_STAGE <= PK_STAGES, "the wide stages fit");
+static_assert(WAVES * PK_NARROW_COLS * O_PITCH * 4 <= PK_STAGES, "the narrow merge fits");
+typedef __attribute__((address_space(3))) void LdsVoid;
+
+struct PackedArgs {
+    AttnArgs a;                 /* q, pools, block_table, seq_lens, B, Hq, Hkv, G, window, scale_log2, max_len, out */
+    const int32_t *cu;          /* [B + 1] */
+    int rows;                   /* rows of q and out */
+    float *part_wide, *part_narrow;   /* [slots][cols][128] O, then [slots][cols][2] (max, sum) */
+    long long wide_slots, narrow_slots;
+    int units;                  /* arrival counts */
+    int *tickets, *done, *arrived;    /* [8], [1], [units]; zero between launches */
+};
+
+/* A sequence's rows, its pages [pg0, pg0 + np) (pg0 even) and how they are cut: nch chunks of s pages from pg0. tiles = 0:
+ * no rows; < 0: a length that does not fit (its rows become NaN). */
+struct PkSeq {
+    int row0, n, len, pg0, np, tiles, s, nch;
+    bool narrow;
+};
+
+__device__ __forceinline__ PkSeq pk_plan(const PackedArgs &p, int cu0, int cu1, int len) {
+    const AttnArgs &a = p.a;
+    PkSeq q = {};
+    q.row0 = min(max(cu0, 0), p.rows);
+    q.n = min(max(cu1, q.row0), p.rows) - q.row0;
+    if (q.n == 0) return q;
+    q.len = len;
+    if (q.len < q.n || q.len > a.max_len) {
+        q.tiles = -1;
+        return q;
+    }
+    const int first = a.window >= 0 ? max(q.len - q.n - a.window, 0) : 0;
+    q.pg0 = (first / PAGE) & ~1;
+    q.np = (q.len - 1) / PAGE + 1 - q.pg0;
+    const int tpt = 16 / a.G, tpw = tpt * PK_NT;
+    q.narrow = q.n <= tpw;
+    if (q.narrow) {
+        q.tiles = 1;
+        q.s = PK_NARROW_SPLIT;
+    } else {
+        q.tiles = (q.n - 1) / (WAVES * tpw) + 1;
+        const int want = max(PK_WIDE_ITEMS / (q.tiles * a.Hkv), 1);
+        q.s = min(max(((q.np - 1) / want + 1 + 31) & ~31, PK_WIDE_MIN), PK_WIDE_MAX);
+    }
+    q.nch = (q.np - 1) / q.s + 1;
+    return q;
+}
+
+__device__ __forceinline__ PkSeq pk_plan(const PackedArgs &p, int b) {
+    return pk_plan(p, p.cu[b], p.cu[b + 1], p.a.seq_lens[b]);
+}
+
+/* This lane, as a value the compiler cannot compute ahead: nothing made of it is kept in registers across items. */
+__device__ __forceinline__ int pk_lane() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t & (WAVE - 1);
+}
+
+/* A value that is the same in every lane, as a scalar register's. */
+__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+/* Exclusive prefix sums of two values a thread over the workgroup's 256 threads. */
+__device__ __forceinline__ void pk_scan(long long (&v)[2], long long (&part)[2][WAVES]) {
+    const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        long long s = v[k];
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) {
+            const long long t = __shfl_up(s, o, WAVE);
+            if (lane >= o) s += t;
+        }
+        if (lane == WAVE - 1) part[k][wave] = s;
+        v[k] = s - v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) v[k] += w < wave ? part[k][w] : 0;
+    __syncthreads();
+}
+
+/* A workgroup barrier that drains no asynchronous copy; memory accesses do not move across it. */
+__device__ __forceinline__ void pk_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ int pk_lds_offset(const unsigned char *p) {
+    return (int)(uintptr_t)(__attribute__((address_space(3))) const unsigned char *)p;
+}
+
+/* s_waitcnt operands (gfx9 encoding: vmcnt in bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8). */
+constexpr int pk_wait(int vmcnt, int lgkmcnt) { return (vmcnt & 15) | (vmcnt >> 4) << 14 | 7 << 4 | lgkmcnt << 8; }
+
+/* One partial's O [cols][128] and (max, sum) [cols][2]. */
+struct PkPart {
+    float *o, *ml;
+};
+__device__ __forceinline__ PkPart pk_part(float *base, long long slots, int cols, long long slot) {
+    return PkPart{base + slot * cols * HEAD_DIM, base + slots * cols * HEAD_DIM + slot * cols * 2};
+}
+
+/* What an item works on: the KV head, its tokens t0 .. t0 + tn - 1 of the sequence, pages [pg0, pg1) of its chunk. */
+struct PkItem {
+    PkSeq q;
+    int b, kvh, t0, tn, pg0, pg1;
+};
+
+/* Column c of wave tile t (first token wt0) -> its token (< 0: not live). */
+__device__ __forceinline__ int pk_token(const AttnArgs &a, int wt0, int end, int t, int c) {
+    const int tpt = 16 / a.G, tok = wt0 + t * tpt + c / a.G;
+    return c < tpt * a.G && tok < end ? tok : -1;
+}
+
+__device__ __forceinline__ long long pk_row(const PackedArgs &p, const PkItem &it, int tok, int c) {
+    return ((long long)it.q.row0 + tok) * p.a.Hq + it.kvh * p.a.G + c % p.a.G;
+}
+
+/* Per-column key bounds of a wave whose first token is wt0 (end: one past the item's last), and its query operand. */
+template <int NT>
+__device__ __forceinline__ void pk_columns(const PackedArgs &p, const PkItem &it, int wt0, int end, int lane,
+                                           KeyBounds<NT> &kb, uint4 (&raw)[NT][4]) {
+    const AttnArgs &a = p.a;
+    const int c = lane & 15, g = lane >> 4, start = it.q.len - it.q.n, tpt = 16 / a.G;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int tok = pk_token(a, wt0, end, t, c), pos = start + tok;
+        kb.hi[t] = tok >= 0 ? pos : -1;
+        kb.lo[t] = tok >= 0 && a.window >= 0 ? max(pos - a.window, 0) : 0;
+#pragma unroll
+        for (int cc = 0; cc < 4; cc++)
+            raw[t][cc] = tok >= 0 ? *reinterpret_cast<const uint4 *>(a.q + pk_row(p, it, tok, c) * HEAD_DIM + g * 32 + cc * 8)
+                                  : uint4{0u, 0u, 0u, 0u};
+    }
+    const int last = min(wt0 + NT * tpt, end) - 1;
+    kb.full_hi = start + wt0;
+    kb.full_lo = a.window >= 0 ? max(start + last - a.window, 0) : 0;
+    kb.written_hi = it.q.len - 1;
+}
+
+/* A pair's operands from a stage: four 16-byte reads a lane (K: at = the stage's LDS byte, V: 4 KiB on) and the lane's
+ * scales of both pages (K: sc = the scales' LDS byte, V: 64 on), in registers when this returns. The compiler would make
+ * ordinary reads of the stages wait for every copy in flight into any of them (it cannot tell one stage from another);
+ * these wait for nothing but themselves, the caller having waited for the stage's own copies. */
+__device__ __forceinline__ void pk_read(int at, int sc, int lane, PairRegs &k) {
+    u32x4 a0, a1, b0, b1, sa, sb;
+    asm volatile("ds_read_b128 %0, %6\n\t"
+                 "ds_read_b128 %1, %6 offset:1024\n\t"
+                 "ds_read_b128 %2, %6 offset:2048\n\t"
+                 "ds_read_b128 %3, %6 offset:3072\n\t"
+                 "ds_read_b128 %4, %7\n\t"
+                 "ds_read_b128 %5, %7 offset:128\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(a0), "=&v"(a1), "=&v"(b0), "=&v"(b1), "=&v"(sa), "=&v"(sb)
+                 : "v"(at + lane * 16), "v"(sc + (lane >> 4) * 16)
+                 : "memory");
+    k.a0 = uint4{a0[0], a0[1], a0[2], a0[3]};
+    k.a1 = uint4{a1[0], a1[1], a1[2], a1[3]};
+    k.b0 = uint4{b0[0], b0[1], b0[2], b0[3]};
+    k.b1 = uint4{b1[0], b1[1], b1[2], b1[3]};
+    k.sa = float4{__uint_as_float(sa[0]), __uint_as_float(sa[1]), __uint_as_float(sa[2]), __uint_as_float(sa[3])};
+    k.sb = float4{__uint_as_float(sb[0]), __uint_as_float(sb[1]), __uint_as_float(sb[2]), __uint_as_float(sb[3])};
+}
+
+/* A stage's place in LDS, for one wave. */
+struct PkAt {
+    int at, scales;
+};
+
+/* One pair's scores, softmax and PV, as nc_attend.h's pair_update (same sums, same lazy rescale: a column keeps its
+ * reference maximum until a score passes it by 8 in log2) but tile after tile, so that one tile's scores and exponentials
+ * are live at a time. MASKED: some key of the pair is not seen by some column, or not written. What is not seen takes no
+ * part whatever its bytes: its exponential and its product with the V scale are replaced by zero, and the V codes of keys
+ * that are not written are cleared. */
+template <int NT, bool MASKED, typename Freed>
+__device__ __forceinline__ void pk_update(int lpa, bool has_b, PkAt stage, const QOp (&qb)[NT], const KeyBounds<NT> &kb,
+                                          WaveState<NT> &st, int lane, Freed freed) {
+    const int key_a = lpa * PAGE + (lane >> 4) * 4, key_b = key_a + PAGE;
+    PairRegs k, v;
+    pk_read(stage.at, stage.scales, lane, k);
+    f32x4 sa[NT], sb[NT];
+    __builtin_amdgcn_s_setprio(1);   /* the other wave of the SIMD runs its VALU while these products issue */
+    page_scores<NT>(k.a0, k.a1, qb, sa);
+    page_scores<NT>(k.b0, k.b1, qb, sb);
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);   /* K's registers are free, and V's reads take less than the products */
+    pk_read(stage.at + 2 * PAGE_BYTES, stage.scales + PAGE * 4, lane, v);
+    freed();
+    if (MASKED) {
+        const int na = min(max(kb.written_hi - key_a + 1, 0), 4), nb = has_b ? min(max(kb.written_hi - key_b + 1, 0), 4) : 0;
+        const uint32_t ma = na >= 4 ? 0xFFFFFFFFu : (1u << (8 * na)) - 1u, mb = nb >= 4 ? 0xFFFFFFFFu : (1u << (8 * nb)) - 1u;
+        v.a0 = and4(v.a0, ma); v.a1 = and4(v.a1, ma);
+        v.b0 = and4(v.b0, mb); v.b1 = and4(v.b1, mb);
+    }
+    const float ks[8] = {k.sa.x * st.sl2, k.sa.y * st.sl2, k.sa.z * st.sl2, k.sa.w * st.sl2,
+                         k.sb.x * st.sl2, k.sb.y * st.sl2, k.sb.z * st.sl2, k.sb.w * st.sl2};
+    const float vs[8] = {v.sa.x, v.sa.y, v.sa.z, v.sa.w, v.sb.x, v.sb.y, v.sb.z, v.sb.w};
+    bf16x8 pv[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const auto seen = [&](int i) {
+            const int key = (i < 4 ? key_a : key_b) + (i & 3);
+            return !MASKED || ((i < 4 || has_b) && key >= kb.lo[t] && key <= kb.hi[t]);
+        };
+        const float negm = -st.m[t];   /* +inf before the first key: every live p is +inf, the slow path */
+        float p[8], most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(i < 4 ? sa[t][i] : sb[t][i - 4], ks[i], negm));
+            p[i] = seen(i) ? e : 0.0f;
+            most = fmaxf(most, p[i]);
+        }
+        if (__any(!(most <= 256.0f))) {   /* a column's maximum passed its reference by more than 2^8 (or has none yet) */
+            const float pc = pair_max32(pair_max16(most));   /* the column's largest over its four row groups */
+            if (pc > 256.0f) {
+                float sc[8], mt = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    sc[i] = seen(i) ? (i < 4 ? sa[t][i] : sb[t][i - 4]) * ks[i] : -INFINITY;
+                    mt = fmaxf(mt, sc[i]);
+                }
+                mt = pair_max32(pair_max16(mt));
+                const float mnew = fmaxf(st.m[t], mt);
+                const float alpha = mnew == st.m[t] ? 1.0f : __builtin_amdgcn_exp2f(st.m[t] - mnew);
+#pragma unroll
+                for (int d = 0; d < 8; d++) st.o[t][d] *= alpha;
+                st.l[t] *= alpha;
+                st.m[t] = mnew;
+                const float base = mnew == -INFINITY ? 0.0f : mnew;
+#pragma unroll
+                for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(sc[i] - base);
+            }
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            sum += p[i];
+            pv[t][i] = (__bf16)(seen(i) ? p[i] * vs[i] : 0.0f);
+        }
+        st.l[t] += sum;
+    }
+#pragma unroll
+    for (int d = 0; d < 8; d++) {
+        const bf16x8 va = fp8x8_to_bf16(dword(d < 4 ? v.a0 : v.a1, d & 3), dword(d < 4 ? v.b0 : v.b1, d & 3));
+#pragma unroll
+        for (int t = 0; t < NT; t++) st.o[t][d] = mfma16x16x32(va, pv[t], st.o[t][d]);
+    }
+}
+
+/* freed() is called once the stage's bytes are in registers. */
+template <int NT, typename Freed>
+__device__ __forceinline__ void pk_pair(int lpa, bool has_b, PkAt stage, const QOp (&qb)[NT], const KeyBounds<NT> &kb,
+                                        WaveState<NT> &st, int lane, Freed freed) {
+    const int end = lpa * PAGE + 2 * PAGE - 1;
+    if (has_b && lpa * PAGE >= kb.full_lo && end <= kb.full_hi && end <= kb.written_hi)
+        pk_update<NT, false>(lpa, has_b, stage, qb, kb, st, lane, freed);
+    else
+        pk_update<NT, true>(lpa, has_b, stage, qb, kb, st, lane, freed);
+}
+
+/* --- wide items */
+
+/* One stage's copies: wave w K bytes [1024 w, 1024 w + 1024) of the pair (pages a, a, b, b), the same of V, and all 256
+ * scale bytes into its own slot; every wave always issues three. */
+__device__ __forceinline__ void pk_fetch_wide(const AttnArgs &a, const int *tab, int npages, int s, int kvh, unsigned char *st,
+                                              int wave, int lane) {
+    const int la = 2 * min(s, (npages - 1) / 2), lb = la + 1 < npages ? la + 1 : la;   /* past the range: its last pair */
+    const int pa = __builtin_amdgcn_readfirstlane(tab[la]), pb = __builtin_amdgcn_readfirstlane(tab[lb]);
+    const long long ph = (long long)(wave < 2 ? pa : pb) * a.Hkv + kvh;
+    const int half = (wave & 1) * 1024;
+    __builtin_amdgcn_global_load_lds((const void *)(a.k_pages + ph * PAGE_BYTES + half + lane * 16),
+                                     (LdsVoid *)(st + wave * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void *)(a.v_pages + ph * PAGE_BYTES + half + lane * 16),
+                                     (LdsVoid *)(st + 2 * PAGE_BYTES + wave * 1024), 16, 0, 0);
+    const long long sh = (long long)(lane < 32 ? pa : pb) * a.Hkv + kvh;
+    __builtin_amdgcn_global_load_lds((const void *)(a.kv_scale + sh * 2 * PAGE + (lane & 31)),
+                                     (LdsVoid *)(st + PK_SCALE_AT + wave * PK_SCALE_BYTES), 4, 0, 0);
+}
+
+__device__ __forceinline__ void pk_wide(const PackedArgs &p, const PkItem &it, int chunks, long long slot,
+                                        unsigned char *stages, int *tab) {
+    const AttnArgs &a = p.a;
+    const int lane = pk_lane(), wave = uni((int)threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int tpw = 16 / a.G * PK_NT, start = it.q.len - it.q.n;
+    const int wt0 = it.t0 + wave * tpw, end = it.t0 + it.tn, npages = it.pg1 - it.pg0;
+    const bool on = wt0 < end;
+    const int last = min(wt0 + tpw, end) - 1;
+    /* the wave's own pages within the chunk's */
+    const int w0 = max((a.window >= 0 ? max(start + wt0 - a.window, 0) : 0) / PAGE, it.pg0);
+    const int w1 = on ? min((start + last) / PAGE + 1, it.pg1) : 0;
+    const int32_t *bt = a.block_table + (long long)it.b * a.max_pages + it.pg0;
+    bool bad = false;   /* an entry outside the pool among the pairs this wave computes */
+    for (int i = threadIdx.x; i < npages; i += 256) {
+        const int e = bt[i];
+        tab[i] = (unsigned)e < (unsigned)a.num_pages ? e : -1;
+    }
+    KeyBounds<PK_NT> kb;
+    uint4 raw[PK_NT][4];
+    pk_columns<PK_NT>(p, it, wt0, end, lane, kb, raw);
+    QOp qb[PK_NT];
+    q8_from_raw<PK_NT>(raw, qb);
+    WaveState<PK_NT> ws;
+    state_init(ws);
+    ws.sl2 = a.scale_log2;
+    __syncthreads();
+    for (int i = (max(w0 - it.pg0, 0) & ~1) + lane; i < min(npages, (w1 - it.pg0 + 1) & ~1); i += WAVE) bad |= tab[i] < 0;
+    ws.bad = __any(bad);
+    __syncthreads();
+    for (int i = threadIdx.x; i < npages; i += 256) tab[i] = max(tab[i], 0);   /* only read: those waves report NaN */
+    __syncthreads();
+
+    const int lds = pk_lds_offset(stages), count = (npages + 1) / 2;
+    for (int s = 0; s < PK_AHEAD; s++) pk_fetch_wide(a, tab, npages, s, it.kvh, stages + s * PK_WIDE_STAGE, wave, lane);
+    /* step s: this wave's copies of stage s have landed (then everyone's, after the barrier, and everyone's reads of the
+     * stage before are done); refill that buffer with stage s + PK_AHEAD; compute stage s */
+    for (int s = 0, buf = 0; s < count; s++) {
+        __builtin_amdgcn_s_waitcnt(pk_wait(3 * (PK_AHEAD - 1), 15));
+        pk_barrier();
+        const int into = buf == 0 ? PK_WIDE_BUFS - 1 : buf - 1;   /* (s + PK_AHEAD) % PK_WIDE_BUFS */
+        pk_fetch_wide(a, tab, npages, s + PK_AHEAD, it.kvh, stages + into * PK_WIDE_STAGE, wave, lane);
+        const int lpa = it.pg0 + 2 * s;
+        if (lpa + 1 >= w0 && lpa < w1) {
+            const int at = lds + buf * PK_WIDE_STAGE;
+            pk_pair<PK_NT>(lpa, 2 * s + 1 < npages, PkAt{at, at + PK_SCALE_AT + wave * PK_SCALE_BYTES}, qb, kb, ws, lane, [] {});
+        }
+        buf = buf == PK_WIDE_BUFS - 1 ? 0 : buf + 1;
+    }
+    __builtin_amdgcn_s_waitcnt(0);   /* every copy has landed before the stages and the table are used again */
+    pk_barrier();
+
+    const PkPart part = pk_part(p.part_wide, p.wide_slots, PK_WIDE_COLS, slot);
+    const Rsrc ro = page_rsrc(part.o, PK_WIDE_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_WIDE_COLS * 8);
+#pragma unroll
+    for (int t = 0; t < PK_NT; t++) {
+        ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
+        const int tok = pk_token(a, wt0, end, t, c);
+        if (tok < 0) continue;
+        if (chunks == 1) {
+            uint16_t *dst = a.out + pk_row(p, it, tok, c) * HEAD_DIM;
+            const float inv = 1.0f / ws.l[t];
+#pragma unroll
+            for (int d = 0; d < 8; d++) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = ws.bad ? NAN : ws.o[t][d][i] * inv;
+                store_bf16x4(dst + 16 * d + 4 * g, v);
+            }
+        } else {
+            const int col = (wave * PK_NT + t) * 16 + c;
+#pragma unroll
+            for (int d = 0; d < 8; d++)
+                part_store(ro, (col * HEAD_DIM + 16 * d + 4 * g) * 4,
+                           float4{ws.o[t][d][0], ws.o[t][d][1], ws.o[t][d][2], ws.o[t][d][3]});
+            if (g == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(
+                    u32x2{__float_as_uint(ws.bad ? NAN : ws.m[t]), __float_as_uint(ws.l[t])}, rm, col * 8, 0, SC1);
+        }
+    }
+}
+
+/* --- narrow items */
+
+/* One pair's copies into a wave's stage: four of 1 KiB a page, through descriptors of one page (live false: of no range, so nothing is read), and the 256 scale bytes. Nine in all. */
+__device__ __forceinline__ void pk_fetch_narrow(const AttnArgs &a, int pa, int pb, bool live, int kvh, unsigned char *st,
+                                                int lane) {
+    const long long ha = (long long)pa * a.Hkv + kvh, hb = (long long)pb * a.Hkv + kvh;
+    const int bytes = live ? PAGE_BYTES : 0;
+    const Rsrc ka = page_rsrc(a.k_pages + ha * PAGE_BYTES, bytes), kb = page_rsrc(a.k_pages + hb * PAGE_BYTES, bytes);
+    const Rsrc va = page_rsrc(a.v_pages + ha * PAGE_BYTES, bytes), vb = page_rsrc(a.v_pages + hb * PAGE_BYTES, bytes);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(ka, (LdsVoid *)st, 16, lane * 16, 0, 0, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(ka, (LdsVoid *)(st + 1024), 16, lane * 16 + 1024, 0, 0, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(kb, (LdsVoid *)(st + 2048), 16, lane * 16, 0, 0, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(kb, (LdsVoid *)(st + 3072), 16, lane * 16 + 1024, 0, 0, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(va, (LdsVoid *)(st + 4096), 16, lane * 16, 0, 0, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(va, (LdsVoid *)(st + 5120), 16, lane * 16 + 1024, 0, 0, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(vb, (LdsVoid *)(st + 6144), 16, lane * 16, 0, 0, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(vb, (LdsVoid *)(st + 7168), 16, lane * 16 + 1024, 0, 0, 2);
+    __builtin_amdgcn_global_load_lds((const void *)(a.kv_scale + (lane < 32 ? ha : hb) * 2 * PAGE + (lane & 31)),
+                                     (LdsVoid *)(st + PK_SCALE_AT), 4, 0, 0);
+}
+
+template <int NT>
+__device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it, int chunks, long long slot,
+                                          unsigned char *stages, float (&sh_m)[WAVES][PK_NARROW_COLS],
+                                          float (&sh_l)[WAVES][PK_NARROW_COLS]) {
+    const AttnArgs &a = p.a;
+    const int lane = pk_lane(), wave = uni((int)threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int pairs = (it.pg1 - it.pg0 + 1) / 2, mine = (pairs - wave + 3) / 4;
+    /* lane j: the entry of page j & 1 of this wave's pair j / 2 (a second page past the range: the first) */
+    const int32_t *bt = a.block_table + (long long)it.b * a.max_pages;
+    int lp = it.pg0 + 2 * (wave + 4 * (lane >> 1)) + (lane & 1);
+    if ((lane & 1) && lp >= it.pg1) lp--;
+    int entry = lp < it.pg1 ? bt[lp] : 0;
+    const bool bad = __any((unsigned)entry >= (unsigned)a.num_pages);
+    if ((unsigned)entry >= (unsigned)a.num_pages) entry = 0;
+
+    KeyBounds<NT> kb;
+    uint4 raw[NT][4];
+    pk_columns<NT>(p, it, 0, it.tn, lane, kb, raw);
+    WaveState<NT> ws;
+    state_init(ws);
+    ws.sl2 = a.scale_log2;
+    ws.bad = bad;
+    if (mine > 0) {
+        unsigned char *ring = stages + wave * PK_NARROW_BUFS * PK_NARROW_STAGE;
+        const int lds = pk_lds_offset(ring);
+        const auto fetch = [&](int i, int buf) {
+            const int j = i < mine ? 2 * i : 0;
+            pk_fetch_narrow(a, __builtin_amdgcn_readlane(entry, j), __builtin_amdgcn_readlane(entry, j + 1), i < mine, it.kvh,
+                            ring + buf * PK_NARROW_STAGE, lane);
+        };
+        fetch(0, 0);
+        fetch(1, 1);
+        QOp qb[NT];
+        q8_from_raw<NT>(raw, qb);
+        for (int i = 0; i < mine; i++) {
+            const int at = lds + (i & 1) * PK_NARROW_STAGE;
+            __builtin_amdgcn_s_waitcnt(pk_wait(9, 15));   /* all but the younger pair's copies have landed */
+            const int lpa = it.pg0 + 2 * (wave + 4 * i);
+            pk_pair<NT>(lpa, lpa + 1 < it.pg1, PkAt{at, at + PK_SCALE_AT}, qb, kb, ws, lane, [&] { fetch(i + 2, i & 1); });
+        }
+    }
+    /* the four waves' states: (max, sum) of every column, then O */
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
+        if (g == 0) {
+            sh_m[wave][t * 16 + c] = ws.bad ? NAN : ws.m[t];
+            sh_l[wave][t * 16 + c] = ws.l[t];
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0);   /* no copy is in flight into the stages */
+    __syncthreads();
+    float *merged = reinterpret_cast<float *>(stages);   /* [wave][column][O_PITCH] */
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int d = 0; d < 8; d++)
+            *reinterpret_cast<f32x4 *>(merged + ((wave * NT + t) * 16 + c) * O_PITCH + 16 * d + 4 * g) = ws.o[t][d];
+    __syncthreads();
+    const PkPart part = pk_part(p.part_narrow, p.narrow_slots, PK_NARROW_COLS, slot);
+    const Rsrc ro = page_rsrc(part.o, PK_NARROW_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_NARROW_COLS * 8);
+    for (int i = threadIdx.x; i < NT * 16 * (HEAD_DIM / 4); i += 256) {
+        const int col = i >> 5, quad = i & 31, tok = pk_token(a, 0, it.tn, col >> 4, col & 15);
+        if (tok < 0) continue;
+        float m = sh_m[0][col], l = 0.0f;
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) m = fmaxf(m, sh_m[w][col]);
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        bool any_bad = false;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float mw = sh_m[w][col];
+            any_bad = any_bad || mw != mw;
+            const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+            o += *reinterpret_cast<const f32x4 *>(merged + (w * NT * 16 + col) * O_PITCH + 4 * quad) * f;
+            l += sh_l[w][col] * f;
+        }
+        if (chunks == 1) {
+            float v[4];
+            const float inv = 1.0f / l;
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = any_bad ? NAN : o[k] * inv;
+            store_bf16x4(a.out + pk_row(p, it, tok, col & 15) * HEAD_DIM + 4 * quad, v);
+        } else {
+            part_store(ro, (col * HEAD_DIM + 4 * quad) * 4, float4{o[0], o[1], o[2], o[3]});
+            if (quad == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(any_bad ? NAN : m), __float_as_uint(l)}, rm,
+                                                      col * 8, 0, SC1);
+        }
+    }
+    __syncthreads();   /* the stages are used again */
+}
+
+/* The merge of a (tile, KV head)'s partials in slots slot0 .. slot0 + chunks - 1, in chunk order, into its bf16 rows. */
+__device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, bool narrow, int chunks, long long slot0) {
+    const AttnArgs &a = p.a;
+    const int cols = narrow ? PK_NARROW_COLS : PK_WIDE_COLS;
+    const PkPart part = pk_part(narrow ? p.part_narrow : p.part_wide, narrow ? p.narrow_slots : p.wide_slots, cols, slot0);
+    constexpr int NB = 4;   /* chunks whose loads are issued together */
+    for (int i = threadIdx.x; i < cols * (HEAD_DIM / 4); i += 256) {
+        const int col = i >> 5, quad = i & 31;
+        const int tok = pk_token(a, it.t0, it.t0 + it.tn, col >> 4, col & 15);   /* a wave's tiles follow the last one's */
+        if (tok < 0) continue;
+        float m = -INFINITY, l = 0.0f;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j0 = 0; j0 < chunks; j0 += NB) {
+            f32x4 oj[NB];
+            float mj[NB], lj[NB];
+#pragma unroll
+            for (int k = 0; k < NB; k++) {
+                const int j = min(j0 + k, chunks - 1);
+                /* sc1: past this XCD's L2, where another workgroup's stores are not seen */
+                const Rsrc ro = page_rsrc(part.o + (long long)j * cols * HEAD_DIM, cols * HEAD_DIM * 4);
+                const Rsrc rm = page_rsrc(part.ml + (long long)j * cols * 2, cols * 8);
+                oj[k] = part_load(ro, (col * HEAD_DIM + 4 * quad) * 4);
+                const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(rm, col * 8, 0, SC1);
+                mj[k] = j0 + k < chunks ? __uint_as_float(w[0]) : -INFINITY;
+                lj[k] = __uint_as_float(w[1]);
+            }
+            float mb = m;
+#pragma unroll
+            for (int k = 0; k < NB; k++) mb = fmaxf(mb, mj[k]);
+            const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mb);
+            o *= keep;
+            l *= keep;
+            m = mb;
+#pragma unroll
+            for (int k = 0; k < NB; k++) {
+                const float f = mj[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mj[k] - mb);   /* NaN: a bad page */
+                o += oj[k] * f;
+                l += lj[k] * f;
+            }
+        }
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = o[k] / l;
+        store_bf16x4(a.out + pk_row(p, it, tok, col & 15) * HEAD_DIM + 4 * quad, v);
+    }
+}
+
+__global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
+    /* [5][B + 1], of the sequences before each: wide items, narrow items, units, wide slots, narrow slots */
+    extern __shared__ int pk_cum[];
+    __shared__ __align__(16) unsigned char stages[PK_STAGES];
+    __shared__ int tab[PK_WIDE_MAX];
+    __shared__ float sh_m[WAVES][PK_NARROW_COLS], sh_l[WAVES][PK_NARROW_COLS];
+    __shared__ long long scan[2][WAVES];
+    __shared__ int sh_next;
+    const AttnArgs &a = p.a;
+    const int B = a.B;
+    int *wide = pk_cum, *narrow = wide + B + 1, *units = narrow + B + 1, *wslots = units + B + 1, *nslots = wslots + B + 1;
+    bool fits = true;
+    {
+        const int per = (B + 255) / 256, b0 = min((int)threadIdx.x * per, B), b1 = min(b0 + per, B);
+        long long items[2] = {0, 0}, slots[2] = {0, 0}, un[2] = {0, 0};
+        for (int b = b0; b < b1; b++) {
+            const PkSeq q = pk_plan(p, b);
+            const int u = max(q.tiles, 0) * a.Hkv, n = u * q.nch;
+            wide[b] = q.narrow ? 0 : n;
+            narrow[b] = q.narrow ? n : 0;
+            wslots[b] = !q.narrow && q.nch > 1 ? n : 0;
+            nslots[b] = q.narrow && q.nch > 1 ? n : 0;
+            units[b] = q.nch > 1 ? u : 0;
+            items[0] += wide[b]; items[1] += narrow[b];
+            slots[0] += wslots[b]; slots[1] += nslots[b];
+            un[0] += units[b];
+        }
+        pk_scan(items, scan);
+        pk_scan(slots, scan);
+        pk_scan(un, scan);
+        for (int b = b0; b < b1; b++) {
+            const int v[5] = {wide[b], narrow[b], units[b], wslots[b], nslots[b]};
+            wide[b] = (int)min(items[0], (long long)INT_MAX); narrow[b] = (int)min(items[1], (long long)INT_MAX);
+            units[b] = (int)min(un[0], (long long)INT_MAX);
+            wslots[b] = (int)min(slots[0], (long long)INT_MAX); nslots[b] = (int)min(slots[1], (long long)INT_MAX);
+            items[0] += v[0]; items[1] += v[1]; un[0] += v[2]; slots[0] += v[3]; slots[1] += v[4];
+        }
+        if (b1 == B && b0 < b1) {
+            wide[B] = (int)min(items[0], (long long)INT_MAX); narrow[B] = (int)min(items[1], (long long)INT_MAX);
+            units[B] = (int)min(un[0], (long long)INT_MAX);
+            wslots[B] = (int)min(slots[0], (long long)INT_MAX); nslots[B] = (int)min(slots[1], (long long)INT_MAX);
+        }
+        __syncthreads();
+        /* row offsets that overlap could ask for more than the host sized the workspace for */
+        fits = wslots[B] <= p.wide_slots && nslots[B] <= p.narrow_slots && units[B] <= p.units &&
+               (long long)wide[B] + narrow[B] < INT_MAX;
+    }
+    /* rows of sequences whose length does not fit */
+    for (int b = blockIdx.x; b < B; b += gridDim.x) {
+        const PkSeq q = pk_plan(p, b);
+        if (q.tiles >= 0 && fits) continue;
+        uint2 *dst = reinterpret_cast<uint2 *>(a.out + (long long)q.row0 * a.Hq * HEAD_DIM);
+        const long long quads = (long long)q.n * a.Hq * (HEAD_DIM / 4);
+        for (long long i = threadIdx.x; i < quads; i += 256) dst[i] = uint2{0x7FC07FC0u, 0x7FC07FC0u};
+    }
+    if (!fits) return;   /* every workgroup: no ticket is taken */
+
+    const int NW = uni(wide[B]), N = uni(NW + narrow[B]), G = gridDim.x;
+    for (int k = blockIdx.x; k < N;) {
+        const bool is_wide = k < NW;
+        const int *cum = is_wide ? wide : narrow;
+        const int kk = is_wide ? k : k - NW;
+        PkItem it;
+        it.b = uni(find_sequence(cum, B, kk));
+        it.q = pk_plan(p, uni(p.cu[it.b]), uni(p.cu[it.b + 1]), uni(a.seq_lens[it.b]));
+        /* a sequence's items: the last tiles first, then the chunks, its KV heads fastest */
+        const int local = uni(kk - cum[it.b]), rest = local / a.Hkv;
+        it.kvh = local - rest * a.Hkv;
+        const int tile = it.q.tiles - 1 - rest / it.q.nch, j = rest % it.q.nch;
+        const int tokens = is_wide ? WAVES * PK_NT * (16 / a.G) : it.q.n;
+        it.t0 = tile * tokens;
+        it.tn = min(it.q.n - it.t0, tokens);
+        /* the tile's own pages, its chunks [j0, j1), this chunk's pages within */
+        const int start = it.q.len - it.q.n;
+        const int lo = ((a.window >= 0 ? max(start + it.t0 - a.window, 0) : 0) / PAGE) & ~1;
+        const int hi = (start + it.t0 + it.tn - 1) / PAGE + 1;
+        const int j0 = (lo - it.q.pg0) / it.q.s, j1 = (hi - 1 - it.q.pg0) / it.q.s + 1;
+        it.pg0 = max(it.q.pg0 + j * it.q.s, lo);
+        it.pg1 = min(it.q.pg0 + (j + 1) * it.q.s, hi);
+        if (it.pg0 < it.pg1) {
+            const int chunks = j1 - j0, unit = uni(units[it.b]) + tile * a.Hkv + it.kvh;
+            const long long slot0 = uni((is_wide ? wslots : nslots)[it.b]) + ((long long)tile * a.Hkv + it.kvh) * it.q.nch;
+            if (is_wide)
+                pk_wide(p, it, chunks, slot0 + j - j0, stages, tab);
+            else if (it.tn <= 16 / a.G)
+                pk_narrow<1>(p, it, chunks, slot0 + j - j0, stages, sh_m, sh_l);
+            else
+                pk_narrow<2>(p, it, chunks, slot0 + j - j0, stages, sh_m, sh_l);
+            if (chunks > 1) {
+                __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* this wave's part of the partial is at the coherent level */
+                __syncthreads();
+                if (threadIdx.x == 0)
+                    sh_next = __hip_atomic_fetch_add(p.arrived + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __syncthreads();
+                const int prior = uni(sh_next);
+                if (prior == chunks - 1) {
+                    pk_merge(p, it, !is_wide, chunks, slot0);
+                    if (threadIdx.x == 0)
+                        __hip_atomic_store(p.arrived + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();   /* sh_next is used again */
+            }
+        }
+        if (N <= G) break;
+        if (threadIdx.x == 0) {   /* queue x holds the items G + x, G + x + 8, ...; its own first, then the others' */
+            int next = INT_MAX;
+            for (int i = 0; i < PK_QUEUES && next == INT_MAX; i++) {
+                const int x = ((int)blockIdx.x + i) % PK_QUEUES;
+                const long long at = G + x;
+                if (at >= N) continue;
+                const int have = (int)((N - at + PK_QUEUES - 1) / PK_QUEUES);
+                if (__hip_atomic_load(p.tickets + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) >= have) continue;
+                const int got = __hip_atomic_fetch_add(p.tickets + x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (got < have) next = (int)(at + (long long)got * PK_QUEUES);
+            }
+            sh_next = next;
+        }
+        __syncthreads();
+        k = uni(sh_next);
+        __syncthreads();
+    }
+    if (N > G && threadIdx.x == 0) {   /* the last workgroup to leave returns the tickets */
+        if (__hip_atomic_fetch_add(p.done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == G - 1) {
+            for (int x = 0; x < PK_QUEUES; x++)
+                __hip_atomic_store(p.tickets + x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(p.done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+}
+
+/* The most partials and arrival counts a launch of these sizes can need, whatever its lengths (pk_plan): a narrow sequence
+ * is Hkv units of ceil(pages / PK_NARROW_SPLIT) chunks. A wide one has at least tpw + 1 rows; all of them together have at
+ * most rows / TW + their number tiles, each Hkv units, cut into at most ceil(pages / PK_WIDE_MIN) chunks, and no sequence
+ * into more than PK_WIDE_ITEMS items unless its chunks would pass PK_WIDE_MAX pages. */
+struct PkSizes {
+    long long wide_slots, narrow_slots, units;
+};
+
+static PkSizes pk_sizes(long long rows, int B, int Hq, int Hkv, int max_seq_len, int window) {
+    const int tpt = 16 / (Hq / Hkv), tpw = tpt * PK_NT;
+    long long np = ((long long)max_seq_len - 1) / PAGE + 1;
+    /* a windowed sequence of n rows sees n + window keys, from an even page */
+    if (window >= 0) np = min(np, (rows + window) / PAGE + 3);
+    const long long nw = min((long long)B, rows / (tpw + 1)), tiles = rows / (WAVES * tpw) + nw;
+    PkSizes z = {};
+    const long long nch = (np - 1) / PK_NARROW_SPLIT + 1, wch = (np - 1) / PK_WIDE_MIN + 1, most = (np - 1) / PK_WIDE_MAX + 1;
+    if (nch > 1) z.narrow_slots = min((long long)B, rows) * Hkv * nch;
+    if (wch > 1) z.wide_slots = min(tiles * Hkv * wch, nw * PK_WIDE_ITEMS + (most > 1 ? tiles * Hkv * most : 0));
+    z.units = (nch > 1 ? min((long long)B, rows) : 0) * Hkv + (wch > 1 ? tiles * Hkv : 0);
+    return z;
+}
+
+static size_t pk_part_bytes(const PkSizes &z) {
+    return (size_t)(z.wide_slots * PK_WIDE_COLS + z.narrow_slots * PK_NARROW_COLS) * (HEAD_DIM + 2) * sizeof(float);
+}
+
+/* As attention.hip's decode workspace: partials from the start, int32 counts (tickets, done, arrivals) in the last 1/256,
+ * whose place depends on the workspace's size alone. */
+static size_t pk_count_region(size_t bytes) { return (bytes - ((bytes >> 8) & ~(size_t)3)) & ~(size_t)3; }
+static size_t pk_count_bytes(const PkSizes &z) { return (size_t)(z.units + PK_QUEUES + 1) * sizeof(int); }
+
+static bool pk_shape_ok(long long rows, int B, int Hq, int Hkv, int max_seq_len) {
+    return rows > 0 && rows <= 1LL << 24 && B > 0 && B <= PK_MAX_BATCH && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 &&
+           Hq / Hkv <= 16 && Hkv <= 1024 && max_seq_len > 0;
+}
+
+static int device_packed_grid() {
+    static int grid[64] = {0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 512;
+    if (!grid[dev]) grid[dev] = 2 * device_cus() / PK_QUEUES * PK_QUEUES;
+    return max(grid[dev], PK_QUEUES);
+}
+
+}  // namespace nc
+
+using namespace nc;
+
+extern "C" size_t nc_packed_workspace_bytes(long long rows, int B, int Hq, int Hkv, int max_seq_len, int window) {
+    if (!pk_shape_ok(rows, B, Hq, Hkv, max_seq_len)) return 0;
+    const PkSizes z = pk_sizes(rows, B, Hq, Hkv, max_seq_len, window);
+    if (z.wide_slots > INT_MAX || z.narrow_slots > INT_MAX || z.units > INT_MAX / 2) return 0;
+    size_t k = max((pk_part_bytes(z) + 254) / 255, pk_count_bytes(z));
+    return 256 * ((k + 3) & ~(size_t)3);
+}
+
+extern "C" int nc_packed_attn_fp8(const void *q, const void *k_pages, const void *v_pages, const float *kv_scale,
+                                  const int32_t *block_table, int max_pages, int num_pages, const int32_t *cu_seqlens,
+                                  const int32_t *seq_lens, long long rows, int B, int Hq, int Hkv, int max_seq_len,
+                                  int window, float sm_scale, void *out, void *workspace, size_t workspace_bytes,
+                                  void *stream) {
+    if (!q || !k_pages || !v_pages || !kv_scale || !block_table || !cu_seqlens || !seq_lens || !out || !workspace)
+        return NC_ERR_NULL;
+    if (!pk_shape_ok(rows, B, Hq, Hkv, max_seq_len) || max_pages <= 0 || num_pages <= 0 ||
+        (long long)max_pages * PAGE < max_seq_len)
+        return NC_ERR_SHAPE;
+    const size_t need = nc_packed_workspace_bytes(rows, B, Hq, Hkv, max_seq_len, window);
+    if (need == 0) return NC_ERR_SHAPE;
+    const PkSizes z = pk_sizes(rows, B, Hq, Hkv, max_seq_len, window);
+    const size_t counts = pk_count_region(workspace_bytes);
+    if (pk_part_bytes(z) > counts || pk_count_bytes(z) > workspace_bytes - counts) return NC_ERR_WORKSPACE;
+    PackedArgs p = {};
+    AttnArgs &a = p.a;
+    a.q = (const uint16_t *)q;
+    a.k_pages = (const uint8_t *)k_pages; a.v_pages = (const uint8_t *)v_pages; a.kv_scale = kv_scale;
+    a.block_table = block_table; a.max_pages = max_pages; a.num_pages = num_pages;
+    a.seq_lens = seq_lens;
+    a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.window = window;
+    a.scale_log2 = sm_scale * LOG2E;
+    a.max_len = max_seq_len;
+    a.out = (uint16_t *)out;
+    p.cu = cu_seqlens;
+    p.rows = (int)rows;
+    p.part_wide = (float *)workspace;
+    p.part_narrow = p.part_wide + z.wide_slots * PK_WIDE_COLS * (HEAD_DIM + 2);
+    p.wide_slots = z.wide_slots; p.narrow_slots = z.narrow_slots;
+    p.units = (int)z.units;
+    p.tickets = (int *)((char *)workspace + counts);
+    p.done = p.tickets + PK_QUEUES;
+    p.arrived = p.done + 1;
+    hipLaunchKernelGGL(packed_attn_kernel, dim3(device_packed_grid()), dim3(256), 5 * (B + 1) * sizeof(int),
+                       (hipStream_t)stream, p);
+    return (int)hipGetLastError();
+}

@@ -28,7 +28,7 @@ LIB_DIR = PACKAGE / "lib"
 LIBRARY = LIB_DIR / "libnanochat_kv.so"
 DECODE_LIBRARY = LIB_DIR / "libnanochat_decode.so"
 KERNEL_SOURCES = [CSRC / "kv_append.hip", CSRC / "attention.hip", CSRC / "ve_gate.hip", CSRC / "flash_attn.hip",
-                  CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip", CSRC / "paging.hip", CSRC / "sample.hip"]
+                  CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip", CSRC / "paging.hip", CSRC / "sample.hip", CSRC / "packed_attn.hip"]
 DECODE_SOURCES = [CSRC / "decoder.hip", CSRC / "slot_gemm.hip"]
 SOURCES = KERNEL_SOURCES + DECODE_SOURCES
 HEADERS = [CSRC / "nc_device.h", CSRC / "nc_internal.h", CSRC / "nc_row.h", CSRC / "nc_attend.h", INCLUDE / "nanochat_amd.h", INCLUDE / "nanochat_decode.h"]
@@ -96,6 +96,9 @@ SIGNATURES = {
                                     c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_void_p], c_int),
     "nc_prefill_attn_fp8": ([c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int,
                              c_int, c_int, c_int, c_float, c_void_p, c_void_p], c_int),
+    "nc_packed_workspace_bytes": ([c_longlong] + [c_int] * 5, c_size_t),
+    "nc_packed_attn_fp8": ([c_void_p] * 5 + [c_int, c_int, c_void_p, c_void_p, c_longlong] + [c_int] * 5 +
+                           [c_float, c_void_p, c_void_p, c_size_t, c_void_p], c_int),
     "nc_debug_read_pages": ([c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_void_p], c_int),
     "ve_forward": ([c_void_p, c_void_p, c_longlong] + [c_void_p] * 5 + [c_longlong, c_void_p], None),
     "ve_backward": ([c_void_p, c_longlong] + [c_void_p] * 8 + [c_longlong, c_void_p], None),

@@ -57,6 +57,62 @@ def test_append_rows_rejects(lib):
     assert lib.nc_qk_norm_rope_append_rows_fp8(*append_args(rows=0)) == 0
 
 
+def packed_args(**over):
+    args = dict(q=DUMMY, k_pages=DUMMY, v_pages=DUMMY, kv_scale=DUMMY, block_table=DUMMY, max_pages=16, num_pages=8,
+                cu_seqlens=DUMMY, seq_lens=DUMMY, rows=4, B=2, Hq=16, Hkv=4, max_seq_len=256, window=-1, sm_scale=0.1,
+                out=DUMMY, workspace=DUMMY, workspace_bytes=1 << 30, stream=None)
+    return list((args | over).values())
+
+
+def test_packed_attention_rejects(lib):
+    for name in ("q", "k_pages", "v_pages", "kv_scale", "block_table", "cu_seqlens", "seq_lens", "out", "workspace"):
+        assert lib.nc_packed_attn_fp8(*packed_args(**{name: None})) == -1, name
+    for over in (dict(rows=0), dict(rows=2 ** 24 + 1), dict(B=0), dict(B=1025), dict(Hq=6), dict(Hq=68), dict(Hkv=0),
+                 dict(max_seq_len=0), dict(max_seq_len=257), dict(max_pages=0), dict(num_pages=0)):
+        assert lib.nc_packed_attn_fp8(*packed_args(**over)) == -2, over
+    need = lib.nc_packed_workspace_bytes(4096, 64, 16, 4, 8192, -1)
+    assert need > 0
+    assert lib.nc_packed_attn_fp8(*packed_args(rows=4096, B=64, max_pages=512, max_seq_len=8192,
+                                               workspace_bytes=need - 1024)) == -3
+
+
+def plan(rows, n, length, hq, hkv, window):
+    """The cut of a sequence as packed_attn.hip's pk_plan makes it: (units, items, partials a kind)."""
+    tpt, page = 16 // (hq // hkv), 16
+    first = max(length - n - window, 0) if window >= 0 else 0
+    pg0 = first // page & ~1
+    pages = (length - 1) // page + 1 - pg0
+    if n <= 2 * tpt:
+        tiles, cut = 1, 128
+    else:
+        tiles = (n - 1) // (8 * tpt) + 1
+        want = max(256 // (tiles * hkv), 1)
+        cut = min(max(((pages - 1) // want + 1 + 31) & ~31, 128), 1024)
+    chunks = (pages - 1) // cut + 1
+    return (n <= 2 * tpt, tiles * hkv * chunks if chunks > 1 else 0, tiles * hkv if chunks > 1 else 0)
+
+
+def test_packed_workspace_holds_every_launch(lib):
+    """Whatever the lengths, the partials and counts of a launch fit what the host asked for (the kernel refuses the rest)."""
+    import random
+
+    rng = random.Random(0)
+    for _ in range(3000):
+        hq, hkv = rng.choice([(4, 4), (16, 4), (16, 1), (13, 13), (10, 2)])
+        batch, most = rng.randint(1, 40), rng.choice([100, 3000, 20000, 70000])
+        window = rng.choice([-1, -1, 0, 700, 30000])
+        new = [min(rng.choice([0, 1, 3, 33, 200, 3000]), most) for _ in range(batch)]
+        rows = max(sum(new), 1) + rng.choice([0, 5])
+        lens = [rng.randint(max(n, 1), most) if rng.random() < 0.7 else most for n in new]
+        plans = [plan(rows, n, length, hq, hkv, window) for n, length in zip(new, lens) if n]
+        wide = sum(p[1] for p in plans if not p[0])
+        narrow = sum(p[1] for p in plans if p[0])
+        parts = (wide * 128 + narrow * 32) * 130 * 4
+        counts = 4 * (sum(p[2] for p in plans) + 9)
+        need = lib.nc_packed_workspace_bytes(rows, batch, hq, hkv, most, window)
+        assert parts <= need - need // 256 and counts <= need // 256, (hq, hkv, new, lens, window)
+
+
 def sample_args(**over):
     args = dict(logits=DUMMY, is_bf16=0, row_stride=100, rows=4, vocab=100, uniform=DUMMY, temperature=DUMMY, top_k=None,
                 top_p=None, min_p=None, mask=None, mask_stride=0, tokens=DUMMY, stream=None)
