@@ -12,16 +12,17 @@
  * below about 80 columns (rows times the heads of a KV head) the pages' bytes take longer than the products. Hence two
  * kinds of work items, each one workgroup of four waves, both streaming pages into LDS by asynchronous copies:
  *
- *   narrow  at most 32 columns: the four waves take the chunk's page pairs in turn, each through a ring of its own with two
- *           pairs in flight and no barrier, and merge their four softmax states through LDS at the end
- *   wide    a tile of up to 128 columns, 32 a wave: all waves walk the same pairs, each pair fetched once (PK_AHEAD ahead)
+ *   narrow  at most 32 columns: one wave takes a chunk of the keys by itself, page pairs through a ring of its own in LDS
+ *           with two pairs in flight; waves meet at no barrier, so one's start or merge hides behind the others' streams
+ *   wide    a tile of up to 128 columns, 32 a wave: the four waves of a workgroup walk the same pairs, each fetched once
+ *           (PK_AHEAD ahead)
  *
  * A sequence's keys are cut into chunks (pk_plan), so that few rows over many keys still fill the chip; a (tile, KV head)
- * of several chunks leaves one partial (O, max, sum) in fp32 a chunk, and the workgroup that finishes its last chunk merges
- * them in order. The cuts depend on nothing but the sequence's own numbers, so its output bits do not depend on the rest
- * of the launch. Items are taken in the order wide, narrow: the first by workgroup index, later ones from eight queues
- * (an XCD's workgroups take every eighth item, which keeps a KV head's pages in that XCD's L2), so that unequal items even
- * out.
+ * of several chunks leaves one partial (O, max, sum) in fp32 a chunk, and whoever finishes its last chunk merges them in
+ * order. The cuts depend on nothing but the sequence's own numbers, so its output bits do not depend on the rest of the
+ * launch. A workgroup takes wide items while there are any, then its waves narrow ones: the first by workgroup index, later
+ * ones from eight queues (an XCD's workgroups take every eighth item, which keeps a KV head's pages in that XCD's L2), so
+ * that unequal items even out.
  */
 #include <limits.h>
 
@@ -35,12 +36,15 @@ constexpr int PK_NARROW_COLS = 16 * PK_NT;
 constexpr int PK_WIDE_COLS = WAVES * 16 * PK_NT;
 constexpr int PK_MAX_BATCH = 1024;
 constexpr int PK_QUEUES = 8;                   /* XCDs */
-constexpr int PK_NARROW_SPLIT = 128;           /* pages of a narrow chunk */
+constexpr int PK_NARROW_SPLIT = 64;            /* pages of a narrow chunk */
+constexpr int PK_SHORT_SPLIT = 16;             /* of one of a sequence of at most PK_SHORT pages */
+constexpr int PK_MIN_TAIL = 4;                 /* a last chunk of fewer pages joins the one before it */
+constexpr int PK_SHORT = PK_NARROW_SPLIT + PK_MIN_TAIL - 1;
 constexpr int PK_WIDE_MIN = 128;               /* least and most pages of a wide chunk */
 constexpr int PK_WIDE_MAX = 1024;
 constexpr int PK_WIDE_ITEMS = 256;             /* items a wide sequence is cut into at most, if its chunks stay that long */
 constexpr int PK_AHEAD = 3;                    /* wide: pairs in flight */
-static_assert(PK_NARROW_SPLIT <= 256, "a wave's block-table entries of a narrow chunk: one a lane");
+static_assert(PK_SHORT <= 2 * WAVE, "a narrow chunk's block-table entries: two a lane");
 
 /* One stage: the pair's K (2 x 2 KiB), V (2 x 2 KiB) and scales (per page 16 of K, then 16 of V; wide: a copy a wave). */
 constexpr int PK_SCALE_AT = 4 * PAGE_BYTES, PK_SCALE_BYTES = 256;
@@ -48,7 +52,6 @@ constexpr int PK_WIDE_STAGE = PK_SCALE_AT + WAVES * PK_SCALE_BYTES, PK_WIDE_BUFS
 constexpr int PK_NARROW_STAGE = PK_SCALE_AT + PK_SCALE_BYTES, PK_NARROW_BUFS = 2;
 constexpr int PK_STAGES = WAVES * PK_NARROW_BUFS * PK_NARROW_STAGE;   /* bytes of LDS */
 static_assert(PK_WIDE_BUFS * PK_WIDE_STAGE <= PK_STAGES, "the wide stages fit");
-static_assert(WAVES * PK_NARROW_COLS * O_PITCH * 4 <= PK_STAGES, "the narrow merge fits");
 typedef __attribute__((address_space(3))) void LdsVoid;
 
 struct PackedArgs {
@@ -58,7 +61,7 @@ struct PackedArgs {
     float *part_wide, *part_narrow;   /* [slots][cols][128] O, then [slots][cols][2] (max, sum) */
     long long wide_slots, narrow_slots;
     int units;                  /* arrival counts */
-    int *tickets, *done, *arrived;    /* [8], [1], [units]; zero between launches */
+    int *tickets, *done, *arrived;    /* [2][8] (wide, narrow), [1], [units]; zero between launches */
 };
 
 /* A sequence's rows, its pages [pg0, pg0 + np) (pg0 even) and how they are cut: nch chunks of s pages from pg0. tiles = 0:
@@ -86,13 +89,15 @@ __device__ __forceinline__ PkSeq pk_plan(const PackedArgs &p, int cu0, int cu1, 
     q.narrow = q.n <= tpw;
     if (q.narrow) {
         q.tiles = 1;
-        q.s = PK_NARROW_SPLIT;
+        q.s = q.np <= PK_SHORT ? PK_SHORT_SPLIT : PK_NARROW_SPLIT;
+        q.nch = (q.np - 1) / q.s + 1;
+        q.nch -= q.nch > 1 && q.np - (q.nch - 1) * q.s < PK_MIN_TAIL;
     } else {
         q.tiles = (q.n - 1) / (WAVES * tpw) + 1;
         const int want = max(PK_WIDE_ITEMS / (q.tiles * a.Hkv), 1);
         q.s = min(max(((q.np - 1) / want + 1 + 31) & ~31, PK_WIDE_MIN), PK_WIDE_MAX);
+        q.nch = (q.np - 1) / q.s + 1;
     }
-    q.nch = (q.np - 1) / q.s + 1;
     return q;
 }
 
@@ -170,10 +175,18 @@ __device__ __forceinline__ long long pk_row(const PackedArgs &p, const PkItem &i
     return ((long long)it.q.row0 + tok) * p.a.Hq + it.kvh * p.a.G + c % p.a.G;
 }
 
+/* Keys of a wave: in tile t a lane's column sees [lo[t], hi[t]]; the pairs from page in0 (even) up to in1 are seen whole by
+ * every column; keys past written_hi are not cache contents. */
+template <int NT>
+struct PkBounds {
+    int lo[NT], hi[NT];
+    int in0, in1, written_hi;
+};
+
 /* Per-column key bounds of a wave whose first token is wt0 (end: one past the item's last), and its query operand. */
 template <int NT>
 __device__ __forceinline__ void pk_columns(const PackedArgs &p, const PkItem &it, int wt0, int end, int lane,
-                                           KeyBounds<NT> &kb, uint4 (&raw)[NT][4]) {
+                                           PkBounds<NT> &kb, uint4 (&raw)[NT][4]) {
     const AttnArgs &a = p.a;
     const int c = lane & 15, g = lane >> 4, start = it.q.len - it.q.n, tpt = 16 / a.G;
 #pragma unroll
@@ -187,9 +200,10 @@ __device__ __forceinline__ void pk_columns(const PackedArgs &p, const PkItem &it
                                   : uint4{0u, 0u, 0u, 0u};
     }
     const int last = min(wt0 + NT * tpt, end) - 1;
-    kb.full_hi = start + wt0;
-    kb.full_lo = a.window >= 0 ? max(start + last - a.window, 0) : 0;
     kb.written_hi = it.q.len - 1;
+    const int whole_lo = a.window >= 0 ? max(start + last - a.window, 0) : 0, whole_hi = min(start + wt0, kb.written_hi);
+    kb.in0 = ((whole_lo + PAGE - 1) / PAGE + 1) & ~1;
+    kb.in1 = min((whole_hi + 1) / PAGE, it.pg1) & ~1;
 }
 
 /* A pair's operands from a stage: four 16-byte reads a lane (K: at = the stage's LDS byte, V: 4 KiB on) and the lane's
@@ -216,100 +230,173 @@ __device__ __forceinline__ void pk_read(int at, int sc, int lane, PairRegs &k) {
     k.sb = float4{__uint_as_float(sb[0]), __uint_as_float(sb[1]), __uint_as_float(sb[2]), __uint_as_float(sb[3])};
 }
 
+/* Four zeros in registers of their own, for the products that start a sum (the compiler would set them anew each time). */
+__device__ __forceinline__ f32x4 pk_zero() {
+    f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+    asm volatile("" : "+v"(z));
+    return z;
+}
+
+/* x, of which nothing is computed before this point (work of rare paths would move ahead of their branches). */
+__device__ __forceinline__ int pk_here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 /* A stage's place in LDS, for one wave. */
 struct PkAt {
     int at, scales;
 };
 
-/* One pair's scores, softmax and PV, as nc_attend.h's pair_update (same sums, same lazy rescale: a column keeps its
- * reference maximum until a score passes it by 8 in log2) but tile after tile, so that one tile's scores and exponentials
- * are live at a time. MASKED: some key of the pair is not seen by some column, or not written. What is not seen takes no
- * part whatever its bytes: its exponential and its product with the V scale are replaced by zero, and the V codes of keys
- * that are not written are cleared. */
-template <int NT, bool MASKED, typename Freed>
-__device__ __forceinline__ void pk_update(int lpa, bool has_b, PkAt stage, const QOp (&qb)[NT], const KeyBounds<NT> &kb,
-                                          WaveState<NT> &st, int lane, Freed freed) {
-    const int key_a = lpa * PAGE + (lane >> 4) * 4, key_b = key_a + PAGE;
+constexpr float PK_RESCALE = 2048.0f;
+
+/* One pair's scores, softmax and PV. The lazy rescale, as in nc_attend.h: a column keeps its reference maximum m, and its
+ * exponentials p = exp2(s - m) grow past one, until the sum of a lane's eight passes PK_RESCALE (the sum is made anyway,
+ * where the largest would take eight more instructions); then the column moves to its new maximum. The decision and what
+ * it does depend on the column's own scores. A pair that holds keys which some column does not see, or that are not
+ * written, is masked: what is not seen takes no part whatever its bytes (its exponential and its product with the V scale
+ * are replaced by zero, and the V codes of keys that are not written are cleared). freed() is called once the stage's
+ * bytes are in registers. */
+template <int NT, typename Freed>
+__device__ __forceinline__ void pk_pair(int lpa, bool has_b, PkAt stage, const QOp (&qb)[NT], const PkBounds<NT> &kb,
+                                        const f32x4 &zero, WaveState<NT> &st, int lane, Freed freed) {
+    const int key_a = lpa * PAGE + (lane >> 4) * 4;
     PairRegs k, v;
     pk_read(stage.at, stage.scales, lane, k);
-    f32x4 sa[NT], sb[NT];
-    __builtin_amdgcn_s_setprio(1);   /* the other wave of the SIMD runs its VALU while these products issue */
-    page_scores<NT>(k.a0, k.a1, qb, sa);
-    page_scores<NT>(k.b0, k.b1, qb, sb);
-    __builtin_amdgcn_s_setprio(0);
+    f32x4 sc[NT][2];
+    {
+        const i32x8 a = {(int)k.a0.x, (int)k.a0.y, (int)k.a0.z, (int)k.a0.w, (int)k.a1.x, (int)k.a1.y, (int)k.a1.z, (int)k.a1.w};
+        const i32x8 b = {(int)k.b0.x, (int)k.b0.y, (int)k.b0.z, (int)k.b0.w, (int)k.b1.x, (int)k.b1.y, (int)k.b1.z, (int)k.b1.w};
+        __builtin_amdgcn_s_setprio(1);   /* the other wave of the SIMD runs its VALU while these products issue */
+#pragma unroll
+        for (int t = 0; t < NT; t++) {   /* independent products between two that add up */
+            sc[t][0] = mfma_fp8(a, qb[t].hi, qb[t].scale, zero);
+            sc[t][1] = mfma_fp8(b, qb[t].hi, qb[t].scale, zero);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            sc[t][0] = mfma_fp8(a, qb[t].lo, qb[t].scale, sc[t][0]);
+            sc[t][1] = mfma_fp8(b, qb[t].lo, qb[t].scale, sc[t][1]);
+        }
+        __builtin_amdgcn_s_setprio(0);
+    }
     __builtin_amdgcn_sched_barrier(0);   /* K's registers are free, and V's reads take less than the products */
-    pk_read(stage.at + 2 * PAGE_BYTES, stage.scales + PAGE * 4, lane, v);
-    freed();
-    if (MASKED) {
-        const int na = min(max(kb.written_hi - key_a + 1, 0), 4), nb = has_b ? min(max(kb.written_hi - key_b + 1, 0), 4) : 0;
+    const float ks[8] = {k.sa.x * st.sl2, k.sa.y * st.sl2, k.sa.z * st.sl2, k.sa.w * st.sl2,
+                         k.sb.x * st.sl2, k.sb.y * st.sl2, k.sb.z * st.sl2, k.sb.w * st.sl2};
+    const auto vs = [&](int i) { return i < 4 ? (&v.sa.x)[i] : (&v.sb.x)[i - 4]; };
+    /* key: the lane's first key of page a */
+    const auto seen = [&](int key, int t, int i) {
+        key += (i < 4 ? 0 : PAGE) + (i & 3);
+        return (i < 4 || has_b) && key >= kb.lo[t] && key <= kb.hi[t];
+    };
+    const auto sum8 = [](const float (&x)[8]) {
+        return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    };
+    float pv[NT][8], sum[NT];
+    if (lpa >= kb.in0 && lpa < kb.in1) {   /* V is read on both paths: one path's changes to it cost the other no copy */
+        pk_read(stage.at + 2 * PAGE_BYTES, stage.scales + PAGE * 4, lane, v);
+        freed();
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float negm = -st.m[t];   /* +inf before the first key: every p is +inf, the slow path */
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], ks[i], negm));
+            sum[t] = sum8(e);
+#pragma unroll
+            for (int i = 0; i < 8; i++) pv[t][i] = e[i] * vs(i);
+        }
+    } else {
+        const int key = pk_here(key_a);
+        pk_read(stage.at + 2 * PAGE_BYTES, stage.scales + PAGE * 4, lane, v);
+        freed();
+        const int na = min(max(kb.written_hi - key + 1, 0), 4), nb = has_b ? min(max(kb.written_hi - key - PAGE + 1, 0), 4) : 0;
         const uint32_t ma = na >= 4 ? 0xFFFFFFFFu : (1u << (8 * na)) - 1u, mb = nb >= 4 ? 0xFFFFFFFFu : (1u << (8 * nb)) - 1u;
         v.a0 = and4(v.a0, ma); v.a1 = and4(v.a1, ma);
         v.b0 = and4(v.b0, mb); v.b1 = and4(v.b1, mb);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float negm = -st.m[t];
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], ks[i], negm));
+                e[i] = seen(key, t, i) ? e[i] : 0.0f;
+                pv[t][i] = seen(key, t, i) ? e[i] * vs(i) : 0.0f;
+            }
+            sum[t] = sum8(e);
+        }
     }
-    const float ks[8] = {k.sa.x * st.sl2, k.sa.y * st.sl2, k.sa.z * st.sl2, k.sa.w * st.sl2,
-                         k.sb.x * st.sl2, k.sb.y * st.sl2, k.sb.z * st.sl2, k.sb.w * st.sl2};
-    const float vs[8] = {v.sa.x, v.sa.y, v.sa.z, v.sa.w, v.sb.x, v.sb.y, v.sb.z, v.sb.w};
-    bf16x8 pv[NT];
+    bool fine = true;
+#pragma unroll
+    for (int t = 0; t < NT; t++) fine = fine && sum[t] <= PK_RESCALE;
+    if (__any(!fine)) {
+        const int key = pk_here(key_a);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            /* by selections, not a branch a lane */
+            const bool move = pair_max32(pair_max16(sum[t])) > PK_RESCALE;   /* the column's largest over its four groups */
+            float mt = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; i++) mt = fmaxf(mt, seen(key, t, i) ? sc[t][i >> 2][i & 3] * ks[i] : -INFINITY);
+            mt = pair_max32(pair_max16(mt));
+            const float mnew = move ? fmaxf(st.m[t], mt) : st.m[t];
+            const float alpha = mnew == st.m[t] ? 1.0f : __builtin_amdgcn_exp2f(st.m[t] - mnew);
+            const float base = mnew == -INFINITY ? 0.0f : mnew;
+#pragma unroll
+            for (int d = 0; d < 8; d++) st.o[t][d] *= alpha;
+            st.l[t] *= alpha;
+            st.m[t] = mnew;
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], ks[i], -base));
+                e[i] = seen(key, t, i) ? e[i] : 0.0f;
+                pv[t][i] = seen(key, t, i) ? e[i] * vs(i) : 0.0f;
+            }
+            sum[t] = sum8(e);
+        }
+    }
+    bf16x8 pb[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        const auto seen = [&](int i) {
-            const int key = (i < 4 ? key_a : key_b) + (i & 3);
-            return !MASKED || ((i < 4 || has_b) && key >= kb.lo[t] && key <= kb.hi[t]);
-        };
-        const float negm = -st.m[t];   /* +inf before the first key: every live p is +inf, the slow path */
-        float p[8], most = 0.0f;
+        st.l[t] += sum[t];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(i < 4 ? sa[t][i] : sb[t][i - 4], ks[i], negm));
-            p[i] = seen(i) ? e : 0.0f;
-            most = fmaxf(most, p[i]);
-        }
-        if (__any(!(most <= 256.0f))) {   /* a column's maximum passed its reference by more than 2^8 (or has none yet) */
-            const float pc = pair_max32(pair_max16(most));   /* the column's largest over its four row groups */
-            if (pc > 256.0f) {
-                float sc[8], mt = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    sc[i] = seen(i) ? (i < 4 ? sa[t][i] : sb[t][i - 4]) * ks[i] : -INFINITY;
-                    mt = fmaxf(mt, sc[i]);
-                }
-                mt = pair_max32(pair_max16(mt));
-                const float mnew = fmaxf(st.m[t], mt);
-                const float alpha = mnew == st.m[t] ? 1.0f : __builtin_amdgcn_exp2f(st.m[t] - mnew);
-#pragma unroll
-                for (int d = 0; d < 8; d++) st.o[t][d] *= alpha;
-                st.l[t] *= alpha;
-                st.m[t] = mnew;
-                const float base = mnew == -INFINITY ? 0.0f : mnew;
-#pragma unroll
-                for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(sc[i] - base);
-            }
-        }
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            sum += p[i];
-            pv[t][i] = (__bf16)(seen(i) ? p[i] * vs[i] : 0.0f);
-        }
-        st.l[t] += sum;
+        for (int i = 0; i < 8; i++) pb[t][i] = (__bf16)pv[t][i];
     }
 #pragma unroll
     for (int d = 0; d < 8; d++) {
         const bf16x8 va = fp8x8_to_bf16(dword(d < 4 ? v.a0 : v.a1, d & 3), dword(d < 4 ? v.b0 : v.b1, d & 3));
 #pragma unroll
-        for (int t = 0; t < NT; t++) st.o[t][d] = mfma16x16x32(va, pv[t], st.o[t][d]);
+        for (int t = 0; t < NT; t++) st.o[t][d] = mfma16x16x32(va, pb[t], st.o[t][d]);
     }
 }
 
-/* freed() is called once the stage's bytes are in registers. */
-template <int NT, typename Freed>
-__device__ __forceinline__ void pk_pair(int lpa, bool has_b, PkAt stage, const QOp (&qb)[NT], const KeyBounds<NT> &kb,
-                                        WaveState<NT> &st, int lane, Freed freed) {
-    const int end = lpa * PAGE + 2 * PAGE - 1;
-    if (has_b && lpa * PAGE >= kb.full_lo && end <= kb.full_hi && end <= kb.written_hi)
-        pk_update<NT, false>(lpa, has_b, stage, qb, kb, st, lane, freed);
-    else
-        pk_update<NT, true>(lpa, has_b, stage, qb, kb, st, lane, freed);
+/* Column `col` (c of tile t, token tok; < 0: none) of a wave's state: its bf16 row, or its part of a partial. */
+template <int NT>
+__device__ __forceinline__ void pk_store(const PackedArgs &p, const PkItem &it, int chunks, WaveState<NT> &ws, int t, int tok,
+                                         int col, int c, int g, Rsrc ro, Rsrc rm) {
+    ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
+    if (tok < 0) return;
+    if (chunks == 1) {
+        uint16_t *dst = p.a.out + pk_row(p, it, tok, c) * HEAD_DIM;
+        const float inv = 1.0f / ws.l[t];
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = ws.bad ? NAN : ws.o[t][d][i] * inv;
+            store_bf16x4(dst + 16 * d + 4 * g, v);
+        }
+    } else {
+#pragma unroll
+        for (int d = 0; d < 8; d++)
+            part_store(ro, (col * HEAD_DIM + 16 * d + 4 * g) * 4,
+                       float4{ws.o[t][d][0], ws.o[t][d][1], ws.o[t][d][2], ws.o[t][d][3]});
+        if (g == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(
+                u32x2{__float_as_uint(ws.bad ? NAN : ws.m[t]), __float_as_uint(ws.l[t])}, rm, col * 8, 0, SC1);
+    }
 }
 
 /* --- wide items */
@@ -348,7 +435,7 @@ __device__ __forceinline__ void pk_wide(const PackedArgs &p, const PkItem &it, i
         const int e = bt[i];
         tab[i] = (unsigned)e < (unsigned)a.num_pages ? e : -1;
     }
-    KeyBounds<PK_NT> kb;
+    PkBounds<PK_NT> kb;
     uint4 raw[PK_NT][4];
     pk_columns<PK_NT>(p, it, wt0, end, lane, kb, raw);
     QOp qb[PK_NT];
@@ -363,53 +450,40 @@ __device__ __forceinline__ void pk_wide(const PackedArgs &p, const PkItem &it, i
     for (int i = threadIdx.x; i < npages; i += 256) tab[i] = max(tab[i], 0);   /* only read: those waves report NaN */
     __syncthreads();
 
+    const f32x4 zero = pk_zero();
     const int lds = pk_lds_offset(stages), count = (npages + 1) / 2;
     for (int s = 0; s < PK_AHEAD; s++) pk_fetch_wide(a, tab, npages, s, it.kvh, stages + s * PK_WIDE_STAGE, wave, lane);
     /* step s: this wave's copies of stage s have landed (then everyone's, after the barrier, and everyone's reads of the
-     * stage before are done); refill that buffer with stage s + PK_AHEAD; compute stage s */
-    for (int s = 0, buf = 0; s < count; s++) {
+     * stage before are done); refill that buffer with stage s + PK_AHEAD; compute stage s where it meets this wave's pages.
+     * Loops of their own for the stages before and after those: a branch around the pair inside one loop would cost a copy
+     * of the accumulators a step */
+    int s = 0, buf = 0;
+    const auto advance = [&]() {
         __builtin_amdgcn_s_waitcnt(pk_wait(3 * (PK_AHEAD - 1), 15));
         pk_barrier();
         const int into = buf == 0 ? PK_WIDE_BUFS - 1 : buf - 1;   /* (s + PK_AHEAD) % PK_WIDE_BUFS */
         pk_fetch_wide(a, tab, npages, s + PK_AHEAD, it.kvh, stages + into * PK_WIDE_STAGE, wave, lane);
-        const int lpa = it.pg0 + 2 * s;
-        if (lpa + 1 >= w0 && lpa < w1) {
-            const int at = lds + buf * PK_WIDE_STAGE;
-            pk_pair<PK_NT>(lpa, 2 * s + 1 < npages, PkAt{at, at + PK_SCALE_AT + wave * PK_SCALE_BYTES}, qb, kb, ws, lane, [] {});
-        }
+    };
+    const auto next = [&]() {
+        s++;
         buf = buf == PK_WIDE_BUFS - 1 ? 0 : buf + 1;
+    };
+    const int s0 = min(max(w0 - it.pg0, 0) / 2, count), s1 = min(max(w1 - it.pg0 + 1, 0) / 2, count);
+    for (; s < s0; next()) advance();
+    for (; s < s1; next()) {
+        advance();
+        const int at = lds + buf * PK_WIDE_STAGE, lpa = it.pg0 + 2 * s;
+        pk_pair<PK_NT>(lpa, lpa + 1 < it.pg1, PkAt{at, at + PK_SCALE_AT + wave * PK_SCALE_BYTES}, qb, kb, zero, ws, lane, [] {});
     }
+    for (; s < count; next()) advance();
     __builtin_amdgcn_s_waitcnt(0);   /* every copy has landed before the stages and the table are used again */
     pk_barrier();
 
     const PkPart part = pk_part(p.part_wide, p.wide_slots, PK_WIDE_COLS, slot);
     const Rsrc ro = page_rsrc(part.o, PK_WIDE_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_WIDE_COLS * 8);
 #pragma unroll
-    for (int t = 0; t < PK_NT; t++) {
-        ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
-        const int tok = pk_token(a, wt0, end, t, c);
-        if (tok < 0) continue;
-        if (chunks == 1) {
-            uint16_t *dst = a.out + pk_row(p, it, tok, c) * HEAD_DIM;
-            const float inv = 1.0f / ws.l[t];
-#pragma unroll
-            for (int d = 0; d < 8; d++) {
-                float v[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = ws.bad ? NAN : ws.o[t][d][i] * inv;
-                store_bf16x4(dst + 16 * d + 4 * g, v);
-            }
-        } else {
-            const int col = (wave * PK_NT + t) * 16 + c;
-#pragma unroll
-            for (int d = 0; d < 8; d++)
-                part_store(ro, (col * HEAD_DIM + 16 * d + 4 * g) * 4,
-                           float4{ws.o[t][d][0], ws.o[t][d][1], ws.o[t][d][2], ws.o[t][d][3]});
-            if (g == 0)
-                __builtin_amdgcn_raw_buffer_store_b64(
-                    u32x2{__float_as_uint(ws.bad ? NAN : ws.m[t]), __float_as_uint(ws.l[t])}, rm, col * 8, 0, SC1);
-        }
-    }
+    for (int t = 0; t < PK_NT; t++)
+        pk_store<PK_NT>(p, it, chunks, ws, t, pk_token(a, wt0, end, t, c), (wave * PK_NT + t) * 16 + c, c, g, ro, rm);
 }
 
 /* --- narrow items */
@@ -433,145 +507,135 @@ __device__ __forceinline__ void pk_fetch_narrow(const AttnArgs &a, int pa, int p
                                      (LdsVoid *)(st + PK_SCALE_AT), 4, 0, 0);
 }
 
+/* By one wave: the item's chunk from the first page to the last, its output or partial. */
 template <int NT>
 __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it, int chunks, long long slot,
-                                          unsigned char *stages, float (&sh_m)[WAVES][PK_NARROW_COLS],
-                                          float (&sh_l)[WAVES][PK_NARROW_COLS]) {
+                                          unsigned char *ring) {
     const AttnArgs &a = p.a;
-    const int lane = pk_lane(), wave = uni((int)threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
-    const int pairs = (it.pg1 - it.pg0 + 1) / 2, mine = (pairs - wave + 3) / 4;
-    /* lane j: the entry of page j & 1 of this wave's pair j / 2 (a second page past the range: the first) */
-    const int32_t *bt = a.block_table + (long long)it.b * a.max_pages;
-    int lp = it.pg0 + 2 * (wave + 4 * (lane >> 1)) + (lane & 1);
-    if ((lane & 1) && lp >= it.pg1) lp--;
-    int entry = lp < it.pg1 ? bt[lp] : 0;
-    const bool bad = __any((unsigned)entry >= (unsigned)a.num_pages);
-    if ((unsigned)entry >= (unsigned)a.num_pages) entry = 0;
-
-    KeyBounds<NT> kb;
-    uint4 raw[NT][4];
-    pk_columns<NT>(p, it, 0, it.tn, lane, kb, raw);
+    const int lane = pk_lane(), c = lane & 15, g = lane >> 4;
+    const int npages = it.pg1 - it.pg0, pairs = (npages + 1) / 2;
+    /* lane j: entries j and 64 + j of the chunk */
+    const int32_t *bt = a.block_table + (long long)it.b * a.max_pages + it.pg0;
+    int e0 = lane < npages ? bt[lane] : 0, e1 = WAVE + lane < npages ? bt[WAVE + lane] : 0;
     WaveState<NT> ws;
     state_init(ws);
     ws.sl2 = a.scale_log2;
-    ws.bad = bad;
-    if (mine > 0) {
-        unsigned char *ring = stages + wave * PK_NARROW_BUFS * PK_NARROW_STAGE;
-        const int lds = pk_lds_offset(ring);
-        const auto fetch = [&](int i, int buf) {
-            const int j = i < mine ? 2 * i : 0;
-            pk_fetch_narrow(a, __builtin_amdgcn_readlane(entry, j), __builtin_amdgcn_readlane(entry, j + 1), i < mine, it.kvh,
-                            ring + buf * PK_NARROW_STAGE, lane);
-        };
-        fetch(0, 0);
-        fetch(1, 1);
-        QOp qb[NT];
-        q8_from_raw<NT>(raw, qb);
-        for (int i = 0; i < mine; i++) {
-            const int at = lds + (i & 1) * PK_NARROW_STAGE;
-            __builtin_amdgcn_s_waitcnt(pk_wait(9, 15));   /* all but the younger pair's copies have landed */
-            const int lpa = it.pg0 + 2 * (wave + 4 * i);
-            pk_pair<NT>(lpa, lpa + 1 < it.pg1, PkAt{at, at + PK_SCALE_AT}, qb, kb, ws, lane, [&] { fetch(i + 2, i & 1); });
-        }
+    ws.bad = __any((unsigned)e0 >= (unsigned)a.num_pages || (unsigned)e1 >= (unsigned)a.num_pages);
+    if ((unsigned)e0 >= (unsigned)a.num_pages) e0 = 0;   /* only read: the item reports NaN */
+    if ((unsigned)e1 >= (unsigned)a.num_pages) e1 = 0;
+    const auto entry = [&](int e) {
+        const int lo = __builtin_amdgcn_readlane(e0, e & (WAVE - 1)), hi = __builtin_amdgcn_readlane(e1, e & (WAVE - 1));
+        return e < WAVE ? lo : hi;
+    };
+    PkBounds<NT> kb;
+    uint4 raw[NT][4];
+    pk_columns<NT>(p, it, 0, it.tn, lane, kb, raw);
+    const f32x4 zero = pk_zero();
+    const int lds = pk_lds_offset(ring);
+    const auto fetch = [&](int i, int buf) {
+        const int la = i < pairs ? 2 * i : 0, lb = la + 1 < npages ? la + 1 : la;   /* no second page: the first again */
+        pk_fetch_narrow(a, entry(la), entry(lb), i < pairs, it.kvh, ring + buf * PK_NARROW_STAGE, lane);
+    };
+    fetch(0, 0);
+    fetch(1, 1);
+    QOp qb[NT];
+    q8_from_raw<NT>(raw, qb);
+    for (int i = 0; i < pairs; i++) {
+        const int at = lds + (i & 1) * PK_NARROW_STAGE, lpa = it.pg0 + 2 * i;
+        __builtin_amdgcn_s_waitcnt(pk_wait(9, 15));   /* all but the younger pair's copies have landed */
+        pk_pair<NT>(lpa, lpa + 1 < it.pg1, PkAt{at, at + PK_SCALE_AT}, qb, kb, zero, ws, lane,
+                    [&] { fetch(i + 2, i & 1); });
     }
-    /* the four waves' states: (max, sum) of every column, then O */
-#pragma unroll
-    for (int t = 0; t < NT; t++) {
-        ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
-        if (g == 0) {
-            sh_m[wave][t * 16 + c] = ws.bad ? NAN : ws.m[t];
-            sh_l[wave][t * 16 + c] = ws.l[t];
-        }
-    }
-    __builtin_amdgcn_s_waitcnt(0);   /* no copy is in flight into the stages */
-    __syncthreads();
-    float *merged = reinterpret_cast<float *>(stages);   /* [wave][column][O_PITCH] */
-#pragma unroll
-    for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int d = 0; d < 8; d++)
-            *reinterpret_cast<f32x4 *>(merged + ((wave * NT + t) * 16 + c) * O_PITCH + 16 * d + 4 * g) = ws.o[t][d];
-    __syncthreads();
     const PkPart part = pk_part(p.part_narrow, p.narrow_slots, PK_NARROW_COLS, slot);
     const Rsrc ro = page_rsrc(part.o, PK_NARROW_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_NARROW_COLS * 8);
-    for (int i = threadIdx.x; i < NT * 16 * (HEAD_DIM / 4); i += 256) {
-        const int col = i >> 5, quad = i & 31, tok = pk_token(a, 0, it.tn, col >> 4, col & 15);
-        if (tok < 0) continue;
-        float m = sh_m[0][col], l = 0.0f;
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) m = fmaxf(m, sh_m[w][col]);
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        bool any_bad = false;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const float mw = sh_m[w][col];
-            any_bad = any_bad || mw != mw;
-            const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
-            o += *reinterpret_cast<const f32x4 *>(merged + (w * NT * 16 + col) * O_PITCH + 4 * quad) * f;
-            l += sh_l[w][col] * f;
-        }
-        if (chunks == 1) {
-            float v[4];
-            const float inv = 1.0f / l;
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = any_bad ? NAN : o[k] * inv;
-            store_bf16x4(a.out + pk_row(p, it, tok, col & 15) * HEAD_DIM + 4 * quad, v);
-        } else {
-            part_store(ro, (col * HEAD_DIM + 4 * quad) * 4, float4{o[0], o[1], o[2], o[3]});
-            if (quad == 0)
-                __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(any_bad ? NAN : m), __float_as_uint(l)}, rm,
-                                                      col * 8, 0, SC1);
-        }
-    }
-    __syncthreads();   /* the stages are used again */
+    for (int t = 0; t < NT; t++) pk_store<NT>(p, it, chunks, ws, t, pk_token(a, 0, it.tn, t, c), t * 16 + c, c, g, ro, rm);
+    __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* nothing is in flight into the ring, and the partial is out */
 }
 
-/* The merge of a (tile, KV head)'s partials in slots slot0 .. slot0 + chunks - 1, in chunk order, into its bf16 rows. */
-__device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, bool narrow, int chunks, long long slot0) {
+/* The merge of a (tile, KV head)'s partials in slots slot0 .. slot0 + chunks - 1, in chunk order, into its bf16 rows, by
+ * `threads` threads, each PK_MERGE pieces of four dims at a time (the loads of PK_MERGE pieces of two chunks in flight: the
+ * merge is bound by their latency). */
+constexpr int PK_MERGE = 4;
+
+__device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, bool narrow, int chunks, long long slot0,
+                                         int thread, int threads) {
     const AttnArgs &a = p.a;
-    const int cols = narrow ? PK_NARROW_COLS : PK_WIDE_COLS;
+    const int cols = narrow ? PK_NARROW_COLS : PK_WIDE_COLS, pieces = cols * (HEAD_DIM / 4);
     const PkPart part = pk_part(narrow ? p.part_narrow : p.part_wide, narrow ? p.narrow_slots : p.wide_slots, cols, slot0);
-    constexpr int NB = 4;   /* chunks whose loads are issued together */
-    for (int i = threadIdx.x; i < cols * (HEAD_DIM / 4); i += 256) {
-        const int col = i >> 5, quad = i & 31;
-        const int tok = pk_token(a, it.t0, it.t0 + it.tn, col >> 4, col & 15);   /* a wave's tiles follow the last one's */
-        if (tok < 0) continue;
-        float m = -INFINITY, l = 0.0f;
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int j0 = 0; j0 < chunks; j0 += NB) {
-            f32x4 oj[NB];
-            float mj[NB], lj[NB];
+    constexpr int NB = 2;
+    for (int i0 = thread; i0 < pieces; i0 += PK_MERGE * threads) {
+        int tok[PK_MERGE];
+        bool some = false;
+        float m[PK_MERGE], l[PK_MERGE];
+        f32x4 o[PK_MERGE];
 #pragma unroll
-            for (int k = 0; k < NB; k++) {
-                const int j = min(j0 + k, chunks - 1);
-                /* sc1: past this XCD's L2, where another workgroup's stores are not seen */
+        for (int k = 0; k < PK_MERGE; k++) {
+            const int col = (i0 + k * threads) >> 5;
+            /* a wave's tiles follow the last one's */
+            tok[k] = col < cols ? pk_token(a, it.t0, it.t0 + it.tn, col >> 4, col & 15) : -1;
+            some = some || tok[k] >= 0;
+            m[k] = -INFINITY;
+            l[k] = 0.0f;
+            o[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        if (!__any(some)) continue;
+        for (int j0 = 0; j0 < chunks; j0 += NB) {
+            f32x4 oj[NB][PK_MERGE];
+            float mj[NB][PK_MERGE], lj[NB][PK_MERGE];
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                const int j = min(j0 + n, chunks - 1);
+                /* sc1: past this XCD's L2, where another workgroup's stores are not seen; out of range reads zeros */
                 const Rsrc ro = page_rsrc(part.o + (long long)j * cols * HEAD_DIM, cols * HEAD_DIM * 4);
                 const Rsrc rm = page_rsrc(part.ml + (long long)j * cols * 2, cols * 8);
-                oj[k] = part_load(ro, (col * HEAD_DIM + 4 * quad) * 4);
-                const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(rm, col * 8, 0, SC1);
-                mj[k] = j0 + k < chunks ? __uint_as_float(w[0]) : -INFINITY;
-                lj[k] = __uint_as_float(w[1]);
-            }
-            float mb = m;
 #pragma unroll
-            for (int k = 0; k < NB; k++) mb = fmaxf(mb, mj[k]);
-            const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mb);
-            o *= keep;
-            l *= keep;
-            m = mb;
-#pragma unroll
-            for (int k = 0; k < NB; k++) {
-                const float f = mj[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mj[k] - mb);   /* NaN: a bad page */
-                o += oj[k] * f;
-                l += lj[k] * f;
+                for (int k = 0; k < PK_MERGE; k++) {
+                    const int i = i0 + k * threads;
+                    oj[n][k] = part_load(ro, i * 16);
+                    const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(rm, (i >> 5) * 8, 0, SC1);
+                    mj[n][k] = __uint_as_float(w[0]);
+                    lj[n][k] = __uint_as_float(w[1]);
+                }
             }
+#pragma unroll
+            for (int k = 0; k < PK_MERGE; k++)
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    if (j0 + n >= chunks) continue;
+                    const float mb = fmaxf(m[k], mj[n][k]);
+                    const float keep = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - mb);
+                    const float f = mj[n][k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mj[n][k] - mb);   /* NaN: a bad page */
+                    o[k] = o[k] * keep + oj[n][k] * f;
+                    l[k] = l[k] * keep + lj[n][k] * f;
+                    m[k] = mb;
+                }
         }
-        float v[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = o[k] / l;
-        store_bf16x4(a.out + pk_row(p, it, tok, col & 15) * HEAD_DIM + 4 * quad, v);
+        for (int k = 0; k < PK_MERGE; k++) {
+            if (tok[k] < 0) continue;
+            const int i = i0 + k * threads, col = i >> 5;
+            float v[4];
+#pragma unroll
+            for (int d = 0; d < 4; d++) v[d] = o[k][d] / l[k];
+            store_bf16x4(a.out + pk_row(p, it, tok[k], col & 15) * HEAD_DIM + 4 * (i & 31), v);
+        }
     }
+}
+
+/* The next of the N items from `first` on that nobody took: queue x holds the items first + x, first + x + 8, ...; queue
+ * `own` before the others. One lane calls it. */
+__device__ __forceinline__ int pk_ticket(int *tickets, int first, int N, int own) {
+    for (int i = 0; i < PK_QUEUES; i++) {
+        const int x = (own + i) % PK_QUEUES;
+        const long long at = (long long)first + x;
+        if (at >= N) continue;
+        const int have = (int)((N - at + PK_QUEUES - 1) / PK_QUEUES);
+        if (__hip_atomic_load(tickets + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) >= have) continue;
+        const int got = __hip_atomic_fetch_add(tickets + x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (got < have) return (int)(at + (long long)got * PK_QUEUES);
+    }
+    return INT_MAX;
 }
 
 __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
@@ -579,7 +643,6 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
     extern __shared__ int pk_cum[];
     __shared__ __align__(16) unsigned char stages[PK_STAGES];
     __shared__ int tab[PK_WIDE_MAX];
-    __shared__ float sh_m[WAVES][PK_NARROW_COLS], sh_l[WAVES][PK_NARROW_COLS];
     __shared__ long long scan[2][WAVES];
     __shared__ int sh_next;
     const AttnArgs &a = p.a;
@@ -631,19 +694,15 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
     }
     if (!fits) return;   /* every workgroup: no ticket is taken */
 
-    const int NW = uni(wide[B]), N = uni(NW + narrow[B]), G = gridDim.x;
-    for (int k = blockIdx.x; k < N;) {
-        const bool is_wide = k < NW;
-        const int *cum = is_wide ? wide : narrow;
-        const int kk = is_wide ? k : k - NW;
+    const int NW = uni(wide[B]), NN = uni(narrow[B]), G = gridDim.x;
+    for (int k = blockIdx.x; k < NW;) {
         PkItem it;
-        it.b = uni(find_sequence(cum, B, kk));
+        it.b = uni(find_sequence(wide, B, k));
         it.q = pk_plan(p, uni(p.cu[it.b]), uni(p.cu[it.b + 1]), uni(a.seq_lens[it.b]));
         /* a sequence's items: the last tiles first, then the chunks, its KV heads fastest */
-        const int local = uni(kk - cum[it.b]), rest = local / a.Hkv;
+        const int local = uni(k - wide[it.b]), rest = local / a.Hkv;
         it.kvh = local - rest * a.Hkv;
-        const int tile = it.q.tiles - 1 - rest / it.q.nch, j = rest % it.q.nch;
-        const int tokens = is_wide ? WAVES * PK_NT * (16 / a.G) : it.q.n;
+        const int tile = it.q.tiles - 1 - rest / it.q.nch, j = rest % it.q.nch, tokens = WAVES * PK_NT * (16 / a.G);
         it.t0 = tile * tokens;
         it.tn = min(it.q.n - it.t0, tokens);
         /* the tile's own pages, its chunks [j0, j1), this chunk's pages within */
@@ -655,13 +714,8 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
         it.pg1 = min(it.q.pg0 + (j + 1) * it.q.s, hi);
         if (it.pg0 < it.pg1) {
             const int chunks = j1 - j0, unit = uni(units[it.b]) + tile * a.Hkv + it.kvh;
-            const long long slot0 = uni((is_wide ? wslots : nslots)[it.b]) + ((long long)tile * a.Hkv + it.kvh) * it.q.nch;
-            if (is_wide)
-                pk_wide(p, it, chunks, slot0 + j - j0, stages, tab);
-            else if (it.tn <= 16 / a.G)
-                pk_narrow<1>(p, it, chunks, slot0 + j - j0, stages, sh_m, sh_l);
-            else
-                pk_narrow<2>(p, it, chunks, slot0 + j - j0, stages, sh_m, sh_l);
+            const long long slot0 = uni(wslots[it.b]) + ((long long)tile * a.Hkv + it.kvh) * it.q.nch;
+            pk_wide(p, it, chunks, slot0 + j - j0, stages, tab);
             if (chunks > 1) {
                 __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* this wave's part of the partial is at the coherent level */
                 __syncthreads();
@@ -670,42 +724,71 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
                 __syncthreads();
                 const int prior = uni(sh_next);
                 if (prior == chunks - 1) {
-                    pk_merge(p, it, !is_wide, chunks, slot0);
+                    pk_merge(p, it, false, chunks, slot0, threadIdx.x, 256);
                     if (threadIdx.x == 0)
                         __hip_atomic_store(p.arrived + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
-                __syncthreads();   /* sh_next is used again */
             }
         }
-        if (N <= G) break;
-        if (threadIdx.x == 0) {   /* queue x holds the items G + x, G + x + 8, ...; its own first, then the others' */
-            int next = INT_MAX;
-            for (int i = 0; i < PK_QUEUES && next == INT_MAX; i++) {
-                const int x = ((int)blockIdx.x + i) % PK_QUEUES;
-                const long long at = G + x;
-                if (at >= N) continue;
-                const int have = (int)((N - at + PK_QUEUES - 1) / PK_QUEUES);
-                if (__hip_atomic_load(p.tickets + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) >= have) continue;
-                const int got = __hip_atomic_fetch_add(p.tickets + x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (got < have) next = (int)(at + (long long)got * PK_QUEUES);
-            }
-            sh_next = next;
-        }
+        if (NW <= G) break;
+        __syncthreads();   /* sh_next and the stages are used again */
+        if (threadIdx.x == 0) sh_next = pk_ticket(p.tickets, G, NW, blockIdx.x % PK_QUEUES);
         __syncthreads();
         k = uni(sh_next);
-        __syncthreads();
     }
-    if (N > G && threadIdx.x == 0) {   /* the last workgroup to leave returns the tickets */
-        if (__hip_atomic_fetch_add(p.done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == G - 1) {
-            for (int x = 0; x < PK_QUEUES; x++)
-                __hip_atomic_store(p.tickets + x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(p.done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+
+    /* the waves on their own; with no wide items before them, the first by index */
+    const int lane = threadIdx.x & (WAVE - 1), wave = uni((int)threadIdx.x >> 6);
+    const int first = NW ? 0 : WAVES * G;
+    unsigned char *ring = stages + wave * PK_NARROW_BUFS * PK_NARROW_STAGE;
+    for (int k = NW ? -1 : blockIdx.x + G * wave;;) {
+        if (k < 0 || k >= NN) {
+            if (NN <= first) break;
+            int next = 0;
+            if (lane == 0) next = pk_ticket(p.tickets + PK_QUEUES, first, NN, blockIdx.x % PK_QUEUES);
+            k = uni(next);
+            if (k >= NN) break;
         }
+        PkItem it;
+        it.b = uni(find_sequence(narrow, B, k));
+        it.q = pk_plan(p, uni(p.cu[it.b]), uni(p.cu[it.b + 1]), uni(a.seq_lens[it.b]));
+        const int local = uni(k - narrow[it.b]), j = local / a.Hkv;   /* the chunks, its KV heads fastest */
+        it.kvh = local - j * a.Hkv;
+        it.t0 = 0;
+        it.tn = it.q.n;
+        it.pg0 = it.q.pg0 + j * it.q.s;
+        it.pg1 = j == it.q.nch - 1 ? it.q.pg0 + it.q.np : it.pg0 + it.q.s;
+        const int chunks = it.q.nch;
+        const long long slot0 = uni(nslots[it.b]) + (long long)it.kvh * chunks;
+        if (it.tn <= 16 / a.G)
+            pk_narrow<1>(p, it, chunks, slot0 + j, ring);
+        else
+            pk_narrow<2>(p, it, chunks, slot0 + j, ring);
+        if (chunks > 1) {
+            int *count = p.arrived + uni(units[it.b]) + it.kvh;
+            int prior = 0;
+            if (lane == 0) prior = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (uni(prior) == chunks - 1) {
+                pk_merge(p, it, true, chunks, slot0, lane, WAVE);
+                if (lane == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        k = -1;
+    }
+    /* where tickets were taken, the last workgroup to leave returns them */
+    if (NW <= G && NN <= first) return;
+    __syncthreads();
+    if (threadIdx.x == 0 &&
+        __hip_atomic_fetch_add(p.done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == G - 1) {
+        for (int x = 0; x < 2 * PK_QUEUES; x++)
+            __hip_atomic_store(p.tickets + x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(p.done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
 /* The most partials and arrival counts a launch of these sizes can need, whatever its lengths (pk_plan): a narrow sequence
- * is Hkv units of ceil(pages / PK_NARROW_SPLIT) chunks. A wide one has at least tpw + 1 rows; all of them together have at
+ * is Hkv units of at most ceil(pages / PK_NARROW_SPLIT) chunks, or ceil(pages / PK_SHORT_SPLIT) if short. A wide one has at least tpw + 1 rows; all of them together have at
  * most rows / TW + their number tiles, each Hkv units, cut into at most ceil(pages / PK_WIDE_MIN) chunks, and no sequence
  * into more than PK_WIDE_ITEMS items unless its chunks would pass PK_WIDE_MAX pages. */
 struct PkSizes {
@@ -719,7 +802,7 @@ static PkSizes pk_sizes(long long rows, int B, int Hq, int Hkv, int max_seq_len,
     if (window >= 0) np = min(np, (rows + window) / PAGE + 3);
     const long long nw = min((long long)B, rows / (tpw + 1)), tiles = rows / (WAVES * tpw) + nw;
     PkSizes z = {};
-    const long long nch = (np - 1) / PK_NARROW_SPLIT + 1, wch = (np - 1) / PK_WIDE_MIN + 1, most = (np - 1) / PK_WIDE_MAX + 1;
+    const long long nch = max((min(np, (long long)PK_SHORT) - 1) / PK_SHORT_SPLIT + 1, (np - 1) / PK_NARROW_SPLIT + 1), wch = (np - 1) / PK_WIDE_MIN + 1, most = (np - 1) / PK_WIDE_MAX + 1;
     if (nch > 1) z.narrow_slots = min((long long)B, rows) * Hkv * nch;
     if (wch > 1) z.wide_slots = min(tiles * Hkv * wch, nw * PK_WIDE_ITEMS + (most > 1 ? tiles * Hkv * most : 0));
     z.units = (nch > 1 ? min((long long)B, rows) : 0) * Hkv + (wch > 1 ? tiles * Hkv : 0);
@@ -733,7 +816,7 @@ static size_t pk_part_bytes(const PkSizes &z) {
 /* As attention.hip's decode workspace: partials from the start, int32 counts (tickets, done, arrivals) in the last 1/256,
  * whose place depends on the workspace's size alone. */
 static size_t pk_count_region(size_t bytes) { return (bytes - ((bytes >> 8) & ~(size_t)3)) & ~(size_t)3; }
-static size_t pk_count_bytes(const PkSizes &z) { return (size_t)(z.units + PK_QUEUES + 1) * sizeof(int); }
+static size_t pk_count_bytes(const PkSizes &z) { return (size_t)(z.units + 2 * PK_QUEUES + 1) * sizeof(int); }
 
 static bool pk_shape_ok(long long rows, int B, int Hq, int Hkv, int max_seq_len) {
     return rows > 0 && rows <= 1LL << 24 && B > 0 && B <= PK_MAX_BATCH && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 &&
@@ -792,7 +875,7 @@ extern "C" int nc_packed_attn_fp8(const void *q, const void *k_pages, const void
     p.wide_slots = z.wide_slots; p.narrow_slots = z.narrow_slots;
     p.units = (int)z.units;
     p.tickets = (int *)((char *)workspace + counts);
-    p.done = p.tickets + PK_QUEUES;
+    p.done = p.tickets + 2 * PK_QUEUES;
     p.arrived = p.done + 1;
     hipLaunchKernelGGL(packed_attn_kernel, dim3(device_packed_grid()), dim3(256), 5 * (B + 1) * sizeof(int),
                        (hipStream_t)stream, p);
