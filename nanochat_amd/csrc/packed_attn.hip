@@ -13,14 +13,16 @@
  * kinds of work items, each one workgroup of four waves, both streaming pages into LDS by asynchronous copies:
  *
  *   narrow  at most 32 columns: one wave takes a chunk of the keys by itself, page pairs through a ring of its own in LDS
- *           with two pairs in flight; waves meet at no barrier, so one's start or merge hides behind the others' streams
+ *           with two pairs in flight; waves meet at no barrier, so one's start or merge hides behind the others' streams.
+ *           A sequence of at most PK_SHORT pages is not cut but shared by the four waves of a workgroup, which merge
+ *           through LDS ("alone": it costs no round trips through memory, which is what a short one's time is made of)
  *   wide    a tile of up to 128 columns, 32 a wave: the four waves of a workgroup walk the same pairs, each fetched once
  *           (PK_AHEAD ahead)
  *
  * A sequence's keys are cut into chunks (pk_plan), so that few rows over many keys still fill the chip; a (tile, KV head)
  * of several chunks leaves one partial (O, max, sum) in fp32 a chunk, and whoever finishes its last chunk merges them in
  * order. The cuts depend on nothing but the sequence's own numbers, so its output bits do not depend on the rest of the
- * launch. A workgroup takes wide items while there are any, then its waves narrow ones: the first by workgroup index, later
+ * launch. A workgroup takes wide and alone items while there are any, then its waves narrow ones: the first by workgroup index, later
  * ones from eight queues (an XCD's workgroups take every eighth item, which keeps a KV head's pages in that XCD's L2), so
  * that unequal items even out.
  */
@@ -37,14 +39,14 @@ constexpr int PK_WIDE_COLS = WAVES * 16 * PK_NT;
 constexpr int PK_MAX_BATCH = 1024;
 constexpr int PK_QUEUES = 8;                   /* XCDs */
 constexpr int PK_NARROW_SPLIT = 64;            /* pages of a narrow chunk */
-constexpr int PK_SHORT_SPLIT = 16;             /* of one of a sequence of at most PK_SHORT pages */
 constexpr int PK_MIN_TAIL = 4;                 /* a last chunk of fewer pages joins the one before it */
-constexpr int PK_SHORT = PK_NARROW_SPLIT + PK_MIN_TAIL - 1;
+constexpr int PK_SHORT = 2 * PK_NARROW_SPLIT;  /* a narrow sequence of at most so many pages is not cut */
 constexpr int PK_WIDE_MIN = 128;               /* least and most pages of a wide chunk */
 constexpr int PK_WIDE_MAX = 1024;
 constexpr int PK_WIDE_ITEMS = 256;             /* items a wide sequence is cut into at most, if its chunks stay that long */
 constexpr int PK_AHEAD = 3;                    /* wide: pairs in flight */
-static_assert(PK_SHORT <= 2 * WAVE, "a narrow chunk's block-table entries: two a lane");
+static_assert(PK_SHORT <= 2 * WAVE && PK_NARROW_SPLIT + PK_MIN_TAIL <= 2 * WAVE,
+              "a narrow item's block-table entries: two a lane");
 
 /* One stage: the pair's K (2 x 2 KiB), V (2 x 2 KiB) and scales (per page 16 of K, then 16 of V; wide: a copy a wave). */
 constexpr int PK_SCALE_AT = 4 * PAGE_BYTES, PK_SCALE_BYTES = 256;
@@ -61,21 +63,22 @@ struct PackedArgs {
     float *part_wide, *part_narrow;   /* [slots][cols][128] O, then [slots][cols][2] (max, sum) */
     long long wide_slots, narrow_slots;
     int units;                  /* arrival counts */
-    int *tickets, *done, *arrived;    /* [2][8] (wide, narrow), [1], [units]; zero between launches */
+    int tpt;                    /* tokens of a 16-column tile: 16 / G */
+    int *tickets, *done, *arrived;    /* [2][8][PK_LINE] (workgroups, waves), [PK_LINE], [units]; zero between launches */
 };
 
 /* A sequence's rows, its pages [pg0, pg0 + np) (pg0 even) and how they are cut: nch chunks of s pages from pg0. tiles = 0:
  * no rows; < 0: a length that does not fit (its rows become NaN). */
 struct PkSeq {
     int row0, n, len, pg0, np, tiles, s, nch;
-    bool narrow;
+    bool narrow, alone;   /* narrow; and of at most PK_SHORT pages: one item, four waves */
 };
 
-__device__ __forceinline__ PkSeq pk_plan(const PackedArgs &p, int cu0, int cu1, int len) {
+__device__ __forceinline__ PkSeq pk_plan(const PackedArgs &p, int row0, int n, int len) {
     const AttnArgs &a = p.a;
     PkSeq q = {};
-    q.row0 = min(max(cu0, 0), p.rows);
-    q.n = min(max(cu1, q.row0), p.rows) - q.row0;
+    q.row0 = row0;
+    q.n = n;
     if (q.n == 0) return q;
     q.len = len;
     if (q.len < q.n || q.len > a.max_len) {
@@ -85,24 +88,21 @@ __device__ __forceinline__ PkSeq pk_plan(const PackedArgs &p, int cu0, int cu1, 
     const int first = a.window >= 0 ? max(q.len - q.n - a.window, 0) : 0;
     q.pg0 = (first / PAGE) & ~1;
     q.np = (q.len - 1) / PAGE + 1 - q.pg0;
-    const int tpt = 16 / a.G, tpw = tpt * PK_NT;
+    const int tpw = p.tpt * PK_NT;
     q.narrow = q.n <= tpw;
     if (q.narrow) {
         q.tiles = 1;
-        q.s = q.np <= PK_SHORT ? PK_SHORT_SPLIT : PK_NARROW_SPLIT;
-        q.nch = (q.np - 1) / q.s + 1;
+        q.alone = q.np <= PK_SHORT;
+        q.s = PK_NARROW_SPLIT;
+        q.nch = q.alone ? 1 : (q.np - 1) / q.s + 1;
         q.nch -= q.nch > 1 && q.np - (q.nch - 1) * q.s < PK_MIN_TAIL;
     } else {
-        q.tiles = (q.n - 1) / (WAVES * tpw) + 1;
-        const int want = max(PK_WIDE_ITEMS / (q.tiles * a.Hkv), 1);
-        q.s = min(max(((q.np - 1) / want + 1 + 31) & ~31, PK_WIDE_MIN), PK_WIDE_MAX);
-        q.nch = (q.np - 1) / q.s + 1;
+        q.tiles = (int)((unsigned)(q.n - 1) / (unsigned)(WAVES * tpw)) + 1;
+        const unsigned want = max((unsigned)PK_WIDE_ITEMS / (unsigned)(q.tiles * a.Hkv), 1u);
+        q.s = min(max((int)(((unsigned)(q.np - 1) / want + 1 + 31) & ~31u), PK_WIDE_MIN), PK_WIDE_MAX);
+        q.nch = (int)((unsigned)(q.np - 1) / (unsigned)q.s) + 1;
     }
     return q;
-}
-
-__device__ __forceinline__ PkSeq pk_plan(const PackedArgs &p, int b) {
-    return pk_plan(p, p.cu[b], p.cu[b + 1], p.a.seq_lens[b]);
 }
 
 /* This lane, as a value the compiler cannot compute ahead: nothing made of it is kept in registers across items. */
@@ -115,26 +115,32 @@ __device__ __forceinline__ int pk_lane() {
 /* A value that is the same in every lane, as a scalar register's. */
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-/* Exclusive prefix sums of two values a thread over the workgroup's 256 threads. */
-__device__ __forceinline__ void pk_scan(long long (&v)[2], long long (&part)[2][WAVES]) {
+constexpr int PK_SUMS = 6;   /* of the sequences before each: wide, alone and narrow items, units, wide and narrow slots */
+
+/* a + b, at most INT_MAX (a, b >= 0): counts that only overlapping row offsets could make so large. */
+__device__ __forceinline__ int pk_add(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)INT_MAX); }
+
+/* Exclusive prefix sums of PK_SUMS values a thread over the workgroup's 256 threads. Within a wave by DPP: shifts by 1, 2,
+ * 4 and 8 within rows of 16 lanes, then a row's last sum added to the next row's, and the lower half's to the upper's. */
+__device__ __forceinline__ void pk_scan(int (&v)[PK_SUMS], int (&part)[PK_SUMS][WAVES]) {
     const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int k = 0; k < 2; k++) {
-        long long s = v[k];
-#pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) {
-            const long long t = __shfl_up(s, o, WAVE);
-            if (lane >= o) s += t;
-        }
+    for (int k = 0; k < PK_SUMS; k++) {
+        int s = v[k];
+        s = pk_add(s, __builtin_amdgcn_update_dpp(0, s, 0x111, 0xF, 0xF, false));
+        s = pk_add(s, __builtin_amdgcn_update_dpp(0, s, 0x112, 0xF, 0xF, false));
+        s = pk_add(s, __builtin_amdgcn_update_dpp(0, s, 0x114, 0xF, 0xF, false));
+        s = pk_add(s, __builtin_amdgcn_update_dpp(0, s, 0x118, 0xF, 0xF, false));
+        s = pk_add(s, __builtin_amdgcn_update_dpp(0, s, 0x142, 0xA, 0xF, false));
+        s = pk_add(s, __builtin_amdgcn_update_dpp(0, s, 0x143, 0xC, 0xF, false));
         if (lane == WAVE - 1) part[k][wave] = s;
-        v[k] = s - v[k];
+        v[k] = (int)__builtin_amdgcn_update_dpp(0, s, 0x138, 0xF, 0xF, false);   /* the lane before's, 0 in lane 0 */
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2; k++)
+    for (int k = 0; k < PK_SUMS; k++)
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) v[k] += w < wave ? part[k][w] : 0;
-    __syncthreads();
+        for (int w = 0; w < WAVES; w++) v[k] = pk_add(v[k], w < wave ? part[k][w] : 0);
 }
 
 /* A workgroup barrier that drains no asynchronous copy; memory accesses do not move across it. */
@@ -166,13 +172,13 @@ struct PkItem {
 };
 
 /* Column c of wave tile t (first token wt0) -> its token (< 0: not live). */
-__device__ __forceinline__ int pk_token(const AttnArgs &a, int wt0, int end, int t, int c) {
-    const int tpt = 16 / a.G, tok = wt0 + t * tpt + c / a.G;
-    return c < tpt * a.G && tok < end ? tok : -1;
+__device__ __forceinline__ int pk_token(const PackedArgs &p, int wt0, int end, int t, int c) {
+    const int tok = wt0 + t * p.tpt + (int)((unsigned)c / (unsigned)p.a.G);
+    return c < p.tpt * p.a.G && tok < end ? tok : -1;
 }
 
 __device__ __forceinline__ long long pk_row(const PackedArgs &p, const PkItem &it, int tok, int c) {
-    return ((long long)it.q.row0 + tok) * p.a.Hq + it.kvh * p.a.G + c % p.a.G;
+    return ((long long)it.q.row0 + tok) * p.a.Hq + it.kvh * p.a.G + (int)((unsigned)c % (unsigned)p.a.G);
 }
 
 /* Keys of a wave: in tile t a lane's column sees [lo[t], hi[t]]; the pairs from page in0 (even) up to in1 are seen whole by
@@ -188,10 +194,10 @@ template <int NT>
 __device__ __forceinline__ void pk_columns(const PackedArgs &p, const PkItem &it, int wt0, int end, int lane,
                                            PkBounds<NT> &kb, uint4 (&raw)[NT][4]) {
     const AttnArgs &a = p.a;
-    const int c = lane & 15, g = lane >> 4, start = it.q.len - it.q.n, tpt = 16 / a.G;
+    const int c = lane & 15, g = lane >> 4, start = it.q.len - it.q.n, tpt = p.tpt;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        const int tok = pk_token(a, wt0, end, t, c), pos = start + tok;
+        const int tok = pk_token(p, wt0, end, t, c), pos = start + tok;
         kb.hi[t] = tok >= 0 ? pos : -1;
         kb.lo[t] = tok >= 0 && a.window >= 0 ? max(pos - a.window, 0) : 0;
 #pragma unroll
@@ -422,7 +428,7 @@ __device__ __forceinline__ void pk_wide(const PackedArgs &p, const PkItem &it, i
                                         unsigned char *stages, int *tab) {
     const AttnArgs &a = p.a;
     const int lane = pk_lane(), wave = uni((int)threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-    const int tpw = 16 / a.G * PK_NT, start = it.q.len - it.q.n;
+    const int tpw = p.tpt * PK_NT, start = it.q.len - it.q.n;
     const int wt0 = it.t0 + wave * tpw, end = it.t0 + it.tn, npages = it.pg1 - it.pg0;
     const bool on = wt0 < end;
     const int last = min(wt0 + tpw, end) - 1;
@@ -483,7 +489,7 @@ __device__ __forceinline__ void pk_wide(const PackedArgs &p, const PkItem &it, i
     const Rsrc ro = page_rsrc(part.o, PK_WIDE_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_WIDE_COLS * 8);
 #pragma unroll
     for (int t = 0; t < PK_NT; t++)
-        pk_store<PK_NT>(p, it, chunks, ws, t, pk_token(a, wt0, end, t, c), (wave * PK_NT + t) * 16 + c, c, g, ro, rm);
+        pk_store<PK_NT>(p, it, chunks, ws, t, pk_token(p, wt0, end, t, c), (wave * PK_NT + t) * 16 + c, c, g, ro, rm);
 }
 
 /* --- narrow items */
@@ -507,14 +513,16 @@ __device__ __forceinline__ void pk_fetch_narrow(const AttnArgs &a, int pa, int p
                                      (LdsVoid *)(st + PK_SCALE_AT), 4, 0, 0);
 }
 
-/* By one wave: the item's chunk from the first page to the last, its output or partial. */
-template <int NT>
+/* The item's page pairs first, first + stride, ... by one wave. ALONE: the four waves of a workgroup share the item so and
+ * merge their states through LDS (stages, ml); else one wave has it all and leaves its output or partial. */
+template <int NT, bool ALONE>
 __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it, int chunks, long long slot,
-                                          unsigned char *ring) {
+                                          unsigned char *ring, int first, unsigned char *stages, float *ml) {
+    constexpr int stride = ALONE ? WAVES : 1;
     const AttnArgs &a = p.a;
     const int lane = pk_lane(), c = lane & 15, g = lane >> 4;
-    const int npages = it.pg1 - it.pg0, pairs = (npages + 1) / 2;
-    /* lane j: entries j and 64 + j of the chunk */
+    const int npages = it.pg1 - it.pg0, pairs = max(((npages + 1) / 2 - first + stride - 1) / stride, 0);
+    /* lane j: entries j and 64 + j of the item's pages */
     const int32_t *bt = a.block_table + (long long)it.b * a.max_pages + it.pg0;
     int e0 = lane < npages ? bt[lane] : 0, e1 = WAVE + lane < npages ? bt[WAVE + lane] : 0;
     WaveState<NT> ws;
@@ -533,7 +541,8 @@ __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it,
     const f32x4 zero = pk_zero();
     const int lds = pk_lds_offset(ring);
     const auto fetch = [&](int i, int buf) {
-        const int la = i < pairs ? 2 * i : 0, lb = la + 1 < npages ? la + 1 : la;   /* no second page: the first again */
+        const int la = i < pairs ? 2 * (first + stride * i) : 0, lb = la + 1 < npages ? la + 1 : la;   /* no second page: the
+                                                                                                       * first again */
         pk_fetch_narrow(a, entry(la), entry(lb), i < pairs, it.kvh, ring + buf * PK_NARROW_STAGE, lane);
     };
     fetch(0, 0);
@@ -541,39 +550,73 @@ __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it,
     QOp qb[NT];
     q8_from_raw<NT>(raw, qb);
     for (int i = 0; i < pairs; i++) {
-        const int at = lds + (i & 1) * PK_NARROW_STAGE, lpa = it.pg0 + 2 * i;
+        const int at = lds + (i & 1) * PK_NARROW_STAGE, lpa = it.pg0 + 2 * (first + stride * i);
         __builtin_amdgcn_s_waitcnt(pk_wait(9, 15));   /* all but the younger pair's copies have landed */
         pk_pair<NT>(lpa, lpa + 1 < it.pg1, PkAt{at, at + PK_SCALE_AT}, qb, kb, zero, ws, lane,
                     [&] { fetch(i + 2, i & 1); });
     }
-    const PkPart part = pk_part(p.part_narrow, p.narrow_slots, PK_NARROW_COLS, slot);
-    const Rsrc ro = page_rsrc(part.o, PK_NARROW_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_NARROW_COLS * 8);
+    if constexpr (!ALONE) {
+        const PkPart part = pk_part(p.part_narrow, p.narrow_slots, PK_NARROW_COLS, slot);
+        const Rsrc ro = page_rsrc(part.o, PK_NARROW_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_NARROW_COLS * 8);
 #pragma unroll
-    for (int t = 0; t < NT; t++) pk_store<NT>(p, it, chunks, ws, t, pk_token(a, 0, it.tn, t, c), t * 16 + c, c, g, ro, rm);
-    __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* nothing is in flight into the ring, and the partial is out */
+        for (int t = 0; t < NT; t++) pk_store<NT>(p, it, chunks, ws, t, pk_token(p, 0, it.tn, t, c), t * 16 + c, c, g, ro, rm);
+        return;   /* the caller waits for the stores, and for the copies that read nothing */
+    }
+    float *merged = reinterpret_cast<float *>(stages), *sums = ml + WAVES * PK_NARROW_COLS;
+    __builtin_amdgcn_s_waitcnt(0);   /* no copy of this wave's is in flight into the stages; then no one's */
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
+        const int row = (first * NT + t) * 16 + c;
+        if (g == 0) {
+            ml[row] = ws.bad ? NAN : ws.m[t];
+            sums[row] = ws.l[t];
+        }
+#pragma unroll
+        for (int d = 0; d < 8; d++) *reinterpret_cast<f32x4 *>(merged + row * O_PITCH + 16 * d + 4 * g) = ws.o[t][d];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 16 * (HEAD_DIM / 4); i += 256) {
+        const int col = i >> 5, quad = i & 31, tok = pk_token(p, 0, it.tn, col >> 4, col & 15);
+        if (tok < 0) continue;
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) m = fmaxf(m, ml[w * NT * 16 + col]);
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float mw = ml[w * NT * 16 + col];
+            const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - m);   /* NaN: a bad page */
+            o += *reinterpret_cast<const f32x4 *>(merged + (w * NT * 16 + col) * O_PITCH + 4 * quad) * f;
+            l += sums[w * NT * 16 + col] * f;
+        }
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = o[k] / l;
+        store_bf16x4(a.out + pk_row(p, it, tok, col & 15) * HEAD_DIM + 4 * quad, v);
+    }
 }
 
 /* The merge of a (tile, KV head)'s partials in slots slot0 .. slot0 + chunks - 1, in chunk order, into its bf16 rows, by
- * `threads` threads, each PK_MERGE pieces of four dims at a time (the loads of PK_MERGE pieces of two chunks in flight: the
- * merge is bound by their latency). */
-constexpr int PK_MERGE = 4;
-
+ * `threads` threads, each P pieces of four dims at a time and NB chunks' loads of them in flight: the merge is bound by
+ * their latency, so few columns take many chunks at a time and many columns few. */
+template <int P, int NB>
 __device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, bool narrow, int chunks, long long slot0,
                                          int thread, int threads) {
     const AttnArgs &a = p.a;
     const int cols = narrow ? PK_NARROW_COLS : PK_WIDE_COLS, pieces = cols * (HEAD_DIM / 4);
     const PkPart part = pk_part(narrow ? p.part_narrow : p.part_wide, narrow ? p.narrow_slots : p.wide_slots, cols, slot0);
-    constexpr int NB = 2;
-    for (int i0 = thread; i0 < pieces; i0 += PK_MERGE * threads) {
-        int tok[PK_MERGE];
+    for (int i0 = thread; i0 < pieces; i0 += P * threads) {
+        int tok[P];
         bool some = false;
-        float m[PK_MERGE], l[PK_MERGE];
-        f32x4 o[PK_MERGE];
+        float m[P], l[P];
+        f32x4 o[P];
 #pragma unroll
-        for (int k = 0; k < PK_MERGE; k++) {
+        for (int k = 0; k < P; k++) {
             const int col = (i0 + k * threads) >> 5;
             /* a wave's tiles follow the last one's */
-            tok[k] = col < cols ? pk_token(a, it.t0, it.t0 + it.tn, col >> 4, col & 15) : -1;
+            tok[k] = col < cols ? pk_token(p, it.t0, it.t0 + it.tn, col >> 4, col & 15) : -1;
             some = some || tok[k] >= 0;
             m[k] = -INFINITY;
             l[k] = 0.0f;
@@ -581,16 +624,18 @@ __device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, 
         }
         if (!__any(some)) continue;
         for (int j0 = 0; j0 < chunks; j0 += NB) {
-            f32x4 oj[NB][PK_MERGE];
-            float mj[NB][PK_MERGE], lj[NB][PK_MERGE];
+            f32x4 oj[NB][P];
+            float mj[NB][P], lj[NB][P];
 #pragma unroll
             for (int n = 0; n < NB; n++) {
-                const int j = min(j0 + n, chunks - 1);
-                /* sc1: past this XCD's L2, where another workgroup's stores are not seen; out of range reads zeros */
-                const Rsrc ro = page_rsrc(part.o + (long long)j * cols * HEAD_DIM, cols * HEAD_DIM * 4);
-                const Rsrc rm = page_rsrc(part.ml + (long long)j * cols * 2, cols * 8);
+                /* sc1: past this XCD's L2, where another workgroup's stores are not seen. Past the last chunk: descriptors
+                 * of no range (zeros, no access) */
+                const bool live = j0 + n < chunks;
+                const long long j = live ? j0 + n : 0;
+                const Rsrc ro = page_rsrc(part.o + j * cols * HEAD_DIM, live ? cols * HEAD_DIM * 4 : 0);
+                const Rsrc rm = page_rsrc(part.ml + j * cols * 2, live ? cols * 8 : 0);
 #pragma unroll
-                for (int k = 0; k < PK_MERGE; k++) {
+                for (int k = 0; k < P; k++) {
                     const int i = i0 + k * threads;
                     oj[n][k] = part_load(ro, i * 16);
                     const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(rm, (i >> 5) * 8, 0, SC1);
@@ -599,7 +644,7 @@ __device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, 
                 }
             }
 #pragma unroll
-            for (int k = 0; k < PK_MERGE; k++)
+            for (int k = 0; k < P; k++)
 #pragma unroll
                 for (int n = 0; n < NB; n++) {
                     if (j0 + n >= chunks) continue;
@@ -612,7 +657,7 @@ __device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, 
                 }
         }
 #pragma unroll
-        for (int k = 0; k < PK_MERGE; k++) {
+        for (int k = 0; k < P; k++) {
             if (tok[k] < 0) continue;
             const int i = i0 + k * threads, col = i >> 5;
             float v[4];
@@ -623,137 +668,180 @@ __device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, 
     }
 }
 
-/* The next of the N items from `first` on that nobody took: queue x holds the items first + x, first + x + 8, ...; queue
- * `own` before the others. One lane calls it. */
-__device__ __forceinline__ int pk_ticket(int *tickets, int first, int N, int own) {
-    for (int i = 0; i < PK_QUEUES; i++) {
-        const int x = (own + i) % PK_QUEUES;
-        const long long at = (long long)first + x;
-        if (at >= N) continue;
-        const int have = (int)((N - at + PK_QUEUES - 1) / PK_QUEUES);
-        if (__hip_atomic_load(tickets + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) >= have) continue;
-        const int got = __hip_atomic_fetch_add(tickets + x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (got < have) return (int)(at + (long long)got * PK_QUEUES);
+/* Tickets: queue x holds the items first + x, first + x + 8, ... below N, its count on a line of its own (atomics on one
+ * line wait for each other, wherever they come from). pk_draw takes a ticket of queue x. pk_next makes an item of one drawn
+ * from queue `own`, or draws from whichever queue has some left (INT_MAX: none has); a whole wave calls it. Items are drawn
+ * when the one before is done: drawn earlier, an item would wait for it. */
+constexpr int PK_LINE = 32;   /* ints of a 128-byte line */
+
+__device__ __forceinline__ int pk_draw(int *tickets, int x) {
+    return __hip_atomic_fetch_add(tickets + x * PK_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ int pk_have(int first, int N, int x) {   /* items of queue x */
+    return N - first > x ? (N - first - x - 1) / PK_QUEUES + 1 : 0;
+}
+
+__device__ __forceinline__ int pk_next(int *tickets, int first, int N, int own, int got, int lane) {
+    int x = own;
+    got = uni(got);
+    for (;;) {
+        if (got < pk_have(first, N, x)) return first + x + got * PK_QUEUES;
+        /* lane i < 8: queue own + i */
+        const int y = (own + lane) % PK_QUEUES;
+        const int taken = lane < PK_QUEUES ? __hip_atomic_load(tickets + y * PK_LINE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                                           : INT_MAX;
+        const unsigned long long left = __ballot(taken < pk_have(first, N, y));
+        if (!left) return INT_MAX;
+        x = (own + __ffsll(left) - 1) % PK_QUEUES;
+        got = 0;
+        if (lane == 0) got = pk_draw(tickets, x);
+        got = uni(got);
     }
-    return INT_MAX;
 }
 
 __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
-    /* [5][B + 1], of the sequences before each: wide items, narrow items, units, wide slots, narrow slots */
-    extern __shared__ int pk_cum[];
+    extern __shared__ int pk_lds[];   /* [PK_SUMS][B + 1] prefix sums, then [3][B]: row0, n, len */
     __shared__ __align__(16) unsigned char stages[PK_STAGES];
     __shared__ int tab[PK_WIDE_MAX];
-    __shared__ long long scan[2][WAVES];
+    __shared__ int scan[PK_SUMS][WAVES];
     __shared__ int sh_next;
     const AttnArgs &a = p.a;
     const int B = a.B;
-    int *wide = pk_cum, *narrow = wide + B + 1, *units = narrow + B + 1, *wslots = units + B + 1, *nslots = wslots + B + 1;
+    int *wide = pk_lds, *alone = wide + B + 1, *narrow = alone + B + 1, *units = narrow + B + 1, *wslots = units + B + 1,
+        *nslots = wslots + B + 1, *row0 = nslots + B + 1, *count = row0 + B, *length = count + B;
     bool fits = true;
     {
         const int per = (B + 255) / 256, b0 = min((int)threadIdx.x * per, B), b1 = min(b0 + per, B);
-        long long items[2] = {0, 0}, slots[2] = {0, 0}, un[2] = {0, 0};
+        int sum[PK_SUMS] = {0, 0, 0, 0, 0, 0};
         for (int b = b0; b < b1; b++) {
-            const PkSeq q = pk_plan(p, b);
-            const int u = max(q.tiles, 0) * a.Hkv, n = u * q.nch;
-            wide[b] = q.narrow ? 0 : n;
-            narrow[b] = q.narrow ? n : 0;
-            wslots[b] = !q.narrow && q.nch > 1 ? n : 0;
-            nslots[b] = q.narrow && q.nch > 1 ? n : 0;
-            units[b] = q.nch > 1 ? u : 0;
-            items[0] += wide[b]; items[1] += narrow[b];
-            slots[0] += wslots[b]; slots[1] += nslots[b];
-            un[0] += units[b];
+            const int c0 = p.cu[b], c1 = p.cu[b + 1], len = a.seq_lens[b];
+            row0[b] = min(max(c0, 0), p.rows);
+            count[b] = min(max(c1, row0[b]), p.rows) - row0[b];
+            length[b] = len;
+            const PkSeq q = pk_plan(p, row0[b], count[b], len);
+            const long long u64 = (long long)max(q.tiles, 0) * a.Hkv;
+            const int u = (int)min(u64, (long long)INT_MAX), n = (int)min(u64 * q.nch, (long long)INT_MAX);
+            const int cut = q.nch > 1 ? n : 0;
+            const int v[PK_SUMS] = {q.narrow ? 0 : n, q.narrow && q.alone ? n : 0, q.narrow && !q.alone ? n : 0,
+                                    q.nch > 1 ? u : 0, q.narrow ? 0 : cut, q.narrow ? cut : 0};
+#pragma unroll
+            for (int k = 0; k < PK_SUMS; k++) {
+                wide[k * (B + 1) + b] = v[k];
+                sum[k] = pk_add(sum[k], v[k]);
+            }
         }
-        pk_scan(items, scan);
-        pk_scan(slots, scan);
-        pk_scan(un, scan);
-        for (int b = b0; b < b1; b++) {
-            const int v[5] = {wide[b], narrow[b], units[b], wslots[b], nslots[b]};
-            wide[b] = (int)min(items[0], (long long)INT_MAX); narrow[b] = (int)min(items[1], (long long)INT_MAX);
-            units[b] = (int)min(un[0], (long long)INT_MAX);
-            wslots[b] = (int)min(slots[0], (long long)INT_MAX); nslots[b] = (int)min(slots[1], (long long)INT_MAX);
-            items[0] += v[0]; items[1] += v[1]; un[0] += v[2]; slots[0] += v[3]; slots[1] += v[4];
-        }
-        if (b1 == B && b0 < b1) {
-            wide[B] = (int)min(items[0], (long long)INT_MAX); narrow[B] = (int)min(items[1], (long long)INT_MAX);
-            units[B] = (int)min(un[0], (long long)INT_MAX);
-            wslots[B] = (int)min(slots[0], (long long)INT_MAX); nslots[B] = (int)min(slots[1], (long long)INT_MAX);
+        pk_scan(sum, scan);
+#pragma unroll
+        for (int k = 0; k < PK_SUMS; k++) {
+            for (int b = b0; b < b1; b++) {
+                const int v = wide[k * (B + 1) + b];
+                wide[k * (B + 1) + b] = sum[k];
+                sum[k] = pk_add(sum[k], v);
+            }
+            if (b1 == B && b0 < b1) wide[k * (B + 1) + B] = sum[k];
         }
         __syncthreads();
         /* row offsets that overlap could ask for more than the host sized the workspace for */
         fits = wslots[B] <= p.wide_slots && nslots[B] <= p.narrow_slots && units[B] <= p.units &&
-               (long long)wide[B] + narrow[B] < INT_MAX;
+               (long long)wide[B] + alone[B] < INT_MAX / 2 && narrow[B] < INT_MAX / 2;
     }
     /* rows of sequences whose length does not fit */
     for (int b = blockIdx.x; b < B; b += gridDim.x) {
-        const PkSeq q = pk_plan(p, b);
-        if (q.tiles >= 0 && fits) continue;
-        uint2 *dst = reinterpret_cast<uint2 *>(a.out + (long long)q.row0 * a.Hq * HEAD_DIM);
-        const long long quads = (long long)q.n * a.Hq * (HEAD_DIM / 4);
+        if (fits && (count[b] == 0 || (length[b] >= count[b] && length[b] <= a.max_len))) continue;
+        uint2 *dst = reinterpret_cast<uint2 *>(a.out + (long long)row0[b] * a.Hq * HEAD_DIM);
+        const long long quads = (long long)count[b] * a.Hq * (HEAD_DIM / 4);
         for (long long i = threadIdx.x; i < quads; i += 256) dst[i] = uint2{0x7FC07FC0u, 0x7FC07FC0u};
     }
     if (!fits) return;   /* every workgroup: no ticket is taken */
 
-    const int NW = uni(wide[B]), NN = uni(narrow[B]), G = gridDim.x;
-    for (int k = blockIdx.x; k < NW;) {
+    /* wide and alone items, by workgroups */
+    const int NW = uni(wide[B]), N = uni(NW + alone[B]), NN = uni(narrow[B]), G = gridDim.x, own = blockIdx.x % PK_QUEUES;
+    const auto plan = [&](int b) { return pk_plan(p, uni(row0[b]), uni(count[b]), uni(length[b])); };
+    for (int k = blockIdx.x; k < N;) {
+        int got = 0;
+        bool drawn = false;
         PkItem it;
-        it.b = uni(find_sequence(wide, B, k));
-        it.q = pk_plan(p, uni(p.cu[it.b]), uni(p.cu[it.b + 1]), uni(a.seq_lens[it.b]));
-        /* a sequence's items: the last tiles first, then the chunks, its KV heads fastest */
-        const int local = uni(k - wide[it.b]), rest = local / a.Hkv;
-        it.kvh = local - rest * a.Hkv;
-        const int tile = it.q.tiles - 1 - rest / it.q.nch, j = rest % it.q.nch, tokens = WAVES * PK_NT * (16 / a.G);
-        it.t0 = tile * tokens;
-        it.tn = min(it.q.n - it.t0, tokens);
-        /* the tile's own pages, its chunks [j0, j1), this chunk's pages within */
-        const int start = it.q.len - it.q.n;
-        const int lo = ((a.window >= 0 ? max(start + it.t0 - a.window, 0) : 0) / PAGE) & ~1;
-        const int hi = (start + it.t0 + it.tn - 1) / PAGE + 1;
-        const int j0 = (lo - it.q.pg0) / it.q.s, j1 = (hi - 1 - it.q.pg0) / it.q.s + 1;
-        it.pg0 = max(it.q.pg0 + j * it.q.s, lo);
-        it.pg1 = min(it.q.pg0 + (j + 1) * it.q.s, hi);
-        if (it.pg0 < it.pg1) {
-            const int chunks = j1 - j0, unit = uni(units[it.b]) + tile * a.Hkv + it.kvh;
-            const long long slot0 = uni(wslots[it.b]) + ((long long)tile * a.Hkv + it.kvh) * it.q.nch;
-            pk_wide(p, it, chunks, slot0 + j - j0, stages, tab);
-            if (chunks > 1) {
-                __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* this wave's part of the partial is at the coherent level */
-                __syncthreads();
-                if (threadIdx.x == 0)
-                    sh_next = __hip_atomic_fetch_add(p.arrived + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __syncthreads();
-                const int prior = uni(sh_next);
-                if (prior == chunks - 1) {
-                    pk_merge(p, it, false, chunks, slot0, threadIdx.x, 256);
+        if (k < NW) {
+            it.b = uni(find_sequence(wide, B, k));
+            it.q = plan(it.b);
+            /* a sequence's items: the last tiles first, then the chunks, its KV heads fastest */
+            const int local = uni(k - wide[it.b]), rest = (int)((unsigned)local / (unsigned)a.Hkv);
+            it.kvh = local - rest * a.Hkv;
+            const int back = (int)((unsigned)rest / (unsigned)it.q.nch);
+            const int tile = it.q.tiles - 1 - back, j = rest - back * it.q.nch, tokens = WAVES * PK_NT * p.tpt;
+            it.t0 = tile * tokens;
+            it.tn = min(it.q.n - it.t0, tokens);
+            /* the tile's own pages, its chunks [j0, j1), this chunk's pages within */
+            const int start = it.q.len - it.q.n;
+            const int lo = ((a.window >= 0 ? max(start + it.t0 - a.window, 0) : 0) / PAGE) & ~1;
+            const int hi = (start + it.t0 + it.tn - 1) / PAGE + 1;
+            const int j0 = (lo - it.q.pg0) / it.q.s, j1 = (hi - 1 - it.q.pg0) / it.q.s + 1;
+            it.pg0 = max(it.q.pg0 + j * it.q.s, lo);
+            it.pg1 = min(it.q.pg0 + (j + 1) * it.q.s, hi);
+            if (it.pg0 < it.pg1) {
+                const int chunks = j1 - j0, unit = uni(units[it.b]) + tile * a.Hkv + it.kvh;
+                const long long slot0 = uni(wslots[it.b]) + ((long long)tile * a.Hkv + it.kvh) * it.q.nch;
+                pk_wide(p, it, chunks, slot0 + j - j0, stages, tab);
+                if (chunks > 1) {
+                    drawn = N > G;
+                    if (drawn && threadIdx.x == 0) got = pk_draw(p.tickets, own);
+                    __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* this wave's part of the partial is out */
+                    __syncthreads();
                     if (threadIdx.x == 0)
-                        __hip_atomic_store(p.arrived + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        sh_next = __hip_atomic_fetch_add(p.arrived + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    __syncthreads();
+                    if (uni(sh_next) == chunks - 1) {
+                        pk_merge<4, 4>(p, it, false, chunks, slot0, threadIdx.x, 256);
+                        if (threadIdx.x == 0)
+                            __hip_atomic_store(p.arrived + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    }
                 }
             }
+        } else {
+            it.b = uni(find_sequence(alone, B, k - NW));
+            it.q = plan(it.b);
+            it.kvh = uni(k - NW - alone[it.b]);
+            it.t0 = 0;
+            it.tn = it.q.n;
+            it.pg0 = it.q.pg0;
+            it.pg1 = it.q.pg0 + it.q.np;
+            const int wave = uni((int)threadIdx.x >> 6);
+            unsigned char *ring = stages + wave * PK_NARROW_BUFS * PK_NARROW_STAGE;
+            if (it.tn <= p.tpt)
+                pk_narrow<1, true>(p, it, 1, 0, ring, wave, stages, reinterpret_cast<float *>(tab));
+            else
+                pk_narrow<2, true>(p, it, 1, 0, ring, wave, stages, reinterpret_cast<float *>(tab));
         }
-        if (NW <= G) break;
-        __syncthreads();   /* sh_next and the stages are used again */
-        if (threadIdx.x == 0) sh_next = pk_ticket(p.tickets, G, NW, blockIdx.x % PK_QUEUES);
+        if (N <= G) break;
+        __syncthreads();   /* sh_next, the stages and the table are used again */
+        if (threadIdx.x < WAVE) {
+            if (!drawn && threadIdx.x == 0) got = pk_draw(p.tickets, own);
+            sh_next = pk_next(p.tickets, G, N, own, got, threadIdx.x);
+        }
         __syncthreads();
         k = uni(sh_next);
     }
     __syncthreads();
 
-    /* the waves on their own; with no wide items before them, the first by index */
+    /* narrow items by the waves on their own, the first by index in the workgroups that had none of the others (so that
+     * not every wave of the chip starts with a ticket) */
     const int lane = threadIdx.x & (WAVE - 1), wave = uni((int)threadIdx.x >> 6);
-    const int first = NW ? 0 : WAVES * G;
+    const int free = max(G - N, 0), first = WAVES * free;
     unsigned char *ring = stages + wave * PK_NARROW_BUFS * PK_NARROW_STAGE;
-    for (int k = NW ? -1 : blockIdx.x + G * wave;;) {
-        if (k < 0 || k >= NN) {
-            if (NN <= first) break;
-            int next = 0;
-            if (lane == 0) next = pk_ticket(p.tickets + PK_QUEUES, first, NN, blockIdx.x % PK_QUEUES);
-            k = uni(next);
-            if (k >= NN) break;
-        }
+    int *tickets = p.tickets + PK_QUEUES * PK_LINE;
+    const bool queued = NN > first;
+    int k = (int)blockIdx.x - N + free * wave;
+    if ((int)blockIdx.x < N) {
+        int got = 0;
+        if (queued && lane == 0) got = pk_draw(tickets, own);
+        k = queued ? pk_next(tickets, first, NN, own, got, lane) : NN;
+    }
+    while (k < NN) {
         PkItem it;
         it.b = uni(find_sequence(narrow, B, k));
-        it.q = pk_plan(p, uni(p.cu[it.b]), uni(p.cu[it.b + 1]), uni(a.seq_lens[it.b]));
-        const int local = uni(k - narrow[it.b]), j = local / a.Hkv;   /* the chunks, its KV heads fastest */
+        it.q = plan(it.b);
+        const int local = uni(k - narrow[it.b]), j = (int)((unsigned)local / (unsigned)a.Hkv);   /* the chunks, its KV heads fastest */
         it.kvh = local - j * a.Hkv;
         it.t0 = 0;
         it.tn = it.q.n;
@@ -761,34 +849,41 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
         it.pg1 = j == it.q.nch - 1 ? it.q.pg0 + it.q.np : it.pg0 + it.q.s;
         const int chunks = it.q.nch;
         const long long slot0 = uni(nslots[it.b]) + (long long)it.kvh * chunks;
-        if (it.tn <= 16 / a.G)
-            pk_narrow<1>(p, it, chunks, slot0 + j, ring);
+        if (it.tn <= p.tpt)
+            pk_narrow<1, false>(p, it, chunks, slot0 + j, ring, 0, nullptr, nullptr);
         else
-            pk_narrow<2>(p, it, chunks, slot0 + j, ring);
+            pk_narrow<2, false>(p, it, chunks, slot0 + j, ring, 0, nullptr, nullptr);
+        int got = 0;
+        if (queued && lane == 0) got = pk_draw(tickets, own);
+        __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* nothing is in flight into the ring, and the partial is out */
         if (chunks > 1) {
-            int *count = p.arrived + uni(units[it.b]) + it.kvh;
+            int *arrived = p.arrived + uni(units[it.b]) + it.kvh;
             int prior = 0;
-            if (lane == 0) prior = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (lane == 0) prior = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (uni(prior) == chunks - 1) {
-                pk_merge(p, it, true, chunks, slot0, lane, WAVE);
-                if (lane == 0) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (it.tn * a.G <= 4)
+                    pk_merge<2, 16>(p, it, true, chunks, slot0, lane, WAVE);
+                else
+                    pk_merge<4, 8>(p, it, true, chunks, slot0, lane, WAVE);
+                if (lane == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
-        k = -1;
+        if (!queued) break;
+        k = pk_next(tickets, first, NN, own, got, lane);
     }
     /* where tickets were taken, the last workgroup to leave returns them */
-    if (NW <= G && NN <= first) return;
+    if (N <= G && !queued) return;
     __syncthreads();
     if (threadIdx.x == 0 &&
         __hip_atomic_fetch_add(p.done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == G - 1) {
         for (int x = 0; x < 2 * PK_QUEUES; x++)
-            __hip_atomic_store(p.tickets + x, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(p.tickets + x * PK_LINE, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __hip_atomic_store(p.done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
 /* The most partials and arrival counts a launch of these sizes can need, whatever its lengths (pk_plan): a narrow sequence
- * is Hkv units of at most ceil(pages / PK_NARROW_SPLIT) chunks, or ceil(pages / PK_SHORT_SPLIT) if short. A wide one has at least tpw + 1 rows; all of them together have at
+ * longer than PK_SHORT pages is Hkv units of at most ceil(pages / PK_NARROW_SPLIT) chunks. A wide one has at least tpw + 1 rows; all of them together have at
  * most rows / TW + their number tiles, each Hkv units, cut into at most ceil(pages / PK_WIDE_MIN) chunks, and no sequence
  * into more than PK_WIDE_ITEMS items unless its chunks would pass PK_WIDE_MAX pages. */
 struct PkSizes {
@@ -802,7 +897,7 @@ static PkSizes pk_sizes(long long rows, int B, int Hq, int Hkv, int max_seq_len,
     if (window >= 0) np = min(np, (rows + window) / PAGE + 3);
     const long long nw = min((long long)B, rows / (tpw + 1)), tiles = rows / (WAVES * tpw) + nw;
     PkSizes z = {};
-    const long long nch = max((min(np, (long long)PK_SHORT) - 1) / PK_SHORT_SPLIT + 1, (np - 1) / PK_NARROW_SPLIT + 1), wch = (np - 1) / PK_WIDE_MIN + 1, most = (np - 1) / PK_WIDE_MAX + 1;
+    const long long nch = np <= PK_SHORT ? 1 : (np - 1) / PK_NARROW_SPLIT + 1, wch = (np - 1) / PK_WIDE_MIN + 1, most = (np - 1) / PK_WIDE_MAX + 1;
     if (nch > 1) z.narrow_slots = min((long long)B, rows) * Hkv * nch;
     if (wch > 1) z.wide_slots = min(tiles * Hkv * wch, nw * PK_WIDE_ITEMS + (most > 1 ? tiles * Hkv * most : 0));
     z.units = (nch > 1 ? min((long long)B, rows) : 0) * Hkv + (wch > 1 ? tiles * Hkv : 0);
@@ -816,7 +911,7 @@ static size_t pk_part_bytes(const PkSizes &z) {
 /* As attention.hip's decode workspace: partials from the start, int32 counts (tickets, done, arrivals) in the last 1/256,
  * whose place depends on the workspace's size alone. */
 static size_t pk_count_region(size_t bytes) { return (bytes - ((bytes >> 8) & ~(size_t)3)) & ~(size_t)3; }
-static size_t pk_count_bytes(const PkSizes &z) { return (size_t)(z.units + 2 * PK_QUEUES + 1) * sizeof(int); }
+static size_t pk_count_bytes(const PkSizes &z) { return (size_t)(z.units + (2 * PK_QUEUES + 1) * PK_LINE) * sizeof(int); }
 
 static bool pk_shape_ok(long long rows, int B, int Hq, int Hkv, int max_seq_len) {
     return rows > 0 && rows <= 1LL << 24 && B > 0 && B <= PK_MAX_BATCH && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 &&
@@ -874,10 +969,10 @@ extern "C" int nc_packed_attn_fp8(const void *q, const void *k_pages, const void
     p.part_narrow = p.part_wide + z.wide_slots * PK_WIDE_COLS * (HEAD_DIM + 2);
     p.wide_slots = z.wide_slots; p.narrow_slots = z.narrow_slots;
     p.units = (int)z.units;
+    p.tpt = 16 / a.G;
     p.tickets = (int *)((char *)workspace + counts);
-    p.done = p.tickets + 2 * PK_QUEUES;
-    p.arrived = p.done + 1;
-    hipLaunchKernelGGL(packed_attn_kernel, dim3(device_packed_grid()), dim3(256), 5 * (B + 1) * sizeof(int),
-                       (hipStream_t)stream, p);
+    p.done = p.tickets + 2 * PK_QUEUES * PK_LINE;
+    p.arrived = p.done + PK_LINE;
+    hipLaunchKernelGGL(packed_attn_kernel, dim3(device_packed_grid()), dim3(256), (PK_SUMS * (B + 1) + 3 * B) * sizeof(int), (hipStream_t)stream, p);
     return (int)hipGetLastError();
 }

@@ -83,7 +83,7 @@ def plan(rows, n, length, hq, hkv, window):
     pg0 = first // page & ~1
     pages = (length - 1) // page + 1 - pg0
     if n <= 2 * tpt:
-        tiles, cut = 1, 16 if pages <= 67 else 64
+        tiles, cut = 1, 128 if pages <= 128 else 64
     else:
         tiles = (n - 1) // (8 * tpt) + 1
         want = max(256 // (tiles * hkv), 1)
@@ -108,7 +108,7 @@ def test_packed_workspace_holds_every_launch(lib):
         wide = sum(p[1] for p in plans if not p[0])
         narrow = sum(p[1] for p in plans if p[0])
         parts = (wide * 128 + narrow * 32) * 130 * 4
-        counts = 4 * (sum(p[2] for p in plans) + 17)
+        counts = 4 * (sum(p[2] for p in plans) + 17 * 32)
         need = lib.nc_packed_workspace_bytes(rows, batch, hq, hkv, most, window)
         assert parts <= need - need // 256 and counts <= need // 256, (hq, hkv, new, lens, window)
 
