@@ -51,8 +51,9 @@ static_assert(PK_SHORT <= 2 * WAVE && PK_NARROW_SPLIT + PK_MIN_TAIL <= 2 * WAVE,
 /* One stage: the pair's K (2 x 2 KiB), V (2 x 2 KiB) and scales (per page 16 of K, then 16 of V; wide: a copy a wave). */
 constexpr int PK_SCALE_AT = 4 * PAGE_BYTES, PK_SCALE_BYTES = 256;
 constexpr int PK_WIDE_STAGE = PK_SCALE_AT + WAVES * PK_SCALE_BYTES, PK_WIDE_BUFS = PK_AHEAD + 1;
-constexpr int PK_NARROW_STAGE = PK_SCALE_AT + PK_SCALE_BYTES, PK_NARROW_BUFS = 2;
-constexpr int PK_STAGES = WAVES * PK_NARROW_BUFS * PK_NARROW_STAGE;   /* bytes of LDS */
+constexpr int PK_NARROW_STAGE = PK_SCALE_AT + PK_SCALE_BYTES;
+constexpr int PK_BUFS = 2, PK_DEEP = 4;   /* pairs of a narrow wave's ring: two workgroups a CU, or one */
+constexpr int PK_STAGES = WAVES * PK_BUFS * PK_NARROW_STAGE;   /* bytes of LDS, the least */
 static_assert(PK_WIDE_BUFS * PK_WIDE_STAGE <= PK_STAGES, "the wide stages fit");
 typedef __attribute__((address_space(3))) void LdsVoid;
 
@@ -64,6 +65,7 @@ struct PackedArgs {
     long long wide_slots, narrow_slots;
     int units;                  /* arrival counts */
     int tpt;                    /* tokens of a 16-column tile: 16 / G */
+    int bufs;                   /* PK_BUFS or PK_DEEP */
     int *tickets, *done, *arrived;    /* [2][8][PK_LINE] (workgroups, waves), [PK_LINE], [units]; zero between launches */
 };
 
@@ -189,16 +191,20 @@ struct PkBounds {
     int in0, in1, written_hi;
 };
 
-/* Per-column key bounds of a wave whose first token is wt0 (end: one past the item's last), and its query operand. */
+/* Per-column key bounds of a wave whose first token is wt0 (end: one past the item's last), its query operand and the
+ * columns' references. */
 template <int NT>
 __device__ __forceinline__ void pk_columns(const PackedArgs &p, const PkItem &it, int wt0, int end, int lane,
-                                           PkBounds<NT> &kb, uint4 (&raw)[NT][4]) {
+                                           PkBounds<NT> &kb, uint4 (&raw)[NT][4], WaveState<NT> &st) {
     const AttnArgs &a = p.a;
     const int c = lane & 15, g = lane >> 4, start = it.q.len - it.q.n, tpt = p.tpt;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const int tok = pk_token(p, wt0, end, t, c), pos = start + tok;
         kb.hi[t] = tok >= 0 ? pos : -1;
+        /* a column that is not live has zero scores: with a finite reference they never ask for a rescale (one that did, on
+         * every pair, took half the time of a wave with few columns) */
+        st.m[t] = tok >= 0 ? -INFINITY : 0.0f;
         kb.lo[t] = tok >= 0 && a.window >= 0 ? max(pos - a.window, 0) : 0;
 #pragma unroll
         for (int cc = 0; cc < 4; cc++)
@@ -443,11 +449,11 @@ __device__ __forceinline__ void pk_wide(const PackedArgs &p, const PkItem &it, i
     }
     PkBounds<PK_NT> kb;
     uint4 raw[PK_NT][4];
-    pk_columns<PK_NT>(p, it, wt0, end, lane, kb, raw);
-    QOp qb[PK_NT];
-    q8_from_raw<PK_NT>(raw, qb);
     WaveState<PK_NT> ws;
     state_init(ws);
+    pk_columns<PK_NT>(p, it, wt0, end, lane, kb, raw, ws);
+    QOp qb[PK_NT];
+    q8_from_raw<PK_NT>(raw, qb);
     ws.sl2 = a.scale_log2;
     __syncthreads();
     for (int i = (max(w0 - it.pg0, 0) & ~1) + lane; i < min(npages, (w1 - it.pg0 + 1) & ~1); i += WAVE) bad |= tab[i] < 0;
@@ -537,7 +543,7 @@ __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it,
     };
     PkBounds<NT> kb;
     uint4 raw[NT][4];
-    pk_columns<NT>(p, it, 0, it.tn, lane, kb, raw);
+    pk_columns<NT>(p, it, 0, it.tn, lane, kb, raw, ws);
     const f32x4 zero = pk_zero();
     const int lds = pk_lds_offset(ring);
     const auto fetch = [&](int i, int buf) {
@@ -545,15 +551,18 @@ __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it,
                                                                                                        * first again */
         pk_fetch_narrow(a, entry(la), entry(lb), i < pairs, it.kvh, ring + buf * PK_NARROW_STAGE, lane);
     };
-    fetch(0, 0);
-    fetch(1, 1);
+    const int bufs = p.bufs;
+    for (int i = 0; i < bufs; i++) fetch(i, i);
     QOp qb[NT];
     q8_from_raw<NT>(raw, qb);
     for (int i = 0; i < pairs; i++) {
-        const int at = lds + (i & 1) * PK_NARROW_STAGE, lpa = it.pg0 + 2 * (first + stride * i);
-        __builtin_amdgcn_s_waitcnt(pk_wait(9, 15));   /* all but the younger pair's copies have landed */
+        const int buf = i & (bufs - 1), at = lds + buf * PK_NARROW_STAGE, lpa = it.pg0 + 2 * (first + stride * i);
+        /* all but the younger pairs' copies have landed */
+        if (bufs == PK_BUFS) __builtin_amdgcn_s_waitcnt(pk_wait(9 * (PK_BUFS - 1), 15));
+        else __builtin_amdgcn_s_waitcnt(pk_wait(9 * (PK_DEEP - 1), 15));
+        asm volatile("" ::: "memory");
         pk_pair<NT>(lpa, lpa + 1 < it.pg1, PkAt{at, at + PK_SCALE_AT}, qb, kb, zero, ws, lane,
-                    [&] { fetch(i + 2, i & 1); });
+                    [&] { fetch(i + bufs, buf); });
     }
     if constexpr (!ALONE) {
         const PkPart part = pk_part(p.part_narrow, p.narrow_slots, PK_NARROW_COLS, slot);
@@ -701,8 +710,9 @@ __device__ __forceinline__ int pk_next(int *tickets, int first, int N, int own, 
 }
 
 __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
-    extern __shared__ int pk_lds[];   /* [PK_SUMS][B + 1] prefix sums, then [3][B]: row0, n, len */
-    __shared__ __align__(16) unsigned char stages[PK_STAGES];
+    /* the stages, WAVES bufs PK_NARROW_STAGE bytes; [PK_SUMS][B + 1] prefix sums; [3][B]: row0, n, len */
+    extern __shared__ __align__(16) unsigned char stages[];
+    int *pk_lds = reinterpret_cast<int *>(stages + WAVES * p.bufs * PK_NARROW_STAGE);
     __shared__ int tab[PK_WIDE_MAX];
     __shared__ int scan[PK_SUMS][WAVES];
     __shared__ int sh_next;
@@ -732,15 +742,19 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
             }
         }
         pk_scan(sum, scan);
+        for (int b = b0; b < b1; b++) {
+            int v[PK_SUMS];
 #pragma unroll
-        for (int k = 0; k < PK_SUMS; k++) {
-            for (int b = b0; b < b1; b++) {
-                const int v = wide[k * (B + 1) + b];
+            for (int k = 0; k < PK_SUMS; k++) v[k] = wide[k * (B + 1) + b];
+#pragma unroll
+            for (int k = 0; k < PK_SUMS; k++) {
                 wide[k * (B + 1) + b] = sum[k];
-                sum[k] = pk_add(sum[k], v);
+                sum[k] = pk_add(sum[k], v[k]);
             }
-            if (b1 == B && b0 < b1) wide[k * (B + 1) + B] = sum[k];
         }
+        if (b1 == B && b0 < b1)
+#pragma unroll
+            for (int k = 0; k < PK_SUMS; k++) wide[k * (B + 1) + B] = sum[k];
         __syncthreads();
         /* row offsets that overlap could ask for more than the host sized the workspace for */
         fits = wslots[B] <= p.wide_slots && nslots[B] <= p.narrow_slots && units[B] <= p.units &&
@@ -807,7 +821,7 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
             it.pg0 = it.q.pg0;
             it.pg1 = it.q.pg0 + it.q.np;
             const int wave = uni((int)threadIdx.x >> 6);
-            unsigned char *ring = stages + wave * PK_NARROW_BUFS * PK_NARROW_STAGE;
+            unsigned char *ring = stages + wave * p.bufs * PK_NARROW_STAGE;
             if (it.tn <= p.tpt)
                 pk_narrow<1, true>(p, it, 1, 0, ring, wave, stages, reinterpret_cast<float *>(tab));
             else
@@ -828,7 +842,7 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
      * not every wave of the chip starts with a ticket) */
     const int lane = threadIdx.x & (WAVE - 1), wave = uni((int)threadIdx.x >> 6);
     const int free = max(G - N, 0), first = WAVES * free;
-    unsigned char *ring = stages + wave * PK_NARROW_BUFS * PK_NARROW_STAGE;
+    unsigned char *ring = stages + wave * p.bufs * PK_NARROW_STAGE;
     int *tickets = p.tickets + PK_QUEUES * PK_LINE;
     const bool queued = NN > first;
     int k = (int)blockIdx.x - N + free * wave;
@@ -888,6 +902,7 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
  * into more than PK_WIDE_ITEMS items unless its chunks would pass PK_WIDE_MAX pages. */
 struct PkSizes {
     long long wide_slots, narrow_slots, units;
+    long long items, narrow_chunks;   /* wide items at most; a narrow sequence's chunks at most */
 };
 
 static PkSizes pk_sizes(long long rows, int B, int Hq, int Hkv, int max_seq_len, int window) {
@@ -900,6 +915,8 @@ static PkSizes pk_sizes(long long rows, int B, int Hq, int Hkv, int max_seq_len,
     const long long nch = np <= PK_SHORT ? 1 : (np - 1) / PK_NARROW_SPLIT + 1, wch = (np - 1) / PK_WIDE_MIN + 1, most = (np - 1) / PK_WIDE_MAX + 1;
     if (nch > 1) z.narrow_slots = min((long long)B, rows) * Hkv * nch;
     if (wch > 1) z.wide_slots = min(tiles * Hkv * wch, nw * PK_WIDE_ITEMS + (most > 1 ? tiles * Hkv * most : 0));
+    z.items = max(z.wide_slots, tiles * Hkv);
+    z.narrow_chunks = nch;
     z.units = (nch > 1 ? min((long long)B, rows) : 0) * Hkv + (wch > 1 ? tiles * Hkv : 0);
     return z;
 }
@@ -916,14 +933,6 @@ static size_t pk_count_bytes(const PkSizes &z) { return (size_t)(z.units + (2 * 
 static bool pk_shape_ok(long long rows, int B, int Hq, int Hkv, int max_seq_len) {
     return rows > 0 && rows <= 1LL << 24 && B > 0 && B <= PK_MAX_BATCH && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 &&
            Hq / Hkv <= 16 && Hkv <= 1024 && max_seq_len > 0;
-}
-
-static int device_packed_grid() {
-    static int grid[64] = {0};
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 512;
-    if (!grid[dev]) grid[dev] = 2 * device_cus() / PK_QUEUES * PK_QUEUES;
-    return max(grid[dev], PK_QUEUES);
 }
 
 }  // namespace nc
@@ -973,6 +982,13 @@ extern "C" int nc_packed_attn_fp8(const void *q, const void *k_pages, const void
     p.tickets = (int *)((char *)workspace + counts);
     p.done = p.tickets + 2 * PK_QUEUES * PK_LINE;
     p.arrived = p.done + PK_LINE;
-    hipLaunchKernelGGL(packed_attn_kernel, dim3(device_packed_grid()), dim3(256), (PK_SUMS * (B + 1) + 3 * B) * sizeof(int), (hipStream_t)stream, p);
+    /* Where the launch cannot have more work than one workgroup a CU, one is launched with rings twice as deep: a wave that
+     * streams alone waits for memory (one sequence, 1,029 keys, 6 heads: 17.8 -> DEEP_US us). The results do not change. */
+    const int cus = device_cus() / PK_QUEUES * PK_QUEUES;
+    const long long few = min((long long)B, rows) * Hkv;
+    const bool deep = z.items + few <= cus && few * z.narrow_chunks <= (long long)WAVES * cus;
+    p.bufs = deep ? PK_DEEP : PK_BUFS;
+    const size_t lds = (size_t)WAVES * p.bufs * PK_NARROW_STAGE + (PK_SUMS * (B + 1) + 3 * B) * sizeof(int);
+    hipLaunchKernelGGL(packed_attn_kernel, dim3(max(deep ? cus : 2 * cus, PK_QUEUES)), dim3(256), lds, (hipStream_t)stream, p);
     return (int)hipGetLastError();
 }
