@@ -17,7 +17,7 @@
  *           A sequence of at most PK_SHORT pages is not cut but shared by the four waves of a workgroup, which merge
  *           through LDS ("alone": it costs no round trips through memory, which is what a short one's time is made of)
  *   wide    a tile of up to 128 columns, 32 a wave: the four waves of a workgroup walk the same pairs, each fetched once
- *           (PK_AHEAD ahead)
+ *           (two stages of two pairs ahead)
  *
  * A sequence's keys are cut into chunks (pk_plan), so that few rows over many keys still fill the chip; a (tile, KV head)
  * of several chunks leaves one partial (O, max, sum) in fp32 a chunk, and whoever finishes its last chunk merges them in
@@ -44,13 +44,14 @@ constexpr int PK_SHORT = 2 * PK_NARROW_SPLIT;  /* a narrow sequence of at most s
 constexpr int PK_WIDE_MIN = 128;               /* least and most pages of a wide chunk */
 constexpr int PK_WIDE_MAX = 1024;
 constexpr int PK_WIDE_ITEMS = 256;             /* items a wide sequence is cut into at most, if its chunks stay that long */
-constexpr int PK_AHEAD = 3;                    /* wide: pairs in flight */
+constexpr int PK_AHEAD = 2;                    /* wide: stages of two pairs in flight */
 static_assert(PK_SHORT <= 2 * WAVE && PK_NARROW_SPLIT + PK_MIN_TAIL <= 2 * WAVE,
               "a narrow item's block-table entries: two a lane");
 
-/* One stage: the pair's K (2 x 2 KiB), V (2 x 2 KiB) and scales (per page 16 of K, then 16 of V; wide: a copy a wave). */
+/* A pair in a stage: K (2 x 2 KiB), V (2 x 2 KiB), and its scales, per page 16 of K, then 16 of V. A narrow stage is one
+ * pair, scales last; a wide one two pairs, then both pairs' scales for each wave. */
 constexpr int PK_SCALE_AT = 4 * PAGE_BYTES, PK_SCALE_BYTES = 256;
-constexpr int PK_WIDE_STAGE = PK_SCALE_AT + WAVES * PK_SCALE_BYTES, PK_WIDE_BUFS = PK_AHEAD + 1;
+constexpr int PK_WIDE_STAGE = 2 * PK_SCALE_AT + WAVES * 2 * PK_SCALE_BYTES, PK_WIDE_BUFS = PK_AHEAD + 1;
 constexpr int PK_NARROW_STAGE = PK_SCALE_AT + PK_SCALE_BYTES;
 constexpr int PK_BUFS = 2, PK_DEEP = 4;   /* pairs of a narrow wave's ring: two workgroups a CU, or one */
 constexpr int PK_STAGES = WAVES * PK_BUFS * PK_NARROW_STAGE;   /* bytes of LDS, the least */
@@ -384,118 +385,234 @@ __device__ __forceinline__ void pk_pair(int lpa, bool has_b, PkAt stage, const Q
     }
 }
 
-/* Column `col` (c of tile t, token tok; < 0: none) of a wave's state: its bf16 row, or its part of a partial. */
+/* A column of tile t (c of it, token tok): its bf16 row; or its part of a partial, column `col` there. l: of all groups. */
 template <int NT>
-__device__ __forceinline__ void pk_store(const PackedArgs &p, const PkItem &it, int chunks, WaveState<NT> &ws, int t, int tok,
-                                         int col, int c, int g, Rsrc ro, Rsrc rm) {
-    ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
-    if (tok < 0) return;
-    if (chunks == 1) {
-        uint16_t *dst = p.a.out + pk_row(p, it, tok, c) * HEAD_DIM;
-        const float inv = 1.0f / ws.l[t];
+__device__ __forceinline__ void pk_store_row(const PackedArgs &p, const PkItem &it, const WaveState<NT> &ws, int t, int tok, int c,
+                                             int g) {
+    uint16_t *dst = p.a.out + pk_row(p, it, tok, c) * HEAD_DIM;
+    const float inv = 1.0f / ws.l[t];
 #pragma unroll
-        for (int d = 0; d < 8; d++) {
-            float v[4];
+    for (int d = 0; d < 8; d++) {
+        float v[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = ws.bad ? NAN : ws.o[t][d][i] * inv;
-            store_bf16x4(dst + 16 * d + 4 * g, v);
-        }
-    } else {
+        for (int i = 0; i < 4; i++) v[i] = ws.bad ? NAN : ws.o[t][d][i] * inv;
+        store_bf16x4(dst + 16 * d + 4 * g, v);
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ void pk_store_part(const WaveState<NT> &ws, int t, int col, int g, Rsrc ro, Rsrc rm) {
 #pragma unroll
-        for (int d = 0; d < 8; d++)
-            part_store(ro, (col * HEAD_DIM + 16 * d + 4 * g) * 4,
-                       float4{ws.o[t][d][0], ws.o[t][d][1], ws.o[t][d][2], ws.o[t][d][3]});
-        if (g == 0)
-            __builtin_amdgcn_raw_buffer_store_b64(
-                u32x2{__float_as_uint(ws.bad ? NAN : ws.m[t]), __float_as_uint(ws.l[t])}, rm, col * 8, 0, SC1);
+    for (int d = 0; d < 8; d++)
+        part_store(ro, (col * HEAD_DIM + 16 * d + 4 * g) * 4,
+                   float4{ws.o[t][d][0], ws.o[t][d][1], ws.o[t][d][2], ws.o[t][d][3]});
+    if (g == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(ws.bad ? NAN : ws.m[t]), __float_as_uint(ws.l[t])}, rm,
+                                              col * 8, 0, SC1);
+}
+
+/* Tickets: queue x holds the items first + x, first + x + 8, ... below N, its count on a line of its own (atomics on one
+ * line wait for each other, wherever they come from). pk_draw takes a ticket of queue x. pk_next makes an item of one drawn
+ * from queue `own`, or draws from whichever queue has some left (INT_MAX: none has); a whole wave calls it. Items are drawn
+ * when the one before is done: drawn earlier, an item would wait for it. */
+constexpr int PK_LINE = 32;   /* ints of a 128-byte line */
+
+__device__ __forceinline__ int pk_draw(int *tickets, int x) {
+    return __hip_atomic_fetch_add(tickets + x * PK_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ int pk_have(int first, int N, int x) {   /* items of queue x */
+    return N - first > x ? (N - first - x - 1) / PK_QUEUES + 1 : 0;
+}
+
+__device__ __forceinline__ int pk_next(int *tickets, int first, int N, int own, int got, int lane) {
+    int x = own;
+    got = uni(got);
+    for (;;) {
+        if (got < pk_have(first, N, x)) return first + x + got * PK_QUEUES;
+        /* lane i < 8: queue own + i */
+        const int y = (own + lane) % PK_QUEUES;
+        const int taken = lane < PK_QUEUES ? __hip_atomic_load(tickets + y * PK_LINE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                                           : INT_MAX;
+        const unsigned long long left = __ballot(taken < pk_have(first, N, y));
+        if (!left) return INT_MAX;
+        x = (own + __ffsll(left) - 1) % PK_QUEUES;
+        got = 0;
+        if (lane == 0) got = pk_draw(tickets, x);
+        got = uni(got);
     }
 }
 
 /* --- wide items */
 
-/* One stage's copies: wave w K bytes [1024 w, 1024 w + 1024) of the pair (pages a, a, b, b), the same of V, and all 256
- * scale bytes into its own slot; every wave always issues three. */
+/* One stage's copies, two pairs (pages 4 s .. 4 s + 3 of the chunk; past its end, its last one again): wave w page w's K and
+ * V (two of 1 KiB each) and all four pages' scales into its own slot (two of 256 bytes); every wave always issues six. */
 __device__ __forceinline__ void pk_fetch_wide(const AttnArgs &a, const int *tab, int npages, int s, int kvh, unsigned char *st,
                                               int wave, int lane) {
-    const int la = 2 * min(s, (npages - 1) / 2), lb = la + 1 < npages ? la + 1 : la;   /* past the range: its last pair */
-    const int pa = __builtin_amdgcn_readfirstlane(tab[la]), pb = __builtin_amdgcn_readfirstlane(tab[lb]);
-    const long long ph = (long long)(wave < 2 ? pa : pb) * a.Hkv + kvh;
-    const int half = (wave & 1) * 1024;
-    __builtin_amdgcn_global_load_lds((const void *)(a.k_pages + ph * PAGE_BYTES + half + lane * 16),
-                                     (LdsVoid *)(st + wave * 1024), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds((const void *)(a.v_pages + ph * PAGE_BYTES + half + lane * 16),
-                                     (LdsVoid *)(st + 2 * PAGE_BYTES + wave * 1024), 16, 0, 0);
-    const long long sh = (long long)(lane < 32 ? pa : pb) * a.Hkv + kvh;
-    __builtin_amdgcn_global_load_lds((const void *)(a.kv_scale + sh * 2 * PAGE + (lane & 31)),
-                                     (LdsVoid *)(st + PK_SCALE_AT + wave * PK_SCALE_BYTES), 4, 0, 0);
+    const int pg = uni(tab[min(4 * s + wave, npages - 1)]);
+    const long long ph = (long long)pg * a.Hkv + kvh;
+    /* pair wave / 2: K of its pages, then V */
+    unsigned char *k = st + (wave >> 1) * PK_SCALE_AT + (wave & 1) * PAGE_BYTES, *v = k + 2 * PAGE_BYTES;
+    __builtin_amdgcn_global_load_lds((const void *)(a.k_pages + ph * PAGE_BYTES + lane * 16), (LdsVoid *)k, 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void *)(a.k_pages + ph * PAGE_BYTES + 1024 + lane * 16), (LdsVoid *)(k + 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void *)(a.v_pages + ph * PAGE_BYTES + lane * 16), (LdsVoid *)v, 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void *)(a.v_pages + ph * PAGE_BYTES + 1024 + lane * 16), (LdsVoid *)(v + 1024), 16, 0, 0);
+    unsigned char *sc = st + 2 * PK_SCALE_AT + wave * 2 * PK_SCALE_BYTES;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const long long sh = (long long)tab[min(4 * s + 2 * h + (lane >> 5), npages - 1)] * a.Hkv + kvh;
+        __builtin_amdgcn_global_load_lds((const void *)(a.kv_scale + sh * 2 * PAGE + (lane & 31)),
+                                         (LdsVoid *)(sc + h * PK_SCALE_BYTES), 4, 0, 0);
+    }
 }
 
-__device__ __forceinline__ void pk_wide(const PackedArgs &p, const PkItem &it, int chunks, long long slot,
-                                        unsigned char *stages, int *tab) {
+/* The merge of a tile's partials by the workgroup that finishes last, in chunk order, from its own state (chunk `own`) and
+ * the others' in slots slot0 ..: a lane loads what it holds itself, eight dims a tile of its columns, a chunk at a time. */
+__device__ __forceinline__ void pk_join(const PackedArgs &p, const PkItem &it, int chunks, int own, long long slot0,
+                                        const WaveState<PK_NT> &ws, const int (&tok)[PK_NT], int wave, int c, int g) {
+    float m[PK_NT], l[PK_NT];
+    f32x4 o[PK_NT][8];
+#pragma unroll
+    for (int t = 0; t < PK_NT; t++) {
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 8; d++) o[t][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (int j = 0; j < chunks; j++) {
+        float mj[PK_NT], lj[PK_NT];
+        f32x4 oj[PK_NT][8];
+        if (j == own) {
+#pragma unroll
+            for (int t = 0; t < PK_NT; t++) {
+                mj[t] = ws.bad ? NAN : ws.m[t];
+                lj[t] = ws.l[t];
+#pragma unroll
+                for (int d = 0; d < 8; d++) oj[t][d] = ws.o[t][d];
+            }
+        } else {   /* sc1: past this XCD's L2, where another workgroup's stores are not seen */
+            const PkPart part = pk_part(p.part_wide, p.wide_slots, PK_WIDE_COLS, slot0 + j);
+            const Rsrc ro = page_rsrc(part.o, PK_WIDE_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_WIDE_COLS * 8);
+#pragma unroll
+            for (int t = 0; t < PK_NT; t++) {
+                const int col = (wave * PK_NT + t) * 16 + c;
+                const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(rm, col * 8, 0, SC1);
+                mj[t] = __uint_as_float(w[0]);
+                lj[t] = __uint_as_float(w[1]);
+#pragma unroll
+                for (int d = 0; d < 8; d++) oj[t][d] = part_load(ro, (col * HEAD_DIM + 16 * d + 4 * g) * 4);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < PK_NT; t++) {
+            const float mb = fmaxf(m[t], mj[t]);
+            const float keep = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - mb);
+            const float f = mj[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mj[t] - mb);   /* NaN: a bad page */
+            l[t] = l[t] * keep + lj[t] * f;
+            m[t] = mb;
+#pragma unroll
+            for (int d = 0; d < 8; d++) o[t][d] = o[t][d] * keep + oj[t][d] * f;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < PK_NT; t++) {
+        if (tok[t] < 0) continue;
+        uint16_t *dst = p.a.out + pk_row(p, it, tok[t], c) * HEAD_DIM;
+        const float inv = 1.0f / l[t];
+#pragma unroll
+        for (int d = 0; d < 8; d++) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = o[t][d][i] * inv;
+            store_bf16x4(dst + 16 * d + 4 * g, v);
+        }
+    }
+}
+
+/* own: this item's place among its tile's chunks, whose partials are in slots slot0 ..; arrived: their count. queue: NULL, or
+ * where thread 0 draws the workgroup's next ticket while its partial is on its way (returned). */
+__device__ __forceinline__ int pk_wide(const PackedArgs &p, const PkItem &it, int chunks, int own, long long slot0, int *arrived,
+                                       unsigned char *stages, int *tab, int &shared, int *queue) {
     const AttnArgs &a = p.a;
     const int lane = pk_lane(), wave = uni((int)threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int tpw = p.tpt * PK_NT, start = it.q.len - it.q.n;
     const int wt0 = it.t0 + wave * tpw, end = it.t0 + it.tn, npages = it.pg1 - it.pg0;
     const bool on = wt0 < end;
     const int last = min(wt0 + tpw, end) - 1;
-    /* the wave's own pages within the chunk's */
+    /* the wave's own pairs within the chunk's */
     const int w0 = max((a.window >= 0 ? max(start + wt0 - a.window, 0) : 0) / PAGE, it.pg0);
-    const int w1 = on ? min((start + last) / PAGE + 1, it.pg1) : 0;
-    const int32_t *bt = a.block_table + (long long)it.b * a.max_pages + it.pg0;
-    bool bad = false;   /* an entry outside the pool among the pairs this wave computes */
-    for (int i = threadIdx.x; i < npages; i += 256) {
-        const int e = bt[i];
-        tab[i] = (unsigned)e < (unsigned)a.num_pages ? e : -1;
-    }
+    const int w1 = on ? min((start + last) / PAGE + 1, it.pg1) : 0, count = (npages + 1) / 2;
+    const int s0 = min(max(w0 - it.pg0, 0) / 2, count), s1 = min(max(w1 - it.pg0 + 1, 0) / 2, count);
     PkBounds<PK_NT> kb;
     uint4 raw[PK_NT][4];
     WaveState<PK_NT> ws;
     state_init(ws);
-    pk_columns<PK_NT>(p, it, wt0, end, lane, kb, raw, ws);
-    QOp qb[PK_NT];
-    q8_from_raw<PK_NT>(raw, qb);
     ws.sl2 = a.scale_log2;
-    __syncthreads();
-    for (int i = (max(w0 - it.pg0, 0) & ~1) + lane; i < min(npages, (w1 - it.pg0 + 1) & ~1); i += WAVE) bad |= tab[i] < 0;
+    pk_columns<PK_NT>(p, it, wt0, end, lane, kb, raw, ws);
+    /* every wave looks at all the entries (is one outside the pool among its pairs'?) and stores a quarter of them */
+    const int32_t *bt = a.block_table + (long long)it.b * a.max_pages + it.pg0;
+    bool bad = false;
+    for (int i = lane; i < npages; i += WAVE) {
+        const int e = bt[i];
+        const bool ok = (unsigned)e < (unsigned)a.num_pages;
+        bad = bad || (!ok && i >= 2 * s0 && i < 2 * s1);
+        if (((i >> 6) & (WAVES - 1)) == wave) tab[i] = ok ? e : 0;   /* only read: those waves report NaN */
+    }
     ws.bad = __any(bad);
     __syncthreads();
-    for (int i = threadIdx.x; i < npages; i += 256) tab[i] = max(tab[i], 0);   /* only read: those waves report NaN */
-    __syncthreads();
-
     const f32x4 zero = pk_zero();
-    const int lds = pk_lds_offset(stages), count = (npages + 1) / 2;
+    const int lds = pk_lds_offset(stages), steps = (count + 1) / 2;
     for (int s = 0; s < PK_AHEAD; s++) pk_fetch_wide(a, tab, npages, s, it.kvh, stages + s * PK_WIDE_STAGE, wave, lane);
+    QOp qb[PK_NT];
+    q8_from_raw<PK_NT>(raw, qb);
     /* step s: this wave's copies of stage s have landed (then everyone's, after the barrier, and everyone's reads of the
-     * stage before are done); refill that buffer with stage s + PK_AHEAD; compute stage s where it meets this wave's pages.
-     * Loops of their own for the stages before and after those: a branch around the pair inside one loop would cost a copy
-     * of the accumulators a step */
-    int s = 0, buf = 0;
-    const auto advance = [&]() {
-        __builtin_amdgcn_s_waitcnt(pk_wait(3 * (PK_AHEAD - 1), 15));
+     * stage before are done); refill that buffer with stage s + PK_AHEAD; compute the stage's pairs that meet this wave's */
+    for (int s = 0, buf = 0; s < steps; s++) {
+        __builtin_amdgcn_s_waitcnt(pk_wait(6 * (PK_AHEAD - 1), 15));
         pk_barrier();
         const int into = buf == 0 ? PK_WIDE_BUFS - 1 : buf - 1;   /* (s + PK_AHEAD) % PK_WIDE_BUFS */
         pk_fetch_wide(a, tab, npages, s + PK_AHEAD, it.kvh, stages + into * PK_WIDE_STAGE, wave, lane);
-    };
-    const auto next = [&]() {
-        s++;
+        const int st = lds + buf * PK_WIDE_STAGE, until = min(2 * s + 2, s1);
+        for (int i = max(2 * s, s0); i < until; i++) {
+            const int at = st + (i & 1) * PK_SCALE_AT, lpa = it.pg0 + 2 * i;
+            pk_pair<PK_NT>(lpa, lpa + 1 < it.pg1, PkAt{at, st + 2 * PK_SCALE_AT + (2 * wave + (i & 1)) * PK_SCALE_BYTES}, qb, kb,
+                           zero, ws, lane, [] {});
+        }
         buf = buf == PK_WIDE_BUFS - 1 ? 0 : buf + 1;
-    };
-    const int s0 = min(max(w0 - it.pg0, 0) / 2, count), s1 = min(max(w1 - it.pg0 + 1, 0) / 2, count);
-    for (; s < s0; next()) advance();
-    for (; s < s1; next()) {
-        advance();
-        const int at = lds + buf * PK_WIDE_STAGE, lpa = it.pg0 + 2 * s;
-        pk_pair<PK_NT>(lpa, lpa + 1 < it.pg1, PkAt{at, at + PK_SCALE_AT + wave * PK_SCALE_BYTES}, qb, kb, zero, ws, lane, [] {});
     }
-    for (; s < count; next()) advance();
+    int prior = 0, got = -1;
+    if (chunks > 1 && threadIdx.x == 0) prior = __hip_atomic_load(arrived, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __builtin_amdgcn_s_waitcnt(0);   /* every copy has landed before the stages and the table are used again */
-    pk_barrier();
-
-    const PkPart part = pk_part(p.part_wide, p.wide_slots, PK_WIDE_COLS, slot);
-    const Rsrc ro = page_rsrc(part.o, PK_WIDE_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_WIDE_COLS * 8);
+    if (threadIdx.x == 0) shared = prior;
+    __syncthreads();
+    int tok[PK_NT];
 #pragma unroll
-    for (int t = 0; t < PK_NT; t++)
-        pk_store<PK_NT>(p, it, chunks, ws, t, pk_token(p, wt0, end, t, c), (wave * PK_NT + t) * 16 + c, c, g, ro, rm);
+    for (int t = 0; t < PK_NT; t++) {
+        ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
+        tok[t] = pk_token(p, wt0, end, t, c);
+    }
+    if (chunks == 1) {
+#pragma unroll
+        for (int t = 0; t < PK_NT; t++)
+            if (tok[t] >= 0) pk_store_row<PK_NT>(p, it, ws, t, tok[t], c, g);
+        return got;
+    }
+    if (uni(shared) != chunks - 1) {   /* others are not done: leave a partial */
+        const PkPart part = pk_part(p.part_wide, p.wide_slots, PK_WIDE_COLS, slot0 + own);
+        const Rsrc ro = page_rsrc(part.o, PK_WIDE_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_WIDE_COLS * 8);
+#pragma unroll
+        for (int t = 0; t < PK_NT; t++)
+            if (tok[t] >= 0) pk_store_part<PK_NT>(ws, t, (wave * PK_NT + t) * 16 + c, g, ro, rm);
+        if (queue && threadIdx.x == 0) got = pk_draw(queue, 0);
+        __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* this wave's part of the partial is out; then everyone's */
+        __syncthreads();
+        if (threadIdx.x == 0) shared = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (uni(shared) != chunks - 1) return got;
+    }
+    pk_join(p, it, chunks, own, slot0, ws, tok, wave, c, g);
+    if (threadIdx.x == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return got;
 }
 
 /* --- narrow items */
@@ -568,7 +685,10 @@ __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it,
         const PkPart part = pk_part(p.part_narrow, p.narrow_slots, PK_NARROW_COLS, slot);
         const Rsrc ro = page_rsrc(part.o, PK_NARROW_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_NARROW_COLS * 8);
 #pragma unroll
-        for (int t = 0; t < NT; t++) pk_store<NT>(p, it, chunks, ws, t, pk_token(p, 0, it.tn, t, c), t * 16 + c, c, g, ro, rm);
+        for (int t = 0; t < NT; t++) {
+            ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
+            if (pk_token(p, 0, it.tn, t, c) >= 0) pk_store_part<NT>(ws, t, t * 16 + c, g, ro, rm);
+        }
         return;   /* the caller waits for the stores, and for the copies that read nothing */
     }
     float *merged = reinterpret_cast<float *>(stages), *sums = ml + WAVES * PK_NARROW_COLS;
@@ -607,24 +727,22 @@ __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it,
     }
 }
 
-/* The merge of a (tile, KV head)'s partials in slots slot0 .. slot0 + chunks - 1, in chunk order, into its bf16 rows, by
- * `threads` threads, each P pieces of four dims at a time and NB chunks' loads of them in flight: the merge is bound by
- * their latency, so few columns take many chunks at a time and many columns few. */
+/* The merge of a narrow unit's partials in slots slot0 .. slot0 + chunks - 1, in chunk order, into its bf16 rows, by one
+ * wave, each lane P pieces of four dims at a time and NB chunks' loads of them in flight: the merge is bound by their
+ * latency, so few columns take many chunks at a time and many columns few. */
 template <int P, int NB>
-__device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, bool narrow, int chunks, long long slot0,
-                                         int thread, int threads) {
+__device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, int chunks, long long slot0, int lane) {
     const AttnArgs &a = p.a;
-    const int cols = narrow ? PK_NARROW_COLS : PK_WIDE_COLS, pieces = cols * (HEAD_DIM / 4);
-    const PkPart part = pk_part(narrow ? p.part_narrow : p.part_wide, narrow ? p.narrow_slots : p.wide_slots, cols, slot0);
-    for (int i0 = thread; i0 < pieces; i0 += P * threads) {
+    constexpr int cols = PK_NARROW_COLS, pieces = cols * (HEAD_DIM / 4);
+    const PkPart part = pk_part(p.part_narrow, p.narrow_slots, cols, slot0);
+    for (int i0 = lane; i0 < pieces; i0 += P * WAVE) {
         int tok[P];
         bool some = false;
         float m[P], l[P];
         f32x4 o[P];
 #pragma unroll
         for (int k = 0; k < P; k++) {
-            const int col = (i0 + k * threads) >> 5;
-            /* a wave's tiles follow the last one's */
+            const int col = (i0 + k * WAVE) >> 5;
             tok[k] = col < cols ? pk_token(p, it.t0, it.t0 + it.tn, col >> 4, col & 15) : -1;
             some = some || tok[k] >= 0;
             m[k] = -INFINITY;
@@ -645,7 +763,7 @@ __device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, 
                 const Rsrc rm = page_rsrc(part.ml + j * cols * 2, live ? cols * 8 : 0);
 #pragma unroll
                 for (int k = 0; k < P; k++) {
-                    const int i = i0 + k * threads;
+                    const int i = i0 + k * WAVE;
                     oj[n][k] = part_load(ro, i * 16);
                     const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(rm, (i >> 5) * 8, 0, SC1);
                     mj[n][k] = __uint_as_float(w[0]);
@@ -668,44 +786,12 @@ __device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, 
 #pragma unroll
         for (int k = 0; k < P; k++) {
             if (tok[k] < 0) continue;
-            const int i = i0 + k * threads, col = i >> 5;
+            const int i = i0 + k * WAVE, col = i >> 5;
             float v[4];
 #pragma unroll
             for (int d = 0; d < 4; d++) v[d] = o[k][d] / l[k];
             store_bf16x4(a.out + pk_row(p, it, tok[k], col & 15) * HEAD_DIM + 4 * (i & 31), v);
         }
-    }
-}
-
-/* Tickets: queue x holds the items first + x, first + x + 8, ... below N, its count on a line of its own (atomics on one
- * line wait for each other, wherever they come from). pk_draw takes a ticket of queue x. pk_next makes an item of one drawn
- * from queue `own`, or draws from whichever queue has some left (INT_MAX: none has); a whole wave calls it. Items are drawn
- * when the one before is done: drawn earlier, an item would wait for it. */
-constexpr int PK_LINE = 32;   /* ints of a 128-byte line */
-
-__device__ __forceinline__ int pk_draw(int *tickets, int x) {
-    return __hip_atomic_fetch_add(tickets + x * PK_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-__device__ __forceinline__ int pk_have(int first, int N, int x) {   /* items of queue x */
-    return N - first > x ? (N - first - x - 1) / PK_QUEUES + 1 : 0;
-}
-
-__device__ __forceinline__ int pk_next(int *tickets, int first, int N, int own, int got, int lane) {
-    int x = own;
-    got = uni(got);
-    for (;;) {
-        if (got < pk_have(first, N, x)) return first + x + got * PK_QUEUES;
-        /* lane i < 8: queue own + i */
-        const int y = (own + lane) % PK_QUEUES;
-        const int taken = lane < PK_QUEUES ? __hip_atomic_load(tickets + y * PK_LINE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-                                           : INT_MAX;
-        const unsigned long long left = __ballot(taken < pk_have(first, N, y));
-        if (!left) return INT_MAX;
-        x = (own + __ffsll(left) - 1) % PK_QUEUES;
-        got = 0;
-        if (lane == 0) got = pk_draw(tickets, x);
-        got = uni(got);
     }
 }
 
@@ -773,8 +859,7 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
     const int NW = uni(wide[B]), N = uni(NW + alone[B]), NN = uni(narrow[B]), G = gridDim.x, own = blockIdx.x % PK_QUEUES;
     const auto plan = [&](int b) { return pk_plan(p, uni(row0[b]), uni(count[b]), uni(length[b])); };
     for (int k = blockIdx.x; k < N;) {
-        int got = 0;
-        bool drawn = false;
+        int got = -1;   /* in thread 0: a ticket already drawn */
         PkItem it;
         if (k < NW) {
             it.b = uni(find_sequence(wide, B, k));
@@ -794,23 +879,9 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
             it.pg0 = max(it.q.pg0 + j * it.q.s, lo);
             it.pg1 = min(it.q.pg0 + (j + 1) * it.q.s, hi);
             if (it.pg0 < it.pg1) {
-                const int chunks = j1 - j0, unit = uni(units[it.b]) + tile * a.Hkv + it.kvh;
                 const long long slot0 = uni(wslots[it.b]) + ((long long)tile * a.Hkv + it.kvh) * it.q.nch;
-                pk_wide(p, it, chunks, slot0 + j - j0, stages, tab);
-                if (chunks > 1) {
-                    drawn = N > G;
-                    if (drawn && threadIdx.x == 0) got = pk_draw(p.tickets, own);
-                    __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* this wave's part of the partial is out */
-                    __syncthreads();
-                    if (threadIdx.x == 0)
-                        sh_next = __hip_atomic_fetch_add(p.arrived + unit, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    __syncthreads();
-                    if (uni(sh_next) == chunks - 1) {
-                        pk_merge<4, 4>(p, it, false, chunks, slot0, threadIdx.x, 256);
-                        if (threadIdx.x == 0)
-                            __hip_atomic_store(p.arrived + unit, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    }
-                }
+                got = pk_wide(p, it, j1 - j0, j - j0, slot0, p.arrived + uni(units[it.b]) + tile * a.Hkv + it.kvh, stages, tab,
+                              sh_next, N > G ? p.tickets + own * PK_LINE : nullptr);
             }
         } else {
             it.b = uni(find_sequence(alone, B, k - NW));
@@ -830,7 +901,7 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
         if (N <= G) break;
         __syncthreads();   /* sh_next, the stages and the table are used again */
         if (threadIdx.x < WAVE) {
-            if (!drawn && threadIdx.x == 0) got = pk_draw(p.tickets, own);
+            if (got < 0 && threadIdx.x == 0) got = pk_draw(p.tickets, own);
             sh_next = pk_next(p.tickets, G, N, own, got, threadIdx.x);
         }
         __syncthreads();
@@ -876,9 +947,9 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
             if (lane == 0) prior = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (uni(prior) == chunks - 1) {
                 if (it.tn * a.G <= 4)
-                    pk_merge<2, 16>(p, it, true, chunks, slot0, lane, WAVE);
+                    pk_merge<2, 16>(p, it, chunks, slot0, lane);
                 else
-                    pk_merge<4, 8>(p, it, true, chunks, slot0, lane, WAVE);
+                    pk_merge<4, 8>(p, it, chunks, slot0, lane);
                 if (lane == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
