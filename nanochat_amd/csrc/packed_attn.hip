@@ -17,7 +17,7 @@
  *           A sequence of at most PK_SHORT pages is not cut but shared by the four waves of a workgroup, which merge
  *           through LDS ("alone": it costs no round trips through memory, which is what a short one's time is made of)
  *   wide    a tile of up to 128 columns, 32 a wave: the four waves of a workgroup walk the same pairs, each fetched once
- *           (two stages of two pairs ahead)
+ *           (two stages of two pairs ahead); of at most 64 columns two waves take one pair of a stage and two the other
  *
  * A sequence's keys are cut into chunks (pk_plan), so that few rows over many keys still fill the chip; a (tile, KV head)
  * of several chunks leaves one partial (O, max, sum) in fp32 a chunk, and whoever finishes its last chunk merges them in
@@ -469,7 +469,7 @@ __device__ __forceinline__ void pk_fetch_wide(const AttnArgs &a, const int *tab,
 /* The merge of a tile's partials by the workgroup that finishes last, in chunk order, from its own state (chunk `own`) and
  * the others' in slots slot0 ..: a lane loads what it holds itself, eight dims a tile of its columns, a chunk at a time. */
 __device__ __forceinline__ void pk_join(const PackedArgs &p, const PkItem &it, int chunks, int own, long long slot0,
-                                        const WaveState<PK_NT> &ws, const int (&tok)[PK_NT], int wave, int c, int g) {
+                                        const WaveState<PK_NT> &ws, const int (&tok)[PK_NT], int wcol, int c, int g) {
     float m[PK_NT], l[PK_NT];
     f32x4 o[PK_NT][8];
 #pragma unroll
@@ -495,7 +495,7 @@ __device__ __forceinline__ void pk_join(const PackedArgs &p, const PkItem &it, i
             const Rsrc ro = page_rsrc(part.o, PK_WIDE_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_WIDE_COLS * 8);
 #pragma unroll
             for (int t = 0; t < PK_NT; t++) {
-                const int col = (wave * PK_NT + t) * 16 + c;
+                const int col = (wcol * PK_NT + t) * 16 + c;
                 const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(rm, col * 8, 0, SC1);
                 mj[t] = __uint_as_float(w[0]);
                 lj[t] = __uint_as_float(w[1]);
@@ -536,7 +536,10 @@ __device__ __forceinline__ int pk_wide(const PackedArgs &p, const PkItem &it, in
     const AttnArgs &a = p.a;
     const int lane = pk_lane(), wave = uni((int)threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int tpw = p.tpt * PK_NT, start = it.q.len - it.q.n;
-    const int wt0 = it.t0 + wave * tpw, end = it.t0 + it.tn, npages = it.pg1 - it.pg0;
+    /* at most two waves' columns: waves w and w + 2 share them, one the first pair of every stage, one the second */
+    const bool halves = it.tn <= 2 * tpw;
+    const int wcol = halves ? wave & 1 : wave;
+    const int wt0 = it.t0 + wcol * tpw, end = it.t0 + it.tn, npages = it.pg1 - it.pg0;
     const bool on = wt0 < end;
     const int last = min(wt0 + tpw, end) - 1;
     /* the wave's own pairs within the chunk's */
@@ -572,8 +575,9 @@ __device__ __forceinline__ int pk_wide(const PackedArgs &p, const PkItem &it, in
         pk_barrier();
         const int into = buf == 0 ? PK_WIDE_BUFS - 1 : buf - 1;   /* (s + PK_AHEAD) % PK_WIDE_BUFS */
         pk_fetch_wide(a, tab, npages, s + PK_AHEAD, it.kvh, stages + into * PK_WIDE_STAGE, wave, lane);
-        const int st = lds + buf * PK_WIDE_STAGE, until = min(2 * s + 2, s1);
-        for (int i = max(2 * s, s0); i < until; i++) {
+        const int st = lds + buf * PK_WIDE_STAGE;
+        const int from = max(2 * s + (halves ? wave >> 1 : 0), s0), until = min(2 * s + (halves ? (wave >> 1) + 1 : 2), s1);
+        for (int i = from; i < until; i++) {
             const int at = st + (i & 1) * PK_SCALE_AT, lpa = it.pg0 + 2 * i;
             pk_pair<PK_NT>(lpa, lpa + 1 < it.pg1, PkAt{at, st + 2 * PK_SCALE_AT + (2 * wave + (i & 1)) * PK_SCALE_BYTES}, qb, kb,
                            zero, ws, lane, [] {});
@@ -591,6 +595,36 @@ __device__ __forceinline__ int pk_wide(const PackedArgs &p, const PkItem &it, in
         ws.l[t] = pair_sum32(pair_sum16(ws.l[t]));
         tok[t] = pk_token(p, wt0, end, t, c);
     }
+    if (halves) {   /* waves 2 and 3 hand their states over: O [wave][column][O_PITCH] in the stages, (max, sum) in the table */
+        float *o2 = reinterpret_cast<float *>(stages) + wcol * 16 * PK_NT * O_PITCH;
+        float *ml2 = reinterpret_cast<float *>(tab) + wcol * 16 * PK_NT * 2;
+        if (wave >= 2)
+#pragma unroll
+            for (int t = 0; t < PK_NT; t++) {
+                const int col = t * 16 + c;
+                if (g == 0) {
+                    ml2[2 * col] = ws.bad ? NAN : ws.m[t];
+                    ml2[2 * col + 1] = ws.l[t];
+                }
+#pragma unroll
+                for (int d = 0; d < 8; d++) *reinterpret_cast<f32x4 *>(o2 + col * O_PITCH + 16 * d + 4 * g) = ws.o[t][d];
+                tok[t] = -1;
+            }
+        __syncthreads();
+        if (wave < 2)
+#pragma unroll
+            for (int t = 0; t < PK_NT; t++) {
+                const int col = t * 16 + c;
+                const float m2 = ml2[2 * col], mb = fmaxf(ws.m[t], m2);
+                const float f1 = ws.m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ws.m[t] - mb);
+                const float f2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - mb);   /* NaN: a bad page */
+                ws.l[t] = ws.l[t] * f1 + ml2[2 * col + 1] * f2;
+                ws.m[t] = mb;
+#pragma unroll
+                for (int d = 0; d < 8; d++)
+                    ws.o[t][d] = ws.o[t][d] * f1 + *reinterpret_cast<const f32x4 *>(o2 + col * O_PITCH + 16 * d + 4 * g) * f2;
+            }
+    }
     if (chunks == 1) {
 #pragma unroll
         for (int t = 0; t < PK_NT; t++)
@@ -602,7 +636,7 @@ __device__ __forceinline__ int pk_wide(const PackedArgs &p, const PkItem &it, in
         const Rsrc ro = page_rsrc(part.o, PK_WIDE_COLS * HEAD_DIM * 4), rm = page_rsrc(part.ml, PK_WIDE_COLS * 8);
 #pragma unroll
         for (int t = 0; t < PK_NT; t++)
-            if (tok[t] >= 0) pk_store_part<PK_NT>(ws, t, (wave * PK_NT + t) * 16 + c, g, ro, rm);
+            if (tok[t] >= 0) pk_store_part<PK_NT>(ws, t, (wcol * PK_NT + t) * 16 + c, g, ro, rm);
         if (queue && threadIdx.x == 0) got = pk_draw(queue, 0);
         __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* this wave's part of the partial is out; then everyone's */
         __syncthreads();
@@ -610,7 +644,7 @@ __device__ __forceinline__ int pk_wide(const PackedArgs &p, const PkItem &it, in
         __syncthreads();
         if (uni(shared) != chunks - 1) return got;
     }
-    pk_join(p, it, chunks, own, slot0, ws, tok, wave, c, g);
+    pk_join(p, it, chunks, own, slot0, ws, tok, wcol, c, g);
     if (threadIdx.x == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return got;
 }
