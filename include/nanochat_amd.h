@@ -305,6 +305,10 @@ int nc_pages_extend(const int32_t *new_tokens, int slots, int32_t *lengths, int3
 int nc_pages_trim(const int32_t *keep, int slots, int32_t *lengths, int32_t *table, int max_pages, int32_t *free_pages,
                   int32_t *free_count, int num_pages, int32_t *arrived, void *stream);
 
+/* Workspace bytes nc_sample_tokens needs for these sizes, at most 26 MB (0 for unsupported sizes): zero-filled before its
+ * first call, then passed to calls ordered on one stream, of any sizes that it suffices for. It serves no other function. */
+size_t nc_sample_workspace_bytes(long long rows, int vocab);
+
 /*
  * A token a row from its logits and one given uniform number: the token choice of a decoding step (reference
  * model/kernels/decode.cu:170-229, 361-411) for callers with logits of their own. logits: fp32, or bf16 (is_bf16), `rows`
@@ -321,7 +325,8 @@ int nc_pages_trim(const int32_t *keep, int slots, int32_t *lengths, int32_t *tab
  */
 int nc_sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
                      const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
-                     const float *min_p, const uint32_t *mask, long long mask_stride, int32_t *tokens, void *stream);
+                     const float *min_p, const uint32_t *mask, long long mask_stride, int32_t *tokens, void *workspace,
+                     size_t workspace_bytes, void *stream);
 
 /*
  * Measurement only; no counterpart in the reference. Reads n pages of 2 KiB (one (page, head) of K or V codes) from

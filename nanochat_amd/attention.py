@@ -110,7 +110,7 @@ _WORKSPACES: "OrderedDict[tuple, torch.Tensor]" = OrderedDict()
 _WORKSPACE_STREAMS = 8
 
 
-def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+def _workspace(device: torch.device, nbytes: int, kept: OrderedDict = _WORKSPACES) -> torch.Tensor:
     """A decode workspace of at least nbytes for this device and its current stream, kept for reuse. It starts
     zero-filled (its arrival counts must be zero before the first call; every call leaves them zero). Keyed by
     stream, so calls on two streams never share partials or counts. At most _WORKSPACE_STREAMS (device, stream)
@@ -120,12 +120,12 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     emptied (torch.cuda.empty_cache). A stream whose handle is reused after the stream is destroyed picks up the old
     entry, which is safe: its counts are zero whenever no call is in flight."""
     key = (device, torch.cuda.current_stream(device).cuda_stream)
-    ws = _WORKSPACES.pop(key, None)
+    ws = kept.pop(key, None)
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    _WORKSPACES[key] = ws
-    while len(_WORKSPACES) > _WORKSPACE_STREAMS:
-        _WORKSPACES.popitem(last=False)
+    kept[key] = ws
+    while len(kept) > _WORKSPACE_STREAMS:
+        kept.popitem(last=False)
     return ws
 
 

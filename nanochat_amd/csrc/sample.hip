@@ -477,17 +477,873 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(SampleArgs a) {
     if (t == 0) a.out[r] = token;
 }
 
+/* --- Rows of up to ST_MAX_GROUPS slices of 8,192 tokens, a workgroup each: the slice stays in its registers, 16 tokens a
+ * thread, and the workgroups of a row exchange what the next step needs through memory. */
+
+constexpr int ST_WAVES = 8, ST_THREADS = ST_WAVES * WAVE;
+constexpr int ST_E = 16, ST_SLICE = ST_E * ST_THREADS;
+constexpr int ST_STEP = 4 * ST_THREADS;   /* element 4 c + j of thread t: index slice + c ST_STEP + 4 t + j */
+constexpr int ST_MAX_GROUPS = 32;
+constexpr int ST_BINS = 2 * ST_THREADS;
+constexpr int ST_LIST = 256;              /* tokens a range may hold to be settled pairwise */
+constexpr int ST_TOP = 128;               /* the largest top-k settled by lists of candidates */
+constexpr int ST_CAND = 4096;             /* candidates: at most ST_TOP of 32 tokens, or of ST_MAX_GROUPS lists */
+constexpr int ST_LINE = 32;               /* ints of a 128-byte line: counts that several workgroups add to share none */
+constexpr int ST_QUEUES = 8;              /* XCDs */
+constexpr int ST_MAX_WORKGROUPS = 2048;   /* of one launch, when rows are cut: bounds the workspace */
+static_assert(ST_TOP * (ST_SLICE / 256) <= ST_CAND && ST_TOP * ST_MAX_GROUPS <= ST_CAND, "candidates fit");
+
+enum { HD_BEST, HD_LEAST, HD_COUNT, HD_ABOVE, HD_KEYS, HD_SUM, HD_TIES, HD_INDEX, HD_WORDS };
+constexpr int ST_PART = ST_BINS + 2 * ST_LIST + HD_WORDS;   /* words a workgroup publishes: histogram, list, head */
+
+struct SplitArgs {
+    SampleArgs a;
+    long long row0;
+    int rows, groups;      /* of this launch; slices a row */
+    u64 *part;             /* [rows][groups][ST_PART] */
+    int *tickets, *done, *count;   /* [ST_QUEUES], [ST_QUEUES], [rows] lines; zero between launches */
+};
+
+struct SplitShared {
+    union {
+        u64 weight[ST_E * ST_THREADS];   /* element e of thread t: [e ST_THREADS + t] */
+        struct {
+            u64 cand[ST_CAND];
+            u64 top[ST_TOP], top_w[ST_TOP], kept_w[ST_TOP];
+            u64 most[256];
+            int rank[ST_THREADS];
+        };
+    };
+    union {
+        u64 hist[ST_BINS];
+        struct {
+            u64 above[ST_LIST], equal[ST_LIST];
+        };
+    };
+    u64 code[ST_LIST], w[ST_LIST];
+    u64 sum[ST_E / 4 * ST_WAVES];
+    u64 kept[ST_MAX_GROUPS], head[ST_MAX_GROUPS];
+    int start[ST_MAX_GROUPS + 1];
+    u64 found, least_code;
+    uint32_t lo, hi, cut;
+    int bin, n, token, flag;
+};
+static_assert(2 * sizeof(SplitShared) <= 160 * 1024, "two workgroups a CU");
+
+/* A token as one integer: larger for the larger logit, and among equals for the lower index; 0: not allowed. */
+__device__ __forceinline__ u64 token_code(float z, int i) {
+    return z > -INFINITY ? (u64)order_key(z) << 32 | (0xFFFFFFFFu - (uint32_t)i) : 0ull;
+}
+__device__ __forceinline__ int code_index(u64 c) { return (int)(0xFFFFFFFFu - (uint32_t)c); }
+
+/* Words that other workgroups read: past this XCD's L2 (sc1), where another's stores are not seen. */
+__device__ __forceinline__ void publish(u64 *p, u64 v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ u64 peek(const u64 *p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+/* A value that is the same in every lane, as a scalar register's: branches on it are the wave's. */
+__device__ __forceinline__ int alike(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float alike(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
+
+/* Inclusive sums over the lanes by DPP: shifts by 1, 2, 4 and 8 within rows of 16 lanes, then a row's last sum added to the
+ * next row's, and the lower half's to the upper's. */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_add(u64 v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+    return v + ((u64)hi << 32 | lo);
+}
+__device__ __forceinline__ u64 lane_scan64(u64 v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    return dpp_add<0x143, 0xC>(v);
+}
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ u64 lane_sum64(u64 v) { return lane64(lane_scan64(v), WAVE - 1); }
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_max(float v) {
+    const int u = __float_as_int(v);
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(u, u, CTRL, ROWS, 0xF, false)));
+}
+__device__ __forceinline__ float lane_max(float v) {
+    v = dpp_max<0x111, 0xF>(v);
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v);
+    v = dpp_max<0x143, 0xC>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), WAVE - 1));
+}
+
+/* Room for this lane's `count` entries at the end of a list of n: one addition a wave. */
+__device__ __forceinline__ int reserve(int *n, int count, int lane) {
+    const int at = (int)lane_scan64((u64)count);
+    int first = 0;
+    if (lane == WAVE - 1) first = __hip_atomic_fetch_add(n, at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    return __builtin_amdgcn_readlane(first, WAVE - 1) + at - count;
+}
+
+struct Split {
+    const SplitArgs &s;
+    SplitShared &sh;
+    int t, lane, wave;
+    int row, g, G;         /* row of this launch, slice, slices */
+    int first;             /* index of this thread's element 0 */
+    int reached;           /* arrivals that the last wait of this row asked for */
+    u64 *mine;
+
+    __device__ __forceinline__ int index(int e) const { return first + (e >> 2) * ST_STEP + (e & 3); }
+    __device__ __forceinline__ u64 *part(int of) const { return s.part + ((long long)row * G + of) * ST_PART; }
+    __device__ __forceinline__ int *counter() const { return s.count + (long long)row * ST_LINE; }
+
+    /* Once every thread's stores are out: one arrival of this workgroup, its number among the row's. */
+    __device__ __forceinline__ void arrive() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+    /* Until every workgroup of the row has come as far: what they published is there. Workgroups take rows by tickets, so
+     * those of a row whose others have not started are the last G - 1 at most, and every earlier row's can end. */
+    __device__ __forceinline__ void meet() {
+        arrive();
+        if (G > 1) {
+            reached += G;
+            if (t == 0) {
+                __hip_atomic_fetch_add(counter(), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                while (__hip_atomic_load(counter(), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < reached)
+                    __builtin_amdgcn_s_sleep(1);
+            }
+            __syncthreads();
+        }
+    }
+    /* One word of every workgroup's head, into sh.head. The caller met before, and synchronizes after. */
+    __device__ __forceinline__ u64 head_of(int word) const { return peek(part(t) + ST_BINS + 2 * ST_LIST + word); }
+    __device__ __forceinline__ void tell(int word, u64 v) const { publish(mine + ST_BINS + 2 * ST_LIST + word, v); }
+
+    /* The last of a row's workgroups to leave clears its count, the last row's of a queue clears the queue. */
+    __device__ __forceinline__ void leave(bool counted) {
+        if (G == 1 || t != 0) return;
+        if (!counted) {
+            if (__hip_atomic_fetch_add(counter(), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != reached + G - 1) return;
+        }
+        __hip_atomic_store(counter(), 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int y = row % ST_QUEUES, rows = (s.rows - y + ST_QUEUES - 1) / ST_QUEUES;
+        if (__hip_atomic_fetch_add(s.done + y * ST_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == rows - 1) {
+            __hip_atomic_store(s.tickets + y * ST_LINE, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(s.done + y * ST_LINE, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+};
+
+/* Values that the compiler takes as new: what an earlier step made of them is not kept in registers for a later one. */
+template <typename V>
+__device__ __forceinline__ void anew(V (&v)[ST_E]) {
+#pragma unroll
+    for (int e = 0; e < ST_E; e++) asm volatile("" : "+v"(v[e]));
+}
+
+/* This thread's 16 tokens; those not allowed and those past the row's end are -inf. */
+__device__ __forceinline__ void split_load(const Split &q, const SampleArgs &a, long long r, float (&x)[ST_E]) {
+    const char *p = (const char *)a.logits + r * a.stride * (a.bf16 ? 2 : 4);
+    uint32_t allowed = 0xFFFFu;
+    if (a.mask) {
+        allowed = 0;
+        const uint32_t *mask = a.mask + r * a.mask_stride;
+        const int words = (a.vocab + 31) >> 5;
+#pragma unroll
+        for (int c = 0; c < ST_E / 4; c++) {
+            const int i = q.first + c * ST_STEP;
+            allowed |= (mask[min(i >> 5, words - 1)] >> (i & 31) & 0xFu) << (4 * c);
+        }
+    }
+    if (a.wide && (q.g + 1) * ST_SLICE <= a.vocab) {
+        if (a.bf16) {
+            uint2 u[ST_E / 4];
+#pragma unroll
+            for (int c = 0; c < ST_E / 4; c++) u[c] = *reinterpret_cast<const uint2 *>(p + 2LL * (q.first + c * ST_STEP));
+#pragma unroll
+            for (int c = 0; c < ST_E / 4; c++) {
+                x[4 * c] = __uint_as_float(u[c].x << 16); x[4 * c + 1] = __uint_as_float(u[c].x & 0xFFFF0000u);
+                x[4 * c + 2] = __uint_as_float(u[c].y << 16); x[4 * c + 3] = __uint_as_float(u[c].y & 0xFFFF0000u);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < ST_E / 4; c++) {
+                const float4 u = *reinterpret_cast<const float4 *>(p + 4LL * (q.first + c * ST_STEP));
+                x[4 * c] = u.x; x[4 * c + 1] = u.y; x[4 * c + 2] = u.z; x[4 * c + 3] = u.w;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < ST_E; e++) {   /* past the end: the last token's, dropped below */
+            const int i = min(q.index(e), a.vocab - 1);
+            x[e] = a.bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i]) : reinterpret_cast<const float *>(p)[i];
+        }
+#pragma unroll
+        for (int e = 0; e < ST_E; e++) allowed &= ~((uint32_t)(q.index(e) >= a.vocab) << e);
+    }
+#pragma unroll
+    for (int e = 0; e < ST_E; e++)   /* NaN fails the comparison; -0 becomes +0, its equal */
+        x[e] = (allowed >> e & 1) && x[e] > -INFINITY ? x[e] + 0.0f : -INFINITY;
+}
+
+/* The `want` largest of the n codes of sh.cand, in order, in sh.top; returns how many. Every thread must call it, after a
+ * __syncthreads. */
+__device__ __forceinline__ int split_sort(SplitShared &sh, int n, int want) {
+    const int t = threadIdx.x;
+    if (n <= ST_THREADS) {   /* a code's comparisons spread over 512 / n threads */
+        int lanes = 1;
+        while (lanes < n) lanes <<= 1;
+        sh.rank[t] = 0;
+        __syncthreads();
+        const int i = t & (lanes - 1);
+        if (i < n) {
+            const u64 c = sh.cand[i];
+            int above = 0;
+#pragma unroll 4
+            for (int j = t / lanes; j < n; j += ST_THREADS / lanes) above += sh.cand[j] > c;
+            __hip_atomic_fetch_add(&sh.rank[i], above, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        __syncthreads();
+        if (t < n && sh.rank[t] < want) sh.top[sh.rank[t]] = sh.cand[t];
+    } else {
+        for (int i = t; i < n; i += ST_THREADS) {
+            const u64 c = sh.cand[i];
+            int above = 0;
+            for (int j = 0; j < n && above < want; j++) above += sh.cand[j] > c;
+            if (above < want) sh.top[above] = c;
+        }
+    }
+    __syncthreads();
+    return min(n, want);
+}
+
+/* Adds `v` to the candidates if `take`. */
+__device__ __forceinline__ void split_collect(SplitShared &sh, u64 v, bool take) {
+    if (take) sh.cand[__hip_atomic_fetch_add(&sh.n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)] = v;
+}
+
+/* The k <= ST_TOP largest of this slice, in order, in sh.top; returns how many. A code that k of the maxima of 256 groups of
+ * 32 tokens reach is a lower bound of the k-th largest: only the tokens that reach it (in random order about 51 for k = 50,
+ * 177 for 128) are compared pairwise. */
+__device__ __forceinline__ int split_top(const Split &q, float (&x)[ST_E], int k) {
+    SplitShared &sh = q.sh;
+    const int t = q.t;
+    u64 best = 0;
+#pragma unroll
+    for (int e = 0; e < ST_E; e++) best = max(best, token_code(x[e], q.index(e)));
+    best = max(best, (u64)__shfl_xor(best, 1, WAVE));
+    if (k == 1) {
+#pragma unroll
+        for (int o = 2; o < WAVE; o <<= 1) best = max(best, (u64)__shfl_xor(best, o, WAVE));
+        if (q.lane == 0) sh.sum[q.wave] = best;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < ST_WAVES; w++) best = max(best, sh.sum[w]);
+        if (t == 0) sh.top[0] = best;
+        __syncthreads();
+        return best != 0;
+    }
+    if (t == 0) sh.n = 0;
+    if ((t & 1) == 0) sh.most[t >> 1] = best;
+    __syncthreads();
+    if (q.wave == 0) {   /* by bisection, to k to k + 8 of the maxima, but at most ST_TOP */
+        u64 m[4], hi = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            m[j] = sh.most[j * WAVE + q.lane];
+            hi = max(hi, m[j]);
+        }
+        const auto reach = [&](u64 code) {
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) n += __popcll(__ballot(m[j] >= code));
+            return n;
+        };
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) hi = max(hi, (u64)__shfl_xor(hi, o, WAVE));
+        hi = lane64(hi, 0);
+        const int most = min(k + 8, ST_TOP);
+        u64 lo = 1;
+        for (int n = reach(lo); n > most && lo < hi;) {
+            const u64 mid = lo + (hi - lo + 1) / 2;
+            const int of = reach(mid);
+            if (of >= k) {
+                lo = mid;
+                n = of;
+            } else {
+                hi = mid - 1;
+            }
+        }
+        if (q.lane == 0) sh.least_code = lo;
+    }
+    __syncthreads();
+    const u64 least = sh.least_code;
+    anew(x);
+    int count = 0;
+#pragma unroll
+    for (int e = 0; e < ST_E; e++) count += token_code(x[e], q.index(e)) >= least;
+    int at = reserve(&sh.n, count, q.lane);
+    if (count) {
+#pragma unroll
+        for (int e = 0; e < ST_E; e++) {
+            const u64 c = token_code(x[e], q.index(e));
+            if (c >= least) sh.cand[at++] = c;
+        }
+    }
+    __syncthreads();
+    return split_sort(sh, alike(sh.n), k);
+}
+
+/* The smallest of this slice's tokens, in index order, whose running sum of m(e), over the elements of the set `in`, reaches
+ * `goal`, which its total does. Every thread must call it. */
+template <typename M>
+__device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 goal) {
+    SplitShared &sh = q.sh;
+    u64 own[ST_E / 4], scan[ST_E / 4];
+#pragma unroll
+    for (int c = 0; c < ST_E / 4; c++) {
+        own[c] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) own[c] += in >> (4 * c + j) & 1 ? m(4 * c + j) : 0;
+        scan[c] = lane_scan64(own[c]);
+        if (q.lane == WAVE - 1) sh.sum[c * ST_WAVES + q.wave] = scan[c];
+    }
+    __syncthreads();
+    const u64 part = q.lane < ST_E / 4 * ST_WAVES ? sh.sum[q.lane] : 0, upto = lane_scan64(part) - part;
+#pragma unroll
+    for (int c = 0; c < ST_E / 4; c++) {
+        u64 before = lane64(upto, c * ST_WAVES + q.wave) + scan[c] - own[c];
+        if (before < goal && goal <= before + own[c]) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const u64 v = in >> (4 * c + j) & 1 ? m(4 * c + j) : 0;
+                if (before < goal && goal <= before + v) sh.token = q.index(4 * c + j);
+                before += v;
+            }
+        }
+    }
+    __syncthreads();
+    return sh.token;
+}
+
+/* find_cut over the slices of a row: where the running sum of m(e), over the elements of the sets `live`, the larger value
+ * first, reaches target(total). Ranges of values are narrowed by histograms, which the workgroups publish and each adds up,
+ * until the tokens of the one that holds the cut fit a list, which each settles pairwise. sh.kept: per slice the weight of
+ * the tokens down to the cut that weigh least_w or more (not SPLIT). Every thread of every workgroup of the row calls it. */
+template <bool SPLIT, typename Target>
+__device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t live, float zmax, float range, u64 least_w,
+                                         Target target) {
+    SplitShared &sh = q.sh;
+    const int lane = q.lane, wave = q.wave, G = q.G;
+    int t = q.t;
+    u64 *base_part = q.part(0);
+    const auto m = [&](int e) { return SPLIT ? 1ull : sh.weight[e * ST_THREADS + t]; };
+    const float scale = range > 0.0f && range < INFINITY ? (ST_BINS - 1) / range : 0.0f;
+    /* a range whose products are NaN or past the last bin: the last bin; monotone in z in every case */
+    const auto bin_of = [&](float z) { return z == zmax ? 0 : (int)fminf((zmax - z) * scale, (float)(ST_BINS - 1)); };
+    u64 goal = 0, base = 0;
+    uint32_t lo = 0u, hi = 0xFFFFFFFFu;   /* once a range of values is split again: its keys */
+    int keyed = 0;
+    u64 base_above = 0;
+    for (;;) {
+        /* one body for the first level and the others, and no address or set kept in registers from one to the next */
+        asm volatile("" : "+s"(keyed), "+s"(lo), "+s"(hi), "+s"(base_part), "+v"(t), "+v"(q.first), "+v"(live));
+        const auto part = [&](int o) { return base_part + (long long)o * ST_PART; };
+        const auto listed = [&](u64 code) {   /* what a token of this slice counts */
+            const int i = code_index(code) - q.g * ST_SLICE;
+            return SPLIT ? 1ull : sh.weight[(i / ST_STEP * 4 + i % 4) * ST_THREADS + i % ST_STEP / 4];
+        };
+        const auto head_of = [&](int word) { return peek(part(lane) + ST_BINS + 2 * ST_LIST + word); };
+        const auto tell = [&](int word, u64 v) { publish(part(q.g) + ST_BINS + 2 * ST_LIST + word, v); };
+        int shift = 0;
+        if (keyed)
+            while ((hi - lo) >> shift >= ST_BINS) shift++;
+        anew(x);
+        __syncthreads();
+        sh.hist[t] = sh.hist[t + ST_THREADS] = 0;
+        if (t == 0) {
+            sh.n = 0;
+            sh.lo = 0xFFFFFFFFu;
+            sh.hi = 0u;
+        }
+        __syncthreads();
+        uint32_t bins[ST_E / 2];   /* two elements' a register; ST_BINS: not live */
+#pragma unroll
+        for (int e = 0; e < ST_E; e++) {
+            int b = keyed ? (int)((hi - order_key(x[e])) >> shift) : bin_of(x[e]);
+            b = live >> e & 1 ? b : ST_BINS;
+            bins[e / 2] = e & 1 ? bins[e / 2] | (uint32_t)b << 16 : (uint32_t)b;
+            if (b < ST_BINS)
+                __hip_atomic_fetch_add(&sh.hist[b], m(e), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (e & 1) asm volatile("" : "+v"(bins[e / 2]));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+        u64 v[2] = {sh.hist[2 * t], sh.hist[2 * t + 1]};
+        if (G > 1) {
+            publish(part(q.g) + 2 * t, v[0]);
+            publish(part(q.g) + 2 * t + 1, v[1]);
+            q.meet();
+            v[0] = v[1] = 0;
+            for (int o = 0; o < G; o++) {
+                v[0] += peek(part(o) + 2 * t);
+                v[1] += peek(part(o) + 2 * t + 1);
+            }
+        }
+        const u64 scan = lane_scan64(v[0] + v[1]);
+        if (lane == WAVE - 1) sh.sum[wave] = scan;
+        __syncthreads();
+        u64 before = scan - v[0] - v[1], total = 0;
+#pragma unroll
+        for (int o = 0; o < ST_WAVES; o++) {
+            before += o < wave ? sh.sum[o] : 0;
+            total += sh.sum[o];
+        }
+        if (!keyed) {
+            goal = target(total);
+            if (alike(goal > total)) return Cut{false, 0u, 0};
+        }
+        const u64 rest = goal - base;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            if (before < rest && rest <= before + v[k]) {
+                sh.bin = 2 * t + k;
+                sh.found = before;
+            }
+            before += v[k];
+        }
+        __syncthreads();
+        const int bin = alike(sh.bin);
+        base += sh.found;
+
+        anew(x);
+        asm volatile("" : "+v"(t), "+v"(live), "+v"(q.first));
+        u64 above = 0;
+        uint32_t least = 0xFFFFFFFFu, most = 0u;
+        const auto slot = [&](int e) { return (int)(bins[e / 2] >> (e & 1) * 16 & 0xFFFFu); };
+        live = 0;
+#pragma unroll
+        for (int e = 0; e < ST_E; e++) {
+            const int b = slot(e);
+            live |= (uint32_t)(b == bin) << e;
+            if (!SPLIT) {   /* on top of the levels' before */
+                const u64 v = m(e);
+                base_above += b < bin && v >= least_w ? v : 0;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("" : "+v"(base_above));
+        above = base_above;
+        const int count = __popc(live);
+        int at = reserve(&sh.n, count, lane);
+        if (count) {
+#pragma unroll
+            for (int e = 0; e < ST_E; e++) {
+                if (live >> e & 1) {
+                    const uint32_t k = order_key(x[e]);
+                    if (at < ST_LIST) sh.code[at] = token_code(x[e], q.index(e));
+                    at++;
+                    least = min(least, k);
+                    most = max(most, k);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        asm volatile("" : "+v"(live));
+        if (most) {
+            __hip_atomic_fetch_min(&sh.lo, least, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            __hip_atomic_fetch_max(&sh.hi, most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        if (!SPLIT) {
+            above = lane_sum64(above);
+            if (lane == 0) sh.sum[wave] = above;
+        }
+        __syncthreads();
+        int n = alike(sh.n);
+        if (!SPLIT) {
+            above = 0;
+#pragma unroll
+            for (int v = 0; v < ST_WAVES; v++) above += sh.sum[v];
+        }
+        if (G > 1) {
+            if (t < min(n, ST_LIST)) {
+                publish(part(q.g) + ST_BINS + t, sh.code[t]);
+                publish(part(q.g) + ST_BINS + ST_LIST + t, listed(sh.code[t]));
+            }
+            if (t == 0) {
+                tell(HD_COUNT, (u64)n);
+                tell(HD_ABOVE, above);
+                tell(HD_KEYS, (u64)sh.lo << 32 | sh.hi);
+            }
+            q.meet();
+            if (wave == 0) {
+                int count = 0;
+                uint32_t l = 0xFFFFFFFFu, h = 0u;
+                if (lane < G) {
+                    count = (int)head_of(HD_COUNT);
+                    const u64 keys = head_of(HD_KEYS);
+                    l = (uint32_t)(keys >> 32);
+                    h = (uint32_t)keys;
+                    sh.kept[lane] = head_of(HD_ABOVE);
+                    sh.head[lane] = (u64)count;
+                }
+                int end = count;
+#pragma unroll
+                for (int o = 1; o < WAVE; o <<= 1) {
+                    const int up = __shfl_up(end, o, WAVE);
+                    if (lane >= o) end += up;
+                    l = min(l, (uint32_t)__shfl_xor(l, o, WAVE));
+                    h = max(h, (uint32_t)__shfl_xor(h, o, WAVE));
+                }
+                if (lane < G) sh.start[lane + 1] = end;
+                if (lane == 0) {
+                    sh.start[0] = 0;
+                    sh.lo = l;
+                    sh.hi = h;
+                }
+            }
+            __syncthreads();
+            n = alike(sh.start[G]);
+            if (n <= ST_LIST) {
+                for (int o = wave; o < G; o += ST_WAVES)
+                    for (int i = lane; i < sh.start[o + 1] - sh.start[o]; i += WAVE) {
+                        sh.code[sh.start[o] + i] = peek(part(o) + ST_BINS + i);
+                        sh.w[sh.start[o] + i] = peek(part(o) + ST_BINS + ST_LIST + i);
+                    }
+            }
+        } else {
+            if (t < min(n, ST_LIST)) sh.w[t] = listed(sh.code[t]);
+            if (t == 0) {
+                sh.kept[0] = above;
+                sh.head[0] = (u64)n;
+            }
+        }
+        if (t < ST_LIST) sh.above[t] = sh.equal[t] = 0;
+        __syncthreads();
+        lo = (uint32_t)alike((int)sh.lo);
+        hi = (uint32_t)alike((int)sh.hi);
+        keyed = 1;
+        if (n <= ST_LIST) {
+            int lanes = 1;
+            while (lanes < n) lanes <<= 1;
+            const int i = t & (lanes - 1);
+            if (i < n) {
+                const u64 c = sh.code[i];
+                u64 more = 0, same = 0;
+#pragma unroll 4
+                for (int j = t / lanes; j < n; j += ST_THREADS / lanes) {
+                    const u64 cj = sh.code[j], wj = sh.w[j];
+                    more += (SPLIT ? cj > c : cj >> 32 > c >> 32) ? wj : 0;
+                    same += !SPLIT && cj >> 32 == c >> 32 ? wj : 0;
+                }
+                __hip_atomic_fetch_add(&sh.above[i], more, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (!SPLIT) __hip_atomic_fetch_add(&sh.equal[i], same, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+            __syncthreads();
+            if (t < n) {
+                const u64 more = base + sh.above[t], own = SPLIT ? sh.w[t] : sh.equal[t];
+                if (more < goal && goal <= more + own) {   /* one token, or one value's equals, who write the same */
+                    sh.cut = (uint32_t)(sh.code[t] >> 32);
+                    sh.token = SPLIT ? code_index(sh.code[t]) : 0x7FFFFFFF;
+                }
+                if (!SPLIT && more < goal && sh.w[t] >= least_w)
+                    __hip_atomic_fetch_add(&sh.kept[code_index(sh.code[t]) / ST_SLICE], sh.w[t], __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+            __syncthreads();
+            return Cut{true, sh.cut, sh.token};
+        }
+        if (lo == hi) {   /* one value */
+            if (!SPLIT) {
+                if (t < G && sh.head[t]) {
+                    const u64 of = G > 1 ? peek(part(t) + ST_BINS + ST_LIST) : sh.w[0];   /* every one's weight */
+                    if (of >= least_w) sh.kept[t] += sh.head[t] * of;
+                }
+                __syncthreads();
+                return Cut{true, lo, 0x7FFFFFFF};
+            }
+            u64 before_us = 0;
+            for (int o = 0; o < q.g; o++) before_us += sh.head[o];
+            const u64 rest1 = goal - base, ours = sh.head[q.g];
+            int idx = 0;
+            const bool holds = before_us < rest1 && rest1 <= before_us + ours;
+            if (alike(holds)) idx = split_pick(q, live, m, rest1 - before_us);
+            if (G > 1) {
+                if (t == 0) tell(HD_INDEX, holds ? (u64)idx + 1 : 0ull);
+                q.meet();
+                if (t < G) {
+                    const u64 of = head_of(HD_INDEX);
+                    if (of) sh.token = (int)of - 1;
+                }
+                __syncthreads();
+                idx = sh.token;
+            }
+            return Cut{true, lo, idx};
+        }
+    }
+}
+
+__global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
+    __shared__ SplitShared sh;
+    const SampleArgs &a = s.a;
+    Split q = {s, sh};
+    q.t = threadIdx.x;
+    q.lane = q.t & (WAVE - 1);
+    q.wave = q.t >> 6;
+    q.G = s.groups;
+    q.row = blockIdx.x;
+    q.g = 0;
+    if (q.G > 1) {   /* every eighth workgroup, which one XCD runs, draws on one queue, and a row is one queue's */
+        const int y = blockIdx.x % ST_QUEUES, rows = (s.rows - y + ST_QUEUES - 1) / ST_QUEUES;
+        if ((int)(blockIdx.x / ST_QUEUES) >= rows * q.G) return;
+        if (q.t == 0)
+            sh.n = __hip_atomic_fetch_add(s.tickets + y * ST_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        const int ticket = alike(sh.n);
+        q.row = y + ticket / q.G * ST_QUEUES;
+        q.g = ticket % q.G;
+    }
+    q.first = q.g * ST_SLICE + 4 * q.t;
+    q.reached = 0;
+    q.mine = q.part(q.g);
+    const int t = q.t, lane = q.lane, wave = q.wave, G = q.G;
+    const long long r = s.row0 + q.row;
+    float x[ST_E];
+    split_load(q, a, r, x);
+    const float T = alike(a.temperature[r]), u = alike(a.uniform[r]), p = a.top_p ? alike(a.top_p[r]) : 1.0f;
+    const bool greedy = !(T > 0.0f);
+    const int k = greedy ? 1 : a.top_k ? alike(a.top_k[r]) : 0;
+    const double floor_w = a.min_p ? fmin(fmax((double)alike(a.min_p[r]), 0.0), 1.0) : 0.0;   /* NaN: 0 */
+    const double per_log2 = 1.4426950408889634 / (double)T;
+    int S = 62;   /* the row's weights sum below 2^62 */
+    while (S > 0 && (1LL << (62 - S)) < a.vocab) S--;
+    S = min(S, 46);
+    const u64 least_w = (u64)ceil(__builtin_ldexp(floor_w, S));
+    const auto mass_goal = [&](u64 total) { return max((u64)ceil(fmax((double)p, 0.0) * (double)total), 1ull); };
+    const auto choice = [&](u64 total) {   /* the first running sum above u total */
+        const u64 at = u > 0.0f ? (u < 1.0f ? (u64)((double)u * (double)total) : total) : 0ull;
+        return min(at, total - 1) + 1;
+    };
+    float zmax = 0.0f;
+    const auto weight = [&](float z) {
+        return z == zmax ? 1ull << S : z == -INFINITY ? 0ull : fixed_exp2(((double)z - (double)zmax) * per_log2, S);
+    };
+
+    if (k > 0 && k <= ST_TOP) {
+        __syncthreads();   /* sh.n held the ticket */
+        int n = alike(split_top(q, x, k));
+        if (G > 1) {
+            if (t < n) publish(q.mine + ST_BINS + t, sh.top[t]);
+            if (t == 0) q.tell(HD_COUNT, (u64)n);
+            q.arrive();
+            if (t == 0) {
+                sh.flag = __hip_atomic_fetch_add(q.counter(), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == G - 1;
+                sh.n = 0;
+            }
+            __syncthreads();
+            if (!alike(sh.flag)) return;
+            /* every list's ceil(k / G)-th: k tokens reach the least of them */
+            const int quota = (k + G - 1) / G;
+            if (wave == 0) {
+                u64 least = ~0ull;
+                if (lane < G) {
+                    const int count = (int)q.head_of(HD_COUNT);
+                    sh.head[lane] = (u64)count;
+                    least = count >= quota ? peek(q.part(lane) + ST_BINS + quota - 1) : 1ull;
+                }
+#pragma unroll
+                for (int o = 1; o < WAVE; o <<= 1) least = min(least, (u64)__shfl_xor(least, o, WAVE));
+                if (lane == 0) sh.least_code = least;
+            }
+            __syncthreads();
+            const u64 least = sh.least_code;
+            for (int o = wave; o < G; o += ST_WAVES)
+                for (int i = lane; i < (int)sh.head[o]; i += WAVE) {
+                    const u64 c = peek(q.part(o) + ST_BINS + i);
+                    split_collect(sh, c, c >= least);
+                }
+            __syncthreads();
+            n = alike(split_sort(sh, alike(sh.n), k));
+            q.leave(true);
+        }
+        if (n == 0 || k == 1) {
+            if (t == 0) a.out[r] = n == 0 ? -1 : code_index(sh.top[0]);
+            return;
+        }
+        zmax = key_value((uint32_t)(sh.top[0] >> 32));
+        if (t < n) sh.top_w[t] = weight(key_value((uint32_t)(sh.top[t] >> 32)));
+        __syncthreads();
+        if (t < n) {
+            const u64 c = sh.top[t];
+            u64 more = 0, total = 0;
+            for (int j = 0; j < n; j++) {
+                const u64 w = sh.top_w[j];
+                more += sh.top[j] >> 32 > c >> 32 ? w : 0;
+                total += w;
+            }
+            const u64 w = sh.top_w[t];
+            sh.kept_w[t] = w >= least_w && (!(p < 1.0f) || more < mass_goal(total)) ? w : 0;
+        }
+        __syncthreads();
+        if (t < n) {
+            const int idx = code_index(sh.top[t]);
+            u64 before = 0, total = 0;
+            for (int j = 0; j < n; j++) {
+                const u64 w = sh.kept_w[j];
+                before += code_index(sh.top[j]) < idx ? w : 0;
+                total += w;
+            }
+            const u64 goal = choice(total);
+            if (before < goal && goal <= before + sh.kept_w[t]) a.out[r] = idx;
+        }
+        return;
+    }
+
+    /* the largest allowed logit and the smallest */
+    float most = -INFINITY, least = INFINITY;
+#pragma unroll
+    for (int e = 0; e < ST_E; e++) {
+        most = fmaxf(most, x[e]);
+        least = fminf(least, x[e] > -INFINITY ? x[e] : INFINITY);
+    }
+    for (int round = 0; round < (G > 1 ? 2 : 1); round++) {
+        if (round) {
+            if (t == 0) q.tell(HD_BEST, (u64)__float_as_uint(most) << 32 | __float_as_uint(least));
+            q.meet();
+            if (t < G) {
+                const u64 of = q.head_of(HD_BEST);
+                most = __uint_as_float((uint32_t)(of >> 32));
+                least = __uint_as_float((uint32_t)of);
+            }
+        }
+        most = lane_max(most);
+        least = -lane_max(-least);
+        if (lane == 0) sh.sum[wave] = (u64)__float_as_uint(most) << 32 | __float_as_uint(least);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < ST_WAVES; w++) {
+            most = fmaxf(most, __uint_as_float((uint32_t)(sh.sum[w] >> 32)));
+            least = fminf(least, __uint_as_float((uint32_t)sh.sum[w]));
+        }
+        __syncthreads();
+    }
+    most = alike(most);
+    least = alike(least);
+    if (most == -INFINITY) {
+        if (t == 0 && q.g == 0) a.out[r] = -1;
+        q.leave(false);
+        return;
+    }
+    zmax = most;
+    anew(x);
+
+    if (k > 0 && k < a.vocab) {
+        uint32_t live = 0;
+#pragma unroll
+        for (int e = 0; e < ST_E; e++) live |= (uint32_t)(x[e] > -INFINITY) << e;
+        const Cut top = split_cut<true>(q, x, live, zmax, zmax - least, 0ull,
+                                        [&](u64) { return (u64)k; });
+        if (top.some) {
+            const float z = key_value(top.key);
+#pragma unroll
+            for (int e = 0; e < ST_E; e++)   /* past the k largest: dropped */
+                if (!(x[e] > z || (x[e] == z && q.index(e) <= top.idx))) x[e] = -INFINITY;
+        }
+    }
+    anew(x);
+    uint32_t live = 0;
+#pragma unroll
+    for (int e = 0; e < ST_E; e++) {
+        const u64 v = weight(x[e]);
+        sh.weight[e * ST_THREADS + t] = v;   /* read by this thread alone */
+        live |= (uint32_t)(v != 0) << e;
+        if (e & 1) __builtin_amdgcn_sched_barrier(0);   /* two at a time: more would need more registers */
+    }
+    float least_z = -INFINITY;   /* the nucleus' smallest logit */
+    if (p < 1.0f) {
+        /* values 47 log2 units below the largest weigh nothing */
+        const Cut mass = split_cut<false>(q, x, live, zmax,
+                                          fminf(zmax - least, 33.0f * T), least_w, mass_goal);
+        if (mass.some) least_z = key_value(mass.key);
+    } else {
+        u64 own = 0;
+#pragma unroll
+        for (int e = 0; e < ST_E; e++) {
+            const u64 v = sh.weight[e * ST_THREADS + t];
+            own += v >= least_w ? v : 0;
+        }
+        own = lane_sum64(own);
+        if (lane == 0) sh.sum[wave] = own;
+        __syncthreads();
+        if (t == 0) {
+            own = 0;
+#pragma unroll
+            for (int v = 0; v < ST_WAVES; v++) own += sh.sum[v];
+            if (G > 1) q.tell(HD_SUM, own);
+            else sh.kept[0] = own;
+        }
+        q.meet();
+        if (G > 1) {
+            if (t < G) sh.kept[t] = q.head_of(HD_SUM);
+            __syncthreads();
+        }
+    }
+    u64 total = 0, before = 0;
+    for (int o = 0; o < G; o++) {
+        before += o < q.g ? sh.kept[o] : 0;
+        total += sh.kept[o];
+    }
+    const u64 goal = choice(total), ours = sh.kept[q.g];
+    __syncthreads();
+    if (alike(before < goal && goal <= before + ours)) {
+        uint32_t kept = 0;
+#pragma unroll
+        for (int e = 0; e < ST_E; e++) kept |= (uint32_t)(x[e] >= least_z && sh.weight[e * ST_THREADS + t] >= least_w) << e;
+        const int token = split_pick(q, kept, [&](int e) { return sh.weight[e * ST_THREADS + t]; }, goal - before);
+        if (t == 0) a.out[r] = token;
+    }
+    q.leave(false);
+}
+
 }  // namespace nc
 
 using namespace nc;
 
+static int split_groups(int vocab) { return (vocab + ST_SLICE - 1) / ST_SLICE; }
+
+/* Rows of a launch that cuts rows into `groups` slices. */
+static long long split_rows(long long rows, int groups) {
+    return rows < ST_MAX_WORKGROUPS / groups ? rows : ST_MAX_WORKGROUPS / groups;
+}
+
+/* The counts come first, in the same place whatever the sizes, so that every call finds them as the one before left them. */
+constexpr size_t ST_COUNT_BYTES = (2 * ST_QUEUES + ST_MAX_WORKGROUPS / 2) * ST_LINE * sizeof(int);
+
+extern "C" size_t nc_sample_workspace_bytes(long long rows, int vocab) {
+    if (rows < 0 || rows > 1LL << 22 || vocab <= 0 || vocab > 1 << 24) return 0;
+    const int groups = split_groups(vocab);
+    if (groups == 1 || groups > ST_MAX_GROUPS || rows == 0) return 16;
+    return ST_COUNT_BYTES + (size_t)split_rows(rows, groups) * groups * ST_PART * sizeof(u64);
+}
+
 extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
                                 const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
                                 const float *min_p, const uint32_t *mask, long long mask_stride, int32_t *tokens,
-                                void *stream) {
-    if (!logits || !uniform || !temperature || !tokens) return NC_ERR_NULL;
+                                void *workspace, size_t workspace_bytes, void *stream) {
+    if (!logits || !uniform || !temperature || !tokens || !workspace) return NC_ERR_NULL;
     if (rows < 0 || rows > 1LL << 22 || vocab <= 0 || vocab > 1 << 24 || row_stride < vocab ||
-        (mask && mask_stride < ((long long)vocab + 31) / 32))
+        (mask && mask_stride < ((long long)vocab + 31) / 32) || (uintptr_t)workspace % 16 ||
+        workspace_bytes < nc_sample_workspace_bytes(rows, vocab))
         return NC_ERR_SHAPE;
     if (rows == 0) return NC_OK;
     SampleArgs a = {};
@@ -496,6 +1352,25 @@ extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_s
     a.uniform = uniform; a.temperature = temperature; a.top_p = top_p; a.min_p = min_p; a.top_k = top_k;
     a.mask = mask; a.mask_stride = mask_stride;
     a.out = tokens;
-    hipLaunchKernelGGL(sample_kernel, dim3((unsigned)rows), dim3(SM_THREADS), 0, (hipStream_t)stream, a);
-    return (int)hipGetLastError();
+    const int groups = split_groups(vocab);
+    if (groups > ST_MAX_GROUPS) {
+        hipLaunchKernelGGL(sample_kernel, dim3((unsigned)rows), dim3(SM_THREADS), 0, (hipStream_t)stream, a);
+        return (int)hipGetLastError();
+    }
+    SplitArgs s = {};
+    s.a = a;
+    s.groups = groups;
+    const long long most = groups == 1 ? rows : split_rows(rows, groups);
+    s.tickets = (int *)workspace;
+    s.done = s.tickets + ST_QUEUES * ST_LINE;
+    s.count = s.done + ST_QUEUES * ST_LINE;
+    s.part = (u64 *)((char *)workspace + ST_COUNT_BYTES);
+    for (s.row0 = 0; s.row0 < rows; s.row0 += most) {
+        s.rows = (int)(rows - s.row0 < most ? rows - s.row0 : most);
+        const int grid = groups == 1 ? s.rows : (s.rows + ST_QUEUES - 1) / ST_QUEUES * ST_QUEUES * groups;
+        hipLaunchKernelGGL(split_kernel, dim3((unsigned)grid), dim3(ST_THREADS), 0, (hipStream_t)stream, s);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return (int)e;
+    }
+    return NC_OK;
 }

@@ -121,8 +121,9 @@ SIGNATURES = {
                                c_int),
     "nc_qk_norm_rope_append_rows_fp8": ([c_void_p, c_longlong, c_longlong, c_int, c_int] + [c_void_p] * 6 +
                                         [c_int] + [c_void_p] * 4 + [c_int, c_void_p], c_int),
+    "nc_sample_workspace_bytes": ([c_longlong, c_int], c_size_t),
     "nc_sample_tokens": ([c_void_p, c_int, c_longlong, c_longlong, c_int] + [c_void_p] * 6 +
-                         [c_longlong, c_void_p, c_void_p], c_int),
+                         [c_longlong, c_void_p, c_void_p, c_size_t, c_void_p], c_int),
     "nc_pages_extend": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int] + [c_void_p] * 6,
                         c_int),
     "nc_pages_trim": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p], c_int),

@@ -1,9 +1,22 @@
 """A token a row from logits (csrc/sample.hip): temperature, top-k, top-p (nucleus), min-p and allowed-token masks, from
 given uniform numbers. The decoder runtime (decoder.py) chooses its own tokens, with noise of its own; this is for callers
 that hold the logits, such as a step made of attention.packed_attention and library products."""
+import functools
+from collections import OrderedDict
+
 import torch
 
+from .attention import _workspace
 from .native import check, device_guard, hip_library, pointer, stream
+
+
+_WORKSPACES: OrderedDict = OrderedDict()
+
+
+@functools.lru_cache(maxsize=256)
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    """nc_sample_workspace_bytes, kept per shape."""
+    return hip_library().nc_sample_workspace_bytes(rows, vocab)
 
 
 def _per_row(t: torch.Tensor | None, name: str, dtype: torch.dtype, logits: torch.Tensor) -> int | None:
@@ -19,7 +32,7 @@ def _per_row(t: torch.Tensor | None, name: str, dtype: torch.dtype, logits: torc
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor,
                   top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None,
                   min_p: torch.Tensor | None = None, mask: torch.Tensor | None = None,
-                  out: torch.Tensor | None = None) -> torch.Tensor:
+                  out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """logits fp32 or bf16 [rows, vocab] (contiguous rows, any row stride), uniform fp32 [rows] in [0, 1) -> tokens int32
     [rows], -1 where no token is allowed.
 
@@ -29,8 +42,10 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature: torc
     decoder's masks). Of the allowed tokens whose logit is neither NaN nor -inf, with weights exp((z - max z) /
     temperature): the top_k largest stay (the lower index first among equals), of those the tokens with less than top_p of
     their weight strictly above them, of those the ones of at least min_p times the largest; the token is the first, in
-    index order, whose running weight exceeds uniform times what is left. One launch; a row's token does not depend on the
-    other rows."""
+    index order, whose running weight exceeds uniform times what is left. A row's token does not depend on the other rows.
+    A workspace passed in (at least sample_workspace_bytes) must have been zero-filled before its first use and only used
+    by these calls since, one stream at a time. Without one, calls on a stream share a cached workspace; a call that is
+    being captured into a graph gets one of the graph's own."""
     if logits.dim() != 2 or not logits.is_cuda:
         raise ValueError("logits must be a device tensor [rows, vocab]")
     if logits.dtype not in (torch.float32, torch.bfloat16):
@@ -54,9 +69,16 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature: torc
     _per_row(out, "out", torch.int32, logits)
     if rows == 0:
         return out
+    need = sample_workspace_bytes(rows, vocab)
     with device_guard(logits):
+        if workspace is None:
+            workspace = (torch.zeros(need, dtype=torch.uint8, device=logits.device)
+                         if torch.cuda.is_current_stream_capturing() else _workspace(logits.device, need, _WORKSPACES))
+        nbytes = workspace.numel() * workspace.element_size()
+        if nbytes < need or not workspace.is_contiguous() or workspace.device != logits.device or workspace.data_ptr() % 16:
+            raise ValueError(f"workspace must be a contiguous 16-byte aligned tensor of at least {need} bytes on {logits.device}")
         check(hip_library().nc_sample_tokens(
             pointer(logits), logits.dtype == torch.bfloat16, logits.stride(0) if rows > 1 else vocab, rows, vocab,
             *settings, pointer(mask) if mask is not None else None, mask.size(1) if mask is not None else 0,
-            pointer(out), stream()))
+            pointer(out), pointer(workspace), nbytes, stream()))
     return out

@@ -115,16 +115,20 @@ def test_packed_workspace_holds_every_launch(lib):
 
 def sample_args(**over):
     args = dict(logits=DUMMY, is_bf16=0, row_stride=100, rows=4, vocab=100, uniform=DUMMY, temperature=DUMMY, top_k=None,
-                top_p=None, min_p=None, mask=None, mask_stride=0, tokens=DUMMY, stream=None)
+                top_p=None, min_p=None, mask=None, mask_stride=0, tokens=DUMMY, workspace=DUMMY, workspace_bytes=1 << 26, stream=None)
     return list((args | over).values())
 
 
 def test_sample_rejects(lib):
-    for name in ("logits", "uniform", "temperature", "tokens"):
+    for name in ("logits", "uniform", "temperature", "tokens", "workspace"):
         assert lib.nc_sample_tokens(*sample_args(**{name: None})) == -1, name
     for over in (dict(rows=-1), dict(rows=2 ** 22 + 1), dict(vocab=0), dict(vocab=2 ** 24 + 1, row_stride=2 ** 25),
-                 dict(row_stride=99), dict(mask=DUMMY, mask_stride=3)):
+                 dict(row_stride=99), dict(mask=DUMMY, mask_stride=3), dict(workspace=ctypes.c_void_p(0x1008)), dict(workspace_bytes=15),
+                 dict(vocab=8193, row_stride=8193, workspace_bytes=lib.nc_sample_workspace_bytes(4, 8193) - 1)):
         assert lib.nc_sample_tokens(*sample_args(**over)) == -2, over
+    for rows, vocab in ((-1, 8), (2 ** 22 + 1, 8), (1, 0), (1, 2 ** 24 + 1)):
+        assert lib.nc_sample_workspace_bytes(rows, vocab) == 0
+    assert max(lib.nc_sample_workspace_bytes(2 ** 22, v) for v in (8192, 8193, 16385, 50257, 2 ** 18, 2 ** 18 + 1)) < 27e6
     assert lib.nc_sample_tokens(*sample_args(rows=0)) == 0
 
 
