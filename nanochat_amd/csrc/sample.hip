@@ -516,16 +516,14 @@ struct SplitShared {
     };
     union {
         u64 hist[ST_BINS];
-        struct {
-            u64 above[ST_LIST], equal[ST_LIST];
-        };
+        u64 above[ST_LIST];
     };
     u64 code[ST_LIST], w[ST_LIST];
     u64 sum[ST_E / 4 * ST_WAVES];
     u64 kept[ST_MAX_GROUPS], head[ST_MAX_GROUPS];
     int start[ST_MAX_GROUPS + 1];
     u64 found, least_code;
-    uint32_t lo, hi, cut;
+    uint32_t lo, hi;
     int bin, n, token, flag;
 };
 static_assert(2 * sizeof(SplitShared) <= 160 * 1024, "two workgroups a CU");
@@ -570,6 +568,22 @@ __device__ __forceinline__ u64 lane64(u64 v, int lane) {
 }
 __device__ __forceinline__ u64 lane_sum64(u64 v) { return lane64(lane_scan64(v), WAVE - 1); }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_max(u64 v) {
+    const uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+    const uint32_t l = __builtin_amdgcn_update_dpp((int)lo, (int)lo, CTRL, ROWS, 0xF, false);
+    const uint32_t h = __builtin_amdgcn_update_dpp((int)hi, (int)hi, CTRL, ROWS, 0xF, false);
+    return max(v, (u64)h << 32 | l);
+}
+__device__ __forceinline__ u64 lane_max64(u64 v) {
+    v = dpp_max<0x111, 0xF>(v);
+    v = dpp_max<0x112, 0xF>(v);
+    v = dpp_max<0x114, 0xF>(v);
+    v = dpp_max<0x118, 0xF>(v);
+    v = dpp_max<0x142, 0xA>(v);
+    v = dpp_max<0x143, 0xC>(v);
+    return lane64(v, WAVE - 1);
+}
 template <int CTRL, int ROWS>
 __device__ __forceinline__ float dpp_max(float v) {
     const int u = __float_as_int(v);
@@ -743,8 +757,7 @@ __device__ __forceinline__ int split_top(const Split &q, float (&x)[ST_E], int k
     for (int e = 0; e < ST_E; e++) best = max(best, token_code(x[e], q.index(e)));
     best = max(best, (u64)__shfl_xor(best, 1, WAVE));
     if (k == 1) {
-#pragma unroll
-        for (int o = 2; o < WAVE; o <<= 1) best = max(best, (u64)__shfl_xor(best, o, WAVE));
+        best = lane_max64(best);
         if (q.lane == 0) sh.sum[q.wave] = best;
         __syncthreads();
 #pragma unroll
@@ -757,11 +770,12 @@ __device__ __forceinline__ int split_top(const Split &q, float (&x)[ST_E], int k
     if ((t & 1) == 0) sh.most[t >> 1] = best;
     __syncthreads();
     if (q.wave == 0) {   /* by bisection, to k to k + 8 of the maxima, but at most ST_TOP */
-        u64 m[4], hi = 0;
+        u64 m[4], hi = 0, none = ~0ull;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             m[j] = sh.most[j * WAVE + q.lane];
             hi = max(hi, m[j]);
+            none = min(none, m[j] - 1);   /* a group without a token: the largest */
         }
         const auto reach = [&](u64 code) {
             int n = 0;
@@ -769,11 +783,10 @@ __device__ __forceinline__ int split_top(const Split &q, float (&x)[ST_E], int k
             for (int j = 0; j < 4; j++) n += __popcll(__ballot(m[j] >= code));
             return n;
         };
-#pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) hi = max(hi, (u64)__shfl_xor(hi, o, WAVE));
-        hi = lane64(hi, 0);
+        hi = lane_max64(hi);
         const int most = min(k + 8, ST_TOP);
-        u64 lo = 1;
+        u64 lo = ~lane_max64(~none) + 1;   /* the least of the maxima */
+        if (lo == 0 || reach(lo) < k) lo = 1;
         for (int n = reach(lo); n > most && lo < hi;) {
             const u64 mid = lo + (hi - lo + 1) / 2;
             const int of = reach(mid);
@@ -838,7 +851,8 @@ __device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 
 
 /* find_cut over the slices of a row: where the running sum of m(e), over the elements of the sets `live`, the larger value
  * first, reaches target(total). Ranges of values are narrowed by histograms, which the workgroups publish and each adds up,
- * until the tokens of the one that holds the cut fit a list, which each settles pairwise. sh.kept: per slice the weight of
+ * until the tokens of the one that holds the cut fit a list, which each settles pairwise. Between two histograms, and between
+ * two lists, there is always a meeting after the first is read. sh.kept: per slice the weight of
  * the tokens down to the cut that weigh least_w or more (not SPLIT). Every thread of every workgroup of the row calls it. */
 template <bool SPLIT, typename Target>
 __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t live, float zmax, float range, u64 least_w,
@@ -873,21 +887,27 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
         sh.hist[t] = sh.hist[t + ST_THREADS] = 0;
         if (t == 0) {
             sh.n = 0;
+            sh.least_code = ~0ull;
             sh.lo = 0xFFFFFFFFu;
             sh.hi = 0u;
         }
         __syncthreads();
+        u64 rest_of = 0;
         uint32_t bins[ST_E / 2];   /* two elements' a register; ST_BINS: not live */
 #pragma unroll
         for (int e = 0; e < ST_E; e++) {
             int b = keyed ? (int)((hi - order_key(x[e])) >> shift) : bin_of(x[e]);
             b = live >> e & 1 ? b : ST_BINS;
             bins[e / 2] = e & 1 ? bins[e / 2] | (uint32_t)b << 16 : (uint32_t)b;
-            if (b < ST_BINS)
+            if (b < ST_BINS - 1)
                 __hip_atomic_fetch_add(&sh.hist[b], m(e), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            rest_of += b == ST_BINS - 1 ? m(e) : 0;   /* many may be past the range: one addition a wave */
             if (e & 1) asm volatile("" : "+v"(bins[e / 2]));
             __builtin_amdgcn_sched_barrier(0);
         }
+        rest_of = lane_sum64(rest_of);
+        if (lane == 0 && rest_of)
+            __hip_atomic_fetch_add(&sh.hist[ST_BINS - 1], rest_of, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         __syncthreads();
         u64 v[2] = {sh.hist[2 * t], sh.hist[2 * t + 1]};
         if (G > 1) {
@@ -895,9 +915,19 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
             publish(part(q.g) + 2 * t + 1, v[1]);
             q.meet();
             v[0] = v[1] = 0;
-            for (int o = 0; o < G; o++) {
-                v[0] += peek(part(o) + 2 * t);
-                v[1] += peek(part(o) + 2 * t + 1);
+            for (int o = 0; o < G; o += 8) {   /* eight loads in flight */
+                u64 other[8][2];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const u64 *p = part(min(o + k, G - 1)) + 2 * t;
+                    other[k][0] = peek(p);
+                    other[k][1] = peek(p + 1);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    v[0] += o + k < G ? other[k][0] : 0;
+                    v[1] += o + k < G ? other[k][1] : 0;
+                }
             }
         }
         const u64 scan = lane_scan64(v[0] + v[1]);
@@ -911,7 +941,10 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
         }
         if (!keyed) {
             goal = target(total);
-            if (alike(goal > total)) return Cut{false, 0u, 0};
+            if (alike(goal > total)) {
+                q.meet();   /* the histograms are published over by the next cut: not before everyone has read these */
+                return Cut{false, 0u, 0};
+            }
         }
         const u64 rest = goal - base;
 #pragma unroll
@@ -1026,42 +1059,42 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
             if (t == 0) {
                 sh.kept[0] = above;
                 sh.head[0] = (u64)n;
+                sh.start[0] = 0;
+                sh.start[1] = n;
             }
         }
-        if (t < ST_LIST) sh.above[t] = sh.equal[t] = 0;
         __syncthreads();
         lo = (uint32_t)alike((int)sh.lo);
         hi = (uint32_t)alike((int)sh.hi);
         keyed = 1;
-        if (n <= ST_LIST) {
-            int lanes = 1;
-            while (lanes < n) lanes <<= 1;
-            const int i = t & (lanes - 1);
-            if (i < n) {
-                const u64 c = sh.code[i];
-                u64 more = 0, same = 0;
+        if (n <= ST_LIST) {   /* 512 / n lanes, up to 16, that are neighbours compare one token with the others */
+            int parts = 16;
+            while (parts > 2 && parts * n > ST_THREADS) parts >>= 1;
+            const int i = t / parts;
+            const u64 c = i < n ? sh.code[i] : ~0ull;
+            u64 more = 0;
 #pragma unroll 4
-                for (int j = t / lanes; j < n; j += ST_THREADS / lanes) {
-                    const u64 cj = sh.code[j], wj = sh.w[j];
-                    more += (SPLIT ? cj > c : cj >> 32 > c >> 32) ? wj : 0;
-                    same += !SPLIT && cj >> 32 == c >> 32 ? wj : 0;
-                }
-                __hip_atomic_fetch_add(&sh.above[i], more, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                if (!SPLIT) __hip_atomic_fetch_add(&sh.equal[i], same, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            for (int j = t % parts; j < n; j += parts)
+                more += (SPLIT ? sh.code[j] > c : (uint32_t)(sh.code[j] >> 32) > (uint32_t)(c >> 32)) ? sh.w[j] : 0;
+            for (int o = 1; o < parts; o <<= 1) more += (u64)__shfl_xor(more, o, WAVE);
+            if (i < n && t % parts == 0) {   /* the cut is the last that less than the goal lies above */
+                const bool in = base + more < goal;
+                if (in) __hip_atomic_fetch_min(&sh.least_code, c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (!SPLIT) sh.above[i] = in && sh.w[i] >= least_w ? sh.w[i] : 0;
             }
             __syncthreads();
-            if (t < n) {
-                const u64 more = base + sh.above[t], own = SPLIT ? sh.w[t] : sh.equal[t];
-                if (more < goal && goal <= more + own) {   /* one token, or one value's equals, who write the same */
-                    sh.cut = (uint32_t)(sh.code[t] >> 32);
-                    sh.token = SPLIT ? code_index(sh.code[t]) : 0x7FFFFFFF;
+            const u64 last = sh.least_code;
+            const Cut cut = {true, (uint32_t)(last >> 32), SPLIT ? code_index(last) : 0x7FFFFFFF};
+            if (!SPLIT) {
+                for (int o = wave; o < G; o += ST_WAVES) {
+                    u64 own = 0;
+                    for (int k = sh.start[o] + lane; k < sh.start[o + 1]; k += WAVE) own += sh.above[k];
+                    own = lane_sum64(own);
+                    if (lane == 0) sh.kept[o] += own;
                 }
-                if (!SPLIT && more < goal && sh.w[t] >= least_w)
-                    __hip_atomic_fetch_add(&sh.kept[code_index(sh.code[t]) / ST_SLICE], sh.w[t], __ATOMIC_RELAXED,
-                                           __HIP_MEMORY_SCOPE_WORKGROUP);
             }
             __syncthreads();
-            return Cut{true, sh.cut, sh.token};
+            return cut;
         }
         if (lo == hi) {   /* one value */
             if (!SPLIT) {
@@ -1111,6 +1144,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
         __syncthreads();
         const int ticket = alike(sh.n);
         q.row = y + ticket / q.G * ST_QUEUES;
+        if (q.row >= s.rows) return;   /* counts that were not zero: no access out of bounds */
         q.g = ticket % q.G;
     }
     q.first = q.g * ST_SLICE + 4 * q.t;
@@ -1271,9 +1305,10 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     }
     float least_z = -INFINITY;   /* the nucleus' smallest logit */
     if (p < 1.0f) {
-        /* values 47 log2 units below the largest weigh nothing */
-        const Cut mass = split_cut<false>(q, x, live, zmax,
-                                          fminf(zmax - least, 33.0f * T), least_w, mass_goal);
+        /* Values further below the largest than T ln(vocab / (1 - p)) weigh less than 1 - p of it together: the cut is not
+         * among them, nor 47 log2 units below, where they weigh nothing. The first ranges need not tell them apart. */
+        const float range = T * fminf(__logf((float)a.vocab / (1.0f - fmaxf(p, 0.0f))), 33.0f);
+        const Cut mass = split_cut<false>(q, x, live, zmax, fminf(zmax - least, range), least_w, mass_goal);
         if (mass.some) least_z = key_value(mass.key);
     } else {
         u64 own = 0;

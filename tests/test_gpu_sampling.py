@@ -193,3 +193,62 @@ def test_refusals(device):
         with pytest.raises(TypeError):
             sample_tokens(**{**dict(logits=z, uniform=u, temperature=u), **bad})
     assert sample_tokens(z[:0], u[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("vocab", [700, 8192, 8193, 20000, 262144, 262145])
+def test_few_allowed_tokens(device, vocab):
+    """Fewer allowed tokens than top-k asks for, in few places of the row or crowded in one, and none at all."""
+    rows = 10
+    u, t, rng = draws(rows, 11)
+    logits = torch.from_numpy(rng.normal(size=(rows, vocab)).astype(np.float32))
+    bits = np.zeros((rows, -(-vocab // 32) * 32), bool)
+    for r in range(rows):
+        if r % 3 == 0:
+            bits[r, rng.integers(0, vocab, r)] = True
+        elif r % 3 == 1:
+            at = int(rng.integers(0, vocab - 200))
+            bits[r, at:at + 40 * r] = True
+        else:
+            bits[r, vocab - r:vocab] = True
+    bits[:, vocab:] = False
+    mask = torch.from_numpy(np.packbits(bits, axis=1, bitorder="little").view(np.int32))
+    allowed = bits[:, :vocab]
+    for k in (1, 2, 50, 128, 129, 400):
+        for p in (1.0, 0.9):
+            kk, pp = np.full(rows, k), np.full(rows, p, np.float32)
+            compare(run(logits, device, u, t, top_k=kk, top_p=pp, mask=mask), logits, u, t, top_k=kk, top_p=pp, allowed=allowed)
+    compare(run(logits, device, u, t, top_p=np.full(rows, 0.7, np.float32), mask=mask), logits, u, t,
+            top_p=np.full(rows, 0.7, np.float32), allowed=allowed)
+
+
+@pytest.mark.parametrize("order", ["up", "down", "blocks"])
+def test_sorted_rows(device, order):
+    """Logits in an order that puts the largest into few threads, and equal logits everywhere."""
+    rows, vocab = 8, 30000
+    u, t, rng = draws(rows, 12)
+    z = np.sort(rng.normal(size=(rows, vocab)).astype(np.float32), axis=1)
+    if order == "down":
+        z = z[:, ::-1].copy()
+    elif order == "blocks":
+        z = np.roll(z.reshape(rows, -1, 8)[:, rng.permutation(vocab // 8)].reshape(rows, vocab), 3, axis=1)
+        z[4:] = 1.5
+    logits = torch.from_numpy(z)
+    for k in (1, 3, 100, 127, 128, 129, 5000):
+        kk = np.full(rows, k)
+        compare(run(logits, device, u, t, top_k=kk), logits, u, t, top_k=kk)
+    pp = rng.uniform(0.1, 1.0, rows).astype(np.float32)
+    compare(run(logits, device, u, t, top_p=pp), logits, u, t, top_p=pp)
+
+
+def test_rows_of_several_launches(device):
+    """More slices than one launch takes (2,048), calls of other sizes between them on the same workspace."""
+    vocab, rows = 9000, 1500
+    u, t, rng = draws(rows, 13)
+    logits = torch.from_numpy(rng.normal(size=(rows, vocab)).astype(np.float32) * 3)
+    k = np.where(rng.random(rows) < 0.5, 0, 30)
+    p = np.full(rows, 0.9, np.float32)
+    got = run(logits, device, u, t, top_k=k, top_p=p)
+    few = run(logits[:3], device, u[:3], t[:3], top_k=k[:3], top_p=p[:3])
+    assert np.array_equal(few, got[:3]) and np.array_equal(got, run(logits, device, u, t, top_k=k, top_p=p))
+    some = rng.permutation(rows)[:60]
+    compare(got[some], logits[some], u[some], t[some], top_k=k[some], top_p=p[some])
