@@ -10,21 +10,27 @@
  * The step over two pages (scores, softmax, PV) is nc_attend.h's. What bounds a sequence depends on its rows: a page of a
  * KV head is 2 KiB of K, 2 KiB of V and 128 bytes of scales for 16 keys, and each query column costs 512 flops a key, so
  * below about 80 columns (rows times the heads of a KV head) the pages' bytes take longer than the products. Hence two
- * kinds of work items, each one workgroup of four waves, both streaming pages into LDS by asynchronous copies:
+ * kinds of work items, both streaming pages into LDS by asynchronous copies:
  *
  *   narrow  at most 32 columns: one wave takes a chunk of the keys by itself, page pairs through a ring of its own in LDS
  *           with two pairs in flight; waves meet at no barrier, so one's start or merge hides behind the others' streams.
  *           A sequence of at most PK_SHORT pages is not cut but shared by the four waves of a workgroup, which merge
  *           through LDS ("alone": it costs no round trips through memory, which is what a short one's time is made of)
  *   wide    a tile of up to 128 columns, 32 a wave: the four waves of a workgroup walk the same pairs, each fetched once
- *           (two stages of two pairs ahead); of at most 64 columns two waves take one pair of a stage and two the other
+ *           (two stages of two pairs ahead); of at most 64 columns two waves take one pair of a stage and two the other,
+ *           so that no wave idles (64 sequences of 64 columns over 8,192 keys: 172 us, and 207 by two waves of the four)
  *
  * A sequence's keys are cut into chunks (pk_plan), so that few rows over many keys still fill the chip; a (tile, KV head)
  * of several chunks leaves one partial (O, max, sum) in fp32 a chunk, and whoever finishes its last chunk merges them in
  * order. The cuts depend on nothing but the sequence's own numbers, so its output bits do not depend on the rest of the
- * launch. A workgroup takes wide and alone items while there are any, then its waves narrow ones: the first by workgroup index, later
- * ones from eight queues (an XCD's workgroups take every eighth item, which keeps a KV head's pages in that XCD's L2), so
- * that unequal items even out.
+ * launch. A workgroup takes wide and alone items while there are any, then its waves narrow ones: the first by workgroup
+ * index, later ones from eight queues (an XCD's workgroups take every eighth item, which keeps a KV head's pages in that
+ * XCD's L2), so that unequal items even out.
+ *
+ * Measured (16 query heads, 4 KV heads): 64 sequences of 8,192 keys, one row each 98 us (5.6 TB/s of pages), 4 rows each
+ * 110 us (5.0), 16 rows each 172 us; 8 prompt chunks of 257 to 512 rows over at most 4,096 keys 175 us (736 TFLOP/s of the
+ * keys a row may see), 2 prompts of 4,096 rows 173 us (795). One sequence, 5 rows of 6 heads over 1,029 keys: 14 us, most of
+ * it round trips to memory one after the other (the plan, the block table, pages, the output).
  */
 #include <limits.h>
 
@@ -38,12 +44,18 @@ constexpr int PK_NARROW_COLS = 16 * PK_NT;
 constexpr int PK_WIDE_COLS = WAVES * 16 * PK_NT;
 constexpr int PK_MAX_BATCH = 1024;
 constexpr int PK_QUEUES = 8;                   /* XCDs */
-constexpr int PK_NARROW_SPLIT = 64;            /* pages of a narrow chunk */
+/* Pages of a narrow chunk: 64 sequences of 8,192 keys, 4 rows each, take 110 us with 64 pages and 154 with 32 (twice the
+ * partials); one of 32,768 keys 34.6 and 32.7. */
+constexpr int PK_NARROW_SPLIT = 64;
 constexpr int PK_MIN_TAIL = 4;                 /* a last chunk of fewer pages joins the one before it */
-constexpr int PK_SHORT = 2 * PK_NARROW_SPLIT;  /* a narrow sequence of at most so many pages is not cut */
-constexpr int PK_WIDE_MIN = 128;               /* least and most pages of a wide chunk */
-constexpr int PK_WIDE_MAX = 1024;
-constexpr int PK_WIDE_ITEMS = 256;             /* items a wide sequence is cut into at most, if its chunks stay that long */
+/* A narrow sequence of at most so many pages is not cut: 1,029 keys take 14.0 us whole, 25.5 in two partials. */
+constexpr int PK_SHORT = 2 * PK_NARROW_SPLIT;
+/* Least and most pages of a wide chunk, and the items that a wide sequence is cut into at most if its chunks stay that long.
+ * Short chunks fill the chip when a sequence is alone, and cost partials when it is not: one chunk of 512 rows over 8,192 keys
+ * takes 69 us with 128 pages at least and 113 with 256, eight of them over at most 4,096 keys 175 and 153 (64 pages: 69 and
+ * 204). A cut by what else the launch holds would make a sequence's bits depend on it. 128 items: 114 us for the first, and
+ * 260 instead of 175 for 4 chunks of 200 to 700 rows among 60 decoding sequences. */
+constexpr int PK_WIDE_MIN = 128, PK_WIDE_MAX = 1024, PK_WIDE_ITEMS = 256;
 constexpr int PK_AHEAD = 2;                    /* wide: stages of two pairs in flight */
 static_assert(PK_SHORT <= 2 * WAVE && PK_NARROW_SPLIT + PK_MIN_TAIL <= 2 * WAVE,
               "a narrow item's block-table entries: two a lane");
@@ -53,8 +65,8 @@ static_assert(PK_SHORT <= 2 * WAVE && PK_NARROW_SPLIT + PK_MIN_TAIL <= 2 * WAVE,
 constexpr int PK_SCALE_AT = 4 * PAGE_BYTES, PK_SCALE_BYTES = 256;
 constexpr int PK_WIDE_STAGE = 2 * PK_SCALE_AT + WAVES * 2 * PK_SCALE_BYTES, PK_WIDE_BUFS = PK_AHEAD + 1;
 constexpr int PK_NARROW_STAGE = PK_SCALE_AT + PK_SCALE_BYTES;
-constexpr int PK_BUFS = 2, PK_DEEP = 4;   /* pairs of a narrow wave's ring: two workgroups a CU, or one */
-constexpr int PK_STAGES = WAVES * PK_BUFS * PK_NARROW_STAGE;   /* bytes of LDS, the least */
+constexpr int PK_BUFS = 2;                     /* pairs of a narrow wave's ring */
+constexpr int PK_STAGES = WAVES * PK_BUFS * PK_NARROW_STAGE;   /* bytes of LDS */
 static_assert(PK_WIDE_BUFS * PK_WIDE_STAGE <= PK_STAGES, "the wide stages fit");
 typedef __attribute__((address_space(3))) void LdsVoid;
 
@@ -66,7 +78,6 @@ struct PackedArgs {
     long long wide_slots, narrow_slots;
     int units;                  /* arrival counts */
     int tpt;                    /* tokens of a 16-column tile: 16 / G */
-    int bufs;                   /* PK_BUFS or PK_DEEP */
     int *tickets, *done, *arrived;    /* [2][8][PK_LINE] (workgroups, waves), [PK_LINE], [units]; zero between launches */
 };
 
@@ -651,7 +662,8 @@ __device__ __forceinline__ int pk_wide(const PackedArgs &p, const PkItem &it, in
 
 /* --- narrow items */
 
-/* One pair's copies into a wave's stage: four of 1 KiB a page, through descriptors of one page (live false: of no range, so nothing is read), and the 256 scale bytes. Nine in all. */
+/* One pair's copies into a wave's stage: four of 1 KiB a page, through descriptors of one page (live false: of no range, so
+ * nothing is read), and the 256 scale bytes. Nine in all. */
 __device__ __forceinline__ void pk_fetch_narrow(const AttnArgs &a, int pa, int pb, bool live, int kvh, unsigned char *st,
                                                 int lane) {
     const long long ha = (long long)pa * a.Hkv + kvh, hb = (long long)pb * a.Hkv + kvh;
@@ -702,18 +714,17 @@ __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it,
                                                                                                        * first again */
         pk_fetch_narrow(a, entry(la), entry(lb), i < pairs, it.kvh, ring + buf * PK_NARROW_STAGE, lane);
     };
-    const int bufs = p.bufs;
-    for (int i = 0; i < bufs; i++) fetch(i, i);
+#pragma unroll
+    for (int i = 0; i < PK_BUFS; i++) fetch(i, i);
     QOp qb[NT];
     q8_from_raw<NT>(raw, qb);
     for (int i = 0; i < pairs; i++) {
-        const int buf = i & (bufs - 1), at = lds + buf * PK_NARROW_STAGE, lpa = it.pg0 + 2 * (first + stride * i);
+        const int buf = i & (PK_BUFS - 1), at = lds + buf * PK_NARROW_STAGE, lpa = it.pg0 + 2 * (first + stride * i);
         /* all but the younger pairs' copies have landed */
-        if (bufs == PK_BUFS) __builtin_amdgcn_s_waitcnt(pk_wait(9 * (PK_BUFS - 1), 15));
-        else __builtin_amdgcn_s_waitcnt(pk_wait(9 * (PK_DEEP - 1), 15));
+        __builtin_amdgcn_s_waitcnt(pk_wait(9 * (PK_BUFS - 1), 15));
         asm volatile("" ::: "memory");
         pk_pair<NT>(lpa, lpa + 1 < it.pg1, PkAt{at, at + PK_SCALE_AT}, qb, kb, zero, ws, lane,
-                    [&] { fetch(i + bufs, buf); });
+                    [&] { fetch(i + PK_BUFS, buf); });
     }
     if constexpr (!ALONE) {
         const PkPart part = pk_part(p.part_narrow, p.narrow_slots, PK_NARROW_COLS, slot);
@@ -830,9 +841,9 @@ __device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, 
 }
 
 __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
-    /* the stages, WAVES bufs PK_NARROW_STAGE bytes; [PK_SUMS][B + 1] prefix sums; [3][B]: row0, n, len */
+    /* the stages, PK_STAGES bytes; [PK_SUMS][B + 1] prefix sums; [3][B]: row0, n, len */
     extern __shared__ __align__(16) unsigned char stages[];
-    int *pk_lds = reinterpret_cast<int *>(stages + WAVES * p.bufs * PK_NARROW_STAGE);
+    int *pk_lds = reinterpret_cast<int *>(stages + PK_STAGES);
     __shared__ int tab[PK_WIDE_MAX];
     __shared__ int scan[PK_SUMS][WAVES];
     __shared__ int sh_next;
@@ -926,7 +937,7 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
             it.pg0 = it.q.pg0;
             it.pg1 = it.q.pg0 + it.q.np;
             const int wave = uni((int)threadIdx.x >> 6);
-            unsigned char *ring = stages + wave * p.bufs * PK_NARROW_STAGE;
+            unsigned char *ring = stages + wave * PK_BUFS * PK_NARROW_STAGE;
             if (it.tn <= p.tpt)
                 pk_narrow<1, true>(p, it, 1, 0, ring, wave, stages, reinterpret_cast<float *>(tab));
             else
@@ -947,7 +958,7 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
      * not every wave of the chip starts with a ticket) */
     const int lane = threadIdx.x & (WAVE - 1), wave = uni((int)threadIdx.x >> 6);
     const int free = max(G - N, 0), first = WAVES * free;
-    unsigned char *ring = stages + wave * p.bufs * PK_NARROW_STAGE;
+    unsigned char *ring = stages + wave * PK_BUFS * PK_NARROW_STAGE;
     int *tickets = p.tickets + PK_QUEUES * PK_LINE;
     const bool queued = NN > first;
     int k = (int)blockIdx.x - N + free * wave;
@@ -1002,12 +1013,12 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
 }
 
 /* The most partials and arrival counts a launch of these sizes can need, whatever its lengths (pk_plan): a narrow sequence
- * longer than PK_SHORT pages is Hkv units of at most ceil(pages / PK_NARROW_SPLIT) chunks. A wide one has at least tpw + 1 rows; all of them together have at
- * most rows / TW + their number tiles, each Hkv units, cut into at most ceil(pages / PK_WIDE_MIN) chunks, and no sequence
- * into more than PK_WIDE_ITEMS items unless its chunks would pass PK_WIDE_MAX pages. */
+ * longer than PK_SHORT pages is Hkv units of at most ceil(pages / PK_NARROW_SPLIT) chunks. A wide one has at least tpw + 1
+ * rows; all of them together have at most rows / (WAVES tpw) + their number tiles, each Hkv units, cut into at most
+ * ceil(pages / PK_WIDE_MIN) chunks, and no sequence into more than PK_WIDE_ITEMS items unless its chunks would pass
+ * PK_WIDE_MAX pages. */
 struct PkSizes {
     long long wide_slots, narrow_slots, units;
-    long long items, narrow_chunks;   /* wide items at most; a narrow sequence's chunks at most */
 };
 
 static PkSizes pk_sizes(long long rows, int B, int Hq, int Hkv, int max_seq_len, int window) {
@@ -1017,11 +1028,10 @@ static PkSizes pk_sizes(long long rows, int B, int Hq, int Hkv, int max_seq_len,
     if (window >= 0) np = min(np, (rows + window) / PAGE + 3);
     const long long nw = min((long long)B, rows / (tpw + 1)), tiles = rows / (WAVES * tpw) + nw;
     PkSizes z = {};
-    const long long nch = np <= PK_SHORT ? 1 : (np - 1) / PK_NARROW_SPLIT + 1, wch = (np - 1) / PK_WIDE_MIN + 1, most = (np - 1) / PK_WIDE_MAX + 1;
+    const long long nch = np <= PK_SHORT ? 1 : (np - 1) / PK_NARROW_SPLIT + 1;
+    const long long wch = (np - 1) / PK_WIDE_MIN + 1, most = (np - 1) / PK_WIDE_MAX + 1;
     if (nch > 1) z.narrow_slots = min((long long)B, rows) * Hkv * nch;
     if (wch > 1) z.wide_slots = min(tiles * Hkv * wch, nw * PK_WIDE_ITEMS + (most > 1 ? tiles * Hkv * most : 0));
-    z.items = max(z.wide_slots, tiles * Hkv);
-    z.narrow_chunks = nch;
     z.units = (nch > 1 ? min((long long)B, rows) : 0) * Hkv + (wch > 1 ? tiles * Hkv : 0);
     return z;
 }
@@ -1087,13 +1097,8 @@ extern "C" int nc_packed_attn_fp8(const void *q, const void *k_pages, const void
     p.tickets = (int *)((char *)workspace + counts);
     p.done = p.tickets + 2 * PK_QUEUES * PK_LINE;
     p.arrived = p.done + PK_LINE;
-    /* Where the launch cannot have more work than one workgroup a CU, one is launched with rings twice as deep: a wave that
-     * streams alone waits for memory (one sequence, 1,029 keys, 6 heads: 17.8 -> DEEP_US us). The results do not change. */
+    const size_t lds = PK_STAGES + (PK_SUMS * (B + 1) + 3 * B) * sizeof(int);
     const int cus = device_cus() / PK_QUEUES * PK_QUEUES;
-    const long long few = min((long long)B, rows) * Hkv;
-    const bool deep = z.items + few <= cus && few * z.narrow_chunks <= (long long)WAVES * cus;
-    p.bufs = deep ? PK_DEEP : PK_BUFS;
-    const size_t lds = (size_t)WAVES * p.bufs * PK_NARROW_STAGE + (PK_SUMS * (B + 1) + 3 * B) * sizeof(int);
-    hipLaunchKernelGGL(packed_attn_kernel, dim3(max(deep ? cus : 2 * cus, PK_QUEUES)), dim3(256), lds, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(packed_attn_kernel, dim3(max(2 * cus, PK_QUEUES)), dim3(256), lds, (hipStream_t)stream, p);
     return (int)hipGetLastError();
 }

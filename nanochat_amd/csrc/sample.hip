@@ -13,10 +13,19 @@
  * as exact as its weights (2^-47 of the largest at 65,536 tokens): a border between two tokens moves by less than that
  * share. In float32 a border among many small weights would move by about their size.
  *
- * One workgroup of 16 waves takes a row, wave w a contiguous run of it, so that a sum in index order is a sum over waves,
- * then over one wave. No sort: the place where a running count (top-k) or
- * weight (top-p) in order of value reaches its target is found by a histogram over 4,096 ranges of the value, then among
- * the few tokens of the range that holds it, or by finer histograms where it holds many.
+ * No sort: the place where a running count (top-k) or weight (top-p) in order of value reaches its target is found by a
+ * histogram over ranges of the value, then among the few tokens of the range that holds it, or by finer histograms where it
+ * holds many.
+ *
+ * split_kernel takes rows of up to 262,144 tokens, a workgroup for every 8,192, which stay in its registers. What bounds it
+ * is neither bytes nor operations (a row of 65,536 fp32 logits is 256 KiB) but the steps one after the other, each ending
+ * where the row's workgroups need one another: the largest logit; the histogram; the list; about 2.5 us a meeting through
+ * memory. Greedy rows and a top-k of at most 128 need no meeting: every slice leaves its k largest in order, and the last
+ * workgroup to arrive does the rest on k tokens. Measured: one row of 65,536 fp32 logits with top-p 27 us (one workgroup
+ * with the row read again for every step: 114), with top-k 15; 128 such rows of mixed settings, a quarter greedy, 35 (89);
+ * 333 rows of 32,768 masked bf16 logits with top-p 84 (140), where the workgroups' two a CU come in three rounds.
+ * sample_kernel takes longer rows: one workgroup of 16 waves reads the row again for every step, wave w a contiguous run of
+ * it, so that a sum in index order is a sum over waves, then over one wave (400,000 tokens with top-p: 680 us).
  */
 #include <math.h>
 
@@ -478,7 +487,10 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(SampleArgs a) {
 }
 
 /* --- Rows of up to ST_MAX_GROUPS slices of 8,192 tokens, a workgroup each: the slice stays in its registers, 16 tokens a
- * thread, and the workgroups of a row exchange what the next step needs through memory. */
+ * thread, and the workgroups of a row exchange what the next step needs through memory. 512 threads of at most 128 registers
+ * and the weights in LDS leave room for two workgroups a CU, one working while the other waits: one workgroup a CU (no
+ * spilled registers, 149 of them) takes 25 us for one row instead of 27, but 124 instead of 88 for 333 rows, and slices of
+ * 1,024 threads with 8 tokens each 30 and 150. */
 
 constexpr int ST_WAVES = 8, ST_THREADS = ST_WAVES * WAVE;
 constexpr int ST_E = 16, ST_SLICE = ST_E * ST_THREADS;
@@ -493,7 +505,7 @@ constexpr int ST_QUEUES = 8;              /* XCDs */
 constexpr int ST_MAX_WORKGROUPS = 2048;   /* of one launch, when rows are cut: bounds the workspace */
 static_assert(ST_TOP * (ST_SLICE / 256) <= ST_CAND && ST_TOP * ST_MAX_GROUPS <= ST_CAND, "candidates fit");
 
-enum { HD_BEST, HD_LEAST, HD_COUNT, HD_ABOVE, HD_KEYS, HD_SUM, HD_TIES, HD_INDEX, HD_WORDS };
+enum { HD_BEST, HD_COUNT, HD_ABOVE, HD_LEAST, HD_MOST, HD_SUM, HD_WORDS };
 constexpr int ST_PART = ST_BINS + 2 * ST_LIST + HD_WORDS;   /* words a workgroup publishes: histogram, list, head */
 
 struct SplitArgs {
@@ -522,8 +534,7 @@ struct SplitShared {
     u64 sum[ST_E / 4 * ST_WAVES];
     u64 kept[ST_MAX_GROUPS], head[ST_MAX_GROUPS];
     int start[ST_MAX_GROUPS + 1];
-    u64 found, least_code;
-    uint32_t lo, hi;
+    u64 found, least_code, lo, hi;
     int bin, n, token, flag;
 };
 static_assert(2 * sizeof(SplitShared) <= 160 * 1024, "two workgroups a CU");
@@ -544,6 +555,9 @@ __device__ __forceinline__ u64 peek(const u64 *p) {
 
 /* A value that is the same in every lane, as a scalar register's: branches on it are the wave's. */
 __device__ __forceinline__ int alike(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ u64 alike(u64 x) {
+    return (u64)(uint32_t)alike((int)(uint32_t)(x >> 32)) << 32 | (uint32_t)alike((int)(uint32_t)x);
+}
 __device__ __forceinline__ float alike(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 
 /* Inclusive sums over the lanes by DPP: shifts by 1, 2, 4 and 8 within rows of 16 lanes, then a row's last sum added to the
@@ -823,6 +837,7 @@ template <typename M>
 __device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 goal) {
     SplitShared &sh = q.sh;
     u64 own[ST_E / 4], scan[ST_E / 4];
+    asm volatile("" : "+v"(in));
 #pragma unroll
     for (int c = 0; c < ST_E / 4; c++) {
         own[c] = 0;
@@ -830,6 +845,7 @@ __device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 
         for (int j = 0; j < 4; j++) own[c] += in >> (4 * c + j) & 1 ? m(4 * c + j) : 0;
         scan[c] = lane_scan64(own[c]);
         if (q.lane == WAVE - 1) sh.sum[c * ST_WAVES + q.wave] = scan[c];
+        __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
     const u64 part = q.lane < ST_E / 4 * ST_WAVES ? sh.sum[q.lane] : 0, upto = lane_scan64(part) - part;
@@ -844,6 +860,7 @@ __device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 
                 before += v;
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
     return sh.token;
@@ -852,8 +869,8 @@ __device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 
 /* find_cut over the slices of a row: where the running sum of m(e), over the elements of the sets `live`, the larger value
  * first, reaches target(total). Ranges of values are narrowed by histograms, which the workgroups publish and each adds up,
  * until the tokens of the one that holds the cut fit a list, which each settles pairwise. Between two histograms, and between
- * two lists, there is always a meeting after the first is read. sh.kept: per slice the weight of
- * the tokens down to the cut that weigh least_w or more (not SPLIT). Every thread of every workgroup of the row calls it. */
+ * two lists, there is always a meeting after the first is read. sh.kept: per slice the weight of the tokens down to the cut
+ * that weigh least_w or more (not SPLIT). Every thread of every workgroup of the row calls it. */
 template <bool SPLIT, typename Target>
 __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t live, float zmax, float range, u64 least_w,
                                          Target target) {
@@ -866,12 +883,14 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
     /* a range whose products are NaN or past the last bin: the last bin; monotone in z in every case */
     const auto bin_of = [&](float z) { return z == zmax ? 0 : (int)fminf((zmax - z) * scale, (float)(ST_BINS - 1)); };
     u64 goal = 0, base = 0;
-    uint32_t lo = 0u, hi = 0xFFFFFFFFu;   /* once a range of values is split again: its keys */
+    /* once a range of values is split again: by its keys, or its tokens' codes where equals are told apart */
+    u64 lo = 0, hi = ~0ull;
+    const auto key = [&](int e) { return SPLIT ? token_code(x[e], q.index(e)) : (u64)order_key(x[e]); };
     int keyed = 0;
     u64 base_above = 0;
     for (;;) {
         /* one body for the first level and the others, and no address or set kept in registers from one to the next */
-        asm volatile("" : "+s"(keyed), "+s"(lo), "+s"(hi), "+s"(base_part), "+v"(t), "+v"(q.first), "+v"(live));
+        asm volatile("" : "+s"(keyed), "+s"(base_part), "+v"(t), "+v"(q.first), "+v"(live));
         const auto part = [&](int o) { return base_part + (long long)o * ST_PART; };
         const auto listed = [&](u64 code) {   /* what a token of this slice counts */
             const int i = code_index(code) - q.g * ST_SLICE;
@@ -888,22 +907,26 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
         if (t == 0) {
             sh.n = 0;
             sh.least_code = ~0ull;
-            sh.lo = 0xFFFFFFFFu;
-            sh.hi = 0u;
+            sh.lo = ~0ull;
+            sh.hi = 0;
         }
         __syncthreads();
-        u64 rest_of = 0;
+        u64 rest_of = 0, w4[4];
         uint32_t bins[ST_E / 2];   /* two elements' a register; ST_BINS: not live */
 #pragma unroll
         for (int e = 0; e < ST_E; e++) {
-            int b = keyed ? (int)((hi - order_key(x[e])) >> shift) : bin_of(x[e]);
+            int b = keyed ? (int)min((hi - key(e)) >> shift, (u64)ST_BINS) : bin_of(x[e]);
             b = live >> e & 1 ? b : ST_BINS;
             bins[e / 2] = e & 1 ? bins[e / 2] | (uint32_t)b << 16 : (uint32_t)b;
+            if (e % 4 == 0) {   /* four weights' loads in flight */
+#pragma unroll
+                for (int k = 0; k < 4; k++) w4[k] = m(e + k);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (b < ST_BINS - 1)
-                __hip_atomic_fetch_add(&sh.hist[b], m(e), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            rest_of += b == ST_BINS - 1 ? m(e) : 0;   /* many may be past the range: one addition a wave */
-            if (e & 1) asm volatile("" : "+v"(bins[e / 2]));
-            __builtin_amdgcn_sched_barrier(0);
+                __hip_atomic_fetch_add(&sh.hist[b], w4[e % 4], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            rest_of += b == ST_BINS - 1 ? w4[e % 4] : 0;   /* many may be past the range: one addition a wave */
+            if (e & 1) asm volatile("" : "+v"(bins[e / 2]), "+v"(rest_of));
         }
         rest_of = lane_sum64(rest_of);
         if (lane == 0 && rest_of)
@@ -915,19 +938,10 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
             publish(part(q.g) + 2 * t + 1, v[1]);
             q.meet();
             v[0] = v[1] = 0;
-            for (int o = 0; o < G; o += 8) {   /* eight loads in flight */
-                u64 other[8][2];
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const u64 *p = part(min(o + k, G - 1)) + 2 * t;
-                    other[k][0] = peek(p);
-                    other[k][1] = peek(p + 1);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    v[0] += o + k < G ? other[k][0] : 0;
-                    v[1] += o + k < G ? other[k][1] : 0;
-                }
+#pragma unroll 4
+            for (int o = 0; o < G; o++) {
+                v[0] += peek(part(o) + 2 * t);
+                v[1] += peek(part(o) + 2 * t + 1);
             }
         }
         const u64 scan = lane_scan64(v[0] + v[1]);
@@ -941,7 +955,7 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
         }
         if (!keyed) {
             goal = target(total);
-            if (alike(goal > total)) {
+            if (alike((int)(goal > total))) {
                 q.meet();   /* the histograms are published over by the next cut: not before everyone has read these */
                 return Cut{false, 0u, 0};
             }
@@ -962,7 +976,7 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
         anew(x);
         asm volatile("" : "+v"(t), "+v"(live), "+v"(q.first));
         u64 above = 0;
-        uint32_t least = 0xFFFFFFFFu, most = 0u;
+        u64 least = ~0ull, most = 0;
         const auto slot = [&](int e) { return (int)(bins[e / 2] >> (e & 1) * 16 & 0xFFFFu); };
         live = 0;
 #pragma unroll
@@ -973,7 +987,7 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
                 const u64 v = m(e);
                 base_above += b < bin && v >= least_w ? v : 0;
             }
-            __builtin_amdgcn_sched_barrier(0);
+            if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
         asm volatile("" : "+v"(base_above));
         above = base_above;
@@ -983,7 +997,7 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
 #pragma unroll
             for (int e = 0; e < ST_E; e++) {
                 if (live >> e & 1) {
-                    const uint32_t k = order_key(x[e]);
+                    const u64 k = key(e);
                     if (at < ST_LIST) sh.code[at] = token_code(x[e], q.index(e));
                     at++;
                     least = min(least, k);
@@ -1016,17 +1030,17 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
             if (t == 0) {
                 tell(HD_COUNT, (u64)n);
                 tell(HD_ABOVE, above);
-                tell(HD_KEYS, (u64)sh.lo << 32 | sh.hi);
+                tell(HD_LEAST, sh.lo);
+                tell(HD_MOST, sh.hi);
             }
             q.meet();
             if (wave == 0) {
                 int count = 0;
-                uint32_t l = 0xFFFFFFFFu, h = 0u;
+                u64 l = ~0ull, h = 0;
                 if (lane < G) {
                     count = (int)head_of(HD_COUNT);
-                    const u64 keys = head_of(HD_KEYS);
-                    l = (uint32_t)(keys >> 32);
-                    h = (uint32_t)keys;
+                    l = head_of(HD_LEAST);
+                    h = head_of(HD_MOST);
                     sh.kept[lane] = head_of(HD_ABOVE);
                     sh.head[lane] = (u64)count;
                 }
@@ -1035,9 +1049,9 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
                 for (int o = 1; o < WAVE; o <<= 1) {
                     const int up = __shfl_up(end, o, WAVE);
                     if (lane >= o) end += up;
-                    l = min(l, (uint32_t)__shfl_xor(l, o, WAVE));
-                    h = max(h, (uint32_t)__shfl_xor(h, o, WAVE));
                 }
+                l = ~lane_max64(~l);
+                h = lane_max64(h);
                 if (lane < G) sh.start[lane + 1] = end;
                 if (lane == 0) {
                     sh.start[0] = 0;
@@ -1064,64 +1078,42 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
             }
         }
         __syncthreads();
-        lo = (uint32_t)alike((int)sh.lo);
-        hi = (uint32_t)alike((int)sh.hi);
+        lo = alike(sh.lo);
+        hi = alike(sh.hi);
         keyed = 1;
-        if (n <= ST_LIST) {   /* 512 / n lanes, up to 16, that are neighbours compare one token with the others */
-            int parts = 16;
-            while (parts > 2 && parts * n > ST_THREADS) parts >>= 1;
-            const int i = t / parts;
-            const u64 c = i < n ? sh.code[i] : ~0ull;
-            u64 more = 0;
+        if (n <= ST_LIST) {
+            if (t < ST_LIST) sh.above[t] = 0;
+            __syncthreads();
+            int lanes = 1;
+            while (lanes < n) lanes <<= 1;
+            const int i = t & (lanes - 1);
+            if (i < n) {
+                const u64 c = sh.code[i];
+                u64 more = 0;
 #pragma unroll 4
-            for (int j = t % parts; j < n; j += parts)
-                more += (SPLIT ? sh.code[j] > c : (uint32_t)(sh.code[j] >> 32) > (uint32_t)(c >> 32)) ? sh.w[j] : 0;
-            for (int o = 1; o < parts; o <<= 1) more += (u64)__shfl_xor(more, o, WAVE);
-            if (i < n && t % parts == 0) {   /* the cut is the last that less than the goal lies above */
-                const bool in = base + more < goal;
-                if (in) __hip_atomic_fetch_min(&sh.least_code, c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                if (!SPLIT) sh.above[i] = in && sh.w[i] >= least_w ? sh.w[i] : 0;
+                for (int j = t / lanes; j < n; j += ST_THREADS / lanes)
+                    more += (SPLIT ? sh.code[j] > c : (uint32_t)(sh.code[j] >> 32) > (uint32_t)(c >> 32)) ? sh.w[j] : 0;
+                __hip_atomic_fetch_add(&sh.above[i], more, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+            __syncthreads();
+            if (t < n) {
+                const bool in = base + sh.above[t] < goal;
+                if (in) __hip_atomic_fetch_min(&sh.least_code, sh.code[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (!SPLIT && in && sh.w[t] >= least_w)
+                    __hip_atomic_fetch_add(&sh.kept[code_index(sh.code[t]) / ST_SLICE], sh.w[t], __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_WORKGROUP);
             }
             __syncthreads();
             const u64 last = sh.least_code;
-            const Cut cut = {true, (uint32_t)(last >> 32), SPLIT ? code_index(last) : 0x7FFFFFFF};
-            if (!SPLIT) {
-                for (int o = wave; o < G; o += ST_WAVES) {
-                    u64 own = 0;
-                    for (int k = sh.start[o] + lane; k < sh.start[o + 1]; k += WAVE) own += sh.above[k];
-                    own = lane_sum64(own);
-                    if (lane == 0) sh.kept[o] += own;
-                }
+            return Cut{true, (uint32_t)(last >> 32), SPLIT ? code_index(last) : 0x7FFFFFFF};
+        }
+        if (!SPLIT && lo == hi) {   /* one value */
+            if (t < G && sh.head[t]) {
+                const u64 of = G > 1 ? peek(part(t) + ST_BINS + ST_LIST) : sh.w[0];   /* every one's weight */
+                if (of >= least_w) sh.kept[t] += sh.head[t] * of;
             }
             __syncthreads();
-            return cut;
-        }
-        if (lo == hi) {   /* one value */
-            if (!SPLIT) {
-                if (t < G && sh.head[t]) {
-                    const u64 of = G > 1 ? peek(part(t) + ST_BINS + ST_LIST) : sh.w[0];   /* every one's weight */
-                    if (of >= least_w) sh.kept[t] += sh.head[t] * of;
-                }
-                __syncthreads();
-                return Cut{true, lo, 0x7FFFFFFF};
-            }
-            u64 before_us = 0;
-            for (int o = 0; o < q.g; o++) before_us += sh.head[o];
-            const u64 rest1 = goal - base, ours = sh.head[q.g];
-            int idx = 0;
-            const bool holds = before_us < rest1 && rest1 <= before_us + ours;
-            if (alike(holds)) idx = split_pick(q, live, m, rest1 - before_us);
-            if (G > 1) {
-                if (t == 0) tell(HD_INDEX, holds ? (u64)idx + 1 : 0ull);
-                q.meet();
-                if (t < G) {
-                    const u64 of = head_of(HD_INDEX);
-                    if (of) sh.token = (int)of - 1;
-                }
-                __syncthreads();
-                idx = sh.token;
-            }
-            return Cut{true, lo, idx};
+            return Cut{true, (uint32_t)lo, 0x7FFFFFFF};
         }
     }
 }
@@ -1301,7 +1293,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
         const u64 v = weight(x[e]);
         sh.weight[e * ST_THREADS + t] = v;   /* read by this thread alone */
         live |= (uint32_t)(v != 0) << e;
-        if (e & 1) __builtin_amdgcn_sched_barrier(0);   /* two at a time: more would need more registers */
+        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);   /* four at a time: more would need more registers */
     }
     float least_z = -INFINITY;   /* the nucleus' smallest logit */
     if (p < 1.0f) {
@@ -1340,7 +1332,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     }
     const u64 goal = choice(total), ours = sh.kept[q.g];
     __syncthreads();
-    if (alike(before < goal && goal <= before + ours)) {
+    if (alike((int)(before < goal && goal <= before + ours))) {
         uint32_t kept = 0;
 #pragma unroll
         for (int e = 0; e < ST_E; e++) kept |= (uint32_t)(x[e] >= least_z && sh.weight[e * ST_THREADS + t] >= least_w) << e;
