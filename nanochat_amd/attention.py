@@ -59,7 +59,7 @@ def qk_norm_rope_append(qkv: torch.Tensor, num_q_heads: int, cache: PagedKVCache
 
 def _same_device(device: torch.device, **tensors: torch.Tensor) -> None:
     for name, t in tensors.items():
-        if t.device != device:
+        if t.get_device() != device.index:
             raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
@@ -119,7 +119,7 @@ def _workspace(device: torch.device, nbytes: int, kept: OrderedDict = _WORKSPACE
     caching allocator's pool of the stream it was allocated on, and that pool keeps the block until the cache is
     emptied (torch.cuda.empty_cache). A stream whose handle is reused after the stream is destroyed picks up the old
     entry, which is safe: its counts are zero whenever no call is in flight."""
-    key = (device, torch.cuda.current_stream(device).cuda_stream)
+    key = (device, stream(device))
     ws = kept.pop(key, None)
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)

@@ -207,17 +207,17 @@ def pointer(t) -> int:
     return t.data_ptr()
 
 
-def stream() -> int:
+def stream(device=None) -> int:
     """The current torch stream of the current device (a hipStream_t), which the kernels launch on (reference
-    native.py:47-51). Read through torch's raw-stream getter where it exists, which builds no Stream object (about
-    2 us a call less); torch.cuda.current_stream() otherwise."""
+    native.py:47-51), or of another. Read through torch's raw-stream getter where it exists, which builds no Stream object
+    (about 2 us a call less); torch.cuda.current_stream() otherwise."""
     import torch
 
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     if raw is None:
-        return torch.cuda.current_stream().cuda_stream
+        return torch.cuda.current_stream(device).cuda_stream
     torch.cuda._lazy_init()
-    return raw(torch._C._cuda_getDevice())
+    return raw(torch._C._cuda_getDevice() if device is None or device.index is None else device.index)
 
 
 def device_guard(t):

@@ -63,12 +63,13 @@ class BlockTables:
         if not 0 < rows < 2 ** 31:
             raise ValueError(f"rows must be in [1, 2^31), got {rows}")
         sizes = (self.slots + 1, rows, rows, self.slots)
-        if maps is None:
-            maps = StepMaps(*(torch.empty(n, dtype=torch.int32, device=self.table.device) for n in sizes))
-        for (name, t), n in zip(maps._asdict().items(), sizes):
-            _require(t, name, torch.int32)
-            if t.shape != (n,) or t.device != self.table.device:
-                raise ValueError(f"{name} must be [{n}] on {self.table.device}, got {tuple(t.shape)} on {t.device}")
+        if maps is None:   # one allocation
+            maps = StepMaps(*torch.empty(sum(sizes), dtype=torch.int32, device=self.table.device).split(sizes))
+        else:
+            for (name, t), n in zip(maps._asdict().items(), sizes):
+                _require(t, name, torch.int32)
+                if t.shape != (n,) or t.device != self.table.device:
+                    raise ValueError(f"{name} must be [{n}] on {self.table.device}, got {tuple(t.shape)} on {t.device}")
         with device_guard(self.table):
             check(hip_library().nc_pages_extend(
                 pointer(new_tokens), self.slots, pointer(self.lengths), pointer(self.table), self.max_pages,
