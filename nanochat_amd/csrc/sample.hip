@@ -8,24 +8,27 @@
  *   min-p    of those, the tokens with w_i >= min_p
  *   choice   the first token, in index order, whose running weight exceeds u times the weight of all that are left
  *
- * Weights are integers: exp in float64 (2^x by its Taylor polynomial after splitting off the integer part), times 2^S and
- * rounded. Sums of integers depend on no order, so the LDS histograms may be filled by atomics, and the sums of a row are
- * as exact as its weights (2^-47 of the largest at 65,536 tokens): a border between two tokens moves by less than that
- * share. In float32 a border among many small weights would move by about their size.
+ * Weights are integers: exp in float64 (2^x by a polynomial after splitting off the integer part), times 2^S and rounded.
+ * Sums of integers depend on no order, so the LDS histograms may be filled by atomics, and the sums of a row are as exact as
+ * its weights (2^-47 of the largest at 65,536 tokens): a border between two tokens moves by less than that share. In float32 a
+ * border among many small weights would move by about their size.
  *
  * No sort: the place where a running count (top-k) or weight (top-p) in order of value reaches its target is found by a
  * histogram over ranges of the value, then among the few tokens of the range that holds it, or by finer histograms where it
  * holds many.
  *
- * split_kernel takes rows of up to 262,144 tokens, a workgroup for every 8,192, which stay in its registers. What bounds it
- * is neither bytes nor operations (a row of 65,536 fp32 logits is 256 KiB) but the steps one after the other, each ending
- * where the row's workgroups need one another: the largest logit; the histogram; the list; about 2.5 us a meeting through
- * memory. Greedy rows and a top-k of at most 128 need no meeting: every slice leaves its k largest in order, and the last
- * workgroup to arrive does the rest on k tokens. Measured: one row of 65,536 fp32 logits with top-p 27 us (one workgroup
- * with the row read again for every step: 114), with top-k 15; 128 such rows of mixed settings, a quarter greedy, 35 (89);
- * 333 rows of 32,768 masked bf16 logits with top-p 84 (140), where the workgroups' two a CU come in three rounds.
- * sample_kernel takes longer rows: one workgroup of 16 waves reads the row again for every step, wave w a contiguous run of
- * it, so that a sum in index order is a sum over waves, then over one wave (400,000 tokens with top-p: 680 us).
+ * split_kernel takes up to 512 / ceil(vocab / 8,192) rows of up to 262,144 tokens, a workgroup for every 8,192, which stay
+ * in its registers. What bounds it is neither bytes nor operations (a row of 65,536 fp32 logits is 256 KiB) but the steps one
+ * after the other, each ending where the row's workgroups need one another: the largest logit; the histogram; the list; about
+ * 2.5 us a meeting through memory. Greedy rows and a top-k of at most 128 need no meeting: every slice leaves its k largest in
+ * order, and the last workgroup to arrive does the rest on k tokens. Measured: one row of 65,536 fp32 logits with top-p 27 us,
+ * with top-k 14; 64 rows 39 and 20.
+ *
+ * row_kernel takes a row by one workgroup that reads it again for every step, for more rows and for longer ones. With top-p
+ * it is bound by the exponentials, twice for every token (about 180 cycles of a SIMD for a wave's 64, most of them float64
+ * at half rate): 256 rows of 65,536 tokens 94 us, 333 rows of 32,768 masked bf16 logits, of which 77 wait for a CU, 102. With a
+ * top-k it reads the row twice and the rest is k tokens: 128 rows of 65,536 fp32 logits, a quarter of them greedy, 25 us
+ * (1.3 TB/s of logits).
  */
 #include <math.h>
 
@@ -35,11 +38,6 @@
 namespace nc {
 
 typedef unsigned long long u64;
-
-constexpr int SM_WAVES = 16, SM_THREADS = SM_WAVES * WAVE;
-constexpr int SM_CHUNK = 4 * WAVE;       /* elements of a wave's chunk: four a lane */
-constexpr int SM_BINS = 4 * SM_THREADS;
-constexpr int SM_LIST = SM_THREADS;      /* tokens a range may hold to be settled pairwise */
 
 struct SampleArgs {
     const void *logits;
@@ -52,19 +50,6 @@ struct SampleArgs {
     int32_t *out;
 };
 
-struct SampleShared {
-    u64 hist[SM_BINS];
-    u64 sum[SM_WAVES];
-    u64 found;                           /* a running sum before the range or token that was found */
-    u64 w[SM_LIST], above[SM_LIST], equal[SM_LIST];
-    u64 chunk[16][WAVE];
-    uint32_t key[SM_LIST];
-    int idx[SM_LIST];
-    uint32_t lo, hi;
-    int bin, n, token;
-    uint32_t cut;
-};
-
 /* Order-preserving integer of a float (no NaN, no -0) and back. */
 __device__ __forceinline__ uint32_t order_key(float z) {
     const uint32_t u = __float_as_uint(z);
@@ -74,94 +59,73 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-    for (int o = WAVE / 2; o; o >>= 1) v += __shfl_xor(v, o, WAVE);
-    return v;
-}
-__device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {   /* inclusive */
-#pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) {
-        const u64 t = __shfl_up(v, o, WAVE);
-        if (lane >= o) v += t;
-    }
-    return v;
+/* a b + c with c, a constant, in scalar registers: the compiler would move it into vector registers first, each time. */
+__device__ __forceinline__ double fma_by(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
 }
 
-/* round(2^S 2^x) for x <= 0; x below -100 or NaN: 0. 2^f, |f| <= 1/2, by sum_k (f ln 2)^k / k! up to k = 11, whose rest is
- * below 2^-47 of it. The sum with 2^52 leaves the rounded integer in the low 52 bits (S <= 46). */
+/* round(2^S 2^x) for x <= 0; x below -100 or NaN: 0. 2^f, |f| <= 1/2, by a polynomial of degree 10 fitted for the least
+ * relative error, 2^-52. The sum with 2^52 leaves the rounded integer in the low 52 bits (S <= 46). No branch: elements'
+ * chains run side by side. */
 __device__ __forceinline__ u64 fixed_exp2(double x, int S) {
     x = fmax(x, -100.0);
     const double n = __builtin_rint(x), f = x - n;
-    double p = 4.44553827187081e-10;
-    p = __builtin_fma(p, f, 7.054911620801121e-09);
-    p = __builtin_fma(p, f, 1.0178086009239696e-07);
-    p = __builtin_fma(p, f, 1.3215486790144305e-06);
-    p = __builtin_fma(p, f, 1.5252733804059838e-05);
-    p = __builtin_fma(p, f, 0.00015403530393381606);
-    p = __builtin_fma(p, f, 0.0013333558146428441);
-    p = __builtin_fma(p, f, 0.009618129107628477);
-    p = __builtin_fma(p, f, 0.055504108664821576);
-    p = __builtin_fma(p, f, 0.2402265069591007);
-    p = __builtin_fma(p, f, 0.6931471805599453);
+    double p = fma_by(f, 7.037259617627914e-09, 1.0208538206271505e-07);
+    p = fma_by(p, f, 1.3215662976568588e-06);
+    p = fma_by(p, f, 1.525265811546915e-05);
+    p = fma_by(p, f, 0.00015403529960773235);
+    p = fma_by(p, f, 0.0013333558228561912);
+    p = fma_by(p, f, 0.009618129108034947);
+    p = fma_by(p, f, 0.055504108664458846);
+    p = fma_by(p, f, 0.24022650695908768);
+    p = fma_by(p, f, 0.6931471805599497);
     p = __builtin_fma(p, f, 1.0);
     const double v = __builtin_ldexp(p, (int)n + S) + 0x1p52;
     return (u64)__builtin_bit_cast(long long, v) & 0xFFFFFFFFFFFFFull;
 }
 
-/* One row, read again for each pass. Element j of lane l of chunk c of wave w is index (w per + c) SM_CHUNK + 4 l + j.
- * Elements that are not allowed, and those past the row's end, are -inf. */
-struct Row {
-    const SampleArgs &a;
-    const char *p;
-    const uint32_t *mask;
-    int per, base, lane;
+/* A value that is the same in every lane, as a scalar register's: branches on it are the wave's. */
+__device__ __forceinline__ int alike(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ u64 alike(u64 x) {
+    return (u64)(uint32_t)alike((int)(uint32_t)(x >> 32)) << 32 | (uint32_t)alike((int)(uint32_t)x);
+}
+__device__ __forceinline__ float alike(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 
-    __device__ __forceinline__ Row(const SampleArgs &args, long long row)
-        : a(args), p((const char *)args.logits + row * args.stride * (args.bf16 ? 2 : 4)),
-          mask(args.mask ? args.mask + row * args.mask_stride : nullptr) {
-        per = (a.vocab + SM_WAVES * SM_CHUNK - 1) / (SM_WAVES * SM_CHUNK);
-        lane = threadIdx.x & (WAVE - 1);
-        base = (int)(threadIdx.x >> 6) * per * SM_CHUNK;
+/* What a row's token is chosen by. */
+struct Choice {
+    float T, u, p, zmax;
+    double per_log2;
+    u64 least_w;
+    int S;   /* a weight of 1 is 2^S */
+
+    __device__ __forceinline__ Choice(const SampleArgs &a, long long r, float temperature, float largest)
+        : T(temperature), u(alike(a.uniform[r])), p(a.top_p ? alike(a.top_p[r]) : 1.0f), zmax(largest),
+          per_log2(1.4426950408889634 / (double)temperature) {
+        S = 62;   /* the row's weights sum below 2^62 */
+        while (S > 0 && (1LL << (62 - S)) < a.vocab) S--;
+        S = min(S, 46);
+        const double floor_w = a.min_p ? fmin(fmax((double)alike(a.min_p[r]), 0.0), 1.0) : 0.0;   /* NaN: 0 */
+        least_w = (u64)ceil(__builtin_ldexp(floor_w, S));
     }
-
-    __device__ __forceinline__ int index(int c) const { return base + c * SM_CHUNK + 4 * lane; }
-
-    __device__ __forceinline__ void fetch(int c, float (&x)[4]) const {
-        const int i = index(c);
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = -INFINITY;
-        if (i >= a.vocab) return;
-        if (a.wide && i + 3 < a.vocab) {
-            if (a.bf16) {
-                const uint2 u = *reinterpret_cast<const uint2 *>(p + 2LL * i);
-                x[0] = __uint_as_float(u.x << 16); x[1] = __uint_as_float(u.x & 0xFFFF0000u);
-                x[2] = __uint_as_float(u.y << 16); x[3] = __uint_as_float(u.y & 0xFFFF0000u);
-            } else {
-                const float4 u = *reinterpret_cast<const float4 *>(p + 4LL * i);
-                x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j < a.vocab)
-                    x[j] = a.bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i + j])
-                                  : reinterpret_cast<const float *>(p)[i + j];
-        }
-        const uint32_t allowed = mask ? mask[i >> 5] >> (i & 31) : 0xFu;
-#pragma unroll
-        for (int j = 0; j < 4; j++)   /* NaN fails the comparison; -0 becomes +0, its equal */
-            x[j] = (allowed >> j & 1) && x[j] > -INFINITY ? x[j] + 0.0f : -INFINITY;
+    __device__ __forceinline__ u64 weight(float z) const {
+        /* the largest's equals: 2^S, infinite ones too; -inf: 0 */
+        return fixed_exp2(z == zmax ? 0.0 : ((double)z - (double)zmax) * per_log2, S);
     }
-
-    /* f(c, values) for every chunk of this wave. */
-    template <typename F>
-    __device__ __forceinline__ void each(F &&f) const {
-        for (int c = 0; c < per; c++) {
-            float x[4];
-            fetch(c, x);
-            f(c, x);
-        }
+    /* The nucleus: tokens with less than this above them. */
+    __device__ __forceinline__ u64 mass(u64 total) const {
+        return max((u64)ceil(fmax((double)p, 0.0) * (double)total), 1ull);
+    }
+    /* The first running sum above u total. */
+    __device__ __forceinline__ u64 choice(u64 total) const {
+        const u64 at = u > 0.0f ? (u < 1.0f ? (u64)((double)u * (double)total) : total) : 0ull;
+        return min(at, total - 1) + 1;
+    }
+    /* Values further below the largest than T ln(vocab / (1 - p)) weigh less than 1 - p of it together: the nucleus' border is
+     * not among them, nor 47 log2 units below, where they weigh nothing. The first ranges need not tell them apart. */
+    __device__ __forceinline__ float range(int vocab) const {
+        return T * fminf(__logf((float)vocab / (1.0f - fmaxf(p, 0.0f))), 33.0f);
     }
 };
 
@@ -172,319 +136,6 @@ struct Cut {
     uint32_t key;
     int idx;
 };
-
-/* The bins' sums in order: sh.bin is the first bin at which the running sum reaches target(total), sh.found the sum
- * before it. Returns whether there is one. Every thread must call it. */
-template <typename Target>
-__device__ __forceinline__ bool find_bin(SampleShared &sh, Target target) {
-    const int t = threadIdx.x, lane = t & (WAVE - 1), wave = t >> 6;
-    u64 v[4], own = 0;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        v[k] = sh.hist[4 * t + k];
-        own += v[k];
-    }
-    const u64 scan = wave_scan64(own, lane);
-    if (lane == WAVE - 1) sh.sum[wave] = scan;
-    __syncthreads();
-    u64 before = scan - own, total = 0;
-#pragma unroll
-    for (int w = 0; w < SM_WAVES; w++) {
-        before += w < wave ? sh.sum[w] : 0;
-        total += sh.sum[w];
-    }
-    const u64 goal = target(total);
-    if (before < goal && goal <= before + own) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (before < goal && goal <= before + v[k]) {
-                sh.bin = 4 * t + k;
-                sh.found = before;
-            }
-            before += v[k];
-        }
-    }
-    __syncthreads();
-    return goal <= total;
-}
-
-/* The smallest index whose running sum of m(z, index), in index order, reaches goal(total); -1 without one. Every thread
- * must call it. */
-template <typename M, typename Goal>
-__device__ __forceinline__ int select_in_order(SampleShared &sh, const Row &row, M m, Goal goal) {
-    const int lane = row.lane, wave = threadIdx.x >> 6;
-    u64 s = 0;
-    row.each([&](int c, const float (&x)[4]) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) s += m(x[j], row.index(c) + j);
-    });
-    s = wave_sum64(s);
-    __syncthreads();
-    if (lane == 0) sh.sum[wave] = s;
-    if (threadIdx.x == 0) sh.token = -1;
-    __syncthreads();
-    u64 before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < SM_WAVES; w++) {
-        before += w < wave ? sh.sum[w] : 0;
-        total += sh.sum[w];
-    }
-    const u64 g = goal(total);
-    if (before < g && g <= before + s) {   /* this wave holds it: its chunks, 16 at a time */
-        for (int c0 = 0; c0 < row.per; c0 += 16) {
-#pragma unroll
-            for (int k = 0; k < 16; k++) sh.chunk[k][lane] = 0;
-            row.each([&](int c, const float (&x)[4]) {
-                if (c < c0 || c >= c0 + 16) return;
-                u64 v = 0;
-#pragma unroll
-                for (int j = 0; j < 4; j++) v += m(x[j], row.index(c) + j);
-                sh.chunk[c - c0][lane] = v;
-            });
-            __builtin_amdgcn_wave_barrier();   /* one wave's LDS accesses complete in order */
-            u64 part = 0;                      /* chunk lane / 4: 16 of its lanes, then the four quarters */
-#pragma unroll
-            for (int k = 0; k < 16; k++) part += sh.chunk[lane >> 2][(lane & 3) * 16 + k];
-            part += __shfl_xor(part, 1, WAVE);
-            part += __shfl_xor(part, 2, WAVE);
-            const u64 upto = before + wave_scan64((lane & 3) == 3 ? part : 0, lane);
-            const u64 hit = __ballot((lane & 3) == 3 && upto - part < g && g <= upto);
-            if (!hit) {
-                before = __shfl(upto, WAVE - 1, WAVE);
-                continue;
-            }
-            const int at = __ffsll(hit) - 1, c1 = at >> 2;
-            const u64 base = __shfl(upto - part, at, WAVE);
-            const u64 v = sh.chunk[c1][lane], end = base + wave_scan64(v, lane);
-            row.each([&](int c, const float (&x)[4]) {
-                if (c != c0 + c1 || !(end - v < g && g <= end)) return;
-                u64 run = end - v;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const u64 w = m(x[j], row.index(c) + j);
-                    if (run < g && g <= run + w) sh.token = row.index(c) + j;
-                    run += w;
-                }
-            });
-            break;
-        }
-    }
-    __syncthreads();
-    return sh.token;
-}
-
-/* Over the elements that in(z, index) keeps, in order of value, the larger first: where the running sum of m(z) reaches
- * target(total). SPLIT: equals are taken one by one, the lower index first (m is 1), and the cut's idx is the last one
- * taken; else they are taken together. `range`: the values below zmax - range need no telling apart. Every thread must
- * call it. */
-template <bool SPLIT, typename In, typename M, typename Target>
-__device__ __forceinline__ Cut find_cut(SampleShared &sh, const Row &row, float zmax, float range, In in, M m, Target target) {
-    const int t = threadIdx.x, lane = row.lane, wave = t >> 6;
-    const float scale = range > 0.0f && range < INFINITY ? (SM_BINS - 1) / range : 0.0f;
-    /* a range whose products are NaN or past the last bin: the last bin; monotone in z in every case */
-    const auto bin_of = [&](float z) { return z == zmax ? 0 : (int)fminf((zmax - z) * scale, (float)(SM_BINS - 1)); };
-    const auto clear = [&]() {
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 4; k++) sh.hist[t + k * SM_THREADS] = 0;
-        if (t == 0) sh.n = 0;
-        __syncthreads();
-    };
-    u64 goal = 0;
-    clear();
-    row.each([&](int c, const float (&x)[4]) {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (in(x[j], row.index(c) + j))
-                __hip_atomic_fetch_add(&sh.hist[bin_of(x[j])], m(x[j]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    });
-    const bool some = find_bin(sh, [&](u64 total) { return goal = target(total); });
-    if (!some) return Cut{false, 0u, 0};
-    const int bin = sh.bin;
-    u64 base = sh.found;
-    uint32_t lo = 0u, hi = 0xFFFFFFFFu;   /* once a range of values is split again: its keys */
-    bool keyed = false;
-    for (;;) {
-        const auto member = [&](float z, int i) {
-            if (!in(z, i)) return false;
-            const uint32_t k = order_key(z);
-            return keyed ? k >= lo && k <= hi : bin_of(z) == bin;
-        };
-        row.each([&](int c, const float (&x)[4]) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (member(x[j], row.index(c) + j)) {
-                    const int at = __hip_atomic_fetch_add(&sh.n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                    if (at < SM_LIST) {
-                        sh.key[at] = order_key(x[j]);
-                        sh.idx[at] = row.index(c) + j;
-                        sh.w[at] = m(x[j]);
-                    }
-                }
-        });
-        sh.above[t] = sh.equal[t] = 0;
-        __syncthreads();
-        const int n = sh.n;
-        if (n <= SM_LIST) {   /* pairwise, every token's list split over 1,024 / n threads */
-            int lanes = 1;
-            while (lanes < n) lanes <<= 1;
-            const int i = t & (lanes - 1);
-            if (i < n) {
-                const uint32_t k = sh.key[i];
-                const int id = sh.idx[i];
-                u64 above = 0, equal = 0;
-                for (int j = t / lanes; j < n; j += SM_THREADS / lanes) {
-                    const uint32_t kj = sh.key[j];
-                    const u64 w = sh.w[j];
-                    above += kj > k || (SPLIT && kj == k && sh.idx[j] < id) ? w : 0;
-                    equal += !SPLIT && kj == k ? w : 0;
-                }
-                __hip_atomic_fetch_add(&sh.above[i], above, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                if (!SPLIT) __hip_atomic_fetch_add(&sh.equal[i], equal, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            }
-            __syncthreads();
-            if (t < n) {
-                const u64 above = base + sh.above[t], own = SPLIT ? sh.w[t] : sh.equal[t];
-                if (above < goal && goal <= above + own) {   /* one token, or one value's equals, who write the same */
-                    sh.cut = sh.key[t];
-                    sh.token = SPLIT ? sh.idx[t] : 0x7FFFFFFF;
-                }
-            }
-            __syncthreads();
-            return Cut{true, sh.cut, sh.token};
-        }
-        if (!keyed) {   /* the least and largest key of the range */
-            uint32_t least = 0xFFFFFFFFu, most = 0u;
-            row.each([&](int c, const float (&x)[4]) {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (member(x[j], row.index(c) + j)) {
-                        least = min(least, order_key(x[j]));
-                        most = max(most, order_key(x[j]));
-                    }
-            });
-            __syncthreads();
-            if (t == 0) sh.lo = 0xFFFFFFFFu, sh.hi = 0u;
-            __syncthreads();
-            __hip_atomic_fetch_min(&sh.lo, least, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            __hip_atomic_fetch_max(&sh.hi, most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            __syncthreads();
-            lo = sh.lo;
-            hi = sh.hi;
-            keyed = true;
-        }
-        if (lo == hi) {   /* one value */
-            int idx = 0x7FFFFFFF;
-            if (SPLIT) {
-                const u64 rest = goal - base;
-                idx = select_in_order(sh, row, [&](float z, int i) { return (u64)(in(z, i) && order_key(z) == lo); },
-                                      [&](u64) { return rest; });
-            }
-            return Cut{true, lo, idx};
-        }
-        int shift = 0;
-        while ((hi - lo) >> shift >= SM_BINS) shift++;
-        clear();
-        row.each([&](int c, const float (&x)[4]) {   /* the larger keys first */
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (member(x[j], row.index(c) + j))
-                    __hip_atomic_fetch_add(&sh.hist[(hi - order_key(x[j])) >> shift], m(x[j]), __ATOMIC_RELAXED,
-                                           __HIP_MEMORY_SCOPE_WORKGROUP);
-        });
-        const u64 rest = goal - base;
-        find_bin(sh, [&](u64) { return rest; });
-        base += sh.found;
-        const uint32_t top = hi - ((uint32_t)sh.bin << shift);
-        const uint32_t span = (1u << shift) - 1u;
-        lo = top - lo > span ? top - span : lo;
-        hi = top;
-    }
-}
-
-__global__ void __launch_bounds__(SM_THREADS) sample_kernel(SampleArgs a) {
-    __shared__ SampleShared sh;
-    const long long r = blockIdx.x;
-    const int t = threadIdx.x, lane = t & (WAVE - 1), wave = t >> 6;
-    const Row row(a, r);
-
-    /* the largest allowed logit (the lowest index among equals) and the smallest */
-    u64 best = 0;
-    float least = INFINITY;
-    row.each([&](int c, const float (&x)[4]) {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (x[j] > -INFINITY) {
-                best = max(best, (u64)order_key(x[j]) << 32 | (0xFFFFFFFFu - (uint32_t)(row.index(c) + j)));
-                least = fminf(least, x[j]);
-            }
-    });
-#pragma unroll
-    for (int o = WAVE / 2; o; o >>= 1) {
-        best = max(best, (u64)__shfl_xor(best, o, WAVE));
-        least = fminf(least, __shfl_xor(least, o, WAVE));
-    }
-    if (lane == 0) {
-        sh.sum[wave] = best;
-        sh.idx[wave] = (int)__float_as_uint(least);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < SM_WAVES; w++) {
-        best = max(best, sh.sum[w]);
-        least = fminf(least, __uint_as_float((uint32_t)sh.idx[w]));
-    }
-    const float T = a.temperature[r];
-    if (best == 0 || !(T > 0.0f)) {   /* nothing allowed; or the largest logit */
-        if (t == 0) a.out[r] = best == 0 ? -1 : (int)(0xFFFFFFFFu - (uint32_t)best);
-        return;
-    }
-
-    const float zmax = key_value((uint32_t)(best >> 32));
-    const double zmaxd = zmax, per_log2 = 1.4426950408889634 / (double)T;
-    int S = 62;   /* the row's weights sum below 2^62 */
-    while (S > 0 && (1LL << (62 - S)) < a.vocab) S--;
-    S = min(S, 46);
-    const auto weight = [&](float z) {
-        return z == zmax ? 1ull << S : z == -INFINITY ? 0ull : fixed_exp2(((double)z - zmaxd) * per_log2, S);
-    };
-
-    Cut top = {false, 0u, 0};
-    const int k = a.top_k ? a.top_k[r] : 0;
-    if (k > 0 && k < a.vocab)
-        top = find_cut<true>(sh, row, zmax, zmax - least, [&](float z, int) { return z > -INFINITY; },
-                             [&](float) { return 1ull; }, [&](u64) { return (u64)k; });
-    const float top_z = top.some ? key_value(top.key) : -INFINITY;
-    const auto ranked = [&](float z, int i) {   /* among the k largest */
-        return z > top_z || (top.some && z == top_z && i <= top.idx);
-    };
-
-    float least_z = -INFINITY;   /* the nucleus' smallest logit */
-    const float p = a.top_p ? a.top_p[r] : 1.0f;
-    if (p < 1.0f) {
-        /* values 47 log2 units below the largest weigh nothing: one bin for them all */
-        const Cut mass = find_cut<false>(sh, row, zmax, fminf(zmax - least, 33.0f * T), ranked, weight, [&](u64 total) {
-            return max((u64)ceil(fmax((double)p, 0.0) * (double)total), 1ull);
-        });
-        if (mass.some) least_z = key_value(mass.key);
-    }
-    const double floor_w = a.min_p ? fmin(fmax((double)a.min_p[r], 0.0), 1.0) : 0.0;   /* NaN: 0 */
-    const u64 least_w = (u64)ceil(__builtin_ldexp(floor_w, S));
-    const float u = a.uniform[r];
-    const int token = select_in_order(
-        sh, row,
-        [&](float z, int i) {
-            if (!(z >= least_z && ranked(z, i))) return 0ull;
-            const u64 w = weight(z);
-            return w >= least_w ? w : 0ull;
-        },
-        [&](u64 total) {   /* the first running sum above u total */
-            const u64 at = u > 0.0f ? (u < 1.0f ? (u64)((double)u * (double)total) : total) : 0ull;
-            return min(at, total - 1) + 1;
-        });
-    if (t == 0) a.out[r] = token;
-}
 
 /* --- Rows of up to ST_MAX_GROUPS slices of 8,192 tokens, a workgroup each: the slice stays in its registers, 16 tokens a
  * thread, and the workgroups of a row exchange what the next step needs through memory. 512 threads of at most 128 registers
@@ -502,7 +153,7 @@ constexpr int ST_TOP = 128;               /* the largest top-k settled by lists 
 constexpr int ST_CAND = 4096;             /* candidates: at most ST_TOP of 32 tokens, or of ST_MAX_GROUPS lists */
 constexpr int ST_LINE = 32;               /* ints of a 128-byte line: counts that several workgroups add to share none */
 constexpr int ST_QUEUES = 8;              /* XCDs */
-constexpr int ST_MAX_WORKGROUPS = 2048;   /* of one launch, when rows are cut: bounds the workspace */
+constexpr int ST_MAX_WORKGROUPS = 512;    /* of rows that are cut: as many as run at once, two a CU */
 static_assert(ST_TOP * (ST_SLICE / 256) <= ST_CAND && ST_TOP * ST_MAX_GROUPS <= ST_CAND, "candidates fit");
 
 enum { HD_BEST, HD_COUNT, HD_ABOVE, HD_LEAST, HD_MOST, HD_SUM, HD_WORDS };
@@ -510,8 +161,7 @@ constexpr int ST_PART = ST_BINS + 2 * ST_LIST + HD_WORDS;   /* words a workgroup
 
 struct SplitArgs {
     SampleArgs a;
-    long long row0;
-    int rows, groups;      /* of this launch; slices a row */
+    int rows, groups;      /* slices a row */
     u64 *part;             /* [rows][groups][ST_PART] */
     int *tickets, *done, *count;   /* [ST_QUEUES], [ST_QUEUES], [rows] lines; zero between launches */
 };
@@ -552,13 +202,6 @@ __device__ __forceinline__ void publish(u64 *p, u64 v) {
 __device__ __forceinline__ u64 peek(const u64 *p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-
-/* A value that is the same in every lane, as a scalar register's: branches on it are the wave's. */
-__device__ __forceinline__ int alike(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ u64 alike(u64 x) {
-    return (u64)(uint32_t)alike((int)(uint32_t)(x >> 32)) << 32 | (uint32_t)alike((int)(uint32_t)x);
-}
-__device__ __forceinline__ float alike(float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); }
 
 /* Inclusive sums over the lanes by DPP: shifts by 1, 2, 4 and 8 within rows of 16 lanes, then a row's last sum added to the
  * next row's, and the lower half's to the upper's. */
@@ -625,7 +268,7 @@ struct Split {
     const SplitArgs &s;
     SplitShared &sh;
     int t, lane, wave;
-    int row, g, G;         /* row of this launch, slice, slices */
+    int row, g, G;         /* row, slice, slices */
     int first;             /* index of this thread's element 0 */
     int reached;           /* arrivals that the last wait of this row asked for */
     u64 *mine;
@@ -724,11 +367,12 @@ __device__ __forceinline__ void split_load(const Split &q, const SampleArgs &a, 
         x[e] = (allowed >> e & 1) && x[e] > -INFINITY ? x[e] + 0.0f : -INFINITY;
 }
 
-/* The `want` largest of the n codes of sh.cand, in order, in sh.top; returns how many. Every thread must call it, after a
- * __syncthreads. */
-__device__ __forceinline__ int split_sort(SplitShared &sh, int n, int want) {
+/* The `want` largest of the n codes of sh.cand, in order, in sh.top; returns how many. Every one of THREADS threads must call
+ * it, after a __syncthreads. */
+template <int THREADS, typename Shared>
+__device__ __forceinline__ int sort_codes(Shared &sh, int n, int want) {
     const int t = threadIdx.x;
-    if (n <= ST_THREADS) {   /* a code's comparisons spread over 512 / n threads */
+    if (n <= THREADS) {   /* a code's comparisons spread over THREADS / n threads */
         int lanes = 1;
         while (lanes < n) lanes <<= 1;
         sh.rank[t] = 0;
@@ -738,13 +382,13 @@ __device__ __forceinline__ int split_sort(SplitShared &sh, int n, int want) {
             const u64 c = sh.cand[i];
             int above = 0;
 #pragma unroll 4
-            for (int j = t / lanes; j < n; j += ST_THREADS / lanes) above += sh.cand[j] > c;
+            for (int j = t / lanes; j < n; j += THREADS / lanes) above += sh.cand[j] > c;
             __hip_atomic_fetch_add(&sh.rank[i], above, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
         __syncthreads();
         if (t < n && sh.rank[t] < want) sh.top[sh.rank[t]] = sh.cand[t];
     } else {
-        for (int i = t; i < n; i += ST_THREADS) {
+        for (int i = t; i < n; i += THREADS) {
             const u64 c = sh.cand[i];
             int above = 0;
             for (int j = 0; j < n && above < want; j++) above += sh.cand[j] > c;
@@ -753,6 +397,73 @@ __device__ __forceinline__ int split_sort(SplitShared &sh, int n, int want) {
     }
     __syncthreads();
     return min(n, want);
+}
+
+/* By one wave: a code that k of the 256 maxima of sh.most reach (0: a group without a token), by bisection k to k + 8 of
+ * them, but at most ST_TOP; 1 if fewer than k groups have a token. */
+template <typename Shared>
+__device__ __forceinline__ u64 least_of_top(const Shared &sh, int lane, int k) {
+    u64 m[4], hi = 0, none = ~0ull;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        m[j] = sh.most[j * WAVE + lane];
+        hi = max(hi, m[j]);
+        none = min(none, m[j] - 1);   /* a group without a token: the largest */
+    }
+    const auto reach = [&](u64 code) {
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) n += __popcll(__ballot(m[j] >= code));
+        return n;
+    };
+    hi = lane_max64(hi);
+    const int most = min(k + 8, ST_TOP);
+    u64 lo = ~lane_max64(~none) + 1;   /* the least of the maxima */
+    if (lo == 0 || reach(lo) < k) lo = 1;
+    for (int n = reach(lo); n > most && lo < hi;) {
+        const u64 mid = lo + (hi - lo + 1) / 2;
+        const int of = reach(mid);
+        if (of >= k) {
+            lo = mid;
+            n = of;
+        } else {
+            hi = mid - 1;
+        }
+    }
+    return lo;
+}
+
+/* The choice among the n <= ST_TOP tokens of sh.top, in order of value: top-p, min-p, then the first in index order at which
+ * the running weight reaches its goal. Every thread must call it, after a __syncthreads. */
+template <typename Shared, typename Weight, typename Goal, typename Choice>
+__device__ __forceinline__ void choose_top(Shared &sh, int n, Weight weight, bool nucleus, Goal mass_goal, u64 least_w,
+                                           Choice choice, int32_t *out) {
+    const int t = threadIdx.x;
+    if (t < n) sh.top_w[t] = weight(key_value((uint32_t)(sh.top[t] >> 32)));
+    __syncthreads();
+    if (t < n) {
+        const u64 c = sh.top[t];
+        u64 more = 0, total = 0;
+        for (int j = 0; j < n; j++) {
+            const u64 w = sh.top_w[j];
+            more += sh.top[j] >> 32 > c >> 32 ? w : 0;
+            total += w;
+        }
+        const u64 w = sh.top_w[t];
+        sh.kept_w[t] = w >= least_w && (!nucleus || more < mass_goal(total)) ? w : 0;
+    }
+    __syncthreads();
+    if (t < n) {
+        const int idx = code_index(sh.top[t]);
+        u64 before = 0, total = 0;
+        for (int j = 0; j < n; j++) {
+            const u64 w = sh.kept_w[j];
+            before += code_index(sh.top[j]) < idx ? w : 0;
+            total += w;
+        }
+        const u64 goal = choice(total);
+        if (before < goal && goal <= before + sh.kept_w[t]) *out = idx;
+    }
 }
 
 /* Adds `v` to the candidates if `take`. */
@@ -783,35 +494,9 @@ __device__ __forceinline__ int split_top(const Split &q, float (&x)[ST_E], int k
     if (t == 0) sh.n = 0;
     if ((t & 1) == 0) sh.most[t >> 1] = best;
     __syncthreads();
-    if (q.wave == 0) {   /* by bisection, to k to k + 8 of the maxima, but at most ST_TOP */
-        u64 m[4], hi = 0, none = ~0ull;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            m[j] = sh.most[j * WAVE + q.lane];
-            hi = max(hi, m[j]);
-            none = min(none, m[j] - 1);   /* a group without a token: the largest */
-        }
-        const auto reach = [&](u64 code) {
-            int n = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) n += __popcll(__ballot(m[j] >= code));
-            return n;
-        };
-        hi = lane_max64(hi);
-        const int most = min(k + 8, ST_TOP);
-        u64 lo = ~lane_max64(~none) + 1;   /* the least of the maxima */
-        if (lo == 0 || reach(lo) < k) lo = 1;
-        for (int n = reach(lo); n > most && lo < hi;) {
-            const u64 mid = lo + (hi - lo + 1) / 2;
-            const int of = reach(mid);
-            if (of >= k) {
-                lo = mid;
-                n = of;
-            } else {
-                hi = mid - 1;
-            }
-        }
-        if (q.lane == 0) sh.least_code = lo;
+    if (q.wave == 0) {
+        const u64 least = least_of_top(sh, q.lane, k);
+        if (q.lane == 0) sh.least_code = least;
     }
     __syncthreads();
     const u64 least = sh.least_code;
@@ -828,7 +513,7 @@ __device__ __forceinline__ int split_top(const Split &q, float (&x)[ST_E], int k
         }
     }
     __syncthreads();
-    return split_sort(sh, alike(sh.n), k);
+    return sort_codes<ST_THREADS>(sh, alike(sh.n), k);
 }
 
 /* The smallest of this slice's tokens, in index order, whose running sum of m(e), over the elements of the set `in`, reaches
@@ -866,7 +551,7 @@ __device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 
     return sh.token;
 }
 
-/* find_cut over the slices of a row: where the running sum of m(e), over the elements of the sets `live`, the larger value
+/* Over the slices of a row: where the running sum of m(e), over the elements of the sets `live`, the larger value
  * first, reaches target(total). Ranges of values are narrowed by histograms, which the workgroups publish and each adds up,
  * until the tokens of the one that holds the cut fit a list, which each settles pairwise. Between two histograms, and between
  * two lists, there is always a meeting after the first is read. sh.kept: per slice the weight of the tokens down to the cut
@@ -1143,27 +828,16 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     q.reached = 0;
     q.mine = q.part(q.g);
     const int t = q.t, lane = q.lane, wave = q.wave, G = q.G;
-    const long long r = s.row0 + q.row;
+    const long long r = q.row;
     float x[ST_E];
     split_load(q, a, r, x);
-    const float T = alike(a.temperature[r]), u = alike(a.uniform[r]), p = a.top_p ? alike(a.top_p[r]) : 1.0f;
+    const float T = alike(a.temperature[r]);
     const bool greedy = !(T > 0.0f);
     const int k = greedy ? 1 : a.top_k ? alike(a.top_k[r]) : 0;
-    const double floor_w = a.min_p ? fmin(fmax((double)alike(a.min_p[r]), 0.0), 1.0) : 0.0;   /* NaN: 0 */
-    const double per_log2 = 1.4426950408889634 / (double)T;
-    int S = 62;   /* the row's weights sum below 2^62 */
-    while (S > 0 && (1LL << (62 - S)) < a.vocab) S--;
-    S = min(S, 46);
-    const u64 least_w = (u64)ceil(__builtin_ldexp(floor_w, S));
-    const auto mass_goal = [&](u64 total) { return max((u64)ceil(fmax((double)p, 0.0) * (double)total), 1ull); };
-    const auto choice = [&](u64 total) {   /* the first running sum above u total */
-        const u64 at = u > 0.0f ? (u < 1.0f ? (u64)((double)u * (double)total) : total) : 0ull;
-        return min(at, total - 1) + 1;
-    };
-    float zmax = 0.0f;
-    const auto weight = [&](float z) {
-        return z == zmax ? 1ull << S : z == -INFINITY ? 0ull : fixed_exp2(((double)z - (double)zmax) * per_log2, S);
-    };
+    Choice with(a, r, T, 0.0f);
+    const auto weight = [&](float z) { return with.weight(z); };
+    const auto mass_goal = [&](u64 total) { return with.mass(total); };
+    const auto choice = [&](u64 total) { return with.choice(total); };
 
     if (k > 0 && k <= ST_TOP) {
         __syncthreads();   /* sh.n held the ticket */
@@ -1199,39 +873,15 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
                     split_collect(sh, c, c >= least);
                 }
             __syncthreads();
-            n = alike(split_sort(sh, alike(sh.n), k));
+            n = alike(sort_codes<ST_THREADS>(sh, alike(sh.n), k));
             q.leave(true);
         }
         if (n == 0 || k == 1) {
             if (t == 0) a.out[r] = n == 0 ? -1 : code_index(sh.top[0]);
             return;
         }
-        zmax = key_value((uint32_t)(sh.top[0] >> 32));
-        if (t < n) sh.top_w[t] = weight(key_value((uint32_t)(sh.top[t] >> 32)));
-        __syncthreads();
-        if (t < n) {
-            const u64 c = sh.top[t];
-            u64 more = 0, total = 0;
-            for (int j = 0; j < n; j++) {
-                const u64 w = sh.top_w[j];
-                more += sh.top[j] >> 32 > c >> 32 ? w : 0;
-                total += w;
-            }
-            const u64 w = sh.top_w[t];
-            sh.kept_w[t] = w >= least_w && (!(p < 1.0f) || more < mass_goal(total)) ? w : 0;
-        }
-        __syncthreads();
-        if (t < n) {
-            const int idx = code_index(sh.top[t]);
-            u64 before = 0, total = 0;
-            for (int j = 0; j < n; j++) {
-                const u64 w = sh.kept_w[j];
-                before += code_index(sh.top[j]) < idx ? w : 0;
-                total += w;
-            }
-            const u64 goal = choice(total);
-            if (before < goal && goal <= before + sh.kept_w[t]) a.out[r] = idx;
-        }
+        with.zmax = key_value((uint32_t)(sh.top[0] >> 32));
+        choose_top(sh, n, weight, with.p < 1.0f, mass_goal, with.least_w, choice, a.out + r);
         return;
     }
 
@@ -1270,14 +920,14 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
         q.leave(false);
         return;
     }
-    zmax = most;
+    with.zmax = most;
     anew(x);
 
     if (k > 0 && k < a.vocab) {
         uint32_t live = 0;
 #pragma unroll
         for (int e = 0; e < ST_E; e++) live |= (uint32_t)(x[e] > -INFINITY) << e;
-        const Cut top = split_cut<true>(q, x, live, zmax, zmax - least, 0ull,
+        const Cut top = split_cut<true>(q, x, live, with.zmax, with.zmax - least, 0ull,
                                         [&](u64) { return (u64)k; });
         if (top.some) {
             const float z = key_value(top.key);
@@ -1296,18 +946,16 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
         if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);   /* four at a time: more would need more registers */
     }
     float least_z = -INFINITY;   /* the nucleus' smallest logit */
-    if (p < 1.0f) {
-        /* Values further below the largest than T ln(vocab / (1 - p)) weigh less than 1 - p of it together: the cut is not
-         * among them, nor 47 log2 units below, where they weigh nothing. The first ranges need not tell them apart. */
-        const float range = T * fminf(__logf((float)a.vocab / (1.0f - fmaxf(p, 0.0f))), 33.0f);
-        const Cut mass = split_cut<false>(q, x, live, zmax, fminf(zmax - least, range), least_w, mass_goal);
+    if (with.p < 1.0f) {
+        const Cut mass = split_cut<false>(q, x, live, with.zmax, fminf(with.zmax - least, with.range(a.vocab)), with.least_w,
+                                          mass_goal);
         if (mass.some) least_z = key_value(mass.key);
     } else {
         u64 own = 0;
 #pragma unroll
         for (int e = 0; e < ST_E; e++) {
             const u64 v = sh.weight[e * ST_THREADS + t];
-            own += v >= least_w ? v : 0;
+            own += v >= with.least_w ? v : 0;
         }
         own = lane_sum64(own);
         if (lane == 0) sh.sum[wave] = own;
@@ -1335,22 +983,406 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     if (alike((int)(before < goal && goal <= before + ours))) {
         uint32_t kept = 0;
 #pragma unroll
-        for (int e = 0; e < ST_E; e++) kept |= (uint32_t)(x[e] >= least_z && sh.weight[e * ST_THREADS + t] >= least_w) << e;
+        for (int e = 0; e < ST_E; e++) kept |= (uint32_t)(x[e] >= least_z && sh.weight[e * ST_THREADS + t] >= with.least_w) << e;
         const int token = split_pick(q, kept, [&](int e) { return sh.weight[e * ST_THREADS + t]; }, goal - before);
         if (t == 0) a.out[r] = token;
     }
     q.leave(false);
 }
 
+/* --- Rows by one workgroup each, read again for every step: where rows are many, or longer than the slices allow. Wave w
+ * takes a contiguous run of the row, so that a sum in index order is a sum over waves, then over one wave. */
+
+constexpr int RW_WAVES = 16, RW_THREADS = RW_WAVES * WAVE;
+constexpr int RW_CHUNK = 4 * WAVE;       /* elements of a wave's chunk: four a lane */
+constexpr int RW_AHEAD = 4;              /* chunks in flight */
+constexpr int RW_BINS = 4 * RW_THREADS;
+constexpr int RW_LIST = 512;             /* tokens a range may hold to be settled pairwise */
+
+struct RowShared {
+    union {
+        u64 hist[RW_BINS];
+        u64 cand[ST_CAND];
+    };
+    u64 top[ST_TOP], top_w[ST_TOP], kept_w[ST_TOP], most[256];
+    int rank[RW_THREADS];
+    u64 code[RW_LIST], w[RW_LIST];
+    u64 sum[RW_WAVES];
+    u64 found, least_code, lo, hi;
+    int bin, n, token;
+};
+
+/* Element j of lane l of chunk c of wave w is index (w per + c) RW_CHUNK + 4 l + j. */
+struct Row {
+    const SampleArgs &a;
+    const char *p;
+    const uint32_t *mask;
+    int per, base, lane;
+
+    __device__ __forceinline__ Row(const SampleArgs &args, long long row)
+        : a(args), p((const char *)args.logits + row * args.stride * (args.bf16 ? 2 : 4)),
+          mask(args.mask ? args.mask + row * args.mask_stride : nullptr) {
+        per = (a.vocab + RW_WAVES * RW_CHUNK - 1) / (RW_WAVES * RW_CHUNK);
+        lane = threadIdx.x & (WAVE - 1);
+        base = alike((int)(threadIdx.x >> 6)) * per * RW_CHUNK;
+    }
+
+    __device__ __forceinline__ int index(int c, int j) const { return base + c * RW_CHUNK + 4 * lane + j; }
+
+    /* Chunks c .. c + 3. Elements that are not allowed, those past the row's end and those of the next wave are -inf. */
+    __device__ __forceinline__ void fetch(int c, float (&x)[4 * RW_AHEAD]) const {
+        uint32_t allowed = 0xFFFFu;
+        if (mask) {
+            allowed = 0;
+#pragma unroll
+            for (int k = 0; k < RW_AHEAD; k++) {
+                const int i = min(index(c + k, 0), a.vocab - 1) & ~3;
+                allowed |= (mask[i >> 5] >> (i & 31) & 0xFu) << (4 * k);
+            }
+        }
+        if (a.wide && c + RW_AHEAD <= per && base + (c + RW_AHEAD) * RW_CHUNK <= a.vocab) {
+            if (a.bf16) {
+                uint2 u[RW_AHEAD];
+#pragma unroll
+                for (int k = 0; k < RW_AHEAD; k++) u[k] = *reinterpret_cast<const uint2 *>(p + 2LL * index(c + k, 0));
+#pragma unroll
+                for (int k = 0; k < RW_AHEAD; k++) {
+                    x[4 * k] = __uint_as_float(u[k].x << 16); x[4 * k + 1] = __uint_as_float(u[k].x & 0xFFFF0000u);
+                    x[4 * k + 2] = __uint_as_float(u[k].y << 16); x[4 * k + 3] = __uint_as_float(u[k].y & 0xFFFF0000u);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < RW_AHEAD; k++) {
+                    const float4 u = *reinterpret_cast<const float4 *>(p + 4LL * index(c + k, 0));
+                    x[4 * k] = u.x; x[4 * k + 1] = u.y; x[4 * k + 2] = u.z; x[4 * k + 3] = u.w;
+                }
+            }
+        } else {
+            const int end = min(base + per * RW_CHUNK, a.vocab);
+#pragma unroll
+            for (int e = 0; e < 4 * RW_AHEAD; e++) {
+                const int i = index(c + e / 4, e % 4), at = min(i, a.vocab - 1);
+                x[e] = a.bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[at]) : reinterpret_cast<const float *>(p)[at];
+                allowed &= ~((uint32_t)(i >= end) << e);
+            }
+        }
+        if (allowed != 0xFFFFu)
+#pragma unroll
+            for (int e = 0; e < 4 * RW_AHEAD; e++)   /* not allowed: NaN */
+                x[e] = __int_as_float(__float_as_int(x[e]) | ~((int)(allowed << (31 - e)) >> 31));
+#pragma unroll
+        for (int e = 0; e < 4 * RW_AHEAD; e++)   /* NaN fails the comparison; -0 becomes +0, its equal */
+            x[e] = (x[e] > -INFINITY ? x[e] : -INFINITY) + 0.0f;
+    }
+
+    /* f(value, index) for every element of this wave. */
+    template <typename F>
+    __device__ __forceinline__ void each(F &&f) const {
+        for (int c = 0; c < per; c += RW_AHEAD) {
+            float x[4 * RW_AHEAD];
+            fetch(c, x);
+#pragma unroll
+            for (int e = 0; e < 4 * RW_AHEAD; e++) f(x[e], index(c + e / 4, e % 4));
+        }
+    }
+};
+
+/* The bins' sums in order: sh.bin is the first bin at which the running sum reaches target(total), sh.found the sum
+ * before it. Returns whether there is one. Every thread must call it. */
+template <typename Target>
+__device__ __forceinline__ bool row_bin(RowShared &sh, Target target) {
+    const int t = threadIdx.x, lane = t & (WAVE - 1), wave = t >> 6;
+    u64 v[4], own = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        v[k] = sh.hist[4 * t + k];
+        own += v[k];
+    }
+    const u64 scan = lane_scan64(own);
+    if (lane == WAVE - 1) sh.sum[wave] = scan;
+    __syncthreads();
+    u64 before = scan - own, total = 0;
+#pragma unroll
+    for (int w = 0; w < RW_WAVES; w++) {
+        before += w < wave ? sh.sum[w] : 0;
+        total += sh.sum[w];
+    }
+    const u64 goal = target(total);
+    if (before < goal && goal <= before + own) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (before < goal && goal <= before + v[k]) {
+                sh.bin = 4 * t + k;
+                sh.found = before;
+            }
+            before += v[k];
+        }
+    }
+    __syncthreads();
+    return alike((int)(goal <= total));
+}
+
+/* Over the elements that in(z, index) keeps, in order of value, the larger first: where the running sum of m(z) reaches
+ * target(total). SPLIT: equals are taken one by one, the lower index first (m is 1), and the cut's idx is the last one
+ * taken; else they are taken together. `range`: the values below zmax - range need no telling apart. Every thread must
+ * call it. */
+template <bool SPLIT, typename In, typename M, typename Target>
+__device__ __forceinline__ Cut row_cut(RowShared &sh, const Row &row, float zmax, float range, In in, M m, Target target) {
+    const int t = threadIdx.x, lane = row.lane, wave = t >> 6;
+    const float scale = range > 0.0f && range < INFINITY ? (RW_BINS - 1) / range : 0.0f;
+    /* a range whose products are NaN or past the last bin: the last bin; monotone in z in every case */
+    const auto bin_of = [&](float z) { return z == zmax ? 0 : (int)fminf((zmax - z) * scale, (float)(RW_BINS - 1)); };
+    const auto key = [&](float z, int i) { return SPLIT ? token_code(z, i) : (u64)order_key(z); };
+    const auto clear = [&]() {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; k++) sh.hist[t + k * RW_THREADS] = 0;
+        if (t == 0) {
+            sh.n = 0;
+            sh.least_code = sh.lo = ~0ull;
+            sh.hi = 0;
+        }
+        __syncthreads();
+    };
+    u64 goal = 0;
+    clear();
+    u64 rest = 0;   /* of the last bin: many may be past the range */
+    row.each([&](float z, int i) {
+        const u64 w = in(z, i) ? m(z) : 0;
+        const int b = bin_of(z);
+        if (b < RW_BINS - 1)
+            __hip_atomic_fetch_add(&sh.hist[b], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        rest += b == RW_BINS - 1 ? w : 0;
+    });
+    rest = lane_sum64(rest);
+    if (lane == 0) __hip_atomic_fetch_add(&sh.hist[RW_BINS - 1], rest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (!row_bin(sh, [&](u64 total) { return goal = target(total); })) return Cut{false, 0u, 0};
+    const int bin = alike(sh.bin);
+    u64 base = sh.found, lo = 0, hi = ~0ull;   /* once a range of values is split again: its keys */
+    bool keyed = false;
+    for (;;) {
+        const auto member = [&](float z, int i) {
+            if (!in(z, i)) return false;
+            if (!keyed) return bin_of(z) == bin;
+            const u64 k = key(z, i);
+            return k >= lo && k <= hi;
+        };
+        row.each([&](float z, int i) {
+            if (member(z, i)) {
+                const int at = __hip_atomic_fetch_add(&sh.n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (at < RW_LIST) {
+                    sh.code[at] = token_code(z, i);
+                    sh.w[at] = m(z);
+                }
+            }
+        });
+        __syncthreads();
+        const int n = alike(sh.n);
+        if (n <= RW_LIST) {   /* pairwise, up to 16 neighbours a token */
+            int parts = 16;
+            while (parts > 2 && parts * n > RW_THREADS) parts >>= 1;
+            const int i = t / parts;
+            const u64 c = i < n ? sh.code[i] : ~0ull;
+            u64 more = 0;
+#pragma unroll 4
+            for (int j = t % parts; j < n; j += parts)
+                more += (SPLIT ? sh.code[j] > c : (uint32_t)(sh.code[j] >> 32) > (uint32_t)(c >> 32)) ? sh.w[j] : 0;
+            for (int o = 1; o < parts; o <<= 1) more += (u64)__shfl_xor(more, o, WAVE);
+            /* the cut is the last that less than the goal lies above */
+            if (i < n && t % parts == 0 && base + more < goal)
+                __hip_atomic_fetch_min(&sh.least_code, c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            __syncthreads();
+            const u64 last = sh.least_code;
+            return Cut{true, (uint32_t)(last >> 32), SPLIT ? code_index(last) : 0x7FFFFFFF};
+        }
+        if (!keyed) {   /* the least and largest key of the range */
+            u64 least = ~0ull, most = 0;
+            row.each([&](float z, int i) {
+                if (member(z, i)) {
+                    least = min(least, key(z, i));
+                    most = max(most, key(z, i));
+                }
+            });
+            least = ~lane_max64(~least);
+            most = lane_max64(most);
+            if (lane == 0) {
+                __hip_atomic_fetch_min(&sh.lo, least, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                __hip_atomic_fetch_max(&sh.hi, most, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+            __syncthreads();
+            lo = alike(sh.lo);
+            hi = alike(sh.hi);
+            keyed = true;
+        }
+        if (!SPLIT && lo == hi) return Cut{true, (uint32_t)lo, 0x7FFFFFFF};   /* one value */
+        int shift = 0;
+        while ((hi - lo) >> shift >= RW_BINS) shift++;
+        clear();
+        row.each([&](float z, int i) {   /* the larger keys first */
+            if (member(z, i))
+                __hip_atomic_fetch_add(&sh.hist[(hi - key(z, i)) >> shift], m(z), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_WORKGROUP);
+        });
+        const u64 still = goal - base;
+        row_bin(sh, [&](u64) { return still; });
+        base += sh.found;
+        const u64 top = hi - ((u64)alike(sh.bin) << shift), span = (1ull << shift) - 1;
+        lo = top - lo > span ? top - span : lo;
+        hi = top;
+    }
+}
+
+/* The first element in index order at which the running sum of m(z, index) reaches goal(total). Every thread must call it. */
+template <typename M, typename Goal>
+__device__ __forceinline__ int row_pick(RowShared &sh, const Row &row, M m, Goal goal) {
+    const int lane = row.lane, wave = threadIdx.x >> 6;
+    u64 s = 0;
+    row.each([&](float z, int i) { s += m(z, i); });
+    s = lane_sum64(s);
+    __syncthreads();
+    if (lane == 0) sh.sum[wave] = s;
+    __syncthreads();
+    u64 before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < RW_WAVES; w++) {
+        before += w < wave ? sh.sum[w] : 0;
+        total += sh.sum[w];
+    }
+    const u64 g = goal(total);
+    if (alike((int)(before < g && g <= before + s))) {   /* this wave holds it */
+        for (int c = 0; c < row.per; c += RW_AHEAD) {
+            float x[4 * RW_AHEAD];
+            row.fetch(c, x);
+            u64 scan[RW_AHEAD];
+            bool found = false;
+#pragma unroll
+            for (int k = 0; k < RW_AHEAD; k++) {
+                u64 v[4], own = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) own += v[j] = m(x[4 * k + j], row.index(c + k, j));
+                scan[k] = lane_scan64(own);
+                u64 run = before + scan[k] - own;
+                if (run < g && g <= run + own) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (run < g && g <= run + v[j]) sh.token = row.index(c + k, j);
+                        run += v[j];
+                    }
+                }
+                before += lane64(scan[k], WAVE - 1);
+                found = found || before >= g;
+            }
+            if (alike((int)found)) break;
+        }
+    }
+    __syncthreads();
+    return sh.token;
+}
+
+__global__ void __launch_bounds__(RW_THREADS) row_kernel(SampleArgs a) {
+    __shared__ RowShared sh;
+    const long long r = blockIdx.x;
+    const int t = threadIdx.x, lane = t & (WAVE - 1), wave = t >> 6;
+    const Row row(a, r);
+
+    /* the largest allowed logit (the lowest index among equals) and the smallest */
+    float most = -INFINITY, least = INFINITY;
+    int at = 0;
+    row.each([&](float z, int i) {
+        at = z > most ? i : at;
+        most = fmaxf(most, z);
+        least = fminf(least, z > -INFINITY ? z : INFINITY);
+    });
+    u64 best = token_code(most, at);
+    const u64 own = best;
+    best = lane_max64(best);
+    least = -lane_max(-least);
+    if (lane == 0) {
+        sh.sum[wave] = best;
+        sh.rank[wave] = __float_as_int(least);
+    }
+    if (t == 0) sh.n = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < RW_WAVES; w++) {
+        best = max(best, sh.sum[w]);
+        least = fminf(least, __int_as_float(sh.rank[w]));
+    }
+    best = alike(best);
+    least = alike(least);
+    const float T = alike(a.temperature[r]);
+    int k = a.top_k ? alike(a.top_k[r]) : 0;
+    if (best == 0 || !(T > 0.0f) || k == 1) {   /* nothing allowed; or the largest logit */
+        if (t == 0) a.out[r] = best == 0 ? -1 : code_index(best);
+        return;
+    }
+    const Choice with(a, r, T, key_value((uint32_t)(best >> 32)));
+
+    if (k > 0 && k <= ST_TOP) {
+        /* as split_top: the tokens that reach a bound which k groups of four threads reach */
+        u64 group = max(own, (u64)__shfl_xor(own, 1, WAVE));
+        group = max(group, (u64)__shfl_xor(group, 2, WAVE));
+        if ((t & 3) == 0) sh.most[t >> 2] = group;
+        __syncthreads();
+        if (wave == 0) {
+            const u64 bound = least_of_top(sh, lane, k);
+            if (lane == 0) sh.least_code = bound;
+        }
+        __syncthreads();
+        const u64 bound = alike(sh.least_code);
+        row.each([&](float z, int i) {
+            const u64 c = token_code(z, i);
+            if (c >= bound) {
+                const int slot = __hip_atomic_fetch_add(&sh.n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (slot < ST_CAND) sh.cand[slot] = c;
+            }
+        });
+        __syncthreads();
+        const int n = alike(sh.n);
+        if (n <= ST_CAND) {   /* more only where the largest tokens crowd in few groups */
+            choose_top(sh, sort_codes<RW_THREADS>(sh, n, k), [&](float z) { return with.weight(z); }, with.p < 1.0f,
+                       [&](u64 total) { return with.mass(total); }, with.least_w, [&](u64 total) { return with.choice(total); },
+                       a.out + r);
+            return;
+        }
+    }
+
+    Cut top = {false, 0u, 0};
+    if (k > 0 && k < a.vocab)
+        top = row_cut<true>(sh, row, with.zmax, with.zmax - least, [&](float z, int) { return z > -INFINITY; },
+                            [&](float) { return 1ull; }, [&](u64) { return (u64)k; });
+    const float top_z = top.some ? key_value(top.key) : -INFINITY;
+    const auto ranked = [&](float z, int i) {   /* among the k largest */
+        return z > top_z || (top.some && z == top_z && i <= top.idx);
+    };
+    float least_z = -INFINITY;   /* the nucleus' smallest logit */
+    if (with.p < 1.0f) {
+        const Cut mass = row_cut<false>(sh, row, with.zmax, fminf(with.zmax - least, with.range(a.vocab)), ranked,
+                                        [&](float z) { return with.weight(z); }, [&](u64 total) { return with.mass(total); });
+        if (mass.some) least_z = key_value(mass.key);
+    }
+    const int token = row_pick(
+        sh, row,
+        [&](float z, int i) {
+            const u64 w = z >= least_z && ranked(z, i) ? with.weight(z) : 0ull;
+            return w >= with.least_w ? w : 0ull;
+        },
+        [&](u64 total) { return with.choice(total); });
+    if (t == 0) a.out[r] = token;
+}
+
 }  // namespace nc
 
 using namespace nc;
 
-static int split_groups(int vocab) { return (vocab + ST_SLICE - 1) / ST_SLICE; }
-
-/* Rows of a launch that cuts rows into `groups` slices. */
-static long long split_rows(long long rows, int groups) {
-    return rows < ST_MAX_WORKGROUPS / groups ? rows : ST_MAX_WORKGROUPS / groups;
+/* Slices of a row, 0 for row_kernel: rows too long for slices, or so many that not all slices run at once. A round of slices
+ * takes 17 to 37 us whatever the rows ask for, most of it waiting for one another, and row_kernel as long as a row's own work:
+ * 128 rows of 65,536 tokens (two rounds of slices) take 35 us in slices and 24 whole with a top-k of 40, 21 and 10 greedily,
+ * 75 and 84 with top-p; 256 rows with top-p 142 and 94, and 64 rows (one round) with a top-k 20 and 23. */
+static int split_groups(long long rows, int vocab) {
+    const int groups = (vocab + ST_SLICE - 1) / ST_SLICE;
+    return groups == 1 || (groups <= ST_MAX_GROUPS && rows * groups <= ST_MAX_WORKGROUPS) ? groups : 0;
 }
 
 /* The counts come first, in the same place whatever the sizes, so that every call finds them as the one before left them. */
@@ -1358,9 +1390,8 @@ constexpr size_t ST_COUNT_BYTES = (2 * ST_QUEUES + ST_MAX_WORKGROUPS / 2) * ST_L
 
 extern "C" size_t nc_sample_workspace_bytes(long long rows, int vocab) {
     if (rows < 0 || rows > 1LL << 22 || vocab <= 0 || vocab > 1 << 24) return 0;
-    const int groups = split_groups(vocab);
-    if (groups == 1 || groups > ST_MAX_GROUPS || rows == 0) return 16;
-    return ST_COUNT_BYTES + (size_t)split_rows(rows, groups) * groups * ST_PART * sizeof(u64);
+    const int groups = split_groups(rows, vocab);
+    return groups <= 1 ? 16 : ST_COUNT_BYTES + (size_t)rows * groups * ST_PART * sizeof(u64);
 }
 
 extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
@@ -1379,25 +1410,20 @@ extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_s
     a.uniform = uniform; a.temperature = temperature; a.top_p = top_p; a.min_p = min_p; a.top_k = top_k;
     a.mask = mask; a.mask_stride = mask_stride;
     a.out = tokens;
-    const int groups = split_groups(vocab);
-    if (groups > ST_MAX_GROUPS) {
-        hipLaunchKernelGGL(sample_kernel, dim3((unsigned)rows), dim3(SM_THREADS), 0, (hipStream_t)stream, a);
+    const int groups = split_groups(rows, vocab);
+    if (groups == 0) {
+        hipLaunchKernelGGL(row_kernel, dim3((unsigned)rows), dim3(RW_THREADS), 0, (hipStream_t)stream, a);
         return (int)hipGetLastError();
     }
     SplitArgs s = {};
     s.a = a;
+    s.rows = (int)rows;
     s.groups = groups;
-    const long long most = groups == 1 ? rows : split_rows(rows, groups);
     s.tickets = (int *)workspace;
     s.done = s.tickets + ST_QUEUES * ST_LINE;
     s.count = s.done + ST_QUEUES * ST_LINE;
     s.part = (u64 *)((char *)workspace + ST_COUNT_BYTES);
-    for (s.row0 = 0; s.row0 < rows; s.row0 += most) {
-        s.rows = (int)(rows - s.row0 < most ? rows - s.row0 : most);
-        const int grid = groups == 1 ? s.rows : (s.rows + ST_QUEUES - 1) / ST_QUEUES * ST_QUEUES * groups;
-        hipLaunchKernelGGL(split_kernel, dim3((unsigned)grid), dim3(ST_THREADS), 0, (hipStream_t)stream, s);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return (int)e;
-    }
-    return NC_OK;
+    const long long grid = groups == 1 ? rows : (rows + ST_QUEUES - 1) / ST_QUEUES * ST_QUEUES * groups;
+    hipLaunchKernelGGL(split_kernel, dim3((unsigned)grid), dim3(ST_THREADS), 0, (hipStream_t)stream, s);
+    return (int)hipGetLastError();
 }

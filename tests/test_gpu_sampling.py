@@ -240,8 +240,8 @@ def test_sorted_rows(device, order):
     compare(run(logits, device, u, t, top_p=pp), logits, u, t, top_p=pp)
 
 
-def test_rows_of_several_launches(device):
-    """More slices than one launch takes (2,048), calls of other sizes between them on the same workspace."""
+def test_calls_of_many_and_few_rows(device):
+    """More rows than are cut into slices, and a call of few between them on the same workspace."""
     vocab, rows = 9000, 1500
     u, t, rng = draws(rows, 13)
     logits = torch.from_numpy(rng.normal(size=(rows, vocab)).astype(np.float32) * 3)
@@ -252,3 +252,35 @@ def test_rows_of_several_launches(device):
     assert np.array_equal(few, got[:3]) and np.array_equal(got, run(logits, device, u, t, top_k=k, top_p=p))
     some = rng.permutation(rows)[:60]
     compare(got[some], logits[some], u[some], t[some], top_k=k[some], top_p=p[some])
+
+
+@pytest.mark.parametrize("rows,vocab,with_k", [(70, 65536, True), (260, 20000, False), (40, 65536, False), (2100, 9000, True),
+                                               (3, 262144, False), (2, 300001, True)])
+def test_many_rows(device, rows, vocab, with_k):
+    """Batches on either side of where rows stop being cut into slices, each row with settings of its own."""
+    u, t, rng = draws(rows, rows)
+    t[::5] = 0.0
+    logits = torch.from_numpy((rng.normal(size=(rows, vocab)) * rng.choice([0.5, 2.5], (rows, 1))).astype(np.float32))
+    k = rng.choice([0, 1, 2, 50, 128, 129, 1000], rows) if with_k else None
+    p = rng.choice([1.0, 0.95, 0.3], rows).astype(np.float32)
+    m = rng.choice([0.0, 0.02], rows).astype(np.float32)
+    got = run(logits, device, u, t, top_k=k, top_p=p, min_p=m)
+    some = rng.permutation(rows)[:48]
+    compare(got[some], logits[some], u[some], t[some], top_k=None if k is None else k[some], top_p=p[some], min_p=m[some])
+
+
+@pytest.mark.parametrize("rows", [5, 80, 260])
+@pytest.mark.parametrize("period,run_of", [(256, 16), (2048, 256), (4096, 64)])
+def test_top_tokens_crowded_in_few_threads(device, rows, period, run_of):
+    """A top-k whose candidates may outnumber their list: the largest tokens in runs that few threads read."""
+    vocab = 65536
+    u, t, rng = draws(rows, 14)
+    z = rng.normal(size=(rows, vocab)).astype(np.float32)
+    z.reshape(rows, -1, period)[:, :, :run_of] += 20
+    z[1] = 2.0                                                       # equals everywhere
+    logits = torch.from_numpy(z)
+    k = rng.choice([2, 100, 128], rows)
+    got = run(logits, device, u, t, top_k=k)
+    some = rng.permutation(rows)[:20]
+    some[0] = 1
+    compare(got[some], logits[some], u[some], t[some], top_k=k[some])
