@@ -26,7 +26,7 @@
  *
  * row_kernel takes a row by one workgroup that reads it again for every step, for more rows and for longer ones. With top-p
  * it is bound by the exponentials, twice for every token (about 180 cycles of a SIMD for a wave's 64, most of them float64
- * at half rate): 256 rows of 65,536 tokens 94 us, 333 rows of 32,768 masked bf16 logits, of which 77 wait for a CU, 102. With a
+ * at half rate): 256 rows of 65,536 tokens 94 us, 333 rows of 32,768 masked bf16 logits 85. With a
  * top-k it reads the row twice and the rest is k tokens: 128 rows of 65,536 fp32 logits, a quarter of them greedy, 25 us
  * (1.3 TB/s of logits).
  */
@@ -995,9 +995,9 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
 
 constexpr int RW_WAVES = 16, RW_THREADS = RW_WAVES * WAVE;
 constexpr int RW_CHUNK = 4 * WAVE;       /* elements of a wave's chunk: four a lane */
-constexpr int RW_AHEAD = 4;              /* chunks in flight */
 constexpr int RW_BINS = 4 * RW_THREADS;
 constexpr int RW_LIST = 512;             /* tokens a range may hold to be settled pairwise */
+constexpr int RW_CUS = 256;              /* rows that run at once, a workgroup a CU */
 
 struct RowShared {
     union {
@@ -1013,6 +1013,7 @@ struct RowShared {
 };
 
 /* Element j of lane l of chunk c of wave w is index (w per + c) RW_CHUNK + 4 l + j. */
+template <int AHEAD>   /* chunks in flight */
 struct Row {
     const SampleArgs &a;
     const char *p;
@@ -1029,30 +1030,31 @@ struct Row {
 
     __device__ __forceinline__ int index(int c, int j) const { return base + c * RW_CHUNK + 4 * lane + j; }
 
-    /* Chunks c .. c + 3. Elements that are not allowed, those past the row's end and those of the next wave are -inf. */
-    __device__ __forceinline__ void fetch(int c, float (&x)[4 * RW_AHEAD]) const {
-        uint32_t allowed = 0xFFFFu;
+    /* Chunks c .. c + AHEAD - 1. Elements that are not allowed, those past the row's end and those of the next wave are -inf. */
+    __device__ __forceinline__ void fetch(int c, float (&x)[4 * AHEAD]) const {
+        constexpr uint32_t all = (1u << 4 * AHEAD) - 1;
+        uint32_t allowed = all;
         if (mask) {
             allowed = 0;
 #pragma unroll
-            for (int k = 0; k < RW_AHEAD; k++) {
+            for (int k = 0; k < AHEAD; k++) {
                 const int i = min(index(c + k, 0), a.vocab - 1) & ~3;
                 allowed |= (mask[i >> 5] >> (i & 31) & 0xFu) << (4 * k);
             }
         }
-        if (a.wide && c + RW_AHEAD <= per && base + (c + RW_AHEAD) * RW_CHUNK <= a.vocab) {
+        if (a.wide && c + AHEAD <= per && base + (c + AHEAD) * RW_CHUNK <= a.vocab) {
             if (a.bf16) {
-                uint2 u[RW_AHEAD];
+                uint2 u[AHEAD];
 #pragma unroll
-                for (int k = 0; k < RW_AHEAD; k++) u[k] = *reinterpret_cast<const uint2 *>(p + 2LL * index(c + k, 0));
+                for (int k = 0; k < AHEAD; k++) u[k] = *reinterpret_cast<const uint2 *>(p + 2LL * index(c + k, 0));
 #pragma unroll
-                for (int k = 0; k < RW_AHEAD; k++) {
+                for (int k = 0; k < AHEAD; k++) {
                     x[4 * k] = __uint_as_float(u[k].x << 16); x[4 * k + 1] = __uint_as_float(u[k].x & 0xFFFF0000u);
                     x[4 * k + 2] = __uint_as_float(u[k].y << 16); x[4 * k + 3] = __uint_as_float(u[k].y & 0xFFFF0000u);
                 }
             } else {
 #pragma unroll
-                for (int k = 0; k < RW_AHEAD; k++) {
+                for (int k = 0; k < AHEAD; k++) {
                     const float4 u = *reinterpret_cast<const float4 *>(p + 4LL * index(c + k, 0));
                     x[4 * k] = u.x; x[4 * k + 1] = u.y; x[4 * k + 2] = u.z; x[4 * k + 3] = u.w;
                 }
@@ -1060,29 +1062,29 @@ struct Row {
         } else {
             const int end = min(base + per * RW_CHUNK, a.vocab);
 #pragma unroll
-            for (int e = 0; e < 4 * RW_AHEAD; e++) {
+            for (int e = 0; e < 4 * AHEAD; e++) {
                 const int i = index(c + e / 4, e % 4), at = min(i, a.vocab - 1);
                 x[e] = a.bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[at]) : reinterpret_cast<const float *>(p)[at];
                 allowed &= ~((uint32_t)(i >= end) << e);
             }
         }
-        if (allowed != 0xFFFFu)
+        if (allowed != all)
 #pragma unroll
-            for (int e = 0; e < 4 * RW_AHEAD; e++)   /* not allowed: NaN */
+            for (int e = 0; e < 4 * AHEAD; e++)   /* not allowed: NaN */
                 x[e] = __int_as_float(__float_as_int(x[e]) | ~((int)(allowed << (31 - e)) >> 31));
 #pragma unroll
-        for (int e = 0; e < 4 * RW_AHEAD; e++)   /* NaN fails the comparison; -0 becomes +0, its equal */
+        for (int e = 0; e < 4 * AHEAD; e++)   /* NaN fails the comparison; -0 becomes +0, its equal */
             x[e] = (x[e] > -INFINITY ? x[e] : -INFINITY) + 0.0f;
     }
 
     /* f(value, index) for every element of this wave. */
     template <typename F>
     __device__ __forceinline__ void each(F &&f) const {
-        for (int c = 0; c < per; c += RW_AHEAD) {
-            float x[4 * RW_AHEAD];
+        for (int c = 0; c < per; c += AHEAD) {
+            float x[4 * AHEAD];
             fetch(c, x);
 #pragma unroll
-            for (int e = 0; e < 4 * RW_AHEAD; e++) f(x[e], index(c + e / 4, e % 4));
+            for (int e = 0; e < 4 * AHEAD; e++) f(x[e], index(c + e / 4, e % 4));
         }
     }
 };
@@ -1127,8 +1129,9 @@ __device__ __forceinline__ bool row_bin(RowShared &sh, Target target) {
  * target(total). SPLIT: equals are taken one by one, the lower index first (m is 1), and the cut's idx is the last one
  * taken; else they are taken together. `range`: the values below zmax - range need no telling apart. Every thread must
  * call it. */
-template <bool SPLIT, typename In, typename M, typename Target>
-__device__ __forceinline__ Cut row_cut(RowShared &sh, const Row &row, float zmax, float range, In in, M m, Target target) {
+template <bool SPLIT, int AHEAD, typename In, typename M, typename Target>
+__device__ __forceinline__ Cut row_cut(RowShared &sh, const Row<AHEAD> &row, float zmax, float range, In in, M m,
+                                       Target target) {
     const int t = threadIdx.x, lane = row.lane, wave = t >> 6;
     const float scale = range > 0.0f && range < INFINITY ? (RW_BINS - 1) / range : 0.0f;
     /* a range whose products are NaN or past the last bin: the last bin; monotone in z in every case */
@@ -1234,8 +1237,8 @@ __device__ __forceinline__ Cut row_cut(RowShared &sh, const Row &row, float zmax
 }
 
 /* The first element in index order at which the running sum of m(z, index) reaches goal(total). Every thread must call it. */
-template <typename M, typename Goal>
-__device__ __forceinline__ int row_pick(RowShared &sh, const Row &row, M m, Goal goal) {
+template <int AHEAD, typename M, typename Goal>
+__device__ __forceinline__ int row_pick(RowShared &sh, const Row<AHEAD> &row, M m, Goal goal) {
     const int lane = row.lane, wave = threadIdx.x >> 6;
     u64 s = 0;
     row.each([&](float z, int i) { s += m(z, i); });
@@ -1251,13 +1254,13 @@ __device__ __forceinline__ int row_pick(RowShared &sh, const Row &row, M m, Goal
     }
     const u64 g = goal(total);
     if (alike((int)(before < g && g <= before + s))) {   /* this wave holds it */
-        for (int c = 0; c < row.per; c += RW_AHEAD) {
-            float x[4 * RW_AHEAD];
+        for (int c = 0; c < row.per; c += AHEAD) {
+            float x[4 * AHEAD];
             row.fetch(c, x);
-            u64 scan[RW_AHEAD];
+            u64 scan[AHEAD];
             bool found = false;
 #pragma unroll
-            for (int k = 0; k < RW_AHEAD; k++) {
+            for (int k = 0; k < AHEAD; k++) {
                 u64 v[4], own = 0;
 #pragma unroll
                 for (int j = 0; j < 4; j++) own += v[j] = m(x[4 * k + j], row.index(c + k, j));
@@ -1280,11 +1283,15 @@ __device__ __forceinline__ int row_pick(RowShared &sh, const Row &row, M m, Goal
     return sh.token;
 }
 
-__global__ void __launch_bounds__(RW_THREADS) row_kernel(SampleArgs a) {
+/* Two forms, with the same results: four chunks in flight, 93 registers, a workgroup a CU; or two chunks and 64 registers, two
+ * workgroups a CU, where there are more rows than CUs: 333 rows of 32,768 tokens with top-p 102 and 85 us, 256 of 65,536 94 and
+ * 95, 128 of them with a top-k 23.6 and 25.0. */
+template <int AHEAD>
+__global__ void __launch_bounds__(RW_THREADS, AHEAD == 4 ? 4 : 8) row_kernel(SampleArgs a) {
     __shared__ RowShared sh;
     const long long r = blockIdx.x;
     const int t = threadIdx.x, lane = t & (WAVE - 1), wave = t >> 6;
-    const Row row(a, r);
+    const Row<AHEAD> row(a, r);
 
     /* the largest allowed logit (the lowest index among equals) and the smallest */
     float most = -INFINITY, least = INFINITY;
@@ -1412,7 +1419,8 @@ extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_s
     a.out = tokens;
     const int groups = split_groups(rows, vocab);
     if (groups == 0) {
-        hipLaunchKernelGGL(row_kernel, dim3((unsigned)rows), dim3(RW_THREADS), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(rows > RW_CUS ? row_kernel<2> : row_kernel<4>, dim3((unsigned)rows), dim3(RW_THREADS), 0,
+                           (hipStream_t)stream, a);
         return (int)hipGetLastError();
     }
     SplitArgs s = {};
