@@ -70,6 +70,8 @@ class BlockTables:
                 _require(t, name, torch.int32)
                 if t.shape != (n,) or t.device != self.table.device:
                     raise ValueError(f"{name} must be [{n}] on {self.table.device}, got {tuple(t.shape)} on {t.device}")
+                if t.data_ptr() < new_tokens.data_ptr() + 4 * self.slots and new_tokens.data_ptr() < t.data_ptr() + 4 * n:
+                    raise ValueError(f"{name} must not share memory with new_tokens, which is read while it is written")
         with device_guard(self.table):
             check(hip_library().nc_pages_extend(
                 pointer(new_tokens), self.slots, pointer(self.lengths), pointer(self.table), self.max_pages,

@@ -104,3 +104,7 @@ def test_refusals(device):
     maps = t.extend(torch.zeros(4, dtype=torch.int32, device=device), 4)
     with pytest.raises(ValueError, match="positions"):
         t.extend(torch.zeros(4, dtype=torch.int32, device=device), 5, maps)
+    with pytest.raises(ValueError, match="share memory"):   # read by every workgroup while one writes what was granted
+        t.extend(maps.granted, 4, maps)
+    t.extend(maps.granted, 4)
+    t.extend(t.lengths, 4, maps)                            # lengths are written after everyone has read them
