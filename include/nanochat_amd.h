@@ -305,8 +305,9 @@ int nc_pages_extend(const int32_t *new_tokens, int slots, int32_t *lengths, int3
 int nc_pages_trim(const int32_t *keep, int slots, int32_t *lengths, int32_t *table, int max_pages, int32_t *free_pages,
                   int32_t *free_count, int num_pages, int32_t *arrived, void *stream);
 
-/* Workspace bytes nc_sample_tokens needs for these sizes, at most 26 MB (0 for unsupported sizes): zero-filled before its
- * first call, then passed to calls ordered on one stream, of any sizes that it suffices for. It serves no other function. */
+/* Workspace bytes nc_sample_tokens needs for these sizes, at most 7 MB (0 for unsupported sizes). Its first 64 KiB (or all
+ * of it, if smaller) are zero-filled before its first call; it is then passed to calls ordered on one stream, of any sizes
+ * that it suffices for. It serves no other function. */
 size_t nc_sample_workspace_bytes(long long rows, int vocab);
 
 /*

@@ -26,9 +26,8 @@
  *
  * row_kernel takes a row by one workgroup that reads it again for every step, for more rows and for longer ones. With top-p
  * it is bound by the exponentials, twice for every token (about 180 cycles of a SIMD for a wave's 64, most of them float64
- * at half rate): 256 rows of 65,536 tokens 94 us, 333 rows of 32,768 masked bf16 logits 85. With a
- * top-k it reads the row twice and the rest is k tokens: 128 rows of 65,536 fp32 logits, a quarter of them greedy, 25 us
- * (1.3 TB/s of logits).
+ * at half rate): 256 rows of 65,536 tokens 94 us, 333 rows of 32,768 masked bf16 logits 85. With a top-k it reads the row
+ * twice and the rest is k tokens: 128 rows of 65,536 fp32 logits, a quarter of them greedy, 25 us (1.3 TB/s of logits).
  */
 #include <math.h>
 
@@ -1394,6 +1393,7 @@ static int split_groups(long long rows, int vocab) {
 
 /* The counts come first, in the same place whatever the sizes, so that every call finds them as the one before left them. */
 constexpr size_t ST_COUNT_BYTES = (2 * ST_QUEUES + ST_MAX_WORKGROUPS / 2) * ST_LINE * sizeof(int);
+static_assert(ST_COUNT_BYTES <= 64 * 1024, "callers zero no more than 64 KiB");
 
 extern "C" size_t nc_sample_workspace_bytes(long long rows, int vocab) {
     if (rows < 0 || rows > 1LL << 22 || vocab <= 0 || vocab > 1 << 24) return 0;
@@ -1413,7 +1413,7 @@ extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_s
     if (rows == 0) return NC_OK;
     SampleArgs a = {};
     a.logits = logits; a.stride = row_stride; a.vocab = vocab; a.bf16 = is_bf16 != 0;
-    a.wide = (uintptr_t)logits % (is_bf16 ? 8 : 16) == 0 && row_stride % 4 == 0;
+    a.wide = (uintptr_t)logits % (is_bf16 ? 8 : 16) == 0 && (row_stride % 4 == 0 || rows == 1);
     a.uniform = uniform; a.temperature = temperature; a.top_p = top_p; a.min_p = min_p; a.top_k = top_k;
     a.mask = mask; a.mask_stride = mask_stride;
     a.out = tokens;

@@ -11,6 +11,7 @@ from .native import check, device_guard, hip_library, pointer, stream
 
 
 _WORKSPACES: OrderedDict = OrderedDict()
+_COUNT_BYTES = 1 << 16   # a workspace's counts lie within its first 64 KiB
 
 
 @functools.lru_cache(maxsize=256)
@@ -72,8 +73,11 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature: torc
     need = sample_workspace_bytes(rows, vocab)
     with device_guard(logits):
         if workspace is None:
-            workspace = (torch.zeros(need, dtype=torch.uint8, device=logits.device)
-                         if torch.cuda.is_current_stream_capturing() else _workspace(logits.device, need, _WORKSPACES))
+            if torch.cuda.is_current_stream_capturing():
+                workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+                workspace[:_COUNT_BYTES].zero_()   # on every replay
+            else:
+                workspace = _workspace(logits.device, need, _WORKSPACES)
         nbytes = workspace.numel() * workspace.element_size()
         if nbytes < need or not workspace.is_contiguous() or workspace.device != logits.device or workspace.data_ptr() % 16:
             raise ValueError(f"workspace must be a contiguous 16-byte aligned tensor of at least {need} bytes on {logits.device}")

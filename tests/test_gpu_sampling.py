@@ -284,3 +284,14 @@ def test_top_tokens_crowded_in_few_threads(device, rows, period, run_of):
     some = rng.permutation(rows)[:20]
     some[0] = 1
     compare(got[some], logits[some], u[some], t[some], top_k=k[some])
+
+
+def test_one_row_of_odd_width(device):
+    """A single row's stride is no one's business: aligned loads, and a last slice that ends inside a group of four."""
+    for vocab in (8193, 50257, 50258, 300003):
+        u, t, rng = draws(1, vocab)
+        for dtype in (torch.float32, torch.bfloat16):
+            logits = torch.from_numpy(rng.normal(size=(1, vocab)).astype(np.float32) * 2).to(dtype)
+            for k, p in ((0, 0.9), (40, 0.9), (0, 1.0)):
+                kk, pp = np.full(1, k), np.full(1, p, np.float32)
+                compare(run(logits, device, u, t, top_k=kk, top_p=pp), logits, u, t, top_k=kk, top_p=pp)
