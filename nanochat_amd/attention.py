@@ -19,7 +19,7 @@ from collections import OrderedDict
 import torch
 
 from .config import HEAD_DIM, PAGE_SIZE
-from .kv_cache import PagedKVCache, _require
+from .kv_cache import PagedKVCache, _require, _require_all
 from .native import check, device_guard, hip_library, pointer, stream
 
 
@@ -57,12 +57,6 @@ def qk_norm_rope_append(qkv: torch.Tensor, num_q_heads: int, cache: PagedKVCache
     return q_out
 
 
-def _same_device(device: torch.device, **tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
-        if t.get_device() != device.index:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
-
-
 def qk_norm_rope_append_packed(qkv: torch.Tensor, num_q_heads: int, cache: PagedKVCache, positions: torch.Tensor,
                                slot_map: torch.Tensor, q_gain: torch.Tensor, k_gain: torch.Tensor, cos: torch.Tensor,
                                sin: torch.Tensor, q_out: torch.Tensor | None = None) -> torch.Tensor:
@@ -79,23 +73,22 @@ def qk_norm_rope_append_packed(qkv: torch.Tensor, num_q_heads: int, cache: Paged
         raise ValueError(f"qkv width {W} != (Hq + 2 Hkv) * {HEAD_DIM} = {(num_q_heads + 2 * Hkv) * HEAD_DIM}")
     if qkv.dtype != torch.bfloat16 or not qkv.is_cuda or qkv.stride(1) != 1 or (rows > 1 and qkv.stride(0) < W):
         raise ValueError("qkv must be a bf16 device tensor with contiguous rows that do not overlap")
-    for name, t in (("q_gain", q_gain), ("k_gain", k_gain), ("cos", cos), ("sin", sin)):
-        _require(t, name, torch.float32)
+    device = qkv.device
+    _require_all(device, torch.float32, q_gain=q_gain, k_gain=k_gain, cos=cos, sin=sin, cache=cache.kv_scale)
+    _require_all(device, torch.int32, positions=positions, slot_map=slot_map)
     if cos.shape != sin.shape or cos.dim() != 2 or cos.size(0) < 1 or cos.size(1) != HEAD_DIM // 2:
         raise ValueError("cos, sin must be [positions, 64]")
     if q_gain.numel() != HEAD_DIM or k_gain.numel() != HEAD_DIM:
         raise ValueError(f"q_gain, k_gain must be [{HEAD_DIM}]")
     for name, t in (("positions", positions), ("slot_map", slot_map)):
-        _require(t, name, torch.int32)
         if t.shape != (rows,):
             raise ValueError(f"{name} must be [{rows}], got {tuple(t.shape)}")
     if q_out is None:
-        q_out = torch.empty(rows, num_q_heads, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device)
-    _require(q_out, "q_out", torch.bfloat16)
-    if q_out.shape != (rows, num_q_heads, HEAD_DIM):
-        raise ValueError(f"q_out must be [{rows}, {num_q_heads}, {HEAD_DIM}]")
-    _same_device(qkv.device, cache=cache.k_pages, positions=positions, slot_map=slot_map, q_gain=q_gain, k_gain=k_gain,
-                 cos=cos, sin=sin, q_out=q_out)
+        q_out = torch.empty(rows, num_q_heads, HEAD_DIM, dtype=torch.bfloat16, device=device)
+    else:
+        _require_all(device, torch.bfloat16, q_out=q_out)
+        if q_out.shape != (rows, num_q_heads, HEAD_DIM):
+            raise ValueError(f"q_out must be [{rows}, {num_q_heads}, {HEAD_DIM}]")
     if rows == 0:
         return q_out
     with device_guard(qkv):
@@ -299,10 +292,11 @@ def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Te
     if q.dim() != 3 or q.size(2) != HEAD_DIM or q.size(1) < 1:
         raise ValueError(f"q must be [rows, Hq, {HEAD_DIM}], got {tuple(q.shape)}")
     rows, Hq, _ = q.shape
+    _require_all(q.device, torch.int32, block_table=block_table, cu_seqlens=cu_seqlens, seq_lens=seq_lens)
+    _require_all(q.device, torch.float32, cache=cache.kv_scale)
     cache.check_table(block_table)
     B = block_table.size(0)
     for name, t, n in (("cu_seqlens", cu_seqlens, B + 1), ("seq_lens", seq_lens, B)):
-        _require(t, name, torch.int32)
         if t.shape != (n,):
             raise ValueError(f"{name} must be [{n}] for a block table of {B} sequences, got {tuple(t.shape)}")
     if not 0 < max_seq_len <= block_table.size(1) * PAGE_SIZE:
@@ -311,10 +305,10 @@ def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Te
         sm_scale = HEAD_DIM ** -0.5
     if out is None:
         out = torch.empty_like(q)
-    _require(out, "out", torch.bfloat16)
-    if out.shape != q.shape:
-        raise ValueError(f"out must be {tuple(q.shape)}")
-    _same_device(q.device, cache=cache.k_pages, block_table=block_table, cu_seqlens=cu_seqlens, seq_lens=seq_lens, out=out)
+    else:
+        _require_all(q.device, torch.bfloat16, out=out)
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {tuple(q.shape)}")
     if rows == 0:
         return out
     window = max(window, -1)

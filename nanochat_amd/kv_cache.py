@@ -26,6 +26,16 @@ def _require(t: torch.Tensor, name: str, dtype: torch.dtype) -> None:
         raise ValueError(f"{name} must be contiguous")
 
 
+def _require_all(device: torch.device, dtype: torch.dtype, **tensors: torch.Tensor) -> None:
+    """_require for several tensors, which must be on `device`: one loop, since such checks are a good part of what a small
+    call takes in Python."""
+    index = device.index
+    for name, t in tensors.items():
+        if t.get_device() != index or t.dtype != dtype or not t.is_contiguous():
+            _require(t, name, dtype)
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
 def pages_for(length: int) -> int:
     """Pages holding `length` positions."""
     return (length + PAGE_SIZE - 1) // PAGE_SIZE

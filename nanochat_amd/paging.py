@@ -50,8 +50,9 @@ class BlockTables:
             _require(getattr(self, name), name, torch.int32)
 
     def _per_slot(self, t: torch.Tensor, name: str) -> None:
-        _require(t, name, torch.int32)
-        if t.shape != (self.slots,) or t.device != self.table.device:
+        if (t.get_device() != self.table.get_device() or t.dtype != torch.int32 or t.shape != (self.slots,) or
+                not t.is_contiguous()):
+            _require(t, name, torch.int32)
             raise ValueError(f"{name} must be [{self.slots}] on {self.table.device}, got {tuple(t.shape)} on {t.device}")
 
     def extend(self, new_tokens: torch.Tensor, rows: int, maps: StepMaps | None = None) -> StepMaps:

@@ -25,7 +25,7 @@ def _per_row(t: torch.Tensor | None, name: str, dtype: torch.dtype, logits: torc
         return None
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.shape != logits.shape[:1] or t.device != logits.device or not t.is_contiguous():
+    if t.dim() != 1 or t.size(0) != logits.size(0) or t.get_device() != logits.get_device() or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous [{logits.size(0)}] tensor on {logits.device}")
     return pointer(t)
 
@@ -67,7 +67,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature: torc
             raise ValueError(f"mask must be contiguous words [{rows}, {-(-vocab // 32)}] on {logits.device}")
     if out is None:
         out = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    _per_row(out, "out", torch.int32, logits)
+    else:
+        _per_row(out, "out", torch.int32, logits)
     if rows == 0:
         return out
     need = sample_workspace_bytes(rows, vocab)

@@ -295,3 +295,37 @@ def test_one_row_of_odd_width(device):
             for k, p in ((0, 0.9), (40, 0.9), (0, 1.0)):
                 kk, pp = np.full(1, k), np.full(1, p, np.float32)
                 compare(run(logits, device, u, t, top_k=kk, top_p=pp), logits, u, t, top_k=kk, top_p=pp)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(4, 20000), (200, 20000), (300, 20001)])
+def test_extremes_and_masks_in_every_form(device, rows, vocab, dtype):
+    """Rows in slices, a row a workgroup, two workgroups a CU: NaN and infinities in allowed and masked places, the type's
+    lowest and largest values beside ordinary ones (a range of values past the largest number), masks that leave one token."""
+    u, t, rng = draws(rows, 15)
+    t[::7] = 0.0
+    z = rng.normal(size=(rows, vocab)).astype(np.float32)
+    big = torch.finfo(dtype).max
+    for r in range(rows):
+        at = rng.integers(0, vocab, 40)
+        z[r, at] = rng.choice([np.nan, -np.inf, -big, 0.0, -0.0], 40)
+        if r % 4 == 1:
+            z[r, at[0]] = big
+        elif r % 4 == 2:
+            z[r, at[:3]] = np.inf
+        elif r % 4 == 3:
+            z[r] = np.where(rng.random(vocab) < 0.5, -big, z[r])
+    logits = torch.from_numpy(z).to(dtype)
+    bits = rng.random((rows, -(-vocab // 32) * 32)) < 0.6
+    bits[::5] = False
+    bits[::5, 777] = True
+    bits[5::10, 777] = False
+    mask = torch.from_numpy(np.packbits(bits, axis=1, bitorder="little").view(np.int32))
+    k, p = rng.choice([0, 1, 60, 3000], rows), rng.choice([1.0, 0.9], rows).astype(np.float32)
+    m = rng.choice([0.0, 0.1], rows).astype(np.float32)
+    some = rng.permutation(rows)[:40]
+    some[:3] = [0, min(5, rows - 1), 1]
+    for allowed, words in ((None, None), (bits[:, :vocab], mask)):
+        got = run(logits, device, u, t, top_k=k, top_p=p, min_p=m, mask=words)
+        compare(got[some], logits[some], u[some], t[some], top_k=k[some], top_p=p[some], min_p=m[some],
+                allowed=None if allowed is None else allowed[some])
