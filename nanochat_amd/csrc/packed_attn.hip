@@ -239,7 +239,7 @@ __device__ __forceinline__ void pk_read(int at, int sc, int lane, PairRegs &k) {
     asm volatile("ds_read_b128 %0, %6\n\t"
                  "ds_read_b128 %1, %6 offset:1024\n\t"
                  "ds_read_b128 %2, %6 offset:2048\n\t"
-                 "ds_read_b128 %3, %6 offset:3072\n\t"
+                 "ds_read_b128 %3, %6 offset:0xc00\n\t"
                  "ds_read_b128 %4, %7\n\t"
                  "ds_read_b128 %5, %7 offset:128\n\t"
                  "s_waitcnt lgkmcnt(0)"
@@ -673,7 +673,7 @@ __device__ __forceinline__ void pk_fetch_narrow(const AttnArgs &a, int pa, int p
     __builtin_amdgcn_raw_ptr_buffer_load_lds(ka, (LdsVoid *)st, 16, lane * 16, 0, 0, 2);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(ka, (LdsVoid *)(st + 1024), 16, lane * 16 + 1024, 0, 0, 2);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(kb, (LdsVoid *)(st + 2048), 16, lane * 16, 0, 0, 2);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(kb, (LdsVoid *)(st + 3072), 16, lane * 16 + 1024, 0, 0, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(kb, (LdsVoid *)(st + 3 * 1024), 16, lane * 16 + 1024, 0, 0, 2);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(va, (LdsVoid *)(st + 4096), 16, lane * 16, 0, 0, 2);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(va, (LdsVoid *)(st + 5120), 16, lane * 16 + 1024, 0, 0, 2);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(vb, (LdsVoid *)(st + 6144), 16, lane * 16, 0, 0, 2);
