@@ -294,7 +294,7 @@ int nc_packed_attn_fp8(const void *q, const void *k_pages, const void *v_pages, 
  * `rows` suffice. The j-th page granted is free_pages[free_count - 1 - j]. Slot b's tokens become rows cu_seqlens[b] ..
  * cu_seqlens[b + 1] - 1 (cu_seqlens int32 [slots + 1]) at positions lengths[b] ..; positions, slot_map int32 [rows]: a
  * row's position and its cache slot 16 page + position % 16, both -1 past the last row; granted int32 [slots]. lengths,
- * table and free_count are updated.
+ * table and free_count are updated. No output may overlap new_tokens.
  *
  * nc_pages_trim: slot b longer than keep[b] >= 0 falls back to keep[b] tokens; the pages past them leave the table (-1)
  * and join the free list, the first of them (in slot, then page order) topmost.

@@ -172,7 +172,10 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
  * row's codes are eight 16-byte blocks of its page, stored whole. A V block holds four slots of 16 dims: rows r .. r + 3 of
  * the block of rows that sit in slots 4 g .. 4 g + 3 of one page (a quad, found from the slot map alone) store whole
  * blocks, other rows their single bytes: the rows of different sequences in a decoding step, and up to three rows at
- * either end of a block of rows whose position is not its row modulo 4. */
+ * either end of a block of rows whose position is not its row modulo 4.
+ *
+ * Bound by the rows' chain (position and slot, rotary row, norm, LDS, store) where they are few: 64 rows of 16 / 4 heads
+ * 6.2 us; by HBM where they are many: eight chunks of 257 to 512 tokens, 33.6 MB, 11.5 us (2.9 TB/s). */
 struct AppendRowsArgs {
     const uint16_t *qkv;       /* [rows][(Hq + 2 Hkv) 128] at token_stride */
     long long token_stride;

