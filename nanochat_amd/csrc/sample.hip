@@ -17,11 +17,11 @@
  * histogram over ranges of the value, then among the few tokens of the range that holds it, or by finer histograms where it
  * holds many.
  *
- * split_kernel takes up to 512 / ceil(vocab / 8,192) rows of up to 262,144 tokens, a workgroup for every 8,192, which stay
- * in its registers. What bounds it is neither bytes nor operations (a row of 65,536 fp32 logits is 256 KiB) but the steps one
+ * split_kernel takes up to 512 / ceil(vocab / 8,192) rows of up to 262,144 tokens, a workgroup for every 8,192 (or
+ * 4,096), which stay in its registers. What bounds it is neither bytes nor operations (a row of 65,536 fp32 logits is 256 KiB) but the steps one
  * after the other, each ending where the row's workgroups need one another: the largest logit; the histogram; the list; about
  * 2.5 us a meeting through memory. Greedy rows and a top-k of at most 128 need no meeting: every slice leaves its k largest in
- * order, and the last workgroup to arrive does the rest on k tokens. Measured: one row of 65,536 fp32 logits with top-p 27 us,
+ * order, and the last workgroup to arrive does the rest on k tokens. Measured: one row of 65,536 fp32 logits with top-p 26 us,
  * with top-k 14; 64 rows 39 and 20.
  *
  * row_kernel takes a row by one workgroup that reads it again for every step, for more rows and for longer ones. With top-p
@@ -136,14 +136,13 @@ struct Cut {
     int idx;
 };
 
-/* --- Rows of up to ST_MAX_GROUPS slices of 8,192 tokens, a workgroup each: the slice stays in its registers, 16 tokens a
- * thread, and the workgroups of a row exchange what the next step needs through memory. 512 threads of at most 128 registers
+/* --- Rows of up to ST_MAX_GROUPS slices of 8,192 or 4,096 tokens, a workgroup each: the slice stays in its registers, E (16
+ * or 8) tokens a thread, and the workgroups of a row exchange what the next step needs through memory. 512 threads of at most 128 registers
  * and the weights in LDS leave room for two workgroups a CU, one working while the other waits: one workgroup a CU (no
  * spilled registers, 149 of them) takes 25 us for one row instead of 27, but 124 instead of 88 for 333 rows, and slices of
  * 1,024 threads with 8 tokens each 30 and 150. */
 
 constexpr int ST_WAVES = 8, ST_THREADS = ST_WAVES * WAVE;
-constexpr int ST_E = 16, ST_SLICE = ST_E * ST_THREADS;
 constexpr int ST_STEP = 4 * ST_THREADS;   /* element 4 c + j of thread t: index slice + c ST_STEP + 4 t + j */
 constexpr int ST_MAX_GROUPS = 32;
 constexpr int ST_BINS = 2 * ST_THREADS;
@@ -153,7 +152,8 @@ constexpr int ST_CAND = 4096;             /* candidates: at most ST_TOP of 32 to
 constexpr int ST_LINE = 32;               /* ints of a 128-byte line: counts that several workgroups add to share none */
 constexpr int ST_QUEUES = 8;              /* XCDs */
 constexpr int ST_MAX_WORKGROUPS = 512;    /* of rows that are cut: as many as run at once, two a CU */
-static_assert(ST_TOP * (ST_SLICE / 256) <= ST_CAND && ST_TOP * ST_MAX_GROUPS <= ST_CAND, "candidates fit");
+constexpr int ST_MAX_E = 16;              /* tokens a thread: this many, or half */
+static_assert(ST_TOP * (ST_MAX_E * ST_THREADS / 256) <= ST_CAND && ST_TOP * ST_MAX_GROUPS <= ST_CAND, "candidates fit");
 
 enum { HD_BEST, HD_COUNT, HD_ABOVE, HD_LEAST, HD_MOST, HD_SUM, HD_WORDS };
 constexpr int ST_PART = ST_BINS + 2 * ST_LIST + HD_WORDS;   /* words a workgroup publishes: histogram, list, head */
@@ -165,9 +165,10 @@ struct SplitArgs {
     int *tickets, *done, *count;   /* [ST_QUEUES], [ST_QUEUES], [rows] lines; zero between launches */
 };
 
+template <int E>
 struct SplitShared {
     union {
-        u64 weight[ST_E * ST_THREADS];   /* element e of thread t: [e ST_THREADS + t] */
+        u64 weight[E * ST_THREADS];   /* element e of thread t: [e ST_THREADS + t] */
         struct {
             u64 cand[ST_CAND];
             u64 top[ST_TOP], top_w[ST_TOP], kept_w[ST_TOP];
@@ -180,13 +181,13 @@ struct SplitShared {
         u64 above[ST_LIST];
     };
     u64 code[ST_LIST], w[ST_LIST];
-    u64 sum[ST_E / 4 * ST_WAVES];
+    u64 sum[ST_MAX_E / 4 * ST_WAVES];
     u64 kept[ST_MAX_GROUPS], head[ST_MAX_GROUPS];
     int start[ST_MAX_GROUPS + 1];
     u64 found, least_code, lo, hi;
     int bin, n, token, flag;
 };
-static_assert(2 * sizeof(SplitShared) <= 160 * 1024, "two workgroups a CU");
+static_assert(2 * sizeof(SplitShared<ST_MAX_E>) <= 160 * 1024, "two workgroups a CU");
 
 /* A token as one integer: larger for the larger logit, and among equals for the lower index; 0: not allowed. */
 __device__ __forceinline__ u64 token_code(float z, int i) {
@@ -263,9 +264,10 @@ __device__ __forceinline__ int reserve(int *n, int count, int lane) {
     return __builtin_amdgcn_readlane(first, WAVE - 1) + at - count;
 }
 
+template <int E>
 struct Split {
     const SplitArgs &s;
-    SplitShared &sh;
+    SplitShared<E> &sh;
     int t, lane, wave;
     int row, g, G;         /* row, slice, slices */
     int first;             /* index of this thread's element 0 */
@@ -315,54 +317,55 @@ struct Split {
 };
 
 /* Values that the compiler takes as new: what an earlier step made of them is not kept in registers for a later one. */
-template <typename V>
-__device__ __forceinline__ void anew(V (&v)[ST_E]) {
+template <typename V, int E>
+__device__ __forceinline__ void anew(V (&v)[E]) {
 #pragma unroll
-    for (int e = 0; e < ST_E; e++) asm volatile("" : "+v"(v[e]));
+    for (int e = 0; e < E; e++) asm volatile("" : "+v"(v[e]));
 }
 
-/* This thread's 16 tokens; those not allowed and those past the row's end are -inf. */
-__device__ __forceinline__ void split_load(const Split &q, const SampleArgs &a, long long r, float (&x)[ST_E]) {
+/* This thread's tokens; those not allowed and those past the row's end are -inf. */
+template <int E>
+__device__ __forceinline__ void split_load(const Split<E> &q, const SampleArgs &a, long long r, float (&x)[E]) {
     const char *p = (const char *)a.logits + r * a.stride * (a.bf16 ? 2 : 4);
-    uint32_t allowed = 0xFFFFu;
+    uint32_t allowed = (1u << E) - 1;
     if (a.mask) {
         allowed = 0;
         const uint32_t *mask = a.mask + r * a.mask_stride;
         const int words = (a.vocab + 31) >> 5;
 #pragma unroll
-        for (int c = 0; c < ST_E / 4; c++) {
+        for (int c = 0; c < E / 4; c++) {
             const int i = q.first + c * ST_STEP;
             allowed |= (mask[min(i >> 5, words - 1)] >> (i & 31) & 0xFu) << (4 * c);
         }
     }
-    if (a.wide && (q.g + 1) * ST_SLICE <= a.vocab) {
+    if (a.wide && (q.g + 1) * E * ST_THREADS <= a.vocab) {
         if (a.bf16) {
-            uint2 u[ST_E / 4];
+            uint2 u[E / 4];
 #pragma unroll
-            for (int c = 0; c < ST_E / 4; c++) u[c] = *reinterpret_cast<const uint2 *>(p + 2LL * (q.first + c * ST_STEP));
+            for (int c = 0; c < E / 4; c++) u[c] = *reinterpret_cast<const uint2 *>(p + 2LL * (q.first + c * ST_STEP));
 #pragma unroll
-            for (int c = 0; c < ST_E / 4; c++) {
+            for (int c = 0; c < E / 4; c++) {
                 x[4 * c] = __uint_as_float(u[c].x << 16); x[4 * c + 1] = __uint_as_float(u[c].x & 0xFFFF0000u);
                 x[4 * c + 2] = __uint_as_float(u[c].y << 16); x[4 * c + 3] = __uint_as_float(u[c].y & 0xFFFF0000u);
             }
         } else {
 #pragma unroll
-            for (int c = 0; c < ST_E / 4; c++) {
+            for (int c = 0; c < E / 4; c++) {
                 const float4 u = *reinterpret_cast<const float4 *>(p + 4LL * (q.first + c * ST_STEP));
                 x[4 * c] = u.x; x[4 * c + 1] = u.y; x[4 * c + 2] = u.z; x[4 * c + 3] = u.w;
             }
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < ST_E; e++) {   /* past the end: the last token's, dropped below */
+        for (int e = 0; e < E; e++) {   /* past the end: the last token's, dropped below */
             const int i = min(q.index(e), a.vocab - 1);
             x[e] = a.bf16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i]) : reinterpret_cast<const float *>(p)[i];
         }
 #pragma unroll
-        for (int e = 0; e < ST_E; e++) allowed &= ~((uint32_t)(q.index(e) >= a.vocab) << e);
+        for (int e = 0; e < E; e++) allowed &= ~((uint32_t)(q.index(e) >= a.vocab) << e);
     }
 #pragma unroll
-    for (int e = 0; e < ST_E; e++)   /* NaN fails the comparison; -0 becomes +0, its equal */
+    for (int e = 0; e < E; e++)   /* NaN fails the comparison; -0 becomes +0, its equal */
         x[e] = (allowed >> e & 1) && x[e] > -INFINITY ? x[e] + 0.0f : -INFINITY;
 }
 
@@ -466,19 +469,21 @@ __device__ __forceinline__ void choose_top(Shared &sh, int n, Weight weight, boo
 }
 
 /* Adds `v` to the candidates if `take`. */
-__device__ __forceinline__ void split_collect(SplitShared &sh, u64 v, bool take) {
+template <int E>
+__device__ __forceinline__ void split_collect(SplitShared<E> &sh, u64 v, bool take) {
     if (take) sh.cand[__hip_atomic_fetch_add(&sh.n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)] = v;
 }
 
 /* The k <= ST_TOP largest of this slice, in order, in sh.top; returns how many. A code that k of the maxima of 256 groups of
- * 32 tokens reach is a lower bound of the k-th largest: only the tokens that reach it (in random order about 51 for k = 50,
+ * 2 E tokens reach is a lower bound of the k-th largest: only the tokens that reach it (in random order about 51 for k = 50,
  * 177 for 128) are compared pairwise. */
-__device__ __forceinline__ int split_top(const Split &q, float (&x)[ST_E], int k) {
-    SplitShared &sh = q.sh;
+template <int E>
+__device__ __forceinline__ int split_top(const Split<E> &q, float (&x)[E], int k) {
+    SplitShared<E> &sh = q.sh;
     const int t = q.t;
     u64 best = 0;
 #pragma unroll
-    for (int e = 0; e < ST_E; e++) best = max(best, token_code(x[e], q.index(e)));
+    for (int e = 0; e < E; e++) best = max(best, token_code(x[e], q.index(e)));
     best = max(best, (u64)__shfl_xor(best, 1, WAVE));
     if (k == 1) {
         best = lane_max64(best);
@@ -502,11 +507,11 @@ __device__ __forceinline__ int split_top(const Split &q, float (&x)[ST_E], int k
     anew(x);
     int count = 0;
 #pragma unroll
-    for (int e = 0; e < ST_E; e++) count += token_code(x[e], q.index(e)) >= least;
+    for (int e = 0; e < E; e++) count += token_code(x[e], q.index(e)) >= least;
     int at = reserve(&sh.n, count, q.lane);
     if (count) {
 #pragma unroll
-        for (int e = 0; e < ST_E; e++) {
+        for (int e = 0; e < E; e++) {
             const u64 c = token_code(x[e], q.index(e));
             if (c >= least) sh.cand[at++] = c;
         }
@@ -517,13 +522,13 @@ __device__ __forceinline__ int split_top(const Split &q, float (&x)[ST_E], int k
 
 /* The smallest of this slice's tokens, in index order, whose running sum of m(e), over the elements of the set `in`, reaches
  * `goal`, which its total does. Every thread must call it. */
-template <typename M>
-__device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 goal) {
-    SplitShared &sh = q.sh;
-    u64 own[ST_E / 4], scan[ST_E / 4];
+template <int E, typename M>
+__device__ __forceinline__ int split_pick(const Split<E> &q, uint32_t in, M m, u64 goal) {
+    SplitShared<E> &sh = q.sh;
+    u64 own[E / 4], scan[E / 4];
     asm volatile("" : "+v"(in));
 #pragma unroll
-    for (int c = 0; c < ST_E / 4; c++) {
+    for (int c = 0; c < E / 4; c++) {
         own[c] = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) own[c] += in >> (4 * c + j) & 1 ? m(4 * c + j) : 0;
@@ -532,9 +537,9 @@ __device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 
         __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
-    const u64 part = q.lane < ST_E / 4 * ST_WAVES ? sh.sum[q.lane] : 0, upto = lane_scan64(part) - part;
+    const u64 part = q.lane < E / 4 * ST_WAVES ? sh.sum[q.lane] : 0, upto = lane_scan64(part) - part;
 #pragma unroll
-    for (int c = 0; c < ST_E / 4; c++) {
+    for (int c = 0; c < E / 4; c++) {
         u64 before = lane64(upto, c * ST_WAVES + q.wave) + scan[c] - own[c];
         if (before < goal && goal <= before + own[c]) {
 #pragma unroll
@@ -555,10 +560,10 @@ __device__ __forceinline__ int split_pick(const Split &q, uint32_t in, M m, u64 
  * until the tokens of the one that holds the cut fit a list, which each settles pairwise. Between two histograms, and between
  * two lists, there is always a meeting after the first is read. sh.kept: per slice the weight of the tokens down to the cut
  * that weigh least_w or more (not SPLIT). Every thread of every workgroup of the row calls it. */
-template <bool SPLIT, typename Target>
-__device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t live, float zmax, float range, u64 least_w,
+template <bool SPLIT, int E, typename Target>
+__device__ __forceinline__ Cut split_cut(Split<E> &q, float (&x)[E], uint32_t live, float zmax, float range, u64 least_w,
                                          Target target) {
-    SplitShared &sh = q.sh;
+    SplitShared<E> &sh = q.sh;
     const int lane = q.lane, wave = q.wave, G = q.G;
     int t = q.t;
     u64 *base_part = q.part(0);
@@ -577,7 +582,7 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
         asm volatile("" : "+s"(keyed), "+s"(base_part), "+v"(t), "+v"(q.first), "+v"(live));
         const auto part = [&](int o) { return base_part + (long long)o * ST_PART; };
         const auto listed = [&](u64 code) {   /* what a token of this slice counts */
-            const int i = code_index(code) - q.g * ST_SLICE;
+            const int i = code_index(code) - q.g * E * ST_THREADS;
             return SPLIT ? 1ull : sh.weight[(i / ST_STEP * 4 + i % 4) * ST_THREADS + i % ST_STEP / 4];
         };
         const auto head_of = [&](int word) { return peek(part(lane) + ST_BINS + 2 * ST_LIST + word); };
@@ -596,9 +601,9 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
         }
         __syncthreads();
         u64 rest_of = 0, w4[4];
-        uint32_t bins[ST_E / 2];   /* two elements' a register; ST_BINS: not live */
+        uint32_t bins[E / 2];   /* two elements' a register; ST_BINS: not live */
 #pragma unroll
-        for (int e = 0; e < ST_E; e++) {
+        for (int e = 0; e < E; e++) {
             int b = keyed ? (int)min((hi - key(e)) >> shift, (u64)ST_BINS) : bin_of(x[e]);
             b = live >> e & 1 ? b : ST_BINS;
             bins[e / 2] = e & 1 ? bins[e / 2] | (uint32_t)b << 16 : (uint32_t)b;
@@ -664,7 +669,7 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
         const auto slot = [&](int e) { return (int)(bins[e / 2] >> (e & 1) * 16 & 0xFFFFu); };
         live = 0;
 #pragma unroll
-        for (int e = 0; e < ST_E; e++) {
+        for (int e = 0; e < E; e++) {
             const int b = slot(e);
             live |= (uint32_t)(b == bin) << e;
             if (!SPLIT) {   /* on top of the levels' before */
@@ -679,7 +684,7 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
         int at = reserve(&sh.n, count, lane);
         if (count) {
 #pragma unroll
-            for (int e = 0; e < ST_E; e++) {
+            for (int e = 0; e < E; e++) {
                 if (live >> e & 1) {
                     const u64 k = key(e);
                     if (at < ST_LIST) sh.code[at] = token_code(x[e], q.index(e));
@@ -784,7 +789,7 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
                 const bool in = base + sh.above[t] < goal;
                 if (in) __hip_atomic_fetch_min(&sh.least_code, sh.code[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                 if (!SPLIT && in && sh.w[t] >= least_w)
-                    __hip_atomic_fetch_add(&sh.kept[code_index(sh.code[t]) / ST_SLICE], sh.w[t], __ATOMIC_RELAXED,
+                    __hip_atomic_fetch_add(&sh.kept[code_index(sh.code[t]) / (E * ST_THREADS)], sh.w[t], __ATOMIC_RELAXED,
                                            __HIP_MEMORY_SCOPE_WORKGROUP);
             }
             __syncthreads();
@@ -802,10 +807,11 @@ __device__ __forceinline__ Cut split_cut(Split &q, float (&x)[ST_E], uint32_t li
     }
 }
 
+template <int E>
 __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
-    __shared__ SplitShared sh;
+    __shared__ SplitShared<E> sh;
     const SampleArgs &a = s.a;
-    Split q = {s, sh};
+    Split<E> q = {s, sh};
     q.t = threadIdx.x;
     q.lane = q.t & (WAVE - 1);
     q.wave = q.t >> 6;
@@ -823,12 +829,12 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
         if (q.row >= s.rows) return;   /* counts that were not zero: no access out of bounds */
         q.g = ticket % q.G;
     }
-    q.first = q.g * ST_SLICE + 4 * q.t;
+    q.first = q.g * E * ST_THREADS + 4 * q.t;
     q.reached = 0;
     q.mine = q.part(q.g);
     const int t = q.t, lane = q.lane, wave = q.wave, G = q.G;
     const long long r = q.row;
-    float x[ST_E];
+    float x[E];
     split_load(q, a, r, x);
     const float T = alike(a.temperature[r]);
     const bool greedy = !(T > 0.0f);
@@ -887,7 +893,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     /* the largest allowed logit and the smallest */
     float most = -INFINITY, least = INFINITY;
 #pragma unroll
-    for (int e = 0; e < ST_E; e++) {
+    for (int e = 0; e < E; e++) {
         most = fmaxf(most, x[e]);
         least = fminf(least, x[e] > -INFINITY ? x[e] : INFINITY);
     }
@@ -925,20 +931,20 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     if (k > 0 && k < a.vocab) {
         uint32_t live = 0;
 #pragma unroll
-        for (int e = 0; e < ST_E; e++) live |= (uint32_t)(x[e] > -INFINITY) << e;
+        for (int e = 0; e < E; e++) live |= (uint32_t)(x[e] > -INFINITY) << e;
         const Cut top = split_cut<true>(q, x, live, with.zmax, with.zmax - least, 0ull,
                                         [&](u64) { return (u64)k; });
         if (top.some) {
             const float z = key_value(top.key);
 #pragma unroll
-            for (int e = 0; e < ST_E; e++)   /* past the k largest: dropped */
+            for (int e = 0; e < E; e++)   /* past the k largest: dropped */
                 if (!(x[e] > z || (x[e] == z && q.index(e) <= top.idx))) x[e] = -INFINITY;
         }
     }
     anew(x);
     uint32_t live = 0;
 #pragma unroll
-    for (int e = 0; e < ST_E; e++) {
+    for (int e = 0; e < E; e++) {
         const u64 v = weight(x[e]);
         sh.weight[e * ST_THREADS + t] = v;   /* read by this thread alone */
         live |= (uint32_t)(v != 0) << e;
@@ -952,7 +958,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     } else {
         u64 own = 0;
 #pragma unroll
-        for (int e = 0; e < ST_E; e++) {
+        for (int e = 0; e < E; e++) {
             const u64 v = sh.weight[e * ST_THREADS + t];
             own += v >= with.least_w ? v : 0;
         }
@@ -982,7 +988,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     if (alike((int)(before < goal && goal <= before + ours))) {
         uint32_t kept = 0;
 #pragma unroll
-        for (int e = 0; e < ST_E; e++) kept |= (uint32_t)(x[e] >= least_z && sh.weight[e * ST_THREADS + t] >= with.least_w) << e;
+        for (int e = 0; e < E; e++) kept |= (uint32_t)(x[e] >= least_z && sh.weight[e * ST_THREADS + t] >= with.least_w) << e;
         const int token = split_pick(q, kept, [&](int e) { return sh.weight[e * ST_THREADS + t]; }, goal - before);
         if (t == 0) a.out[r] = token;
     }
@@ -1382,12 +1388,17 @@ __global__ void __launch_bounds__(RW_THREADS, AHEAD == 4 ? 4 : 8) row_kernel(Sam
 
 using namespace nc;
 
-/* Slices of a row, 0 for row_kernel: rows too long for slices, or so many that not all slices run at once. A round of slices
- * takes 17 to 37 us whatever the rows ask for, most of it waiting for one another, and row_kernel as long as a row's own work:
- * 128 rows of 65,536 tokens (two rounds of slices) take 35 us in slices and 24 whole with a top-k of 40, 21 and 10 greedily,
- * 75 and 84 with top-p; 256 rows with top-p 142 and 94, and 64 rows (one round) with a top-k 20 and 23. */
-static int split_groups(long long rows, int vocab) {
-    const int groups = (vocab + ST_SLICE - 1) / ST_SLICE;
+/* Slices of a row, of e tokens a thread, or 0 for row_kernel: rows too long for slices, or so many that not all slices run at
+ * once. A round of slices takes 17 to 37 us whatever the rows ask for, most of it waiting for one another, and row_kernel as
+ * long as a row's own work: 128 rows of 65,536 tokens (two rounds of slices) take 35 us in slices and 24 whole with a top-k of
+ * 40, 21 and 10 greedily, 75 and 84 with top-p; 256 rows with top-p 142 and 94, and 64 rows (one round) with a top-k 20 and 23.
+ * Half slices where one suffices, or where they are at most one a CU and few to a row: one row of 3,000 tokens 15 -> 11 us,
+ * 16 rows of 32,768 tokens 25.6 -> 23.5; but two a CU, for 32 rows of 65,536 tokens, take 37 us and whole slices 31. */
+static int split_groups(long long rows, int vocab, int &e) {
+    const int half = ST_MAX_E / 2 * ST_THREADS, halves = (vocab + half - 1) / half;
+    e = halves == 1 || (halves > 2 && halves <= ST_MAX_GROUPS / 2 && rows * halves <= ST_MAX_WORKGROUPS / 2) ? ST_MAX_E / 2
+                                                                                                    : ST_MAX_E;
+    const int slice = e * ST_THREADS, groups = (vocab + slice - 1) / slice;
     return groups == 1 || (groups <= ST_MAX_GROUPS && rows * groups <= ST_MAX_WORKGROUPS) ? groups : 0;
 }
 
@@ -1397,7 +1408,8 @@ static_assert(ST_COUNT_BYTES <= 64 * 1024, "callers zero no more than 64 KiB");
 
 extern "C" size_t nc_sample_workspace_bytes(long long rows, int vocab) {
     if (rows < 0 || rows > 1LL << 22 || vocab <= 0 || vocab > 1 << 24) return 0;
-    const int groups = split_groups(rows, vocab);
+    int e;
+    const int groups = split_groups(rows, vocab, e);
     return groups <= 1 ? 16 : ST_COUNT_BYTES + (size_t)rows * groups * ST_PART * sizeof(u64);
 }
 
@@ -1417,7 +1429,8 @@ extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_s
     a.uniform = uniform; a.temperature = temperature; a.top_p = top_p; a.min_p = min_p; a.top_k = top_k;
     a.mask = mask; a.mask_stride = mask_stride;
     a.out = tokens;
-    const int groups = split_groups(rows, vocab);
+    int e;
+    const int groups = split_groups(rows, vocab, e);
     if (groups == 0) {
         hipLaunchKernelGGL(rows > RW_CUS ? row_kernel<2> : row_kernel<4>, dim3((unsigned)rows), dim3(RW_THREADS), 0,
                            (hipStream_t)stream, a);
@@ -1432,6 +1445,6 @@ extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_s
     s.count = s.done + ST_QUEUES * ST_LINE;
     s.part = (u64 *)((char *)workspace + ST_COUNT_BYTES);
     const long long grid = groups == 1 ? rows : (rows + ST_QUEUES - 1) / ST_QUEUES * ST_QUEUES * groups;
-    hipLaunchKernelGGL(split_kernel, dim3((unsigned)grid), dim3(ST_THREADS), 0, (hipStream_t)stream, s);
+    hipLaunchKernelGGL(e == ST_MAX_E ? split_kernel<ST_MAX_E> : split_kernel<ST_MAX_E / 2>, dim3((unsigned)grid), dim3(ST_THREADS), 0, (hipStream_t)stream, s);
     return (int)hipGetLastError();
 }
