@@ -683,10 +683,10 @@ __device__ __forceinline__ void pk_fetch_narrow(const AttnArgs &a, int pa, int p
 }
 
 /* The item's page pairs first, first + stride, ... by one wave. ALONE: the four waves of a workgroup share the item so and
- * merge their states through LDS (stages, ml); else one wave has it all and leaves its output or partial. */
+ * merge their states through LDS (stages, ml); else one wave has a chunk to itself and leaves a partial. */
 template <int NT, bool ALONE>
-__device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it, int chunks, long long slot,
-                                          unsigned char *ring, int first, unsigned char *stages, float *ml) {
+__device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it, long long slot, unsigned char *ring, int first,
+                                          unsigned char *stages, float *ml) {
     constexpr int stride = ALONE ? WAVES : 1;
     const AttnArgs &a = p.a;
     const int lane = pk_lane(), c = lane & 15, g = lane >> 4;
@@ -939,9 +939,9 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
             const int wave = uni((int)threadIdx.x >> 6);
             unsigned char *ring = stages + wave * PK_BUFS * PK_NARROW_STAGE;
             if (it.tn <= p.tpt)
-                pk_narrow<1, true>(p, it, 1, 0, ring, wave, stages, reinterpret_cast<float *>(tab));
+                pk_narrow<1, true>(p, it, 0, ring, wave, stages, reinterpret_cast<float *>(tab));
             else
-                pk_narrow<2, true>(p, it, 1, 0, ring, wave, stages, reinterpret_cast<float *>(tab));
+                pk_narrow<2, true>(p, it, 0, ring, wave, stages, reinterpret_cast<float *>(tab));
         }
         if (N <= G) break;
         __syncthreads();   /* sh_next, the stages and the table are used again */
@@ -980,23 +980,21 @@ __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
         const int chunks = it.q.nch;
         const long long slot0 = uni(nslots[it.b]) + (long long)it.kvh * chunks;
         if (it.tn <= p.tpt)
-            pk_narrow<1, false>(p, it, chunks, slot0 + j, ring, 0, nullptr, nullptr);
+            pk_narrow<1, false>(p, it, slot0 + j, ring, 0, nullptr, nullptr);
         else
-            pk_narrow<2, false>(p, it, chunks, slot0 + j, ring, 0, nullptr, nullptr);
+            pk_narrow<2, false>(p, it, slot0 + j, ring, 0, nullptr, nullptr);
         int got = 0;
         if (queued && lane == 0) got = pk_draw(tickets, own);
         __builtin_amdgcn_s_waitcnt(pk_wait(0, 15));   /* nothing is in flight into the ring, and the partial is out */
-        if (chunks > 1) {
-            int *arrived = p.arrived + uni(units[it.b]) + it.kvh;
-            int prior = 0;
-            if (lane == 0) prior = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (uni(prior) == chunks - 1) {
-                if (it.tn * a.G <= 4)
-                    pk_merge<2, 16>(p, it, chunks, slot0, lane);
-                else
-                    pk_merge<4, 8>(p, it, chunks, slot0, lane);
-                if (lane == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+        int *arrived = p.arrived + uni(units[it.b]) + it.kvh;   /* an uncut sequence is an "alone" item: there are others */
+        int prior = 0;
+        if (lane == 0) prior = __hip_atomic_fetch_add(arrived, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (uni(prior) == chunks - 1) {
+            if (it.tn * a.G <= 4)
+                pk_merge<2, 16>(p, it, chunks, slot0, lane);
+            else
+                pk_merge<4, 8>(p, it, chunks, slot0, lane);
+            if (lane == 0) __hip_atomic_store(arrived, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         if (!queued) break;
         k = pk_next(tickets, first, NN, own, got, lane);

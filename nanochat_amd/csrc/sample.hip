@@ -278,7 +278,7 @@ struct Split {
     __device__ __forceinline__ u64 *part(int of) const { return s.part + ((long long)row * G + of) * ST_PART; }
     __device__ __forceinline__ int *counter() const { return s.count + (long long)row * ST_LINE; }
 
-    /* Once every thread's stores are out: one arrival of this workgroup, its number among the row's. */
+    /* Until every thread's stores are out. */
     __device__ __forceinline__ void arrive() {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -297,7 +297,7 @@ struct Split {
             __syncthreads();
         }
     }
-    /* One word of every workgroup's head, into sh.head. The caller met before, and synchronizes after. */
+    /* A word of a head: of workgroup t's by thread t, after a meeting, and this workgroup's own. */
     __device__ __forceinline__ u64 head_of(int word) const { return peek(part(t) + ST_BINS + 2 * ST_LIST + word); }
     __device__ __forceinline__ void tell(int word, u64 v) const { publish(mine + ST_BINS + 2 * ST_LIST + word, v); }
 
@@ -1137,7 +1137,7 @@ __device__ __forceinline__ bool row_bin(RowShared &sh, Target target) {
 template <bool SPLIT, int AHEAD, typename In, typename M, typename Target>
 __device__ __forceinline__ Cut row_cut(RowShared &sh, const Row<AHEAD> &row, float zmax, float range, In in, M m,
                                        Target target) {
-    const int t = threadIdx.x, lane = row.lane, wave = t >> 6;
+    const int t = threadIdx.x, lane = row.lane;
     const float scale = range > 0.0f && range < INFINITY ? (RW_BINS - 1) / range : 0.0f;
     /* a range whose products are NaN or past the last bin: the last bin; monotone in z in every case */
     const auto bin_of = [&](float z) { return z == zmax ? 0 : (int)fminf((zmax - z) * scale, (float)(RW_BINS - 1)); };
