@@ -21,8 +21,8 @@
  * 4,096), which stay in its registers. What bounds it is neither bytes nor operations (a row of 65,536 fp32 logits is 256 KiB) but the steps one
  * after the other, each ending where the row's workgroups need one another: the largest logit; the histogram; the list; about
  * 2.5 us a meeting through memory. Greedy rows and a top-k of at most 128 need no meeting: every slice leaves its k largest in
- * order, and the last workgroup to arrive does the rest on k tokens. Measured: one row of 65,536 fp32 logits with top-p 26 us,
- * with top-k 14; 64 rows 39 and 20.
+ * order, and the last workgroup to arrive does the rest on k tokens. Measured: one row of 65,536 fp32 logits with top-p 22 us,
+ * with top-k 14; 64 rows 38 and 20.
  *
  * row_kernel takes a row by one workgroup that reads it again for every step, for more rows and for longer ones. With top-p
  * it is bound by the exponentials, twice for every token (about 180 cycles of a SIMD for a wave's 64, most of them float64
@@ -138,9 +138,9 @@ struct Cut {
 
 /* --- Rows of up to ST_MAX_GROUPS slices of 8,192 or 4,096 tokens, a workgroup each: the slice stays in its registers, E (16
  * or 8) tokens a thread, and the workgroups of a row exchange what the next step needs through memory. 512 threads of at most 128 registers
- * and the weights in LDS leave room for two workgroups a CU, one working while the other waits: one workgroup a CU (no
- * spilled registers, 149 of them) takes 25 us for one row instead of 27, but 124 instead of 88 for 333 rows, and slices of
- * 1,024 threads with 8 tokens each 30 and 150. */
+ * and the weights in LDS leave room for two workgroups a CU, one working while the other waits: measured side by side, one
+ * workgroup a CU (149 registers, none spilled) took 25 us for one row instead of 27, but 124 instead of 88 for 333 rows, and
+ * slices of 1,024 threads with 8 tokens each 30 and 150. */
 
 constexpr int ST_WAVES = 8, ST_THREADS = ST_WAVES * WAVE;
 constexpr int ST_STEP = 4 * ST_THREADS;   /* element 4 c + j of thread t: index slice + c ST_STEP + 4 t + j */
@@ -627,10 +627,19 @@ __device__ __forceinline__ Cut split_cut(Split<E> &q, float (&x)[E], uint32_t li
             publish(part(q.g) + 2 * t + 1, v[1]);
             q.meet();
             v[0] = v[1] = 0;
-#pragma unroll 4
-            for (int o = 0; o < G; o++) {
-                v[0] += peek(part(o) + 2 * t);
-                v[1] += peek(part(o) + 2 * t + 1);
+            for (int o = 0; o < G; o += 8) {   /* eight workgroups' loads in flight */
+                u64 other[8][2];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const u64 *p = part(min(o + k, G - 1)) + 2 * t;
+                    other[k][0] = peek(p);
+                    other[k][1] = peek(p + 1);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    v[0] += o + k < G ? other[k][0] : 0;
+                    v[1] += o + k < G ? other[k][1] : 0;
+                }
             }
         }
         const u64 scan = lane_scan64(v[0] + v[1]);
@@ -751,11 +760,16 @@ __device__ __forceinline__ Cut split_cut(Split<E> &q, float (&x)[E], uint32_t li
             __syncthreads();
             n = alike(sh.start[G]);
             if (n <= ST_LIST) {
-                for (int o = wave; o < G; o += ST_WAVES)
-                    for (int i = lane; i < sh.start[o + 1] - sh.start[o]; i += WAVE) {
-                        sh.code[sh.start[o] + i] = peek(part(o) + ST_BINS + i);
-                        sh.w[sh.start[o] + i] = peek(part(o) + ST_BINS + ST_LIST + i);
-                    }
+                if (t < n) {   /* entry t: of the last workgroup that starts at or before it */
+                    int o = 0;
+#pragma unroll
+                    for (int k = ST_MAX_GROUPS / 2; k; k >>= 1)
+                        if (o + k < G && sh.start[o + k] <= t) o += k;
+                    const u64 *entry = part(o) + ST_BINS + t - sh.start[o];
+                    const u64 code = peek(entry), of = peek(entry + ST_LIST);
+                    sh.code[t] = code;
+                    sh.w[t] = of;
+                }
             }
         } else {
             if (t < min(n, ST_LIST)) sh.w[t] = listed(sh.code[t]);
@@ -1393,7 +1407,7 @@ using namespace nc;
  * long as a row's own work: 128 rows of 65,536 tokens (two rounds of slices) take 35 us in slices and 24 whole with a top-k of
  * 40, 21 and 10 greedily, 75 and 84 with top-p; 256 rows with top-p 142 and 94, and 64 rows (one round) with a top-k 20 and 23.
  * Half slices where one suffices, or where they are at most one a CU and few to a row: one row of 3,000 tokens 15 -> 11 us,
- * 16 rows of 32,768 tokens 25.6 -> 23.5; but two a CU, for 32 rows of 65,536 tokens, take 37 us and whole slices 31. */
+ * 16 rows of 32,768 tokens 25.6 -> 23.5; but two a CU, for 32 rows of 65,536 tokens, took 37 us and whole slices 31. */
 static int split_groups(long long rows, int vocab, int &e) {
     const int half = ST_MAX_E / 2 * ST_THREADS, halves = (vocab + half - 1) / half;
     e = halves == 1 || (halves > 2 && halves <= ST_MAX_GROUPS / 2 && rows * halves <= ST_MAX_WORKGROUPS / 2) ? ST_MAX_E / 2
