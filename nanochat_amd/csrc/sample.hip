@@ -137,10 +137,10 @@ struct Cut {
 };
 
 /* --- Rows of up to ST_MAX_GROUPS slices of 8,192 or 4,096 tokens, a workgroup each: the slice stays in its registers, E (16
- * or 8) tokens a thread, and the workgroups of a row exchange what the next step needs through memory. 512 threads of at most 128 registers
- * and the weights in LDS leave room for two workgroups a CU, one working while the other waits: measured side by side, one
- * workgroup a CU (149 registers, none spilled) took 25 us for one row instead of 27, but 124 instead of 88 for 333 rows, and
- * slices of 1,024 threads with 8 tokens each 30 and 150. */
+ * or 8) tokens a thread, and the workgroups of a row exchange what the next step needs through memory. 512 threads of at most
+ * 128 registers and the weights in LDS leave room for two workgroups a CU, one working while the other waits: measured side by
+ * side, one workgroup a CU (149 registers, none spilled) took 25 us for one row instead of 27, but 124 instead of 88 for 333
+ * rows, and slices of 1,024 threads with 8 tokens each 30 and 150. */
 
 constexpr int ST_WAVES = 8, ST_THREADS = ST_WAVES * WAVE;
 constexpr int ST_STEP = 4 * ST_THREADS;   /* element 4 c + j of thread t: index slice + c ST_STEP + 4 t + j */
