@@ -28,7 +28,7 @@
  * XCD's L2), so that unequal items even out.
  *
  * Measured (16 query heads, 4 KV heads): 64 sequences of 8,192 keys, one row each 98 us (5.6 TB/s of pages), 4 rows each
- * 110 us (5.0), 16 rows each 172 us; 8 prompt chunks of 257 to 512 rows over at most 4,096 keys 175 us (736 TFLOP/s of the
+ * 110 us (5.0), 16 rows each 172 us; 8 prompt chunks of 512 rows, each over 4,096 keys, 175 us (736 TFLOP/s of the
  * keys a row may see), 2 prompts of 4,096 rows 173 us (795). One sequence, 5 rows of 6 heads over 1,029 keys: 14 us, most of
  * it round trips to memory one after the other (the plan, the block table, pages, the output).
  */
@@ -52,7 +52,7 @@ constexpr int PK_MIN_TAIL = 4;                 /* a last chunk of fewer pages jo
 constexpr int PK_SHORT = 2 * PK_NARROW_SPLIT;
 /* Least and most pages of a wide chunk, and the items that a wide sequence is cut into at most if its chunks stay that long.
  * Short chunks fill the chip when a sequence is alone, and cost partials when it is not: one chunk of 512 rows over 8,192 keys
- * takes 69 us with 128 pages at least and 113 with 256, eight of them over at most 4,096 keys 175 and 153 (64 pages: 69 and
+ * takes 69 us with 128 pages at least and 113 with 256, eight of them over 4,096 keys 175 and 153 (64 pages: 69 and
  * 204). A cut by what else the launch holds would make a sequence's bits depend on it. 128 items: 114 us for the first, and
  * 260 instead of 175 for 4 chunks of 200 to 700 rows among 60 decoding sequences. */
 constexpr int PK_WIDE_MIN = 128, PK_WIDE_MAX = 1024, PK_WIDE_ITEMS = 256;
