@@ -322,12 +322,20 @@ size_t nc_sample_workspace_bytes(long long rows, int vocab);
  * (taken into [0, 1]); tokens[row] is the first, in index order, whose running weight exceeds uniform[row] (in [0, 1),
  * else the nearer end; NaN: 0) times the weight of all that are left; -1 where no token is allowed. Weights are held to
  * 2^-46 of the largest (2^(ceil(log2 vocab) - 62) from 65,537 tokens on): smaller ones are never drawn. The result is
- * reproducible and does not depend on the other rows. rows <= 2^22; no rows launch nothing.
+ * reproducible and does not depend on the other rows. Calls on any number of streams may overlap, each with a workspace of
+ * its own: no workgroup waits without bound for one that may not have started. rows <= 2^22; no rows launch nothing.
  */
 int nc_sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
                      const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
                      const float *min_p, const uint32_t *mask, long long mask_stride, int32_t *tokens, void *workspace,
                      size_t workspace_bytes, void *stream);
+
+/* For tests and measurement: nc_sample_tokens, the workgroups that share a row looking for one another `patience` times
+ * (in [0, 65536]) before they give it up and the last of them does it by itself. The tokens are the same. */
+int nc_debug_sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
+                           const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
+                           const float *min_p, const uint32_t *mask, long long mask_stride, int32_t *tokens,
+                           void *workspace, size_t workspace_bytes, int patience, void *stream);
 
 /*
  * Measurement only; no counterpart in the reference. Reads n pages of 2 KiB (one (page, head) of K or V codes) from

@@ -21,7 +21,8 @@
  * 4,096), which stay in its registers. What bounds it is neither bytes nor operations (a row of 65,536 fp32 logits is 256 KiB) but the steps one
  * after the other, each ending where the row's workgroups need one another: the largest logit; the histogram; the list; about
  * 2.5 us a meeting through memory. Greedy rows and a top-k of at most 128 need no meeting: every slice leaves its k largest in
- * order, and the last workgroup to arrive does the rest on k tokens. Measured: one row of 65,536 fp32 logits with top-p 22 us,
+ * order, and the last workgroup to arrive does the rest on k tokens. No meeting waits without bound: where the others
+ * do not come, because the device is crowded, a row is given up and one workgroup does it (nc_meeting.h). Measured: one row of 65,536 fp32 logits with top-p 22 us,
  * with top-k 14; 64 rows 38 and 20.
  *
  * row_kernel takes a row by one workgroup that reads it again for every step, for more rows and for longer ones. With top-p
@@ -32,6 +33,8 @@
 #include <math.h>
 
 #include "nc_device.h"
+#include "nc_internal.h"
+#include "nc_meeting.h"
 #include "nanochat_amd.h"
 
 namespace nc {
@@ -151,7 +154,13 @@ constexpr int ST_TOP = 128;               /* the largest top-k settled by lists 
 constexpr int ST_CAND = 4096;             /* candidates: at most ST_TOP of 32 tokens, or of ST_MAX_GROUPS lists */
 constexpr int ST_LINE = 32;               /* ints of a 128-byte line: counts that several workgroups add to share none */
 constexpr int ST_QUEUES = 8;              /* XCDs */
-constexpr int ST_MAX_WORKGROUPS = 512;    /* of rows that are cut: as many as run at once, two a CU */
+constexpr int ST_MAX_WORKGROUPS = 512;    /* of rows that are cut: as many as run at once on 256 CUs, two a CU */
+/* Looks at a row's word, each a round trip past the L2, before it is given up. The longest meeting is the first, which waits for
+ * the last workgroups to start: 16 looks were enough for 64 rows of 65,536 tokens (42 us; given up after 8 looks 150), not for
+ * 16 rows of 262,144 (71 us; given up 700). What giving up costs is the row done by one workgroup, so waiting about as long
+ * as that takes is at most twice the better choice. */
+constexpr int ST_PATIENCE = 400;
+static_assert(ST_MAX_GROUPS <= MT_MOST_LEFT, "workgroups of a row that have left are counted");
 constexpr int ST_MAX_E = 16;              /* tokens a thread: this many, or half */
 static_assert(ST_TOP * (ST_MAX_E * ST_THREADS / 256) <= ST_CAND && ST_TOP * ST_MAX_GROUPS <= ST_CAND, "candidates fit");
 
@@ -163,6 +172,18 @@ struct SplitArgs {
     int rows, groups;      /* slices a row */
     u64 *part;             /* [rows][groups][ST_PART] */
     int *tickets, *done, *count;   /* [ST_QUEUES], [ST_QUEUES], [rows] lines; zero between launches */
+    int patience;
+};
+
+/* A row's word (nc_meeting.h). */
+struct RowWord {
+    int *p;
+    __device__ __forceinline__ int add(int n) { return __hip_atomic_fetch_add(p, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+    __device__ __forceinline__ int look() const { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+    __device__ __forceinline__ bool swap(int &expected, int desired) {
+        return __hip_atomic_compare_exchange_strong(p, &expected, desired, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                                    __HIP_MEMORY_SCOPE_AGENT);
+    }
 };
 
 template <int E>
@@ -272,6 +293,7 @@ struct Split {
     int row, g, G;         /* row, slice, slices */
     int first;             /* index of this thread's element 0 */
     int reached;           /* arrivals that the last wait of this row asked for */
+    int gone;              /* the row was given up */
     u64 *mine;
 
     __device__ __forceinline__ int index(int e) const { return first + (e >> 2) * ST_STEP + (e & 3); }
@@ -283,36 +305,41 @@ struct Split {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     }
-    /* Until every workgroup of the row has come as far: what they published is there. Workgroups take rows by tickets, so
-     * those of a row whose others have not started are the last G - 1 at most, and every earlier row's can end. */
-    __device__ __forceinline__ void meet() {
+    /* Until every workgroup of the row has come as far: what they published is there. False: the row was given up, by this
+     * workgroup or another, and is to be left at once. Every wait ends (nc_meeting.h), whatever else the device runs. */
+    __device__ __forceinline__ bool meet() {
         arrive();
-        if (G > 1) {
-            reached += G;
-            if (t == 0) {
-                __hip_atomic_fetch_add(counter(), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                while (__hip_atomic_load(counter(), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < reached)
-                    __builtin_amdgcn_s_sleep(1);
+        if (G == 1) return true;
+        reached += G;
+        if (t == 0) {
+            RowWord word{counter()};
+            int seen = word.add(1) + 1, patience = s.patience;
+            Meeting m;
+            while ((m = meeting_look(word, seen, reached, patience)) == MT_WAIT) {
+                __builtin_amdgcn_s_sleep(1);
+                seen = word.look();
             }
-            __syncthreads();
+            sh.flag = m == MT_GONE;
         }
+        __syncthreads();
+        gone = __builtin_amdgcn_readfirstlane(sh.flag);
+        return !gone;
     }
     /* A word of a head: of workgroup t's by thread t, after a meeting, and this workgroup's own. */
     __device__ __forceinline__ u64 head_of(int word) const { return peek(part(t) + ST_BINS + 2 * ST_LIST + word); }
     __device__ __forceinline__ void tell(int word, u64 v) const { publish(mine + ST_BINS + 2 * ST_LIST + word, v); }
 
-    /* The last of a row's workgroups to leave clears its count, the last row's of a queue clears the queue. */
-    __device__ __forceinline__ void leave(bool counted) {
-        if (G == 1 || t != 0) return;
-        if (!counted) {
-            if (__hip_atomic_fetch_add(counter(), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != reached + G - 1) return;
-        }
+    /* The last of a row's workgroups to leave clears its word, the last row's of a queue clears the queue. By thread 0;
+     * whether it is the last. `alone`: nobody else of the row is there. */
+    __device__ __forceinline__ bool leave(bool alone) {
+        if (!alone && !meeting_last(RowWord{counter()}.add(MT_LEFT), G)) return false;
         __hip_atomic_store(counter(), 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const int y = row % ST_QUEUES, rows = (s.rows - y + ST_QUEUES - 1) / ST_QUEUES;
         if (__hip_atomic_fetch_add(s.done + y * ST_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == rows - 1) {
             __hip_atomic_store(s.tickets + y * ST_LINE, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_store(s.done + y * ST_LINE, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
+        return true;
     }
 };
 
@@ -559,7 +586,7 @@ __device__ __forceinline__ int split_pick(const Split<E> &q, uint32_t in, M m, u
  * first, reaches target(total). Ranges of values are narrowed by histograms, which the workgroups publish and each adds up,
  * until the tokens of the one that holds the cut fit a list, which each settles pairwise. Between two histograms, and between
  * two lists, there is always a meeting after the first is read. sh.kept: per slice the weight of the tokens down to the cut
- * that weigh least_w or more (not SPLIT). Every thread of every workgroup of the row calls it. */
+ * that weigh least_w or more (not SPLIT). Every thread of every workgroup of the row calls it, and looks at q.gone after it. */
 template <bool SPLIT, int E, typename Target>
 __device__ __forceinline__ Cut split_cut(Split<E> &q, float (&x)[E], uint32_t live, float zmax, float range, u64 least_w,
                                          Target target) {
@@ -625,7 +652,7 @@ __device__ __forceinline__ Cut split_cut(Split<E> &q, float (&x)[E], uint32_t li
         if (G > 1) {
             publish(part(q.g) + 2 * t, v[0]);
             publish(part(q.g) + 2 * t + 1, v[1]);
-            q.meet();
+            if (!q.meet()) return Cut{false, 0u, 0};
             v[0] = v[1] = 0;
             for (int o = 0; o < G; o += 8) {   /* eight workgroups' loads in flight */
                 u64 other[8][2];
@@ -655,7 +682,7 @@ __device__ __forceinline__ Cut split_cut(Split<E> &q, float (&x)[E], uint32_t li
             goal = target(total);
             if (alike((int)(goal > total))) {
                 q.meet();   /* the histograms are published over by the next cut: not before everyone has read these */
-                return Cut{false, 0u, 0};
+                return Cut{false, 0u, 0};   /* or the row was given up */
             }
         }
         const u64 rest = goal - base;
@@ -731,7 +758,7 @@ __device__ __forceinline__ Cut split_cut(Split<E> &q, float (&x)[E], uint32_t li
                 tell(HD_LEAST, sh.lo);
                 tell(HD_MOST, sh.hi);
             }
-            q.meet();
+            if (!q.meet()) return Cut{false, 0u, 0};
             if (wave == 0) {
                 int count = 0;
                 u64 l = ~0ull, h = 0;
@@ -821,30 +848,14 @@ __device__ __forceinline__ Cut split_cut(Split<E> &q, float (&x)[E], uint32_t li
     }
 }
 
+/* This workgroup's part of its row. Returns whether it is still to leave the row; q.gone: the row was given up, and has no
+ * token. */
 template <int E>
-__global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
-    __shared__ SplitShared<E> sh;
-    const SampleArgs &a = s.a;
-    Split<E> q = {s, sh};
-    q.t = threadIdx.x;
-    q.lane = q.t & (WAVE - 1);
-    q.wave = q.t >> 6;
-    q.G = s.groups;
-    q.row = blockIdx.x;
-    q.g = 0;
-    if (q.G > 1) {   /* every eighth workgroup, which one XCD runs, draws on one queue, and a row is one queue's */
-        const int y = blockIdx.x % ST_QUEUES, rows = (s.rows - y + ST_QUEUES - 1) / ST_QUEUES;
-        if ((int)(blockIdx.x / ST_QUEUES) >= rows * q.G) return;
-        if (q.t == 0)
-            sh.n = __hip_atomic_fetch_add(s.tickets + y * ST_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        const int ticket = alike(sh.n);
-        q.row = y + ticket / q.G * ST_QUEUES;
-        if (q.row >= s.rows) return;   /* counts that were not zero: no access out of bounds */
-        q.g = ticket % q.G;
-    }
+__device__ __forceinline__ bool split_row(Split<E> &q) {
+    SplitShared<E> &sh = q.sh;
+    const SampleArgs &a = q.s.a;
     q.first = q.g * E * ST_THREADS + 4 * q.t;
-    q.reached = 0;
+    q.reached = q.gone = 0;
     q.mine = q.part(q.g);
     const int t = q.t, lane = q.lane, wave = q.wave, G = q.G;
     const long long r = q.row;
@@ -870,7 +881,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
                 sh.n = 0;
             }
             __syncthreads();
-            if (!alike(sh.flag)) return;
+            if (!alike(sh.flag)) return false;
             /* every list's ceil(k / G)-th: k tokens reach the least of them */
             const int quota = (k + G - 1) / G;
             if (wave == 0) {
@@ -893,15 +904,15 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
                 }
             __syncthreads();
             n = alike(sort_codes<ST_THREADS>(sh, alike(sh.n), k));
-            q.leave(true);
+            if (t == 0) q.leave(true);
         }
         if (n == 0 || k == 1) {
             if (t == 0) a.out[r] = n == 0 ? -1 : code_index(sh.top[0]);
-            return;
+            return false;
         }
         with.zmax = key_value((uint32_t)(sh.top[0] >> 32));
         choose_top(sh, n, weight, with.p < 1.0f, mass_goal, with.least_w, choice, a.out + r);
-        return;
+        return false;
     }
 
     /* the largest allowed logit and the smallest */
@@ -914,7 +925,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     for (int round = 0; round < (G > 1 ? 2 : 1); round++) {
         if (round) {
             if (t == 0) q.tell(HD_BEST, (u64)__float_as_uint(most) << 32 | __float_as_uint(least));
-            q.meet();
+            if (!q.meet()) return true;
             if (t < G) {
                 const u64 of = q.head_of(HD_BEST);
                 most = __uint_as_float((uint32_t)(of >> 32));
@@ -936,8 +947,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     least = alike(least);
     if (most == -INFINITY) {
         if (t == 0 && q.g == 0) a.out[r] = -1;
-        q.leave(false);
-        return;
+        return true;
     }
     with.zmax = most;
     anew(x);
@@ -948,6 +958,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
         for (int e = 0; e < E; e++) live |= (uint32_t)(x[e] > -INFINITY) << e;
         const Cut top = split_cut<true>(q, x, live, with.zmax, with.zmax - least, 0ull,
                                         [&](u64) { return (u64)k; });
+        if (q.gone) return true;
         if (top.some) {
             const float z = key_value(top.key);
 #pragma unroll
@@ -968,6 +979,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
     if (with.p < 1.0f) {
         const Cut mass = split_cut<false>(q, x, live, with.zmax, fminf(with.zmax - least, with.range(a.vocab)), with.least_w,
                                           mass_goal);
+        if (q.gone) return true;
         if (mass.some) least_z = key_value(mass.key);
     } else {
         u64 own = 0;
@@ -986,7 +998,7 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
             if (G > 1) q.tell(HD_SUM, own);
             else sh.kept[0] = own;
         }
-        q.meet();
+        if (!q.meet()) return true;
         if (G > 1) {
             if (t < G) sh.kept[t] = q.head_of(HD_SUM);
             __syncthreads();
@@ -1006,33 +1018,35 @@ __global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
         const int token = split_pick(q, kept, [&](int e) { return sh.weight[e * ST_THREADS + t]; }, goal - before);
         if (t == 0) a.out[r] = token;
     }
-    q.leave(false);
+    return true;
 }
 
 /* --- Rows by one workgroup each, read again for every step: where rows are many, or longer than the slices allow. Wave w
  * takes a contiguous run of the row, so that a sum in index order is a sum over waves, then over one wave. */
 
-constexpr int RW_WAVES = 16, RW_THREADS = RW_WAVES * WAVE;
+constexpr int RW_WAVES = 16, RW_THREADS = RW_WAVES * WAVE;   /* of row_kernel; W: of whoever takes a row */
 constexpr int RW_CHUNK = 4 * WAVE;       /* elements of a wave's chunk: four a lane */
-constexpr int RW_BINS = 4 * RW_THREADS;
-constexpr int RW_LIST = 512;             /* tokens a range may hold to be settled pairwise */
-constexpr int RW_CUS = 256;              /* rows that run at once, a workgroup a CU */
 
+template <int W>
 struct RowShared {
+    static constexpr int THREADS = W * WAVE;
+    static constexpr int BINS = 4 * THREADS;
+    static constexpr int LIST = THREADS / 2;   /* tokens a range may hold to be settled pairwise */
     union {
-        u64 hist[RW_BINS];
+        u64 hist[BINS];
         u64 cand[ST_CAND];
     };
     u64 top[ST_TOP], top_w[ST_TOP], kept_w[ST_TOP], most[256];
-    int rank[RW_THREADS];
-    u64 code[RW_LIST], w[RW_LIST];
-    u64 sum[RW_WAVES];
+    int rank[THREADS];
+    u64 code[LIST], w[LIST];
+    u64 sum[W];
     u64 found, least_code, lo, hi;
     int bin, n, token;
 };
+static_assert(sizeof(RowShared<ST_WAVES>) <= sizeof(SplitShared<ST_MAX_E / 2>), "a row that was given up fits");
 
 /* Element j of lane l of chunk c of wave w is index (w per + c) RW_CHUNK + 4 l + j. */
-template <int AHEAD>   /* chunks in flight */
+template <int AHEAD, int W>   /* chunks in flight, waves */
 struct Row {
     const SampleArgs &a;
     const char *p;
@@ -1042,7 +1056,7 @@ struct Row {
     __device__ __forceinline__ Row(const SampleArgs &args, long long row)
         : a(args), p((const char *)args.logits + row * args.stride * (args.bf16 ? 2 : 4)),
           mask(args.mask ? args.mask + row * args.mask_stride : nullptr) {
-        per = (a.vocab + RW_WAVES * RW_CHUNK - 1) / (RW_WAVES * RW_CHUNK);
+        per = (a.vocab + W * RW_CHUNK - 1) / (W * RW_CHUNK);
         lane = threadIdx.x & (WAVE - 1);
         base = alike((int)(threadIdx.x >> 6)) * per * RW_CHUNK;
     }
@@ -1110,8 +1124,8 @@ struct Row {
 
 /* The bins' sums in order: sh.bin is the first bin at which the running sum reaches target(total), sh.found the sum
  * before it. Returns whether there is one. Every thread must call it. */
-template <typename Target>
-__device__ __forceinline__ bool row_bin(RowShared &sh, Target target) {
+template <int W, typename Target>
+__device__ __forceinline__ bool row_bin(RowShared<W> &sh, Target target) {
     const int t = threadIdx.x, lane = t & (WAVE - 1), wave = t >> 6;
     u64 v[4], own = 0;
     __syncthreads();
@@ -1125,7 +1139,7 @@ __device__ __forceinline__ bool row_bin(RowShared &sh, Target target) {
     __syncthreads();
     u64 before = scan - own, total = 0;
 #pragma unroll
-    for (int w = 0; w < RW_WAVES; w++) {
+    for (int w = 0; w < W; w++) {
         before += w < wave ? sh.sum[w] : 0;
         total += sh.sum[w];
     }
@@ -1148,18 +1162,19 @@ __device__ __forceinline__ bool row_bin(RowShared &sh, Target target) {
  * target(total). SPLIT: equals are taken one by one, the lower index first (m is 1), and the cut's idx is the last one
  * taken; else they are taken together. `range`: the values below zmax - range need no telling apart. Every thread must
  * call it. */
-template <bool SPLIT, int AHEAD, typename In, typename M, typename Target>
-__device__ __forceinline__ Cut row_cut(RowShared &sh, const Row<AHEAD> &row, float zmax, float range, In in, M m,
+template <bool SPLIT, int AHEAD, int W, typename In, typename M, typename Target>
+__device__ __forceinline__ Cut row_cut(RowShared<W> &sh, const Row<AHEAD, W> &row, float zmax, float range, In in, M m,
                                        Target target) {
+    constexpr int THREADS = RowShared<W>::THREADS, BINS = RowShared<W>::BINS, LIST = RowShared<W>::LIST;
     const int t = threadIdx.x, lane = row.lane;
-    const float scale = range > 0.0f && range < INFINITY ? (RW_BINS - 1) / range : 0.0f;
+    const float scale = range > 0.0f && range < INFINITY ? (BINS - 1) / range : 0.0f;
     /* a range whose products are NaN or past the last bin: the last bin; monotone in z in every case */
-    const auto bin_of = [&](float z) { return z == zmax ? 0 : (int)fminf((zmax - z) * scale, (float)(RW_BINS - 1)); };
+    const auto bin_of = [&](float z) { return z == zmax ? 0 : (int)fminf((zmax - z) * scale, (float)(BINS - 1)); };
     const auto key = [&](float z, int i) { return SPLIT ? token_code(z, i) : (u64)order_key(z); };
     const auto clear = [&]() {
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < 4; k++) sh.hist[t + k * RW_THREADS] = 0;
+        for (int k = 0; k < 4; k++) sh.hist[t + k * THREADS] = 0;
         if (t == 0) {
             sh.n = 0;
             sh.least_code = sh.lo = ~0ull;
@@ -1173,12 +1188,12 @@ __device__ __forceinline__ Cut row_cut(RowShared &sh, const Row<AHEAD> &row, flo
     row.each([&](float z, int i) {
         const u64 w = in(z, i) ? m(z) : 0;
         const int b = bin_of(z);
-        if (b < RW_BINS - 1)
+        if (b < BINS - 1)
             __hip_atomic_fetch_add(&sh.hist[b], w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        rest += b == RW_BINS - 1 ? w : 0;
+        rest += b == BINS - 1 ? w : 0;
     });
     rest = lane_sum64(rest);
-    if (lane == 0) __hip_atomic_fetch_add(&sh.hist[RW_BINS - 1], rest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    if (lane == 0) __hip_atomic_fetch_add(&sh.hist[BINS - 1], rest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     if (!row_bin(sh, [&](u64 total) { return goal = target(total); })) return Cut{false, 0u, 0};
     const int bin = alike(sh.bin);
     u64 base = sh.found, lo = 0, hi = ~0ull;   /* once a range of values is split again: its keys */
@@ -1193,7 +1208,7 @@ __device__ __forceinline__ Cut row_cut(RowShared &sh, const Row<AHEAD> &row, flo
         row.each([&](float z, int i) {
             if (member(z, i)) {
                 const int at = __hip_atomic_fetch_add(&sh.n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                if (at < RW_LIST) {
+                if (at < LIST) {
                     sh.code[at] = token_code(z, i);
                     sh.w[at] = m(z);
                 }
@@ -1201,9 +1216,9 @@ __device__ __forceinline__ Cut row_cut(RowShared &sh, const Row<AHEAD> &row, flo
         });
         __syncthreads();
         const int n = alike(sh.n);
-        if (n <= RW_LIST) {   /* pairwise, up to 16 neighbours a token */
+        if (n <= LIST) {   /* pairwise, up to 16 neighbours a token */
             int parts = 16;
-            while (parts > 2 && parts * n > RW_THREADS) parts >>= 1;
+            while (parts > 2 && parts * n > THREADS) parts >>= 1;
             const int i = t / parts;
             const u64 c = i < n ? sh.code[i] : ~0ull;
             u64 more = 0;
@@ -1239,7 +1254,7 @@ __device__ __forceinline__ Cut row_cut(RowShared &sh, const Row<AHEAD> &row, flo
         }
         if (!SPLIT && lo == hi) return Cut{true, (uint32_t)lo, 0x7FFFFFFF};   /* one value */
         int shift = 0;
-        while ((hi - lo) >> shift >= RW_BINS) shift++;
+        while ((hi - lo) >> shift >= BINS) shift++;
         clear();
         row.each([&](float z, int i) {   /* the larger keys first */
             if (member(z, i))
@@ -1256,8 +1271,8 @@ __device__ __forceinline__ Cut row_cut(RowShared &sh, const Row<AHEAD> &row, flo
 }
 
 /* The first element in index order at which the running sum of m(z, index) reaches goal(total). Every thread must call it. */
-template <int AHEAD, typename M, typename Goal>
-__device__ __forceinline__ int row_pick(RowShared &sh, const Row<AHEAD> &row, M m, Goal goal) {
+template <int AHEAD, int W, typename M, typename Goal>
+__device__ __forceinline__ int row_pick(RowShared<W> &sh, const Row<AHEAD, W> &row, M m, Goal goal) {
     const int lane = row.lane, wave = threadIdx.x >> 6;
     u64 s = 0;
     row.each([&](float z, int i) { s += m(z, i); });
@@ -1267,7 +1282,7 @@ __device__ __forceinline__ int row_pick(RowShared &sh, const Row<AHEAD> &row, M 
     __syncthreads();
     u64 before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < RW_WAVES; w++) {
+    for (int w = 0; w < W; w++) {
         before += w < wave ? sh.sum[w] : 0;
         total += sh.sum[w];
     }
@@ -1302,15 +1317,12 @@ __device__ __forceinline__ int row_pick(RowShared &sh, const Row<AHEAD> &row, M 
     return sh.token;
 }
 
-/* Two forms, with the same results: four chunks in flight, 93 registers, a workgroup a CU; or two chunks and 64 registers, two
- * workgroups a CU, where there are more rows than CUs: 333 rows of 32,768 tokens with top-p 102 and 85 us, 256 of 65,536 94 and
- * 95, 128 of them with a top-k 23.6 and 25.0. */
-template <int AHEAD>
-__global__ void __launch_bounds__(RW_THREADS, AHEAD == 4 ? 4 : 8) row_kernel(SampleArgs a) {
-    __shared__ RowShared sh;
-    const long long r = blockIdx.x;
+/* A row's token by W waves of one workgroup. */
+template <int AHEAD, int W>
+__device__ __forceinline__ void row_choose(const SampleArgs &a, long long r, RowShared<W> &sh) {
+    constexpr int THREADS = RowShared<W>::THREADS;
     const int t = threadIdx.x, lane = t & (WAVE - 1), wave = t >> 6;
-    const Row<AHEAD> row(a, r);
+    const Row<AHEAD, W> row(a, r);
 
     /* the largest allowed logit (the lowest index among equals) and the smallest */
     float most = -INFINITY, least = INFINITY;
@@ -1331,7 +1343,7 @@ __global__ void __launch_bounds__(RW_THREADS, AHEAD == 4 ? 4 : 8) row_kernel(Sam
     if (t == 0) sh.n = 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < RW_WAVES; w++) {
+    for (int w = 0; w < W; w++) {
         best = max(best, sh.sum[w]);
         least = fminf(least, __int_as_float(sh.rank[w]));
     }
@@ -1346,10 +1358,12 @@ __global__ void __launch_bounds__(RW_THREADS, AHEAD == 4 ? 4 : 8) row_kernel(Sam
     const Choice with(a, r, T, key_value((uint32_t)(best >> 32)));
 
     if (k > 0 && k <= ST_TOP) {
-        /* as split_top: the tokens that reach a bound which k groups of four threads reach */
-        u64 group = max(own, (u64)__shfl_xor(own, 1, WAVE));
-        group = max(group, (u64)__shfl_xor(group, 2, WAVE));
-        if ((t & 3) == 0) sh.most[t >> 2] = group;
+        /* as split_top: the tokens that reach a bound which k of 256 groups of threads reach */
+        constexpr int PER = THREADS / 256;
+        u64 group = own;
+#pragma unroll
+        for (int o = 1; o < PER; o <<= 1) group = max(group, (u64)__shfl_xor(group, o, WAVE));
+        if (t % PER == 0) sh.most[t / PER] = group;
         __syncthreads();
         if (wave == 0) {
             const u64 bound = least_of_top(sh, lane, k);
@@ -1367,7 +1381,7 @@ __global__ void __launch_bounds__(RW_THREADS, AHEAD == 4 ? 4 : 8) row_kernel(Sam
         __syncthreads();
         const int n = alike(sh.n);
         if (n <= ST_CAND) {   /* more only where the largest tokens crowd in few groups */
-            choose_top(sh, sort_codes<RW_THREADS>(sh, n, k), [&](float z) { return with.weight(z); }, with.p < 1.0f,
+            choose_top(sh, sort_codes<THREADS>(sh, n, k), [&](float z) { return with.weight(z); }, with.p < 1.0f,
                        [&](u64 total) { return with.mass(total); }, with.least_w, [&](u64 total) { return with.choice(total); },
                        a.out + r);
             return;
@@ -1396,6 +1410,62 @@ __global__ void __launch_bounds__(RW_THREADS, AHEAD == 4 ? 4 : 8) row_kernel(Sam
         },
         [&](u64 total) { return with.choice(total); });
     if (t == 0) a.out[r] = token;
+}
+
+/* Two forms, with the same results: four chunks in flight, 93 registers, a workgroup a CU; or two chunks and 64 registers, two
+ * workgroups a CU, where there are more rows than CUs: 333 rows of 32,768 tokens with top-p 102 and 85 us, 256 of 65,536 94 and
+ * 95, 128 of them with a top-k 23.6 and 25.0. */
+template <int AHEAD>
+__global__ void __launch_bounds__(RW_THREADS, AHEAD == 4 ? 4 : 8) row_kernel(SampleArgs a) {
+    __shared__ RowShared<RW_WAVES> sh;
+    row_choose<AHEAD>(a, blockIdx.x, sh);
+}
+
+/* split_kernel's arguments, read once more: those that only a row that was given up needs would be kept in scalar registers
+ * all along (100 of them spilled, and one row of 65,536 tokens took 23.4 us instead of 21.7). */
+__device__ __forceinline__ SampleArgs sample_args_again() {
+    const __attribute__((address_space(4))) SplitArgs *p =
+        (const __attribute__((address_space(4))) SplitArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    SampleArgs a;
+    a.logits = p->a.logits; a.stride = p->a.stride; a.vocab = p->a.vocab; a.bf16 = p->a.bf16; a.wide = p->a.wide;
+    a.uniform = p->a.uniform; a.temperature = p->a.temperature; a.top_p = p->a.top_p; a.min_p = p->a.min_p;
+    a.top_k = p->a.top_k; a.mask = p->a.mask; a.mask_stride = p->a.mask_stride; a.out = p->a.out;
+    return a;
+}
+
+/* Rows in slices. A row that was given up is done by the last of its workgroups to leave. */
+template <int E>
+__global__ void __launch_bounds__(ST_THREADS, 4) split_kernel(SplitArgs s) {
+    __shared__ SplitShared<E> sh;
+    Split<E> q = {s, sh};
+    q.t = threadIdx.x;
+    q.lane = q.t & (WAVE - 1);
+    q.wave = q.t >> 6;
+    q.G = s.groups;
+    q.row = blockIdx.x;
+    q.g = 0;
+    if (q.G > 1) {   /* every eighth workgroup, which one XCD runs, draws on one queue, and a row is one queue's */
+        const int y = blockIdx.x % ST_QUEUES, rows = (s.rows - y + ST_QUEUES - 1) / ST_QUEUES;
+        if ((int)(blockIdx.x / ST_QUEUES) >= rows * q.G) return;
+        if (q.t == 0)
+            sh.n = __hip_atomic_fetch_add(s.tickets + y * ST_LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        const int ticket = alike(sh.n);
+        q.row = y + ticket / q.G * ST_QUEUES;
+        if (q.row >= s.rows) return;   /* counts that were not zero: no access out of bounds */
+        q.g = ticket % q.G;
+    }
+    if (!split_row(q) || q.G == 1) return;
+    if (q.t == 0) {
+        const bool last = q.leave(false);
+        sh.token = last;
+    }
+    if (!q.gone) return;
+    __syncthreads();
+    if (!alike(sh.token)) return;
+    __syncthreads();   /* sh.token is read; the same LDS serves the whole row */
+    row_choose<2>(sample_args_again(), alike(q.row), reinterpret_cast<RowShared<ST_WAVES> &>(sh));
 }
 
 }  // namespace nc
@@ -1427,10 +1497,10 @@ extern "C" size_t nc_sample_workspace_bytes(long long rows, int vocab) {
     return groups <= 1 ? 16 : ST_COUNT_BYTES + (size_t)rows * groups * ST_PART * sizeof(u64);
 }
 
-extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
-                                const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
-                                const float *min_p, const uint32_t *mask, long long mask_stride, int32_t *tokens,
-                                void *workspace, size_t workspace_bytes, void *stream) {
+static int sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
+                         const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
+                         const float *min_p, const uint32_t *mask, long long mask_stride, int32_t *tokens, void *workspace,
+                         size_t workspace_bytes, int patience, void *stream) {
     if (!logits || !uniform || !temperature || !tokens || !workspace) return NC_ERR_NULL;
     if (rows < 0 || rows > 1LL << 22 || vocab <= 0 || vocab > 1 << 24 || row_stride < vocab ||
         (mask && mask_stride < ((long long)vocab + 31) / 32) || (uintptr_t)workspace % 16 ||
@@ -1443,10 +1513,11 @@ extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_s
     a.uniform = uniform; a.temperature = temperature; a.top_p = top_p; a.min_p = min_p; a.top_k = top_k;
     a.mask = mask; a.mask_stride = mask_stride;
     a.out = tokens;
-    int e;
-    const int groups = split_groups(rows, vocab, e);
+    int e, groups = split_groups(rows, vocab, e);
+    const int cus = device_cus();
+    if (groups > 1 && rows * groups > 2 * cus) groups = 0;   /* a device of fewer CUs: slices would give rows up */
     if (groups == 0) {
-        hipLaunchKernelGGL(rows > RW_CUS ? row_kernel<2> : row_kernel<4>, dim3((unsigned)rows), dim3(RW_THREADS), 0,
+        hipLaunchKernelGGL(rows > cus ? row_kernel<2> : row_kernel<4>, dim3((unsigned)rows), dim3(RW_THREADS), 0,
                            (hipStream_t)stream, a);
         return (int)hipGetLastError();
     }
@@ -1454,6 +1525,7 @@ extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_s
     s.a = a;
     s.rows = (int)rows;
     s.groups = groups;
+    s.patience = patience;
     s.tickets = (int *)workspace;
     s.done = s.tickets + ST_QUEUES * ST_LINE;
     s.count = s.done + ST_QUEUES * ST_LINE;
@@ -1461,4 +1533,21 @@ extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_s
     const long long grid = groups == 1 ? rows : (rows + ST_QUEUES - 1) / ST_QUEUES * ST_QUEUES * groups;
     hipLaunchKernelGGL(e == ST_MAX_E ? split_kernel<ST_MAX_E> : split_kernel<ST_MAX_E / 2>, dim3((unsigned)grid), dim3(ST_THREADS), 0, (hipStream_t)stream, s);
     return (int)hipGetLastError();
+}
+
+extern "C" int nc_sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
+                                const float *uniform, const float *temperature, const int32_t *top_k, const float *top_p,
+                                const float *min_p, const uint32_t *mask, long long mask_stride, int32_t *tokens,
+                                void *workspace, size_t workspace_bytes, void *stream) {
+    return sample_tokens(logits, is_bf16, row_stride, rows, vocab, uniform, temperature, top_k, top_p, min_p, mask, mask_stride,
+                         tokens, workspace, workspace_bytes, ST_PATIENCE, stream);
+}
+
+extern "C" int nc_debug_sample_tokens(const void *logits, int is_bf16, long long row_stride, long long rows, int vocab,
+                                      const float *uniform, const float *temperature, const int32_t *top_k,
+                                      const float *top_p, const float *min_p, const uint32_t *mask, long long mask_stride,
+                                      int32_t *tokens, void *workspace, size_t workspace_bytes, int patience, void *stream) {
+    if (patience < 0 || patience > 1 << 16) return NC_ERR_SHAPE;
+    return sample_tokens(logits, is_bf16, row_stride, rows, vocab, uniform, temperature, top_k, top_p, min_p, mask, mask_stride,
+                         tokens, workspace, workspace_bytes, patience, stream);
 }

@@ -31,7 +31,8 @@ KERNEL_SOURCES = [CSRC / "kv_append.hip", CSRC / "attention.hip", CSRC / "ve_gat
                   CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip", CSRC / "paging.hip", CSRC / "sample.hip", CSRC / "packed_attn.hip"]
 DECODE_SOURCES = [CSRC / "decoder.hip", CSRC / "slot_gemm.hip"]
 SOURCES = KERNEL_SOURCES + DECODE_SOURCES
-HEADERS = [CSRC / "nc_device.h", CSRC / "nc_internal.h", CSRC / "nc_row.h", CSRC / "nc_attend.h", INCLUDE / "nanochat_amd.h", INCLUDE / "nanochat_decode.h"]
+HEADERS = [CSRC / "nc_device.h", CSRC / "nc_internal.h", CSRC / "nc_row.h", CSRC / "nc_attend.h", CSRC / "nc_meeting.h",
+           INCLUDE / "nanochat_amd.h", INCLUDE / "nanochat_decode.h"]
 HEAD_DIM = 128
 
 # -ffp-contract=off: the append's fp32 order is part of its bit-exact contract (no implicit FMAs).
@@ -124,6 +125,8 @@ SIGNATURES = {
     "nc_sample_workspace_bytes": ([c_longlong, c_int], c_size_t),
     "nc_sample_tokens": ([c_void_p, c_int, c_longlong, c_longlong, c_int] + [c_void_p] * 6 +
                          [c_longlong, c_void_p, c_void_p, c_size_t, c_void_p], c_int),
+    "nc_debug_sample_tokens": ([c_void_p, c_int, c_longlong, c_longlong, c_int] + [c_void_p] * 6 +
+                               [c_longlong, c_void_p, c_void_p, c_size_t, c_int, c_void_p], c_int),
     "nc_pages_extend": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int] + [c_void_p] * 6,
                         c_int),
     "nc_pages_trim": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p], c_int),

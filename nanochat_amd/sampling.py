@@ -44,6 +44,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature: torc
     temperature): the top_k largest stay (the lower index first among equals), of those the tokens with less than top_p of
     their weight strictly above them, of those the ones of at least min_p times the largest; the token is the first, in
     index order, whose running weight exceeds uniform times what is left. A row's token does not depend on the other rows.
+    Calls on different streams may overlap.
     A workspace passed in (at least sample_workspace_bytes) must have been zero-filled before its first use and only used
     by these calls since, one stream at a time. Without one, calls on a stream share a cached workspace; a call that is
     being captured into a graph gets one of the graph's own."""
