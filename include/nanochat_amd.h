@@ -272,8 +272,10 @@ size_t nc_packed_workspace_bytes(long long rows, int B, int Hq, int Hkv, int max
  * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q and out (bf16 [rows][Hq][128]; cu_seqlens int32 [B + 1], as
  * nc_pages_extend makes it), the last of its seq_lens[b] tokens, all already in the cache; the row at position p attends
  * keys [max(p - window, 0), p] (window < 0: all), scores (q . k) * sm_scale, fp32 softmax, out bf16. A sequence longer than
- * max_seq_len (<= max_pages * 16) or shorter than its new tokens gets NaN, and so do the rows of a (row, KV head) that
- * reaches a block-table entry outside [0, num_pages); rows outside every sequence are left as they are. Row offsets are
+ * max_seq_len (<= max_pages * 16) or shorter than its new tokens gets NaN. So does a row that attends keys behind a
+ * block-table entry outside [0, num_pages), and with it any rows of its sequence that one wave computes beside it (up to 32
+ * (row, head) pairs of a KV head); entries whose keys no row of the sequence attends, such as those behind its window, may
+ * hold anything. Rows outside every sequence are left as they are. Row offsets are
  * taken into [0, rows]; if they overlap so that the workspace could not hold the launch, every row gets NaN. A sequence's
  * output bits depend on its own numbers alone, not on the rest of the launch. rows <= 2^24, B <= 1024, Hq / Hkv <= 16.
  */

@@ -283,8 +283,9 @@ def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Te
 
     Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1]) and the last of its seq_lens[b]
     tokens (int32 [B]); its row at position p attends keys [max(p - window, 0), p] through block_table[b]. max_seq_len
-    bounds seq_lens: a longer sequence's rows are NaN, as are those of one shorter than its new tokens. Rows outside every
-    sequence are not written. A sequence's output bits depend on nothing but its own numbers. A workspace passed in must
+    bounds seq_lens: a longer sequence's rows are NaN, as are those of one shorter than its new tokens. Entries of block_table
+    whose keys no row attends (pages behind a window that were given back) may hold anything; one outside the cache that a row
+    does attend makes that row NaN, and others of its sequence beside it. Rows outside every sequence are not written. A sequence's output bits depend on nothing but its own numbers. A workspace passed in must
     have been zero-filled before its first use (torch.zeros, at least packed_workspace_bytes) and only used by these and
     decode_attention's calls since, one stream at a time. Without one, calls on a stream share a cached workspace; a call
     that is being captured into a graph gets one of the graph's own."""

@@ -196,12 +196,18 @@ __device__ __forceinline__ long long pk_row(const PackedArgs &p, const PkItem &i
 }
 
 /* Keys of a wave: in tile t a lane's column sees [lo[t], hi[t]]; the pairs from page in0 (even) up to in1 are seen whole by
- * every column; keys past written_hi are not cache contents. */
+ * every column. No column sees keys outside [first, last], which need not be cache contents: the sequence may end inside
+ * the pair, and a window's first page may be its second, the page before having left the block table. */
 template <int NT>
 struct PkBounds {
     int lo[NT], hi[NT];
-    int in0, in1, written_hi;
+    int in0, in1, first, last;
 };
+
+/* The first key that the sequence's row t sees. */
+__device__ __forceinline__ int pk_first_key(const PackedArgs &p, const PkSeq &q, int t) {
+    return p.a.window >= 0 ? max(q.len - q.n + t - p.a.window, 0) : 0;
+}
 
 /* Per-column key bounds of a wave whose first token is wt0 (end: one past the item's last), its query operand and the
  * columns' references. */
@@ -224,8 +230,9 @@ __device__ __forceinline__ void pk_columns(const PackedArgs &p, const PkItem &it
                                   : uint4{0u, 0u, 0u, 0u};
     }
     const int last = min(wt0 + NT * tpt, end) - 1;
-    kb.written_hi = it.q.len - 1;
-    const int whole_lo = a.window >= 0 ? max(start + last - a.window, 0) : 0, whole_hi = min(start + wt0, kb.written_hi);
+    kb.first = pk_first_key(p, it.q, wt0);
+    kb.last = start + last;
+    const int whole_lo = pk_first_key(p, it.q, last), whole_hi = start + wt0;
     kb.in0 = ((whole_lo + PAGE - 1) / PAGE + 1) & ~1;
     kb.in1 = min((whole_hi + 1) / PAGE, it.pg1) & ~1;
 }
@@ -277,10 +284,10 @@ constexpr float PK_RESCALE = 2048.0f;
 /* One pair's scores, softmax and PV. The lazy rescale, as in nc_attend.h: a column keeps its reference maximum m, and its
  * exponentials p = exp2(s - m) grow past one, until the sum of a lane's eight passes PK_RESCALE (the sum is made anyway,
  * where the largest would take eight more instructions); then the column moves to its new maximum. The decision and what
- * it does depend on the column's own scores. A pair that holds keys which some column does not see, or that are not
- * written, is masked: what is not seen takes no part whatever its bytes (its exponential and its product with the V scale
- * are replaced by zero, and the V codes of keys that are not written are cleared). freed() is called once the stage's
- * bytes are in registers. */
+ * it does depend on the column's own scores. A pair that holds keys which some column does not see is masked: what is not
+ * seen takes no part whatever its bytes (its exponential and its product with the V scale are replaced by zero, and the V
+ * codes of keys that no column sees are cleared; the cache's own codes are never NaN, whatever was appended). freed() is
+ * called once the stage's bytes are in registers. */
 template <int NT, typename Freed>
 __device__ __forceinline__ void pk_pair(int lpa, bool has_b, PkAt stage, const QOp (&qb)[NT], const PkBounds<NT> &kb,
                                         const f32x4 &zero, WaveState<NT> &st, int lane, Freed freed) {
@@ -334,8 +341,12 @@ __device__ __forceinline__ void pk_pair(int lpa, bool has_b, PkAt stage, const Q
         const int key = pk_here(key_a);
         pk_read(stage.at + 2 * PAGE_BYTES, stage.scales + PAGE * 4, lane, v);
         freed();
-        const int na = min(max(kb.written_hi - key + 1, 0), 4), nb = has_b ? min(max(kb.written_hi - key - PAGE + 1, 0), 4) : 0;
-        const uint32_t ma = na >= 4 ? 0xFFFFFFFFu : (1u << (8 * na)) - 1u, mb = nb >= 4 ? 0xFFFFFFFFu : (1u << (8 * nb)) - 1u;
+        const auto upto = [&](int k) {   /* the codes of a lane's four keys, a byte each, that lie below the k-th */
+            const int n = min(max(k, 0), 4);
+            return n >= 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1u;
+        };
+        const uint32_t ma = upto(kb.last - key + 1) & ~upto(kb.first - key);
+        const uint32_t mb = has_b ? upto(kb.last - key - PAGE + 1) & ~upto(kb.first - key - PAGE) : 0u;
         v.a0 = and4(v.a0, ma); v.a1 = and4(v.a1, ma);
         v.b0 = and4(v.b0, mb); v.b1 = and4(v.b1, mb);
 #pragma unroll
@@ -553,8 +564,8 @@ __device__ __forceinline__ int pk_wide(const PackedArgs &p, const PkItem &it, in
     const int wt0 = it.t0 + wcol * tpw, end = it.t0 + it.tn, npages = it.pg1 - it.pg0;
     const bool on = wt0 < end;
     const int last = min(wt0 + tpw, end) - 1;
-    /* the wave's own pairs within the chunk's */
-    const int w0 = max((a.window >= 0 ? max(start + wt0 - a.window, 0) : 0) / PAGE, it.pg0);
+    /* the wave's own pages, and pairs, within the chunk's */
+    const int w0 = max(pk_first_key(p, it.q, wt0) / PAGE, it.pg0);
     const int w1 = on ? min((start + last) / PAGE + 1, it.pg1) : 0, count = (npages + 1) / 2;
     const int s0 = min(max(w0 - it.pg0, 0) / 2, count), s1 = min(max(w1 - it.pg0 + 1, 0) / 2, count);
     PkBounds<PK_NT> kb;
@@ -563,14 +574,14 @@ __device__ __forceinline__ int pk_wide(const PackedArgs &p, const PkItem &it, in
     state_init(ws);
     ws.sl2 = a.scale_log2;
     pk_columns<PK_NT>(p, it, wt0, end, lane, kb, raw, ws);
-    /* every wave looks at all the entries (is one outside the pool among its pairs'?) and stores a quarter of them */
+    /* every wave looks at all the entries (is one outside the pool among its pages'?) and stores a quarter of them */
     const int32_t *bt = a.block_table + (long long)it.b * a.max_pages + it.pg0;
     bool bad = false;
     for (int i = lane; i < npages; i += WAVE) {
         const int e = bt[i];
         const bool ok = (unsigned)e < (unsigned)a.num_pages;
-        bad = bad || (!ok && i >= 2 * s0 && i < 2 * s1);
-        if (((i >> 6) & (WAVES - 1)) == wave) tab[i] = ok ? e : 0;   /* only read: those waves report NaN */
+        bad = bad || (!ok && i >= w0 - it.pg0 && i < w1 - it.pg0);
+        if (((i >> 6) & (WAVES - 1)) == wave) tab[i] = ok ? e : 0;   /* only read: a wave that needs it reports NaN */
     }
     ws.bad = __any(bad);
     __syncthreads();
@@ -693,12 +704,13 @@ __device__ __forceinline__ void pk_narrow(const PackedArgs &p, const PkItem &it,
     const int npages = it.pg1 - it.pg0, pairs = max(((npages + 1) / 2 - first + stride - 1) / stride, 0);
     /* lane j: entries j and 64 + j of the item's pages */
     const int32_t *bt = a.block_table + (long long)it.b * a.max_pages + it.pg0;
-    int e0 = lane < npages ? bt[lane] : 0, e1 = WAVE + lane < npages ? bt[WAVE + lane] : 0;
+    const int before = pk_first_key(p, it.q, 0) / PAGE - it.pg0;   /* a page that no row sees */
+    int e0 = lane < npages && lane >= before ? bt[lane] : 0, e1 = WAVE + lane < npages ? bt[WAVE + lane] : 0;
     WaveState<NT> ws;
     state_init(ws);
     ws.sl2 = a.scale_log2;
     ws.bad = __any((unsigned)e0 >= (unsigned)a.num_pages || (unsigned)e1 >= (unsigned)a.num_pages);
-    if ((unsigned)e0 >= (unsigned)a.num_pages) e0 = 0;   /* only read: the item reports NaN */
+    if ((unsigned)e0 >= (unsigned)a.num_pages) e0 = 0;   /* only read: if a row needs it the item reports NaN */
     if ((unsigned)e1 >= (unsigned)a.num_pages) e1 = 0;
     const auto entry = [&](int e) {
         const int lo = __builtin_amdgcn_readlane(e0, e & (WAVE - 1)), hi = __builtin_amdgcn_readlane(e1, e & (WAVE - 1));
