@@ -268,11 +268,17 @@ def prefill_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.T
     return out
 
 
+def _window32(window: int) -> int:
+    """A window as the C ABI's int, which ctypes would fill with the low 32 bits of a larger one: -1 for none, and at most
+    2^31 - 1, which hides no key either."""
+    return min(max(window, -1), 2 ** 31 - 1)
+
+
 @functools.lru_cache(maxsize=256)
 def packed_workspace_bytes(rows: int, batch: int, num_q_heads: int, num_kv_heads: int, max_seq_len: int,
                            window: int = -1) -> int:
     """nc_packed_workspace_bytes (0: an unsupported shape), kept per shape."""
-    return hip_library().nc_packed_workspace_bytes(rows, batch, num_q_heads, num_kv_heads, max_seq_len, window)
+    return hip_library().nc_packed_workspace_bytes(rows, batch, num_q_heads, num_kv_heads, max_seq_len, _window32(window))
 
 
 def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -312,7 +318,7 @@ def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Te
             raise ValueError(f"out must be {tuple(q.shape)}")
     if rows == 0:
         return out
-    window = max(window, -1)
+    window = _window32(window)
     need = packed_workspace_bytes(rows, B, Hq, cache.num_kv_heads, max_seq_len, window)
     if need == 0:
         raise ValueError(f"unsupported shape: rows={rows}, B={B}, Hq={Hq}, Hkv={cache.num_kv_heads}")

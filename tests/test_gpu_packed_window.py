@@ -82,3 +82,10 @@ def test_a_batch_behind_its_windows(device):
         drop(table, b, max(c - window, 0))
     poison(cache, 0)
     check(packed_attention(q, cache, table, cu, lens, max(lens_l), window), want, size, cu_l)
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5])
+def test_a_window_past_every_position_hides_nothing(device, window):
+    q, cache, table, cu, lens, _, lens_l = setup(device, [1, 60], [3000, 200], 4, 2, seed=4)
+    assert torch.equal(packed_attention(q, cache, table, cu, lens, max(lens_l), window),
+                       packed_attention(q, cache, table, cu, lens, max(lens_l)))
