@@ -30,7 +30,7 @@ enum {
     NC_OK = 0,
     NC_ERR_NULL = -1,       /* a required pointer is NULL */
     NC_ERR_SHAPE = -2,      /* a size or head count out of the supported range */
-    NC_ERR_WORKSPACE = -3,  /* the workspace is smaller than nc_decode_workspace_bytes */
+    NC_ERR_WORKSPACE = -3,  /* the workspace is smaller than its nc_*_workspace_bytes, or not aligned as asked */
 };
 
 /* Text of a status code (static storage). */
@@ -262,8 +262,9 @@ int nc_prefill_attn_fp8(const void *q, const void *k_pages, const void *v_pages,
                         void *out, void *stream);
 
 /* Workspace bytes nc_packed_attn_fp8 needs for these sizes, whatever the lengths on the device (0 for unsupported sizes):
- * partial results, and counts in its last 1/256. As nc_decode_workspace_bytes's: zero-filled before its first call and
- * passed with the same workspace_bytes to every call, by calls ordered on one stream; one workspace may serve both. */
+ * partial results, and counts in its last 1/256. 16-byte aligned, else (as where it is too small) NC_ERR_WORKSPACE. As
+ * nc_decode_workspace_bytes's: zero-filled before its first call and passed with the same workspace_bytes to every call, by
+ * calls ordered on one stream; one workspace may serve both. */
 size_t nc_packed_workspace_bytes(long long rows, int B, int Hq, int Hkv, int max_seq_len, int window);
 
 /*

@@ -596,7 +596,7 @@ extern "C" const char *nc_status_string(int status) {
         case NC_OK: return "ok";
         case NC_ERR_NULL: return "a required pointer is NULL";
         case NC_ERR_SHAPE: return "a size or head count is out of the supported range";
-        case NC_ERR_WORKSPACE: return "the workspace is smaller than nc_decode_workspace_bytes";
+        case NC_ERR_WORKSPACE: return "the workspace is smaller than the call needs (nc_*_workspace_bytes), or not aligned";
         default: return status > 0 ? hipGetErrorString((hipError_t)status) : "unknown status";
     }
 }

@@ -1086,7 +1086,8 @@ extern "C" int nc_packed_attn_fp8(const void *q, const void *k_pages, const void
     if (need == 0) return NC_ERR_SHAPE;
     const PkSizes z = pk_sizes(rows, B, Hq, Hkv, max_seq_len, window);
     const size_t counts = pk_count_region(workspace_bytes);
-    if (pk_part_bytes(z) > counts || pk_count_bytes(z) > workspace_bytes - counts) return NC_ERR_WORKSPACE;
+    if ((uintptr_t)workspace % 16 || pk_part_bytes(z) > counts || pk_count_bytes(z) > workspace_bytes - counts)
+        return NC_ERR_WORKSPACE;
     PackedArgs p = {};
     AttnArgs &a = p.a;
     a.q = (const uint16_t *)q;

@@ -9,3 +9,13 @@ def test_a_window_past_every_position_hides_nothing(lib, window):
     """ctypes passes an integer's low 32 bits: 2^32 + 5 would be a window of 5 keys."""
     assert packed_workspace_bytes(64, 64, 16, 4, 40000, window) == packed_workspace_bytes(64, 64, 16, 4, 40000, -1)
     assert packed_workspace_bytes(64, 64, 16, 4, 40000, -window) == packed_workspace_bytes(64, 64, 16, 4, 40000, -1)
+
+
+def test_a_misaligned_workspace_is_refused(lib):
+    """Its partials are moved by 16-byte accesses."""
+    import ctypes
+
+    dummy = ctypes.c_void_p(0x1000)   # never dereferenced
+    for at in (0x1001, 0x1004, 0x1008):
+        assert lib.nc_packed_attn_fp8(dummy, dummy, dummy, dummy, dummy, 16, 8, dummy, dummy, 4, 2, 16, 4, 256, -1, 0.1, dummy,
+                                      ctypes.c_void_p(at), 1 << 30, None) == -3, at
