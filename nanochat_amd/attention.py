@@ -274,11 +274,16 @@ def _window32(window: int) -> int:
     return min(max(window, -1), 2 ** 31 - 1)
 
 
+PACKED_SEQUENCES = 1024   # of one launch of packed_attention
+
+
 @functools.lru_cache(maxsize=256)
 def packed_workspace_bytes(rows: int, batch: int, num_q_heads: int, num_kv_heads: int, max_seq_len: int,
                            window: int = -1) -> int:
-    """nc_packed_workspace_bytes (0: an unsupported shape), kept per shape."""
-    return hip_library().nc_packed_workspace_bytes(rows, batch, num_q_heads, num_kv_heads, max_seq_len, _window32(window))
+    """nc_packed_workspace_bytes (0: an unsupported shape), kept per shape; of the largest launch for more sequences than one
+    takes."""
+    return hip_library().nc_packed_workspace_bytes(rows, min(batch, PACKED_SEQUENCES), num_q_heads, num_kv_heads, max_seq_len,
+                                                   _window32(window))
 
 
 def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -294,7 +299,8 @@ def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Te
     does attend makes that row NaN, and others of its sequence beside it. Rows outside every sequence are not written. A sequence's output bits depend on nothing but its own numbers. A workspace passed in must
     have been zero-filled before its first use (torch.zeros, at least packed_workspace_bytes) and only used by these and
     decode_attention's calls since, one stream at a time. Without one, calls on a stream share a cached workspace; a call
-    that is being captured into a graph gets one of the graph's own."""
+    that is being captured into a graph gets one of the graph's own. One launch takes 1,024 sequences; a larger batch, up to
+    every slot of a paging.BlockTables, is as many launches, with the same bits."""
     _require(q, "q", torch.bfloat16)
     if q.dim() != 3 or q.size(2) != HEAD_DIM or q.size(1) < 1:
         raise ValueError(f"q must be [rows, Hq, {HEAD_DIM}], got {tuple(q.shape)}")
@@ -321,7 +327,8 @@ def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Te
     window = _window32(window)
     need = packed_workspace_bytes(rows, B, Hq, cache.num_kv_heads, max_seq_len, window)
     if need == 0:
-        raise ValueError(f"unsupported shape: rows={rows}, B={B}, Hq={Hq}, Hkv={cache.num_kv_heads}")
+        raise ValueError(f"unsupported shape: rows={rows}, B={B}, Hq={Hq}, Hkv={cache.num_kv_heads} (at most 2^24 rows, and "
+                         "at most 16 query heads a KV head, as many for each)")
     with device_guard(q):
         if workspace is None:
             if torch.cuda.is_current_stream_capturing():
@@ -332,8 +339,10 @@ def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Te
         nbytes = workspace.numel() * workspace.element_size()
         if nbytes < need or not workspace.is_contiguous() or workspace.device != q.device or workspace.data_ptr() % 16:
             raise ValueError(f"workspace must be a contiguous 16-byte aligned tensor of at least {need} bytes on {q.device}")
-        check(hip_library().nc_packed_attn_fp8(
-            pointer(q), pointer(cache.k_pages), pointer(cache.v_pages), pointer(cache.kv_scale), pointer(block_table),
-            block_table.size(1), cache.num_pages, pointer(cu_seqlens), pointer(seq_lens), rows, B, Hq, cache.num_kv_heads,
-            max_seq_len, window, sm_scale, pointer(out), pointer(workspace), nbytes, stream()))
+        for first in range(0, B, PACKED_SEQUENCES):   # row offsets are those of the whole: each launch writes its own rows
+            check(hip_library().nc_packed_attn_fp8(
+                pointer(q), pointer(cache.k_pages), pointer(cache.v_pages), pointer(cache.kv_scale),
+                pointer(block_table) + 4 * first * block_table.size(1), block_table.size(1), cache.num_pages,
+                pointer(cu_seqlens) + 4 * first, pointer(seq_lens) + 4 * first, rows, min(B - first, PACKED_SEQUENCES), Hq,
+                cache.num_kv_heads, max_seq_len, window, sm_scale, pointer(out), pointer(workspace), nbytes, stream()))
     return out

@@ -19,3 +19,12 @@ def test_a_misaligned_workspace_is_refused(lib):
     for at in (0x1001, 0x1004, 0x1008):
         assert lib.nc_packed_attn_fp8(dummy, dummy, dummy, dummy, dummy, 16, 8, dummy, dummy, 4, 2, 16, 4, 256, -1, 0.1, dummy,
                                       ctypes.c_void_p(at), 1 << 30, None) == -3, at
+
+
+def test_more_sequences_than_a_launch_need_the_largest_launchs_workspace(lib):
+    for rows, length in ((4096, 64), (20000, 40000)):
+        most = packed_workspace_bytes(rows, 1024, 16, 4, length)
+        assert most > 0
+        for batch in (1025, 2000, 4096):
+            assert packed_workspace_bytes(rows, batch, 16, 4, length) == most
+        assert all(packed_workspace_bytes(rows, batch, 16, 4, length) <= most for batch in (1, 7, 100, 976))
