@@ -264,7 +264,10 @@ int nc_prefill_attn_fp8(const void *q, const void *k_pages, const void *v_pages,
 /* Workspace bytes nc_packed_attn_fp8 needs for these sizes, whatever the lengths on the device (0 for unsupported sizes):
  * partial results, and counts in its last 1/256. 16-byte aligned, else (as where it is too small) NC_ERR_WORKSPACE. As
  * nc_decode_workspace_bytes's: zero-filled before its first call and passed with the same workspace_bytes to every call, by
- * calls ordered on one stream; one workspace may serve both. */
+ * calls ordered on one stream; one workspace may serve both. Since the lengths are not known it holds the most partials
+ * there can be, 32 or 128 query columns of 520 bytes each for every chunk of keys: 44 MB for 64 sequences of one row, 16 / 4
+ * heads and 8,192 keys at most, but 1.4 GB for 256 of one row, 32 / 8 heads and 32,768 keys, and 5.5 GB with 8,192 rows.
+ * A smaller max_seq_len (or a window) makes it smaller; up to 2,048 keys no partials are kept. */
 size_t nc_packed_workspace_bytes(long long rows, int B, int Hq, int Hkv, int max_seq_len, int window);
 
 /*
@@ -272,7 +275,8 @@ size_t nc_packed_workspace_bytes(long long rows, int B, int Hq, int Hkv, int max
  * runs one-token and prompt rows apart, model/kernels/decode.cu:567-675, 1041-1051). Sequence b's new tokens are rows
  * cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q and out (bf16 [rows][Hq][128]; cu_seqlens int32 [B + 1], as
  * nc_pages_extend makes it), the last of its seq_lens[b] tokens, all already in the cache; the row at position p attends
- * keys [max(p - window, 0), p] (window < 0: all), scores (q . k) * sm_scale, fp32 softmax, out bf16. A sequence longer than
+ * keys [max(p - window, 0), p] (window < 0: all), scores (q . k) * sm_scale, fp32 softmax (a probability times its key's V
+ * scale is rounded to bf16 for its product with V, as in the other attention entries), out bf16. A sequence longer than
  * max_seq_len (<= max_pages * 16) or shorter than its new tokens gets NaN. So does a row that attends keys behind a
  * block-table entry outside [0, num_pages), and with it any rows of its sequence that one wave computes beside it (up to 32
  * (row, head) pairs of a KV head); entries whose keys no row of the sequence attends, such as those behind its window, may
@@ -310,7 +314,7 @@ int nc_pages_trim(const int32_t *keep, int slots, int32_t *lengths, int32_t *tab
 
 /* Workspace bytes nc_sample_tokens needs for these sizes, at most 7 MB (0 for unsupported sizes). Its first 64 KiB (or all
  * of it, if smaller) are zero-filled before its first call; it is then passed to calls ordered on one stream, of any sizes
- * that it suffices for. It serves no other function. */
+ * that it suffices for. It serves no other function. One that is too small or not 16-byte aligned gives NC_ERR_SHAPE. */
 size_t nc_sample_workspace_bytes(long long rows, int vocab);
 
 /*

@@ -281,7 +281,9 @@ PACKED_SEQUENCES = 1024   # of one launch of packed_attention
 def packed_workspace_bytes(rows: int, batch: int, num_q_heads: int, num_kv_heads: int, max_seq_len: int,
                            window: int = -1) -> int:
     """nc_packed_workspace_bytes (0: an unsupported shape), kept per shape; of the largest launch for more sequences than one
-    takes."""
+    takes. It grows with the sequences (or rows), KV heads and keys that a step may have: 44 MB for 64 sequences of one row,
+    16 / 4 heads and 8,192 keys, 1.4 GB for 256 of one row, 32 / 8 heads and 32,768 keys, 5.5 GB with 8,192 rows; next to
+    nothing up to 2,048 keys."""
     return hip_library().nc_packed_workspace_bytes(rows, min(batch, PACKED_SEQUENCES), num_q_heads, num_kv_heads, max_seq_len,
                                                    _window32(window))
 
@@ -298,8 +300,9 @@ def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Te
     whose keys no row attends (pages behind a window that were given back) may hold anything; one outside the cache that a row
     does attend makes that row NaN, and others of its sequence beside it. Rows outside every sequence are not written. A sequence's output bits depend on nothing but its own numbers. A workspace passed in must
     have been zero-filled before its first use (torch.zeros, at least packed_workspace_bytes) and only used by these and
-    decode_attention's calls since, one stream at a time. Without one, calls on a stream share a cached workspace; a call
-    that is being captured into a graph gets one of the graph's own. One launch takes 1,024 sequences; a larger batch, up to
+    decode_attention's calls since, one stream at a time. Without one, calls on a stream share a cached workspace (up to eight
+    streams' are kept, see packed_workspace_bytes for their size); a call that is being captured into a graph gets one of the
+    graph's own. Softmax and sums are fp32; a probability times its key's V scale is rounded to bf16. One launch takes 1,024 sequences; a larger batch, up to
     every slot of a paging.BlockTables, is as many launches, with the same bits."""
     _require(q, "q", torch.bfloat16)
     if q.dim() != 3 or q.size(2) != HEAD_DIM or q.size(1) < 1:

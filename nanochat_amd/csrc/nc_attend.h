@@ -1,7 +1,7 @@
 /*
- * The page-pair step shared by the attention kernels over the paged fp8 cache (attention.hip, packed_attn.hip): a wave's
- * query operands, its softmax state, the scores, softmax update and PV of two 16-token pages, and the accesses that cross
- * workgroups. attention.hip's header describes the step.
+ * What the attention kernels over the paged fp8 cache share (attention.hip, packed_attn.hip): a wave's query operands, its
+ * softmax state, and the accesses that cross workgroups. The step over two 16-token pages (page_scores to pair_step_k:
+ * scores, softmax update and PV) is attention.hip's, whose header describes it; packed_attn.hip has one of its own.
  */
 #pragma once
 

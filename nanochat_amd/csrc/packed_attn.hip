@@ -7,7 +7,10 @@
  *
  *   o = sum_j exp2(s_j - m) v_j / sum_j exp2(s_j - m),  s_j = (q . k_j) sm_scale log2(e),  m a running maximum
  *
- * The step over two pages (scores, softmax, PV) is nc_attend.h's. What bounds a sequence depends on its rows: a page of a
+ * The step over two pages (pk_pair) is this file's own; the query operand, the softmax state and the accesses across
+ * workgroups are nc_attend.h's. Scores, softmax, sums and O are held in 32 bits; a probability times its key's V scale is
+ * rounded to bf16 for the second product, whose matrix instruction takes bf16 (V codes are exact there), and the output once
+ * more: against float64 about 1.4 times the error of one rounding. What bounds a sequence depends on its rows: a page of a
  * KV head is 2 KiB of K, 2 KiB of V and 128 bytes of scales for 16 keys, and each query column costs 512 flops a key, so
  * below about 80 columns (rows times the heads of a KV head) the pages' bytes take longer than the products. Hence two
  * kinds of work items, both streaming pages into LDS by asynchronous copies:
@@ -18,7 +21,7 @@
  *           through LDS ("alone": it costs no round trips through memory, which is what a short one's time is made of)
  *   wide    a tile of up to 128 columns, 32 a wave: the four waves of a workgroup walk the same pairs, each fetched once
  *           (two stages of two pairs ahead); of at most 64 columns two waves take one pair of a stage and two the other,
- *           so that no wave idles (64 sequences of 64 columns over 8,192 keys: 172 us, and 207 by two waves of the four)
+ *           so that no wave idles (64 sequences of 64 columns over 8,192 keys: 169 us, and 209 by two waves of the four)
  *
  * A sequence's keys are cut into chunks (pk_plan), so that few rows over many keys still fill the chip; a (tile, KV head)
  * of several chunks leaves one partial (O, max, sum) in fp32 a chunk, and whoever finishes its last chunk merges them in
@@ -27,10 +30,12 @@
  * index, later ones from eight queues (an XCD's workgroups take every eighth item, which keeps a KV head's pages in that
  * XCD's L2), so that unequal items even out.
  *
- * Measured (16 query heads, 4 KV heads): 64 sequences of 8,192 keys, one row each 98 us (5.6 TB/s of pages), 4 rows each
- * 110 us (5.0), 16 rows each 172 us; 8 prompt chunks of 512 rows, each over 4,096 keys, 175 us (736 TFLOP/s of the
- * keys a row may see), 2 prompts of 4,096 rows 173 us (795). One sequence, 5 rows of 6 heads over 1,029 keys: 14 us, most of
- * it round trips to memory one after the other (the plan, the block table, pages, the output).
+ * Measured (16 query heads, 4 KV heads): 64 sequences of 8,192 keys, one row each 100 us (5.5 TB/s of pages), 4 rows each
+ * 111 us (5.0), 16 rows each 169 us; 8 prompt chunks of 512 rows, each over 4,096 keys, 174 us (740 TFLOP/s of the
+ * keys a row may see), 2 prompts of 4,096 rows 175 us (787). One sequence, 5 rows of 6 heads over 1,029 keys: 14.5 us, most
+ * of it round trips to memory one after the other (the plan, the block table, pages, the output). These are times of calls in
+ * a row; the first hundred launches after a pause run at a lower clock and take up to a fifth longer where products bound
+ * them (the 8 chunks 213 -> 174 us).
  */
 #include <limits.h>
 
@@ -44,17 +49,17 @@ constexpr int PK_NARROW_COLS = 16 * PK_NT;
 constexpr int PK_WIDE_COLS = WAVES * 16 * PK_NT;
 constexpr int PK_MAX_BATCH = 1024;
 constexpr int PK_QUEUES = 8;                   /* XCDs */
-/* Pages of a narrow chunk: 64 sequences of 8,192 keys, 4 rows each, take 110 us with 64 pages and 154 with 32 (twice the
- * partials); one of 32,768 keys 34.6 and 32.7. */
+/* Pages of a narrow chunk: 64 sequences of 8,192 keys, 4 rows each, take 112 us with 64 pages and 158 with 32 (twice the
+ * partials); one of 32,768 keys 35.6 and 33.2. */
 constexpr int PK_NARROW_SPLIT = 64;
 constexpr int PK_MIN_TAIL = 4;                 /* a last chunk of fewer pages joins the one before it */
-/* A narrow sequence of at most so many pages is not cut: 1,029 keys take 14.0 us whole, 25.5 in two partials. */
+/* A narrow sequence of at most so many pages is not cut: 1,029 keys take 14.4 us whole, 30.4 in two partials. */
 constexpr int PK_SHORT = 2 * PK_NARROW_SPLIT;
 /* Least and most pages of a wide chunk, and the items that a wide sequence is cut into at most if its chunks stay that long.
  * Short chunks fill the chip when a sequence is alone, and cost partials when it is not: one chunk of 512 rows over 8,192 keys
- * takes 69 us with 128 pages at least and 113 with 256, eight of them over 4,096 keys 175 and 153 (64 pages: 69 and
- * 204). A cut by what else the launch holds would make a sequence's bits depend on it. 128 items: 114 us for the first, and
- * 260 instead of 175 for 4 chunks of 200 to 700 rows among 60 decoding sequences. */
+ * takes 71 us with 128 pages at least and 113 with 256, eight of them over 4,096 keys 175 and 152 (64 pages: 70 and
+ * 201). A cut by what else the launch holds would make a sequence's bits depend on it. 128 items: 111 us for the first, and
+ * 253 instead of 179 for 4 chunks of 200 to 700 rows among 60 decoding sequences. */
 constexpr int PK_WIDE_MIN = 128, PK_WIDE_MAX = 1024, PK_WIDE_ITEMS = 256;
 constexpr int PK_AHEAD = 2;                    /* wide: stages of two pairs in flight */
 static_assert(PK_SHORT <= 2 * WAVE && PK_NARROW_SPLIT + PK_MIN_TAIL <= 2 * WAVE,
@@ -853,7 +858,8 @@ __device__ __forceinline__ void pk_merge(const PackedArgs &p, const PkItem &it, 
 }
 
 __global__ void __launch_bounds__(256, 2) packed_attn_kernel(PackedArgs p) {
-    /* the stages, PK_STAGES bytes; [PK_SUMS][B + 1] prefix sums; [3][B]: row0, n, len */
+    /* the stages, PK_STAGES bytes; [PK_SUMS][B + 1] prefix sums; [3][B]: row0, n, len. Two workgroups fit a CU up to 281
+     * sequences; beyond, one: 512 of 2,049 keys take 210 us (5.3 TB/s of pages), 256 take 99 (5.6). */
     extern __shared__ __align__(16) unsigned char stages[];
     int *pk_lds = reinterpret_cast<int *>(stages + PK_STAGES);
     __shared__ int tab[PK_WIDE_MAX];
