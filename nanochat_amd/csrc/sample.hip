@@ -18,12 +18,12 @@
  * holds many.
  *
  * split_kernel takes up to 512 / ceil(vocab / 8,192) rows of up to 262,144 tokens, a workgroup for every 8,192 (or
- * 4,096), which stay in its registers. What bounds it is neither bytes nor operations (a row of 65,536 fp32 logits is 256 KiB) but the steps one
- * after the other, each ending where the row's workgroups need one another: the largest logit; the histogram; the list; about
- * 2.5 us a meeting through memory. Greedy rows and a top-k of at most 128 need no meeting: every slice leaves its k largest in
- * order, and the last workgroup to arrive does the rest on k tokens. No meeting waits without bound: where the others
- * do not come, because the device is crowded, a row is given up and one workgroup does it (nc_meeting.h). Measured: one row of 65,536 fp32 logits with top-p 22 us,
- * with top-k 13; 64 rows 36 and 20.
+ * 4,096), which stay in its registers. What bounds it is neither bytes nor operations (a row of 65,536 fp32 logits is
+ * 256 KiB) but the steps one after the other, each ending where the row's workgroups need one another: the largest logit; the
+ * histogram; the list; about 2.5 us a meeting through memory. Greedy rows and a top-k of at most 128 need no meeting: every
+ * slice leaves its k largest in order, and the last workgroup to arrive does the rest on k tokens. No meeting waits without
+ * bound: where the others do not come, because the device is crowded, a row is given up and one workgroup does it
+ * (nc_meeting.h). Measured: one row of 65,536 fp32 logits with top-p 22 us, with top-k 13; 64 rows 36 and 20.
  *
  * row_kernel takes a row by one workgroup that reads it again for every step, for more rows and for longer ones. With top-p
  * it is bound by the exponentials, twice for every token (about 180 cycles of a SIMD for a wave's 64, most of them float64
