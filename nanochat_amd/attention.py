@@ -294,16 +294,18 @@ def packed_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.Te
     """q bf16 [rows, Hq, 128], the packed rows of sequences with any numbers of new tokens (decoding rows beside prompt
     chunks and draft tokens), already appended -> out bf16 [rows, Hq, 128].
 
-    Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1]) and the last of its seq_lens[b]
-    tokens (int32 [B]); its row at position p attends keys [max(p - window, 0), p] through block_table[b]. max_seq_len
-    bounds seq_lens: a longer sequence's rows are NaN, as are those of one shorter than its new tokens. Entries of block_table
-    whose keys no row attends (pages behind a window that were given back) may hold anything; one outside the cache that a row
-    does attend makes that row NaN, and others of its sequence beside it. Rows outside every sequence are not written. A sequence's output bits depend on nothing but its own numbers. A workspace passed in must
+    Sequence b's new tokens are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [B + 1]) and the last of its
+    seq_lens[b] tokens (int32 [B]); its row at position p attends keys [max(p - window, 0), p] through block_table[b].
+    max_seq_len bounds seq_lens: a longer sequence's rows are NaN, as are those of one shorter than its new tokens.
+    Entries of block_table whose keys no row attends (pages behind a window that were given back) may hold anything; one
+    outside the cache that a row does attend makes that row NaN, and others of its sequence beside it. Rows outside every
+    sequence are not written. A sequence's output bits depend on nothing but its own numbers. A workspace passed in must
     have been zero-filled before its first use (torch.zeros, at least packed_workspace_bytes) and only used by these and
-    decode_attention's calls since, one stream at a time. Without one, calls on a stream share a cached workspace (up to eight
-    streams' are kept, see packed_workspace_bytes for their size); a call that is being captured into a graph gets one of the
-    graph's own. Softmax and sums are fp32; a probability times its key's V scale is rounded to bf16. One launch takes 1,024 sequences; a larger batch, up to
-    every slot of a paging.BlockTables, is as many launches, with the same bits."""
+    decode_attention's calls since, one stream at a time. Without one, calls on a stream share a cached workspace (up to
+    eight streams' are kept, see packed_workspace_bytes for their size); a call that is being captured into a graph gets
+    one of the graph's own. Softmax and sums are fp32; a probability times its key's V scale is rounded to bf16. One
+    launch takes 1,024 sequences; a larger batch, up to every slot of a paging.BlockTables, is as many launches, with the
+    same bits."""
     _require(q, "q", torch.bfloat16)
     if q.dim() != 3 or q.size(2) != HEAD_DIM or q.size(1) < 1:
         raise ValueError(f"q must be [rows, Hq, {HEAD_DIM}], got {tuple(q.shape)}")
