@@ -345,6 +345,54 @@ int nc_debug_sample_tokens(const void *logits, int is_bf16, long long row_stride
                            void *workspace, size_t workspace_bytes, int patience, void *stream);
 
 /*
+ * The 8-bit form of matrices, their products, and the training of linear layers from 8-bit checkpoints; no counterpart in the
+ * reference, whose linear layers are bf16 (model/ops/linear.py:51-57, 135-144). A matrix is held as OCP e4m3fn codes and one
+ * power of two for each block, a byte holding its exponent + 127 (e8m0): blocks of 128 columns of a row for activations and
+ * gradients, 128 x 128 for weights (the last of a row or column may be shorter). The scale is the least power of two s with
+ * max |x| <= 448 s, at least 2^-126 (1 for a block of zeros); a code is x / s rounded to nearest even and stands for code * s. A
+ * block that holds an infinity or a NaN becomes NaN (byte 255, codes 0x7F). Columns are a multiple of 16. Codes are dense and
+ * 16-byte aligned; scales have rows at a stride in bytes that is a multiple of 4, readable to its end, 4-byte aligned.
+ */
+
+/* The 8-bit form of rows of activations: x bf16 or fp32 (is_f32) [rows][cols] at row_stride elements (any alignment of its
+ * type; 16-byte rows are read faster) -> codes [rows][cols], scale [rows][ceil(cols / 128)] at scale_stride bytes. rows *
+ * ceil(cols / 128) < 2^31. */
+int nc_fp8_quantize_rows(const void *x, int is_f32, long long row_stride, long long rows, int cols, void *codes, void *scale,
+                         long long scale_stride, void *stream);
+
+/* The 8-bit form of a weight: w bf16 or fp32 [n][k] at row_stride elements -> codes [n][k], scale [ceil(n / 128)][ceil(k /
+ * 128)], and, unless codes_t is NULL, those of its transpose: codes_t [k][n], scale_t [ceil(k / 128)][ceil(n / 128)] (n then a
+ * multiple of 16). n, k <= 2^20. */
+int nc_fp8_quantize_weight(const void *w, int is_f32, long long row_stride, int n, int k, void *codes, void *scale,
+                           int scale_stride, void *codes_t, void *scale_t, int scale_t_stride, void *stream);
+
+/* out[m][n] = sum_k a[m][k] w[n][k], a [rows][k] and w [n][k] in the 8-bit form, n and k multiples of 16:
+ * nc_fp8_matmul         out bf16 [rows][n]
+ * nc_fp8_matmul_relu2   relu(out)^2 of the fp32 sums in the 8-bit form: codes [rows][n], scale at scale_stride
+ * nc_fp8_matmul_relu2_bwd  out = bf16(sum * 2 sqrt(act)), act [rows][n] in the 8-bit form (as nc_fp8_matmul_relu2 leaves it), and
+ *                       the 8-bit form of out: the gradient before a ReLU^2 whose result act is, from the one behind it
+ * Sums are fp32, but for the eight products of adjacent k that the matrix cores add at a time: of those, bits below 2^-13 of
+ * the largest are dropped (at most 2^-10 of the sum of magnitudes, and 1e-5 to 3e-5 of a result as a rule). The outputs may not overlap the inputs. */
+int nc_fp8_matmul(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
+                  int w_scale_stride, long long rows, int n, int k, void *out, void *stream);
+int nc_fp8_matmul_relu2(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
+                        int w_scale_stride, long long rows, int n, int k, void *codes, void *scale, long long scale_stride,
+                        void *stream);
+int nc_fp8_matmul_relu2_bwd(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
+                            int w_scale_stride, long long rows, int n, int k, const void *act, const void *act_scale,
+                            long long act_scale_stride, void *out, void *codes, void *scale, long long scale_stride,
+                            void *stream);
+
+/* The gradient of a weight from the 8-bit checkpoint of its layer's input: out[i][j] = sum_m dy[m][i] x[m][j], dy bf16
+ * [rows][n1] dense (n1 a multiple of 8), x [rows][n2] in the 8-bit form (scale_stride <= n2). mode 0: out fp32; 1: added to out,
+ * fp32; 2: out bf16. Products are exact and sums fp32, in an order that depends on the sizes alone. rows < 2^31, n1 and n2 <=
+ * 65,536; rows = 0 launches nothing (and leaves out as it is). workspace: nc_fp8_weight_grad_workspace_bytes (-1 for
+ * unsupported sizes), 16-byte aligned, need not be cleared. */
+long long nc_fp8_weight_grad_workspace_bytes(long long rows, int n1, int n2);
+int nc_fp8_weight_grad(const void *dy, const void *codes, const void *scale, long long scale_stride, long long rows, int n1,
+                       int n2, int mode, void *out, void *workspace, long long workspace_bytes, void *stream);
+
+/*
  * Measurement only; no counterpart in the reference. Reads n pages of 2 KiB (one (page, head) of K or V codes) from
  * src (src_bytes, a multiple of 2,048), page order[i] as the i-th (order NULL: page i; an entry outside the buffer
  * reads page 0), with `grid` workgroups of 256 threads, and writes one checksum word per thread to sink

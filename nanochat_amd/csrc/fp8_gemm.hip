@@ -1,0 +1,343 @@
+/*
+ * Products of two matrices in the 8-bit form (nc_fp8.h) on gfx950: out[m][n] = epilogue(sum_k a[m][k] w[n][k]), a with a scale
+ * for each 128 columns of a row, w for each 128 x 128.
+ *
+ * v_mfma_scale_f32_16x16x128_f8f6f4 takes one block a step and applies both scales itself: its A operand holds 16 weight rows,
+ * its B operand 16 activation rows, lane (g = lane / 16, i = lane % 16) bytes 32 g .. + 31 of row i and that row's scale byte.
+ * A wave owns 128 columns n (a block of w, so its scale is one number) and 16 NU rows m. Which weight row is which row of an
+ * A operand is free: operand t's row r is row 32 (r / 4) + 4 t + r % 4 of the wave's 128, so that a lane's results, rows 4 g + e
+ * of operand t = 0 .. 7, are the 32 adjacent columns 32 g + 4 t + e of row m: whole 16-byte stores, and a row's block of 128
+ * meets across four lanes where the epilogue needs its largest magnitude.
+ *
+ * Operands go from memory to LDS by DMA in stages of 128 k (128 bytes a row), two buffers in turn: a stage's wait and one
+ * barrier without a memory fence, the next stage's DMA, then this stage's products. A row keeps its 16-byte piece b at place
+ * b ^ swizzle(row), so that the 16 lanes that an LDS read serves at a time meet in different banks.
+ *
+ * Rows past M and N and columns past K read zeros (offsets past the buffer resource), and are not stored.
+ *
+ * The instruction adds the eight products of a lane's adjacent bytes at 13 bits below the largest of them (measured: beside
+ * 2^16, 2^3 is kept and 2^2 is not, of either sign; products of other eights keep theirs) and everything else in fp32: 1.5e-5
+ * relative error for normal values, 3e-5 with a few channels far above the others, against the 2e-3 of a bf16 result.
+ */
+#include "nanochat_amd.h"
+#include "nc_fp8.h"
+#include "nc_internal.h"
+
+namespace nc {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+typedef __attribute__((address_space(3))) void LdsPtr;
+
+constexpr int FG_ROWB = F8_BLOCK;        /* bytes of a row of a stage: one block */
+constexpr int FG_PAST = 0x7FFF0000;      /* a byte offset past every operand's range */
+
+enum { FG_STORE, FG_RELU2, FG_RELU2_BWD };
+
+struct F8Gemm {
+    const unsigned char *a, *as;         /* [M][K] codes, [M] scale bytes at as_stride */
+    const unsigned char *w, *ws;         /* [N][K] codes, [ceil(N / 128)] scale bytes at ws_stride */
+    long long as_stride;
+    int ws_stride;
+    long long M;
+    int N, K;
+    uint16_t *out;                       /* [M][N] bf16 (STORE, RELU2_BWD) */
+    unsigned char *q, *qs;               /* [M][N] codes and their scales at qs_stride (RELU2, RELU2_BWD: written) */
+    const unsigned char *act, *acts;     /* [M][N] codes and scales at act_stride (RELU2_BWD: read) */
+    long long qs_stride, act_stride;
+};
+
+template <int NU_, int WN_, int WM_> struct FgTile {
+    static constexpr int NU = NU_, WN = WN_, WM = WM_, WAVES = WN * WM, TM = 16 * NU * WM, TN = F8_BLOCK * WN;
+    static constexpr int ROWS = TM + TN, STAGE = ROWS * FG_ROWB, LOADS = ROWS / 8 / WAVES, A_LOADS = TM / 8 / WAVES;
+    static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0, "DMA split");
+};
+typedef FgTile<4, 2, 4> FgFull;      /* 256 x 256, 8 waves */
+typedef FgTile<2, 1, 4> FgHalf;      /* 128 x 128, 4 waves */
+typedef FgTile<1, 1, 4> FgSmall;     /* 64 x 128, 4 waves */
+
+__device__ __forceinline__ Rsrc fg_rsrc(const void *p, long long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
+}
+
+/* A 16-byte LDS read serves lanes 0-3, 12-15, 20-23 and 24-27 together, then 4-11, 16-19 and 28-31, and so the upper half. Two
+ * rows lie side by side over the 64 banks, so 8 rows of one parity, four of one 16-byte piece b and four of b ^ 2, need 8
+ * places. Activation rows i: i / 2 in {0, 1, 6, 7} gives places 0 to 3 (closed under ^ 2), the others 4 to 7. Weight rows 32 q
+ * + 4 t + c stand for i = 4 q + c: the same by q (0, 3 or 1, 2) and c / 2, whatever t is. */
+__device__ __forceinline__ int fg_swizzle_a(int row) {
+    const int k = (row >> 1) & 7;
+    return (k & 3) | (((k + 2) & 4));
+}
+__device__ __forceinline__ int fg_swizzle_w(int row) {
+    const int q = (row >> 5) & 3, u = ((q << 1) & 3) ^ ((q >> 1) * 3);   /* 0, 2, 3, 1 */
+    return ((row >> 1) & 1) | (u << 1);
+}
+
+__device__ __forceinline__ void fg_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <class P>
+__device__ __forceinline__ void fg_fetch(Rsrc ra, Rsrc rw, unsigned char *buf, int j, int K, int wave, int lane) {
+    const int pos = lane & 7;
+#pragma unroll
+    for (int s = 0; s < P::LOADS; s++) {
+        const bool is_a = s < P::A_LOADS;
+        const int q = wave + P::WAVES * s, row = 8 * q + (lane >> 3) - (is_a ? 0 : P::TM);
+        const int piece = pos ^ (is_a ? fg_swizzle_a(row) : fg_swizzle_w(row)), col = j * FG_ROWB + 16 * piece;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(is_a ? ra : rw, (LdsPtr *)(buf + q * 1024), 16,
+                                                 col < K ? row * K + col : FG_PAST, 0, 0, 0);
+    }
+}
+
+__device__ __forceinline__ i32x8 fg_operand(const unsigned char *buf, int lo, int hi) {
+    const u32x4 x = *(const u32x4 *)(buf + lo), y = *(const u32x4 *)(buf + hi);
+    return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+}
+
+/* A stage's products; BYTE: which byte of the scale dwords is its block's. */
+template <class P, int BYTE>
+__device__ __forceinline__ void fg_compute(const unsigned char *buf, f32x4 (&acc)[8][P::NU], const uint32_t (&sa)[P::NU],
+                                           uint32_t sw, int a_at, int w_at) {
+    i32x8 fb[P::NU];
+#pragma unroll
+    for (int u = 0; u < P::NU; u++) fb[u] = fg_operand(buf, a_at + u * 16 * FG_ROWB, (a_at ^ 16) + u * 16 * FG_ROWB);
+#pragma unroll
+    for (int t = 0; t < 8; t++) {
+        const i32x8 fa = fg_operand(buf, w_at + t * 4 * FG_ROWB, (w_at ^ 16) + t * 4 * FG_ROWB);
+#pragma unroll
+        for (int u = 0; u < P::NU; u++)
+            acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb[u], acc[t][u], 0, 0, BYTE, (int)sw, BYTE,
+                                                                         (int)sa[u]);
+    }
+}
+
+/* Stage j from CUR, its successor's DMA into OTHER. */
+#define FG_STEP(j, BYTE, CUR, OTHER)                                              \
+    do {                                                                           \
+        if ((j) < stages) {                                                        \
+            __builtin_amdgcn_s_waitcnt(0);                                         \
+            fg_barrier();                                                          \
+            if ((j) + 1 < stages) fg_fetch<P>(ra, rw, OTHER, (j) + 1, g.K, wave, lane); \
+            fg_compute<P, BYTE>(CUR, acc, sa, sw, a_at, w_at);                     \
+        }                                                                          \
+    } while (0)
+
+template <class P, int EPI>
+__device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, unsigned char *b0, unsigned char *b1) {
+    const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x >> 6, grp = lane >> 4, i = lane & 15;
+    const int wn = wave % P::WN, wm = wave / P::WN;
+    const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
+    const int rows = (int)(g.M - m0 < P::TM ? g.M - m0 : P::TM), cols = g.N - n0 < P::TN ? g.N - n0 : P::TN;
+    const Rsrc ra = fg_rsrc(g.a + m0 * g.K, (long long)rows * g.K);
+    const Rsrc rw = fg_rsrc(g.w + (long long)n0 * g.K, (long long)cols * g.K);
+    const Rsrc rs = fg_rsrc(g.as + m0 * g.as_stride, rows * g.as_stride);
+    const int nb = n0 / F8_BLOCK + wn, row0 = 16 * P::NU * wm + i;
+    const bool some = F8_BLOCK * wn < cols;                   /* the wave has columns */
+    const uint32_t *ws = (const uint32_t *)(g.ws + (long long)(some ? nb : 0) * g.ws_stride);
+
+    f32x4 acc[8][P::NU];
+#pragma unroll
+    for (int t = 0; t < 8; t++)
+#pragma unroll
+        for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t sa[P::NU], na[P::NU], sw, nw = ws[0];
+#pragma unroll
+    for (int u = 0; u < P::NU; u++)
+        na[u] = __builtin_amdgcn_raw_buffer_load_b32(rs, (row0 + 16 * u) * (int)g.as_stride, 0, 0);
+    fg_fetch<P>(ra, rw, b0, 0, g.K, wave, lane);
+    const int a_at = row0 * FG_ROWB + (((2 * grp) ^ fg_swizzle_a(row0)) << 4);
+    const int w_row = F8_BLOCK * wn + 32 * (i >> 2) + (i & 3);
+    const int w_at = (P::TM + w_row) * FG_ROWB + (((2 * grp) ^ fg_swizzle_w(w_row)) << 4);
+    for (int j = 0; j < stages; j += 4) {
+        sw = nw;
+#pragma unroll
+        for (int u = 0; u < P::NU; u++) sa[u] = na[u];
+        if (j + 4 < stages) {   /* the next four blocks' scales */
+            nw = ws[j / 4 + 1];
+#pragma unroll
+            for (int u = 0; u < P::NU; u++)
+                na[u] = __builtin_amdgcn_raw_buffer_load_b32(rs, (row0 + 16 * u) * (int)g.as_stride + j + 4, 0, 0);
+        }
+        FG_STEP(j, 0, b0, b1);
+        FG_STEP(j + 1, 1, b1, b0);
+        FG_STEP(j + 2, 2, b0, b1);
+        FG_STEP(j + 3, 3, b1, b0);
+    }
+
+    if (!some) return;
+    const int c0 = F8_BLOCK * wn + 32 * grp;                  /* this lane's 32 columns from n0 */
+#pragma unroll
+    for (int u = 0; u < P::NU; u++) {
+        const int r = row0 + 16 * u;
+        const bool in = r < rows;
+        const long long at = (m0 + r) * g.N + n0 + c0;
+        float v[32];
+#pragma unroll
+        for (int t = 0; t < 8; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[4 * t + e] = acc[t][u][e];
+        if (EPI == FG_RELU2) {
+            uint32_t m = 0u;
+#pragma unroll
+            for (int k = 0; k < 32; k++) {
+                const float p = v[k] < 0.0f ? 0.0f : v[k];    /* a NaN stays one */
+                v[k] = p * p;
+                const uint32_t b = __float_as_uint(v[k]) & 0x7FFFFFFFu;
+                m = m > b ? m : b;
+            }
+            const uint32_t byte = f8_scale_byte(group_max(m));
+            const float s = f8_scale(byte);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                u32x4 c;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int z = 16 * h + 4 * k;
+                    c[k] = byte == F8_NAN_BYTE ? F8_NAN_CODES : f8_codes(v[z], v[z + 1], v[z + 2], v[z + 3], s);
+                }
+                if (in && c0 + 16 * h < cols) *(u32x4 *)(g.q + at + 16 * h) = c;
+            }
+            if (in && grp == 0) g.qs[(m0 + r) * g.qs_stride + nb] = (unsigned char)byte;
+            continue;
+        }
+        uint32_t o[16];
+        if (EPI == FG_RELU2_BWD) {
+            /* dh = da 2 sqrt(a); a's codes are this lane's 32 columns, its scale the block's */
+            u32x4 c[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+            uint32_t byte = 127u;
+            if (in) {
+                byte = g.acts[(m0 + r) * g.act_stride + nb];
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (c0 + 16 * h < cols) c[h] = *(const u32x4 *)(g.act + at + 16 * h);
+            }
+            const float s = f8_scale(byte);
+            uint32_t m = 0u;
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const uint32_t w = c[k >> 3][(k >> 1) & 3];
+                const auto a = (k & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true)
+                                       : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false);
+                /* v_sqrt_f32 is within an ulp; the result is rounded to bf16 right away */
+                const float x = v[2 * k] * (2.0f * __builtin_amdgcn_sqrtf(a[0]));
+                const float y = v[2 * k + 1] * (2.0f * __builtin_amdgcn_sqrtf(a[1]));
+                o[k] = bf16_pair(x, y);
+                m = pair_amax(m, o[k]);
+            }
+            const uint32_t qb = f8_scale_byte(group_max(pair_top(m)));
+            const float qs = f8_scale(qb);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                u32x4 q;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    q[k] = qb == F8_NAN_BYTE ? F8_NAN_CODES : f8_codes(o[8 * h + 2 * k], o[8 * h + 2 * k + 1], qs);
+                if (in && c0 + 16 * h < cols) *(u32x4 *)(g.q + at + 16 * h) = q;
+            }
+            if (in && grp == 0) g.qs[(m0 + r) * g.qs_stride + nb] = (unsigned char)qb;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; k++) o[k] = bf16_pair(v[2 * k], v[2 * k + 1]);
+        }
+#pragma unroll
+        for (int h = 0; h < 4; h++)
+            if (in && c0 + 8 * h < cols)
+                *(u32x4 *)(g.out + at + 8 * h) = u32x4{o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]};
+    }
+}
+
+/* The order workgroups take tiles in. Workgroup L runs on XCD L % 8, each with its own L2: XCD k gets a contiguous run of the
+ * tiles, numbered in bands of 4 m-tiles walked m first, so that what an XCD runs at once shares operand tiles. */
+__device__ __forceinline__ int2 fg_tile(int l, int count, int nx) {
+    const int k = l % 8, r = l / 8, per = count / 8, extra = count % 8;
+    const int id = k * per + min(k, extra) + r, band = 4 * nx, y0 = id / band * 4, ny = count / nx - y0;
+    const int tall = ny < 4 ? ny : 4, in = id - id / band * band;
+    return int2{in / tall, y0 + in % tall};
+}
+
+template <class P, int EPI>
+__global__ void __launch_bounds__(P::WAVES *WAVE, P::WAVES == 8 ? 2 : 2) fp8_gemm_kernel(F8Gemm g) {
+    __shared__ __align__(16) unsigned char b0[P::STAGE], b1[P::STAGE];   /* distinct objects: reads of one do not wait for
+                                                                            the other's DMA */
+    const int2 t = fg_tile(blockIdx.x, gridDim.x, (g.N + P::TN - 1) / P::TN);
+    fg_run<P, EPI>(g, (long long)t.y * P::TM, t.x * P::TN, b0, b1);
+}
+
+template <class P>
+int fg_launch(const F8Gemm &g, int epi, hipStream_t stream) {
+    const long long tiles = (g.M + P::TM - 1) / P::TM * ((g.N + P::TN - 1) / P::TN);
+    if (tiles >= (1LL << 31)) return NC_ERR_SHAPE;
+    const auto kernel = epi == FG_STORE ? fp8_gemm_kernel<P, FG_STORE>
+                        : epi == FG_RELU2 ? fp8_gemm_kernel<P, FG_RELU2> : fp8_gemm_kernel<P, FG_RELU2_BWD>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(P::WAVES * WAVE), 0, stream, g);
+    return (int)hipGetLastError();
+}
+
+bool misaligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) != 0; }
+bool bad_scales(const void *p, long long stride, int cols) {
+    return misaligned(p, 4) || stride % 4 || stride < (cols + F8_BLOCK - 1) / F8_BLOCK || stride > (1 << 14);
+}
+
+/* Sizes first, then pointers, then their alignment. */
+int fg_check(const F8Gemm &g, int epi) {
+    if (g.M < 0 || g.M > (1LL << 31) || g.N <= 0 || g.K <= 0 || g.N % 16 || g.K % 16 || g.N > (1 << 20) || g.K > (1 << 20))
+        return NC_ERR_SHAPE;
+    if (g.M == 0) return NC_OK;
+    if (!g.a || !g.as || !g.w || !g.ws || (epi != FG_RELU2 && !g.out) || (epi != FG_STORE && (!g.q || !g.qs)) ||
+        (epi == FG_RELU2_BWD && (!g.act || !g.acts)))
+        return NC_ERR_NULL;
+    if (misaligned(g.a, 16) || misaligned(g.w, 16) || misaligned(g.out, 16) || misaligned(g.q, 16) || misaligned(g.act, 16) ||
+        bad_scales(g.as, g.as_stride, g.K) || bad_scales(g.ws, g.ws_stride, g.K) ||
+        (epi != FG_STORE && bad_scales(g.qs, g.qs_stride, g.N)) ||
+        (epi == FG_RELU2_BWD && bad_scales(g.acts, g.act_stride, g.N)))
+        return NC_ERR_SHAPE;
+    return NC_OK;
+}
+
+int fg_gemm(const F8Gemm &g, int epi, void *stream) {
+    const int e = fg_check(g, epi);
+    if (e != NC_OK || g.M == 0) return e;
+    const long long full = (g.M + 255) / 256 * ((g.N + 255) / 256), half = (g.M + 127) / 128 * ((g.N + 127) / 128);
+    const int cus = device_cus();
+    if (full >= cus) return fg_launch<FgFull>(g, epi, (hipStream_t)stream);
+    if (half >= cus) return fg_launch<FgHalf>(g, epi, (hipStream_t)stream);
+    return fg_launch<FgSmall>(g, epi, (hipStream_t)stream);
+}
+
+}  // namespace
+}  // namespace nc
+
+using namespace nc;
+
+extern "C" int nc_fp8_matmul(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
+                             int w_scale_stride, long long rows, int n, int k, void *out, void *stream) {
+    const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
+                      (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, (uint16_t *)out,
+                      nullptr, nullptr, nullptr, nullptr, 0, 0};
+    return fg_gemm(g, FG_STORE, stream);
+}
+
+extern "C" int nc_fp8_matmul_relu2(const void *a, const void *a_scale, long long a_scale_stride, const void *w,
+                                   const void *w_scale, int w_scale_stride, long long rows, int n, int k, void *codes,
+                                   void *scale, long long scale_stride, void *stream) {
+    const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
+                      (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, nullptr,
+                      (unsigned char *)codes, (unsigned char *)scale, nullptr, nullptr, scale_stride, 0};
+    return fg_gemm(g, FG_RELU2, stream);
+}
+
+extern "C" int nc_fp8_matmul_relu2_bwd(const void *a, const void *a_scale, long long a_scale_stride, const void *w,
+                                       const void *w_scale, int w_scale_stride, long long rows, int n, int k,
+                                       const void *act, const void *act_scale, long long act_scale_stride, void *out,
+                                       void *codes, void *scale, long long scale_stride, void *stream) {
+    const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
+                      (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, (uint16_t *)out,
+                      (unsigned char *)codes, (unsigned char *)scale, (const unsigned char *)act,
+                      (const unsigned char *)act_scale, scale_stride, act_scale_stride};
+    return fg_gemm(g, FG_RELU2_BWD, stream);
+}

@@ -1,0 +1,78 @@
+/*
+ * The 8-bit form of matrices (fp8_quant.hip, fp8_gemm.hip, fp8_grad.hip): e4m3 codes and one power of two for each block of
+ * 128 columns of a row (activations, gradients) or 128 x 128 of a weight, kept as its biased exponent (e8m0, a byte). A value
+ * stands for code * 2^(byte - 127).
+ *
+ * The scale is the least power of two s with amax <= 448 s: amax = m 2^e with m in [1, 2) gives 2^(e - 8), doubled where m >
+ * 1.75 (448 = 1.75 2^8). A block of zeros has scale 1. A power of two keeps the codes' relative error at half a step (2^-4)
+ * whatever it is, down to amax 2^-15 / 1.75 or less where e4m3 becomes subnormal; it makes x / s exact, so a code is one
+ * rounding of x, and code * s exact in bf16, which the matrix cores multiply as it is.
+ * A block with an infinity or a NaN becomes NaN whole (byte 255, every code 0x7F): what is made from it is NaN too.
+ */
+#pragma once
+
+#include "nc_device.h"
+
+namespace nc {
+
+constexpr int F8_BLOCK = 128;
+constexpr uint32_t F8_NAN_BYTE = 255, F8_NAN_CODES = 0x7F7F7F7Fu;
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+/* The scale byte for a block's largest magnitude, given as the bits of |x| in fp32 (at or past 0x7F800000: an infinity or a
+ * NaN is in the block). At least 1: 2^-126, so that both the scale and its inverse are normal numbers. */
+__device__ __forceinline__ uint32_t f8_scale_byte(uint32_t amax) {
+    const int e = (int)(amax >> 23) - 8 + ((amax & 0x7FFFFFu) > 0x600000u);
+    const uint32_t byte = e < 1 ? 1u : (uint32_t)e;
+    return amax >= 0x7F800000u ? F8_NAN_BYTE : amax == 0u ? 127u : byte;
+}
+
+__device__ __forceinline__ float f8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+/* Four codes of two bf16 pairs, or of four fp32, over a scale (one rounding each, to nearest even). The converter divides by
+ * the scale's power of two itself; |x| <= 448 s by the choice of s, so nothing saturates. */
+__device__ __forceinline__ uint32_t f8_codes(uint32_t lo, uint32_t hi, float s) {
+    s16x2 r = {0, 0};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, lo), s, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, hi), s, true);
+    return __builtin_bit_cast(uint32_t, r);
+}
+__device__ __forceinline__ uint32_t f8_codes(float a, float b, float c, float d, float s) {
+    s16x2 r = {0, 0};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, s, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, s, true);
+    return __builtin_bit_cast(uint32_t, r);
+}
+
+/* Two fp32 -> a bf16 pair (to nearest even; NaN stays NaN). */
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+
+/* The larger |x| of both halves of two bf16 pairs: their bits without signs order as the magnitudes do. */
+__device__ __forceinline__ uint32_t pair_amax(uint32_t m, uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                                  __builtin_bit_cast(u16x2, w & 0x7FFF7FFFu)));
+}
+/* ... and of a pair's own two, as the bits of an fp32. */
+__device__ __forceinline__ uint32_t pair_top(uint32_t m) {
+    const uint32_t lo = m << 16, hi = m & 0xFFFF0000u;
+    return lo > hi ? lo : hi;
+}
+
+/* Largest over lanes L ^ 1, 2, 4 (8 lanes), over L ^ 16 and L ^ 32 (the four groups of 16 lanes). */
+template <int M> __device__ __forceinline__ uint32_t lane_max_dpp(uint32_t v) {
+    const uint32_t o = __float_as_uint(lane_xor_dpp<M>(__uint_as_float(v)));
+    return v > o ? v : o;
+}
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = a[0] > a[1] ? a[0] : a[1];
+    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return b[0] > b[1] ? b[0] : b[1];
+}
+
+}  // namespace nc

@@ -1,0 +1,516 @@
+"""Linear layers in 8-bit floating point, and their training from 8-bit checkpoints of their inputs (csrc/fp8_quant.hip,
+fp8_gemm.hip, fp8_grad.hip). No counterpart in the reference, whose linear layers and ReLU^2 MLP are bf16
+(model/ops/linear.py:51-57, 135-144).
+
+The 8-bit form of a matrix: e4m3 codes and one power of two for each block, held as its exponent (torch.float8_e8m0fnu).
+Blocks are 128 columns of a row of activations or gradients and 128 x 128 of a weight. The scale is the least s with
+max |x| <= 448 s; a code stands for code * s. A power of two makes that value exact in bf16 and lets the matrix cores apply
+the scales themselves. A block that holds an infinity or a NaN becomes NaN whole.
+
+- quantize_rows, quantize_weight: the 8-bit form of activations, of weights (with that of the transpose, for training)
+- fp8_linear, fp8_mlp: a layer, and a ReLU^2 MLP, on weights held in 8 bits, for serving: one row to many thousand
+- fp8_matmul: the product of activations already in 8 bits
+- checkpointed_linear, checkpointed_mlp: the same in training, as the registered ops nanochat_amd::checkpointed_linear and
+  nanochat_amd::checkpointed_mlp. What is kept for the backward is the 8-bit form of the layer's input (and of the MLP's
+  hidden activations): half of bf16's bytes, and the very operand that the forward product took
+- checkpoint_weight_grad: a weight's gradient from such a checkpoint
+
+Every function launches on the current stream of its input's device and requires device tensors: there is no CPU path."""
+
+from typing import NamedTuple
+
+import torch
+from torch import Tensor
+from torch.autograd.function import FunctionCtx
+
+from .native import check, device_guard, hip_library, pointer, stream
+
+BLOCK = 128
+CODES, SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+class Fp8Weight(NamedTuple):
+    """A weight [N, K] in the 8-bit form: codes [N, K], scale [ceil(N / 128), ceil(K / 128)] (rows at a stride that is a
+    multiple of 4), and for training those of its transpose, codes_t [K, N] and scale_t."""
+    codes: Tensor
+    scale: Tensor
+    codes_t: Tensor | None = None
+    scale_t: Tensor | None = None
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _new_scale(like: Tensor, rows: int, cols: int) -> Tensor:
+    """Scales [rows, ceil(cols / 128)], their rows padded to a multiple of 4 bytes."""
+    blocks = _blocks(cols)
+    return torch.empty(rows, -(-blocks // 4) * 4, dtype=SCALE, device=like.device)[:, :blocks]
+
+
+def _check_codes(codes: Tensor, name: str, device: torch.device) -> None:
+    if codes.dtype != CODES:
+        raise TypeError(f"{name} must be {CODES}, got {codes.dtype}")
+    if not codes.is_cuda or codes.device != device:
+        raise ValueError(f"{name} must be a device tensor on {device}, got {codes.device}")
+    if codes.dim() != 2 or not codes.is_contiguous() or codes.data_ptr() % 16:
+        raise ValueError(f"{name} must be a contiguous, 16-byte aligned matrix")
+    if codes.size(1) % 16:
+        raise ValueError(f"{name} must have a multiple of 16 columns, got {codes.size(1)}")
+
+
+def _check_scale(scale: Tensor, name: str, rows: int, cols: int, device: torch.device) -> int:
+    """A scale tensor's row stride in bytes."""
+    if scale.dtype != SCALE:
+        raise TypeError(f"{name} must be {SCALE}, got {scale.dtype}")
+    blocks = _blocks(cols)
+    if scale.shape != (rows, blocks) or scale.device != device:
+        raise ValueError(f"{name} must be [{rows}, {blocks}] on {device}, got {tuple(scale.shape)} on {scale.device}")
+    pitch = scale.stride(0)
+    if ((blocks > 1 and scale.stride(1) != 1) or pitch % 4 or pitch < blocks or pitch > cols or scale.data_ptr() % 4
+            or scale.storage_offset() + (rows - 1) * pitch + -(-blocks // 4) * 4 > scale.untyped_storage().nbytes()):
+        raise ValueError(f"{name} must have 4-byte aligned rows of adjacent scales, padded to a multiple of 4 bytes")
+    return pitch
+
+
+def _check_weight(w: Fp8Weight, name: str, device: torch.device, transposed: bool = False) -> tuple[int, int]:
+    """(pitch of the scales, of the transpose's or 0) of a weight in the 8-bit form."""
+    _check_codes(w.codes, f"{name}.codes", device)
+    n, k = w.codes.shape
+    pitch = _check_scale(w.scale, f"{name}.scale", _blocks(n), k, device)
+    if not transposed:
+        return pitch, 0
+    if w.codes_t is None or w.scale_t is None:
+        raise ValueError(f"{name} needs its transpose for training: quantize_weight(w, transpose=True)")
+    _check_codes(w.codes_t, f"{name}.codes_t", device)
+    if w.codes_t.shape != (k, n):
+        raise ValueError(f"{name}.codes_t must be {(k, n)}, got {tuple(w.codes_t.shape)}")
+    return pitch, _check_scale(w.scale_t, f"{name}.scale_t", _blocks(k), n, device)
+
+
+def _as_rows(x: Tensor, name: str, dtypes: tuple, of: int = 16) -> Tensor:
+    """x as rows [M, K] of adjacent values that do not overlap: a view where there is one."""
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be a device tensor (the 8-bit layers have no CPU implementation)")
+    if x.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(map(str, dtypes))}, got {x.dtype}")
+    if x.dim() < 1 or x.size(-1) < 1 or x.size(-1) % of:
+        raise ValueError(f"{name} must have a multiple of {of} columns, got {tuple(x.shape)}")
+    if x.dim() != 2:
+        x = x.reshape(-1, x.size(-1))
+    if x.stride(1) != 1 or (x.size(0) > 1 and x.stride(0) < x.size(1)):
+        x = x.contiguous()
+    return x
+
+
+def _quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    rows, cols = x.shape
+    codes, scale = torch.empty(rows, cols, dtype=CODES, device=x.device), _new_scale(x, rows, cols)
+    if rows:
+        check(hip_library().nc_fp8_quantize_rows(pointer(x), x.dtype == F32, x.stride(0) if rows > 1 else cols, rows, cols,
+                                                 pointer(codes), pointer(scale), scale.stride(0), stream()))
+    return codes, scale
+
+
+def quantize_rows(x: Tensor) -> tuple[Tensor, Tensor]:
+    """x bf16 or fp32 [..., K] (K a multiple of 16; rows of any stride, others are copied) -> its 8-bit form: codes
+    e4m3 [rows, K], scale e8m0 [rows, ceil(K / 128)], rows being all leading dimensions."""
+    x = _as_rows(x, "x", (BF16, F32))
+    with device_guard(x):
+        return _quantize(x)
+
+
+def quantize_weight(w: Tensor, transpose: bool = False) -> Fp8Weight:
+    """A weight bf16 or fp32 [N, K], K (and N with its transpose) a multiple of 16 -> its 8-bit form."""
+    if w.dim() != 2:
+        raise ValueError(f"w must be [N, K], got {tuple(w.shape)}")
+    w = _as_rows(w, "w", (BF16, F32))
+    n, k = w.shape
+    if n < 1 or (transpose and n % 16):
+        raise ValueError(f"w must have rows{', a multiple of 16 for its transpose' if transpose else ''}, got {n}")
+    codes, scale = torch.empty(n, k, dtype=CODES, device=w.device), _new_scale(w, _blocks(n), k)
+    codes_t = scale_t = None
+    if transpose:
+        codes_t, scale_t = torch.empty(k, n, dtype=CODES, device=w.device), _new_scale(w, _blocks(k), n)
+    with device_guard(w):
+        check(hip_library().nc_fp8_quantize_weight(
+            pointer(w), w.dtype == F32, w.stride(0) if n > 1 else k, n, k, pointer(codes), pointer(scale), scale.stride(0),
+            pointer(codes_t) if transpose else None, pointer(scale_t) if transpose else None,
+            scale_t.stride(0) if transpose else 0, stream()))
+    return Fp8Weight(codes, scale, codes_t, scale_t)
+
+
+def _product(codes: Tensor, scale: Tensor, w_codes: Tensor, w_scale: Tensor) -> Tensor:
+    rows, k = codes.shape
+    n = w_codes.size(0)
+    out = torch.empty(rows, n, dtype=BF16, device=codes.device)
+    check(hip_library().nc_fp8_matmul(pointer(codes), pointer(scale), scale.stride(0), pointer(w_codes), pointer(w_scale),
+                                      w_scale.stride(0), rows, n, k, pointer(out), stream()))
+    return out
+
+
+def _product_relu2(codes: Tensor, scale: Tensor, w_codes: Tensor, w_scale: Tensor) -> tuple[Tensor, Tensor]:
+    rows, k = codes.shape
+    n = w_codes.size(0)
+    out, out_scale = torch.empty(rows, n, dtype=CODES, device=codes.device), _new_scale(codes, rows, n)
+    check(hip_library().nc_fp8_matmul_relu2(pointer(codes), pointer(scale), scale.stride(0), pointer(w_codes),
+                                            pointer(w_scale), w_scale.stride(0), rows, n, k, pointer(out), pointer(out_scale),
+                                            out_scale.stride(0), stream()))
+    return out, out_scale
+
+
+def _product_relu2_bwd(codes: Tensor, scale: Tensor, w_codes: Tensor, w_scale: Tensor, act: Tensor,
+                       act_scale: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    rows, k = codes.shape
+    n = w_codes.size(0)
+    out, q = torch.empty(rows, n, dtype=BF16, device=codes.device), torch.empty_like(act)
+    q_scale = _new_scale(codes, rows, n)
+    check(hip_library().nc_fp8_matmul_relu2_bwd(
+        pointer(codes), pointer(scale), scale.stride(0), pointer(w_codes), pointer(w_scale), w_scale.stride(0), rows, n, k,
+        pointer(act), pointer(act_scale), act_scale.stride(0), pointer(out), pointer(q), pointer(q_scale), q_scale.stride(0),
+        stream()))
+    return out, q, q_scale
+
+
+def _outputs(n: int, name: str) -> None:
+    if n % 16:
+        raise ValueError(f"{name} must have a multiple of 16 rows for a product, got {n}")
+
+
+def fp8_matmul(codes: Tensor, scale: Tensor, weight: Fp8Weight) -> Tensor:
+    """Activations in the 8-bit form (quantize_rows') [M, K] times a weight's transpose: bf16 [M, N], N and K multiples of
+    16. Sums are fp32, but for the eight products of adjacent columns that the matrix cores add at a time: of those, bits
+    below 2^-13 of the largest are dropped (at most 2^-10 of the sum of magnitudes; 1e-5 to 3e-5 of a result as a rule)."""
+    device = codes.device
+    _check_codes(codes, "codes", device)
+    _check_scale(scale, "scale", codes.size(0), codes.size(1), device)
+    _check_weight(weight, "weight", device)
+    if weight.codes.size(1) != codes.size(1):
+        raise ValueError(f"codes have {codes.size(1)} columns, the weight {weight.codes.size(1)}")
+    _outputs(weight.codes.size(0), "weight")
+    with device_guard(codes):
+        return _product(codes, scale, weight.codes, weight.scale)
+
+
+def _serving_input(x: Tensor, weight: Fp8Weight, name: str) -> Tensor:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} has no backward: use checkpointed_linear or checkpointed_mlp, or torch.no_grad()")
+    rows = _as_rows(x, "x", (BF16,))
+    if weight.codes.dim() != 2 or weight.codes.size(1) != rows.size(1):
+        raise ValueError(f"x has {rows.size(1)} columns for a weight of {tuple(weight.codes.shape)}")
+    return rows
+
+
+def fp8_linear(x: Tensor, weight: Fp8Weight) -> Tensor:
+    """x bf16 [..., K] through a linear layer whose weight [N, K] is held in 8 bits: bf16 [..., N]. Each row of x is taken in
+    its 8-bit form. For serving: no gradient (checkpointed_linear has one)."""
+    rows = _serving_input(x, weight, "fp8_linear")
+    _check_weight(weight, "weight", x.device)
+    _outputs(weight.codes.size(0), "weight")
+    with device_guard(x):
+        out = _product(*_quantize(rows), weight.codes, weight.scale)
+    return out.view(*x.shape[:-1], out.size(1))
+
+
+def fp8_mlp(x: Tensor, fc: Fp8Weight, proj: Fp8Weight) -> Tensor:
+    """x bf16 [..., C] through proj(relu(fc(x))^2), fc [F, C] and proj [N, F] held in 8 bits: bf16 [..., N]. The squared
+    activations are taken in their 8-bit form from fp32 sums. For serving: no gradient (checkpointed_mlp has one)."""
+    rows = _serving_input(x, fc, "fp8_mlp")
+    _check_weight(fc, "fc", x.device)
+    _check_weight(proj, "proj", x.device)
+    if proj.codes.size(1) != fc.codes.size(0):
+        raise ValueError(f"proj {tuple(proj.codes.shape)} does not take fc's {fc.codes.size(0)} outputs")
+    _outputs(proj.codes.size(0), "proj")
+    with device_guard(x):
+        act = _product_relu2(*_quantize(rows), fc.codes, fc.scale)
+        out = _product(*act, proj.codes, proj.scale)
+    return out.view(*x.shape[:-1], out.size(1))
+
+
+# --- training
+
+_GRAD_F32, _GRAD_ADD, _GRAD_BF16 = 0, 1, 2
+
+
+def _weight_grad(dy: Tensor, codes: Tensor, scale: Tensor, out: Tensor, mode: int) -> Tensor:
+    (rows, n1), n2 = dy.shape, codes.size(1)
+    if rows == 0:
+        return out if mode == _GRAD_ADD else out.zero_()
+    lib = hip_library()
+    need = lib.nc_fp8_weight_grad_workspace_bytes(rows, n1, n2)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dy.device)   # an unsupported size: refused by the call
+    check(lib.nc_fp8_weight_grad(pointer(dy), pointer(codes), pointer(scale), scale.stride(0), rows, n1, n2, mode,
+                                 pointer(out), pointer(ws), need, stream()))
+    return out
+
+
+def _dense(t: Tensor) -> Tensor:
+    """t [M, N] with its rows one after another from a 16-byte border, as the weight gradient reads them."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _check_grad(grad: Tensor, shape: tuple, device: torch.device, name: str) -> None:
+    if grad.dtype != F32 or grad.device != device:
+        raise ValueError(f"{name} must be {F32} on {device}, got {grad.dtype} on {grad.device}")
+    if tuple(grad.shape) != tuple(shape) or not grad.is_contiguous() or grad.data_ptr() % 16:
+        raise ValueError(f"{name} must be a contiguous, 16-byte aligned {tuple(shape)}, got {tuple(grad.shape)}")
+
+
+def checkpoint_weight_grad(dy: Tensor, codes: Tensor, scale: Tensor, out: Tensor | None = None,
+                           dtype: torch.dtype = F32) -> Tensor:
+    """The gradient dy^T x of a weight [N, K], dy bf16 [..., N] (N a multiple of 8) the gradient behind the layer and x [M, K] the 8-bit
+    checkpoint of its input (quantize_rows'). Products are exact and sums fp32; the result is fp32, or rounded once to bf16
+    (dtype), or added to out (fp32 [N, K]) when given."""
+    dy = _as_rows(dy, "dy", (BF16,), of=8)
+    _check_codes(codes, "codes", dy.device)
+    _check_scale(scale, "scale", codes.size(0), codes.size(1), dy.device)
+    if dy.size(0) != codes.size(0):
+        raise ValueError(f"dy has {dy.size(0)} rows, the checkpoint {codes.size(0)}")
+    shape = (dy.size(1), codes.size(1))
+    if out is not None:
+        _check_grad(out, shape, dy.device, "out")
+    elif dtype not in (F32, BF16):
+        raise TypeError(f"dtype must be {F32} or {BF16}, got {dtype}")
+    with device_guard(dy):
+        if out is not None:
+            return _weight_grad(_dense(dy), codes, scale, out, _GRAD_ADD)
+        out = torch.empty(shape, dtype=dtype, device=dy.device)
+        return _weight_grad(_dense(dy), codes, scale, out, _GRAD_F32 if dtype == F32 else _GRAD_BF16)
+
+
+def _layer_grad(dy: Tensor, codes: Tensor, scale: Tensor, grad: Tensor | None, wanted: bool, wide: bool) -> Tensor:
+    """A layer's weight gradient as its op returns it: new, or empty where it went into grad or is not wanted."""
+    if not wanted:
+        return dy.new_empty(0)
+    if grad is not None:
+        _weight_grad(dy, codes, scale, grad, _GRAD_ADD)
+        return dy.new_empty(0)
+    out = torch.empty(dy.size(1), codes.size(1), dtype=F32 if wide else BF16, device=dy.device)
+    return _weight_grad(dy, codes, scale, out, _GRAD_F32 if wide else _GRAD_BF16)
+
+
+def _held(weight: Tensor, name: str, codes: Tensor | None, scale: Tensor | None, codes_t: Tensor | None,
+          scale_t: Tensor | None, grad: Tensor | None, device: torch.device) -> Fp8Weight:
+    """A layer's arguments checked, and the 8-bit form that its op uses: what it was given, or the weight's own, made now."""
+    if weight.dim() != 2 or weight.size(0) % 16 or weight.size(1) % 16 or weight.numel() == 0:
+        raise ValueError(f"{name} must be [N, K], both multiples of 16, got {tuple(weight.shape)}")
+    if weight.dtype not in (BF16, F32):
+        raise TypeError(f"{name} must be {BF16} or {F32}, got {weight.dtype}")
+    if weight.device != device:
+        raise ValueError(f"{name} must be on {device}, got {weight.device}")
+    if grad is not None:
+        _check_grad(grad, weight.shape, device, f"{name}'s gradient")
+    if codes is None:
+        return quantize_weight(weight, transpose=True)
+    held = Fp8Weight(codes, scale, codes_t, scale_t)
+    _check_weight(held, f"{name} in 8 bits", device, transposed=True)
+    if codes.shape != weight.shape:
+        raise ValueError(f"{name} is {tuple(weight.shape)}, its 8-bit form {tuple(codes.shape)}")
+    return held
+
+
+def _padded(scale: Tensor) -> Tensor:
+    """A new scale tensor with its rows' padding: whole, as an op returns it."""
+    return scale.as_strided((scale.size(0), scale.stride(0)), (scale.stride(0), 1))
+
+
+def _kept(given: bool, w: Fp8Weight) -> tuple[Tensor, Tensor]:
+    """The transpose that an op made, which its backward reads; empty where the caller holds it."""
+    if given:
+        return w.codes.new_empty(0), w.scale.new_empty(0)
+    return w.codes_t, _padded(w.scale_t)
+
+
+def _narrow(scale: Tensor, cols: int) -> Tensor:
+    return scale[:, :_blocks(cols)]
+
+
+@torch.library.custom_op("nanochat_amd::checkpointed_linear", mutates_args=(), device_types="cuda")
+def _linear(x: Tensor, weight: Tensor, codes: Tensor | None, scale: Tensor | None, codes_t: Tensor | None,
+            scale_t: Tensor | None, grad: Tensor | None) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """-> y, then what the backward reads: x's codes and scales, the weight's transposed codes and scales."""
+    rows = _as_rows(x, "x", (BF16,))
+    w = _held(weight, "weight", codes, scale, codes_t, scale_t, grad, x.device)
+    if rows.size(1) != weight.size(1):
+        raise ValueError(f"x has {rows.size(1)} columns for a weight of {tuple(weight.shape)}")
+    with device_guard(x):
+        x8, xs = _quantize(rows)
+        y = _product(x8, xs, w.codes, w.scale)
+    return (y.view(*x.shape[:-1], y.size(1)), x8, _padded(xs), *_kept(codes is not None, w))
+
+
+def _scale_like(like: Tensor, rows: int, cols: int) -> Tensor:
+    return like.new_empty((rows, -(-_blocks(cols) // 4) * 4), dtype=SCALE)
+
+
+def _rows_of(x: Tensor) -> int:
+    n = 1
+    for d in x.shape[:-1]:
+        n = n * d
+    return n
+
+
+@_linear.register_fake
+def _(x, weight, codes, scale, codes_t, scale_t, grad):
+    rows, (n, k) = _rows_of(x), weight.shape
+    made = codes is None
+    return (x.new_empty((*x.shape[:-1], n)), x.new_empty((rows, k), dtype=CODES), _scale_like(x, rows, k),
+            x.new_empty((k, n) if made else (0,), dtype=CODES),
+            _scale_like(x, _blocks(k), n) if made else x.new_empty(0, dtype=SCALE))
+
+
+@torch.library.custom_op("nanochat_amd::checkpointed_linear_bwd", mutates_args=("grad",), device_types="cuda")
+def _linear_bwd(dy: Tensor, x8: Tensor, xs: Tensor, codes_t: Tensor, scale_t: Tensor, grad: Tensor | None, need_x: bool,
+                need_w: bool, wide: bool) -> tuple[Tensor, Tensor]:
+    """-> dx [rows, K], dw (either empty where it is not wanted; dw also where it was added into grad)."""
+    rows = _as_rows(dy, "dy", (BF16,))
+    xs = _narrow(xs, x8.size(1))
+    with device_guard(dy):
+        dx = _product(*_quantize(rows), codes_t, scale_t) if need_x else dy.new_empty(0)
+        return dx, _layer_grad(_dense(rows) if need_w else rows, x8, xs, grad, need_w, wide)
+
+
+@_linear_bwd.register_fake
+def _(dy, x8, xs, codes_t, scale_t, grad, need_x, need_w, wide):
+    k = x8.size(1)
+    return (dy.new_empty((x8.size(0), k) if need_x else (0,)),
+            dy.new_empty((dy.size(-1), k), dtype=F32 if wide else BF16) if need_w and grad is None else dy.new_empty(0))
+
+
+def _linear_context(ctx: FunctionCtx, inputs: tuple, output: tuple) -> None:
+    x, weight, codes, _, codes_t, scale_t, grad = inputs
+    _, x8, xs, made_t, made_ts = output
+    ctx.x_shape, ctx.wide = x.shape, weight.dtype == F32
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.save_for_backward(x8, xs, *((codes_t, scale_t) if codes is not None else (made_t, made_ts)), grad)
+
+
+def _linear_backward(ctx: FunctionCtx, dy: Tensor | None, *_: Tensor | None) -> tuple:
+    if dy is None:
+        return (None,) * 7
+    x8, xs, codes_t, scale_t, grad = ctx.saved_tensors
+    need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or grad is not None
+    dx, dw = _linear_bwd(dy, x8, xs, codes_t, scale_t, grad, need_x, need_w, ctx.wide)
+    return (dx.view(ctx.x_shape) if need_x else None, dw if need_w and grad is None else None, *(None,) * 5)
+
+
+_linear.register_autograd(_linear_backward, setup_context=_linear_context)
+
+
+_NOT_HELD = (None, None, None, None)
+
+
+def checkpointed_linear(x: Tensor, weight: Tensor, weight8: Fp8Weight | None = None, grad: Tensor | None = None) -> Tensor:
+    """x bf16 [..., K] through a linear layer in 8-bit products, bf16 [..., N], differentiable in x and weight (bf16 or fp32
+    [N, K], N and K multiples of 16). Kept for the backward is x's 8-bit form alone, not x. With x8, dy8, w8 the 8-bit forms:
+
+        y = x8 w8^T      dx = dy8 w8      dw = dy^T x8   (dy itself, fp32 sums)
+
+    weight8: quantize_weight(weight, transpose=True), which a program that uses a weight more than once a step keeps; made in
+    the call when absent. grad: None (dw is returned to autograd, in the weight's type), or an fp32 [N, K] buffer that dw is
+    added to in the backward, autograd then getting none for the weight. The gradients themselves cannot be differentiated."""
+    return _linear(x, weight, *(weight8 or _NOT_HELD), grad)[0]
+
+
+@torch.library.custom_op("nanochat_amd::checkpointed_mlp", mutates_args=(), device_types="cuda")
+def _mlp(x: Tensor, fc: Tensor, proj: Tensor, fc_codes: Tensor | None, fc_scale: Tensor | None, fc_codes_t: Tensor | None,
+         fc_scale_t: Tensor | None, fc_grad: Tensor | None, proj_codes: Tensor | None, proj_scale: Tensor | None,
+         proj_codes_t: Tensor | None, proj_scale_t: Tensor | None,
+         proj_grad: Tensor | None) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """-> y, then what the backward reads: the codes and scales of x, of the hidden activations, and of both transposes."""
+    rows = _as_rows(x, "x", (BF16,))
+    f = _held(fc, "fc", fc_codes, fc_scale, fc_codes_t, fc_scale_t, fc_grad, x.device)
+    p = _held(proj, "proj", proj_codes, proj_scale, proj_codes_t, proj_scale_t, proj_grad, x.device)
+    if rows.size(1) != fc.size(1) or proj.size(1) != fc.size(0):
+        raise ValueError(f"x has {rows.size(1)} columns, fc is {tuple(fc.shape)}, proj {tuple(proj.shape)}")
+    with device_guard(x):
+        x8, xs = _quantize(rows)
+        a8, a_s = _product_relu2(x8, xs, f.codes, f.scale)
+        y = _product(a8, a_s, p.codes, p.scale)
+    return (y.view(*x.shape[:-1], y.size(1)), x8, _padded(xs), a8, _padded(a_s), *_kept(fc_codes is not None, f),
+            *_kept(proj_codes is not None, p))
+
+
+@_mlp.register_fake
+def _(x, fc, proj, fc_codes, fc_scale, fc_codes_t, fc_scale_t, fc_grad, proj_codes, proj_scale, proj_codes_t, proj_scale_t,
+      proj_grad):
+    rows, (hidden, k), n = _rows_of(x), fc.shape, proj.size(0)
+
+    def kept(made, rows_t, cols_t):
+        return (x.new_empty((rows_t, cols_t) if made else (0,), dtype=CODES),
+                _scale_like(x, _blocks(rows_t), cols_t) if made else x.new_empty(0, dtype=SCALE))
+
+    return (x.new_empty((*x.shape[:-1], n)), x.new_empty((rows, k), dtype=CODES), _scale_like(x, rows, k),
+            x.new_empty((rows, hidden), dtype=CODES), _scale_like(x, rows, hidden), *kept(fc_codes is None, k, hidden),
+            *kept(proj_codes is None, hidden, n))
+
+
+@torch.library.custom_op("nanochat_amd::checkpointed_mlp_bwd", mutates_args=("fc_grad", "proj_grad"), device_types="cuda")
+def _mlp_bwd(dy: Tensor, x8: Tensor, xs: Tensor, a8: Tensor, a_s: Tensor, fc_codes_t: Tensor, fc_scale_t: Tensor,
+             proj_codes_t: Tensor, proj_scale_t: Tensor, fc_grad: Tensor | None, proj_grad: Tensor | None, need_x: bool,
+             need_fc: bool, need_proj: bool, fc_wide: bool, proj_wide: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """-> dx [rows, C], dfc, dproj (each empty where it is not wanted, or was added into its buffer)."""
+    rows = _as_rows(dy, "dy", (BF16,))
+    xs, a_s = _narrow(xs, x8.size(1)), _narrow(a_s, a8.size(1))
+    with device_guard(dy):
+        dx, dfc = dy.new_empty(0), dy.new_empty(0)
+        if need_x or need_fc:
+            dh, dh8, dhs = _product_relu2_bwd(*_quantize(rows), proj_codes_t, proj_scale_t, a8, a_s)
+            if need_x:
+                dx = _product(dh8, dhs, fc_codes_t, fc_scale_t)
+            dfc = _layer_grad(dh, x8, xs, fc_grad, need_fc, fc_wide)
+        dproj = _layer_grad(_dense(rows) if need_proj else rows, a8, a_s, proj_grad, need_proj, proj_wide)
+    return dx, dfc, dproj
+
+
+@_mlp_bwd.register_fake
+def _(dy, x8, xs, a8, a_s, fc_codes_t, fc_scale_t, proj_codes_t, proj_scale_t, fc_grad, proj_grad, need_x, need_fc, need_proj,
+      fc_wide, proj_wide):
+    (rows, k), hidden, n = x8.shape, a8.size(1), dy.size(-1)
+    return (dy.new_empty((rows, k) if need_x else (0,)),
+            dy.new_empty((hidden, k), dtype=F32 if fc_wide else BF16) if need_fc and fc_grad is None else dy.new_empty(0),
+            dy.new_empty((n, hidden), dtype=F32 if proj_wide else BF16) if need_proj and proj_grad is None else dy.new_empty(0))
+
+
+def _mlp_context(ctx: FunctionCtx, inputs: tuple, output: tuple) -> None:
+    x, fc, proj = inputs[:3]
+    f, p = inputs[3:8], inputs[8:13]
+    _, x8, xs, a8, a_s, f_t, f_ts, p_t, p_ts = output
+    ctx.x_shape, ctx.fc_wide, ctx.proj_wide = x.shape, fc.dtype == F32, proj.dtype == F32
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.save_for_backward(x8, xs, a8, a_s, *(f[2:4] if f[0] is not None else (f_t, f_ts)),
+                          *(p[2:4] if p[0] is not None else (p_t, p_ts)), f[4], p[4])
+
+
+def _mlp_backward(ctx: FunctionCtx, dy: Tensor | None, *_: Tensor | None) -> tuple:
+    if dy is None:
+        return (None,) * 13
+    saved = ctx.saved_tensors
+    fc_grad, proj_grad = saved[8:]
+    need_x = ctx.needs_input_grad[0]
+    need_fc, need_proj = ctx.needs_input_grad[1] or fc_grad is not None, ctx.needs_input_grad[2] or proj_grad is not None
+    dx, dfc, dproj = _mlp_bwd(dy, *saved, need_x, need_fc, need_proj, ctx.fc_wide, ctx.proj_wide)
+    return (dx.view(ctx.x_shape) if need_x else None, dfc if need_fc and fc_grad is None else None,
+            dproj if need_proj and proj_grad is None else None, *(None,) * 10)
+
+
+_mlp.register_autograd(_mlp_backward, setup_context=_mlp_context)
+
+
+def checkpointed_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc8: Fp8Weight | None = None, proj8: Fp8Weight | None = None,
+                     fc_grad: Tensor | None = None, proj_grad: Tensor | None = None) -> Tensor:
+    """x bf16 [..., C] through proj(relu(fc(x))^2) in 8-bit products, bf16 [..., N], differentiable in x, fc [F, C] and proj
+    [N, F] (bf16 or fp32, all sizes multiples of 16). Kept for the backward are the 8-bit forms of x and of the squared
+    activations a, C + F bytes a token where bf16 keeps x, the sums before the square and the squares in 2 C + 4 F. With x8
+    and so on the 8-bit forms, f8 and p8 the weights':
+
+        a = relu(x8 f8^T)^2      y = a8 p8^T      dh = bf16((dy8 p8) 2 sqrt(a8))
+        dx = dh8 f8      dfc = dh^T x8      dproj = dy^T a8
+
+    The derivative of the square is read from the checkpoint itself: 2 relu(h) = 2 sqrt(a). fc8, proj8, fc_grad and proj_grad
+    as checkpointed_linear's weight8 and grad."""
+    return _mlp(x, fc, proj, *(fc8 or _NOT_HELD), fc_grad, *(proj8 or _NOT_HELD), proj_grad)[0]
