@@ -58,10 +58,6 @@ typedef FgTile<4, 2, 4> FgFull;      /* 256 x 256, 8 waves */
 typedef FgTile<2, 1, 4> FgHalf;      /* 128 x 128, 4 waves */
 typedef FgTile<1, 1, 4> FgSmall;     /* 64 x 128, 4 waves */
 
-__device__ __forceinline__ Rsrc fg_rsrc(const void *p, long long bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
-}
-
 /* A 16-byte LDS read serves lanes 0-3, 12-15, 20-23 and 24-27 together, then 4-11, 16-19 and 28-31, and so the upper half. Two
  * rows lie side by side over the 64 banks, so 8 rows of one parity, four of one 16-byte piece b and four of b ^ 2, need 8
  * places. Activation rows i: i / 2 in {0, 1, 6, 7} gives places 0 to 3 (closed under ^ 2), the others 4 to 7. Weight rows 32 q
@@ -116,58 +112,215 @@ __device__ __forceinline__ void fg_compute(const unsigned char *buf, f32x4 (&acc
     }
 }
 
+/* What a wave knows of its tile. */
+struct FgPlace {
+    int lane, wave, grp, i, wn, wm;
+    int rows, cols;              /* of the tile that exist */
+    int row0, nb;                /* the wave's first row of a (this lane's), and its block of w */
+    bool some;                   /* the wave has columns */
+};
+
+template <class P>
+__device__ __forceinline__ FgPlace fg_place(const F8Gemm &g, long long m0, int n0) {
+    FgPlace p;
+    p.lane = threadIdx.x & (WAVE - 1);
+    p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    p.grp = p.lane >> 4;
+    p.i = p.lane & 15;
+    p.wn = p.wave % P::WN;
+    p.wm = p.wave / P::WN;
+    p.rows = __builtin_amdgcn_readfirstlane((int)(g.M - m0 < P::TM ? g.M - m0 : P::TM));
+    p.cols = g.N - n0 < P::TN ? g.N - n0 : P::TN;
+    p.row0 = 16 * P::NU * p.wm + p.i;
+    p.nb = n0 / F8_BLOCK + p.wn;
+    p.some = F8_BLOCK * p.wn < p.cols;
+    return p;
+}
+
+/* The scale dwords (four blocks) of a wave's operands: of its rows of a by lane, of its block of w. */
+template <class P> struct FgScales {
+    Rsrc rs;
+    int at, step;
+    Rsrc rw;
+    uint32_t a[P::NU], w, next_a[P::NU], next_w;
+    __device__ __forceinline__ FgScales(const F8Gemm &g, const FgPlace &p, long long m0) {
+        rs = f8_rsrc(g.as + m0 * g.as_stride, p.rows * g.as_stride);
+        at = p.row0 * (int)g.as_stride;
+        step = 16 * (int)g.as_stride;
+        rw = f8_rsrc(g.ws + (long long)(p.some ? p.nb : 0) * g.ws_stride, g.ws_stride);
+    }
+    __device__ __forceinline__ void fetch(int group) {
+        next_w = __builtin_amdgcn_raw_buffer_load_b32(rw, 4 * group, 0, 0);   /* the same for all lanes */
+#pragma unroll
+        for (int u = 0; u < P::NU; u++) next_a[u] = __builtin_amdgcn_raw_buffer_load_b32(rs, at + u * step + 4 * group, 0, 0);
+    }
+    __device__ __forceinline__ void shift() {   /* the next block's byte lowest */
+        w >>= 8;
+#pragma unroll
+        for (int u = 0; u < P::NU; u++) a[u] >>= 8;
+    }
+    __device__ __forceinline__ void turn() {
+        w = next_w;
+#pragma unroll
+        for (int u = 0; u < P::NU; u++) a[u] = next_a[u];
+    }
+};
+
 /* Stage j from CUR, its successor's DMA into OTHER. */
 #define FG_STEP(j, BYTE, CUR, OTHER)                                              \
     do {                                                                           \
         if ((j) < stages) {                                                        \
             __builtin_amdgcn_s_waitcnt(0);                                         \
             fg_barrier();                                                          \
-            if ((j) + 1 < stages) fg_fetch<P>(ra, rw, OTHER, (j) + 1, g.K, wave, lane); \
-            fg_compute<P, BYTE>(CUR, acc, sa, sw, a_at, w_at);                     \
+            if ((j) + 1 < stages) fg_fetch<P>(ra, rw, OTHER, (j) + 1, g.K, p.wave, p.lane); \
+            fg_compute<P, BYTE>(CUR, acc, sc.a, sc.w, a_at, w_at);                 \
         }                                                                          \
     } while (0)
 
-template <class P, int EPI>
-__device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, unsigned char *b0, unsigned char *b1) {
-    const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x >> 6, grp = lane >> 4, i = lane & 15;
-    const int wn = wave % P::WN, wm = wave / P::WN;
+/* The K walk of the smaller tiles: two or more workgroups a CU, each with a wave a SIMD, run beside one another. */
+template <class P>
+__device__ __forceinline__ void fg_walk_simple(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0,
+                                               unsigned char *b1, f32x4 (&acc)[8][P::NU]) {
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
-    const int rows = (int)(g.M - m0 < P::TM ? g.M - m0 : P::TM), cols = g.N - n0 < P::TN ? g.N - n0 : P::TN;
-    const Rsrc ra = fg_rsrc(g.a + m0 * g.K, (long long)rows * g.K);
-    const Rsrc rw = fg_rsrc(g.w + (long long)n0 * g.K, (long long)cols * g.K);
-    const Rsrc rs = fg_rsrc(g.as + m0 * g.as_stride, rows * g.as_stride);
-    const int nb = n0 / F8_BLOCK + wn, row0 = 16 * P::NU * wm + i;
-    const bool some = F8_BLOCK * wn < cols;                   /* the wave has columns */
-    const uint32_t *ws = (const uint32_t *)(g.ws + (long long)(some ? nb : 0) * g.ws_stride);
-
-    f32x4 acc[8][P::NU];
-#pragma unroll
-    for (int t = 0; t < 8; t++)
-#pragma unroll
-        for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t sa[P::NU], na[P::NU], sw, nw = ws[0];
-#pragma unroll
-    for (int u = 0; u < P::NU; u++)
-        na[u] = __builtin_amdgcn_raw_buffer_load_b32(rs, (row0 + 16 * u) * (int)g.as_stride, 0, 0);
-    fg_fetch<P>(ra, rw, b0, 0, g.K, wave, lane);
-    const int a_at = row0 * FG_ROWB + (((2 * grp) ^ fg_swizzle_a(row0)) << 4);
-    const int w_row = F8_BLOCK * wn + 32 * (i >> 2) + (i & 3);
-    const int w_at = (P::TM + w_row) * FG_ROWB + (((2 * grp) ^ fg_swizzle_w(w_row)) << 4);
+    const Rsrc ra = f8_rsrc(g.a + m0 * g.K, (long long)p.rows * g.K);
+    const Rsrc rw = f8_rsrc(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
+    FgScales<P> sc(g, p, m0);
+    sc.fetch(0);
+    fg_fetch<P>(ra, rw, b0, 0, g.K, p.wave, p.lane);
+    const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
+    const int w_row = F8_BLOCK * p.wn + 32 * (p.i >> 2) + (p.i & 3);
+    const int w_at = (P::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
     for (int j = 0; j < stages; j += 4) {
-        sw = nw;
-#pragma unroll
-        for (int u = 0; u < P::NU; u++) sa[u] = na[u];
-        if (j + 4 < stages) {   /* the next four blocks' scales */
-            nw = ws[j / 4 + 1];
-#pragma unroll
-            for (int u = 0; u < P::NU; u++)
-                na[u] = __builtin_amdgcn_raw_buffer_load_b32(rs, (row0 + 16 * u) * (int)g.as_stride + j + 4, 0, 0);
-        }
+        sc.turn();
+        if (j + 4 < stages) sc.fetch(j / 4 + 1);
         FG_STEP(j, 0, b0, b1);
         FG_STEP(j + 1, 1, b1, b0);
         FG_STEP(j + 2, 2, b0, b1);
         FG_STEP(j + 3, 3, b1, b0);
     }
+}
+
+/* The K walk of the full tile: waves 0-3 and 4-7, one of each a SIMD, take turns: while one's 32 products keep the matrix core
+ * busy, the other reads its next 12 operands into registers. A phase ends with a barrier; waves 0-3 read stage j in phase 2 j
+ * and multiply in 2 j + 1, waves 4-7 a phase later. Waves 0-3 issue stage j + 1's DMA in phase 2 j, when every wave has read
+ * stage j - 1, and wait for it at the end of phase 2 j + 1. */
+/* The products as inline assembly: accumulators that stay in the same four AGPRs for the whole walk ("+a"), where the compiler
+ * moved them about. It does not see matrix instructions there and inserts none of their wait states; they are kept by
+ * construction. Operands are written by LDS reads alone, waited for at the phase's end; scales by memory reads and shifts before
+ * that wait; an accumulator is used again 31 products later, and read only 32 wait states after the last product. */
+__device__ __forceinline__ void fg_mfma(f32x4 &c, const i32x8 &w, const i32x8 &a, uint32_t sw, uint32_t sa) {
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+                 : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
+}
+
+/* The full tile's DMA, by waves 0-3: instruction s = 0 .. 7 of a and of w moves rows 32 s + 8 wave + lane / 8. */
+struct FgDma {
+    Rsrc ra, rw;
+    int first, ca, cw, K, wave;   /* the lane's row 0 offset, and its pieces' offsets for s = 0 */
+    __device__ __forceinline__ FgDma(const F8Gemm &g, const FgPlace &p, long long m0, int n0) {
+        ra = f8_rsrc(g.a + m0 * g.K, (long long)p.rows * g.K);
+        rw = f8_rsrc(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
+        K = g.K;
+        wave = p.wave & 3;
+        const int row = 8 * wave + (p.lane >> 3), pos = p.lane & 7;
+        first = row * K;
+        ca = (pos ^ fg_swizzle_a(row)) << 4;
+        cw = (pos ^ fg_swizzle_w(row)) << 4;
+    }
+    __device__ __forceinline__ void issue(unsigned char *buf, int j) const {
+        const int k = j * FG_ROWB;
+        int ca = this->ca, cw = this->cw;
+        asm volatile("" : "+v"(ca), "+v"(cw));   /* opaque: the 16 offsets are made here, not kept in registers */
+#pragma unroll
+        for (int s = 0; s < 16; s++) {
+            const int c = s < 8 ? ca : cw ^ (fg_swizzle_w(32 * s) << 4);   /* rows 32 s on: only bits 5 and 6 of w's change */
+            int off = first + (c + k + 32 * (s & 7) * K);
+            if (k + FG_ROWB > K) off = c + k < K ? off : FG_PAST;   /* a short last block */
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(s < 8 ? ra : rw, (LdsPtr *)(buf + (wave + 4 * s) * 1024), 16, off, 0, 0, 0);
+        }
+    }
+};
+
+__device__ __forceinline__ void fg_phase_end() {
+    __builtin_amdgcn_sched_barrier(0);
+    fg_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+}
+constexpr int FG_WAIT_LDS = 0xC07F;   /* s_waitcnt lgkmcnt(0) alone */
+constexpr int FG_WAIT_DMA = 0x0F70;   /* s_waitcnt vmcnt(0) alone */
+
+__device__ __forceinline__ void fg_walk(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *lds,
+                                        f32x4 (&acc)[8][4], FgFull *) {
+    const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
+    const bool first = p.wave < 4;
+    const FgDma dma(g, p, m0, n0);
+    FgScales<FgFull> sc(g, p, m0);
+#pragma unroll
+    for (int t = 0; t < 8; t++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) asm volatile("" : "=a"(acc[t][u]) : "0"(acc[t][u]));
+    sc.fetch(0);
+    if (first) dma.issue(lds, 0);
+    const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
+    const int w_row = F8_BLOCK * p.wn + 32 * (p.i >> 2) + (p.i & 3);
+    const int w_at = (FgFull::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
+    __builtin_amdgcn_s_waitcnt(0);
+    fg_phase_end();
+    if (!first) fg_phase_end();
+    for (int j = 0; j < stages; j++) {
+        const unsigned char *cur = lds + (j & 1) * FgFull::STAGE;
+        i32x8 fa[4], fw[8];
+#pragma unroll
+        for (int u = 0; u < 4; u++) fa[u] = fg_operand(cur, a_at + u * 16 * FG_ROWB, (a_at ^ 16) + u * 16 * FG_ROWB);
+#pragma unroll
+        for (int t = 0; t < 8; t++) fw[t] = fg_operand(cur, w_at + t * 4 * FG_ROWB, (w_at ^ 16) + t * 4 * FG_ROWB);
+        __builtin_amdgcn_sched_barrier(0);
+        if ((j & 3) == 0) {
+            sc.turn();
+            sc.fetch(j / 4 + 1);   /* past the last: zeros, or other rows', used by nothing */
+        } else {
+            sc.shift();
+        }
+        if (first && j + 1 < stages) dma.issue(lds + ((j + 1) & 1) * FgFull::STAGE, j + 1);
+        __builtin_amdgcn_s_waitcnt(FG_WAIT_LDS);
+        fg_phase_end();
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int t = 0; t < 8; t++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) fg_mfma(acc[t][u], fw[t], fa[u], sc.w, sc.a[u]);
+        __builtin_amdgcn_s_setprio(0);
+        if (first) __builtin_amdgcn_s_waitcnt(FG_WAIT_DMA);
+        fg_phase_end();
+    }
+    if (first) fg_phase_end();
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");   /* 32 wait states; no read moves above */
+#pragma unroll
+    for (int t = 0; t < 8; t++)
+#pragma unroll
+        for (int u = 0; u < 4; u++) asm volatile("" : "+a"(acc[t][u]));
+}
+template <class P>
+__device__ __forceinline__ void fg_walk(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0,
+                                        unsigned char *b1, f32x4 (&acc)[8][P::NU], P *) {
+    fg_walk_simple<P>(g, p, m0, n0, b0, b1, acc);
+}
+
+template <class P, int EPI>
+__device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, unsigned char *b0, unsigned char *b1) {
+    const FgPlace p = fg_place<P>(g, m0, n0);
+    f32x4 acc[8][P::NU];
+#pragma unroll
+    for (int t = 0; t < 8; t++)
+#pragma unroll
+        for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (P::WAVES == 8) fg_walk(g, p, m0, n0, b0, acc, (P *)nullptr);
+    else fg_walk(g, p, m0, n0, b0, b1, acc, (P *)nullptr);
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));   /* made again, not kept through the walk */
+    const int grp = (tid & (WAVE - 1)) >> 4, row0 = 16 * P::NU * p.wm + (tid & 15);
+    const int rows = p.rows, cols = p.cols, nb = p.nb, wn = p.wn;
+    const bool some = p.some;
 
     if (!some) return;
     const int c0 = F8_BLOCK * wn + 32 * grp;                  /* this lane's 32 columns from n0 */
@@ -262,8 +415,8 @@ __device__ __forceinline__ int2 fg_tile(int l, int count, int nx) {
 
 template <class P, int EPI>
 __global__ void __launch_bounds__(P::WAVES *WAVE, P::WAVES == 8 ? 2 : 2) fp8_gemm_kernel(F8Gemm g) {
-    __shared__ __align__(16) unsigned char b0[P::STAGE], b1[P::STAGE];   /* distinct objects: reads of one do not wait for
-                                                                            the other's DMA */
+    /* the smaller tiles: distinct objects, as reads of one do not wait for the other's DMA */
+    __shared__ __align__(16) unsigned char b0[P::STAGE * (P::WAVES == 8 ? 2 : 1)], b1[P::WAVES == 8 ? 16 : P::STAGE];
     const int2 t = fg_tile(blockIdx.x, gridDim.x, (g.N + P::TN - 1) / P::TN);
     fg_run<P, EPI>(g, (long long)t.y * P::TM, t.x * P::TN, b0, b1);
 }

@@ -45,10 +45,6 @@ struct F8Grad {
     void *out;                                /* PART: fp32 [slices][N1][N2]; else the result [N1][N2] */
 };
 
-__device__ __forceinline__ Rsrc gr_rsrc(const void *p, long long bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
-}
-
 /* Stage j of dy: instruction q moves rows 2 q, 2 q + 1; lane l row 2 q + l / 32, LDS piece (l % 32) / 2, half l % 2. */
 __device__ __forceinline__ void gr_fetch(Rsrc rs, unsigned char *lds, int j, int N, int c0, int wave, int lane) {
 #pragma unroll
@@ -150,10 +146,10 @@ __global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grad p) {
     const int i0 = tile / p.tiles2 * GR_T, j0 = tile % p.tiles2 * GR_T;
     const long long m0 = (long long)slice * p.rows;
     const int rows = (int)(p.M - m0 < p.rows ? p.M - m0 : p.rows);   /* > 0: the host makes no empty slice */
-    const Rsrc ra = gr_rsrc(p.dy + m0 * p.N1, (long long)rows * p.N1 * 2);
+    const Rsrc ra = f8_rsrc(p.dy + m0 * p.N1, (long long)rows * p.N1 * 2);
     XSource xsrc;
-    xsrc.codes = gr_rsrc(p.x + m0 * p.N2, (long long)rows * p.N2);
-    xsrc.scales = gr_rsrc(p.xs + m0 * p.xs_stride, rows * p.xs_stride);
+    xsrc.codes = f8_rsrc(p.x + m0 * p.N2, (long long)rows * p.N2);
+    xsrc.scales = f8_rsrc(p.xs + m0 * p.xs_stride, rows * p.xs_stride);
     const int xcol = j0 + 16 * (tid & 15);
     xsrc.at = xcol < p.N2 ? (tid >> 4) * p.N2 + xcol : GR_PAST;
     xsrc.scale_at = (tid >> 4) * (int)p.xs_stride + xcol / F8_BLOCK;
@@ -185,7 +181,7 @@ __global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grad p) {
     const int live = p.N1 - i0 < GR_T ? p.N1 - i0 : GR_T;
     const unsigned row_bytes = (unsigned)p.N2 * SIZE;
     const long long first = ((MODE == GR_PART ? (long long)slice * p.N1 : 0) + i0) * p.N2;
-    const Rsrc ro = gr_rsrc((unsigned char *)p.out + first * SIZE, (long long)live * row_bytes);
+    const Rsrc ro = f8_rsrc((unsigned char *)p.out + first * SIZE, (long long)live * row_bytes);
     unsigned at[4];
 #pragma unroll
     for (int u = 0; u < 4; u++) {

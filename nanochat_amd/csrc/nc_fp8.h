@@ -63,6 +63,16 @@ __device__ __forceinline__ uint32_t pair_top(uint32_t m) {
     return lo > hi ? lo : hi;
 }
 
+/* A buffer resource from values that are the same in every lane. A 64-bit comparison or product on the way to them leaves them in
+ * vector registers, and each access would then loop over the lanes' resources; a lane's value read back keeps them scalar. */
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t f8_rsrc(const void *p, long long bytes) {
+    const uint64_t a = (uint64_t)p;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc((void *)((uint64_t)hi << 32 | lo), (short)0,
+                                             __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+}
+
 /* Largest over lanes L ^ 1, 2, 4 (8 lanes), over L ^ 16 and L ^ 32 (the four groups of 16 lanes). */
 template <int M> __device__ __forceinline__ uint32_t lane_max_dpp(uint32_t v) {
     const uint32_t o = __float_as_uint(lane_xor_dpp<M>(__uint_as_float(v)));
