@@ -5,9 +5,9 @@
  * v_mfma_scale_f32_16x16x128_f8f6f4 takes one block a step and applies both scales itself: its A operand holds 16 weight rows,
  * its B operand 16 activation rows, lane (g = lane / 16, i = lane % 16) bytes 32 g .. + 31 of row i and that row's scale byte.
  * A wave owns 128 columns n (a block of w, so its scale is one number) and 16 NU rows m. Which weight row is which row of an
- * A operand is free: operand t's row r is row 32 (r / 4) + 4 t + r % 4 of the wave's 128, so that a lane's results, rows 4 g + e
- * of operand t = 0 .. 7, are the 32 adjacent columns 32 g + 4 t + e of row m: whole 16-byte stores, and a row's block of 128
- * meets across four lanes where the epilogue needs its largest magnitude.
+ * A operand is free: rows 4 q + e of two operands are 8 adjacent columns (of four, 16, where only codes are stored), so that a
+ * lane holds whole 16-byte pieces of a row of the result, its neighbours (lanes 16 on) the next ones, and a store instruction
+ * fills whole 64-byte sectors. A row's block of 128 meets across four lanes where the epilogue needs its largest magnitude.
  *
  * Operands go from memory to LDS by DMA in stages of 128 k (128 bytes a row), two buffers in turn: a stage's wait and one
  * barrier without a memory fence, the next stage's DMA, then this stage's products. A row keeps its 16-byte piece b at place
@@ -27,6 +27,7 @@ namespace nc {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 typedef __attribute__((address_space(3))) void LdsPtr;
@@ -35,6 +36,8 @@ constexpr int FG_ROWB = F8_BLOCK;        /* bytes of a row of a stage: one block
 constexpr int FG_PAST = 0x7FFF0000;      /* a byte offset past every operand's range */
 
 enum { FG_STORE, FG_RELU2, FG_RELU2_BWD };
+/* log2 of the adjacent columns of a lane: 16 bytes of bf16, or of codes where those are all that is stored */
+template <int EPI> constexpr int fg_width() { return EPI == FG_RELU2 ? 4 : 3; }
 
 struct F8Gemm {
     const unsigned char *a, *as;         /* [M][K] codes, [M] scale bytes at as_stride */
@@ -60,14 +63,20 @@ typedef FgTile<1, 1, 4> FgSmall;     /* 64 x 128, 4 waves */
 
 /* A 16-byte LDS read serves lanes 0-3, 12-15, 20-23 and 24-27 together, then 4-11, 16-19 and 28-31, and so the upper half. Two
  * rows lie side by side over the 64 banks, so 8 rows of one parity, four of one 16-byte piece b and four of b ^ 2, need 8
- * places. Activation rows i: i / 2 in {0, 1, 6, 7} gives places 0 to 3 (closed under ^ 2), the others 4 to 7. Weight rows 32 q
- * + 4 t + c stand for i = 4 q + c: the same by q (0, 3 or 1, 2) and c / 2, whatever t is. */
+ * places. Activation rows i: i / 2 in {0, 1, 6, 7} gives places 0 to 3 (closed under ^ 2), the others 4 to 7. A weight row that
+ * stands for i = 4 q + c has the same by q (0, 3 or 1, 2) and c / 2, whichever operand t it belongs to. */
 __device__ __forceinline__ int fg_swizzle_a(int row) {
     const int k = (row >> 1) & 7;
     return (k & 3) | (((k + 2) & 4));
 }
-__device__ __forceinline__ int fg_swizzle_w(int row) {
-    const int q = (row >> 5) & 3, u = ((q << 1) & 3) ^ ((q >> 1) * 3);   /* 0, 2, 3, 1 */
+/* The column (0 .. 127 of a wave's block) of row 4 q + e of operand t, and the same but for e of an epilogue's element. W: log2
+ * of the adjacent columns that a lane holds, 3 or 4. */
+template <int W> __host__ __device__ constexpr int fg_column(int t, int q) {
+    constexpr int run = 1 << (W - 2);   /* operands that share a run of columns */
+    return ((t / run) << (W + 2)) + (q << W) + 4 * (t % run);
+}
+template <int W> __device__ __forceinline__ int fg_swizzle_w(int row) {
+    const int q = (row >> W) & 3, u = ((q << 1) & 3) ^ ((q >> 1) * 3);   /* 0, 2, 3, 1 */
     return ((row >> 1) & 1) | (u << 1);
 }
 
@@ -77,14 +86,14 @@ __device__ __forceinline__ void fg_barrier() {
     asm volatile("" ::: "memory");
 }
 
-template <class P>
+template <class P, int W>
 __device__ __forceinline__ void fg_fetch(Rsrc ra, Rsrc rw, unsigned char *buf, int j, int K, int wave, int lane) {
     const int pos = lane & 7;
 #pragma unroll
     for (int s = 0; s < P::LOADS; s++) {
         const bool is_a = s < P::A_LOADS;
         const int q = wave + P::WAVES * s, row = 8 * q + (lane >> 3) - (is_a ? 0 : P::TM);
-        const int piece = pos ^ (is_a ? fg_swizzle_a(row) : fg_swizzle_w(row)), col = j * FG_ROWB + 16 * piece;
+        const int piece = pos ^ (is_a ? fg_swizzle_a(row) : fg_swizzle_w<W>(row)), col = j * FG_ROWB + 16 * piece;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(is_a ? ra : rw, (LdsPtr *)(buf + q * 1024), 16,
                                                  col < K ? row * K + col : FG_PAST, 0, 0, 0);
     }
@@ -96,7 +105,7 @@ __device__ __forceinline__ i32x8 fg_operand(const unsigned char *buf, int lo, in
 }
 
 /* A stage's products; BYTE: which byte of the scale dwords is its block's. */
-template <class P, int BYTE>
+template <class P, int W, int BYTE>
 __device__ __forceinline__ void fg_compute(const unsigned char *buf, f32x4 (&acc)[8][P::NU], const uint32_t (&sa)[P::NU],
                                            uint32_t sw, int a_at, int w_at) {
     i32x8 fb[P::NU];
@@ -104,7 +113,7 @@ __device__ __forceinline__ void fg_compute(const unsigned char *buf, f32x4 (&acc
     for (int u = 0; u < P::NU; u++) fb[u] = fg_operand(buf, a_at + u * 16 * FG_ROWB, (a_at ^ 16) + u * 16 * FG_ROWB);
 #pragma unroll
     for (int t = 0; t < 8; t++) {
-        const i32x8 fa = fg_operand(buf, w_at + t * 4 * FG_ROWB, (w_at ^ 16) + t * 4 * FG_ROWB);
+        const i32x8 fa = fg_operand(buf, w_at + fg_column<W>(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column<W>(t, 0) * FG_ROWB);
 #pragma unroll
         for (int u = 0; u < P::NU; u++)
             acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb[u], acc[t][u], 0, 0, BYTE, (int)sw, BYTE,
@@ -172,13 +181,13 @@ template <class P> struct FgScales {
         if ((j) < stages) {                                                        \
             __builtin_amdgcn_s_waitcnt(0);                                         \
             fg_barrier();                                                          \
-            if ((j) + 1 < stages) fg_fetch<P>(ra, rw, OTHER, (j) + 1, g.K, p.wave, p.lane); \
-            fg_compute<P, BYTE>(CUR, acc, sc.a, sc.w, a_at, w_at);                 \
+            if ((j) + 1 < stages) fg_fetch<P, W>(ra, rw, OTHER, (j) + 1, g.K, p.wave, p.lane); \
+            fg_compute<P, W, BYTE>(CUR, acc, sc.a, sc.w, a_at, w_at);                 \
         }                                                                          \
     } while (0)
 
 /* The K walk of the smaller tiles: two or more workgroups a CU, each with a wave a SIMD, run beside one another. */
-template <class P>
+template <class P, int W>
 __device__ __forceinline__ void fg_walk_simple(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0,
                                                unsigned char *b1, f32x4 (&acc)[8][P::NU]) {
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
@@ -186,10 +195,10 @@ __device__ __forceinline__ void fg_walk_simple(const F8Gemm &g, const FgPlace &p
     const Rsrc rw = f8_rsrc(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
     FgScales<P> sc(g, p, m0);
     sc.fetch(0);
-    fg_fetch<P>(ra, rw, b0, 0, g.K, p.wave, p.lane);
+    fg_fetch<P, W>(ra, rw, b0, 0, g.K, p.wave, p.lane);
     const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
-    const int w_row = F8_BLOCK * p.wn + 32 * (p.i >> 2) + (p.i & 3);
-    const int w_at = (P::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
+    const int w_row = F8_BLOCK * p.wn + fg_column<W>(0, p.i >> 2) + (p.i & 3);
+    const int w_at = (P::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w<W>(w_row)) << 4);
     for (int j = 0; j < stages; j += 4) {
         sc.turn();
         if (j + 4 < stages) sc.fetch(j / 4 + 1);
@@ -202,8 +211,8 @@ __device__ __forceinline__ void fg_walk_simple(const F8Gemm &g, const FgPlace &p
 
 /* The K walk of the full tile: waves 0-3 and 4-7, one of each a SIMD, take turns: while one's 32 products keep the matrix core
  * busy, the other reads its next 12 operands into registers. A phase ends with a barrier; waves 0-3 read stage j in phase 2 j
- * and multiply in 2 j + 1, waves 4-7 a phase later. Waves 0-3 issue stage j + 1's DMA in phase 2 j, when every wave has read
- * stage j - 1, and wait for it at the end of phase 2 j + 1. */
+ * and multiply in 2 j + 1, waves 4-7 a phase later. Stage j + 1's DMA is issued in phase 2 j, when every wave has read stage j -
+ * 1: by waves 0-3 among their reads, by waves 4-7 among their products. It has landed at the end of phase 2 j + 1. */
 /* The products as inline assembly: accumulators that stay in the same four AGPRs for the whole walk ("+a"), where the compiler
  * moved them about. It does not see matrix instructions there and inserts none of their wait states; they are kept by
  * construction. Operands are written by LDS reads alone, waited for at the phase's end; scales by memory reads and shifts before
@@ -213,33 +222,70 @@ __device__ __forceinline__ void fg_mfma(f32x4 &c, const i32x8 &w, const i32x8 &a
                  : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
 }
 
-/* The full tile's DMA, by waves 0-3: instruction s = 0 .. 7 of a and of w moves rows 32 s + 8 wave + lane / 8. */
-struct FgDma {
-    Rsrc ra, rw;
-    int first, ca, cw, K, wave;   /* the lane's row 0 offset, and its pieces' offsets for s = 0 */
-    __device__ __forceinline__ FgDma(const F8Gemm &g, const FgPlace &p, long long m0, int n0) {
-        ra = f8_rsrc(g.a + m0 * g.K, (long long)p.rows * g.K);
-        rw = f8_rsrc(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
+/* The full tile's DMA: instruction s = 0 .. 3 of a and of w moves rows 64 s + 8 wave + lane / 8; every fourth stage another
+ * brings the scale dwords of its four blocks (waves 0-3: of rows 64 wave + lane; wave 4: of the two blocks of w). Inline
+ * assembly: the compiler would have every LDS read that follows wait for it. Nothing else of the walk loads or writes LDS, and
+ * the waits are the walk's. */
+constexpr int FG_SCALES = 1280;   /* bytes of a group's scales in LDS: 256 dwords of a, then w's, behind both stage buffers */
+template <int W> struct FgDma {
+    u32x4 ra, rw, rs;
+    uint32_t lds, scales;         /* this wave's addresses in stage buffer 0 and in the first scale buffer */
+    int first, ca, cw, K;         /* the lane's row of s = 0, and its pieces */
+    int scale_at;
+    int oa, ow;                   /* a stage's offsets */
+    uint32_t to;
+    static __device__ __forceinline__ u32x4 words(const void *p, long long bytes) {
+        const uint64_t at = (uint64_t)p;
+        return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) & 0xFFFFu,
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+    }
+    __device__ __forceinline__ FgDma(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0) {
+        ra = words(g.a + m0 * g.K, (long long)p.rows * g.K);
+        rw = words(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
+        const bool of_a = p.wave < 4;
+        const int blocks = (p.cols + F8_BLOCK - 1) / F8_BLOCK;
+        rs = of_a ? words(g.as + m0 * g.as_stride, p.rows * g.as_stride)
+                  : words(g.ws + (long long)(n0 / F8_BLOCK) * g.ws_stride, (long long)blocks * g.ws_stride);
+        scale_at = of_a ? (64 * p.wave + p.lane) * (int)g.as_stride : p.lane < blocks ? p.lane * g.ws_stride : FG_PAST;
+        lds = (uint32_t)reinterpret_cast<uintptr_t>((LdsPtr *)b0) + p.wave * 1024;
+        scales = (uint32_t)reinterpret_cast<uintptr_t>((LdsPtr *)b0) + 2 * FgFull::STAGE + p.wave * 256;
         K = g.K;
-        wave = p.wave & 3;
-        const int row = 8 * wave + (p.lane >> 3), pos = p.lane & 7;
+        const int row = 8 * p.wave + (p.lane >> 3), pos = p.lane & 7;
         first = row * K;
         ca = (pos ^ fg_swizzle_a(row)) << 4;
-        cw = (pos ^ fg_swizzle_w(row)) << 4;
+        cw = (pos ^ fg_swizzle_w<W>(row)) << 4;   /* rows 64 on have the same */
     }
-    __device__ __forceinline__ void issue(unsigned char *buf, int j) const {
+    static __device__ __forceinline__ void load(uint32_t to, int off, const u32x4 &r) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(to), "v"(off), "s"(r)
+                     : "memory");
+    }
+    /* Stage j's offsets, and its scales' DMA where it is the first of four. */
+    __device__ __forceinline__ void stage(int j, int wave) {
         const int k = j * FG_ROWB;
-        int ca = this->ca, cw = this->cw;
-        asm volatile("" : "+v"(ca), "+v"(cw));   /* opaque: the 16 offsets are made here, not kept in registers */
-#pragma unroll
-        for (int s = 0; s < 16; s++) {
-            const int c = s < 8 ? ca : cw ^ (fg_swizzle_w(32 * s) << 4);   /* rows 32 s on: only bits 5 and 6 of w's change */
-            int off = first + (c + k + 32 * (s & 7) * K);
-            if (k + FG_ROWB > K) off = c + k < K ? off : FG_PAST;   /* a short last block */
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(s < 8 ? ra : rw, (LdsPtr *)(buf + (wave + 4 * s) * 1024), 16, off, 0, 0, 0);
+        oa = first + ca + k;
+        ow = first + cw + k;
+        if (k + FG_ROWB > K) {   /* a short last block: pieces past it lie past the range, also with 192 K added */
+            oa = ca + k < K ? oa : FG_PAST;
+            ow = cw + k < K ? ow : FG_PAST;
         }
+        to = lds + (j & 1) * FgFull::STAGE;
+        if ((j & 3) == 0 && wave <= 4)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                         :: "s"(scales + ((j >> 2) & 1) * FG_SCALES), "v"(scale_at + j), "s"(rs) : "memory");
+    }
+    template <int S> __device__ __forceinline__ void issue() const {   /* S: 0 .. 3 a, 4 .. 7 w */
+        load(to + S * 8192, (S < 4 ? oa : ow) + 64 * (S & 3) * K, S < 4 ? ra : rw);
     }
 };
+
+template <int I> struct FgIndex { static constexpr int value = I; };
+template <int N, int I = 0, class F> __device__ __forceinline__ void fg_unroll(F &&f) {
+    if constexpr (I < N) {
+        f(FgIndex<I>{});
+        fg_unroll<N, I + 1>(f);
+    }
+}
 
 __device__ __forceinline__ void fg_phase_end() {
     __builtin_amdgcn_sched_barrier(0);
@@ -249,46 +295,62 @@ __device__ __forceinline__ void fg_phase_end() {
 constexpr int FG_WAIT_LDS = 0xC07F;   /* s_waitcnt lgkmcnt(0) alone */
 constexpr int FG_WAIT_DMA = 0x0F70;   /* s_waitcnt vmcnt(0) alone */
 
-__device__ __forceinline__ void fg_walk(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *lds,
-                                        f32x4 (&acc)[8][4], FgFull *) {
+template <int W>
+__device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *lds,
+                                             f32x4 (&acc)[8][4]) {
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
     const bool first = p.wave < 4;
-    const FgDma dma(g, p, m0, n0);
-    FgScales<FgFull> sc(g, p, m0);
+    FgDma<W> dma(g, p, m0, n0, lds);
 #pragma unroll
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int u = 0; u < 4; u++) asm volatile("" : "=a"(acc[t][u]) : "0"(acc[t][u]));
-    sc.fetch(0);
-    if (first) dma.issue(lds, 0);
+    dma.stage(0, p.wave);
+    fg_unroll<8>([&](auto s) { dma.template issue<decltype(s)::value>(); });
     const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
-    const int w_row = F8_BLOCK * p.wn + 32 * (p.i >> 2) + (p.i & 3);
-    const int w_at = (FgFull::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
+    const int w_row = F8_BLOCK * p.wn + fg_column<W>(0, p.i >> 2) + (p.i & 3);
+    const int w_at = (FgFull::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w<W>(w_row)) << 4);
+    const unsigned char *scales = lds + 2 * FgFull::STAGE;
     __builtin_amdgcn_s_waitcnt(0);
     fg_phase_end();
-    if (!first) fg_phase_end();
-    for (int j = 0; j < stages; j++) {
-        const unsigned char *cur = lds + (j & 1) * FgFull::STAGE;
-        i32x8 fa[4], fw[8];
-#pragma unroll
-        for (int u = 0; u < 4; u++) fa[u] = fg_operand(cur, a_at + u * 16 * FG_ROWB, (a_at ^ 16) + u * 16 * FG_ROWB);
-#pragma unroll
-        for (int t = 0; t < 8; t++) fw[t] = fg_operand(cur, w_at + t * 4 * FG_ROWB, (w_at ^ 16) + t * 4 * FG_ROWB);
-        __builtin_amdgcn_sched_barrier(0);
-        if ((j & 3) == 0) {
-            sc.turn();
-            sc.fetch(j / 4 + 1);   /* past the last: zeros, or other rows', used by nothing */
-        } else {
-            sc.shift();
+    if (!first) {   /* phase 0 */
+        if (1 < stages) {
+            dma.stage(1, p.wave);
+            fg_unroll<8>([&](auto s) { dma.template issue<decltype(s)::value>(); });
         }
-        if (first && j + 1 < stages) dma.issue(lds + ((j + 1) & 1) * FgFull::STAGE, j + 1);
-        __builtin_amdgcn_s_waitcnt(FG_WAIT_LDS);
         fg_phase_end();
-        __builtin_amdgcn_s_setprio(1);
+    }
+    for (int j = 0; j < stages; j++) {
+        const unsigned char *cur = lds + (j & 1) * FgFull::STAGE, *sc = scales + ((j >> 2) & 1) * FG_SCALES + (j & 3);
+        i32x8 fa[4], fw[8];
+        uint32_t sa[4], sw;
+        const bool mine = first && j + 1 < stages, next = !first && j + 2 < stages;
+        if (mine) {
+            dma.stage(j + 1, p.wave);
+            fg_unroll<8>([&](auto s) { dma.template issue<decltype(s)::value>(); });
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            sa[u] = sc[(p.row0 + 16 * u) * 4];
+            fa[u] = fg_operand(cur, a_at + u * 16 * FG_ROWB, (a_at ^ 16) + u * 16 * FG_ROWB);
+        }
+        sw = sc[1024 + 4 * p.wn];
 #pragma unroll
         for (int t = 0; t < 8; t++)
+            fw[t] = fg_operand(cur, w_at + fg_column<W>(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column<W>(t, 0) * FG_ROWB);
+        __builtin_amdgcn_s_waitcnt(FG_WAIT_LDS);
+        if (!first) __builtin_amdgcn_s_waitcnt(FG_WAIT_DMA);
+        fg_phase_end();
+        __builtin_amdgcn_s_setprio(1);
+        if (next) dma.stage(j + 2, p.wave);
+        fg_unroll<8>([&](auto t) {
+            constexpr int T = decltype(t)::value;
 #pragma unroll
-            for (int u = 0; u < 4; u++) fg_mfma(acc[t][u], fw[t], fa[u], sc.w, sc.a[u]);
+            for (int u = 0; u < 4; u++) {
+                fg_mfma(acc[T][u], fw[T], fa[u], sw, sa[u]);
+                if (u == 1 && next) dma.template issue<T>();
+            }
+        });
         __builtin_amdgcn_s_setprio(0);
         if (first) __builtin_amdgcn_s_waitcnt(FG_WAIT_DMA);
         fg_phase_end();
@@ -300,11 +362,6 @@ __device__ __forceinline__ void fg_walk(const F8Gemm &g, const FgPlace &p, long 
 #pragma unroll
         for (int u = 0; u < 4; u++) asm volatile("" : "+a"(acc[t][u]));
 }
-template <class P>
-__device__ __forceinline__ void fg_walk(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0,
-                                        unsigned char *b1, f32x4 (&acc)[8][P::NU], P *) {
-    fg_walk_simple<P>(g, p, m0, n0, b0, b1, acc);
-}
 
 template <class P, int EPI>
 __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, unsigned char *b0, unsigned char *b1) {
@@ -314,8 +371,9 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (P::WAVES == 8) fg_walk(g, p, m0, n0, b0, acc, (P *)nullptr);
-    else fg_walk(g, p, m0, n0, b0, b1, acc, (P *)nullptr);
+    constexpr int W = fg_width<EPI>();
+    if constexpr (P::WAVES == 8) fg_walk_full<W>(g, p, m0, n0, b0, acc);
+    else fg_walk_simple<P, W>(g, p, m0, n0, b0, b1, acc);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));   /* made again, not kept through the walk */
     const int grp = (tid & (WAVE - 1)) >> 4, row0 = 16 * P::NU * p.wm + (tid & 15);
@@ -323,7 +381,9 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
     const bool some = p.some;
 
     if (!some) return;
-    const int c0 = F8_BLOCK * wn + 32 * grp;                  /* this lane's 32 columns from n0 */
+    /* this lane's columns from n0: RUNS runs of 2^W, RUN elements of v each */
+    constexpr int RUN = 1 << W, RUNS = 32 / RUN, STEP = 4 * RUN;
+    const int c0 = F8_BLOCK * wn + RUN * grp;
 #pragma unroll
     for (int u = 0; u < P::NU; u++) {
         const int r = row0 + 16 * u;
@@ -334,7 +394,7 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
         for (int t = 0; t < 8; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) v[4 * t + e] = acc[t][u][e];
-        if (EPI == FG_RELU2) {
+        if constexpr (EPI == FG_RELU2) {
             uint32_t m = 0u;
 #pragma unroll
             for (int k = 0; k < 32; k++) {
@@ -346,61 +406,58 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
             const uint32_t byte = f8_scale_byte(group_max(m));
             const float s = f8_scale(byte);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < RUNS; h++) {
                 u32x4 c;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const int z = 16 * h + 4 * k;
+                    const int z = RUN * h + 4 * k;
                     c[k] = byte == F8_NAN_BYTE ? F8_NAN_CODES : f8_codes(v[z], v[z + 1], v[z + 2], v[z + 3], s);
                 }
-                if (in && c0 + 16 * h < cols) *(u32x4 *)(g.q + at + 16 * h) = c;
+                if (in && c0 + STEP * h < cols) *(u32x4 *)(g.q + at + STEP * h) = c;
             }
             if (in && grp == 0) g.qs[(m0 + r) * g.qs_stride + nb] = (unsigned char)byte;
-            continue;
-        }
-        uint32_t o[16];
-        if (EPI == FG_RELU2_BWD) {
-            /* dh = da 2 sqrt(a); a's codes are this lane's 32 columns, its scale the block's */
-            u32x4 c[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
-            uint32_t byte = 127u;
-            if (in) {
-                byte = g.acts[(m0 + r) * g.act_stride + nb];
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (c0 + 16 * h < cols) c[h] = *(const u32x4 *)(g.act + at + 16 * h);
-            }
-            const float s = f8_scale(byte);
-            uint32_t m = 0u;
-#pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const uint32_t w = c[k >> 3][(k >> 1) & 3];
-                const auto a = (k & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true)
-                                       : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false);
-                /* v_sqrt_f32 is within an ulp; the result is rounded to bf16 right away */
-                const float x = v[2 * k] * (2.0f * __builtin_amdgcn_sqrtf(a[0]));
-                const float y = v[2 * k + 1] * (2.0f * __builtin_amdgcn_sqrtf(a[1]));
-                o[k] = bf16_pair(x, y);
-                m = pair_amax(m, o[k]);
-            }
-            const uint32_t qb = f8_scale_byte(group_max(pair_top(m)));
-            const float qs = f8_scale(qb);
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                u32x4 q;
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    q[k] = qb == F8_NAN_BYTE ? F8_NAN_CODES : f8_codes(o[8 * h + 2 * k], o[8 * h + 2 * k + 1], qs);
-                if (in && c0 + 16 * h < cols) *(u32x4 *)(g.q + at + 16 * h) = q;
-            }
-            if (in && grp == 0) g.qs[(m0 + r) * g.qs_stride + nb] = (unsigned char)qb;
         } else {
+            uint32_t o[16];
+            if constexpr (EPI == FG_RELU2_BWD) {
+                /* dh = da 2 sqrt(a); a's codes are at this lane's columns, its scale the block's */
+                u32x2 c[RUNS];
+                uint32_t byte = 127u;
+                if (in) byte = g.acts[(m0 + r) * g.act_stride + nb];
 #pragma unroll
-            for (int k = 0; k < 16; k++) o[k] = bf16_pair(v[2 * k], v[2 * k + 1]);
+                for (int h = 0; h < RUNS; h++)
+                    c[h] = in && c0 + STEP * h < cols ? *(const u32x2 *)(g.act + at + STEP * h) : u32x2{0u, 0u};
+                const float s = f8_scale(byte);
+                uint32_t m = 0u;
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const uint32_t w = c[k >> 2][(k >> 1) & 1];
+                    const auto a = (k & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false);
+                    /* v_sqrt_f32 is within an ulp; the result is rounded to bf16 right away */
+                    const float x = v[2 * k] * (2.0f * __builtin_amdgcn_sqrtf(a[0]));
+                    const float y = v[2 * k + 1] * (2.0f * __builtin_amdgcn_sqrtf(a[1]));
+                    o[k] = bf16_pair(x, y);
+                    m = pair_amax(m, o[k]);
+                }
+                const uint32_t qb = f8_scale_byte(group_max(pair_top(m)));
+                const float qs = f8_scale(qb);
+#pragma unroll
+                for (int h = 0; h < RUNS; h++) {
+                    const u32x2 q = qb == F8_NAN_BYTE ? u32x2{F8_NAN_CODES, F8_NAN_CODES}
+                                                      : u32x2{f8_codes(o[4 * h], o[4 * h + 1], qs),
+                                                              f8_codes(o[4 * h + 2], o[4 * h + 3], qs)};
+                    if (in && c0 + STEP * h < cols) *(u32x2 *)(g.q + at + STEP * h) = q;
+                }
+                if (in && grp == 0) g.qs[(m0 + r) * g.qs_stride + nb] = (unsigned char)qb;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; k++) o[k] = bf16_pair(v[2 * k], v[2 * k + 1]);
+            }
+#pragma unroll
+            for (int h = 0; h < RUNS; h++)
+                if (in && c0 + STEP * h < cols)
+                    *(u32x4 *)(g.out + at + STEP * h) = u32x4{o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]};
         }
-#pragma unroll
-        for (int h = 0; h < 4; h++)
-            if (in && c0 + 8 * h < cols)
-                *(u32x4 *)(g.out + at + 8 * h) = u32x4{o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]};
     }
 }
 
@@ -416,7 +473,7 @@ __device__ __forceinline__ int2 fg_tile(int l, int count, int nx) {
 template <class P, int EPI>
 __global__ void __launch_bounds__(P::WAVES *WAVE, P::WAVES == 8 ? 2 : 2) fp8_gemm_kernel(F8Gemm g) {
     /* the smaller tiles: distinct objects, as reads of one do not wait for the other's DMA */
-    __shared__ __align__(16) unsigned char b0[P::STAGE * (P::WAVES == 8 ? 2 : 1)], b1[P::WAVES == 8 ? 16 : P::STAGE];
+    __shared__ __align__(16) unsigned char b0[P::WAVES == 8 ? 2 * P::STAGE + 2 * FG_SCALES : P::STAGE], b1[P::WAVES == 8 ? 16 : P::STAGE];
     const int2 t = fg_tile(blockIdx.x, gridDim.x, (g.N + P::TN - 1) / P::TN);
     fg_run<P, EPI>(g, (long long)t.y * P::TM, t.x * P::TN, b0, b1);
 }
