@@ -5,9 +5,9 @@
  * v_mfma_scale_f32_16x16x128_f8f6f4 takes one block a step and applies both scales itself: its A operand holds 16 weight rows,
  * its B operand 16 activation rows, lane (g = lane / 16, i = lane % 16) bytes 32 g .. + 31 of row i and that row's scale byte.
  * A wave owns 128 columns n (a block of w, so its scale is one number) and 16 NU rows m. Which weight row is which row of an
- * A operand is free: rows 4 q + e of two operands are 8 adjacent columns (of four, 16, where only codes are stored), so that a
- * lane holds whole 16-byte pieces of a row of the result, its neighbours (lanes 16 on) the next ones, and a store instruction
- * fills whole 64-byte sectors. A row's block of 128 meets across four lanes where the epilogue needs its largest magnitude.
+ * A operand is free: rows 4 q + e of two operands are 8 adjacent columns, so that a lane holds whole 16-byte pieces of a row of
+ * the result, and a row's block of 128 meets across four lanes where the epilogue needs its largest magnitude. The results go
+ * through LDS once more, so that a store instruction writes four whole rows of 256 bytes.
  *
  * Operands go from memory to LDS by DMA in stages of 128 k (128 bytes a row), two buffers in turn: a stage's wait and one
  * barrier without a memory fence, the next stage's DMA, then this stage's products. A row keeps its 16-byte piece b at place
@@ -36,8 +36,6 @@ constexpr int FG_ROWB = F8_BLOCK;        /* bytes of a row of a stage: one block
 constexpr int FG_PAST = 0x7FFF0000;      /* a byte offset past every operand's range */
 
 enum { FG_STORE, FG_RELU2, FG_RELU2_BWD };
-/* log2 of the adjacent columns of a lane: 16 bytes of bf16, or of codes where those are all that is stored */
-template <int EPI> constexpr int fg_width() { return EPI == FG_RELU2 ? 4 : 3; }
 
 struct F8Gemm {
     const unsigned char *a, *as;         /* [M][K] codes, [M] scale bytes at as_stride */
@@ -69,14 +67,10 @@ __device__ __forceinline__ int fg_swizzle_a(int row) {
     const int k = (row >> 1) & 7;
     return (k & 3) | (((k + 2) & 4));
 }
-/* The column (0 .. 127 of a wave's block) of row 4 q + e of operand t, and the same but for e of an epilogue's element. W: log2
- * of the adjacent columns that a lane holds, 3 or 4. */
-template <int W> __host__ __device__ constexpr int fg_column(int t, int q) {
-    constexpr int run = 1 << (W - 2);   /* operands that share a run of columns */
-    return ((t / run) << (W + 2)) + (q << W) + 4 * (t % run);
-}
-template <int W> __device__ __forceinline__ int fg_swizzle_w(int row) {
-    const int q = (row >> W) & 3, u = ((q << 1) & 3) ^ ((q >> 1) * 3);   /* 0, 2, 3, 1 */
+/* The column (0 .. 127 of a wave's block) of row 4 q of operand t, rows on being columns on. */
+__host__ __device__ constexpr int fg_column(int t, int q) { return 32 * (t / 2) + 8 * q + 4 * (t % 2); }
+__device__ __forceinline__ int fg_swizzle_w(int row) {
+    const int q = (row >> 3) & 3, u = ((q << 1) & 3) ^ ((q >> 1) * 3);   /* 0, 2, 3, 1 */
     return ((row >> 1) & 1) | (u << 1);
 }
 
@@ -86,14 +80,14 @@ __device__ __forceinline__ void fg_barrier() {
     asm volatile("" ::: "memory");
 }
 
-template <class P, int W>
+template <class P>
 __device__ __forceinline__ void fg_fetch(Rsrc ra, Rsrc rw, unsigned char *buf, int j, int K, int wave, int lane) {
     const int pos = lane & 7;
 #pragma unroll
     for (int s = 0; s < P::LOADS; s++) {
         const bool is_a = s < P::A_LOADS;
         const int q = wave + P::WAVES * s, row = 8 * q + (lane >> 3) - (is_a ? 0 : P::TM);
-        const int piece = pos ^ (is_a ? fg_swizzle_a(row) : fg_swizzle_w<W>(row)), col = j * FG_ROWB + 16 * piece;
+        const int piece = pos ^ (is_a ? fg_swizzle_a(row) : fg_swizzle_w(row)), col = j * FG_ROWB + 16 * piece;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(is_a ? ra : rw, (LdsPtr *)(buf + q * 1024), 16,
                                                  col < K ? row * K + col : FG_PAST, 0, 0, 0);
     }
@@ -105,7 +99,7 @@ __device__ __forceinline__ i32x8 fg_operand(const unsigned char *buf, int lo, in
 }
 
 /* A stage's products; BYTE: which byte of the scale dwords is its block's. */
-template <class P, int W, int BYTE>
+template <class P, int BYTE>
 __device__ __forceinline__ void fg_compute(const unsigned char *buf, f32x4 (&acc)[8][P::NU], const uint32_t (&sa)[P::NU],
                                            uint32_t sw, int a_at, int w_at) {
     i32x8 fb[P::NU];
@@ -113,7 +107,7 @@ __device__ __forceinline__ void fg_compute(const unsigned char *buf, f32x4 (&acc
     for (int u = 0; u < P::NU; u++) fb[u] = fg_operand(buf, a_at + u * 16 * FG_ROWB, (a_at ^ 16) + u * 16 * FG_ROWB);
 #pragma unroll
     for (int t = 0; t < 8; t++) {
-        const i32x8 fa = fg_operand(buf, w_at + fg_column<W>(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column<W>(t, 0) * FG_ROWB);
+        const i32x8 fa = fg_operand(buf, w_at + fg_column(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column(t, 0) * FG_ROWB);
 #pragma unroll
         for (int u = 0; u < P::NU; u++)
             acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb[u], acc[t][u], 0, 0, BYTE, (int)sw, BYTE,
@@ -181,13 +175,13 @@ template <class P> struct FgScales {
         if ((j) < stages) {                                                        \
             __builtin_amdgcn_s_waitcnt(0);                                         \
             fg_barrier();                                                          \
-            if ((j) + 1 < stages) fg_fetch<P, W>(ra, rw, OTHER, (j) + 1, g.K, p.wave, p.lane); \
-            fg_compute<P, W, BYTE>(CUR, acc, sc.a, sc.w, a_at, w_at);                 \
+            if ((j) + 1 < stages) fg_fetch<P>(ra, rw, OTHER, (j) + 1, g.K, p.wave, p.lane); \
+            fg_compute<P, BYTE>(CUR, acc, sc.a, sc.w, a_at, w_at);                 \
         }                                                                          \
     } while (0)
 
 /* The K walk of the smaller tiles: two or more workgroups a CU, each with a wave a SIMD, run beside one another. */
-template <class P, int W>
+template <class P>
 __device__ __forceinline__ void fg_walk_simple(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0,
                                                unsigned char *b1, f32x4 (&acc)[8][P::NU]) {
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
@@ -195,10 +189,10 @@ __device__ __forceinline__ void fg_walk_simple(const F8Gemm &g, const FgPlace &p
     const Rsrc rw = f8_rsrc(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
     FgScales<P> sc(g, p, m0);
     sc.fetch(0);
-    fg_fetch<P, W>(ra, rw, b0, 0, g.K, p.wave, p.lane);
+    fg_fetch<P>(ra, rw, b0, 0, g.K, p.wave, p.lane);
     const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
-    const int w_row = F8_BLOCK * p.wn + fg_column<W>(0, p.i >> 2) + (p.i & 3);
-    const int w_at = (P::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w<W>(w_row)) << 4);
+    const int w_row = F8_BLOCK * p.wn + fg_column(0, p.i >> 2) + (p.i & 3);
+    const int w_at = (P::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
     for (int j = 0; j < stages; j += 4) {
         sc.turn();
         if (j + 4 < stages) sc.fetch(j / 4 + 1);
@@ -207,6 +201,8 @@ __device__ __forceinline__ void fg_walk_simple(const F8Gemm &g, const FgPlace &p
         FG_STEP(j + 2, 2, b0, b1);
         FG_STEP(j + 3, 3, b1, b0);
     }
+    __builtin_amdgcn_s_waitcnt(0);
+    fg_barrier();   /* the epilogue writes where other waves may still read */
 }
 
 /* The K walk of the full tile: waves 0-3 and 4-7, one of each a SIMD, take turns: while one's 32 products keep the matrix core
@@ -227,7 +223,7 @@ __device__ __forceinline__ void fg_mfma(f32x4 &c, const i32x8 &w, const i32x8 &a
  * assembly: the compiler would have every LDS read that follows wait for it. Nothing else of the walk loads or writes LDS, and
  * the waits are the walk's. */
 constexpr int FG_SCALES = 1280;   /* bytes of a group's scales in LDS: 256 dwords of a, then w's, behind both stage buffers */
-template <int W> struct FgDma {
+struct FgDma {
     u32x4 ra, rw, rs;
     uint32_t lds, scales;         /* this wave's addresses in stage buffer 0 and in the first scale buffer */
     int first, ca, cw, K;         /* the lane's row of s = 0, and its pieces */
@@ -254,7 +250,7 @@ template <int W> struct FgDma {
         const int row = 8 * p.wave + (p.lane >> 3), pos = p.lane & 7;
         first = row * K;
         ca = (pos ^ fg_swizzle_a(row)) << 4;
-        cw = (pos ^ fg_swizzle_w<W>(row)) << 4;   /* rows 64 on have the same */
+        cw = (pos ^ fg_swizzle_w(row)) << 4;   /* rows 64 on have the same */
     }
     static __device__ __forceinline__ void load(uint32_t to, int off, const u32x4 &r) {
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(to), "v"(off), "s"(r)
@@ -295,28 +291,27 @@ __device__ __forceinline__ void fg_phase_end() {
 constexpr int FG_WAIT_LDS = 0xC07F;   /* s_waitcnt lgkmcnt(0) alone */
 constexpr int FG_WAIT_DMA = 0x0F70;   /* s_waitcnt vmcnt(0) alone */
 
-template <int W>
 __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *lds,
                                              f32x4 (&acc)[8][4]) {
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
     const bool first = p.wave < 4;
-    FgDma<W> dma(g, p, m0, n0, lds);
+    FgDma dma(g, p, m0, n0, lds);
 #pragma unroll
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int u = 0; u < 4; u++) asm volatile("" : "=a"(acc[t][u]) : "0"(acc[t][u]));
     dma.stage(0, p.wave);
-    fg_unroll<8>([&](auto s) { dma.template issue<decltype(s)::value>(); });
+    fg_unroll<8>([&](auto s) { dma.issue<decltype(s)::value>(); });
     const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
-    const int w_row = F8_BLOCK * p.wn + fg_column<W>(0, p.i >> 2) + (p.i & 3);
-    const int w_at = (FgFull::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w<W>(w_row)) << 4);
+    const int w_row = F8_BLOCK * p.wn + fg_column(0, p.i >> 2) + (p.i & 3);
+    const int w_at = (FgFull::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
     const unsigned char *scales = lds + 2 * FgFull::STAGE;
     __builtin_amdgcn_s_waitcnt(0);
     fg_phase_end();
     if (!first) {   /* phase 0 */
         if (1 < stages) {
             dma.stage(1, p.wave);
-            fg_unroll<8>([&](auto s) { dma.template issue<decltype(s)::value>(); });
+            fg_unroll<8>([&](auto s) { dma.issue<decltype(s)::value>(); });
         }
         fg_phase_end();
     }
@@ -327,7 +322,7 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
         const bool mine = first && j + 1 < stages, next = !first && j + 2 < stages;
         if (mine) {
             dma.stage(j + 1, p.wave);
-            fg_unroll<8>([&](auto s) { dma.template issue<decltype(s)::value>(); });
+            fg_unroll<8>([&](auto s) { dma.issue<decltype(s)::value>(); });
         }
 #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -337,7 +332,7 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
         sw = sc[1024 + 4 * p.wn];
 #pragma unroll
         for (int t = 0; t < 8; t++)
-            fw[t] = fg_operand(cur, w_at + fg_column<W>(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column<W>(t, 0) * FG_ROWB);
+            fw[t] = fg_operand(cur, w_at + fg_column(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column(t, 0) * FG_ROWB);
         __builtin_amdgcn_s_waitcnt(FG_WAIT_LDS);
         if (!first) __builtin_amdgcn_s_waitcnt(FG_WAIT_DMA);
         fg_phase_end();
@@ -345,11 +340,13 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
         if (next) dma.stage(j + 2, p.wave);
         fg_unroll<8>([&](auto t) {
             constexpr int T = decltype(t)::value;
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                fg_mfma(acc[T][u], fw[T], fa[u], sw, sa[u]);
-                if (u == 1 && next) dma.template issue<T>();
-            }
+            fg_unroll<4>([&](auto u) {
+                constexpr int U = decltype(u)::value;
+                fg_mfma(acc[T][U], fw[T], fa[U], sw, sa[U]);
+                if constexpr (U == 1) {   /* spread: in bursts they held up the products behind them */
+                    if (next) dma.issue<T>();
+                }
+            });
         });
         __builtin_amdgcn_s_setprio(0);
         if (first) __builtin_amdgcn_s_waitcnt(FG_WAIT_DMA);
@@ -363,6 +360,18 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
         for (int u = 0; u < 4; u++) asm volatile("" : "+a"(acc[t][u]));
 }
 
+/* A wave's part of LDS behind its walk: 16 rows of 256 bytes, then 16 of 128. */
+constexpr int FG_TURN = 16 * 384;
+#ifndef FG_CODE_STORE
+#define FG_CODE_STORE(d, p) __builtin_nontemporal_store(d, p)
+#endif
+__device__ __forceinline__ int fg_code_place(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+/* Lanes of one wave exchange values through LDS, which serves a wave's accesses in order; the compiler keeps the order too. */
+__device__ __forceinline__ void fg_wave_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
 template <class P, int EPI>
 __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, unsigned char *b0, unsigned char *b1) {
     const FgPlace p = fg_place<P>(g, m0, n0);
@@ -371,92 +380,126 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int W = fg_width<EPI>();
-    if constexpr (P::WAVES == 8) fg_walk_full<W>(g, p, m0, n0, b0, acc);
-    else fg_walk_simple<P, W>(g, p, m0, n0, b0, b1, acc);
+    if constexpr (P::WAVES == 8) fg_walk_full(g, p, m0, n0, b0, acc);
+    else fg_walk_simple<P>(g, p, m0, n0, b0, b1, acc);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));   /* made again, not kept through the walk */
-    const int grp = (tid & (WAVE - 1)) >> 4, row0 = 16 * P::NU * p.wm + (tid & 15);
+    const int grp = (tid & (WAVE - 1)) >> 4;
     const int rows = p.rows, cols = p.cols, nb = p.nb, wn = p.wn;
     const bool some = p.some;
 
     if (!some) return;
-    /* this lane's columns from n0: RUNS runs of 2^W, RUN elements of v each */
-    constexpr int RUN = 1 << W, RUNS = 32 / RUN, STEP = 4 * RUN;
-    const int c0 = F8_BLOCK * wn + RUN * grp;
+    const int lane = tid & (WAVE - 1), rows_left = rows - 16 * P::NU * p.wm, col = F8_BLOCK * wn;   /* this wave's */
+    const long long first = m0 + 16 * P::NU * p.wm;
+    unsigned char *mine = b0 + (threadIdx.x >> 6) * FG_TURN;
+    const int r16 = lane & 15;
+    u32x4 act[2], next_act[2];
+    uint32_t act_byte = 127u;
+    /* RELU2_BWD: 16 rows' codes of a, a piece of 16 columns a lane: rows 8 k + lane / 8 */
+    const auto fetch_act = [&](int u) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int r = 16 * u + 8 * k + (lane >> 3), c = col + 16 * (lane & 7);
+            next_act[k] = r < rows_left && c < cols ? *(const u32x4 *)(g.act + (first + r) * g.N + n0 + c) : u32x4{0, 0, 0, 0};
+        }
+    };
+    if constexpr (EPI == FG_RELU2_BWD) fetch_act(0);
 #pragma unroll
     for (int u = 0; u < P::NU; u++) {
-        const int r = row0 + 16 * u;
-        const bool in = r < rows;
-        const long long at = (m0 + r) * g.N + n0 + c0;
+        const int row = 16 * u + r16;                         /* this lane's results: columns 32 h + 8 grp + 0 .. 7 */
         float v[32];
 #pragma unroll
         for (int t = 0; t < 8; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) v[4 * t + e] = acc[t][u][e];
+        u32x2 q[4];
         if constexpr (EPI == FG_RELU2) {
             uint32_t m = 0u;
 #pragma unroll
             for (int k = 0; k < 32; k++) {
-                const float p = v[k] < 0.0f ? 0.0f : v[k];    /* a NaN stays one */
-                v[k] = p * p;
-                const uint32_t b = __float_as_uint(v[k]) & 0x7FFFFFFFu;
+                const float x = __builtin_elementwise_maximum(v[k], 0.0f);   /* a NaN stays one */
+                v[k] = x * x;
+                const uint32_t b = __float_as_uint(v[k]);                     /* no sign but a NaN's, which is above all */
                 m = m > b ? m : b;
             }
             const uint32_t byte = f8_scale_byte(group_max(m));
             const float s = f8_scale(byte);
 #pragma unroll
-            for (int h = 0; h < RUNS; h++) {
-                u32x4 c;
+            for (int h = 0; h < 4; h++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int z = RUN * h + 4 * k;
-                    c[k] = byte == F8_NAN_BYTE ? F8_NAN_CODES : f8_codes(v[z], v[z + 1], v[z + 2], v[z + 3], s);
+                for (int k = 0; k < 2; k++) {
+                    const int z = 8 * h + 4 * k;
+                    q[h][k] = byte == F8_NAN_BYTE ? F8_NAN_CODES : f8_codes(v[z], v[z + 1], v[z + 2], v[z + 3], s);
                 }
-                if (in && c0 + STEP * h < cols) *(u32x4 *)(g.q + at + STEP * h) = c;
-            }
-            if (in && grp == 0) g.qs[(m0 + r) * g.qs_stride + nb] = (unsigned char)byte;
+            if (row < rows_left && grp == 0) g.qs[(first + row) * g.qs_stride + nb] = (unsigned char)byte;
         } else {
             uint32_t o[16];
             if constexpr (EPI == FG_RELU2_BWD) {
-                /* dh = da 2 sqrt(a); a's codes are at this lane's columns, its scale the block's */
-                u32x2 c[RUNS];
-                uint32_t byte = 127u;
-                if (in) byte = g.acts[(m0 + r) * g.act_stride + nb];
+                /* dh = da 2 sqrt(a) */
+                act[0] = next_act[0];
+                act[1] = next_act[1];
+                act_byte = row < rows_left ? g.acts[(first + row) * g.act_stride + nb] : 127u;
+                if (u + 1 < P::NU) fetch_act(u + 1);
+                unsigned char *codes = mine + 16 * 256;
+                fg_wave_order();
 #pragma unroll
-                for (int h = 0; h < RUNS; h++)
-                    c[h] = in && c0 + STEP * h < cols ? *(const u32x2 *)(g.act + at + STEP * h) : u32x2{0u, 0u};
-                const float s = f8_scale(byte);
+                for (int k = 0; k < 2; k++) *(u32x4 *)(codes + fg_code_place(8 * k + (lane >> 3), lane & 7)) = act[k];
+                fg_wave_order();
+                const float s = f8_scale(act_byte);
                 uint32_t m = 0u;
 #pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const uint32_t w = c[k >> 2][(k >> 1) & 1];
-                    const auto a = (k & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, true)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, s, false);
-                    /* v_sqrt_f32 is within an ulp; the result is rounded to bf16 right away */
-                    const float x = v[2 * k] * (2.0f * __builtin_amdgcn_sqrtf(a[0]));
-                    const float y = v[2 * k + 1] * (2.0f * __builtin_amdgcn_sqrtf(a[1]));
-                    o[k] = bf16_pair(x, y);
-                    m = pair_amax(m, o[k]);
-                }
-                const uint32_t qb = f8_scale_byte(group_max(pair_top(m)));
-                const float qs = f8_scale(qb);
+                for (int h = 0; h < 4; h++) {
+                    const u32x2 c = *(const u32x2 *)(codes + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1));
 #pragma unroll
-                for (int h = 0; h < RUNS; h++) {
-                    const u32x2 q = qb == F8_NAN_BYTE ? u32x2{F8_NAN_CODES, F8_NAN_CODES}
-                                                      : u32x2{f8_codes(o[4 * h], o[4 * h + 1], qs),
-                                                              f8_codes(o[4 * h + 2], o[4 * h + 3], qs)};
-                    if (in && c0 + STEP * h < cols) *(u32x2 *)(g.q + at + STEP * h) = q;
+                    for (int k = 0; k < 4; k++) {
+                        const auto a = (k & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[k >> 1], s, true)
+                                               : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[k >> 1], s, false);
+                        /* v_sqrt_f32 is within an ulp; the result is rounded to bf16 right away */
+                        const float x = v[8 * h + 2 * k] * (2.0f * __builtin_amdgcn_sqrtf(a[0]));
+                        const float y = v[8 * h + 2 * k + 1] * (2.0f * __builtin_amdgcn_sqrtf(a[1]));
+                        o[4 * h + k] = bf16_pair(x, y);
+                        m = pair_amax(m, o[4 * h + k]);
+                    }
                 }
-                if (in && grp == 0) g.qs[(m0 + r) * g.qs_stride + nb] = (unsigned char)qb;
+                const uint32_t byte = f8_scale_byte(group_max(pair_top(m)));
+                const float qs = f8_scale(byte);
+#pragma unroll
+                for (int h = 0; h < 4; h++)
+                    q[h] = byte == F8_NAN_BYTE ? u32x2{F8_NAN_CODES, F8_NAN_CODES}
+                                               : u32x2{f8_codes(o[4 * h], o[4 * h + 1], qs),
+                                                       f8_codes(o[4 * h + 2], o[4 * h + 3], qs)};
+                if (row < rows_left && grp == 0) g.qs[(first + row) * g.qs_stride + nb] = (unsigned char)byte;
             } else {
 #pragma unroll
                 for (int k = 0; k < 16; k++) o[k] = bf16_pair(v[2 * k], v[2 * k + 1]);
             }
+            fg_wave_order();
 #pragma unroll
-            for (int h = 0; h < RUNS; h++)
-                if (in && c0 + STEP * h < cols)
-                    *(u32x4 *)(g.out + at + STEP * h) = u32x4{o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]};
+            for (int h = 0; h < 4; h++)
+                *(u32x4 *)(mine + r16 * 256 + (((4 * h + grp) ^ r16) << 4)) =
+                    u32x4{o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]};
+            fg_wave_order();
+#pragma unroll
+            for (int k = 0; k < 4; k++) {   /* four rows an instruction, past the caches: larger than they are, and read much later */
+                const int r = 4 * k + (lane >> 4), c = lane & 15;
+                const u32x4 d = *(const u32x4 *)(mine + r * 256 + ((c ^ r) << 4));
+                if (16 * u + r < rows_left && col + 8 * c < cols)
+                    __builtin_nontemporal_store(d, (u32x4 *)(g.out + (first + 16 * u + r) * g.N + n0 + col + 8 * c));
+            }
+        }
+        if constexpr (EPI != FG_STORE) {
+            unsigned char *codes = mine + 16 * 256;
+            fg_wave_order();
+#pragma unroll
+            for (int h = 0; h < 4; h++) *(u32x2 *)(codes + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1)) = q[h];
+            fg_wave_order();
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int r = 8 * k + (lane >> 3), c = lane & 7;
+                const u32x4 d = *(const u32x4 *)(codes + fg_code_place(r, c));
+                if (16 * u + r < rows_left && col + 16 * c < cols)
+                    FG_CODE_STORE(d, (u32x4 *)(g.q + (first + 16 * u + r) * g.N + n0 + col + 16 * c));
+            }
         }
     }
 }
