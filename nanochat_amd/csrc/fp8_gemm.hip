@@ -219,9 +219,7 @@ __device__ __forceinline__ void fg_mfma(f32x4 &c, const i32x8 &w, const i32x8 &a
 }
 
 /* The full tile's DMA: instruction s = 0 .. 3 of a and of w moves rows 64 s + 8 wave + lane / 8; every fourth stage another
- * brings the scale dwords of its four blocks (waves 0-3: of rows 64 wave + lane; wave 4: of the two blocks of w). Inline
- * assembly: the compiler would have every LDS read that follows wait for it. Nothing else of the walk loads or writes LDS, and
- * the waits are the walk's. */
+ * brings the scale dwords of its four blocks (waves 0-3: of rows 64 wave + lane; wave 4: of the two blocks of w). */
 constexpr int FG_SCALES = 1280;   /* bytes of a group's scales in LDS: 256 dwords of a, then w's, behind both stage buffers */
 struct FgDma {
     u32x4 ra, rw, rs;
@@ -230,31 +228,21 @@ struct FgDma {
     int scale_at;
     int oa, ow;                   /* a stage's offsets */
     uint32_t to;
-    static __device__ __forceinline__ u32x4 words(const void *p, long long bytes) {
-        const uint64_t at = (uint64_t)p;
-        return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) & 0xFFFFu,
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
-    }
     __device__ __forceinline__ FgDma(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0) {
-        ra = words(g.a + m0 * g.K, (long long)p.rows * g.K);
-        rw = words(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
+        ra = f8_words(g.a + m0 * g.K, (long long)p.rows * g.K);
+        rw = f8_words(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
         const bool of_a = p.wave < 4;
         const int blocks = (p.cols + F8_BLOCK - 1) / F8_BLOCK;
-        rs = of_a ? words(g.as + m0 * g.as_stride, p.rows * g.as_stride)
-                  : words(g.ws + (long long)(n0 / F8_BLOCK) * g.ws_stride, (long long)blocks * g.ws_stride);
+        rs = of_a ? f8_words(g.as + m0 * g.as_stride, p.rows * g.as_stride)
+                  : f8_words(g.ws + (long long)(n0 / F8_BLOCK) * g.ws_stride, (long long)blocks * g.ws_stride);
         scale_at = of_a ? (64 * p.wave + p.lane) * (int)g.as_stride : p.lane < blocks ? p.lane * g.ws_stride : FG_PAST;
-        lds = (uint32_t)reinterpret_cast<uintptr_t>((LdsPtr *)b0) + p.wave * 1024;
-        scales = (uint32_t)reinterpret_cast<uintptr_t>((LdsPtr *)b0) + 2 * FgFull::STAGE + p.wave * 256;
+        lds = f8_lds(b0) + p.wave * 1024;
+        scales = f8_lds(b0) + 2 * FgFull::STAGE + p.wave * 256;
         K = g.K;
         const int row = 8 * p.wave + (p.lane >> 3), pos = p.lane & 7;
         first = row * K;
         ca = (pos ^ fg_swizzle_a(row)) << 4;
         cw = (pos ^ fg_swizzle_w(row)) << 4;   /* rows 64 on have the same */
-    }
-    static __device__ __forceinline__ void load(uint32_t to, int off, const u32x4 &r) {
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(to), "v"(off), "s"(r)
-                     : "memory");
     }
     /* Stage j's offsets, and its scales' DMA where it is the first of four. */
     __device__ __forceinline__ void stage(int j, int wave) {
@@ -267,11 +255,10 @@ struct FgDma {
         }
         to = lds + (j & 1) * FgFull::STAGE;
         if ((j & 3) == 0 && wave <= 4)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                         :: "s"(scales + ((j >> 2) & 1) * FG_SCALES), "v"(scale_at + j), "s"(rs) : "memory");
+            f8_dma4(scales + ((j >> 2) & 1) * FG_SCALES, scale_at + j, rs);
     }
     template <int S> __device__ __forceinline__ void issue() const {   /* S: 0 .. 3 a, 4 .. 7 w */
-        load(to + S * 8192, (S < 4 ? oa : ow) + 64 * (S & 3) * K, S < 4 ? ra : rw);
+        f8_dma16(to + S * 8192, (S < 4 ? oa : ow) + 64 * (S & 3) * K, S < 4 ? ra : rw);
     }
 };
 

@@ -6,11 +6,12 @@
  * exact in bf16, so x is unpacked on its way into LDS and the products are v_mfma_f32_16x16x32_bf16, fp32 sums, as exact as
  * those of a bf16 input: only half of that input's bytes are read.
  *
- * A workgroup owns a 256 x 256 tile of the result and a slice of the tokens, walked in stages of 32. dy's 256 columns go into
- * LDS by DMA, three stages ahead (a ring of four); x's 16 codes a thread into registers, three stages ahead, and as 32 bytes of
- * bf16 into one of two LDS buffers the stage before they are used. Both are read transposed (ds_read_b64_tr_b16: four tokens of
- * one column a lane). A 512-byte row keeps its 32-byte piece s at place s ^ (row % 8), so that the eight rows that half a wave
- * reads meet in different banks. Eight waves hold 128 x 64 results each.
+ * A workgroup owns a 256 x 256 tile of the result and a slice of the tokens, walked in stages of 32: four waves, one a SIMD, of
+ * 128 x 128 results each (all 256 AGPRs of a lane), which read the next stage's operands from LDS into the other half of 128
+ * registers between this stage's products. dy's 256 columns go into LDS by DMA four stages ahead, x's codes and scales five
+ * stages ahead; a thread turns its own 32 codes into bf16 two stages before they are multiplied. Operands are read transposed
+ * (ds_read_b64_tr_b16: four tokens of one column a lane). A 512-byte row keeps its 32-byte piece s at place s ^ (row % 8), so
+ * that the eight rows that half a wave reads meet in different banks.
  *
  * The result is small and the sum long: where tiles alone would leave CUs idle the tokens are cut into slices, whose partial
  * tiles fp8_grad_sum_kernel adds in slice order, so the result does not depend on scheduling.
@@ -32,7 +33,7 @@ constexpr int GR_T = 256;                     /* a tile's rows and columns */
 constexpr int GR_KC = 32;                     /* tokens of a stage */
 constexpr int GR_ROWB = GR_T * 2;
 constexpr int GR_OPB = GR_KC * GR_ROWB;       /* a stage's operand in LDS: 16 KiB */
-constexpr int GR_WAVES = 8;
+constexpr int GR_WAVES = 4;
 constexpr int GR_PAST = 0x7FFF0000;           /* a byte offset past every operand's range */
 
 enum { GR_PART, GR_ADD, GR_F32, GR_BF16 };
@@ -41,55 +42,74 @@ struct F8Grad {
     const uint16_t *dy;                       /* [M][N1] */
     const unsigned char *x, *xs;              /* [M][N2], [M] at xs_stride */
     long long xs_stride, M;
-    int N1, N2, tiles2, slices, rows;         /* rows: of a slice, a multiple of GR_KC */
+    int N1, N2, tiles1, tiles2, slices, rows;         /* rows: of a slice, a multiple of GR_KC */
     void *out;                                /* PART: fp32 [slices][N1][N2]; else the result [N1][N2] */
 };
 
-/* Stage j of dy: instruction q moves rows 2 q, 2 q + 1; lane l row 2 q + l / 32, LDS piece (l % 32) / 2, half l % 2. */
-__device__ __forceinline__ void gr_fetch(Rsrc rs, unsigned char *lds, int j, int N, int c0, int wave, int lane) {
-#pragma unroll
-    for (int k = 0; k < GR_OPB / 1024 / GR_WAVES; k++) {
-        const int q = wave + GR_WAVES * k, row = 2 * q + (lane >> 5);
-        const int piece = ((lane & 31) >> 1) ^ (row & 7), col = c0 + piece * 16 + (lane & 1) * 8;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LdsPtr *)(lds + q * 1024), 16,
-                                                 col < N ? ((j * GR_KC + row) * N + col) * 2 : GR_PAST, 0, 0, 0);
-    }
-}
+/* LDS: four stages of dy, two of x in bf16, four of x's codes and of its scale dwords (a token's two blocks lie in one). */
+constexpr int GR_CODES = GR_KC * GR_T;
+constexpr int GR_X = 4 * GR_OPB, GR_XC = GR_X + 2 * GR_OPB, GR_XS = GR_XC + 4 * GR_CODES, GR_LDS = GR_XS + 4 * 256;
 
-/* A thread's 16 codes of a stage of x and their scale byte: token tid / 16, columns 16 (tid % 16) .. + 15 of the tile. */
-struct Codes {
-    u32x4 c;
-    uint32_t byte;
-};
-struct XSource {
-    Rsrc codes, scales;
-    int at, scale_at;        /* this thread's byte offsets in stage 0 (GR_PAST: a column past N2) */
-    int step, scale_step;    /* bytes of a stage */
-    __device__ __forceinline__ Codes fetch(int j) const {
-        Codes f;
-        const bool in = at != GR_PAST;
-        f.c = __builtin_amdgcn_raw_buffer_load_b128(codes, in ? at + j * step : GR_PAST, 0, 0);
-        f.byte = __builtin_amdgcn_raw_buffer_load_b8(scales, in ? scale_at + j * scale_step : GR_PAST, 0, 0);
-        return f;
+/* The DMA of a workgroup, a wave's part. dy: instruction s moves rows 2 q, 2 q + 1, q = wave + 4 s; lane l row 2 q + l / 32, LDS
+ * piece (l % 32) / 2, half l % 2. x's codes: rows 4 q .. + 3, lane l row 4 q + l / 16, columns 16 (l % 16) .. + 15, q = wave + 4 s.
+ * Scales: every wave asks for all 32 tokens' dwords, lane l token l % 32, so that each waits for its own. */
+struct GrDma {
+    f8_u32x4 ra, rx, rs;
+    uint32_t lds;                 /* the workgroup's LDS */
+    uint32_t a, x, s;             /* this lane's offsets of instruction 0 in stage 0 (GR_PAST: a column past the result's) */
+    uint32_t a_row, x_row, s_row; /* bytes of a token */
+    int wave;
+    __device__ __forceinline__ void issue_a(int j, int k) const {   /* k: 0 .. 3 */
+        f8_dma16(lds + (j & 3) * GR_OPB + (wave + 4 * k) * 1024, a + (j * GR_KC + 8 * k) * a_row, ra);
+    }
+    __device__ __forceinline__ void issue_x(int j, int k) const {   /* k: 0, 1 codes, 2 scales */
+        if (k < 2) f8_dma16(lds + GR_XC + (j & 3) * GR_CODES + (wave + 4 * k) * 1024, x + (j * GR_KC + 16 * k) * x_row, rx);
+        else f8_dma4(lds + GR_XS + (j & 3) * 256, s + j * GR_KC * s_row, rs);
     }
 };
 
-/* The codes as bf16 into LDS. Tokens past the slice have codes and byte 0, and stay zeros. */
-__device__ __forceinline__ void gr_unpack(unsigned char *lds, const Codes &f, int tid) {
-    const int row = tid >> 4, piece = tid & 15;
-    const float s = f8_scale(f.byte < 1u ? 1u : f.byte);
-    u32x4 o[2];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        o[i >> 1][2 * (i & 1)] =
-            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)f.c[i], s, false));
-        o[i >> 1][2 * (i & 1) + 1] =
-            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)f.c[i], s, true));
+/* A thread's 2 x 16 codes of a stage of x (tokens tid / 16 and 16 on, columns 16 (tid % 16) .. + 15) and their scales, as its
+ * own wave's DMA left them, on their way to bf16. The empty asm statements keep each conversion where it is written. */
+struct GrUnpack {
+    u32x4 c[2], o[2];
+    float s[2];
+    uint32_t byte[2];
+    template <int K> __device__ __forceinline__ void read(const unsigned char *lds, int j, int tid, int scale_byte) {
+        c[K] = *(const u32x4 *)(lds + GR_XC + (j & 3) * GR_CODES + tid * 16 + 4096 * K);
+        byte[K] = lds[GR_XS + (j & 3) * 256 + ((tid >> 4) + 16 * K) * 4 + scale_byte];
     }
-    u32x4 *to = (u32x4 *)(lds + row * GR_ROWB + ((piece ^ (row & 7)) << 5));
-    to[0] = o[0];
-    to[1] = o[1];
-}
+    /* Tokens past the slice have codes and byte 0, and stay zeros. */
+    template <int K> __device__ __forceinline__ void scale() {
+        asm volatile("" : "+v"(byte[K]));
+        s[K] = f8_scale(byte[K] < 1u ? 1u : byte[K]);
+        asm volatile("" : "+v"(s[K]));
+    }
+    template <int K, int I> __device__ __forceinline__ void convert() {   /* codes 4 I .. + 3 */
+        uint32_t w = c[K][I];
+        asm volatile("" : "+v"(w));
+        uint32_t lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s[K], false));
+        uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, s[K], true));
+        asm volatile("" : "+v"(lo), "+v"(hi));
+        o[I >> 1][2 * (I & 1)] = lo;
+        o[I >> 1][2 * (I & 1) + 1] = hi;
+    }
+    template <int K> __device__ __forceinline__ void write(unsigned char *to, int tid) const {
+        const int row = (tid >> 4) + 16 * K, piece = tid & 15;
+        u32x4 *at = (u32x4 *)(to + row * GR_ROWB + ((piece ^ (row & 7)) << 5));
+        at[0] = o[0];
+        at[1] = o[1];
+    }
+    template <int K> __device__ __forceinline__ void all(const unsigned char *lds, int j, int tid, int scale_byte,
+                                                         unsigned char *to) {
+        read<K>(lds, j, tid, scale_byte);
+        scale<K>();
+        convert<K, 0>();
+        convert<K, 1>();
+        convert<K, 2>();
+        convert<K, 3>();
+        write<K>(to, tid);
+    }
+};
 
 /* The MFMA operand of columns 16 d .. + 15: lane (g, c) gets column 16 d + c of rows 4 g .. + 3, then 16 + 4 g .. + 3. */
 __device__ __forceinline__ bf16x8 gr_operand(const unsigned char *lds, int d, int g, int c) {
@@ -107,91 +127,160 @@ __device__ __forceinline__ void gr_barrier() {
     asm volatile("" ::: "memory");
 }
 
-__device__ __forceinline__ void gr_compute(const unsigned char *a, const unsigned char *b, f32x4 (&acc)[8][4], int wm, int wn,
-                                           int g, int c) {
-    bf16x8 fb[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++) fb[u] = gr_operand(b, 4 * wn + u, g, c);
-#pragma unroll
-    for (int t = 0; t < 8; t++) {
-        const bf16x8 fa = gr_operand(a, 8 * wm + t, g, c);
-#pragma unroll
-        for (int u = 0; u < 4; u++) acc[t][u] = mfma16x16x32(fa, fb[u], acc[t][u]);
-    }
+/* A wave's operands of a stage: 128 columns of dy, 128 of x. */
+struct Operands {
+    bf16x8 a[8], b[8];
+};
+
+/* The products as inline assembly: accumulators that stay in their AGPRs for the whole walk ("+a"; all 256). The compiler sees
+ * no matrix instructions there and inserts none of their wait states; they are kept by construction: operands are written by LDS
+ * reads alone, a step earlier; an accumulator is used again 63 products later, and read 32 wait states after the last one. */
+__device__ __forceinline__ void gr_mfma(f32x4 &c, const bf16x8 &a, const bf16x8 &b) {
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
-/* All but the 6 memory operations issued last have landed (a stage's fetch is x: 2, dy: 2; stage j needs dy of j, issued three
- * steps ago, and x of j + 1, issued two ago before dy of that stage), and this wave's LDS writes are done. */
-__device__ __forceinline__ void gr_wait() { __builtin_amdgcn_s_waitcnt(6 | (0x7 << 4) | (0x0 << 8)); }
+/* All but the DMA of the last two steps (7 a step) has landed, and this wave's LDS reads and writes are done. */
+__device__ __forceinline__ void gr_wait() { __builtin_amdgcn_s_waitcnt(14 | (0x7 << 4) | (0x0 << 8)); }
 
-/* Step j: dy of stage j in A, x of it in B; x of stage j + 1 goes from X1 into the other buffer; stage j + 3 is fetched (dy into
- * the buffer of stage j - 1, which every wave has left). */
-#define GR_STEP(j, A, AFREE, B, BNEXT, X1, X3)                    \
-    do {                                                            \
-        gr_wait();                                                  \
-        gr_barrier();                                               \
-        X3 = xsrc.fetch((j) + 3);                                   \
-        gr_fetch(ra, AFREE, (j) + 3, p.N1, i0, wave, lane);         \
-        gr_unpack(BNEXT, X1, tid);                                  \
-        gr_compute(A, B, acc, wm, wn, g, c);                        \
+/* What a step does between its products, behind product I of 64: a product keeps the matrix core busy for 16 cycles, in which
+ * the wave (one a SIMD) issues up to three more instructions; in a run they would let the core idle. */
+struct GrStep {
+    const unsigned char *lds, *la, *lb;   /* the workgroup's LDS, dy and x of stage j + 1 */
+    unsigned char *to;                    /* where x of stage j + 2 becomes bf16 */
+    int j, tid, scale_byte, wm, wn, g, c;
+    template <int I> __device__ __forceinline__ void side(Operands &next, GrUnpack &f, const GrDma &dma) const {
+        if constexpr (I < 32 && I % 4 == 1) next.b[I / 4] = gr_operand(lb, 8 * wn + I / 4, g, c);
+        if constexpr (I < 32 && I % 4 == 3) next.a[I / 4] = gr_operand(la, 8 * wm + I / 4, g, c);
+        if constexpr (I < 32 && I % 8 == 4) dma.issue_a(j + 4, I / 8);
+        if constexpr (I == 36) dma.issue_x(j + 5, 0);
+        if constexpr (I == 44) dma.issue_x(j + 5, 1);
+        if constexpr (I == 52) dma.issue_x(j + 5, 2);
+        if constexpr (I == 32) f.read<0>(lds, j + 2, tid, scale_byte);
+        if constexpr (I == 34) f.read<1>(lds, j + 2, tid, scale_byte);
+        if constexpr (I == 42) f.scale<0>();
+        if constexpr (I == 43) f.convert<0, 0>();
+        if constexpr (I == 45) f.convert<0, 1>();
+        if constexpr (I == 46) f.convert<0, 2>();
+        if constexpr (I == 47) f.convert<0, 3>();
+        if constexpr (I == 48) f.write<0>(to, tid);
+        if constexpr (I == 50) f.scale<1>();
+        if constexpr (I == 51) f.convert<1, 0>();
+        if constexpr (I == 53) f.convert<1, 1>();
+        if constexpr (I == 54) f.convert<1, 2>();
+        if constexpr (I == 55) f.convert<1, 3>();
+        if constexpr (I == 56) f.write<1>(to, tid);
+    }
+    template <int I = 0>
+    __device__ __forceinline__ void run(f32x4 (&acc)[8][8], const Operands &cur, Operands &next, GrUnpack &f,
+                                        const GrDma &dma) const {
+        if constexpr (I < 64) {
+            gr_mfma(acc[I / 8][I % 8], cur.a[I / 8], cur.b[I % 8]);
+            side<I>(next, f, dma);
+            run<I + 1>(acc, cur, next, f, dma);
+        }
+    }
+};
+
+/* Step j: the products of stage j, whose operands are in CUR, while NEXT takes those of stage j + 1; x of stage j + 2 becomes
+ * bf16; dy of stage j + 4 and x's codes of stage j + 5 are fetched (into the buffers of stages j and j + 1, whose readers are a
+ * barrier behind). EVEN: j's parity, that of its bf16 buffer. */
+#define GR_STEP(j, EVEN, CUR, NEXT)                                                                               \
+    do {                                                                                                           \
+        gr_wait();                                                                                                 \
+        gr_barrier();                                                                                              \
+        const GrStep step = {lds, lds + (((j) + 1) & 3) * GR_OPB, lds + GR_X + (1 - (EVEN)) * GR_OPB,              \
+                             lds + GR_X + (EVEN) * GR_OPB, (j), tid, scale_byte, wm, wn, g, c};                    \
+        GrUnpack f;                                                                                                \
+        step.run(acc, CUR, NEXT, f, dma);                                                                          \
     } while (0)
 
 template <int MODE>
 __global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grad p) {
-    __shared__ __align__(16) unsigned char a0[GR_OPB], a1[GR_OPB], a2[GR_OPB], a3[GR_OPB], b0[GR_OPB], b1[GR_OPB];
-    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid >> 6, g = lane >> 4, c = lane & 15;
-    const int wm = wave >> 2, wn = wave & 3;
-    /* slices fastest: the workgroups that run together read different tokens of the same few columns */
-    const int slice = blockIdx.x % p.slices, tile = blockIdx.x / p.slices;
-    const int i0 = tile / p.tiles2 * GR_T, j0 = tile % p.tiles2 * GR_T;
+    __shared__ __align__(16) unsigned char lds[GR_LDS];
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const int wm = wave >> 1, wn = wave & 1;
+    /* Workgroup L runs on XCD L % 8: each XCD takes a contiguous run of (slice, band of 4 row tiles, column tile, row tile), so
+     * that what it runs at once reads the same tokens of few columns. */
+    const int tiles = p.tiles1 * p.tiles2, l = blockIdx.x, per = gridDim.x / 8, extra = gridDim.x % 8;
+    const int id = l % 8 * per + min(l % 8, extra) + l / 8, slice = id / tiles, tile = id % tiles;
+    const int band = tile / (4 * p.tiles2), tall = min(4, p.tiles1 - 4 * band), in = tile - band * 4 * p.tiles2;
+    const int i0 = (4 * band + in % tall) * GR_T, j0 = in / tall * GR_T;
     const long long m0 = (long long)slice * p.rows;
     const int rows = (int)(p.M - m0 < p.rows ? p.M - m0 : p.rows);   /* > 0: the host makes no empty slice */
-    const Rsrc ra = f8_rsrc(p.dy + m0 * p.N1, (long long)rows * p.N1 * 2);
-    XSource xsrc;
-    xsrc.codes = f8_rsrc(p.x + m0 * p.N2, (long long)rows * p.N2);
-    xsrc.scales = f8_rsrc(p.xs + m0 * p.xs_stride, rows * p.xs_stride);
-    const int xcol = j0 + 16 * (tid & 15);
-    xsrc.at = xcol < p.N2 ? (tid >> 4) * p.N2 + xcol : GR_PAST;
-    xsrc.scale_at = (tid >> 4) * (int)p.xs_stride + xcol / F8_BLOCK;
-    xsrc.step = GR_KC * p.N2;
-    xsrc.scale_step = GR_KC * (int)p.xs_stride;
+    GrDma dma;
+    dma.ra = f8_words(p.dy + m0 * p.N1, (long long)rows * p.N1 * 2);
+    dma.rx = f8_words(p.x + m0 * p.N2, (long long)rows * p.N2);
+    dma.rs = f8_words(p.xs + m0 * p.xs_stride, rows * p.xs_stride);
+    dma.lds = f8_lds(lds);
+    dma.wave = wave;
+    dma.a_row = p.N1 * 2;
+    dma.x_row = p.N2;
+    dma.s_row = (uint32_t)p.xs_stride;
+    {
+        const int row = 2 * wave + (lane >> 5), col = i0 + (((lane & 31) >> 1) ^ (row & 7)) * 16 + (lane & 1) * 8;
+        dma.a = col < p.N1 ? row * dma.a_row + col * 2 : GR_PAST;   /* rows 8 on have the same piece */
+        const int xrow = 4 * wave + (lane >> 4), xcol = j0 + 16 * (lane & 15);
+        dma.x = xcol < p.N2 ? xrow * dma.x_row + xcol : GR_PAST;
+        dma.s = lane < 32 ? lane * dma.s_row + (j0 / F8_BLOCK & ~3) : GR_PAST;
+    }
+    const int scale_byte = (j0 / F8_BLOCK & 3) + ((tid & 15) >> 3);
     const int stages = (rows + GR_KC - 1) / GR_KC;
-    f32x4 acc[8][4];
+    f32x4 acc[8][8];
 #pragma unroll
     for (int t = 0; t < 8; t++)
 #pragma unroll
-        for (int u = 0; u < 4; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    Codes x0 = xsrc.fetch(0);
-    gr_fetch(ra, a0, 0, p.N1, i0, wave, lane);
-    Codes x1 = xsrc.fetch(1);
-    gr_fetch(ra, a1, 1, p.N1, i0, wave, lane);
-    Codes x2 = xsrc.fetch(2), x3;
-    gr_fetch(ra, a2, 2, p.N1, i0, wave, lane);
-    gr_unpack(b0, x0, tid);
-    for (int j = 0; j < stages; j += 4) {   /* stages past the slice read zeros and add nothing */
-        GR_STEP(j, a0, a3, b0, b1, x1, x3);
-        GR_STEP(j + 1, a1, a0, b1, b0, x2, x0);
-        GR_STEP(j + 2, a2, a1, b0, b1, x3, x1);
-        GR_STEP(j + 3, a3, a2, b1, b0, x0, x2);
+        for (int u = 0; u < 8; u++) asm volatile("" : "=a"(acc[t][u]) : "0"(f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+#pragma unroll
+        for (int k = 0; k < 3; k++) dma.issue_x(j, k);
+#pragma unroll
+        for (int k = 0; k < 4; k++) dma.issue_a(j, k);
+    }
+    __builtin_amdgcn_s_waitcnt((18 & 0xF) | ((18 >> 4) << 14) | (0x7 << 4) | (0xF << 8));   /* x of 0 and 1, dy of 0 */
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        GrUnpack f;
+        f.all<0>(lds, j, tid, scale_byte, lds + GR_X + j * GR_OPB);
+        f.all<1>(lds, j, tid, scale_byte, lds + GR_X + j * GR_OPB);
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);   /* the LDS writes */
+    gr_barrier();
+#pragma unroll
+    for (int k = 0; k < 3; k++) dma.issue_x(4, k);
+    Operands o0, o1;
+#pragma unroll
+    for (int t = 0; t < 8; t++) {
+        o0.b[t] = gr_operand(lds + GR_X, 8 * wn + t, g, c);
+        o0.a[t] = gr_operand(lds, 8 * wm + t, g, c);
+    }
+    for (int j = 0; j < stages; j += 2) {   /* a stage past the slice reads zeros and adds nothing */
+        GR_STEP(j, 0, o0, o1);
+        GR_STEP(j + 1, 1, o1, o0);
     }
     __builtin_amdgcn_s_waitcnt(0);   /* no DMA may land in LDS after the workgroup ends */
-    /* lane (g, c) of result tile (t, u): rows i0 + 128 wm + 16 t + 4 g + e, column j0 + 64 wn + 16 u + c; 32-bit offsets into the
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");   /* 32 wait states; no read moves above */
+#pragma unroll
+    for (int t = 0; t < 8; t++)
+#pragma unroll
+        for (int u = 0; u < 8; u++) asm volatile("" : "+a"(acc[t][u]));
+    /* lane (g, c) of result tile (t, u): rows i0 + 128 wm + 16 t + 4 g + e, column j0 + 128 wn + 16 u + c; 32-bit offsets into the
      * tile's rows, those past N1 and columns past N2 outside the range */
     constexpr int SIZE = MODE == GR_BF16 ? 2 : 4;
     const int live = p.N1 - i0 < GR_T ? p.N1 - i0 : GR_T;
     const unsigned row_bytes = (unsigned)p.N2 * SIZE;
     const long long first = ((MODE == GR_PART ? (long long)slice * p.N1 : 0) + i0) * p.N2;
     const Rsrc ro = f8_rsrc((unsigned char *)p.out + first * SIZE, (long long)live * row_bytes);
-    unsigned at[4];
+    unsigned at[8];
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-        const int col = j0 + 64 * wn + 16 * u + c;
+    for (int u = 0; u < 8; u++) {
+        const int col = j0 + 128 * wn + 16 * u + c;
         at[u] = col < p.N2 ? (unsigned)(128 * wm + 4 * g) * row_bytes + (unsigned)col * SIZE : (unsigned)GR_PAST;
     }
-    float old[2][4][4];   /* ADD: the result's rows of t, and of t + 1 in flight */
+    float old[2][8][4];   /* ADD: the result's rows of t, and of t + 1 in flight */
     const auto fetch_old = [&](int t) {
 #pragma unroll
-        for (int u = 0; u < 4; u++)
+        for (int u = 0; u < 8; u++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 old[t & 1][u][e] =
@@ -202,7 +291,7 @@ __global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grad p) {
     for (int t = 0; t < 8; t++) {
         if (MODE == GR_ADD && t < 7) fetch_old(t + 1);
 #pragma unroll
-        for (int u = 0; u < 4; u++)
+        for (int u = 0; u < 8; u++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const unsigned to = at[u] + (16 * t + e) * row_bytes;
@@ -285,7 +374,7 @@ extern "C" int nc_fp8_weight_grad(const void *dy, const void *codes, const void 
     if (!dy || !codes || !scale || !out || !workspace) return NC_ERR_NULL;
     if (((uintptr_t)dy | (uintptr_t)codes | (uintptr_t)out | (uintptr_t)workspace) & 15) return NC_ERR_SHAPE;
     F8Grad p = {(const uint16_t *)dy, (const unsigned char *)codes, (const unsigned char *)scale, scale_stride, rows, n1, n2,
-                (n2 + GR_T - 1) / GR_T, 0, 0, out};
+                (n1 + GR_T - 1) / GR_T, (n2 + GR_T - 1) / GR_T, 0, 0, out};
     grad_slices(rows, n1, n2, p.slices, p.rows);
     if (workspace_bytes < grad_bytes(p.slices, n1, n2)) return NC_ERR_WORKSPACE;
     const long long tiles = (long long)((n1 + GR_T - 1) / GR_T) * p.tiles2;

@@ -73,6 +73,28 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t f8_rsrc(const void *p, long lo
                                              __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
 }
 
+/* DMA from memory to LDS of 16 or 4 bytes a lane (lane l's to `to` + 16 l or 4 l), as inline assembly: the compiler makes every
+ * LDS read that follows its own form wait for it. The kernels that use it load and store nothing else meanwhile, and keep its
+ * waits themselves. An offset past the resource's range reads zeros without an access. */
+typedef uint32_t f8_u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f8_u32x4 f8_words(const void *p, long long bytes) {
+    const uint64_t at = (uint64_t)p;
+    return f8_u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
+                    (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) & 0xFFFFu,
+                    (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+__device__ __forceinline__ void f8_dma16(uint32_t to, uint32_t off, const f8_u32x4 &r) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(to), "v"(off), "s"(r)
+                 : "memory");
+}
+__device__ __forceinline__ void f8_dma4(uint32_t to, uint32_t off, const f8_u32x4 &r) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(to), "v"(off), "s"(r)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t f8_lds(const void *p) {
+    return (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)p);
+}
+
 /* Largest over lanes L ^ 1, 2, 4 (8 lanes), over L ^ 16 and L ^ 32 (the four groups of 16 lanes). */
 template <int M> __device__ __forceinline__ uint32_t lane_max_dpp(uint32_t v) {
     const uint32_t o = __float_as_uint(lane_xor_dpp<M>(__uint_as_float(v)));
