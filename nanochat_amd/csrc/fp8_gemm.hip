@@ -380,17 +380,21 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
     const long long first = m0 + 16 * P::NU * p.wm;
     unsigned char *mine = b0 + (threadIdx.x >> 6) * FG_TURN;
     const int r16 = lane & 15;
-    u32x4 act[2], next_act[2];
-    uint32_t act_byte = 127u;
-    /* RELU2_BWD: 16 rows' codes of a, a piece of 16 columns a lane: rows 8 k + lane / 8 */
-    const auto fetch_act = [&](int u) {
+    /* RELU2_BWD: a's codes, a piece of 16 columns a lane of rows 8 k + lane / 8 of each 16, and its scales; all on their way at once */
+    u32x4 act[P::NU][2];
+    uint32_t act_byte[P::NU];
+    if constexpr (EPI == FG_RELU2_BWD) {
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int r = 16 * u + 8 * k + (lane >> 3), c = col + 16 * (lane & 7);
-            next_act[k] = r < rows_left && c < cols ? *(const u32x4 *)(g.act + (first + r) * g.N + n0 + c) : u32x4{0, 0, 0, 0};
+        for (int u = 0; u < P::NU; u++) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int r = 16 * u + 8 * k + (lane >> 3), c = col + 16 * (lane & 7);
+                act[u][k] = r < rows_left && c < cols ? *(const u32x4 *)(g.act + (first + r) * g.N + n0 + c) : u32x4{0, 0, 0, 0};
+            }
+            const int r = 16 * u + r16;
+            act_byte[u] = r < rows_left ? g.acts[(first + r) * g.act_stride + nb] : 127u;
         }
-    };
-    if constexpr (EPI == FG_RELU2_BWD) fetch_act(0);
+    }
 #pragma unroll
     for (int u = 0; u < P::NU; u++) {
         const int row = 16 * u + r16;                         /* this lane's results: columns 32 h + 8 grp + 0 .. 7 */
@@ -423,16 +427,12 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
             uint32_t o[16];
             if constexpr (EPI == FG_RELU2_BWD) {
                 /* dh = da 2 sqrt(a) */
-                act[0] = next_act[0];
-                act[1] = next_act[1];
-                act_byte = row < rows_left ? g.acts[(first + row) * g.act_stride + nb] : 127u;
-                if (u + 1 < P::NU) fetch_act(u + 1);
                 unsigned char *codes = mine + 16 * 256;
                 fg_wave_order();
 #pragma unroll
-                for (int k = 0; k < 2; k++) *(u32x4 *)(codes + fg_code_place(8 * k + (lane >> 3), lane & 7)) = act[k];
+                for (int k = 0; k < 2; k++) *(u32x4 *)(codes + fg_code_place(8 * k + (lane >> 3), lane & 7)) = act[u][k];
                 fg_wave_order();
-                const float s = f8_scale(act_byte);
+                const float s = f8_scale(act_byte[u]);
                 uint32_t m = 0u;
 #pragma unroll
                 for (int h = 0; h < 4; h++) {

@@ -46,25 +46,36 @@ struct F8Grad {
     void *out;                                /* PART: fp32 [slices][N1][N2]; else the result [N1][N2] */
 };
 
-/* LDS: four stages of dy, two of x in bf16, four of x's codes and of its scale dwords (a token's two blocks lie in one). */
+/* LDS: four stages of dy, two of x in bf16, four of x's codes, eight of its scale dwords (a token's two blocks lie in one). */
 constexpr int GR_CODES = GR_KC * GR_T;
-constexpr int GR_X = 4 * GR_OPB, GR_XC = GR_X + 2 * GR_OPB, GR_XS = GR_XC + 4 * GR_CODES, GR_LDS = GR_XS + 4 * 256;
+constexpr int GR_X = 4 * GR_OPB, GR_XC = GR_X + 2 * GR_OPB, GR_XS = GR_XC + 4 * GR_CODES, GR_LDS = GR_XS + 8 * 128;
 
 /* The DMA of a workgroup, a wave's part. dy: instruction s moves rows 2 q, 2 q + 1, q = wave + 4 s; lane l row 2 q + l / 32, LDS
  * piece (l % 32) / 2, half l % 2. x's codes: rows 4 q .. + 3, lane l row 4 q + l / 16, columns 16 (l % 16) .. + 15, q = wave + 4 s.
- * Scales: every wave asks for all 32 tokens' dwords, lane l token l % 32, so that each waits for its own. */
+ * Scales: every wave asks for all 64 tokens' dwords of two stages, lane l token l, so that each waits for its own. */
 struct GrDma {
     f8_u32x4 ra, rx, rs;
     uint32_t lds;                 /* the workgroup's LDS */
     uint32_t a, x, s;             /* this lane's offsets of instruction 0 in stage 0 (GR_PAST: a column past the result's) */
-    uint32_t a_row, x_row, s_row; /* bytes of a token */
+    uint32_t s_row;               /* bytes of a token's scales */
     int wave;
-    __device__ __forceinline__ void issue_a(int j, int k) const {   /* k: 0 .. 3 */
-        f8_dma16(lds + (j & 3) * GR_OPB + (wave + 4 * k) * 1024, a + (j * GR_KC + 8 * k) * a_row, ra);
+    uint32_t lds_a, lds_x;        /* where the next stage's go */
+    uint32_t a8, a16, a24, x16;   /* bytes of 8, 16, 24 and 16 tokens */
+    __device__ __forceinline__ void at_a(int j) { lds_a = lds + (j & 3) * GR_OPB + wave * 1024; }
+    __device__ __forceinline__ void at_x(int j) { lds_x = lds + GR_XC + (j & 3) * GR_CODES + wave * 1024; }
+    /* Instruction K of the next stage of dy, of x's codes, and (every other stage) the scale dwords of 64 tokens; after the last
+     * one the offsets move on. */
+    template <int K> __device__ __forceinline__ void issue_a() {
+        f8_dma16<4096 * K>(lds_a, a, K == 0 ? 0u : K == 1 ? a8 : K == 2 ? a16 : a24, ra);
+        if constexpr (K == 3) a += 4 * a8;
     }
-    __device__ __forceinline__ void issue_x(int j, int k) const {   /* k: 0, 1 codes, 2 scales */
-        if (k < 2) f8_dma16(lds + GR_XC + (j & 3) * GR_CODES + (wave + 4 * k) * 1024, x + (j * GR_KC + 16 * k) * x_row, rx);
-        else f8_dma4(lds + GR_XS + (j & 3) * 256, s + j * GR_KC * s_row, rs);
+    template <int K> __device__ __forceinline__ void issue_x() {
+        f8_dma16<4096 * K>(lds_x, x, K == 0 ? 0u : x16, rx);
+        if constexpr (K == 1) x += 2 * x16;
+    }
+    __device__ __forceinline__ void issue_s(int j) {   /* stages j and j + 1, j even */
+        f8_dma4(lds + GR_XS + (j & 6) * 128, s, rs);
+        s += 2 * GR_KC * s_row;
     }
 };
 
@@ -76,7 +87,7 @@ struct GrUnpack {
     uint32_t byte[2];
     template <int K> __device__ __forceinline__ void read(const unsigned char *lds, int j, int tid, int scale_byte) {
         c[K] = *(const u32x4 *)(lds + GR_XC + (j & 3) * GR_CODES + tid * 16 + 4096 * K);
-        byte[K] = lds[GR_XS + (j & 3) * 256 + ((tid >> 4) + 16 * K) * 4 + scale_byte];
+        byte[K] = lds[GR_XS + (j & 7) * 128 + ((tid >> 4) + 16 * K) * 4 + scale_byte];
     }
     /* Tokens past the slice have codes and byte 0, and stay zeros. */
     template <int K> __device__ __forceinline__ void scale() {
@@ -139,8 +150,9 @@ __device__ __forceinline__ void gr_mfma(f32x4 &c, const bf16x8 &a, const bf16x8 
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
-/* All but the DMA of the last two steps (7 a step) has landed, and this wave's LDS reads and writes are done. */
-__device__ __forceinline__ void gr_wait() { __builtin_amdgcn_s_waitcnt(14 | (0x7 << 4) | (0x0 << 8)); }
+/* All but the DMA of the last two steps (6 and 7: an odd one brings scales) has landed, and this wave's LDS reads and writes are
+ * done. */
+__device__ __forceinline__ void gr_wait() { __builtin_amdgcn_s_waitcnt(13 | (0x7 << 4) | (0x0 << 8)); }
 
 /* What a step does between its products, behind product I of 64: a product keeps the matrix core busy for 16 cycles, in which
  * the wave (one a SIMD) issues up to three more instructions; in a run they would let the core idle. */
@@ -148,13 +160,15 @@ struct GrStep {
     const unsigned char *lds, *la, *lb;   /* the workgroup's LDS, dy and x of stage j + 1 */
     unsigned char *to;                    /* where x of stage j + 2 becomes bf16 */
     int j, tid, scale_byte, wm, wn, g, c;
-    template <int I> __device__ __forceinline__ void side(Operands &next, GrUnpack &f, const GrDma &dma) const {
+    template <int I, bool EVEN> __device__ __forceinline__ void side(Operands &next, GrUnpack &f, GrDma &dma) const {
         if constexpr (I < 32 && I % 4 == 1) next.b[I / 4] = gr_operand(lb, 8 * wn + I / 4, g, c);
         if constexpr (I < 32 && I % 4 == 3) next.a[I / 4] = gr_operand(la, 8 * wm + I / 4, g, c);
-        if constexpr (I < 32 && I % 8 == 4) dma.issue_a(j + 4, I / 8);
-        if constexpr (I == 36) dma.issue_x(j + 5, 0);
-        if constexpr (I == 44) dma.issue_x(j + 5, 1);
-        if constexpr (I == 52) dma.issue_x(j + 5, 2);
+        if constexpr (I == 2) dma.at_a(j + 4);
+        if constexpr (I < 32 && I % 8 == 4) dma.issue_a<I / 8>();
+        if constexpr (I == 35) dma.at_x(j + 5);
+        if constexpr (I == 37) dma.issue_x<0>();
+        if constexpr (I == 40) dma.issue_x<1>();
+        if constexpr (I == 58 && !EVEN) dma.issue_s(j + 5);
         if constexpr (I == 32) f.read<0>(lds, j + 2, tid, scale_byte);
         if constexpr (I == 34) f.read<1>(lds, j + 2, tid, scale_byte);
         if constexpr (I == 42) f.scale<0>();
@@ -170,13 +184,12 @@ struct GrStep {
         if constexpr (I == 55) f.convert<1, 3>();
         if constexpr (I == 56) f.write<1>(to, tid);
     }
-    template <int I = 0>
-    __device__ __forceinline__ void run(f32x4 (&acc)[8][8], const Operands &cur, Operands &next, GrUnpack &f,
-                                        const GrDma &dma) const {
+    template <bool EVEN, int I = 0>
+    __device__ __forceinline__ void run(f32x4 (&acc)[8][8], const Operands &cur, Operands &next, GrUnpack &f, GrDma &dma) const {
         if constexpr (I < 64) {
             gr_mfma(acc[I / 8][I % 8], cur.a[I / 8], cur.b[I % 8]);
-            side<I>(next, f, dma);
-            run<I + 1>(acc, cur, next, f, dma);
+            side<I, EVEN>(next, f, dma);
+            run<EVEN, I + 1>(acc, cur, next, f, dma);
         }
     }
 };
@@ -191,7 +204,7 @@ struct GrStep {
         const GrStep step = {lds, lds + (((j) + 1) & 3) * GR_OPB, lds + GR_X + (1 - (EVEN)) * GR_OPB,              \
                              lds + GR_X + (EVEN) * GR_OPB, (j), tid, scale_byte, wm, wn, g, c};                    \
         GrUnpack f;                                                                                                \
-        step.run(acc, CUR, NEXT, f, dma);                                                                          \
+        step.run<(EVEN) == 0>(acc, CUR, NEXT, f, dma);                                                                          \
     } while (0)
 
 template <int MODE>
@@ -213,15 +226,17 @@ __global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grad p) {
     dma.rs = f8_words(p.xs + m0 * p.xs_stride, rows * p.xs_stride);
     dma.lds = f8_lds(lds);
     dma.wave = wave;
-    dma.a_row = p.N1 * 2;
-    dma.x_row = p.N2;
     dma.s_row = (uint32_t)p.xs_stride;
+    dma.a8 = 16 * p.N1;
+    dma.a16 = 32 * p.N1;
+    dma.a24 = 48 * p.N1;
+    dma.x16 = 16 * p.N2;
     {
         const int row = 2 * wave + (lane >> 5), col = i0 + (((lane & 31) >> 1) ^ (row & 7)) * 16 + (lane & 1) * 8;
-        dma.a = col < p.N1 ? row * dma.a_row + col * 2 : GR_PAST;   /* rows 8 on have the same piece */
+        dma.a = col < p.N1 ? (uint32_t)(row * p.N1 + col) * 2 : GR_PAST;   /* rows 8 on have the same piece */
         const int xrow = 4 * wave + (lane >> 4), xcol = j0 + 16 * (lane & 15);
-        dma.x = xcol < p.N2 ? xrow * dma.x_row + xcol : GR_PAST;
-        dma.s = lane < 32 ? lane * dma.s_row + (j0 / F8_BLOCK & ~3) : GR_PAST;
+        dma.x = xcol < p.N2 ? (uint32_t)(xrow * p.N2 + xcol) : GR_PAST;
+        dma.s = lane * dma.s_row + (j0 / F8_BLOCK & ~3);
     }
     const int scale_byte = (j0 / F8_BLOCK & 3) + ((tid & 15) >> 3);
     const int stages = (rows + GR_KC - 1) / GR_KC;
@@ -230,14 +245,22 @@ __global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grad p) {
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int u = 0; u < 8; u++) asm volatile("" : "=a"(acc[t][u]) : "0"(f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
+    const auto fetch_x = [&](int j) {
+        if (!(j & 1)) dma.issue_s(j);
+        dma.at_x(j);
+        dma.issue_x<0>();
+        dma.issue_x<1>();
+    };
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-#pragma unroll
-        for (int k = 0; k < 3; k++) dma.issue_x(j, k);
-#pragma unroll
-        for (int k = 0; k < 4; k++) dma.issue_a(j, k);
+        fetch_x(j);
+        dma.at_a(j);
+        dma.issue_a<0>();
+        dma.issue_a<1>();
+        dma.issue_a<2>();
+        dma.issue_a<3>();
     }
-    __builtin_amdgcn_s_waitcnt((18 & 0xF) | ((18 >> 4) << 14) | (0x7 << 4) | (0xF << 8));   /* x of 0 and 1, dy of 0 */
+    __builtin_amdgcn_s_waitcnt((17 & 0xF) | ((17 >> 4) << 14) | (0x7 << 4) | (0xF << 8));   /* x of 0 and 1, dy of 0 */
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         GrUnpack f;
@@ -246,8 +269,7 @@ __global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grad p) {
     }
     __builtin_amdgcn_s_waitcnt(0xC07F);   /* the LDS writes */
     gr_barrier();
-#pragma unroll
-    for (int k = 0; k < 3; k++) dma.issue_x(4, k);
+    fetch_x(4);
     Operands o0, o1;
 #pragma unroll
     for (int t = 0; t < 8; t++) {
@@ -328,20 +350,40 @@ __global__ void __launch_bounds__(256) fp8_grad_sum_kernel(const float4 *part, i
 
 constexpr int GR_MIN_ROWS = 4 * GR_KC;   /* a shorter slice is mostly the ring's start */
 
-/* Token slices: as many as fill the CUs with tiles, none under GR_MIN_ROWS rows unless it is the only one and none whose
- * operand slice passes 1 GiB. */
+/* What M tokens take in us by a model of measured parts, one workgroup a CU: rounds of workgroups, each a slice's stages and ten
+ * more for its start and its end; a stage 0.6 and up to 0.15 more with every CU at work (clock, and the L2s shared); a slice's
+ * partial tiles out and back at 4.5 TB/s. One slice has none. */
+double grad_time(long long tiles, long long elements, int cus, long long slices, long long rows) {
+    const double rounds = (double)((tiles * slices + cus - 1) / cus), busy = (double)(tiles * slices) / (rounds * cus);
+    const double partials = slices == 1 ? 0.0 : 3.0 + slices * elements * 8.0 / 4.5e6;
+    return rounds * (rows / GR_KC + 10) * (0.6 + 0.15 * busy) + partials;
+}
+
+/* Token slices: the best of a few counts by grad_time (small ones, steps of about a quarter above, and those that just fill one
+ * to six rounds), none under GR_MIN_ROWS rows unless it is the only one and none whose operand slice passes 1 GiB. */
 void grad_slices(long long M, int N1, int N2, int &slices, int &rows) {
     const long long tiles = (long long)((N1 + GR_T - 1) / GR_T) * ((N2 + GR_T - 1) / GR_T);
     const long long wide = (long long)N1 * 2 > N2 ? (long long)N1 * 2 : N2;
     const long long fit = (1LL << 30) / wide / GR_KC * GR_KC;
-    long long s = device_cus() / tiles;
-    const long long most = (M + GR_MIN_ROWS - 1) / GR_MIN_ROWS, least = (M + fit - 1) / fit;
-    s = s < most ? s : most;
-    s = s > 1 ? s : 1;
-    s = s > least ? s : least;
-    rows = (int)(((M + s - 1) / s + GR_KC - 1) / GR_KC * GR_KC);
-    if (rows > fit) rows = (int)fit;
-    slices = (int)((M + rows - 1) / rows);
+    const long long least = (M + fit - 1) / fit, most = (M + GR_MIN_ROWS - 1) / GR_MIN_ROWS;
+    const int cus = device_cus();
+    double best = -1.0;
+    slices = rows = 0;
+    auto consider = [&](long long s) {
+        s = s < most ? s : most;
+        s = s > least ? s : least;
+        const long long r = ((M + s - 1) / s + GR_KC - 1) / GR_KC * GR_KC;
+        if (r > fit) return;
+        s = (M + r - 1) / r;   /* no empty slice */
+        const double t = grad_time(tiles, (long long)N1 * N2, cus, s, r);
+        if (best >= 0.0 && t >= best) return;
+        best = t;
+        slices = (int)s;
+        rows = (int)r;
+    };
+    for (long long s = 1; s <= most && (s == 1 || tiles * s <= 6LL * cus); s += s < 8 ? 1 : s / 4) consider(s);
+    for (int k = 1; k <= 6; k++)
+        if (k * cus >= tiles) consider(k * cus / tiles);
 }
 
 /* One slice needs none (never 0 where there is a call). */

@@ -91,6 +91,12 @@ __device__ __forceinline__ void f8_dma4(uint32_t to, uint32_t off, const f8_u32x
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(to), "v"(off), "s"(r)
                  : "memory");
 }
+/* f8_dma16 to base + STEP, from off + more, in three instructions. */
+template <int STEP> __device__ __forceinline__ void f8_dma16(uint32_t base, uint32_t off, uint32_t more, const f8_u32x4 &r) {
+    uint32_t at;
+    asm volatile("s_add_u32 m0, %1, %2\n\tv_add_u32 %0, %4, %3\n\tbuffer_load_dwordx4 %0, %5, 0 offen lds"
+                 : "=&v"(at) : "s"(base), "i"(STEP), "v"(off), "s"(more), "s"(r) : "memory", "scc");
+}
 __device__ __forceinline__ uint32_t f8_lds(const void *p) {
     return (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)p);
 }
