@@ -501,7 +501,7 @@ __device__ __forceinline__ int2 fg_tile(int l, int count, int nx) {
 }
 
 template <class P, int EPI>
-__global__ void __launch_bounds__(P::WAVES *WAVE, P::WAVES == 8 ? 2 : 2) fp8_gemm_kernel(F8Gemm g) {
+__global__ void __launch_bounds__(P::WAVES *WAVE, 2) fp8_gemm_kernel(F8Gemm g) {
     /* the smaller tiles: distinct objects, as reads of one do not wait for the other's DMA */
     __shared__ __align__(16) unsigned char b0[P::WAVES == 8 ? 2 * P::STAGE + 2 * FG_SCALES : P::STAGE], b1[P::WAVES == 8 ? 16 : P::STAGE];
     const int2 t = fg_tile(blockIdx.x, gridDim.x, (g.N + P::TN - 1) / P::TN);
@@ -542,6 +542,8 @@ int fg_check(const F8Gemm &g, int epi) {
 int fg_gemm(const F8Gemm &g, int epi, void *stream) {
     const int e = fg_check(g, epi);
     if (e != NC_OK || g.M == 0) return e;
+    if (epi == FG_STORE && fp8_some_takes(g.M, g.K))
+        return fp8_some(g.a, g.as, g.as_stride, g.w, g.ws, g.ws_stride, (int)g.M, g.N, g.K, false, g.out, (hipStream_t)stream);
     const long long full = (g.M + 255) / 256 * ((g.N + 255) / 256), half = (g.M + 127) / 128 * ((g.N + 127) / 128);
     const int cus = device_cus();
     if (full >= cus) return fg_launch<FgFull>(g, epi, (hipStream_t)stream);

@@ -65,10 +65,10 @@ def _check_scale(scale: Tensor, name: str, rows: int, cols: int, device: torch.d
     if scale.dtype != SCALE:
         raise TypeError(f"{name} must be {SCALE}, got {scale.dtype}")
     blocks = _blocks(cols)
-    if scale.shape != (rows, blocks) or scale.device != device:
+    if scale.dim() != 2 or scale.shape != (rows, blocks) or scale.device != device:
         raise ValueError(f"{name} must be [{rows}, {blocks}] on {device}, got {tuple(scale.shape)} on {scale.device}")
-    pitch = scale.stride(0)
-    if ((blocks > 1 and scale.stride(1) != 1) or pitch % 4 or pitch < blocks or pitch > cols or scale.data_ptr() % 4
+    pitch, step = scale.stride()
+    if ((blocks > 1 and step != 1) or pitch % 4 or pitch < blocks or pitch > cols or scale.data_ptr() % 4
             or scale.storage_offset() + (rows - 1) * pitch + -(-blocks // 4) * 4 > scale.untyped_storage().nbytes()):
         raise ValueError(f"{name} must have 4-byte aligned rows of adjacent scales, padded to a multiple of 4 bytes")
     return pitch
@@ -76,17 +76,18 @@ def _check_scale(scale: Tensor, name: str, rows: int, cols: int, device: torch.d
 
 def _check_weight(w: Fp8Weight, name: str, device: torch.device, transposed: bool = False) -> tuple[int, int]:
     """(pitch of the scales, of the transpose's or 0) of a weight in the 8-bit form."""
-    _check_codes(w.codes, f"{name}.codes", device)
-    n, k = w.codes.shape
-    pitch = _check_scale(w.scale, f"{name}.scale", _blocks(n), k, device)
+    codes, scale, codes_t, scale_t = w
+    _check_codes(codes, f"{name}.codes", device)
+    n, k = codes.shape
+    pitch = _check_scale(scale, f"{name}.scale", _blocks(n), k, device)
     if not transposed:
         return pitch, 0
-    if w.codes_t is None or w.scale_t is None:
+    if codes_t is None or scale_t is None:
         raise ValueError(f"{name} needs its transpose for training: quantize_weight(w, transpose=True)")
-    _check_codes(w.codes_t, f"{name}.codes_t", device)
-    if w.codes_t.shape != (k, n):
-        raise ValueError(f"{name}.codes_t must be {(k, n)}, got {tuple(w.codes_t.shape)}")
-    return pitch, _check_scale(w.scale_t, f"{name}.scale_t", _blocks(k), n, device)
+    _check_codes(codes_t, f"{name}.codes_t", device)
+    if codes_t.shape != (k, n):
+        raise ValueError(f"{name}.codes_t must be {(k, n)}, got {tuple(codes_t.shape)}")
+    return pitch, _check_scale(scale_t, f"{name}.scale_t", _blocks(k), n, device)
 
 
 def _as_rows(x: Tensor, name: str, dtypes: tuple, of: int = 16) -> Tensor:
@@ -202,30 +203,46 @@ def _serving_input(x: Tensor, weight: Fp8Weight, name: str) -> Tensor:
     return rows
 
 
+def _workspace(x: Tensor, need: int) -> Tensor:
+    return torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)   # an unsupported size: refused by the call
+
+
 def fp8_linear(x: Tensor, weight: Fp8Weight) -> Tensor:
     """x bf16 [..., K] through a linear layer whose weight [N, K] is held in 8 bits: bf16 [..., N]. Each row of x is taken in
     its 8-bit form. For serving: no gradient (checkpointed_linear has one)."""
     rows = _serving_input(x, weight, "fp8_linear")
-    _check_weight(weight, "weight", x.device)
-    _outputs(weight.codes.size(0), "weight")
+    pitch, _ = _check_weight(weight, "weight", x.device)
+    (m, k), n = rows.shape, weight.codes.size(0)
+    _outputs(n, "weight")
     with device_guard(x):
-        out = _product(*_quantize(rows), weight.codes, weight.scale)
-    return out.view(*x.shape[:-1], out.size(1))
+        lib = hip_library()
+        out, stride, ws, need = torch.empty(m, n, dtype=BF16, device=x.device), rows.stride(0), None, 0
+        if m > 16 or rows.data_ptr() % 16 or (m > 1 and (stride % 8 or stride > 1 << 22)):
+            need = lib.nc_fp8_linear_workspace_bytes(m, k)
+            ws = _workspace(x, need)
+        check(lib.nc_fp8_linear(rows.data_ptr(), 0, stride, weight.codes.data_ptr(), weight.scale.data_ptr(), pitch, m, n, k,
+                                out.data_ptr(), None if ws is None else ws.data_ptr(), need, stream()))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 
 def fp8_mlp(x: Tensor, fc: Fp8Weight, proj: Fp8Weight) -> Tensor:
     """x bf16 [..., C] through proj(relu(fc(x))^2), fc [F, C] and proj [N, F] held in 8 bits: bf16 [..., N]. The squared
     activations are taken in their 8-bit form from fp32 sums. For serving: no gradient (checkpointed_mlp has one)."""
     rows = _serving_input(x, fc, "fp8_mlp")
-    _check_weight(fc, "fc", x.device)
-    _check_weight(proj, "proj", x.device)
-    if proj.codes.size(1) != fc.codes.size(0):
+    fc_pitch, _ = _check_weight(fc, "fc", x.device)
+    proj_pitch, _ = _check_weight(proj, "proj", x.device)
+    (m, c), (n, hidden) = rows.shape, proj.codes.shape
+    if hidden != fc.codes.size(0):
         raise ValueError(f"proj {tuple(proj.codes.shape)} does not take fc's {fc.codes.size(0)} outputs")
-    _outputs(proj.codes.size(0), "proj")
+    _outputs(n, "proj")
     with device_guard(x):
-        act = _product_relu2(*_quantize(rows), fc.codes, fc.scale)
-        out = _product(*act, proj.codes, proj.scale)
-    return out.view(*x.shape[:-1], out.size(1))
+        lib = hip_library()
+        need = lib.nc_fp8_mlp_workspace_bytes(m, c, hidden)
+        out, ws = torch.empty(m, n, dtype=BF16, device=x.device), _workspace(x, need)
+        check(lib.nc_fp8_mlp(rows.data_ptr(), rows.stride(0), fc.codes.data_ptr(), fc.scale.data_ptr(), fc_pitch,
+                             proj.codes.data_ptr(), proj.scale.data_ptr(), proj_pitch, m, c, hidden, n, out.data_ptr(),
+                             ws.data_ptr(), need, stream()))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 
 # --- training
@@ -239,7 +256,7 @@ def _weight_grad(dy: Tensor, codes: Tensor, scale: Tensor, out: Tensor, mode: in
         return out if mode == _GRAD_ADD else out.zero_()
     lib = hip_library()
     need = lib.nc_fp8_weight_grad_workspace_bytes(rows, n1, n2)
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dy.device)   # an unsupported size: refused by the call
+    ws = _workspace(dy, need)
     check(lib.nc_fp8_weight_grad(pointer(dy), pointer(codes), pointer(scale), scale.stride(0), rows, n1, n2, mode,
                                  pointer(out), pointer(ws), need, stream()))
     return out

@@ -29,7 +29,7 @@ LIBRARY = LIB_DIR / "libnanochat_kv.so"
 DECODE_LIBRARY = LIB_DIR / "libnanochat_decode.so"
 KERNEL_SOURCES = [CSRC / "kv_append.hip", CSRC / "attention.hip", CSRC / "ve_gate.hip", CSRC / "flash_attn.hip",
                   CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip", CSRC / "paging.hip", CSRC / "sample.hip", CSRC / "packed_attn.hip",
-                  CSRC / "fp8_quant.hip", CSRC / "fp8_gemm.hip", CSRC / "fp8_grad.hip"]
+                  CSRC / "fp8_quant.hip", CSRC / "fp8_gemm.hip", CSRC / "fp8_grad.hip", CSRC / "fp8_skinny.hip"]
 DECODE_SOURCES = [CSRC / "decoder.hip", CSRC / "slot_gemm.hip"]
 SOURCES = KERNEL_SOURCES + DECODE_SOURCES
 HEADERS = [CSRC / "nc_device.h", CSRC / "nc_internal.h", CSRC / "nc_row.h", CSRC / "nc_attend.h", CSRC / "nc_meeting.h",
@@ -140,6 +140,12 @@ SIGNATURES = {
                              c_void_p, c_longlong, c_void_p], c_int),
     "nc_fp8_matmul_relu2_bwd": ([c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_void_p,
                                  c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_void_p], c_int),
+    "nc_fp8_linear_workspace_bytes": ([c_longlong, c_int], c_longlong),
+    "nc_fp8_linear": ([c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p,
+                       c_longlong, c_void_p], c_int),
+    "nc_fp8_mlp_workspace_bytes": ([c_longlong, c_int, c_int], c_longlong),
+    "nc_fp8_mlp": ([c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int,
+                    c_void_p, c_void_p, c_longlong, c_void_p], c_int),
     "nc_fp8_weight_grad_workspace_bytes": ([c_longlong, c_int, c_int], c_longlong),
     "nc_fp8_weight_grad": ([c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p,
                             c_longlong, c_void_p], c_int),

@@ -112,6 +112,40 @@ def test_products_refuse(lib):
         assert lib.nc_fp8_matmul_relu2_bwd(*args, *rest, None) == bad, i
 
 
+def linear_args(**over):
+    return list((dict(x=DUMMY, f32=0, stride=256, w=DUMMY, w_scale=DUMMY, w_pitch=4, rows=40, n=32, k=256, out=DUMMY, ws=DUMMY,
+                      bytes=2 ** 20, stream=None) | over).values())
+
+
+def mlp_args(**over):
+    return list((dict(x=DUMMY, stride=256, fc=DUMMY, fc_scale=DUMMY, fc_pitch=4, proj=DUMMY, proj_scale=DUMMY, proj_pitch=4, rows=40,
+                      c=256, hidden=512, n=32, out=DUMMY, ws=DUMMY, bytes=2 ** 20, stream=None) | over).values())
+
+
+def test_serving_refuses(lib):
+    for name in ("x", "w", "w_scale", "out", "ws"):
+        assert lib.nc_fp8_linear(*linear_args(**{name: None})) == -1, name
+    odd = ctypes.c_void_p(0x1008)
+    for over in (dict(rows=-1), dict(n=0), dict(n=40), dict(k=0), dict(k=72), dict(n=2 ** 20 + 16), dict(k=2 ** 20 + 16),
+                 dict(rows=2 ** 30), dict(stride=255), dict(w_pitch=1), dict(w_pitch=6), dict(w=odd), dict(out=odd),
+                 dict(x=ctypes.c_void_p(0x1001)), dict(x=ctypes.c_void_p(0x1002), f32=1)):
+        assert lib.nc_fp8_linear(*linear_args(**over)) == -2, over
+    need = lib.nc_fp8_linear_workspace_bytes(40, 256)
+    assert need >= 40 * 256 + 40 * 2 and lib.nc_fp8_linear(*linear_args(bytes=need - 1)) == -3
+    assert lib.nc_fp8_linear(*linear_args(ws=odd)) == -3 and lib.nc_fp8_linear(*linear_args(rows=0)) == 0
+    for few in (dict(x=odd, ws=None), dict(rows=16, stride=257, ws=None), dict(rows=9, f32=1, ws=None)):   # these need it
+        assert lib.nc_fp8_linear(*linear_args(**(dict(rows=2) | few))) == -1, few
+    assert lib.nc_fp8_linear_workspace_bytes(1, 24) == -1 and lib.nc_fp8_linear_workspace_bytes(-1, 16) == -1
+    for name in ("x", "fc", "fc_scale", "proj", "proj_scale", "out", "ws"):
+        assert lib.nc_fp8_mlp(*mlp_args(**{name: None})) == -1, name
+    for over in (dict(rows=-1), dict(c=0), dict(c=40), dict(hidden=500), dict(n=20), dict(hidden=2 ** 20 + 16), dict(stride=255),
+                 dict(fc_pitch=1), dict(proj_pitch=2), dict(fc=odd), dict(proj=odd), dict(out=odd)):
+        assert lib.nc_fp8_mlp(*mlp_args(**over)) == -2, over
+    need = lib.nc_fp8_mlp_workspace_bytes(40, 256, 512)
+    assert lib.nc_fp8_mlp(*mlp_args(bytes=need - 1)) == -3 and lib.nc_fp8_mlp(*mlp_args(ws=odd)) == -3
+    assert lib.nc_fp8_mlp(*mlp_args(rows=0)) == 0 and lib.nc_fp8_mlp_workspace_bytes(40, 256, 500) == -1
+
+
 def test_weight_gradient_refuses(lib):
     for name in ("dy", "codes", "scale", "out", "ws"):
         assert lib.nc_fp8_weight_grad(*grad_args(**{name: None})) == -1, name

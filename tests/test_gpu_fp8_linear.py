@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from nanochat_amd import fp8_linear as fl
+from nanochat_amd.native import hip_library, stream
 from oracle import fp8_block as fb
 
 pytestmark = pytest.mark.gpu
@@ -231,6 +232,77 @@ def test_serving_layers(device, rows):
     close(codes_of(z), a @ pv.T, err @ np.abs(pv).T + 2.0 ** -8 * np.abs(a @ pv.T) + (2.0 ** -10 + 1040 * EPS) * ((a + err) @ np.abs(pv).T))
     exact = fb.through(a, 1) @ pv.T
     assert np.linalg.norm(codes_of(z) - exact) <= 2.0 ** -6 * np.linalg.norm(exact)
+
+
+# rows of w and of x a workgroup takes: by the number of rows of x and of (16 rows of w) x (32 of x) against the CUs (256)
+FEW = [(rows, 400, 2064) for rows in (1, 2, 8, 9, 15, 16, 17, 31, 32, 33, 100, 127, 128)]
+FEW += [(1, 16, 20000), (16, 33024, 144), (3, 4992, 400), (20, 48, 16400), (20, 4800, 272), (32, 33024, 144), (40, 4816, 144),
+        (64, 2064, 1296), (97, 9616, 144), (128, 33040, 272), (128, 16, 16384), (77, 16, 16)]
+
+
+@pytest.mark.parametrize("rows,n,k", FEW)
+def test_few_rows(device, rows, n, k):
+    """Up to 128 rows, which read the weight once: from rows of any alignment, from codes, and with nothing written behind them."""
+    gen = torch.Generator().manual_seed(rows + n + k)
+    x = rowwise(gen, rows, k)
+    w, wv = weight(gen, device, n, k)
+    x8 = fb.through(x.double().numpy(), 1)
+    want, mag = x8 @ wv.T, np.abs(x8) @ np.abs(wv).T
+    slack = 2.0 ** -8 * np.abs(want) + (2.0 ** -10 + k * EPS) * mag
+    odd = torch.zeros(rows, k + 3, dtype=BF16, device=device)
+    odd[:, 1:k + 1] = x.to(device)
+    padded = torch.full((rows, k + 24), float("nan"), dtype=BF16, device=device)
+    padded[:, 16:k + 16] = x.to(device)
+    for y in (fl.fp8_linear(x.to(device), w), fl.fp8_linear(odd[:, 1:k + 1], w), fl.fp8_linear(padded[:, 16:k + 16], w),
+              fl.fp8_matmul(*fl.quantize_rows(x.to(device)), w)):
+        close(codes_of(y), want, slack)
+        assert np.linalg.norm(codes_of(y) - want) <= 2.0 ** -8 * np.linalg.norm(want)
+    lib, out = hip_library(), torch.full((rows + 1, n), 7.0, dtype=BF16, device=device)
+    xd, xf = x.to(device), x.float().to(device)
+    for t, f32 in ((xd, 0), (xf, 1)):
+        need = lib.nc_fp8_linear_workspace_bytes(rows, k)
+        ws = torch.full((need + 64,), 9, dtype=torch.uint8, device=device)
+        assert lib.nc_fp8_linear(t.data_ptr(), f32, k, w.codes.data_ptr(), w.scale.data_ptr(), w.scale.stride(0), rows, n, k,
+                                 out.data_ptr(), ws.data_ptr(), need, stream()) == 0
+        close(codes_of(out[:rows]), want, slack)
+        assert bool((out[rows] == 7).all()) and bool((ws[need:] == 9).all())
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17, 33, 128])
+@pytest.mark.parametrize("c,hidden,n", [(400, 2064, 144), (144, 9616, 32), (1280, 528, 4816)])
+def test_few_rows_mlp(device, rows, c, hidden, n):
+    """An MLP's squared activations from exact products: their codes are those of float64's, but for values that lie on the border
+    of two codes, and the result is off by its own rounding alone."""
+    gen = torch.Generator().manual_seed(rows + c + n)
+    x = rowwise(gen, rows, c)
+    fc, fcv = weight(gen, device, hidden, c)
+    proj, pv = weight(gen, device, n, hidden)
+    want = fb.through(np.maximum(fb.through(x.double().numpy(), 1) @ fcv.T, 0.0) ** 2, 1) @ pv.T
+    lib, out = hip_library(), torch.full((rows + 1, n), 7.0, dtype=BF16, device=device)
+    need = lib.nc_fp8_mlp_workspace_bytes(rows, c, hidden)
+    ws, xd = torch.full((need + 64,), 9, dtype=torch.uint8, device=device), x.to(device)
+    assert lib.nc_fp8_mlp(xd.data_ptr(), c, fc.codes.data_ptr(), fc.scale.data_ptr(), fc.scale.stride(0), proj.codes.data_ptr(),
+                          proj.scale.data_ptr(), proj.scale.stride(0), rows, c, hidden, n, out.data_ptr(), ws.data_ptr(), need,
+                          stream()) == 0
+    assert bool((out[rows] == 7).all()) and bool((ws[need:] == 9).all())
+    z = fl.fp8_mlp(xd, fc, proj)
+    assert torch.equal(z, out[:rows])
+    assert np.linalg.norm(codes_of(z) - want) <= 2.0 ** -8 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("rows", [5, 12, 40, 140])
+def test_rows_that_are_not_finite(device, rows):
+    """A NaN or an infinity makes its own row NaN and no other."""
+    gen = torch.Generator().manual_seed(rows)
+    x = rowwise(gen, rows, 400).to(device)
+    w, fc, proj = (weight(gen, device, *s)[0] for s in ((272, 400), (640, 400), (144, 640)))
+    y, z = fl.fp8_linear(x, w), fl.fp8_mlp(x, fc, proj)
+    bad = x.clone()
+    bad[1, 7], bad[3, 300] = float("nan"), float("inf")
+    ill = torch.zeros(rows, dtype=torch.bool, device=device)
+    ill[1] = ill[3] = True
+    for got, want in ((fl.fp8_linear(bad, w), y), (fl.fp8_mlp(bad, fc, proj), z)):
+        assert bool(got[ill].isnan().all()) and torch.equal(got[~ill], want[~ill])
 
 
 # --- weight gradients
