@@ -386,10 +386,11 @@ int nc_fp8_matmul_relu2_bwd(const void *a, const void *a_scale, long long a_scal
 /* A layer, out = x8 w^T, and a ReLU^2 MLP, out = a8 proj^T with a = relu(x8 fc^T)^2, for serving: x8, a8 the 8-bit forms of x's
  * rows (bf16, or fp32 for a layer with is_f32; [rows][k] at row_stride elements, any alignment of its type) and of the squares of the
  * fp32 sums, w [n][k], fc [hidden][c] and proj [n][hidden] held in 8 bits, out bf16 [rows][n], all widths multiples of 16 up to 2^20.
- * Up to 128 rows are bound by reading the weights once, and up to 16 with 16-byte aligned rows are one launch a product. workspace:
- * nc_fp8_*_workspace_bytes (-1 for unsupported sizes), 16-byte aligned, need not be cleared; it may be NULL for a layer of up to 16
- * bf16 or 8 fp32 rows that are 16-byte aligned and at most 2^22 elements apart. A call's workspace is its own until it has run. */
-long long nc_fp8_linear_workspace_bytes(long long rows, int k);
+ * A few rows are bound by reading the weights once; up to 16 that can be read 16 bytes at a time, on few enough outputs, are one
+ * launch a product. workspace: nc_fp8_*_workspace_bytes (-1 for unsupported sizes; of a layer, for the x and row_stride of the call,
+ * and 0 where none is read: it may then be NULL), 16-byte aligned, need not be cleared. A call's workspace is its own until it has
+ * run. */
+long long nc_fp8_linear_workspace_bytes(const void *x, int is_f32, long long row_stride, long long rows, int n, int k);
 int nc_fp8_linear(const void *x, int is_f32, long long row_stride, const void *w, const void *w_scale, int w_scale_stride,
                   long long rows, int n, int k, void *out, void *workspace, long long workspace_bytes, void *stream);
 long long nc_fp8_mlp_workspace_bytes(long long rows, int c, int hidden);

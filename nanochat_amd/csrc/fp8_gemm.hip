@@ -29,8 +29,6 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef __amdgpu_buffer_rsrc_t Rsrc;
-typedef __attribute__((address_space(3))) void LdsPtr;
 
 constexpr int FG_ROWB = F8_BLOCK;        /* bytes of a row of a stage: one block */
 constexpr int FG_PAST = 0x7FFF0000;      /* a byte offset past every operand's range */
@@ -50,14 +48,14 @@ struct F8Gemm {
     long long qs_stride, act_stride;
 };
 
-template <int NU_, int WN_, int WM_> struct FgTile {
-    static constexpr int NU = NU_, WN = WN_, WM = WM_, WAVES = WN * WM, TM = 16 * NU * WM, TN = F8_BLOCK * WN;
+template <int NU_, int WN_, int WM_, int RING_> struct FgTile {
+    static constexpr int NU = NU_, WN = WN_, WM = WM_, RING = RING_, WAVES = WN * WM, TM = 16 * NU * WM, TN = F8_BLOCK * WN;
     static constexpr int ROWS = TM + TN, STAGE = ROWS * FG_ROWB, LOADS = ROWS / 8 / WAVES, A_LOADS = TM / 8 / WAVES;
     static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0, "DMA split");
 };
-typedef FgTile<4, 2, 4> FgFull;      /* 256 x 256, 8 waves */
-typedef FgTile<2, 1, 4> FgHalf;      /* 128 x 128, 4 waves */
-typedef FgTile<1, 1, 4> FgSmall;     /* 64 x 128, 4 waves */
+typedef FgTile<4, 2, 4, 2> FgFull;   /* 256 x 256, 8 waves, two stages in LDS */
+typedef FgTile<2, 1, 4, 2> FgHalf;   /* 128 x 128, 4 waves */
+typedef FgTile<1, 1, 4, 3> FgSmall;  /* 64 x 128, 4 waves */
 
 /* A 16-byte LDS read serves lanes 0-3, 12-15, 20-23 and 24-27 together, then 4-11, 16-19 and 28-31, and so the upper half. Two
  * rows lie side by side over the 64 banks, so 8 rows of one parity, four of one 16-byte piece b and four of b ^ 2, need 8
@@ -80,16 +78,11 @@ __device__ __forceinline__ void fg_barrier() {
     asm volatile("" ::: "memory");
 }
 
-template <class P>
-__device__ __forceinline__ void fg_fetch(Rsrc ra, Rsrc rw, unsigned char *buf, int j, int K, int wave, int lane) {
-    const int pos = lane & 7;
-#pragma unroll
-    for (int s = 0; s < P::LOADS; s++) {
-        const bool is_a = s < P::A_LOADS;
-        const int q = wave + P::WAVES * s, row = 8 * q + (lane >> 3) - (is_a ? 0 : P::TM);
-        const int piece = pos ^ (is_a ? fg_swizzle_a(row) : fg_swizzle_w(row)), col = j * FG_ROWB + 16 * piece;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(is_a ? ra : rw, (LdsPtr *)(buf + q * 1024), 16,
-                                                 col < K ? row * K + col : FG_PAST, 0, 0, 0);
+template <int I> struct FgIndex { static constexpr int value = I; };
+template <int N, int I = 0, class F> __device__ __forceinline__ void fg_unroll(F &&f) {
+    if constexpr (I < N) {
+        f(FgIndex<I>{});
+        fg_unroll<N, I + 1>(f);
     }
 }
 
@@ -98,20 +91,45 @@ __device__ __forceinline__ i32x8 fg_operand(const unsigned char *buf, int lo, in
     return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
 }
 
-/* A stage's products; BYTE: which byte of the scale dwords is its block's. */
-template <class P, int BYTE>
+/* A stage's products; BYTE: which byte of the scale dwords is its block's. EXACT: from the values in bf16, four instructions in
+ * place of one (codes 8 Q .. + 7 of each lane's 32 in instruction Q). */
+template <int BYTE> __device__ __forceinline__ float fg_scale(uint32_t s) { return f8_scale((s >> (8 * BYTE)) & 0xFFu); }
+template <int Q> __device__ __forceinline__ bf16x8 fg_values(const i32x8 &c, float s) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[2 * Q + i], s, false));
+        o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[2 * Q + i], s, true));
+    }
+    return __builtin_bit_cast(bf16x8, o);
+}
+template <class P, int BYTE, bool EXACT>
 __device__ __forceinline__ void fg_compute(const unsigned char *buf, f32x4 (&acc)[8][P::NU], const uint32_t (&sa)[P::NU],
                                            uint32_t sw, int a_at, int w_at) {
     i32x8 fb[P::NU];
 #pragma unroll
     for (int u = 0; u < P::NU; u++) fb[u] = fg_operand(buf, a_at + u * 16 * FG_ROWB, (a_at ^ 16) + u * 16 * FG_ROWB);
+    if constexpr (EXACT) {
+        static_assert(P::NU == 1, "one operand of a");
+        const float s = fg_scale<BYTE>(sa[0]), t_s = fg_scale<BYTE>(sw);
+        bf16x8 b[4];
+        fg_unroll<4>([&](auto q) { b[decltype(q)::value] = fg_values<decltype(q)::value>(fb[0], s); });
 #pragma unroll
-    for (int t = 0; t < 8; t++) {
-        const i32x8 fa = fg_operand(buf, w_at + fg_column(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column(t, 0) * FG_ROWB);
+        for (int t = 0; t < 8; t++) {
+            const i32x8 fa = fg_operand(buf, w_at + fg_column(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column(t, 0) * FG_ROWB);
+            fg_unroll<4>([&](auto q) {
+                acc[t][0] = mfma16x16x32(fg_values<decltype(q)::value>(fa, t_s), b[decltype(q)::value], acc[t][0]);
+            });
+        }
+    } else {
 #pragma unroll
-        for (int u = 0; u < P::NU; u++)
-            acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb[u], acc[t][u], 0, 0, BYTE, (int)sw, BYTE,
-                                                                         (int)sa[u]);
+        for (int t = 0; t < 8; t++) {
+            const i32x8 fa = fg_operand(buf, w_at + fg_column(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column(t, 0) * FG_ROWB);
+#pragma unroll
+            for (int u = 0; u < P::NU; u++)
+                acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fa, fb[u], acc[t][u], 0, 0, BYTE, (int)sw, BYTE,
+                                                                             (int)sa[u]);
+        }
     }
 }
 
@@ -140,69 +158,64 @@ __device__ __forceinline__ FgPlace fg_place(const F8Gemm &g, long long m0, int n
     return p;
 }
 
-/* The scale dwords (four blocks) of a wave's operands: of its rows of a by lane, of its block of w. */
-template <class P> struct FgScales {
-    Rsrc rs;
-    int at, step;
-    Rsrc rw;
-    uint32_t a[P::NU], w, next_a[P::NU], next_w;
-    __device__ __forceinline__ FgScales(const F8Gemm &g, const FgPlace &p, long long m0) {
-        rs = f8_rsrc(g.as + m0 * g.as_stride, p.rows * g.as_stride);
-        at = p.row0 * (int)g.as_stride;
-        step = 16 * (int)g.as_stride;
-        rw = f8_rsrc(g.ws + (long long)(p.some ? p.nb : 0) * g.ws_stride, g.ws_stride);
-    }
-    __device__ __forceinline__ void fetch(int group) {
-        next_w = __builtin_amdgcn_raw_buffer_load_b32(rw, 4 * group, 0, 0);   /* the same for all lanes */
+/* The K walk of the smaller tiles, four waves: P::RING stages in LDS, the DMA of RING - 1 ahead. Each wave moves 8 rows of every 32,
+ * and every fourth stage the scale dwords of its own operands' next four blocks (its rows of a by lane, its block of w). */
+constexpr int FG_OWN = 512;   /* bytes of a wave's scales of four stages: 64 dwords of a, then w's */
+template <class P, bool EXACT>
+__device__ __forceinline__ void fg_walk_ring(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *lds,
+                                             f32x4 (&acc)[8][P::NU]) {
+    const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK, K = g.K;
+    const u32x4 ra = f8_words(g.a + m0 * K, (long long)p.rows * K), rw = f8_words(g.w + (long long)n0 * K, (long long)p.cols * K);
+    const u32x4 rsa = f8_words(g.as + m0 * g.as_stride, p.rows * g.as_stride);
+    const u32x4 rsw = f8_words(g.ws + (long long)p.nb * g.ws_stride, g.ws_stride);
+    const uint32_t base = f8_lds(lds) + p.wave * 1024;
+    unsigned char *const scales = lds + P::RING * P::STAGE + p.wave * 2 * FG_OWN;
+    const uint32_t scale_to = f8_lds(scales);
+    const int row = 8 * p.wave + (p.lane >> 3), first = row * K;   /* rows 32 on have the same pieces */
+    const int ca = ((p.lane & 7) ^ fg_swizzle_a(row)) << 4, cw = ((p.lane & 7) ^ fg_swizzle_w(row)) << 4;
+    const int scale_at = p.lane < 16 * P::NU ? (16 * P::NU * p.wm + p.lane) * (int)g.as_stride : FG_PAST;
+    const auto fetch = [&](int j, int slot) {   /* a stage past the last: zeros, without an access */
+        const int k = j * FG_ROWB;
+        const int oa = k + ca < K ? first + ca + k : FG_PAST, ow = k + cw < K ? first + cw + k : FG_PAST;
+        const uint32_t to = base + slot * P::STAGE;
+        if ((j & 3) == 0) {
+            f8_dma4(scale_to + ((j >> 2) & 1) * FG_OWN, scale_at + j, rsa);
+            f8_dma4(scale_to + ((j >> 2) & 1) * FG_OWN + 256, j, rsw);
+        }
 #pragma unroll
-        for (int u = 0; u < P::NU; u++) next_a[u] = __builtin_amdgcn_raw_buffer_load_b32(rs, at + u * step + 4 * group, 0, 0);
-    }
-    __device__ __forceinline__ void shift() {   /* the next block's byte lowest */
-        w >>= 8;
+        for (int s = 0; s < P::A_LOADS; s++) f8_dma16(to + 4096 * s, oa + 32 * s * K, ra);
 #pragma unroll
-        for (int u = 0; u < P::NU; u++) a[u] >>= 8;
-    }
-    __device__ __forceinline__ void turn() {
-        w = next_w;
+        for (int s = 0; s < P::LOADS - P::A_LOADS; s++) f8_dma16(to + 4096 * (P::A_LOADS + s), ow + 32 * s * K, rw);
+    };
 #pragma unroll
-        for (int u = 0; u < P::NU; u++) a[u] = next_a[u];
-    }
-};
-
-/* Stage j from CUR, its successor's DMA into OTHER. */
-#define FG_STEP(j, BYTE, CUR, OTHER)                                              \
-    do {                                                                           \
-        if ((j) < stages) {                                                        \
-            __builtin_amdgcn_s_waitcnt(0);                                         \
-            fg_barrier();                                                          \
-            if ((j) + 1 < stages) fg_fetch<P>(ra, rw, OTHER, (j) + 1, g.K, p.wave, p.lane); \
-            fg_compute<P, BYTE>(CUR, acc, sc.a, sc.w, a_at, w_at);                 \
-        }                                                                          \
-    } while (0)
-
-/* The K walk of the smaller tiles: two or more workgroups a CU, each with a wave a SIMD, run beside one another. */
-template <class P>
-__device__ __forceinline__ void fg_walk_simple(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0,
-                                               unsigned char *b1, f32x4 (&acc)[8][P::NU]) {
-    const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
-    const Rsrc ra = f8_rsrc(g.a + m0 * g.K, (long long)p.rows * g.K);
-    const Rsrc rw = f8_rsrc(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
-    FgScales<P> sc(g, p, m0);
-    sc.fetch(0);
-    fg_fetch<P>(ra, rw, b0, 0, g.K, p.wave, p.lane);
+    for (int j = 0; j < P::RING - 1; j++) fetch(j, j);
     const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
-    const int w_row = F8_BLOCK * p.wn + fg_column(0, p.i >> 2) + (p.i & 3);
+    const int w_row = fg_column(0, p.i >> 2) + (p.i & 3);
     const int w_at = (P::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
-    for (int j = 0; j < stages; j += 4) {
-        sc.turn();
-        if (j + 4 < stages) sc.fetch(j / 4 + 1);
-        FG_STEP(j, 0, b0, b1);
-        FG_STEP(j + 1, 1, b1, b0);
-        FG_STEP(j + 2, 2, b0, b1);
-        FG_STEP(j + 3, 3, b1, b0);
-    }
+    uint32_t sa[P::NU], sw = 0;
+    int slot = 0, last = P::RING - 1;
+    for (int j0 = 0; j0 < stages; j0 += 4)
+        fg_unroll<4>([&](auto which) {
+            constexpr int BYTE = decltype(which)::value;
+            const int j = j0 + BYTE;
+            if (j >= stages) return;
+            /* all but the RING - 2 newest stages has landed, and what this wave read of the slot filled next is in registers */
+            constexpr int NEWER = (P::RING - 2) * P::LOADS + 2 * ((BYTE + P::RING - 2) / 4);
+            __builtin_amdgcn_s_waitcnt((NEWER & 0xF) | ((NEWER >> 4) << 14) | (0x7 << 4) | (0x0 << 8));
+            fg_barrier();
+            fetch(j + P::RING - 1, last);
+            if constexpr (BYTE == 0) {
+                const unsigned char *own = scales + ((j >> 2) & 1) * FG_OWN;
+#pragma unroll
+                for (int u = 0; u < P::NU; u++) sa[u] = *(const uint32_t *)(own + 4 * (16 * u + p.i));
+                sw = *(const uint32_t *)(own + 256);
+            }
+            fg_compute<P, BYTE, EXACT>(lds + slot * P::STAGE, acc, sa, sw, a_at, w_at);
+            last = slot;
+            slot = slot + 1 == P::RING ? 0 : slot + 1;
+        });
     __builtin_amdgcn_s_waitcnt(0);
-    fg_barrier();   /* the epilogue writes where other waves may still read */
+    fg_barrier();   /* the epilogue writes where other waves may still read and DMA may still land */
 }
 
 /* The K walk of the full tile: waves 0-3 and 4-7, one of each a SIMD, take turns: while one's 32 products keep the matrix core
@@ -261,14 +274,6 @@ struct FgDma {
         f8_dma16(to + S * 8192, (S < 4 ? oa : ow) + 64 * (S & 3) * K, S < 4 ? ra : rw);
     }
 };
-
-template <int I> struct FgIndex { static constexpr int value = I; };
-template <int N, int I = 0, class F> __device__ __forceinline__ void fg_unroll(F &&f) {
-    if constexpr (I < N) {
-        f(FgIndex<I>{});
-        fg_unroll<N, I + 1>(f);
-    }
-}
 
 __device__ __forceinline__ void fg_phase_end() {
     __builtin_amdgcn_sched_barrier(0);
@@ -349,9 +354,6 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
 
 /* A wave's part of LDS behind its walk: 16 rows of 256 bytes, then 16 of 128. */
 constexpr int FG_TURN = 16 * 384;
-#ifndef FG_CODE_STORE
-#define FG_CODE_STORE(d, p) __builtin_nontemporal_store(d, p)
-#endif
 __device__ __forceinline__ int fg_code_place(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 /* Lanes of one wave exchange values through LDS, which serves a wave's accesses in order; the compiler keeps the order too. */
 __device__ __forceinline__ void fg_wave_order() {
@@ -360,7 +362,7 @@ __device__ __forceinline__ void fg_wave_order() {
 }
 
 template <class P, int EPI>
-__device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, unsigned char *b0, unsigned char *b1) {
+__device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, unsigned char *b0) {
     const FgPlace p = fg_place<P>(g, m0, n0);
     f32x4 acc[8][P::NU];
 #pragma unroll
@@ -368,7 +370,7 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
 #pragma unroll
         for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (P::WAVES == 8) fg_walk_full(g, p, m0, n0, b0, acc);
-    else fg_walk_simple<P>(g, p, m0, n0, b0, b1, acc);
+    else fg_walk_ring<P, P::NU == 1 && EPI == FG_RELU2>(g, p, m0, n0, b0, acc);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));   /* made again, not kept through the walk */
     const int grp = (tid & (WAVE - 1)) >> 4;
@@ -485,7 +487,7 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
                 const int r = 8 * k + (lane >> 3), c = lane & 7;
                 const u32x4 d = *(const u32x4 *)(codes + fg_code_place(r, c));
                 if (16 * u + r < rows_left && col + 16 * c < cols)
-                    FG_CODE_STORE(d, (u32x4 *)(g.q + (first + 16 * u + r) * g.N + n0 + col + 16 * c));
+                    __builtin_nontemporal_store(d, (u32x4 *)(g.q + (first + 16 * u + r) * g.N + n0 + col + 16 * c));
             }
         }
     }
@@ -502,10 +504,9 @@ __device__ __forceinline__ int2 fg_tile(int l, int count, int nx) {
 
 template <class P, int EPI>
 __global__ void __launch_bounds__(P::WAVES *WAVE, 2) fp8_gemm_kernel(F8Gemm g) {
-    /* the smaller tiles: distinct objects, as reads of one do not wait for the other's DMA */
-    __shared__ __align__(16) unsigned char b0[P::WAVES == 8 ? 2 * P::STAGE + 2 * FG_SCALES : P::STAGE], b1[P::WAVES == 8 ? 16 : P::STAGE];
+    __shared__ __align__(16) unsigned char lds[P::RING * P::STAGE + (P::WAVES == 8 ? 2 * FG_SCALES : P::WAVES * 2 * FG_OWN)];
     const int2 t = fg_tile(blockIdx.x, gridDim.x, (g.N + P::TN - 1) / P::TN);
-    fg_run<P, EPI>(g, (long long)t.y * P::TM, t.x * P::TN, b0, b1);
+    fg_run<P, EPI>(g, (long long)t.y * P::TM, t.x * P::TN, lds);
 }
 
 template <class P>
@@ -539,16 +540,20 @@ int fg_check(const F8Gemm &g, int epi) {
     return NC_OK;
 }
 
+/* Small tiles while they all run at once; then by rounds, of a full tile a CU or of two halves, which take about 8 to 5 (full and
+ * half tiles of 1,664 k, us: 515 x 16,384 22.0, 25.0; 300 x 16,384 21.8, 13.7; 200 x 65,536 32.5, 38.9; 128 x 65,536 29.3, 25.9;
+ * 2,500 x 4,992 23.7, 27.6; 1,001 x 4,992 21.7, 13.4. Small and half: 256 x 4,992 7.7, 11.0; 128 x 16,384 8.2, 11.7; 515 x 4,992,
+ * 351 small ones, 11.6, 11.3; 300 x 16,384, 640, 18.5, 13.7). */
 int fg_gemm(const F8Gemm &g, int epi, void *stream) {
     const int e = fg_check(g, epi);
     if (e != NC_OK || g.M == 0) return e;
-    if (epi == FG_STORE && fp8_some_takes(g.M, g.K))
-        return fp8_some(g.a, g.as, g.as_stride, g.w, g.ws, g.ws_stride, (int)g.M, g.N, g.K, false, g.out, (hipStream_t)stream);
-    const long long full = (g.M + 255) / 256 * ((g.N + 255) / 256), half = (g.M + 127) / 128 * ((g.N + 127) / 128);
-    const int cus = device_cus();
-    if (full >= cus) return fg_launch<FgFull>(g, epi, (hipStream_t)stream);
-    if (half >= cus) return fg_launch<FgHalf>(g, epi, (hipStream_t)stream);
-    return fg_launch<FgSmall>(g, epi, (hipStream_t)stream);
+    const long long cus = device_cus(), full = (g.M + 255) / 256 * ((g.N + 255) / 256);
+    const long long half = (g.M + 127) / 128 * ((g.N + 127) / 128), small = (g.M + 63) / 64 * ((g.N + 127) / 128);
+    if (epi == FG_STORE && fp8_some_takes(g.M, g.N, g.K, cus))
+        return fp8_some(g.a, g.as, g.as_stride, g.w, g.ws, g.ws_stride, (int)g.M, g.N, g.K, g.out, (hipStream_t)stream);
+    if (small <= cus) return fg_launch<FgSmall>(g, epi, (hipStream_t)stream);
+    if (8 * ((full + cus - 1) / cus) <= 5 * ((half + 2 * cus - 1) / (2 * cus))) return fg_launch<FgFull>(g, epi, (hipStream_t)stream);
+    return fg_launch<FgHalf>(g, epi, (hipStream_t)stream);
 }
 
 }  // namespace

@@ -128,35 +128,23 @@ template <bool RELU2> __device__ __forceinline__ void sk_product(f32x4 &acc, con
                                                                (int)x.byte);
     }
 }
-template <bool RELU2> __device__ __forceinline__ float sk_result(float v) {
-    if constexpr (!RELU2) return v;
-    const float r = __builtin_elementwise_maximum(v, 0.0f);   /* a NaN stays one */
-    return r * r;
-}
-
-template <int XT, int RT, bool RELU2>
+template <int XT, bool RELU2>
 __global__ void __launch_bounds__(SK_WAVES *WAVE, 4) fp8_few_kernel(Skinny p) {
-    __shared__ __align__(16) f32x4 part[SK_WAVES][RT][WAVE];
+    __shared__ __align__(16) f32x4 part[SK_WAVES][WAVE];
     const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i16 = lane & 15;
-    const int n0 = blockIdx.x * 16 * RT, cols = min(p.N - n0, 16 * RT);
-    const Rsrc rw = f8_rsrc(p.w + (long long)n0 * p.K, (long long)cols * p.K);
+    const int n0 = blockIdx.x * 16;
+    const Rsrc rw = f8_rsrc(p.w + (long long)n0 * p.K, 16LL * p.K);
     const Rsrc rx = f8_rsrc(p.x, p.M * p.row_bytes);
-    const unsigned char *ws = p.ws + (long long)(n0 / F8_BLOCK) * p.ws_stride;   /* 16 RT rows lie in one block */
-    f32x4 acc[RT];
-#pragma unroll
-    for (int t = 0; t < RT; t++) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    constexpr int AHEAD = RT == 1 ? 3 : XT == SK_F32 ? 1 : 2;   /* blocks of w on their way beside the present one; one of x */
-    Raw<SK_CODES> w[AHEAD + 1][RT];
+    const unsigned char *ws = p.ws + (long long)(n0 / F8_BLOCK) * p.ws_stride;   /* 16 rows lie in one block */
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int AHEAD = 3;   /* blocks of w on their way beside the present one; one of x */
+    Raw<SK_CODES> w[AHEAD + 1];
     Raw<XT> x, next;
     const auto fetch = [&](int slot, int kb) {
         if (kb >= p.blocks) return;
-#pragma unroll
-        for (int t = 0; t < RT; t++) {
-            w[slot][t].load(rw, (unsigned)((16 * t + i16) * p.K), kb, g, p.K);
-            w[slot][t].byte = ws[kb];
-        }
+        w[slot].load(rw, (unsigned)(i16 * p.K), kb, g, p.K);
+        w[slot].byte = ws[kb];
     };
     const auto fetch_x = [&](int kb) {
         if (kb < p.blocks) next.load(rx, (unsigned)(i16 * p.row_bytes), kb, g, p.K);
@@ -172,29 +160,29 @@ __global__ void __launch_bounds__(SK_WAVES *WAVE, 4) fp8_few_kernel(Skinny p) {
             x = next;
             fetch_x(kb + SK_WAVES);
             fetch((a + AHEAD) % (AHEAD + 1), kb + SK_WAVES * AHEAD);
-            const Codes32 cx = x.codes();
-#pragma unroll
-            for (int t = 0; t < RT; t++) sk_product<RELU2>(acc[t], w[a][t].codes(), cx);
+            sk_product<RELU2>(acc, w[a].codes(), x.codes());
         }
     }
-#pragma unroll
-    for (int t = 0; t < RT; t++) part[wave][t][lane] = acc[t];
+    part[wave][lane] = acc;
     __syncthreads();
-    for (int t = wave; t < RT; t += SK_WAVES) {
-        f32x4 v = part[0][t][lane];
+    if (wave > 0 || i16 >= p.M) return;
+    f32x4 v = part[0][lane];   /* columns 4 g .. 4 g + 3 of row i16 */
 #pragma unroll
-        for (int s = 1; s < SK_WAVES; s++) {
-            const f32x4 o = part[s][t][lane];
+    for (int s = 1; s < SK_WAVES; s++) {
+        const f32x4 o = part[s][lane];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = v[e] + o[e];
+        for (int e = 0; e < 4; e++) v[e] = v[e] + o[e];
+    }
+    const long long at = (long long)i16 * p.N + n0 + 4 * g;
+    if constexpr (RELU2) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float r = __builtin_elementwise_maximum(v[e], 0.0f);   /* a NaN stays one */
+            v[e] = r * r;
         }
-        const int c = 16 * t + 4 * g;   /* columns c .. c + 3 of row i16 */
-        if (c >= cols || i16 >= p.M) continue;
-        const long long at = (long long)i16 * p.N + n0 + c;
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = sk_result<RELU2>(v[e]);
-        if constexpr (RELU2) *(f32x4 *)((float *)p.out + at) = v;
-        else *(u32x2 *)((uint16_t *)p.out + at) = u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+        *(f32x4 *)((float *)p.out + at) = v;
+    } else {
+        *(u32x2 *)((uint16_t *)p.out + at) = u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
     }
 }
 
@@ -207,9 +195,10 @@ __device__ __forceinline__ int sk_swizzle(int row) {
 
 /* Step j: blocks j S + s of k. */
 constexpr int SK_BLOCKS = 128;   /* of a row at most: their scales are kept in LDS */
-template <int MT, int RW, int S, bool RELU2>
-__global__ void __launch_bounds__(SK_WAVES *WAVE, S *MT >= 16 ? 2 : 4) fp8_some_kernel(Skinny p) {
+template <int RW, int S>
+__global__ void __launch_bounds__(SK_WAVES *WAVE, S == 8 ? 2 : 4) fp8_some_kernel(Skinny p) {
     static_assert(RW * S == SK_WAVES, "waves");
+    constexpr int MT = 2;   /* 32 rows of x */
     constexpr int BLOCK = 16 * MT * F8_BLOCK, STEP = S * BLOCK;              /* bytes of x in LDS: of a block, of a step */
     constexpr int RING = STEP <= 16384 ? 4 : 3, DMAS = STEP / 1024 / SK_WAVES;
     constexpr int SUMS = SK_WAVES * MT * 1024, COLS = 16 * RW, PITCH = SK_BLOCKS + 4;
@@ -286,7 +275,7 @@ __global__ void __launch_bounds__(SK_WAVES *WAVE, S *MT >= 16 ? 2 : 4) fp8_some_
                     for (int e = 0; e < 4; e++) cx.c[4 * h + e] = v[e];
                 }
                 cx.byte = kb < p.blocks ? scales[row * PITCH + kb] : 0u;
-                sk_product<RELU2>(acc[u], cw, cx);
+                sk_product<false>(acc[u], cw, cx);
             }
         }
     }
@@ -307,66 +296,35 @@ __global__ void __launch_bounds__(SK_WAVES *WAVE, S *MT >= 16 ? 2 : 4) fp8_some_
         for (int k = 1; k < S; k++)
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = v[e] + sums[(k * 16 * MT + row) * COLS + c + e];
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = sk_result<RELU2>(v[e]);
-        const long long at = (long long)(m0 + row) * p.N + n0 + c;
-        if constexpr (RELU2) {
-            *(f32x4 *)((float *)p.out + at) = f32x4{v[0], v[1], v[2], v[3]};
-            *(f32x4 *)((float *)p.out + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
-        } else {
-            *(u32x4 *)((uint16_t *)p.out + at) = u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]),
-                                                       bf16_pair(v[6], v[7])};
-        }
+        *(u32x4 *)((uint16_t *)p.out + (long long)(m0 + row) * p.N + n0 + c) =
+            u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
     }
 }
 
-template <int XT, bool RELU2> int few_launch(const Skinny &p, hipStream_t stream) {
-    /* 16 rows of w a wave, while that makes at most eight workgroups a CU; else 32, which read x half as often */
-    const long long ones = (p.N + 15) / 16;
-    const int rt = ones <= 8LL * device_cus() ? 1 : 2;
-    const dim3 grid((unsigned)((p.N + 16 * rt - 1) / (16 * rt))), block(SK_WAVES * WAVE);
-    const auto kernel = rt == 1 ? fp8_few_kernel<XT, 1, RELU2> : fp8_few_kernel<XT, 2, RELU2>;
-    hipLaunchKernelGGL(kernel, grid, block, 0, stream, p);
-    return (int)hipGetLastError();
-}
-
-template <int MT, int RW, int S, bool RELU2> int some_go(const Skinny &p, hipStream_t stream) {
-    const int parts = (p.M + 16 * MT - 1) / (16 * MT);
-    hipLaunchKernelGGL((fp8_some_kernel<MT, RW, S, RELU2>), dim3((unsigned)((p.N + 16 * RW - 1) / (16 * RW) * parts)),
+template <int RW, int S> int some_go(const Skinny &p, hipStream_t stream) {
+    const int parts = (p.M + 31) / 32;
+    hipLaunchKernelGGL((fp8_some_kernel<RW, S>), dim3((unsigned)((p.N + 16 * RW - 1) / (16 * RW) * parts)),
                        dim3(SK_WAVES * WAVE), 0, stream, p);
     return (int)hipGetLastError();
 }
-/*
- * Workgroups enough for the chip first, by few rows of w each; then few reads of x, by many. With 32 rows of x a workgroup, by the
- * number of (16 rows of w) x (32 rows of x): fewer than a CU's one, the eight waves split k; fewer than two, two rows by four; up to
- * eight, four by two. Past eight, x's reads bound it and a workgroup takes all its rows at once, with 64 and then with 128 rows of
- * w. Microseconds (16 x 1, 32 x 1, 64 x 1 rows of w with 32 of x; 64 and 128 with 128 of x):
- *    64 x 1,280 x 1,280     4.8   5.3   6.3  10.7  13.3        128 x 1,664 x 6,656    17.4  12.4  18.6  29.9  42.3
- *   128 x 4,992 x 1,664    21.8  13.7  12.0  15.0  17.9         64 x 16,384 x 1,664   33.5  17.1  12.2  14.3  16.6
- *   128 x 16,384 x 1,664   64.7  30.1  21.7  16.0  18.1        128 x 65,536 x 1,664    274   118  82.1  61.9  44.1
- *    32 x 65,536 x 1,664   71.6  36.5  28.1  51.1  34.9
- */
-template <bool RELU2> int some_any(const Skinny &p, hipStream_t stream) {
-    const long long cus = device_cus(), tiles = (p.N + 15) / 16, all = tiles * ((p.M + 31) / 32);
-    if (all < cus) return some_go<2, 1, 8, RELU2>(p, stream);
-    if (all < 2 * cus) return some_go<2, 2, 4, RELU2>(p, stream);
-    if (p.M <= 32 || all <= 8 * cus) return some_go<2, 4, 2, RELU2>(p, stream);
-    return tiles <= 8 * cus ? some_go<8, 4, 2, RELU2>(p, stream) : some_go<8, 8, 1, RELU2>(p, stream);
-}
 
-/* x bf16 or fp32 of up to 16 rows, taken as it is: rows must be readable 16 bytes at a time. In fp32 (an MLP's squared activations)
- * every workgroup's reads of x tell sooner: 1,664 outputs of 6,656 take 8.1 us for a row and 16.7 for 16, against 8.9 and about 4 to
- * put them in 8 bits first. */
-bool few_takes(const void *x, bool f32, long long row_stride, long long rows) {
-    const long long size = f32 ? 4 : 2;
-    return rows <= (f32 ? 8 : 16) && !((uintptr_t)x & 15) && (rows == 1 || (row_stride * size % 16 == 0 && row_stride <= 1 << 22));
+/* x bf16 or fp32 taken as it is: rows must be readable 16 bytes at a time. Every workgroup reads x, which tells with many of them and
+ * many rows; else it is two launches to put x in 8 bits first. Microseconds for 1, 4, 8 and 16 rows, against the two launches:
+ *    1,280 x 1,280   3.2   3.3   3.5   3.8 (6.8 to 7.4)     16,384 x 1,664    8.8   9.4  10.5  11.8 (10.0 to 10.4)
+ *    4,992 x 1,664   5.0   5.4   5.7   6.7 (8.2 to 9.1)     65,536 x 1,664   25.4  25.9  27.7  31.4 (24.8 to 25.7)
+ * and from an MLP's squares in fp32, all of it, 6,656 wide: 14.0  16.4  19.0 (18.0 and more). */
+bool few_takes(const void *x, bool f32, long long row_stride, long long rows, int n) {
+    const long long size = f32 ? 4 : 2, tiles = n / 16, cus = device_cus();
+    return rows <= (f32 ? 4 : 16) && tiles <= 4 * cus && rows * tiles <= 32 * cus && !((uintptr_t)x & 15) &&
+           (rows == 1 || (row_stride * size % 16 == 0 && row_stride <= 1 << 22));
 }
 int few(const void *x, bool f32, long long row_stride, const void *w, const void *ws, int ws_stride, int rows, int n, int k,
         bool relu2, void *out, hipStream_t stream) {
     const Skinny p = {x, (rows > 1 ? row_stride : k) * (f32 ? 4 : 2), nullptr, 0, ws_stride, (const unsigned char *)w,
                       (const unsigned char *)ws, rows, n, k, (k + F8_BLOCK - 1) / F8_BLOCK, out};
-    if (relu2) return few_launch<SK_BF16, true>(p, stream);
-    return f32 ? few_launch<SK_F32, false>(p, stream) : few_launch<SK_BF16, false>(p, stream);
+    const auto kernel = relu2 ? fp8_few_kernel<SK_BF16, true> : f32 ? fp8_few_kernel<SK_F32, false> : fp8_few_kernel<SK_BF16, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(n / 16)), dim3(SK_WAVES * WAVE), 0, stream, p);
+    return (int)hipGetLastError();
 }
 
 /* Parts of a workspace, one after another. */
@@ -387,7 +345,7 @@ bool weight_pitch(int stride, int k) { return stride >= (k + F8_BLOCK - 1) / F8_
 
 int linear(const void *x, int is_f32, long long row_stride, const void *w, const void *ws, int ws_stride, long long rows, int n,
            int k, void *out, void *workspace, hipStream_t stream) {
-    if (few_takes(x, is_f32, row_stride, rows))
+    if (few_takes(x, is_f32, row_stride, rows, n))
         return few(x, is_f32, row_stride, w, ws, ws_stride, (int)rows, n, k, false, out, stream);
     const Form f(workspace, rows, k);
     const int status = nc_fp8_quantize_rows(x, is_f32, row_stride, rows, k, f.codes, f.scale, f.pitch, stream);
@@ -396,21 +354,27 @@ int linear(const void *x, int is_f32, long long row_stride, const void *w, const
 
 }  // namespace
 
-bool fp8_some_takes(long long rows, int k) { return rows <= 128 && k <= SK_BLOCKS * F8_BLOCK; }
+/* The number of (16 rows of w) x (32 rows of x): the waves of a workgroup split k eight ways while there are fewer than the CUs, four
+ * ways while there are fewer than twice as many. */
+static long long some_tiles(long long rows, int n) { return (n + 15) / 16 * ((rows + 31) / 32); }
+bool fp8_some_takes(long long rows, int n, int k, long long cus) {
+    return k <= SK_BLOCKS * F8_BLOCK && some_tiles(rows, n) < 2 * cus;
+}
 
 int fp8_some(const void *codes, const void *scale, long long scale_stride, const void *w, const void *w_scale, int w_scale_stride,
-             int rows, int n, int k, bool relu2, void *out, hipStream_t stream) {
+             int rows, int n, int k, void *out, hipStream_t stream) {
     const Skinny p = {codes, k, (const unsigned char *)scale, (int)scale_stride, w_scale_stride, (const unsigned char *)w,
                       (const unsigned char *)w_scale, rows, n, k, (k + F8_BLOCK - 1) / F8_BLOCK, out};
-    return relu2 ? some_any<true>(p, stream) : some_any<false>(p, stream);
+    return some_tiles(rows, n) < device_cus() ? some_go<1, 8>(p, stream) : some_go<2, 4>(p, stream);
 }
 
 }  // namespace nc
 
 using namespace nc;
 
-extern "C" long long nc_fp8_linear_workspace_bytes(long long rows, int k) {
-    return serve_sizes(rows, 16, k) ? Form(nullptr, rows, k).bytes : -1;
+extern "C" long long nc_fp8_linear_workspace_bytes(const void *x, int is_f32, long long row_stride, long long rows, int n, int k) {
+    if (!serve_sizes(rows, n, k)) return -1;
+    return rows == 0 || few_takes(x, is_f32, row_stride, rows, n) ? 0 : Form(nullptr, rows, k).bytes;
 }
 
 extern "C" int nc_fp8_linear(const void *x, int is_f32, long long row_stride, const void *w, const void *w_scale,
@@ -422,17 +386,16 @@ extern "C" int nc_fp8_linear(const void *x, int is_f32, long long row_stride, co
     if (rows == 0) return NC_OK;
     if (!x || !w || !w_scale || !out) return NC_ERR_NULL;
     if (misaligned(x, is_f32 ? 4 : 2) || misaligned(w, 16) || misaligned(w_scale, 4) || misaligned(out, 16)) return NC_ERR_SHAPE;
-    if (!few_takes(x, is_f32, row_stride, rows)) {
-        if (!workspace) return NC_ERR_NULL;
-        if (misaligned(workspace, 16) || workspace_bytes < nc_fp8_linear_workspace_bytes(rows, k)) return NC_ERR_WORKSPACE;
-    }
+    const long long need = nc_fp8_linear_workspace_bytes(x, is_f32, row_stride, rows, n, k);
+    if (need > 0 && !workspace) return NC_ERR_NULL;
+    if (need > 0 && (misaligned(workspace, 16) || workspace_bytes < need)) return NC_ERR_WORKSPACE;
     return linear(x, is_f32, row_stride, w, w_scale, w_scale_stride, rows, n, k, out, workspace, (hipStream_t)stream);
 }
 
-/* x's form, then the squared activations: in fp32 and then in the 8-bit form for a few rows, in the 8-bit form alone for many. */
+/* x's form, then the squared activations: in the 8-bit form, or for up to 16 rows in fp32 and then in that form. */
 extern "C" long long nc_fp8_mlp_workspace_bytes(long long rows, int c, int hidden) {
     if (!serve_sizes(rows, hidden, c) || !serve_sizes(rows, 16, hidden)) return -1;
-    return Form(nullptr, rows, c).bytes + Form(nullptr, rows, hidden).bytes + (fp8_some_takes(rows, 16) ? 4 * rows * hidden : 0);
+    return Form(nullptr, rows, c).bytes + Form(nullptr, rows, hidden).bytes + (rows <= 16 ? 4 * rows * hidden : 0);
 }
 
 extern "C" int nc_fp8_mlp(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
@@ -449,20 +412,15 @@ extern "C" int nc_fp8_mlp(const void *x, long long row_stride, const void *fc, c
     if (misaligned(workspace, 16) || workspace_bytes < nc_fp8_mlp_workspace_bytes(rows, c, hidden)) return NC_ERR_WORKSPACE;
     const hipStream_t s = (hipStream_t)stream;
     const Form f(workspace, rows, c), a(f.codes + f.bytes, rows, hidden);
-    float *const act = (float *)(a.codes + a.bytes);
-    int status;
-    if (few_takes(x, false, row_stride, rows)) {
-        status = few(x, false, row_stride, fc, fc_scale, fc_scale_stride, (int)rows, hidden, c, true, act, s);
-    } else {
-        status = nc_fp8_quantize_rows(x, 0, row_stride, rows, c, f.codes, f.scale, f.pitch, stream);
-        if (status) return status;
-        if (!fp8_some_takes(rows, c)) {
-            status = nc_fp8_matmul_relu2(f.codes, f.scale, f.pitch, fc, fc_scale, fc_scale_stride, rows, hidden, c, a.codes,
-                                         a.scale, a.pitch, stream);
-            return status ? status : nc_fp8_matmul(a.codes, a.scale, a.pitch, proj, proj_scale, proj_scale_stride, rows, n,
-                                                   hidden, out, stream);
-        }
-        status = fp8_some(f.codes, f.scale, f.pitch, fc, fc_scale, fc_scale_stride, (int)rows, hidden, c, true, act, s);
+    if (few_takes(x, false, row_stride, rows, hidden)) {
+        float *const act = (float *)(a.codes + a.bytes);
+        const int status = few(x, false, row_stride, fc, fc_scale, fc_scale_stride, (int)rows, hidden, c, true, act, s);
+        return status ? status : linear(act, 1, hidden, proj, proj_scale, proj_scale_stride, rows, n, hidden, out, a.codes, s);
     }
-    return status ? status : linear(act, 1, hidden, proj, proj_scale, proj_scale_stride, rows, n, hidden, out, a.codes, s);
+    int status = nc_fp8_quantize_rows(x, 0, row_stride, rows, c, f.codes, f.scale, f.pitch, stream);
+    if (!status)
+        status = nc_fp8_matmul_relu2(f.codes, f.scale, f.pitch, fc, fc_scale, fc_scale_stride, rows, hidden, c, a.codes, a.scale,
+                                     a.pitch, stream);
+    return status ? status : nc_fp8_matmul(a.codes, a.scale, a.pitch, proj, proj_scale, proj_scale_stride, rows, n, hidden, out,
+                                           stream);
 }

@@ -52,10 +52,10 @@ int prefill_runs(const uint16_t *q, const uint8_t *k_pages, const uint8_t *v_pag
                  const int32_t *run_row0, const int32_t *run_count, const int32_t *run_slot, int runs, int max_count,
                  int Hq, int Hkv, int window, float sm_scale, uint16_t *out, hipStream_t stream);
 
-/* fp8_skinny.hip: nc_fp8_matmul for the few rows that fp8_some_takes; relu2: relu(sum)^2 in fp32 from exact products. */
-bool fp8_some_takes(long long rows, int k);
+/* fp8_skinny.hip: nc_fp8_matmul of few results, which fp8_some_takes tells. */
+bool fp8_some_takes(long long rows, int n, int k, long long cus);
 int fp8_some(const void *codes, const void *scale, long long scale_stride, const void *w, const void *w_scale, int w_scale_stride,
-             int rows, int n, int k, bool relu2, void *out, hipStream_t stream);
+             int rows, int n, int k, void *out, hipStream_t stream);
 
 /* The decode step's GEMM operands: out[n][r] = epilogue(sum_k x[n][k] w[r][k]), bf16 operands, fp32 sums,
  * N <= SG_MAX_N rows. */

@@ -216,12 +216,11 @@ def fp8_linear(x: Tensor, weight: Fp8Weight) -> Tensor:
     _outputs(n, "weight")
     with device_guard(x):
         lib = hip_library()
-        out, stride, ws, need = torch.empty(m, n, dtype=BF16, device=x.device), rows.stride(0), None, 0
-        if m > 16 or rows.data_ptr() % 16 or (m > 1 and (stride % 8 or stride > 1 << 22)):
-            need = lib.nc_fp8_linear_workspace_bytes(m, k)
-            ws = _workspace(x, need)
-        check(lib.nc_fp8_linear(rows.data_ptr(), 0, stride, weight.codes.data_ptr(), weight.scale.data_ptr(), pitch, m, n, k,
-                                out.data_ptr(), None if ws is None else ws.data_ptr(), need, stream()))
+        out, at, stride = torch.empty(m, n, dtype=BF16, device=x.device), rows.data_ptr(), rows.stride(0)
+        need = lib.nc_fp8_linear_workspace_bytes(at, 0, stride, m, n, k)
+        ws = _workspace(x, need) if need else None
+        check(lib.nc_fp8_linear(at, 0, stride, weight.codes.data_ptr(), weight.scale.data_ptr(), pitch, m, n, k, out.data_ptr(),
+                                ws.data_ptr() if need else None, need, stream()))
     return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 

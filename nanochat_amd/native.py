@@ -140,7 +140,7 @@ SIGNATURES = {
                              c_void_p, c_longlong, c_void_p], c_int),
     "nc_fp8_matmul_relu2_bwd": ([c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_void_p,
                                  c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_void_p], c_int),
-    "nc_fp8_linear_workspace_bytes": ([c_longlong, c_int], c_longlong),
+    "nc_fp8_linear_workspace_bytes": ([c_void_p, c_int, c_longlong, c_longlong, c_int, c_int], c_longlong),
     "nc_fp8_linear": ([c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p,
                        c_longlong, c_void_p], c_int),
     "nc_fp8_mlp_workspace_bytes": ([c_longlong, c_int, c_int], c_longlong),

@@ -234,7 +234,7 @@ def test_serving_layers(device, rows):
     assert np.linalg.norm(codes_of(z) - exact) <= 2.0 ** -6 * np.linalg.norm(exact)
 
 
-# rows of w and of x a workgroup takes: by the number of rows of x and of (16 rows of w) x (32 of x) against the CUs (256)
+# by the number of rows, of outputs, and of (16 outputs) x (32 rows) against the CUs (256)
 FEW = [(rows, 400, 2064) for rows in (1, 2, 8, 9, 15, 16, 17, 31, 32, 33, 100, 127, 128)]
 FEW += [(1, 16, 20000), (16, 33024, 144), (3, 4992, 400), (20, 48, 16400), (20, 4800, 272), (32, 33024, 144), (40, 4816, 144),
         (64, 2064, 1296), (97, 9616, 144), (128, 33040, 272), (128, 16, 16384), (77, 16, 16)]
@@ -260,7 +260,7 @@ def test_few_rows(device, rows, n, k):
     lib, out = hip_library(), torch.full((rows + 1, n), 7.0, dtype=BF16, device=device)
     xd, xf = x.to(device), x.float().to(device)
     for t, f32 in ((xd, 0), (xf, 1)):
-        need = lib.nc_fp8_linear_workspace_bytes(rows, k)
+        need = lib.nc_fp8_linear_workspace_bytes(t.data_ptr(), f32, k, rows, n, k)
         ws = torch.full((need + 64,), 9, dtype=torch.uint8, device=device)
         assert lib.nc_fp8_linear(t.data_ptr(), f32, k, w.codes.data_ptr(), w.scale.data_ptr(), w.scale.stride(0), rows, n, k,
                                  out.data_ptr(), ws.data_ptr(), need, stream()) == 0
