@@ -408,6 +408,34 @@ int nc_fp8_weight_grad(const void *dy, const void *codes, const void *scale, lon
                        int n2, int mode, void *out, void *workspace, long long workspace_bytes, void *stream);
 
 /*
+ * The training of a layer and of a ReLU^2 MLP, a direction a call, from the parts above. All in the 8-bit form are at strides as
+ * there; rows bf16 at row_stride elements; all widths are multiples of 16.
+ *   forward   codes, scale = x in the 8-bit form: the checkpoint; linear: out = it w^T; mlp: act, act_scale = relu(it fc^T)^2 in the
+ *             8-bit form, the second checkpoint, and out = it proj^T
+ *   backward  dy bf16 [rows][n] (dense, 16-byte aligned, where a weight gradient reads it) -> dx bf16 [rows][k] (not wanted where
+ *             NULL), from the weights' transposes in the 8-bit form, and dw in nc_fp8_weight_grad's mode, or -1 where it is not wanted:
+ *             dx = dy8 w8, dw = dy^T x8; dh = bf16((dy8 p8) 2 sqrt(a8)), dx = dh8 f8, dfc = dh^T x8, dproj = dy^T a8. rows = 0
+ *             launches nothing and leaves all outputs as they are.
+ * workspace: nc_fp8_*_bwd_workspace_bytes (-1 for unsupported arguments), 16-byte aligned, need not be cleared.
+ */
+int nc_fp8_linear_fwd(const void *x, long long row_stride, const void *w, const void *w_scale, int w_scale_stride, long long rows,
+                      int n, int k, void *codes, void *scale, long long scale_stride, void *out, void *stream);
+long long nc_fp8_linear_bwd_workspace_bytes(long long rows, int n, int k, int need_x, int mode);
+int nc_fp8_linear_bwd(const void *dy, long long row_stride, const void *codes, const void *scale, long long scale_stride,
+                      const void *codes_t, const void *scale_t, int scale_t_stride, long long rows, int n, int k, void *dx,
+                      void *dw, int mode, void *workspace, long long workspace_bytes, void *stream);
+int nc_fp8_mlp_fwd(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
+                   const void *proj, const void *proj_scale, int proj_scale_stride, long long rows, int c, int hidden, int n,
+                   void *codes, void *scale, long long scale_stride, void *act, void *act_scale, long long act_scale_stride,
+                   void *out, void *stream);
+long long nc_fp8_mlp_bwd_workspace_bytes(long long rows, int c, int hidden, int n, int need_x, int fc_mode, int proj_mode);
+int nc_fp8_mlp_bwd(const void *dy, long long row_stride, const void *codes, const void *scale, long long scale_stride,
+                   const void *act, const void *act_scale, long long act_scale_stride, const void *fc_codes_t,
+                   const void *fc_scale_t, int fc_scale_t_stride, const void *proj_codes_t, const void *proj_scale_t,
+                   int proj_scale_t_stride, long long rows, int c, int hidden, int n, void *dx, void *dfc, int fc_mode,
+                   void *dproj, int proj_mode, void *workspace, long long workspace_bytes, void *stream);
+
+/*
  * Measurement only; no counterpart in the reference. Reads n pages of 2 KiB (one (page, head) of K or V codes) from
  * src (src_bytes, a multiple of 2,048), page order[i] as the i-th (order NULL: page i; an entry outside the buffer
  * reads page 0), with `grid` workgroups of 256 threads, and writes one checksum word per thread to sink

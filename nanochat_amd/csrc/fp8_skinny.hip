@@ -327,15 +327,6 @@ int few(const void *x, bool f32, long long row_stride, const void *w, const void
     return (int)hipGetLastError();
 }
 
-/* Parts of a workspace, one after another. */
-long long scale_pitch(int cols) { return ((cols + F8_BLOCK - 1) / F8_BLOCK + 3) / 4 * 4; }
-long long up16(long long n) { return (n + 15) / 16 * 16; }
-struct Form {                      /* rows in the 8-bit form */
-    unsigned char *codes, *scale;
-    long long pitch, bytes;
-    Form(void *at, long long rows, int cols)
-        : codes((unsigned char *)at), scale(codes + rows * cols), pitch(scale_pitch(cols)), bytes(rows * cols + up16(rows * pitch)) {}
-};
 bool serve_sizes(long long rows, int n, int k) {
     return rows >= 0 && n > 0 && k > 0 && n % 16 == 0 && k % 16 == 0 && n <= 1 << 20 && k <= 1 << 20 &&
            rows <= (1LL << 31) / ((k + F8_BLOCK - 1) / F8_BLOCK) - 32;
@@ -347,7 +338,7 @@ int linear(const void *x, int is_f32, long long row_stride, const void *w, const
            int k, void *out, void *workspace, hipStream_t stream) {
     if (few_takes(x, is_f32, row_stride, rows, n))
         return few(x, is_f32, row_stride, w, ws, ws_stride, (int)rows, n, k, false, out, stream);
-    const Form f(workspace, rows, k);
+    const F8Form f(workspace, rows, k);
     const int status = nc_fp8_quantize_rows(x, is_f32, row_stride, rows, k, f.codes, f.scale, f.pitch, stream);
     return status ? status : nc_fp8_matmul(f.codes, f.scale, f.pitch, w, ws, ws_stride, rows, n, k, out, stream);
 }
@@ -374,7 +365,7 @@ using namespace nc;
 
 extern "C" long long nc_fp8_linear_workspace_bytes(const void *x, int is_f32, long long row_stride, long long rows, int n, int k) {
     if (!serve_sizes(rows, n, k)) return -1;
-    return rows == 0 || few_takes(x, is_f32, row_stride, rows, n) ? 0 : Form(nullptr, rows, k).bytes;
+    return rows == 0 || few_takes(x, is_f32, row_stride, rows, n) ? 0 : f8_form_bytes(rows, k);
 }
 
 extern "C" int nc_fp8_linear(const void *x, int is_f32, long long row_stride, const void *w, const void *w_scale,
@@ -395,7 +386,7 @@ extern "C" int nc_fp8_linear(const void *x, int is_f32, long long row_stride, co
 /* x's form, then the squared activations: in the 8-bit form, or for up to 16 rows in fp32 and then in that form. */
 extern "C" long long nc_fp8_mlp_workspace_bytes(long long rows, int c, int hidden) {
     if (!serve_sizes(rows, hidden, c) || !serve_sizes(rows, 16, hidden)) return -1;
-    return Form(nullptr, rows, c).bytes + Form(nullptr, rows, hidden).bytes + (rows <= 16 ? 4 * rows * hidden : 0);
+    return f8_form_bytes(rows, c) + f8_form_bytes(rows, hidden) + (rows <= 16 ? 4 * rows * hidden : 0);
 }
 
 extern "C" int nc_fp8_mlp(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
@@ -411,7 +402,7 @@ extern "C" int nc_fp8_mlp(const void *x, long long row_stride, const void *fc, c
         return NC_ERR_SHAPE;
     if (misaligned(workspace, 16) || workspace_bytes < nc_fp8_mlp_workspace_bytes(rows, c, hidden)) return NC_ERR_WORKSPACE;
     const hipStream_t s = (hipStream_t)stream;
-    const Form f(workspace, rows, c), a(f.codes + f.bytes, rows, hidden);
+    const F8Form f(workspace, rows, c), a(f.codes + f.bytes, rows, hidden);
     if (few_takes(x, false, row_stride, rows, hidden)) {
         float *const act = (float *)(a.codes + a.bytes);
         const int status = few(x, false, row_stride, fc, fc_scale, fc_scale_stride, (int)rows, hidden, c, true, act, s);

@@ -113,4 +113,14 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
     return b[0] > b[1] ? b[0] : b[1];
 }
 
+/* Rows in the 8-bit form in a workspace: their codes, then their scales at a padded stride. */
+static inline long long f8_pitch(int cols) { return ((cols + F8_BLOCK - 1) / F8_BLOCK + 3) / 4 * 4; }
+static inline long long f8_form_bytes(long long rows, int cols) { return rows * cols + (rows * f8_pitch(cols) + 15) / 16 * 16; }
+struct F8Form {
+    unsigned char *codes, *scale;
+    long long pitch, bytes;
+    F8Form(void *at, long long rows, int cols)
+        : codes((unsigned char *)at), scale(codes + rows * cols), pitch(f8_pitch(cols)), bytes(f8_form_bytes(rows, cols)) {}
+};
+
 }  // namespace nc

@@ -29,7 +29,8 @@ LIBRARY = LIB_DIR / "libnanochat_kv.so"
 DECODE_LIBRARY = LIB_DIR / "libnanochat_decode.so"
 KERNEL_SOURCES = [CSRC / "kv_append.hip", CSRC / "attention.hip", CSRC / "ve_gate.hip", CSRC / "flash_attn.hip",
                   CSRC / "prefill_gemm.hip", CSRC / "train_gemm.hip", CSRC / "paging.hip", CSRC / "sample.hip", CSRC / "packed_attn.hip",
-                  CSRC / "fp8_quant.hip", CSRC / "fp8_gemm.hip", CSRC / "fp8_grad.hip", CSRC / "fp8_skinny.hip"]
+                  CSRC / "fp8_quant.hip", CSRC / "fp8_gemm.hip", CSRC / "fp8_grad.hip", CSRC / "fp8_skinny.hip",
+                  CSRC / "fp8_layers.hip"]
 DECODE_SOURCES = [CSRC / "decoder.hip", CSRC / "slot_gemm.hip"]
 SOURCES = KERNEL_SOURCES + DECODE_SOURCES
 HEADERS = [CSRC / "nc_device.h", CSRC / "nc_internal.h", CSRC / "nc_row.h", CSRC / "nc_attend.h", CSRC / "nc_meeting.h",
@@ -149,6 +150,17 @@ SIGNATURES = {
     "nc_fp8_weight_grad_workspace_bytes": ([c_longlong, c_int, c_int], c_longlong),
     "nc_fp8_weight_grad": ([c_void_p, c_void_p, c_void_p, c_longlong, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p,
                             c_longlong, c_void_p], c_int),
+    "nc_fp8_linear_fwd": ([c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p,
+                           c_longlong, c_void_p, c_void_p], c_int),
+    "nc_fp8_linear_bwd_workspace_bytes": ([c_longlong, c_int, c_int, c_int, c_int], c_longlong),
+    "nc_fp8_linear_bwd": ([c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_longlong, c_int,
+                           c_int, c_void_p, c_void_p, c_int, c_void_p, c_longlong, c_void_p], c_int),
+    "nc_fp8_mlp_fwd": ([c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int,
+                        c_int, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p], c_int),
+    "nc_fp8_mlp_bwd_workspace_bytes": ([c_longlong] + [c_int] * 6, c_longlong),
+    "nc_fp8_mlp_bwd": ([c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_void_p, c_void_p,
+                        c_int, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p,
+                        c_int, c_void_p, c_longlong, c_void_p], c_int),
     "nc_pages_trim": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p], c_int),
 }
 

@@ -54,6 +54,15 @@ def test_gradients_reach_their_inputs():
         assert (got[1] is None) if buf is not None else got[1].shape == fc.shape
 
 
+def test_gradients_have_no_gradient():
+    x = torch.empty(4, 128, dtype=BF16, device="meta", requires_grad=True)
+    w = torch.empty(128, 128, device="meta", requires_grad=True)
+    for y in (fl.checkpointed_linear(x, w), fl.checkpointed_mlp(x, w, w)):
+        dx, = torch.autograd.grad(y.float().pow(2).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            dx.float().sum().backward()
+
+
 def rows_args(**over):
     return list((dict(x=DUMMY, f32=0, stride=256, rows=3, cols=256, codes=DUMMY, scale=DUMMY, pitch=4, stream=None) | over).values())
 
@@ -147,6 +156,49 @@ def test_serving_refuses(lib):
     need = lib.nc_fp8_mlp_workspace_bytes(40, 256, 512)
     assert lib.nc_fp8_mlp(*mlp_args(bytes=need - 1)) == -3 and lib.nc_fp8_mlp(*mlp_args(ws=odd)) == -3
     assert lib.nc_fp8_mlp(*mlp_args(rows=0)) == 0 and lib.nc_fp8_mlp_workspace_bytes(40, 256, 500) == -1
+
+
+def test_training_refuses(lib):
+    def fwd(**over):
+        a = dict(x=DUMMY, stride=256, w=DUMMY, w_scale=DUMMY, w_pitch=4, rows=3, n=32, k=256, codes=DUMMY, scale=DUMMY, pitch=4,
+                 out=DUMMY, stream=None) | over
+        return lib.nc_fp8_linear_fwd(*a.values())
+
+    def bwd(**over):
+        a = dict(dy=DUMMY, stride=32, codes=DUMMY, scale=DUMMY, pitch=4, codes_t=DUMMY, scale_t=DUMMY, pitch_t=4, rows=3, n=32,
+                 k=256, dx=DUMMY, dw=DUMMY, mode=0, ws=DUMMY, bytes=2 ** 20, stream=None) | over
+        return lib.nc_fp8_linear_bwd(*a.values())
+
+    def mlp_fwd(**over):
+        a = dict(x=DUMMY, stride=256, fc=DUMMY, fc_scale=DUMMY, fc_pitch=4, proj=DUMMY, proj_scale=DUMMY, proj_pitch=4, rows=3,
+                 c=256, hidden=512, n=32, codes=DUMMY, scale=DUMMY, pitch=4, act=DUMMY, act_scale=DUMMY, act_pitch=4, out=DUMMY,
+                 stream=None) | over
+        return lib.nc_fp8_mlp_fwd(*a.values())
+
+    def mlp_bwd(**over):
+        a = dict(dy=DUMMY, stride=32, codes=DUMMY, scale=DUMMY, pitch=4, act=DUMMY, act_scale=DUMMY, act_pitch=4, fct=DUMMY,
+                 fct_scale=DUMMY, fct_pitch=4, pt=DUMMY, pt_scale=DUMMY, pt_pitch=4, rows=3, c=256, hidden=512, n=32, dx=DUMMY,
+                 dfc=DUMMY, fc_mode=0, dproj=DUMMY, proj_mode=0, ws=DUMMY, bytes=2 ** 24, stream=None) | over
+        return lib.nc_fp8_mlp_bwd(*a.values())
+
+    odd = ctypes.c_void_p(0x1008)
+    for call, names in ((fwd, ("x", "w", "w_scale", "codes", "scale", "out")),
+                        (bwd, ("dy", "codes", "scale", "codes_t", "scale_t", "dw", "ws")),
+                        (mlp_fwd, ("x", "fc", "fc_scale", "proj", "proj_scale", "codes", "scale", "act", "act_scale", "out")),
+                        (mlp_bwd, ("dy", "codes", "scale", "act", "act_scale", "fct", "fct_scale", "pt", "pt_scale", "dfc",
+                                   "dproj", "ws"))):
+        for name in names:
+            assert call(**{name: None}) == -1, (call, name)
+        for over in (dict(rows=-1), dict(n=24), dict(n=0)):
+            assert call(**over) == -2, (call, over)
+        assert call(rows=0) == 0
+    assert fwd(k=72) == fwd(w=odd) == fwd(out=odd) == fwd(pitch=1) == mlp_fwd(hidden=500) == mlp_fwd(act=odd) == -2
+    assert bwd(mode=3) == bwd(stride=40) == mlp_bwd(fc_mode=-2) == mlp_bwd(stride=40) == mlp_bwd(c=2 ** 20 + 16) == -2
+    need = lib.nc_fp8_linear_bwd_workspace_bytes(3, 32, 256, 1, 0)
+    assert bwd(bytes=need - 1) == bwd(ws=odd) == -3
+    need = lib.nc_fp8_mlp_bwd_workspace_bytes(3, 256, 512, 32, 1, 0, 0)
+    assert mlp_bwd(bytes=need - 1) == mlp_bwd(ws=odd) == -3
+    assert lib.nc_fp8_linear_bwd_workspace_bytes(3, 32, 256, 0, -1) == 0 == lib.nc_fp8_mlp_bwd_workspace_bytes(3, 256, 512, 32, 0, -1, -1)
 
 
 def test_weight_gradient_refuses(lib):

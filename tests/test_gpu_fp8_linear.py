@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from nanochat_amd import fp8_linear as fl
+from nanochat_amd import fp8_linear as fl, native
 from nanochat_amd.native import hip_library, stream
 from oracle import fp8_block as fb
 
@@ -56,6 +56,28 @@ def form(gen, device, rows, cols, spread=True):
 def weight(gen, device, n, k, transpose=False):
     w = fl.quantize_weight((torch.randn(n, k, generator=gen) * k ** -0.5).to(device), transpose)
     return w, fb.values(codes_of(w.codes), exps_of(w.scale), 128)
+
+
+def product_relu2(codes, scale, w):
+    rows, k = codes.shape
+    n = w.codes.size(0)
+    out, out_scale = torch.empty(rows, n, dtype=fl.CODES, device=codes.device), fl._new_scale(codes, rows, n)
+    native.check(hip_library().nc_fp8_matmul_relu2(codes.data_ptr(), scale.data_ptr(), scale.stride(0), w.codes.data_ptr(),
+                                                   w.scale.data_ptr(), w.scale.stride(0), rows, n, k, out.data_ptr(),
+                                                   out_scale.data_ptr(), out_scale.stride(0), stream()))
+    return out, out_scale
+
+
+def product_relu2_bwd(codes, scale, w, act, act_scale):
+    rows, k = codes.shape
+    n = w.codes.size(0)
+    out, q = torch.empty(rows, n, dtype=BF16, device=codes.device), torch.empty_like(act)
+    q_scale = fl._new_scale(codes, rows, n)
+    native.check(hip_library().nc_fp8_matmul_relu2_bwd(
+        codes.data_ptr(), scale.data_ptr(), scale.stride(0), w.codes.data_ptr(), w.scale.data_ptr(), w.scale.stride(0), rows, n, k,
+        act.data_ptr(), act_scale.data_ptr(), act_scale.stride(0), out.data_ptr(), q.data_ptr(), q_scale.data_ptr(),
+        q_scale.stride(0), stream()))
+    return out, q, q_scale
 
 
 # --- the 8-bit form
@@ -107,7 +129,7 @@ def test_blocks_that_are_not_finite(device, bad):
         w, wv = weight(gen, device, 144, 384)
         y = fl.fp8_matmul(codes, scale, w)
         assert bool(torch.isnan(y[5]).all()) and not bool(torch.isnan(y[[4, 6]]).any())
-        a8, a_s = fl._product_relu2(codes, scale, w.codes, w.scale)
+        a8, a_s = product_relu2(codes, scale, w)
         assert bool(torch.isnan(a8[5].float()).all()) and not bool(torch.isnan(a8[[4, 6]].float()).any())
         dy = bf(gen, 40, 144).to(device)
         dw = fl.checkpoint_weight_grad(dy, codes, scale)
@@ -163,7 +185,7 @@ def test_product_relu2(device, rows, n, k):
     gen = torch.Generator().manual_seed(rows + n + k)
     codes, scale, x = form(gen, device, rows, k)
     w, wv = weight(gen, device, n, k)
-    a8, a_s = fl._product_relu2(codes, scale, w.codes, w.scale)
+    a8, a_s = product_relu2(codes, scale, w)
     h, off = x @ wv.T, (2.0 ** -10 + k * EPS) * (np.abs(x) @ np.abs(wv).T)
     want = np.maximum(h, 0.0) ** 2
     slack = 2 * np.maximum(h, 0.0) * off + off * off + 4 * EPS * want
@@ -184,7 +206,7 @@ def test_product_relu2_backward(device, rows, n, k):
     w, wv = weight(gen, device, n, k)
     a8, a_s = fl.quantize_rows((rowwise(gen, rows, n).float().clamp(min=0) ** 2).to(device))
     root = 2 * np.sqrt(fb.values(codes_of(a8), exps_of(a_s), 1))
-    dh, q, q_s = fl._product_relu2_bwd(codes, scale, w.codes, w.scale, a8, a_s)
+    dh, q, q_s = product_relu2_bwd(codes, scale, w, a8, a_s)
     want, off = (x @ wv.T) * root, (2.0 ** -10 + k * EPS) * (np.abs(x) @ np.abs(wv).T) * root
     close(codes_of(dh), want, 2.0 ** -8 * np.abs(want) + off + 4 * EPS * np.abs(want))
     assert same_form(q, q_s, codes_of(dh), 1)
@@ -390,7 +412,7 @@ def test_training_mlp(device, m, c, f, n, dtype):
     x8, f8, p8, dy8 = fb.through(xd, 1), fb.through(fd, 128), fb.through(pd, 128), fb.through(dyd, 1)
     q = fl.quantize_weight(fc.detach())
     codes, scale = fl.quantize_rows(x.detach())
-    a8, a_s = fl._product_relu2(codes, scale, q.codes, q.scale)
+    a8, a_s = product_relu2(codes, scale, q)
     a = fb.values(codes_of(a8), exps_of(a_s), 1)
     close(codes_of(y.detach()), a @ p8.T, 2.0 ** -8 * np.abs(a @ p8.T) + (2.0 ** -10 + f * EPS) * (a @ np.abs(p8).T))
     mag = np.abs(dyd).T @ a
