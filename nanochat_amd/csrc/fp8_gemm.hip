@@ -540,20 +540,44 @@ int fg_check(const F8Gemm &g, int epi) {
     return NC_OK;
 }
 
-/* Small tiles while they all run at once; then by rounds, of a full tile a CU or of two halves, which take about 8 to 5 (full and
- * half tiles of 1,664 k, us: 515 x 16,384 22.0, 25.0; 300 x 16,384 21.8, 13.7; 200 x 65,536 32.5, 38.9; 128 x 65,536 29.3, 25.9;
- * 2,500 x 4,992 23.7, 27.6; 1,001 x 4,992 21.7, 13.4. Small and half: 256 x 4,992 7.7, 11.0; 128 x 16,384 8.2, 11.7; 515 x 4,992,
- * 351 small ones, 11.6, 11.3; 300 x 16,384, 640, 18.5, 13.7). */
+/* The first rows of g, or those behind them. */
+F8Gemm fg_rows(F8Gemm g, long long from, long long count) {
+    g.a += from * g.K;
+    g.as += from * g.as_stride;
+    if (g.out) g.out += from * g.N;
+    if (g.q) g.q += from * g.N, g.qs += from * g.qs_stride;
+    if (g.act) g.act += from * g.N, g.acts += from * g.act_stride;
+    g.M = count;
+    return g;
+}
+
+/*
+ * Small tiles while they all run at once; else by rounds, of a full tile a CU (8 parts of time), of two half tiles a CU (5; one alone
+ * 4), or whole rounds of full tiles and half tiles for the rows left, a launch more (1). Microseconds of full and half tiles of 1,664 k:
+ * 515 x 16,384 22.0, 25.0; 300 x 16,384 21.8, 13.7; 200 x 65,536 32.5, 38.9; 128 x 65,536 29.3, 25.9; 2,500 x 4,992 23.7, 27.6;
+ * 1,001 x 4,992 21.7, 13.4. Of small and half: 256 x 4,992 7.7, 11.0; 128 x 16,384 8.2, 11.7; 515 x 4,992, 351 small ones, 11.6,
+ * 11.3; 300 x 16,384, 640, 18.5, 13.7. All sum in the same order.
+ */
+long long fg_half_time(long long tiles, long long cus) { return tiles <= cus ? 4 : 5 * ((tiles + 2 * cus - 1) / (2 * cus)); }
 int fg_gemm(const F8Gemm &g, int epi, void *stream) {
     const int e = fg_check(g, epi);
     if (e != NC_OK || g.M == 0) return e;
-    const long long cus = device_cus(), full = (g.M + 255) / 256 * ((g.N + 255) / 256);
-    const long long half = (g.M + 127) / 128 * ((g.N + 127) / 128), small = (g.M + 63) / 64 * ((g.N + 127) / 128);
+    const hipStream_t s = (hipStream_t)stream;
+    const long long cus = device_cus(), nx = (g.N + 255) / 256, full = (g.M + 255) / 256 * nx, half_nx = (g.N + 127) / 128;
+    const long long small = (g.M + 63) / 64 * half_nx;
     if (epi == FG_STORE && fp8_some_takes(g.M, g.N, g.K, cus))
-        return fp8_some(g.a, g.as, g.as_stride, g.w, g.ws, g.ws_stride, (int)g.M, g.N, g.K, g.out, (hipStream_t)stream);
-    if (small <= cus) return fg_launch<FgSmall>(g, epi, (hipStream_t)stream);
-    if (8 * ((full + cus - 1) / cus) <= 5 * ((half + 2 * cus - 1) / (2 * cus))) return fg_launch<FgFull>(g, epi, (hipStream_t)stream);
-    return fg_launch<FgHalf>(g, epi, (hipStream_t)stream);
+        return fp8_some(g.a, g.as, g.as_stride, g.w, g.ws, g.ws_stride, (int)g.M, g.N, g.K, g.out, s);
+    if (small <= cus) return fg_launch<FgSmall>(g, epi, s);
+    const long long full_time = 8 * ((full + cus - 1) / cus), half_time = fg_half_time((g.M + 127) / 128 * half_nx, cus);
+    const long long rounds = full / cus, top = rounds * cus / nx * 256;   /* rows of whole rounds: less than M, or all are whole */
+    if (top > 0 && top < g.M) {
+        const long long split = 8 * rounds + fg_half_time((g.M - top + 127) / 128 * half_nx, cus) + 1;
+        if (split < full_time && split < half_time) {
+            const int status = fg_launch<FgFull>(fg_rows(g, 0, top), epi, s);
+            return status ? status : fg_launch<FgHalf>(fg_rows(g, top, g.M - top), epi, s);
+        }
+    }
+    return full_time <= half_time ? fg_launch<FgFull>(g, epi, s) : fg_launch<FgHalf>(g, epi, s);
 }
 
 }  // namespace
