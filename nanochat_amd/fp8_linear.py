@@ -398,17 +398,17 @@ def _fake_linear_bwd(dy, x8, xs, codes_t, scale_t, grad, need_x, need_w, wide):
 def _linear_context(ctx: FunctionCtx, inputs: tuple, output: tuple) -> None:
     x, weight, codes, _, codes_t, scale_t, grad = inputs
     _, x8, xs, made_t, made_ts = output
-    ctx.x_shape, ctx.wide = x.shape, weight.dtype == F32
+    ctx.x_shape, ctx.wide, ctx.grad = x.shape, weight.dtype == F32, grad   # grad not saved: it may change until it is added to
     ctx.set_materialize_grads(False)
     ctx.mark_non_differentiable(*output[1:])
-    ctx.save_for_backward(x8, xs, *((codes_t, scale_t) if codes is not None else (made_t, made_ts)), grad)
+    ctx.save_for_backward(x8, xs, *((codes_t, scale_t) if codes is not None else (made_t, made_ts)))
 
 
 @once_differentiable
 def _linear_backward(ctx: FunctionCtx, dy: Tensor | None, *_: Tensor | None) -> tuple:
     if dy is None:
         return (None,) * 7
-    x8, xs, codes_t, scale_t, grad = ctx.saved_tensors
+    (x8, xs, codes_t, scale_t), grad = ctx.saved_tensors, ctx.grad
     need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or grad is not None
     dx, dw = _linear_bwd(dy, x8, xs, codes_t, scale_t, grad, need_x, need_w, ctx.wide)
     return (dx.view(ctx.x_shape) if need_x else None, dw if need_w and grad is None else None, *(None,) * 5)
@@ -508,21 +508,21 @@ def _mlp_context(ctx: FunctionCtx, inputs: tuple, output: tuple) -> None:
     f, p = inputs[3:8], inputs[8:13]
     _, x8, xs, a8, a_s, f_t, f_ts, p_t, p_ts = output
     ctx.x_shape, ctx.fc_wide, ctx.proj_wide = x.shape, fc.dtype == F32, proj.dtype == F32
+    ctx.fc_grad, ctx.proj_grad = f[4], p[4]
     ctx.set_materialize_grads(False)
     ctx.mark_non_differentiable(*output[1:])
     ctx.save_for_backward(x8, xs, a8, a_s, *(f[2:4] if f[0] is not None else (f_t, f_ts)),
-                          *(p[2:4] if p[0] is not None else (p_t, p_ts)), f[4], p[4])
+                          *(p[2:4] if p[0] is not None else (p_t, p_ts)))
 
 
 @once_differentiable
 def _mlp_backward(ctx: FunctionCtx, dy: Tensor | None, *_: Tensor | None) -> tuple:
     if dy is None:
         return (None,) * 13
-    saved = ctx.saved_tensors
-    fc_grad, proj_grad = saved[8:]
+    fc_grad, proj_grad = ctx.fc_grad, ctx.proj_grad
     need_x = ctx.needs_input_grad[0]
     need_fc, need_proj = ctx.needs_input_grad[1] or fc_grad is not None, ctx.needs_input_grad[2] or proj_grad is not None
-    dx, dfc, dproj = _mlp_bwd(dy, *saved, need_x, need_fc, need_proj, ctx.fc_wide, ctx.proj_wide)
+    dx, dfc, dproj = _mlp_bwd(dy, *ctx.saved_tensors, fc_grad, proj_grad, need_x, need_fc, need_proj, ctx.fc_wide, ctx.proj_wide)
     return (dx.view(ctx.x_shape) if need_x else None, dfc if need_fc and fc_grad is None else None,
             dproj if need_proj and proj_grad is None else None, *(None,) * 10)
 

@@ -428,6 +428,23 @@ def test_training_mlp(device, m, c, f, n, dtype):
     close(codes_of(dx), want, off8 @ np.abs(f8) + (2.0 ** -10 + f * EPS) * m8 + 2.0 ** -8 * m8)
 
 
+def test_one_buffer_for_two_uses(device):
+    """A weight used twice adds both its gradients to one buffer, which may be cleared between the forward and the backward."""
+    gen = torch.Generator().manual_seed(11)
+    w, x, dy = (torch.randn(256, 256, generator=gen) / 16).to(device), bf(gen, 70, 256).to(device), bf(gen, 70, 256).to(device)
+    grad, wl, xl = torch.ones(256, 256, device=device), w.clone().requires_grad_(), x.clone().requires_grad_()
+    version = grad._version
+    y = fl.checkpointed_mlp(fl.checkpointed_linear(xl, wl, grad=grad), wl, wl, fc_grad=grad, proj_grad=grad)
+    grad.zero_()
+    y.backward(dy)
+    assert grad._version > version + 1 and wl.grad is None
+    one, got = w.clone().requires_grad_(), x.clone().requires_grad_()
+    fl.checkpointed_mlp(fl.checkpointed_linear(got, one), one, one).backward(dy)
+    assert torch.equal(xl.grad, got.grad)
+    # three fp32 sums added in another order
+    assert bool(((grad - one.grad).abs() <= 4 * EPS * (one.grad.abs() + grad.abs().max())).all())
+
+
 def test_gradients_by_differences(device):
     """<gradient, v> against (L(+v) - L(-v)) / 2 of the layers without 8-bit rounding, in float64, where every value, weight and
     direction is positive: nothing cancels, so each factor's 2^-4 (and a bf16 rounding here and there) bounds the whole. dx of
@@ -574,6 +591,28 @@ def test_training_step_captured_with_eager_work_between(device):
         w8 = [fl.quantize_weight(w) for w in weights]
         h = inputs[0][0] + fl.fp8_linear(fl.fp8_linear(inputs[0][0], w8[0]), w8[1])
         assert torch.equal(h + fl.fp8_mlp(h, w8[2], w8[3]), want[0][0])
+
+
+@pytest.mark.parametrize("rows", [1, 12, 40, 300])
+def test_serving_captured(device, rows):
+    """Serving layers in a graph, replayed on new inputs with eager calls between."""
+    gen = torch.Generator().manual_seed(rows)
+    w, fc, proj = (weight(gen, device, *s)[0] for s in ((1296, 640), (2576, 640), (656, 2576)))
+    inputs = [bf(gen, rows, 640).to(device) for _ in range(4)]
+    x, s = inputs[0].clone(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        fl.fp8_linear(x, w), fl.fp8_mlp(x, fc, proj)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, z = fl.fp8_linear(x, w), fl.fp8_mlp(x, fc, proj)
+    for new in inputs[1:]:
+        x.copy_(new)
+        want = fl.fp8_linear(new, w), fl.fp8_mlp(new, fc, proj)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(z, want[1])
 
 
 def test_two_streams_at_once(device):
