@@ -9,15 +9,25 @@
  * the result, and a row's block of 128 meets across four lanes where the epilogue needs its largest magnitude. The results go
  * through LDS once more, so that a store instruction writes four whole rows of 256 bytes.
  *
- * Operands go from memory to LDS by DMA in stages of 128 k (128 bytes a row), two buffers in turn: a stage's wait and one
- * barrier without a memory fence, the next stage's DMA, then this stage's products. A row keeps its 16-byte piece b at place
- * b ^ swizzle(row), so that the 16 lanes that an LDS read serves at a time meet in different banks.
+ * Operands go from memory to LDS by DMA in stages of 128 k (128 bytes a row: rows of 64 took twice as long for a byte). A row keeps
+ * its 16-byte piece b at place b ^ swizzle(row), so that the 16 lanes that an LDS read serves at a time meet in different banks.
+ *
+ * Full tiles, 256 x 256 (two stages in LDS, one workgroup a CU): two waves a SIMD take turns at the matrix core. Bound by it: a stage
+ * takes 1.0 us, a tile about 8 more for its first stage and its results (8,192^3 411 us, 2,676 TFLOP/s; 65,536 x 4,992 x 1,664
+ * 504 us, 2,159; 65,536 x 1,664 x 6,656 599 us, 2,423; the ReLU^2 form of 65,536 x 6,656 x 1,664 615, its backward 858, which
+ * reads and writes 1.7 GB besides). Half tiles, 128 x 128, two workgroups a CU, and small ones, 64 x 128, three stages in LDS: for
+ * results that make fewer tiles; bound by LDS reads, 0.6 and 0.42 us a stage (1,001 x 5,120 x 1,280 11 us; 128 x 65,536 x 1,664
+ * 26 us, 4.2 TB/s of weights; 128 x 4,992 x 1,664 7.6). A ring of six stages for the small tile, of four for the half, took
+ * longer (8.7, 10.4 for 7.6 and 10.8): fewer workgroups a CU.
  *
  * Rows past M and N and columns past K read zeros (offsets past the buffer resource), and are not stored.
  *
  * The instruction adds the eight products of a lane's adjacent bytes at 13 bits below the largest of them (measured: beside
  * 2^16, 2^3 is kept and 2^2 is not, of either sign; products of other eights keep theirs) and everything else in fp32: 1.5e-5
- * relative error for normal values, 3e-5 with a few channels far above the others, against the 2e-3 of a bf16 result.
+ * relative error for normal values, 3e-5 with a few channels far above the others, against the 2e-3 of a bf16 result. Before a
+ * ReLU^2, whose result is rounded to 8 bits next, such an error lands on another code now and then: an MLP's result was 0.0029 off
+ * float64's in place of 0.0017. The small tiles, which have the time, take those products exactly, from the values in bf16; the
+ * others would take twice as long.
  */
 #include "nanochat_amd.h"
 #include "nc_fp8.h"
@@ -46,7 +56,12 @@ struct F8Gemm {
     unsigned char *q, *qs;               /* [M][N] codes and their scales at qs_stride (RELU2, RELU2_BWD: written) */
     const unsigned char *act, *acts;     /* [M][N] codes and scales at act_stride (RELU2_BWD: read) */
     long long qs_stride, act_stride;
+    bool q_stays;                        /* the codes are left in the caches */
 };
+/* Codes are what the next product reads: left in the caches (256 MB behind the L2s) where they fit with what else it takes. An MLP of
+ * 9,995 x 1,280/5,120, 51 MB of codes, 170 us past the caches, 157 through them; the training of 65,536 x 1,664/6,656, 436 MB, 5,108
+ * and 5,170. */
+constexpr long long FG_STAYS = 128LL << 20;
 
 template <int NU_, int WN_, int WM_, int RING_> struct FgTile {
     static constexpr int NU = NU_, WN = WN_, WM = WM_, RING = RING_, WAVES = WN * WM, TM = 16 * NU * WM, TN = F8_BLOCK * WN;
@@ -158,7 +173,7 @@ __device__ __forceinline__ FgPlace fg_place(const F8Gemm &g, long long m0, int n
     return p;
 }
 
-/* The K walk of the smaller tiles, four waves: P::RING stages in LDS, the DMA of RING - 1 ahead. Each wave moves 8 rows of every 32,
+/* The K walk of the smaller tiles, four waves: P::RING stages in LDS, the DMA of the next RING - 1 on its way. Each wave moves 8 rows of every 32,
  * and every fourth stage the scale dwords of its own operands' next four blocks (its rows of a by lane, its block of w). */
 constexpr int FG_OWN = 512;   /* bytes of a wave's scales of four stages: 64 dwords of a, then w's */
 template <class P, bool EXACT>
@@ -486,8 +501,11 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
             for (int k = 0; k < 2; k++) {
                 const int r = 8 * k + (lane >> 3), c = lane & 7;
                 const u32x4 d = *(const u32x4 *)(codes + fg_code_place(r, c));
-                if (16 * u + r < rows_left && col + 16 * c < cols)
-                    __builtin_nontemporal_store(d, (u32x4 *)(g.q + (first + 16 * u + r) * g.N + n0 + col + 16 * c));
+                if (16 * u + r < rows_left && col + 16 * c < cols) {
+                    u32x4 *const to = (u32x4 *)(g.q + (first + 16 * u + r) * g.N + n0 + col + 16 * c);
+                    if (g.q_stays) *to = d;
+                    else __builtin_nontemporal_store(d, to);
+                }
             }
         }
     }
@@ -559,12 +577,13 @@ F8Gemm fg_rows(F8Gemm g, long long from, long long count) {
  * 11.3; 300 x 16,384, 640, 18.5, 13.7. All sum in the same order.
  */
 long long fg_half_time(long long tiles, long long cus) { return tiles <= cus ? 4 : 5 * ((tiles + 2 * cus - 1) / (2 * cus)); }
-int fg_gemm(const F8Gemm &g, int epi, void *stream) {
+int fg_gemm(F8Gemm g, int epi, void *stream) {
     const int e = fg_check(g, epi);
     if (e != NC_OK || g.M == 0) return e;
     const hipStream_t s = (hipStream_t)stream;
     const long long cus = device_cus(), nx = (g.N + 255) / 256, full = (g.M + 255) / 256 * nx, half_nx = (g.N + 127) / 128;
     const long long small = (g.M + 63) / 64 * half_nx;
+    g.q_stays = g.M * g.N <= FG_STAYS;
     if (epi == FG_STORE && fp8_some_takes(g.M, g.N, g.K, cus))
         return fp8_some(g.a, g.as, g.as_stride, g.w, g.ws, g.ws_stride, (int)g.M, g.N, g.K, g.out, s);
     if (small <= cus) return fg_launch<FgSmall>(g, epi, s);
@@ -589,7 +608,7 @@ extern "C" int nc_fp8_matmul(const void *a, const void *a_scale, long long a_sca
                              int w_scale_stride, long long rows, int n, int k, void *out, void *stream) {
     const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
                       (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, (uint16_t *)out,
-                      nullptr, nullptr, nullptr, nullptr, 0, 0};
+                      nullptr, nullptr, nullptr, nullptr, 0, 0, false};
     return fg_gemm(g, FG_STORE, stream);
 }
 
@@ -598,7 +617,7 @@ extern "C" int nc_fp8_matmul_relu2(const void *a, const void *a_scale, long long
                                    void *scale, long long scale_stride, void *stream) {
     const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
                       (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, nullptr,
-                      (unsigned char *)codes, (unsigned char *)scale, nullptr, nullptr, scale_stride, 0};
+                      (unsigned char *)codes, (unsigned char *)scale, nullptr, nullptr, scale_stride, 0, false};
     return fg_gemm(g, FG_RELU2, stream);
 }
 
@@ -609,6 +628,6 @@ extern "C" int nc_fp8_matmul_relu2_bwd(const void *a, const void *a_scale, long 
     const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
                       (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, (uint16_t *)out,
                       (unsigned char *)codes, (unsigned char *)scale, (const unsigned char *)act,
-                      (const unsigned char *)act_scale, scale_stride, act_scale_stride};
+                      (const unsigned char *)act_scale, scale_stride, act_scale_stride, false};
     return fg_gemm(g, FG_RELU2_BWD, stream);
 }

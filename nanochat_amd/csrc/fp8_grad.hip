@@ -15,6 +15,10 @@
  *
  * The result is small and the sum long: where tiles alone would leave CUs idle the tokens are cut into slices, whose partial
  * tiles fp8_grad_sum_kernel adds in slice order, so the result does not depend on scheduling.
+ *
+ * Bound by the matrix cores at bf16's rate and by the LDS reads beside them: 65,536 x 4,992 x 1,664 943 us (1,154 TFLOP/s; a library
+ * product of 8,192^3 reaches 1,530), x 6,656 x 1,664 1,206, x 1,664 x 6,656 1,176; 16,384 x 5,120 x 1,280 199; 1,001 x 5,120 x 1,280
+ * 30, mostly its partial tiles. Eight waves of 64 x 128 with operands made by all took 1,444 where this takes 943.
  */
 #include "nanochat_amd.h"
 #include "nc_fp8.h"

@@ -1,24 +1,23 @@
 /*
- * Products of a few rows with a weight in the 8-bit form (nc_fp8.h) on gfx950: out[m][n] = epilogue(sum_k x8[m][k] w[n][k]) for at
- * most 128 rows m (a decoding step, draft tokens), x8 the 8-bit form of x's rows, made on the way for up to 16 rows. Bound by
- * reading w once.
+ * Products of few results with a weight in the 8-bit form (nc_fp8.h) on gfx950, out[m][n] = epilogue(sum_k x8[m][k] w[n][k]), x8 the
+ * 8-bit form of x's rows: a decoding step, draft tokens. Then a layer and an MLP for serving as one call each. Bound by reading w once,
+ * and below about 8 MB of it by latency: a launch, a row's way through k, the sums.
  *
- * Up to 16 rows (fp8_few_kernel): a wave holds 16 RT rows of w and x's 16 and walks blocks of 128 k, both operands from memory
- * straight into registers: lane (g = lane / 16, i = lane % 16) takes bytes 16 g .. + 15 and 64 + 16 g .. + 15 of row i's block, so
- * that a load instruction reads 64 adjacent bytes a row. Which k stands where in a product does not matter as long as both
- * operands agree. The eight waves of a workgroup take every eighth block. x comes in bf16 or fp32: a row's block lies in four
- * lanes, which find its largest magnitude together and make the codes that nc_fp8_quantize_rows makes.
+ * Up to 16 rows, x as it is (fp8_few_kernel): a workgroup holds 16 rows of w and x's 16, its eight waves take every eighth block of 128
+ * k, both operands from memory straight into registers: lane (g = lane / 16, i = lane % 16) takes bytes 16 g .. + 15 and 64 + 16 g ..
+ * + 15 of row i's block, so that a load instruction reads 64 adjacent bytes a row. Which k stands where in a product does not matter
+ * as long as both operands agree. x comes in bf16 or fp32: a row's block lies in four lanes, which find its largest magnitude together
+ * and make the codes that nc_fp8_quantize_rows makes. One row: 4,992 x 1,664 5.0 us, 16,384 x 1,664 8.7 us (3.1 TB/s of weights).
  *
- * 17 to 128 rows (fp8_some_kernel): x's codes would be read again by every wave, many times w's bytes. They go into LDS by DMA, a
- * ring of steps; eight waves stand RW by rows of w and S by blocks of k, w still straight into registers, up to six blocks ahead.
+ * Few tiles, x in 8 bits (fp8_some_kernel): the tiles of fp8_gemm.hip would leave CUs idle and walk a long k alone. 32 rows of x a
+ * workgroup, x's codes in LDS by DMA (a ring of steps), as all eight waves read them; the waves stand RW by 16 rows of w and S by blocks
+ * of k, w still straight into registers, up to six blocks ahead. 128 x 1,664 x 6,656 12.4 us (small tiles 21.3), 128 x 1,280 x 1,280
+ * 5.5 (6.2), 17 x 4,992 x 1,664 6.4 (7.5).
  *
  * The waves' fp32 sums meet in LDS and are added in a fixed order.
  *
- * Products: v_mfma_scale_f32_16x16x128_f8f6f4 for a bf16 result. Before a ReLU^2, whose result is rounded to 8 bits next, the
- * values are turned into bf16 (exact) and multiplied by v_mfma_f32_16x16x32_bf16, four instructions in place of one: the 8-bit
- * instruction drops bits below 2^-13 of the largest of eight products, and a sum off by 3e-5 lands on another code now and then
- * (the MLP's error against float64 was 0.0030 with it, 0.0017 without). There is time for it here; there is none in the products of
- * many rows.
+ * Products: v_mfma_scale_f32_16x16x128_f8f6f4 for a bf16 result; before a ReLU^2 exact ones, as fp8_gemm.hip says, by
+ * v_mfma_f32_16x16x32_bf16 from the values in bf16.
  */
 #include "nanochat_amd.h"
 #include "nc_fp8.h"
@@ -193,7 +192,8 @@ __device__ __forceinline__ int sk_swizzle(int row) {
     return (k & 3) | ((k + 2) & 4);
 }
 
-/* Step j: blocks j S + s of k. */
+/* Step j: blocks j S + s of k. RW, S 1, 8 and 2, 4, us: 64 x 1,280 x 1,280 4.8, 5.3; 128 x 1,280 x 1,280 8.4, 5.4; 64 x 1,664 x 6,656
+ * 9.6, 12.3; 128 x 1,664 x 6,656 17.4, 12.4; 17 x 4,992 x 1,664 8.9, 6.4. */
 constexpr int SK_BLOCKS = 128;   /* of a row at most: their scales are kept in LDS */
 template <int RW, int S>
 __global__ void __launch_bounds__(SK_WAVES *WAVE, S == 8 ? 2 : 4) fp8_some_kernel(Skinny p) {

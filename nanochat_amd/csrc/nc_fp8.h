@@ -1,12 +1,12 @@
 /*
- * The 8-bit form of matrices (fp8_quant.hip, fp8_gemm.hip, fp8_grad.hip): e4m3 codes and one power of two for each block of
+ * The 8-bit form of matrices (fp8_quant.hip, fp8_gemm.hip, fp8_skinny.hip, fp8_grad.hip): e4m3 codes and one power of two for each block of
  * 128 columns of a row (activations, gradients) or 128 x 128 of a weight, kept as its biased exponent (e8m0, a byte). A value
  * stands for code * 2^(byte - 127).
  *
  * The scale is the least power of two s with amax <= 448 s: amax = m 2^e with m in [1, 2) gives 2^(e - 8), doubled where m >
  * 1.75 (448 = 1.75 2^8). A block of zeros has scale 1. A power of two keeps the codes' relative error at half a step (2^-4)
  * whatever it is, down to amax 2^-15 / 1.75 or less where e4m3 becomes subnormal; it makes x / s exact, so a code is one
- * rounding of x, and code * s exact in bf16, which the matrix cores multiply as it is.
+ * rounding of x, and code * s exact in bf16 (from s = 2^-124 on), which the matrix cores multiply as it is.
  * A block with an infinity or a NaN becomes NaN whole (byte 255, every code 0x7F): what is made from it is NaN too.
  */
 #pragma once
