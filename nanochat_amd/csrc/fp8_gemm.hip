@@ -12,13 +12,14 @@
  * Operands go from memory to LDS by DMA in stages of 128 k (128 bytes a row: rows of 64 took twice as long for a byte). A row keeps
  * its 16-byte piece b at place b ^ swizzle(row), so that the 16 lanes that an LDS read serves at a time meet in different banks.
  *
- * Full tiles, 256 x 256 (two stages in LDS, one workgroup a CU): two waves a SIMD take turns at the matrix core. Bound by it: a stage
- * takes 1.0 us, a tile about 8 more for its first stage and its results (8,192^3 411 us, 2,676 TFLOP/s; 65,536 x 4,992 x 1,664
- * 504 us, 2,159; 65,536 x 1,664 x 6,656 599 us, 2,423; the ReLU^2 form of 65,536 x 6,656 x 1,664 615, its backward 858, which
- * reads and writes 1.7 GB besides). Half tiles, 128 x 128, two workgroups a CU, and small ones, 64 x 128, three stages in LDS: for
- * results that make fewer tiles; bound by LDS reads, 0.6 and 0.42 us a stage (1,001 x 5,120 x 1,280 11 us; 128 x 65,536 x 1,664
- * 26 us, 4.2 TB/s of weights; 128 x 4,992 x 1,664 7.6). A ring of six stages for the small tile, of four for the half, took
- * longer (8.7, 10.4 for 7.6 and 10.8): fewer workgroups a CU.
+ * Full tiles, 256 x 256 (two stages in LDS, one workgroup a CU): two waves a SIMD take turns at the matrix core. Bound by it: a
+ * stage takes 1.5 us (2,810 TFLOP/s over 256 CUs; a library product of 8,192^3 reaches 3,040), a tile about 5 more for its first
+ * operands and its results: 8,192^3 411 us (2,676 TFLOP/s); 65,536 x 4,992 x 1,664 496 (2,195); 65,536 x 1,664 x 6,656 599 (2,423); the
+ * ReLU^2 form of 65,536 x 6,656 x 1,664 615; its backward, which moves 1.7 GB besides, 858. Half tiles, 128 x 128, two workgroups a
+ * CU, and small ones, 64 x 128, three stages in LDS: for results that make fewer tiles. Bound by LDS reads and latency, 0.65 and 0.42
+ * us a stage: 1,001 x 5,120 x 1,280 11 us; 128 x 65,536 x 1,664 26 us (4.2 TB/s of weights); 128 x 4,992 x 1,664 7.6. Rings of six
+ * stages in small tiles and of four in half tiles leave room for one workgroup a CU: 256 x 4,992 x 1,664 7.7 -> 8.8 us, 1,001 x 4,992
+ * 13.4 -> 19.9.
  *
  * Rows past M and N and columns past K read zeros (offsets past the buffer resource), and are not stored.
  *
