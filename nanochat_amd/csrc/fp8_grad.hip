@@ -50,6 +50,12 @@ struct F8Grad {
     void *out;                                /* PART: fp32 [slices][N1][N2]; else the result [N1][N2] */
 };
 
+/* Two results over the same tokens in one launch: the first workgroups' and the others'. */
+struct F8Grads {
+    F8Grad of[2];
+    int first;                                /* workgroups of the first result */
+};
+
 /* LDS: four stages of dy, two of x in bf16, four of x's codes, eight of its scale dwords (a token's two blocks lie in one). */
 constexpr int GR_CODES = GR_KC * GR_T;
 constexpr int GR_X = 4 * GR_OPB, GR_XC = GR_X + 2 * GR_OPB, GR_XS = GR_XC + 4 * GR_CODES, GR_LDS = GR_XS + 8 * 128;
@@ -212,13 +218,16 @@ struct GrStep {
     } while (0)
 
 template <int MODE>
-__global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grad p) {
+__global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grads both) {
     __shared__ __align__(16) unsigned char lds[GR_LDS];
+    const bool second = (int)blockIdx.x >= both.first;
+    const F8Grad &p = both.of[second];
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const int wm = wave >> 1, wn = wave & 1;
     /* Workgroup L runs on XCD L % 8: each XCD takes a contiguous run of (slice, band of 4 row tiles, column tile, row tile), so
      * that what it runs at once reads the same tokens of few columns. */
-    const int tiles = p.tiles1 * p.tiles2, l = blockIdx.x, per = gridDim.x / 8, extra = gridDim.x % 8;
+    const int tiles = p.tiles1 * p.tiles2, l = second ? blockIdx.x - both.first : blockIdx.x;
+    const int count = second ? gridDim.x - both.first : both.first, per = count / 8, extra = count % 8;
     const int id = l % 8 * per + min(l % 8, extra) + l / 8, slice = id / tiles, tile = id % tiles;
     const int band = tile / (4 * p.tiles2), tall = min(4, p.tiles1 - 4 * band), in = tile - band * 4 * p.tiles2;
     const int i0 = (4 * band + in % tall) * GR_T, j0 = in / tall * GR_T;
@@ -363,79 +372,147 @@ double grad_time(long long tiles, long long elements, int cus, long long slices,
     return rounds * (rows / GR_KC + 10) * (0.6 + 0.15 * busy) + partials;
 }
 
-/* Token slices: the best of a few counts by grad_time (small ones, steps of about a quarter above, and those that just fill one
- * to six rounds), none under GR_MIN_ROWS rows unless it is the only one and none whose operand slice passes 1 GiB. */
-void grad_slices(long long M, int N1, int N2, int &slices, int &rows) {
-    const long long tiles = (long long)((N1 + GR_T - 1) / GR_T) * ((N2 + GR_T - 1) / GR_T);
-    const long long wide = (long long)N1 * 2 > N2 ? (long long)N1 * 2 : N2;
-    const long long fit = (1LL << 30) / wide / GR_KC * GR_KC;
+/* How the tokens of one result, or of two in one launch, are cut. */
+struct GrPlan {
+    int slices, rows;
+    double time;
+};
+/* The best of a few counts by grad_time (small ones, steps of about a quarter above, and those that just fill one to six rounds),
+ * no slice under GR_MIN_ROWS rows unless it is the only one and none whose operand slice passes 1 GiB. */
+GrPlan grad_plan(long long M, long long tiles, long long elements, long long row_bytes) {
+    const long long fit = (1LL << 30) / row_bytes / GR_KC * GR_KC;
     const long long least = (M + fit - 1) / fit, most = (M + GR_MIN_ROWS - 1) / GR_MIN_ROWS;
     const int cus = device_cus();
-    double best = -1.0;
-    slices = rows = 0;
+    GrPlan best = {0, 0, -1.0};
     auto consider = [&](long long s) {
         s = s < most ? s : most;
         s = s > least ? s : least;
         const long long r = ((M + s - 1) / s + GR_KC - 1) / GR_KC * GR_KC;
         if (r > fit) return;
         s = (M + r - 1) / r;   /* no empty slice */
-        const double t = grad_time(tiles, (long long)N1 * N2, cus, s, r);
-        if (best >= 0.0 && t >= best) return;
-        best = t;
-        slices = (int)s;
-        rows = (int)r;
+        const double t = grad_time(tiles, elements, cus, s, r);
+        if (best.time < 0.0 || t < best.time) best = {(int)s, (int)r, t};
     };
     for (long long s = 1; s <= most && (s == 1 || tiles * s <= 6LL * cus); s += s < 8 ? 1 : s / 4) consider(s);
     for (int k = 1; k <= 6; k++)
         if (k * cus >= tiles) consider(k * cus / tiles);
+    return best;
+}
+int tiles_of(int n) { return (n + GR_T - 1) / GR_T; }
+long long row_of(int n1, int n2) { return 2LL * n1 > n2 ? 2LL * n1 : n2; }
+GrPlan grad_alone(long long M, int n1, int n2) {
+    return grad_plan(M, (long long)tiles_of(n1) * tiles_of(n2), (long long)n1 * n2, row_of(n1, n2));
+}
+/* Both in one launch, where that takes less time than one after the other (with slices = 0: it does not). 200 tiles for 256 CUs are
+ * one round in place of two of 100: 1,001 tokens x (5,120 x 1,280 and 1,280 x 5,120) 64 -> 34 us. */
+GrPlan grad_both(long long M, const int (&n1)[2], const int (&n2)[2]) {
+    const long long r0 = row_of(n1[0], n2[0]), r1 = row_of(n1[1], n2[1]);
+    const GrPlan both = grad_plan(M, (long long)tiles_of(n1[0]) * tiles_of(n2[0]) + (long long)tiles_of(n1[1]) * tiles_of(n2[1]),
+                                  (long long)n1[0] * n2[0] + (long long)n1[1] * n2[1], r0 > r1 ? r0 : r1);
+    return both.time < 0.95 * (grad_alone(M, n1[0], n2[0]).time + grad_alone(M, n1[1], n2[1]).time) ? both : GrPlan{0, 0, 0.0};
 }
 
 /* One slice needs none (never 0 where there is a call). */
-long long grad_bytes(int slices, int N1, int N2) { return slices == 1 ? 16 : (long long)slices * N1 * N2 * 4; }
+long long grad_bytes(int slices, long long elements) { return slices == 1 ? 16 : slices * elements * 4; }
 
 bool grad_fits(long long M, int N1, int N2) {
     return M >= 0 && M < (1LL << 31) && N1 > 0 && N2 > 0 && N1 % 8 == 0 && N2 % 16 == 0 && N1 <= 65536 && N2 <= 65536;
 }
 
+/* Sizes first, then pointers, then their alignment. A slice's scales take no more bytes than its codes. */
+int grad_check(const GradOf &g, long long rows, const void *workspace) {
+    if (!grad_fits(rows, g.n1, g.n2) || g.mode < 0 || g.mode > 2 || g.scale_stride < (g.n2 + F8_BLOCK - 1) / F8_BLOCK ||
+        g.scale_stride > g.n2)
+        return NC_ERR_SHAPE;
+    if (rows == 0) return NC_OK;
+    if (!g.dy || !g.codes || !g.scale || !g.out || !workspace) return NC_ERR_NULL;
+    return ((uintptr_t)g.dy | (uintptr_t)g.codes | (uintptr_t)g.out | (uintptr_t)workspace) & 15 ? NC_ERR_SHAPE : NC_OK;
+}
+
+int grad_launch(const GradOf *g, int results, const GrPlan &plan, long long rows, void *workspace, hipStream_t s) {
+    F8Grads both = {};
+    int workgroups = 0;
+    char *part = (char *)workspace;
+    void *parts[2];
+    for (int i = 0; i < results; i++) {
+        both.of[i] = {(const uint16_t *)g[i].dy, (const unsigned char *)g[i].codes, (const unsigned char *)g[i].scale,
+                      g[i].scale_stride, rows, g[i].n1, g[i].n2, tiles_of(g[i].n1), tiles_of(g[i].n2), plan.slices, plan.rows,
+                      plan.slices == 1 ? g[i].out : part};
+        parts[i] = part;
+        part += (long long)plan.slices * g[i].n1 * g[i].n2 * 4;
+        workgroups += both.of[i].tiles1 * both.of[i].tiles2 * plan.slices;
+        if (i == 0) both.first = workgroups;
+    }
+    const auto kernel = plan.slices > 1    ? fp8_grad_kernel<GR_PART>
+                        : g[0].mode == 0   ? fp8_grad_kernel<GR_F32>
+                        : g[0].mode == 1   ? fp8_grad_kernel<GR_ADD> : fp8_grad_kernel<GR_BF16>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)workgroups), dim3(GR_WAVES * WAVE), 0, s, both);
+    for (int i = 0; plan.slices > 1 && i < results; i++) {
+        const long long n4 = (long long)g[i].n1 * g[i].n2 / 4;
+        const auto sum = g[i].mode == 0 ? fp8_grad_sum_kernel<GR_F32> : g[i].mode == 1 ? fp8_grad_sum_kernel<GR_ADD>
+                                                                                           : fp8_grad_sum_kernel<GR_BF16>;
+        hipLaunchKernelGGL(sum, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, s, (const float4 *)parts[i], plan.slices, n4,
+                           g[i].out);
+    }
+    return (int)hipGetLastError();
+}
+
+/* Two results can share a launch that writes them itself only in one mode; partials are alike. */
+GrPlan grad_shared(long long rows, const int (&n1)[2], const int (&n2)[2], int mode0, int mode1) {
+    const GrPlan both = grad_both(rows, n1, n2);
+    return both.slices > 1 || mode0 == mode1 ? both : GrPlan{0, 0, 0.0};
+}
+
 }  // namespace
+
+long long fp8_weight_grads_bytes(long long rows, int n1, int n2, int mode, int m1, int m2, int other) {
+    if (!grad_fits(rows, n1, n2) || !grad_fits(rows, m1, m2)) return -1;
+    if (rows == 0) return 0;
+    const int a[2] = {n1, m1}, b[2] = {n2, m2};
+    const GrPlan both = grad_shared(rows, a, b, mode, other);
+    const long long x = nc_fp8_weight_grad_workspace_bytes(rows, n1, n2), y = nc_fp8_weight_grad_workspace_bytes(rows, m1, m2);
+    const long long z = both.slices ? grad_bytes(both.slices, (long long)n1 * n2 + (long long)m1 * m2) : 0;
+    return x > y ? x > z ? x : z : y > z ? y : z;   /* both plans: which one it is depends on the results' places */
+}
+
+/* Results that overlap (one buffer that both are added to) are not made at once. */
+static bool grads_overlap(const GradOf (&g)[2]) {
+    const char *at[2], *end[2];
+    for (int i = 0; i < 2; i++) {
+        at[i] = (const char *)g[i].out;
+        end[i] = at[i] + (long long)g[i].n1 * g[i].n2 * (g[i].mode == 2 ? 2 : 4);
+    }
+    return at[0] < end[1] && at[1] < end[0];
+}
+
+int fp8_weight_grads(const GradOf (&g)[2], long long rows, void *workspace, long long workspace_bytes, hipStream_t stream) {
+    for (int i = 0; i < 2; i++)
+        if (const int e = grad_check(g[i], rows, workspace)) return e;
+    if (rows == 0) return NC_OK;
+    const int a[2] = {g[0].n1, g[1].n1}, b[2] = {g[0].n2, g[1].n2};
+    const GrPlan both = grad_shared(rows, a, b, g[0].mode, g[1].mode);
+    if (workspace_bytes < fp8_weight_grads_bytes(rows, a[0], b[0], g[0].mode, a[1], b[1], g[1].mode)) return NC_ERR_WORKSPACE;
+    if (both.slices && !grads_overlap(g)) return grad_launch(g, 2, both, rows, workspace, stream);
+    const int status = grad_launch(g, 1, grad_alone(rows, a[0], b[0]), rows, workspace, stream);
+    return status ? status : grad_launch(g + 1, 1, grad_alone(rows, a[1], b[1]), rows, workspace, stream);
+}
+
 }  // namespace nc
 
 using namespace nc;
 
 extern "C" long long nc_fp8_weight_grad_workspace_bytes(long long rows, int n1, int n2) {
     if (!grad_fits(rows, n1, n2)) return -1;
-    if (rows == 0) return 0;
-    int slices, per;
-    grad_slices(rows, n1, n2, slices, per);
-    return grad_bytes(slices, n1, n2);
+    return rows == 0 ? 0 : grad_bytes(grad_alone(rows, n1, n2).slices, (long long)n1 * n2);
 }
 
 extern "C" int nc_fp8_weight_grad(const void *dy, const void *codes, const void *scale, long long scale_stride, long long rows,
                                   int n1, int n2, int mode, void *out, void *workspace, long long workspace_bytes,
                                   void *stream) {
-    if (!grad_fits(rows, n1, n2) || mode < 0 || mode > 2 || scale_stride < (n2 + F8_BLOCK - 1) / F8_BLOCK ||
-        scale_stride > n2)   /* a slice's scales take no more bytes than its codes */
-        return NC_ERR_SHAPE;
-    if (rows == 0) return NC_OK;
-    if (!dy || !codes || !scale || !out || !workspace) return NC_ERR_NULL;
-    if (((uintptr_t)dy | (uintptr_t)codes | (uintptr_t)out | (uintptr_t)workspace) & 15) return NC_ERR_SHAPE;
-    F8Grad p = {(const uint16_t *)dy, (const unsigned char *)codes, (const unsigned char *)scale, scale_stride, rows, n1, n2,
-                (n1 + GR_T - 1) / GR_T, (n2 + GR_T - 1) / GR_T, 0, 0, out};
-    grad_slices(rows, n1, n2, p.slices, p.rows);
-    if (workspace_bytes < grad_bytes(p.slices, n1, n2)) return NC_ERR_WORKSPACE;
-    const long long tiles = (long long)((n1 + GR_T - 1) / GR_T) * p.tiles2;
-    const dim3 grid((unsigned)(tiles * p.slices)), block(GR_WAVES * WAVE);
-    const hipStream_t s = (hipStream_t)stream;
-    if (p.slices == 1) {
-        const auto kernel = mode == 0 ? fp8_grad_kernel<GR_F32> : mode == 1 ? fp8_grad_kernel<GR_ADD> : fp8_grad_kernel<GR_BF16>;
-        hipLaunchKernelGGL(kernel, grid, block, 0, s, p);
-        return (int)hipGetLastError();
-    }
-    p.out = workspace;
-    hipLaunchKernelGGL(fp8_grad_kernel<GR_PART>, grid, block, 0, s, p);
-    const long long n4 = (long long)n1 * n2 / 4;
-    const auto sum = mode == 0 ? fp8_grad_sum_kernel<GR_F32> : mode == 1 ? fp8_grad_sum_kernel<GR_ADD>
-                                                                           : fp8_grad_sum_kernel<GR_BF16>;
-    hipLaunchKernelGGL(sum, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, s, (const float4 *)workspace, p.slices, n4, out);
-    return (int)hipGetLastError();
+    const GradOf g = {dy, codes, scale, scale_stride, n1, n2, mode, out};
+    const int e = grad_check(g, rows, workspace);
+    if (e != NC_OK || rows == 0) return e;
+    const GrPlan plan = grad_alone(rows, n1, n2);
+    if (workspace_bytes < grad_bytes(plan.slices, (long long)n1 * n2)) return NC_ERR_WORKSPACE;
+    return grad_launch(&g, 1, plan, rows, workspace, (hipStream_t)stream);
 }

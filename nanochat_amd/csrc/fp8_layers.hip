@@ -90,10 +90,11 @@ extern "C" long long nc_fp8_mlp_bwd_workspace_bytes(long long rows, int c, int h
     if (!layer_sizes(rows, hidden, c) || !layer_sizes(rows, c, hidden) || !layer_sizes(rows, n, hidden) ||
         !layer_sizes(rows, hidden, n) || fc_mode < NONE || fc_mode > 2 || proj_mode < NONE || proj_mode > 2)
         return -1;
-    const long long f = grad_need(rows, hidden, c, fc_mode), p = grad_need(rows, n, hidden, proj_mode);
-    if (f < 0 || p < 0) return -1;
     const bool inner = need_x || fc_mode != NONE;
-    return (inner ? f8_form_bytes(rows, n) + up16(2 * rows * hidden) + f8_form_bytes(rows, hidden) : 0) + (f > p ? f : p);
+    const long long grads = fc_mode != NONE && proj_mode != NONE
+                                ? fp8_weight_grads_bytes(rows, hidden, c, fc_mode, n, hidden, proj_mode)
+                            : fc_mode != NONE ? grad_need(rows, hidden, c, fc_mode) : grad_need(rows, n, hidden, proj_mode);
+    return grads < 0 ? -1 : (inner ? f8_form_bytes(rows, n) + up16(2 * rows * hidden) + f8_form_bytes(rows, hidden) : 0) + grads;
 }
 
 extern "C" int nc_fp8_mlp_bwd(const void *dy, long long row_stride, const void *codes, const void *scale, long long scale_stride,
@@ -110,13 +111,12 @@ extern "C" int nc_fp8_mlp_bwd(const void *dy, long long row_stride, const void *
         return NC_ERR_NULL;
     if (misaligned(workspace, 16) || workspace_bytes < need) return NC_ERR_WORKSPACE;
     int status = NC_OK;
-    unsigned char *rest = (unsigned char *)workspace;
+    unsigned char *rest = (unsigned char *)workspace, *dh = nullptr;
     if (inner) {
         const F8Form f(rest, rows, n);
-        unsigned char *const dh = rest + f.bytes;
+        dh = rest + f.bytes;
         const F8Form h(dh + up16(2 * rows * hidden), rows, hidden);
         rest = h.codes + h.bytes;
-        const long long left = need - (rest - (unsigned char *)workspace);
         status = nc_fp8_quantize_rows(dy, 0, row_stride, rows, n, f.codes, f.scale, f.pitch, stream);
         if (!status)
             status = nc_fp8_matmul_relu2_bwd(f.codes, f.scale, f.pitch, proj_codes_t, proj_scale_t, proj_scale_t_stride, rows,
@@ -124,11 +124,16 @@ extern "C" int nc_fp8_mlp_bwd(const void *dy, long long row_stride, const void *
         if (!status && dx)
             status = nc_fp8_matmul(h.codes, h.scale, h.pitch, fc_codes_t, fc_scale_t, fc_scale_t_stride, rows, c, hidden, dx,
                                    stream);
-        if (!status && fc_mode != NONE)
-            status = nc_fp8_weight_grad(dh, codes, scale, scale_stride, rows, hidden, c, fc_mode, dfc, rest, left, stream);
     }
+    const long long left = need - (rest - (unsigned char *)workspace);
+    if (!status && fc_mode != NONE && proj_mode != NONE) {
+        const GradOf g[2] = {{dh, codes, scale, scale_stride, hidden, c, fc_mode, dfc},
+                             {dy, act, act_scale, act_scale_stride, n, hidden, proj_mode, dproj}};
+        return fp8_weight_grads(g, rows, rest, left, (hipStream_t)stream);
+    }
+    if (!status && fc_mode != NONE)
+        status = nc_fp8_weight_grad(dh, codes, scale, scale_stride, rows, hidden, c, fc_mode, dfc, rest, left, stream);
     if (!status && proj_mode != NONE)
-        status = nc_fp8_weight_grad(dy, act, act_scale, act_scale_stride, rows, n, hidden, proj_mode, dproj, rest,
-                                    need - (rest - (unsigned char *)workspace), stream);
+        status = nc_fp8_weight_grad(dy, act, act_scale, act_scale_stride, rows, n, hidden, proj_mode, dproj, rest, left, stream);
     return status;
 }

@@ -57,6 +57,17 @@ bool fp8_some_takes(long long rows, int n, int k, long long cus);
 int fp8_some(const void *codes, const void *scale, long long scale_stride, const void *w, const void *w_scale, int w_scale_stride,
              int rows, int n, int k, void *out, hipStream_t stream);
 
+/* fp8_grad.hip: two nc_fp8_weight_grad over the same tokens, in one launch where that is faster; the workspace for two results n1 x n2
+ * and m1 x m2 in modes mode and other (-1: unsupported sizes). */
+struct GradOf {
+    const void *dy, *codes, *scale;
+    long long scale_stride;
+    int n1, n2, mode;
+    void *out;
+};
+long long fp8_weight_grads_bytes(long long rows, int n1, int n2, int mode, int m1, int m2, int other);
+int fp8_weight_grads(const GradOf (&g)[2], long long rows, void *workspace, long long workspace_bytes, hipStream_t stream);
+
 /* The decode step's GEMM operands: out[n][r] = epilogue(sum_k x[n][k] w[r][k]), bf16 operands, fp32 sums,
  * N <= SG_MAX_N rows. */
 constexpr int SG_MAX_N = 128;

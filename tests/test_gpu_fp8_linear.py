@@ -428,6 +428,29 @@ def test_training_mlp(device, m, c, f, n, dtype):
     close(codes_of(dx), want, off8 @ np.abs(f8) + (2.0 ** -10 + f * EPS) * m8 + 2.0 ** -8 * m8)
 
 
+@pytest.mark.parametrize("rows", [1, 33, 700, 9000])
+@pytest.mark.parametrize("fc_type,proj_type,add", [(F32, F32, False), (BF16, BF16, False), (F32, BF16, False), (F32, F32, True)])
+def test_both_weight_gradients_of_an_mlp(device, rows, fc_type, proj_type, add):
+    """dfc and dproj, which may share a launch, against float64 from the operands that the op's own parts make."""
+    gen = torch.Generator().manual_seed(rows)
+    c, hidden, n = 272, 1040, 144
+    x, dy = rowwise(gen, rows, c).to(device), bf(gen, rows, n).to(device)
+    fc = (torch.randn(hidden, c, generator=gen) / 16).to(fc_type).to(device).requires_grad_()
+    proj = (torch.randn(n, hidden, generator=gen) / 32).to(proj_type).to(device).requires_grad_()
+    buffers = [torch.full(w.shape, 3.0, device=device) for w in (fc, proj)] if add else [None, None]
+    y = fl.checkpointed_mlp(x, fc, proj, fc_grad=buffers[0], proj_grad=buffers[1])
+    got = torch.autograd.grad(y, (fc, proj), dy, allow_unused=True) if not add else (y.backward(dy), buffers)[1]
+    x8 = fl.quantize_rows(x)
+    f8, p8 = fl.quantize_weight(fc.detach(), True), fl.quantize_weight(proj.detach(), True)
+    act = product_relu2(*x8, f8)
+    dh = product_relu2_bwd(*fl.quantize_rows(dy), fl.Fp8Weight(p8.codes_t, p8.scale_t), *act)[0]
+    full = lambda codes, scale: torch.from_numpy(fb.values(codes_of(codes), exps_of(scale), 1))   # noqa: E731
+    for g, left, right, t in zip(got, (dh, dy), (full(*x8), full(*act)), (fc_type, proj_type)):
+        left = left.double().cpu()
+        want, mag = left.t() @ right + (3.0 if add else 0.0), left.abs().t() @ right.abs() + (3.0 if add else 0.0)
+        close(codes_of(g), want.numpy(), (mag * (rows + 2) * EPS + (2.0 ** -8 * want.abs() if t == BF16 else 0.0)).numpy())
+
+
 def test_one_buffer_for_two_uses(device):
     """A weight used twice adds both its gradients to one buffer, which may be cleared between the forward and the backward."""
     gen = torch.Generator().manual_seed(11)
