@@ -299,11 +299,32 @@ __device__ __forceinline__ void fg_phase_end() {
 constexpr int FG_WAIT_LDS = 0xC07F;   /* s_waitcnt lgkmcnt(0) alone */
 constexpr int FG_WAIT_DMA = 0x0F70;   /* s_waitcnt vmcnt(0) alone */
 
+/* RELU2_BWD: a wave's 64 x 128 codes of a, which come as a stage behind the last, into the buffer that is free by then: 8 rows an
+ * instruction, their places fg_code_place's. From memory behind the walk they took 7 us a tile of 37 (65,536 x 6,656 x 1,664). */
+struct FgAct {
+    u32x4 r;
+    uint32_t at, to;
+    int N;
+    __device__ __forceinline__ FgAct(const F8Gemm &g, const FgPlace &p, long long m0, int n0, const unsigned char *buffer) {
+        r = f8_words(g.act + m0 * g.N + n0, (long long)p.rows * g.N - n0);
+        const int row = p.lane >> 3, col = F8_BLOCK * p.wn + 16 * ((p.lane & 7) ^ row);
+        N = g.N;
+        at = col < p.cols ? (uint32_t)((64 * p.wm + row) * N + col) : (uint32_t)FG_PAST;   /* also with 56 N added */
+        to = f8_lds(buffer) + p.wave * 8192;
+    }
+    template <int S> __device__ __forceinline__ void issue() const { f8_dma16(to + S * 1024, at + 8 * S * N, r); }
+};
+
+template <bool ACT>
 __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *lds,
                                              f32x4 (&acc)[8][4]) {
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
     const bool first = p.wave < 4;
     FgDma dma(g, p, m0, n0, lds);
+    const auto fetch_act = [&]() {
+        const FgAct act(g, p, m0, n0, lds + (stages & 1) * FgFull::STAGE);
+        fg_unroll<8>([&](auto s) { act.issue<decltype(s)::value>(); });
+    };
 #pragma unroll
     for (int t = 0; t < 8; t++)
 #pragma unroll
@@ -320,6 +341,8 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
         if (1 < stages) {
             dma.stage(1, p.wave);
             fg_unroll<8>([&](auto s) { dma.issue<decltype(s)::value>(); });
+        } else if (ACT) {
+            fetch_act();
         }
         fg_phase_end();
     }
@@ -332,6 +355,7 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
             dma.stage(j + 1, p.wave);
             fg_unroll<8>([&](auto s) { dma.issue<decltype(s)::value>(); });
         }
+        if (ACT && first && j + 1 == stages) fetch_act();
 #pragma unroll
         for (int u = 0; u < 4; u++) {
             sa[u] = sc[(p.row0 + 16 * u) * 4];
@@ -346,6 +370,7 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
         fg_phase_end();
         __builtin_amdgcn_s_setprio(1);
         if (next) dma.stage(j + 2, p.wave);
+        if (ACT && !first && j + 2 == stages) fetch_act();
         fg_unroll<8>([&](auto t) {
             constexpr int T = decltype(t)::value;
             fg_unroll<4>([&](auto u) {
@@ -385,7 +410,13 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (P::WAVES == 8) fg_walk_full(g, p, m0, n0, b0, acc);
+    constexpr bool FULL = P::WAVES == 8, ACT_STAGE = FULL && EPI == FG_RELU2_BWD;
+    uint32_t act_bytes = 127u;   /* ACT_STAGE: the scale byte of the wave's row `lane` */
+    if constexpr (ACT_STAGE) {
+        const int row = 64 * p.wm + p.lane;
+        if (row < p.rows && p.some) act_bytes = g.acts[(m0 + row) * g.act_stride + p.nb];
+    }
+    if constexpr (FULL) fg_walk_full<ACT_STAGE>(g, p, m0, n0, b0, acc);
     else fg_walk_ring<P, P::NU == 1 && EPI == FG_RELU2>(g, p, m0, n0, b0, acc);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));   /* made again, not kept through the walk */
@@ -396,12 +427,18 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
     if (!some) return;
     const int lane = tid & (WAVE - 1), rows_left = rows - 16 * P::NU * p.wm, col = F8_BLOCK * wn;   /* this wave's */
     const long long first = m0 + 16 * P::NU * p.wm;
-    unsigned char *mine = b0 + (threadIdx.x >> 6) * FG_TURN;
+    const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
+    unsigned char *mine = b0 + (threadIdx.x >> 6) * FG_TURN + (ACT_STAGE ? (stages - 1 & 1) * P::STAGE : 0);
+    const unsigned char *act_at = b0 + (stages & 1) * P::STAGE + (threadIdx.x >> 6) * 8192;   /* ACT_STAGE */
     const int r16 = lane & 15;
-    /* RELU2_BWD: a's codes, a piece of 16 columns a lane of rows 8 k + lane / 8 of each 16, and its scales; all on their way at once */
+    /* RELU2_BWD: a's scales, and in the smaller tiles its codes, a piece of 16 columns a lane of rows 8 k + lane / 8 of each 16; all on
+     * their way at once */
     u32x4 act[P::NU][2];
     uint32_t act_byte[P::NU];
-    if constexpr (EPI == FG_RELU2_BWD) {
+    if constexpr (ACT_STAGE) {
+#pragma unroll
+        for (int u = 0; u < P::NU; u++) act_byte[u] = __shfl(act_bytes, 16 * u + r16);
+    } else if constexpr (EPI == FG_RELU2_BWD) {
 #pragma unroll
         for (int u = 0; u < P::NU; u++) {
 #pragma unroll
@@ -446,15 +483,18 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
             if constexpr (EPI == FG_RELU2_BWD) {
                 /* dh = da 2 sqrt(a) */
                 unsigned char *codes = mine + 16 * 256;
-                fg_wave_order();
+                if constexpr (!ACT_STAGE) {
+                    fg_wave_order();
 #pragma unroll
-                for (int k = 0; k < 2; k++) *(u32x4 *)(codes + fg_code_place(8 * k + (lane >> 3), lane & 7)) = act[u][k];
-                fg_wave_order();
+                    for (int k = 0; k < 2; k++) *(u32x4 *)(codes + fg_code_place(8 * k + (lane >> 3), lane & 7)) = act[u][k];
+                    fg_wave_order();
+                }
+                const unsigned char *from = ACT_STAGE ? act_at + u * 16 * 128 : codes;
                 const float s = f8_scale(act_byte[u]);
                 uint32_t m = 0u;
 #pragma unroll
                 for (int h = 0; h < 4; h++) {
-                    const u32x2 c = *(const u32x2 *)(codes + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1));
+                    const u32x2 c = *(const u32x2 *)(from + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1));
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const auto a = (k & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[k >> 1], s, true)
