@@ -15,7 +15,7 @@
  * Full tiles, 256 x 256 (two stages in LDS, one workgroup a CU): two waves a SIMD take turns at the matrix core. Bound by it: a
  * stage takes 1.5 us (2,810 TFLOP/s over 256 CUs; a library product of 8,192^3 reaches 3,040), a tile about 5 more for its first
  * operands and its results: 8,192^3 411 us (2,676 TFLOP/s); 65,536 x 4,992 x 1,664 496 (2,195); 65,536 x 1,664 x 6,656 599 (2,423); the
- * ReLU^2 form of 65,536 x 6,656 x 1,664 615; its backward, which moves 1.7 GB besides, 858. Half tiles, 128 x 128, two workgroups a
+ * ReLU^2 form of 65,536 x 6,656 x 1,664 615; its backward, which moves 1.7 GB besides, 829. Half tiles, 128 x 128, two workgroups a
  * CU, and small ones, 64 x 128, three stages in LDS: for results that make fewer tiles. Bound by LDS reads and latency, 0.65 and 0.42
  * us a stage: 1,001 x 5,120 x 1,280 11 us; 128 x 65,536 x 1,664 26 us (4.2 TB/s of weights); 128 x 4,992 x 1,664 7.6. Rings of six
  * stages in small tiles and of four in half tiles leave room for one workgroup a CU: 256 x 4,992 x 1,664 7.7 -> 8.8 us, 1,001 x 4,992
@@ -300,7 +300,7 @@ constexpr int FG_WAIT_LDS = 0xC07F;   /* s_waitcnt lgkmcnt(0) alone */
 constexpr int FG_WAIT_DMA = 0x0F70;   /* s_waitcnt vmcnt(0) alone */
 
 /* RELU2_BWD: a wave's 64 x 128 codes of a, which come as a stage behind the last, into the buffer that is free by then: 8 rows an
- * instruction, their places fg_code_place's. From memory behind the walk they took 7 us a tile of 37 (65,536 x 6,656 x 1,664). */
+ * instruction, their places fg_code_place's. From memory behind the walk they took 4 us more a tile (65,536 x 6,656 x 1,664 861 us -> 829). */
 struct FgAct {
     u32x4 r;
     uint32_t at, to;
