@@ -28,6 +28,7 @@ from .native import check, device_guard, hip_library, pointer, stream
 BLOCK = 128
 CODES, SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu
 BF16, F32 = torch.bfloat16, torch.float32
+MOST = 65536   # a weight's rows and columns in training, as its gradient's kernel has them
 
 
 class Fp8Weight(NamedTuple):
@@ -277,8 +278,8 @@ def _held(weight: Tensor, name: str, codes: Tensor | None, scale: Tensor | None,
           scale_t: Tensor | None, grad: Tensor | None, device: torch.device) -> tuple[Tensor, Tensor, int, Tensor, Tensor]:
     """A layer's arguments checked -> codes, scales and their pitch in the 8-bit form that its op uses, then what its backward
     reads: from what it was given (that then empty, as the caller holds it), or the weight's own form, made now."""
-    if weight.dim() != 2 or weight.size(0) % 16 or weight.size(1) % 16 or weight.numel() == 0:
-        raise ValueError(f"{name} must be [N, K], both multiples of 16, got {tuple(weight.shape)}")
+    if weight.dim() != 2 or weight.size(0) % 16 or weight.size(1) % 16 or weight.numel() == 0 or max(weight.shape) > MOST:
+        raise ValueError(f"{name} must be [N, K], both multiples of 16 up to {MOST}, got {tuple(weight.shape)}")
     if weight.dtype not in (BF16, F32):
         raise TypeError(f"{name} must be {BF16} or {F32}, got {weight.dtype}")
     if weight.device != device:
@@ -430,7 +431,7 @@ _NOT_HELD = (None, None, None, None)
 
 def checkpointed_linear(x: Tensor, weight: Tensor, weight8: Fp8Weight | None = None, grad: Tensor | None = None) -> Tensor:
     """x bf16 [..., K] through a linear layer in 8-bit products, bf16 [..., N], differentiable in x and weight (bf16 or fp32
-    [N, K], N and K multiples of 16). Kept for the backward is x's 8-bit form alone, not x. With x8, dy8, w8 the 8-bit forms:
+    [N, K], N and K multiples of 16 up to 65,536). Kept for the backward is x's 8-bit form alone, not x. With x8, dy8, w8 the 8-bit forms:
 
         y = x8 w8^T      dx = dy8 w8      dw = dy^T x8   (dy itself, fp32 sums)
 
@@ -544,7 +545,7 @@ class _Mlp(torch.autograd.Function):
 def checkpointed_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc8: Fp8Weight | None = None, proj8: Fp8Weight | None = None,
                      fc_grad: Tensor | None = None, proj_grad: Tensor | None = None) -> Tensor:
     """x bf16 [..., C] through proj(relu(fc(x))^2) in 8-bit products, bf16 [..., N], differentiable in x, fc [F, C] and proj
-    [N, F] (bf16 or fp32, all sizes multiples of 16). Kept for the backward are the 8-bit forms of x and of the squared
+    [N, F] (bf16 or fp32, all sizes multiples of 16 up to 65,536). Kept for the backward are the 8-bit forms of x and of the squared
     activations a, C + F bytes a token where bf16 keeps x, the sums before the square and the squares in 2 C + 4 F. With x8
     and so on the 8-bit forms, f8 and p8 the weights':
 

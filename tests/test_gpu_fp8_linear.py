@@ -555,6 +555,33 @@ def test_refusals_on_the_device(device):
     torch.cuda.synchronize()
 
 
+def test_training_refuses_what_its_gradient_cannot_take(device):
+    """Before the forward, not in the backward."""
+    x, w = torch.zeros(2, 16, dtype=BF16, device=device), torch.zeros(65552, 16, dtype=BF16, device=device)
+    for call in (lambda: fl.checkpointed_linear(x, w), lambda: fl.checkpointed_linear(w[:2].view(-1, 16), w),
+                 lambda: fl.checkpointed_mlp(x, w, w.t().contiguous())):
+        with pytest.raises(ValueError, match="65536"):
+            call()
+    y = fl.checkpointed_linear(x.requires_grad_(), w[:65536].requires_grad_())
+    y.sum().backward()
+    assert x.grad.shape == x.shape
+
+
+def test_ops_give_what_their_fakes_say(device):
+    """(The schema check of the same tool multiplies outputs, which torch does not do in 8 bits.)"""
+    gen = torch.Generator().manual_seed(12)
+    x, w, p = bf(gen, 5, 144).to(device), bf(gen, 272, 144).to(device), bf(gen, 32, 272).to(device)
+    some = (None,) * 4
+    utils = ("test_faketensor",)
+    torch.library.opcheck(torch.ops.nanochat_amd.checkpointed_linear, (x, w, *some, None), test_utils=utils)
+    torch.library.opcheck(torch.ops.nanochat_amd.checkpointed_mlp, (x, w, p, *some, None, *some, None), test_utils=utils)
+    out = torch.ops.nanochat_amd.checkpointed_linear(x, w, *some, None)
+    grad = torch.zeros(272, 144, device=device)
+    for buffer in (None, grad):
+        torch.library.opcheck(torch.ops.nanochat_amd.checkpointed_linear_bwd, (out[0], *out[1:], buffer, True, True, False),
+                              test_utils=utils)
+
+
 # --- together
 
 def block(x, layers):
