@@ -66,10 +66,11 @@ constexpr long long FG_STAYS = 128LL << 20;
 
 template <int NU_, int WN_, int WM_, int RING_> struct FgTile {
     static constexpr int NU = NU_, WN = WN_, WM = WM_, RING = RING_, WAVES = WN * WM, TM = 16 * NU * WM, TN = F8_BLOCK * WN;
+    static constexpr bool FULL = TM == 256;
     static constexpr int ROWS = TM + TN, STAGE = ROWS * FG_ROWB, LOADS = ROWS / 8 / WAVES, A_LOADS = TM / 8 / WAVES;
     static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0, "DMA split");
 };
-typedef FgTile<4, 2, 4, 2> FgFull;   /* 256 x 256, 8 waves, two stages in LDS */
+typedef FgTile<8, 2, 2, 2> FgFull;   /* 256 x 256, 4 waves of 128 x 128, two stages in LDS */
 typedef FgTile<2, 1, 4, 2> FgHalf;   /* 128 x 128, 4 waves */
 typedef FgTile<1, 1, 4, 3> FgSmall;  /* 64 x 128, 4 waves */
 
@@ -234,73 +235,59 @@ __device__ __forceinline__ void fg_walk_ring(const F8Gemm &g, const FgPlace &p, 
     fg_barrier();   /* the epilogue writes where other waves may still read and DMA may still land */
 }
 
-/* The K walk of the full tile: waves 0-3 and 4-7, one of each a SIMD, take turns: while one's 32 products keep the matrix core
- * busy, the other reads its next 12 operands into registers. A phase ends with a barrier; waves 0-3 read stage j in phase 2 j
- * and multiply in 2 j + 1, waves 4-7 a phase later. Stage j + 1's DMA is issued in phase 2 j, when every wave has read stage j -
- * 1: by waves 0-3 among their reads, by waves 4-7 among their products. It has landed at the end of phase 2 j + 1. */
-/* The products as inline assembly: accumulators that stay in the same four AGPRs for the whole walk ("+a"), where the compiler
- * moved them about. It does not see matrix instructions there and inserts none of their wait states; they are kept by
- * construction. Operands are written by LDS reads alone, waited for at the phase's end; scales by memory reads and shifts before
- * that wait; an accumulator is used again 31 products later, and read only 32 wait states after the last product. */
+/* The products as inline assembly: accumulators that stay in the same four AGPRs for the whole walk ("+a"; all 256 of a wave, one a
+ * SIMD), where the compiler moved them about. It does not see matrix instructions there and inserts none of their wait states; they
+ * are kept by construction: operands and scales are written by LDS reads alone, a quarter of a stage ahead; an accumulator is used
+ * again 63 products later, and read only 32 wait states after the last product. */
 __device__ __forceinline__ void fg_mfma(f32x4 &c, const i32x8 &w, const i32x8 &a, uint32_t sw, uint32_t sa) {
     asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
                  : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
 }
 
-/* The full tile's DMA: instruction s = 0 .. 3 of a and of w moves rows 64 s + 8 wave + lane / 8; every fourth stage another
- * brings the scale dwords of its four blocks (waves 0-3: of rows 64 wave + lane; wave 4: of the two blocks of w). */
-constexpr int FG_SCALES = 1280;   /* bytes of a group's scales in LDS: 256 dwords of a, then w's, behind both stage buffers */
+/* The full tile's DMA: instruction s = 0 .. 7 of w and of a moves rows 32 s + 8 wave + lane / 8; every fourth stage three more bring the
+ * scale dwords of four blocks that the wave itself needs (its 128 rows of a, its block of w). */
+constexpr int FG_SCALES = 768;    /* bytes of a wave's scales of four blocks: 128 dwords of a, then w's in each lane's place */
 struct FgDma {
-    u32x4 ra, rw, rs;
-    uint32_t lds, scales;         /* this wave's addresses in stage buffer 0 and in the first scale buffer */
-    int first, ca, cw, K;         /* the lane's row of s = 0, and its pieces */
-    int scale_at;
-    int oa, ow;                   /* a stage's offsets */
-    uint32_t to;
+    u32x4 ra, rw, rsa, rsw;
+    uint32_t lds, scales;         /* this wave's addresses in stage buffer 0 and of its first scales */
+    int ca, cw, first, K;         /* the lane's pieces and its row of s = 0 */
+    int scale_at, more;           /* the offset of its row's scales, and of 64 rows */
+    uint32_t oa, ow, to;          /* the stage being fetched */
     __device__ __forceinline__ FgDma(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0) {
         ra = f8_words(g.a + m0 * g.K, (long long)p.rows * g.K);
         rw = f8_words(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
-        const bool of_a = p.wave < 4;
-        const int blocks = (p.cols + F8_BLOCK - 1) / F8_BLOCK;
-        rs = of_a ? f8_words(g.as + m0 * g.as_stride, p.rows * g.as_stride)
-                  : f8_words(g.ws + (long long)(n0 / F8_BLOCK) * g.ws_stride, (long long)blocks * g.ws_stride);
-        scale_at = of_a ? (64 * p.wave + p.lane) * (int)g.as_stride : p.lane < blocks ? p.lane * g.ws_stride : FG_PAST;
+        rsa = f8_words(g.as + m0 * g.as_stride, p.rows * g.as_stride);
+        rsw = f8_words(g.ws + (long long)(p.some ? p.nb : 0) * g.ws_stride, g.ws_stride);
+        scale_at = (128 * p.wm + p.lane) * (int)g.as_stride;
+        more = 64 * (int)g.as_stride;
         lds = f8_lds(b0) + p.wave * 1024;
-        scales = f8_lds(b0) + 2 * FgFull::STAGE + p.wave * 256;
+        scales = f8_lds(b0) + 2 * FgFull::STAGE + p.wave * 2 * FG_SCALES;
         K = g.K;
         const int row = 8 * p.wave + (p.lane >> 3), pos = p.lane & 7;
         first = row * K;
         ca = (pos ^ fg_swizzle_a(row)) << 4;
-        cw = (pos ^ fg_swizzle_w(row)) << 4;   /* rows 64 on have the same */
+        cw = (pos ^ fg_swizzle_w(row)) << 4;   /* rows 32 on have the same */
     }
-    /* Stage j's offsets, and its scales' DMA where it is the first of four. */
-    __device__ __forceinline__ void stage(int j, int wave) {
+    /* Stage j's offsets, and its scales' DMA where it is the first of four. Past K they lie past the range, also with 224 K added. */
+    __device__ __forceinline__ void stage(int j) {
         const int k = j * FG_ROWB;
-        oa = first + ca + k;
-        ow = first + cw + k;
-        if (k + FG_ROWB > K) {   /* a short last block: pieces past it lie past the range, also with 192 K added */
-            oa = ca + k < K ? oa : FG_PAST;
-            ow = cw + k < K ? ow : FG_PAST;
-        }
+        oa = k + ca < K ? first + ca + k : FG_PAST;
+        ow = k + cw < K ? first + cw + k : FG_PAST;
         to = lds + (j & 1) * FgFull::STAGE;
-        if ((j & 3) == 0 && wave <= 4)
-            f8_dma4(scales + ((j >> 2) & 1) * FG_SCALES, scale_at + j, rs);
+        if ((j & 3) == 0) {
+            const uint32_t own = scales + ((j >> 2) & 1) * FG_SCALES;
+            f8_dma4(own, scale_at + j, rsa);
+            f8_dma4(own + 256, scale_at + more + j, rsa);
+            f8_dma4(own + 512, j, rsw);
+        }
     }
-    template <int S> __device__ __forceinline__ void issue() const {   /* S: 0 .. 3 a, 4 .. 7 w */
-        f8_dma16(to + S * 8192, (S < 4 ? oa : ow) + 64 * (S & 3) * K, S < 4 ? ra : rw);
-    }
+    template <int S> __device__ __forceinline__ void issue_w() const { f8_dma16<FgFull::TM * FG_ROWB + S * 4096>(to, ow, 32 * S * K, rw); }
+    template <int S> __device__ __forceinline__ void issue_a() const { f8_dma16<S * 4096>(to, oa, 32 * S * K, ra); }
 };
 
-__device__ __forceinline__ void fg_phase_end() {
-    __builtin_amdgcn_sched_barrier(0);
-    fg_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-}
-constexpr int FG_WAIT_LDS = 0xC07F;   /* s_waitcnt lgkmcnt(0) alone */
-constexpr int FG_WAIT_DMA = 0x0F70;   /* s_waitcnt vmcnt(0) alone */
-
-/* RELU2_BWD: a wave's 64 x 128 codes of a, which come as a stage behind the last, into the buffer that is free by then: 8 rows an
- * instruction, their places fg_code_place's. From memory behind the walk they took 4 us more a tile (65,536 x 6,656 x 1,664 861 us -> 829). */
+/* RELU2_BWD: a wave's 128 x 128 codes of a, which come as a stage behind the last, into the buffer that is free by then: 8 rows an
+ * instruction, their places fg_code_place's. From memory behind the walk they took 4 us more a tile (65,536 x 6,656 x 1,664 861 us
+ * -> 829). */
 struct FgAct {
     u32x4 r;
     uint32_t at, to;
@@ -309,88 +296,137 @@ struct FgAct {
         r = f8_words(g.act + m0 * g.N + n0, (long long)p.rows * g.N - n0);
         const int row = p.lane >> 3, col = F8_BLOCK * p.wn + 16 * ((p.lane & 7) ^ row);
         N = g.N;
-        at = col < p.cols ? (uint32_t)((64 * p.wm + row) * N + col) : (uint32_t)FG_PAST;   /* also with 56 N added */
-        to = f8_lds(buffer) + p.wave * 8192;
+        at = col < p.cols ? (uint32_t)((128 * p.wm + row) * N + col) : (uint32_t)FG_PAST;   /* also with 120 N added */
+        to = f8_lds(buffer) + p.wave * 16384;
     }
     template <int S> __device__ __forceinline__ void issue() const { f8_dma16(to + S * 1024, at + 8 * S * N, r); }
 };
 
+/* All but the N newest DMA have landed, and this wave's LDS reads are done. */
+template <int N> __device__ __forceinline__ void fg_wait() {
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0x0 << 8));
+}
+
+/*
+ * The K walk of the full tile: a wave a SIMD, its 64 products of a stage in four quarters of 16, each of four of w's eight operands
+ * with four of a's: (w low, first of a), (low, second), (high, second), (high, first); what is "first" changes from stage to stage.
+ * So half of w's registers are free from the middle of a stage on and half of a's for its last quarter, and take the next stage's
+ * operands there; the other halves come in the next stage's first half. A stage's buffer has been read by the middle of the stage:
+ * the DMA of the stage after next goes there, w's part in the third quarter, a's in the fourth. Two barriers a stage: in the middle
+ * (everyone has read w of this buffer; w of the next stage has landed) and before the last quarter (a of the next stage has).
+ */
+struct FgWalk {
+    const unsigned char *lds, *own;       /* the workgroup's LDS, this wave's scales */
+    int a_at, w_at, i;
+    i32x8 w[8], a[8];
+    uint32_t sa[2][8], sw[2];             /* scale bytes of even and of odd stages */
+    template <int T> __device__ __forceinline__ void read_w(const unsigned char *buf) {
+        w[T] = fg_operand(buf, w_at + fg_column(T, 0) * FG_ROWB, (w_at ^ 16) + fg_column(T, 0) * FG_ROWB);
+    }
+    template <int U> __device__ __forceinline__ void read_a(const unsigned char *buf) {
+        a[U] = fg_operand(buf, a_at + U * 16 * FG_ROWB, (a_at ^ 16) + U * 16 * FG_ROWB);
+    }
+    template <int U, int ODD> __device__ __forceinline__ void read_scale(int j) {   /* of stage j; U = 8: w's */
+        const unsigned char *sc = own + ((j >> 2) & 1) * FG_SCALES + (j & 3);
+        if constexpr (U == 8) sw[ODD] = sc[512];
+        else sa[ODD][U] = sc[(16 * U + i) * 4];
+    }
+    /* The bytes as whole registers from their reads on: else the compiler clears their upper bits right before the products. */
+    template <int ODD> __device__ __forceinline__ void pin() {
+#pragma unroll
+        for (int u = 0; u < 8; u++) asm volatile("" : "+v"(sa[ODD][u]));
+        asm volatile("" : "+v"(sw[ODD]));
+    }
+    /* What is done behind product I: of stage j, FIRST (its parity) which half of a comes first. act_next: the
+     * DMA is not of stage j + 2 but of act. */
+    template <int I, int FIRST> __device__ __forceinline__ void side(int j, FgDma &dma, bool act_next, const FgAct *act) {
+        const unsigned char *cur = lds + (j & 1) * FgFull::STAGE, *next = lds + (1 - (j & 1)) * FgFull::STAGE;
+        if constexpr (I < 8 && I % 2 == 1) read_a<4 * (1 - FIRST) + I / 2>(cur);
+        if constexpr (I >= 8 && I < 24 && I % 4 == 1) read_w<4 + (I - 8) / 4>(cur);
+        if constexpr (I >= 32 && I < 40 && I % 2 == 1) read_w<(I - 32) / 2>(next);
+        if constexpr (I >= 48 && I < 56 && I % 2 == 1) read_a<4 * (1 - FIRST) + (I - 48) / 2>(next);
+        if constexpr (I >= 56 && I < 62 && I % 2 == 1) {
+            read_scale<3 * ((I - 56) / 2), 1 - FIRST>(j + 1);
+            read_scale<3 * ((I - 56) / 2) + 1, 1 - FIRST>(j + 1);
+            read_scale<3 * ((I - 56) / 2) + 2, 1 - FIRST>(j + 1);
+        }
+        if constexpr (I == 63) pin<1 - FIRST>();
+        if constexpr (I >= 32 && I % 2 == 0) {
+            constexpr int S = (I - 32) / 2;   /* 0 .. 7 w, 8 .. 15 a */
+            if (act_next) act->template issue<S>();
+            else if constexpr (S < 8) dma.template issue_w<S>();
+            else dma.template issue_a<S - 8>();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    template <int I, int FIRST>
+    __device__ __forceinline__ void run(f32x4 (&acc)[8][8], int j, FgDma &dma, bool act_next, const FgAct *act) {
+        if constexpr (I < 64) {
+            constexpr int Q = I / 16, T = 4 * (Q / 2) + I % 16 / 4, U = 4 * ((Q == 0 || Q == 3) ? FIRST : 1 - FIRST) + I % 4;
+            if constexpr (I == 32) {
+                fg_wait<8>();       /* w of stage j + 1; a's eight are newer */
+                fg_barrier();
+                dma.stage(j + 2);
+            }
+            if constexpr (I == 48) {
+                if ((j & 3) == 2) fg_wait<11>();   /* a of stage j + 1; w of stage j + 2 is newer, its scales too where it brought any */
+                else fg_wait<8>();
+                fg_barrier();
+            }
+            fg_mfma(acc[T][U], w[T], a[U], sw[FIRST], sa[FIRST][U]);
+            side<I, FIRST>(j, dma, act_next, act);
+            run<I + 1, FIRST>(acc, j, dma, act_next, act);
+        }
+    }
+};
+
 template <bool ACT>
 __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *lds,
-                                             f32x4 (&acc)[8][4]) {
+                                             f32x4 (&acc)[8][8]) {
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
-    const bool first = p.wave < 4;
     FgDma dma(g, p, m0, n0, lds);
-    const auto fetch_act = [&]() {
-        const FgAct act(g, p, m0, n0, lds + (stages & 1) * FgFull::STAGE);
-        fg_unroll<8>([&](auto s) { act.issue<decltype(s)::value>(); });
-    };
+    const FgAct act(ACT ? g : F8Gemm{}, p, ACT ? m0 : 0, ACT ? n0 : 0, lds + (stages & 1) * FgFull::STAGE);
 #pragma unroll
     for (int t = 0; t < 8; t++)
 #pragma unroll
-        for (int u = 0; u < 4; u++) asm volatile("" : "=a"(acc[t][u]) : "0"(acc[t][u]));
-    dma.stage(0, p.wave);
-    fg_unroll<8>([&](auto s) { dma.issue<decltype(s)::value>(); });
-    const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
+        for (int u = 0; u < 8; u++) asm volatile("" : "=a"(acc[t][u]) : "0"(acc[t][u]));
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        dma.stage(j);
+        if (ACT && j == stages) {
+            fg_unroll<16>([&](auto s) { act.template issue<decltype(s)::value>(); });
+        } else {
+            fg_unroll<8>([&](auto s) { dma.template issue_w<decltype(s)::value>(); });
+            fg_unroll<8>([&](auto s) { dma.template issue_a<decltype(s)::value>(); });
+        }
+    }
+    FgWalk k;
+    k.lds = lds;
+    k.own = lds + 2 * FgFull::STAGE + p.wave * 2 * FG_SCALES;
+    k.i = p.i;
+    k.a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
     const int w_row = F8_BLOCK * p.wn + fg_column(0, p.i >> 2) + (p.i & 3);
-    const int w_at = (FgFull::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
-    const unsigned char *scales = lds + 2 * FgFull::STAGE;
+    k.w_at = (FgFull::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
+    fg_wait<16>();   /* stage 0 */
+    fg_barrier();
+    fg_unroll<4>([&](auto t) {
+        k.template read_w<decltype(t)::value>(lds);
+        k.template read_a<decltype(t)::value>(lds);
+    });
+    fg_unroll<9>([&](auto u) { k.template read_scale<decltype(u)::value, 0>(0); });
+    k.template pin<0>();
+    for (int j = 0; j < stages; j += 2) {
+        k.template run<0, 0>(acc, j, dma, ACT && j + 2 == stages, &act);
+        if (j + 1 >= stages) break;
+        k.template run<0, 1>(acc, j + 1, dma, ACT && j + 3 == stages, &act);
+    }
     __builtin_amdgcn_s_waitcnt(0);
-    fg_phase_end();
-    if (!first) {   /* phase 0 */
-        if (1 < stages) {
-            dma.stage(1, p.wave);
-            fg_unroll<8>([&](auto s) { dma.issue<decltype(s)::value>(); });
-        } else if (ACT) {
-            fetch_act();
-        }
-        fg_phase_end();
-    }
-    for (int j = 0; j < stages; j++) {
-        const unsigned char *cur = lds + (j & 1) * FgFull::STAGE, *sc = scales + ((j >> 2) & 1) * FG_SCALES + (j & 3);
-        i32x8 fa[4], fw[8];
-        uint32_t sa[4], sw;
-        const bool mine = first && j + 1 < stages, next = !first && j + 2 < stages;
-        if (mine) {
-            dma.stage(j + 1, p.wave);
-            fg_unroll<8>([&](auto s) { dma.issue<decltype(s)::value>(); });
-        }
-        if (ACT && first && j + 1 == stages) fetch_act();
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            sa[u] = sc[(p.row0 + 16 * u) * 4];
-            fa[u] = fg_operand(cur, a_at + u * 16 * FG_ROWB, (a_at ^ 16) + u * 16 * FG_ROWB);
-        }
-        sw = sc[1024 + 4 * p.wn];
-#pragma unroll
-        for (int t = 0; t < 8; t++)
-            fw[t] = fg_operand(cur, w_at + fg_column(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column(t, 0) * FG_ROWB);
-        __builtin_amdgcn_s_waitcnt(FG_WAIT_LDS);
-        if (!first) __builtin_amdgcn_s_waitcnt(FG_WAIT_DMA);
-        fg_phase_end();
-        __builtin_amdgcn_s_setprio(1);
-        if (next) dma.stage(j + 2, p.wave);
-        if (ACT && !first && j + 2 == stages) fetch_act();
-        fg_unroll<8>([&](auto t) {
-            constexpr int T = decltype(t)::value;
-            fg_unroll<4>([&](auto u) {
-                constexpr int U = decltype(u)::value;
-                fg_mfma(acc[T][U], fw[T], fa[U], sw, sa[U]);
-                if constexpr (U == 1) {   /* spread: in bursts they held up the products behind them */
-                    if (next) dma.issue<T>();
-                }
-            });
-        });
-        __builtin_amdgcn_s_setprio(0);
-        if (first) __builtin_amdgcn_s_waitcnt(FG_WAIT_DMA);
-        fg_phase_end();
-    }
-    if (first) fg_phase_end();
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");   /* 32 wait states; no read moves above */
+    fg_barrier();   /* the epilogue writes where other waves may still read and DMA may still land */
 #pragma unroll
     for (int t = 0; t < 8; t++)
 #pragma unroll
-        for (int u = 0; u < 4; u++) asm volatile("" : "+a"(acc[t][u]));
+        for (int u = 0; u < 8; u++) asm volatile("" : "+a"(acc[t][u]));
 }
 
 /* A wave's part of LDS behind its walk: 16 rows of 256 bytes, then 16 of 128. */
@@ -410,13 +446,16 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr bool FULL = P::WAVES == 8, ACT_STAGE = FULL && EPI == FG_RELU2_BWD;
-    uint32_t act_bytes = 127u;   /* ACT_STAGE: the scale byte of the wave's row `lane` */
+    constexpr bool ACT_STAGE = P::FULL && EPI == FG_RELU2_BWD;
+    uint32_t act_bytes[2] = {127u, 127u};   /* ACT_STAGE: the scale bytes of the wave's rows `lane` and 64 on */
     if constexpr (ACT_STAGE) {
-        const int row = 64 * p.wm + p.lane;
-        if (row < p.rows && p.some) act_bytes = g.acts[(m0 + row) * g.act_stride + p.nb];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int row = 128 * p.wm + 64 * h + p.lane;
+            if (row < p.rows && p.some) act_bytes[h] = g.acts[(m0 + row) * g.act_stride + p.nb];
+        }
     }
-    if constexpr (FULL) fg_walk_full<ACT_STAGE>(g, p, m0, n0, b0, acc);
+    if constexpr (P::FULL) fg_walk_full<ACT_STAGE>(g, p, m0, n0, b0, acc);
     else fg_walk_ring<P, P::NU == 1 && EPI == FG_RELU2>(g, p, m0, n0, b0, acc);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));   /* made again, not kept through the walk */
@@ -429,7 +468,7 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
     const long long first = m0 + 16 * P::NU * p.wm;
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
     unsigned char *mine = b0 + (threadIdx.x >> 6) * FG_TURN + (ACT_STAGE ? (stages - 1 & 1) * P::STAGE : 0);
-    const unsigned char *act_at = b0 + (stages & 1) * P::STAGE + (threadIdx.x >> 6) * 8192;   /* ACT_STAGE */
+    const unsigned char *act_at = b0 + (stages & 1) * P::STAGE + (threadIdx.x >> 6) * 16384;   /* ACT_STAGE */
     const int r16 = lane & 15;
     /* RELU2_BWD: a's scales, and in the smaller tiles its codes, a piece of 16 columns a lane of rows 8 k + lane / 8 of each 16; all on
      * their way at once */
@@ -437,7 +476,7 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
     uint32_t act_byte[P::NU];
     if constexpr (ACT_STAGE) {
 #pragma unroll
-        for (int u = 0; u < P::NU; u++) act_byte[u] = __shfl(act_bytes, 16 * u + r16);
+        for (int u = 0; u < P::NU; u++) act_byte[u] = __shfl(act_bytes[u / 4], 16 * (u % 4) + r16);
     } else if constexpr (EPI == FG_RELU2_BWD) {
 #pragma unroll
         for (int u = 0; u < P::NU; u++) {
@@ -562,8 +601,8 @@ __device__ __forceinline__ int2 fg_tile(int l, int count, int nx) {
 }
 
 template <class P, int EPI>
-__global__ void __launch_bounds__(P::WAVES *WAVE, 2) fp8_gemm_kernel(F8Gemm g) {
-    __shared__ __align__(16) unsigned char lds[P::RING * P::STAGE + (P::WAVES == 8 ? 2 * FG_SCALES : P::WAVES * 2 * FG_OWN)];
+__global__ void __launch_bounds__(P::WAVES *WAVE, P::FULL ? 1 : 2) fp8_gemm_kernel(F8Gemm g) {
+    __shared__ __align__(16) unsigned char lds[P::RING * P::STAGE + P::WAVES * 2 * (P::FULL ? FG_SCALES : FG_OWN)];
     const int2 t = fg_tile(blockIdx.x, gridDim.x, (g.N + P::TN - 1) / P::TN);
     fg_run<P, EPI>(g, (long long)t.y * P::TM, t.x * P::TN, lds);
 }

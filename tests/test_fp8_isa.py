@@ -16,7 +16,7 @@ import pytest
 from nanochat_amd import native
 from tests.test_prefill_gemm_isa import blocks, loop_lines, regs, wait_states_before_agpr_reads, writer_kind
 
-ASM = {"gemm": ("fp8_gemm.hip", r"_ZN2nc12_GLOBAL__N_115fp8_gemm_kernelINS0_6FgTileILi4ELi2ELi4ELi2EEELi([012])EEEvNS0_6F8GemmE"),
+ASM = {"gemm": ("fp8_gemm.hip", r"_ZN2nc12_GLOBAL__N_115fp8_gemm_kernelINS0_6FgTileILi8ELi2ELi2ELi2EEELi([012])EEEvNS0_6F8GemmE"),
        "grad": ("fp8_grad.hip", r"_ZN2nc12_GLOBAL__N_115fp8_grad_kernelILi([0123])EEEvNS0_7F8GradsE")}
 KERNELS = [("gemm", e) for e in range(3)] + [("grad", m) for m in range(4)]
 
