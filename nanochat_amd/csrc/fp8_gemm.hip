@@ -429,7 +429,7 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
         for (int u = 0; u < 8; u++) asm volatile("" : "+a"(acc[t][u]));
 }
 
-/* A wave's part of LDS behind its walk: 16 rows of 256 bytes, then 16 of 128. */
+/* A wave's parts of LDS behind its walk, two in turn: 16 rows of 256 bytes, then 16 of 128. */
 constexpr int FG_TURN = 16 * 384;
 __device__ __forceinline__ int fg_code_place(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 /* Lanes of one wave exchange values through LDS, which serves a wave's accesses in order; the compiler keeps the order too. */
@@ -489,15 +489,24 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
             act_byte[u] = r < rows_left ? g.acts[(first + r) * g.act_stride + nb] : 127u;
         }
     }
+    /* Rows 16 u + r16: this lane's results, columns 32 h + 8 grp + 0 .. 7, into the wave's turn buffer u % 2 */
+    u32x2 c_next[4];   /* ACT_STAGE: a's codes of the rows after next */
+    const auto read_act = [&](int u) {
 #pragma unroll
-    for (int u = 0; u < P::NU; u++) {
-        const int row = 16 * u + r16;                         /* this lane's results: columns 32 h + 8 grp + 0 .. 7 */
+        for (int h = 0; h < 4; h++)
+            c_next[h] = *(const u32x2 *)(act_at + u * 16 * 128 + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1));
+    };
+    if constexpr (ACT_STAGE) read_act(0);
+    const auto make = [&](int u) {
+        const int row = 16 * u + r16;
+        unsigned char *const turn = mine + u % 2 * P::WAVES * FG_TURN, *const codes = turn + 16 * 256;
         float v[32];
 #pragma unroll
         for (int t = 0; t < 8; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) v[4 * t + e] = acc[t][u][e];
         u32x2 q[4];
+        uint32_t o[16];
         if constexpr (EPI == FG_RELU2) {
             uint32_t m = 0u;
 #pragma unroll
@@ -517,66 +526,73 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
                     q[h][k] = byte == F8_NAN_BYTE ? F8_NAN_CODES : f8_codes(v[z], v[z + 1], v[z + 2], v[z + 3], s);
                 }
             if (row < rows_left && grp == 0) g.qs[(first + row) * g.qs_stride + nb] = (unsigned char)byte;
-        } else {
-            uint32_t o[16];
-            if constexpr (EPI == FG_RELU2_BWD) {
-                /* dh = da 2 sqrt(a) */
-                unsigned char *codes = mine + 16 * 256;
-                if constexpr (!ACT_STAGE) {
-                    fg_wave_order();
+        } else if constexpr (EPI == FG_RELU2_BWD) {
+            /* dh = da 2 sqrt(a) */
+            u32x2 c[4];
+            if constexpr (ACT_STAGE) {
 #pragma unroll
-                    for (int k = 0; k < 2; k++) *(u32x4 *)(codes + fg_code_place(8 * k + (lane >> 3), lane & 7)) = act[u][k];
-                    fg_wave_order();
-                }
-                const unsigned char *from = ACT_STAGE ? act_at + u * 16 * 128 : codes;
-                const float s = f8_scale(act_byte[u]);
-                uint32_t m = 0u;
+                for (int h = 0; h < 4; h++) c[h] = c_next[h];
+                if (u + 1 < P::NU) read_act(u + 1);
+            } else {
+                fg_wave_order();
 #pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    const u32x2 c = *(const u32x2 *)(from + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1));
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const auto a = (k & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[k >> 1], s, true)
-                                               : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[k >> 1], s, false);
-                        /* v_sqrt_f32 is within an ulp; the result is rounded to bf16 right away */
-                        const float x = v[8 * h + 2 * k] * (2.0f * __builtin_amdgcn_sqrtf(a[0]));
-                        const float y = v[8 * h + 2 * k + 1] * (2.0f * __builtin_amdgcn_sqrtf(a[1]));
-                        o[4 * h + k] = bf16_pair(x, y);
-                        m = pair_amax(m, o[4 * h + k]);
-                    }
-                }
-                const uint32_t byte = f8_scale_byte(group_max(pair_top(m)));
-                const float qs = f8_scale(byte);
+                for (int k = 0; k < 2; k++) *(u32x4 *)(codes + fg_code_place(8 * k + (lane >> 3), lane & 7)) = act[u][k];
+                fg_wave_order();
 #pragma unroll
                 for (int h = 0; h < 4; h++)
-                    q[h] = byte == F8_NAN_BYTE ? u32x2{F8_NAN_CODES, F8_NAN_CODES}
-                                               : u32x2{f8_codes(o[4 * h], o[4 * h + 1], qs),
-                                                       f8_codes(o[4 * h + 2], o[4 * h + 3], qs)};
-                if (row < rows_left && grp == 0) g.qs[(first + row) * g.qs_stride + nb] = (unsigned char)byte;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 16; k++) o[k] = bf16_pair(v[2 * k], v[2 * k + 1]);
+                    c[h] = *(const u32x2 *)(codes + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1));
             }
-            fg_wave_order();
+            const float s = f8_scale(act_byte[u]);
+            uint32_t m = 0u;
 #pragma unroll
             for (int h = 0; h < 4; h++)
-                *(u32x4 *)(mine + r16 * 256 + (((4 * h + grp) ^ r16) << 4)) =
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const auto a = (k & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[h][k >> 1], s, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[h][k >> 1], s, false);
+                    /* v_sqrt_f32 is within an ulp; the result is rounded to bf16 right away */
+                    const float x = v[8 * h + 2 * k] * (2.0f * __builtin_amdgcn_sqrtf(a[0]));
+                    const float y = v[8 * h + 2 * k + 1] * (2.0f * __builtin_amdgcn_sqrtf(a[1]));
+                    o[4 * h + k] = bf16_pair(x, y);
+                    m = pair_amax(m, o[4 * h + k]);
+                }
+            const uint32_t byte = f8_scale_byte(group_max(pair_top(m)));
+            const float qs = f8_scale(byte);
+#pragma unroll
+            for (int h = 0; h < 4; h++)
+                q[h] = byte == F8_NAN_BYTE ? u32x2{F8_NAN_CODES, F8_NAN_CODES}
+                                           : u32x2{f8_codes(o[4 * h], o[4 * h + 1], qs), f8_codes(o[4 * h + 2], o[4 * h + 3], qs)};
+            if (row < rows_left && grp == 0) g.qs[(first + row) * g.qs_stride + nb] = (unsigned char)byte;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; k++) o[k] = bf16_pair(v[2 * k], v[2 * k + 1]);
+        }
+        fg_wave_order();
+        if constexpr (EPI != FG_RELU2) {
+#pragma unroll
+            for (int h = 0; h < 4; h++)
+                *(u32x4 *)(turn + r16 * 256 + (((4 * h + grp) ^ r16) << 4)) =
                     u32x4{o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]};
-            fg_wave_order();
+        }
+        if constexpr (EPI != FG_STORE) {
+#pragma unroll
+            for (int h = 0; h < 4; h++) *(u32x2 *)(codes + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1)) = q[h];
+        }
+        fg_wave_order();
+    };
+    /* ... and from there whole rows to memory */
+    const auto send = [&](int u) {
+        const unsigned char *const turn = mine + u % 2 * P::WAVES * FG_TURN, *const codes = turn + 16 * 256;
+        if constexpr (EPI != FG_RELU2) {
 #pragma unroll
             for (int k = 0; k < 4; k++) {   /* four rows an instruction, past the caches: larger than they are, and read much later */
                 const int r = 4 * k + (lane >> 4), c = lane & 15;
-                const u32x4 d = *(const u32x4 *)(mine + r * 256 + ((c ^ r) << 4));
+                const u32x4 d = *(const u32x4 *)(turn + r * 256 + ((c ^ r) << 4));
                 if (16 * u + r < rows_left && col + 8 * c < cols)
                     __builtin_nontemporal_store(d, (u32x4 *)(g.out + (first + 16 * u + r) * g.N + n0 + col + 8 * c));
             }
         }
         if constexpr (EPI != FG_STORE) {
-            unsigned char *codes = mine + 16 * 256;
-            fg_wave_order();
-#pragma unroll
-            for (int h = 0; h < 4; h++) *(u32x2 *)(codes + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1)) = q[h];
-            fg_wave_order();
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const int r = 8 * k + (lane >> 3), c = lane & 7;
@@ -588,7 +604,14 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
                 }
             }
         }
+    };
+    make(0);
+#pragma unroll
+    for (int u = 1; u < P::NU; u++) {   /* the next rows are made while these are on their way through LDS */
+        make(u);
+        send(u - 1);
     }
+    send(P::NU - 1);
 }
 
 /* The order workgroups take tiles in. Workgroup L runs on XCD L % 8, each with its own L2: XCD k gets a contiguous run of the
