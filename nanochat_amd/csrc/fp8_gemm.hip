@@ -12,14 +12,17 @@
  * Operands go from memory to LDS by DMA in stages of 128 k (128 bytes a row: rows of 64 took twice as long for a byte). A row keeps
  * its 16-byte piece b at place b ^ swizzle(row), so that the 16 lanes that an LDS read serves at a time meet in different banks.
  *
- * Full tiles, 256 x 256 (two stages in LDS, one workgroup a CU): two waves a SIMD take turns at the matrix core. Bound by it: a
- * stage takes 1.5 us (2,810 TFLOP/s over 256 CUs; a library product of 8,192^3 reaches 3,040), a tile about 5 more for its first
- * operands and its results: 8,192^3 411 us (2,676 TFLOP/s); 65,536 x 4,992 x 1,664 496 (2,195); 65,536 x 1,664 x 6,656 599 (2,423); the
- * ReLU^2 form of 65,536 x 6,656 x 1,664 615; its backward, which moves 1.7 GB besides, 829. Half tiles, 128 x 128, two workgroups a
- * CU, and small ones, 64 x 128, three stages in LDS: for results that make fewer tiles. Bound by LDS reads and latency, 0.65 and 0.42
- * us a stage: 1,001 x 5,120 x 1,280 11 us; 128 x 65,536 x 1,664 26 us (4.2 TB/s of weights); 128 x 4,992 x 1,664 7.6. Rings of six
- * stages in small tiles and of four in half tiles leave room for one workgroup a CU: 256 x 4,992 x 1,664 7.7 -> 8.8 us, 1,001 x 4,992
- * 13.4 -> 19.9.
+ * Full tiles, 256 x 256 (two stages in LDS, one workgroup a CU): four waves, one a SIMD, of 128 x 128 results each (all 256 AGPRs of a
+ * lane), which take their next operands from LDS between this stage's products. Bound by the matrix core: a stage takes 1.4 us (3,100
+ * TFLOP/s over 256 CUs; a library product of 8,192^3 reaches 3,040), a tile about 5 more for its first operands and its results:
+ * 8,192^3 371 to 385 us (2,960 to 2,860 TFLOP/s); 65,536 x 4,992 x 1,664 459 to 476 (2,370 to 2,290); 65,536 x 1,664 x 6,656 533 to
+ * 548 (2,720 to 2,650); the ReLU^2 form of 65,536 x 6,656 x 1,664 612; its backward, which moves 1.7 GB besides, 843. Eight waves of
+ * 64 x 128 that took turns at the core read half as much again from LDS and took 417, 508, 611 and 642 us for the first four (and
+ * 822 for the backward, whose results two waves a SIMD make in less time than one). Half tiles, 128 x 128, two workgroups a CU, and
+ * small ones, 64 x 128, three stages in LDS: for results that make fewer tiles. Bound by LDS, 0.5 to 0.65 and 0.35 to 0.42 us a
+ * stage: 1,001 x 5,120 x 1,280 11 us; 128 x 65,536 x 1,664 26 us (4.2 TB/s of weights); 128 x 4,992 x 1,664 7.6. Rings of six stages
+ * in small tiles and of four in half tiles leave room for one workgroup a CU: 256 x 4,992 x 1,664 7.7 -> 8.8 us, 1,001 x 4,992 13.4
+ * -> 19.9.
  *
  * Rows past M and N and columns past K read zeros (offsets past the buffer resource), and are not stored.
  *
@@ -675,9 +678,10 @@ F8Gemm fg_rows(F8Gemm g, long long from, long long count) {
 /*
  * Small tiles while they all run at once; else by rounds, of a full tile a CU (8 parts of time), of two half tiles a CU (5; one alone
  * 4), or whole rounds of full tiles and half tiles for the rows left, a launch more (1). Microseconds of full and half tiles of 1,664 k:
- * 515 x 16,384 22.0, 25.0; 300 x 16,384 21.8, 13.7; 200 x 65,536 32.5, 38.9; 128 x 65,536 29.3, 25.9; 2,500 x 4,992 23.7, 27.6;
- * 1,001 x 4,992 21.7, 13.4. Of small and half: 256 x 4,992 7.7, 11.0; 128 x 16,384 8.2, 11.7; 515 x 4,992, 351 small ones, 11.6,
- * 11.3; 300 x 16,384, 640, 18.5, 13.7. All sum in the same order.
+ * 515 x 16,384 21.0, 24.5; 300 x 16,384 20.4, 14.1; 200 x 65,536 29.3, 37.4; 128 x 65,536 28.1, 25.5; 2,500 x 4,992 20.7, 25.4;
+ * 1,001 x 4,992 20.2, 14.1; alone and split, 9,995 x 5,120 x 1,280 73.7, 66.5; 1,500 x 16,384 45.0, 40.6. Of small and half: 256 x
+ * 4,992 8.0, 11.0; 128 x 16,384 8.6, 11.8; 515 x 4,992, 351 small ones, 11.6, 11.5; 300 x 16,384, 640, 18.6, 14.1. All sum in the
+ * same order.
  */
 long long fg_half_time(long long tiles, long long cus) { return tiles <= cus ? 4 : 5 * ((tiles + 2 * cus - 1) / (2 * cus)); }
 int fg_gemm(F8Gemm g, int epi, void *stream) {
