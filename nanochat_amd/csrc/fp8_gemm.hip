@@ -60,12 +60,7 @@ struct F8Gemm {
     unsigned char *q, *qs;               /* [M][N] codes and their scales at qs_stride (RELU2, RELU2_BWD: written) */
     const unsigned char *act, *acts;     /* [M][N] codes and scales at act_stride (RELU2_BWD: read) */
     long long qs_stride, act_stride;
-    bool q_stays;                        /* the codes are left in the caches */
 };
-/* Codes are what the next product reads: left in the caches (256 MB behind the L2s) where they fit with what else it takes. An MLP of
- * 9,995 x 1,280/5,120, 51 MB of codes, 170 us past the caches, 157 through them; the training of 65,536 x 1,664/6,656, 436 MB, 5,108
- * and 5,170. */
-constexpr long long FG_STAYS = 128LL << 20;
 
 template <int NU_, int WN_, int WM_, int RING_> struct FgTile {
     static constexpr int NU = NU_, WN = WN_, WM = WM_, RING = RING_, WAVES = WN * WM, TM = 16 * NU * WM, TN = F8_BLOCK * WN;
@@ -247,6 +242,12 @@ __device__ __forceinline__ void fg_mfma(f32x4 &c, const i32x8 &w, const i32x8 &a
                  : "+a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
 }
 
+/* ... and from nothing: a tile's first stage needs no cleared accumulators. */
+__device__ __forceinline__ void fg_mfma_new(f32x4 &c, const i32x8 &w, const i32x8 &a, uint32_t sw, uint32_t sa) {
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, 0, %3, %4 op_sel_hi:[0,0,0]"
+                 : "=a"(c) : "v"(w), "v"(a), "v"(sw), "v"(sa));
+}
+
 /* The full tile's DMA: instruction s = 0 .. 7 of w and of a moves rows 32 s + 8 wave + lane / 8; every fourth stage three more bring the
  * scale dwords of four blocks that the wave itself needs (its 128 rows of a, its block of w). */
 constexpr int FG_SCALES = 768;    /* bytes of a wave's scales of four blocks: 128 dwords of a, then w's in each lane's place */
@@ -256,7 +257,9 @@ struct FgDma {
     int ca, cw, first, K;         /* the lane's pieces and its row of s = 0 */
     int scale_at, more;           /* the offset of its row's scales, and of 64 rows */
     uint32_t oa, ow, to;          /* the stage being fetched */
-    __device__ __forceinline__ FgDma(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0) {
+    int flip;                     /* the buffer of even stages */
+    __device__ __forceinline__ FgDma(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *b0, int flip)
+        : flip(flip) {
         ra = f8_words(g.a + m0 * g.K, (long long)p.rows * g.K);
         rw = f8_words(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
         rsa = f8_words(g.as + m0 * g.as_stride, p.rows * g.as_stride);
@@ -276,7 +279,7 @@ struct FgDma {
         const int k = j * FG_ROWB;
         oa = k + ca < K ? first + ca + k : FG_PAST;
         ow = k + cw < K ? first + cw + k : FG_PAST;
-        to = lds + (j & 1) * FgFull::STAGE;
+        to = lds + ((j & 1) ^ flip) * FgFull::STAGE;
         if ((j & 3) == 0) {
             const uint32_t own = scales + ((j >> 2) & 1) * FG_SCALES;
             f8_dma4(own, scale_at + j, rsa);
@@ -284,8 +287,14 @@ struct FgDma {
             f8_dma4(own + 512, j, rsw);
         }
     }
-    template <int S> __device__ __forceinline__ void issue_w() const { f8_dma16<FgFull::TM * FG_ROWB + S * 4096>(to, ow, 32 * S * K, rw); }
-    template <int S> __device__ __forceinline__ void issue_a() const { f8_dma16<S * 4096>(to, oa, 32 * S * K, ra); }
+    /* in order of S */
+    template <int S> __device__ __forceinline__ void issue_w() { f8_dma16_on<FgFull::TM * FG_ROWB + S * 4096>(to, ow, 32 * K, rw); }
+    template <int S> __device__ __forceinline__ void issue_a() { f8_dma16_on<S * 4096>(to, oa, 32 * K, ra); }
+    __device__ __forceinline__ void fetch(int j) {
+        stage(j);
+        fg_unroll<8>([&](auto s) { issue_w<decltype(s)::value>(); });
+        fg_unroll<8>([&](auto s) { issue_a<decltype(s)::value>(); });
+    }
 };
 
 /* RELU2_BWD: a wave's 128 x 128 codes of a, which come as a stage behind the last, into the buffer that is free by then: 8 rows an
@@ -320,7 +329,7 @@ template <int N> __device__ __forceinline__ void fg_wait() {
  */
 struct FgWalk {
     const unsigned char *lds, *own;       /* the workgroup's LDS, this wave's scales */
-    int a_at, w_at, i;
+    int a_at, w_at, i, flip;
     i32x8 w[8], a[8];
     uint32_t sa[2][8], sw[2];             /* scale bytes of even and of odd stages */
     template <int T> __device__ __forceinline__ void read_w(const unsigned char *buf) {
@@ -343,7 +352,7 @@ struct FgWalk {
     /* What is done behind product I: of stage j, FIRST (its parity) which half of a comes first. act_next: the
      * DMA is not of stage j + 2 but of act. */
     template <int I, int FIRST> __device__ __forceinline__ void side(int j, FgDma &dma, bool act_next, const FgAct *act) {
-        const unsigned char *cur = lds + (j & 1) * FgFull::STAGE, *next = lds + (1 - (j & 1)) * FgFull::STAGE;
+        const unsigned char *cur = lds + ((j & 1) ^ flip) * FgFull::STAGE, *next = lds + ((j & 1) ^ flip ^ 1) * FgFull::STAGE;
         if constexpr (I < 8 && I % 2 == 1) read_a<4 * (1 - FIRST) + I / 2>(cur);
         if constexpr (I >= 8 && I < 24 && I % 4 == 1) read_w<4 + (I - 8) / 4>(cur);
         if constexpr (I >= 32 && I < 40 && I % 2 == 1) read_w<(I - 32) / 2>(next);
@@ -362,7 +371,7 @@ struct FgWalk {
         }
         __builtin_amdgcn_sched_barrier(0);
     }
-    template <int I, int FIRST>
+    template <int I, int FIRST, bool NEW = false>
     __device__ __forceinline__ void run(f32x4 (&acc)[8][8], int j, FgDma &dma, bool act_next, const FgAct *act) {
         if constexpr (I < 64) {
             constexpr int Q = I / 16, T = 4 * (Q / 2) + I % 16 / 4, U = 4 * ((Q == 0 || Q == 3) ? FIRST : 1 - FIRST) + I % 4;
@@ -376,56 +385,49 @@ struct FgWalk {
                 else fg_wait<8>();
                 fg_barrier();
             }
-            fg_mfma(acc[T][U], w[T], a[U], sw[FIRST], sa[FIRST][U]);
+            if constexpr (NEW) fg_mfma_new(acc[T][U], w[T], a[U], sw[FIRST], sa[FIRST][U]);
+            else fg_mfma(acc[T][U], w[T], a[U], sw[FIRST], sa[FIRST][U]);
             side<I, FIRST>(j, dma, act_next, act);
-            run<I + 1, FIRST>(acc, j, dma, act_next, act);
+            run<I + 1, FIRST, NEW>(acc, j, dma, act_next, act);
         }
     }
 };
 
-template <bool ACT>
-__device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *lds,
-                                             f32x4 (&acc)[8][8]) {
+/* Stage 0 is on its way, and NEWER memory instructions behind it. */
+template <bool ACT, int NEWER>
+__device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, long long m0, int n0, unsigned char *lds, FgDma &dma,
+                                             bool newer, f32x4 (&acc)[8][8]) {
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
-    FgDma dma(g, p, m0, n0, lds);
-    const FgAct act(ACT ? g : F8Gemm{}, p, ACT ? m0 : 0, ACT ? n0 : 0, lds + (stages & 1) * FgFull::STAGE);
-#pragma unroll
-    for (int t = 0; t < 8; t++)
-#pragma unroll
-        for (int u = 0; u < 8; u++) asm volatile("" : "=a"(acc[t][u]) : "0"(acc[t][u]));
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        dma.stage(j);
-        if (ACT && j == stages) {
-            fg_unroll<16>([&](auto s) { act.template issue<decltype(s)::value>(); });
-        } else {
-            fg_unroll<8>([&](auto s) { dma.template issue_w<decltype(s)::value>(); });
-            fg_unroll<8>([&](auto s) { dma.template issue_a<decltype(s)::value>(); });
-        }
-    }
+    const FgAct act(ACT ? g : F8Gemm{}, p, ACT ? m0 : 0, ACT ? n0 : 0, lds + ((stages & 1) ^ dma.flip) * FgFull::STAGE);
+    if (ACT && stages == 1) fg_unroll<16>([&](auto s) { act.template issue<decltype(s)::value>(); });
+    else dma.fetch(1);
     FgWalk k;
     k.lds = lds;
     k.own = lds + 2 * FgFull::STAGE + p.wave * 2 * FG_SCALES;
     k.i = p.i;
+    k.flip = dma.flip;
     k.a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
     const int w_row = F8_BLOCK * p.wn + fg_column(0, p.i >> 2) + (p.i & 3);
     k.w_at = (FgFull::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
-    fg_wait<16>();   /* stage 0 */
+    if (newer) fg_wait<16 + NEWER>();
+    else fg_wait<16>();
     fg_barrier();
+    const unsigned char *b0 = lds + dma.flip * FgFull::STAGE;
     fg_unroll<4>([&](auto t) {
-        k.template read_w<decltype(t)::value>(lds);
-        k.template read_a<decltype(t)::value>(lds);
+        k.template read_w<decltype(t)::value>(b0);
+        k.template read_a<decltype(t)::value>(b0);
     });
     fg_unroll<9>([&](auto u) { k.template read_scale<decltype(u)::value, 0>(0); });
     k.template pin<0>();
-    for (int j = 0; j < stages; j += 2) {
-        k.template run<0, 0>(acc, j, dma, ACT && j + 2 == stages, &act);
+    k.template run<0, 0, true>(acc, 0, dma, ACT && stages == 2, &act);
+    for (int j = 1; j < stages; j += 2) {
+        k.template run<0, 1>(acc, j, dma, ACT && j + 2 == stages, &act);
         if (j + 1 >= stages) break;
-        k.template run<0, 1>(acc, j + 1, dma, ACT && j + 3 == stages, &act);
+        k.template run<0, 0>(acc, j + 1, dma, ACT && j + 3 == stages, &act);
     }
     __builtin_amdgcn_s_waitcnt(0);
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");   /* 32 wait states; no read moves above */
-    fg_barrier();   /* the epilogue writes where other waves may still read and DMA may still land */
+    fg_barrier();   /* what follows writes where other waves may still read and DMA may still land */
 #pragma unroll
     for (int t = 0; t < 8; t++)
 #pragma unroll
@@ -441,37 +443,21 @@ __device__ __forceinline__ void fg_wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+/* A wave's results. turns: the workgroup's part of LDS for them; acts, act_bytes: ACT_STAGE's codes of a, in LDS, and the scale bytes
+ * of the wave's rows `lane` and 64 on. */
 template <class P, int EPI>
-__device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, unsigned char *b0) {
-    const FgPlace p = fg_place<P>(g, m0, n0);
-    f32x4 acc[8][P::NU];
-#pragma unroll
-    for (int t = 0; t < 8; t++)
-#pragma unroll
-        for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+__device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, long long m0, int n0, f32x4 (&acc)[8][P::NU],
+                                           unsigned char *turns, const unsigned char *acts, const uint32_t (&act_bytes)[2]) {
     constexpr bool ACT_STAGE = P::FULL && EPI == FG_RELU2_BWD;
-    uint32_t act_bytes[2] = {127u, 127u};   /* ACT_STAGE: the scale bytes of the wave's rows `lane` and 64 on */
-    if constexpr (ACT_STAGE) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int row = 128 * p.wm + 64 * h + p.lane;
-            if (row < p.rows && p.some) act_bytes[h] = g.acts[(m0 + row) * g.act_stride + p.nb];
-        }
-    }
-    if constexpr (P::FULL) fg_walk_full<ACT_STAGE>(g, p, m0, n0, b0, acc);
-    else fg_walk_ring<P, P::NU == 1 && EPI == FG_RELU2>(g, p, m0, n0, b0, acc);
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));   /* made again, not kept through the walk */
     const int grp = (tid & (WAVE - 1)) >> 4;
     const int rows = p.rows, cols = p.cols, nb = p.nb, wn = p.wn;
-    const bool some = p.some;
-
-    if (!some) return;
+    if (!p.some) return;
     const int lane = tid & (WAVE - 1), rows_left = rows - 16 * P::NU * p.wm, col = F8_BLOCK * wn;   /* this wave's */
     const long long first = m0 + 16 * P::NU * p.wm;
-    const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
-    unsigned char *mine = b0 + (threadIdx.x >> 6) * FG_TURN + (ACT_STAGE ? (stages - 1 & 1) * P::STAGE : 0);
-    const unsigned char *act_at = b0 + (stages & 1) * P::STAGE + (threadIdx.x >> 6) * 16384;   /* ACT_STAGE */
+    unsigned char *mine = turns + (threadIdx.x >> 6) * FG_TURN;
+    const unsigned char *act_at = acts + (threadIdx.x >> 6) * 16384;
     const int r16 = lane & 15;
     /* RELU2_BWD: a's scales, and in the smaller tiles its codes, a piece of 16 columns a lane of rows 8 k + lane / 8 of each 16; all on
      * their way at once */
@@ -600,11 +586,10 @@ __device__ __forceinline__ void fg_run(const F8Gemm &g, long long m0, int n0, un
             for (int k = 0; k < 2; k++) {
                 const int r = 8 * k + (lane >> 3), c = lane & 7;
                 const u32x4 d = *(const u32x4 *)(codes + fg_code_place(r, c));
-                if (16 * u + r < rows_left && col + 16 * c < cols) {
-                    u32x4 *const to = (u32x4 *)(g.q + (first + 16 * u + r) * g.N + n0 + col + 16 * c);
-                    if (g.q_stays) *to = d;
-                    else __builtin_nontemporal_store(d, to);
-                }
+                /* through the caches: the next product reads them (an MLP of 9,995 x 1,280/5,120 170 us past them, 157; the training of
+                 * 65,536 x 1,664/6,656, whose 436 MB do not fit, 5,108 and 5,170) */
+                if (16 * u + r < rows_left && col + 16 * c < cols)
+                    *(u32x4 *)(g.q + (first + 16 * u + r) * g.N + n0 + col + 16 * c) = d;
             }
         }
     };
@@ -626,11 +611,68 @@ __device__ __forceinline__ int2 fg_tile(int l, int count, int nx) {
     return int2{in / tall, y0 + in % tall};
 }
 
-template <class P, int EPI>
-__global__ void __launch_bounds__(P::WAVES *WAVE, P::FULL ? 1 : 2) fp8_gemm_kernel(F8Gemm g) {
-    __shared__ __align__(16) unsigned char lds[P::RING * P::STAGE + P::WAVES * 2 * (P::FULL ? FG_SCALES : FG_OWN)];
+template <class P, int EPI> __device__ __forceinline__ void fg_run(const F8Gemm &g, unsigned char *lds) {
     const int2 t = fg_tile(blockIdx.x, gridDim.x, (g.N + P::TN - 1) / P::TN);
-    fg_run<P, EPI>(g, (long long)t.y * P::TM, t.x * P::TN, lds);
+    const long long m0 = (long long)t.y * P::TM;
+    const FgPlace p = fg_place<P>(g, m0, t.x * P::TN);
+    f32x4 acc[8][P::NU];
+#pragma unroll
+    for (int t = 0; t < 8; t++)
+#pragma unroll
+        for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    fg_walk_ring<P, P::NU == 1 && EPI == FG_RELU2>(g, p, m0, t.x * P::TN, lds, acc);
+    const uint32_t none[2] = {0u, 0u};
+    fg_results<P, EPI>(g, p, m0, t.x * P::TN, acc, lds, lds, none);
+}
+
+/* Full tiles: a workgroup a CU takes every gridDim.x-th of them, and the first stage of the next is fetched while the last one's results
+ * are written (into the buffer that they do not pass through). RELU2_BWD has a's codes in that buffer: a workgroup a tile. */
+template <int EPI> __device__ __forceinline__ void fg_run_full(const F8Gemm &g, int tiles, unsigned char *lds) {
+    constexpr bool ACT_STAGE = EPI == FG_RELU2_BWD;
+    constexpr int STORES = EPI == FG_STORE ? 32 : 24;   /* of a whole tile, a wave's instructions: 4 a 16 rows, or 2 and a scale's */
+    typedef FgFull P;
+    const int nx = (g.N + P::TN - 1) / P::TN, stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
+    int2 t = fg_tile(blockIdx.x, tiles, nx);
+    FgPlace p = fg_place<P>(g, (long long)t.y * P::TM, t.x * P::TN);
+    FgDma dma(g, p, (long long)t.y * P::TM, t.x * P::TN, lds, 0);
+    dma.fetch(0);
+    bool stores = false;
+    for (int l = blockIdx.x;;) {
+        const long long m0 = (long long)t.y * P::TM;
+        const int n0 = t.x * P::TN;
+        uint32_t act_bytes[2] = {127u, 127u};
+        if constexpr (ACT_STAGE) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int row = 128 * p.wm + 64 * h + p.lane;
+                if (row < p.rows && p.some) act_bytes[h] = g.acts[(m0 + row) * g.act_stride + p.nb];
+            }
+        }
+        f32x4 acc[8][8];
+        fg_walk_full<ACT_STAGE, STORES>(g, p, m0, n0, lds, dma, stores, acc);
+        const int flip = (stages & 1) ^ dma.flip;   /* the buffer of a stage behind the last */
+        const FgPlace done = p;
+        l += gridDim.x;
+        const bool more = !ACT_STAGE && l < tiles;
+        if (more) {
+            t = fg_tile(l, tiles, nx);
+            p = fg_place<P>(g, (long long)t.y * P::TM, t.x * P::TN);
+            dma = FgDma(g, p, (long long)t.y * P::TM, t.x * P::TN, lds, flip);
+            dma.fetch(0);
+        }
+        fg_results<P, EPI>(g, done, m0, n0, acc, lds + (flip ^ 1) * P::STAGE, lds + flip * P::STAGE, act_bytes);
+        if (!more) return;
+        stores = done.rows == P::TM && done.cols == P::TN;   /* all were issued */
+        __builtin_amdgcn_s_waitcnt(0xC07F);   /* the LDS reads */
+        fg_barrier();
+    }
+}
+
+template <class P, int EPI>
+__global__ void __launch_bounds__(P::WAVES *WAVE, P::FULL ? 1 : 2) fp8_gemm_kernel(F8Gemm g, int tiles) {
+    __shared__ __align__(16) unsigned char lds[P::RING * P::STAGE + P::WAVES * 2 * (P::FULL ? FG_SCALES : FG_OWN)];
+    if constexpr (P::FULL) fg_run_full<EPI>(g, tiles, lds);
+    else fg_run<P, EPI>(g, lds);
 }
 
 template <class P>
@@ -639,7 +681,8 @@ int fg_launch(const F8Gemm &g, int epi, hipStream_t stream) {
     if (tiles >= (1LL << 31)) return NC_ERR_SHAPE;
     const auto kernel = epi == FG_STORE ? fp8_gemm_kernel<P, FG_STORE>
                         : epi == FG_RELU2 ? fp8_gemm_kernel<P, FG_RELU2> : fp8_gemm_kernel<P, FG_RELU2_BWD>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(P::WAVES * WAVE), 0, stream, g);
+    const long long cus = device_cus(), grid = P::FULL && epi != FG_RELU2_BWD && tiles > cus ? cus : tiles;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(P::WAVES * WAVE), 0, stream, g, (int)tiles);
     return (int)hipGetLastError();
 }
 
@@ -684,13 +727,12 @@ F8Gemm fg_rows(F8Gemm g, long long from, long long count) {
  * same order.
  */
 long long fg_half_time(long long tiles, long long cus) { return tiles <= cus ? 4 : 5 * ((tiles + 2 * cus - 1) / (2 * cus)); }
-int fg_gemm(F8Gemm g, int epi, void *stream) {
+int fg_gemm(const F8Gemm &g, int epi, void *stream) {
     const int e = fg_check(g, epi);
     if (e != NC_OK || g.M == 0) return e;
     const hipStream_t s = (hipStream_t)stream;
     const long long cus = device_cus(), nx = (g.N + 255) / 256, full = (g.M + 255) / 256 * nx, half_nx = (g.N + 127) / 128;
     const long long small = (g.M + 63) / 64 * half_nx;
-    g.q_stays = g.M * g.N <= FG_STAYS;
     if (epi == FG_STORE && fp8_some_takes(g.M, g.N, g.K, cus))
         return fp8_some(g.a, g.as, g.as_stride, g.w, g.ws, g.ws_stride, (int)g.M, g.N, g.K, g.out, s);
     if (small <= cus) return fg_launch<FgSmall>(g, epi, s);
@@ -715,7 +757,7 @@ extern "C" int nc_fp8_matmul(const void *a, const void *a_scale, long long a_sca
                              int w_scale_stride, long long rows, int n, int k, void *out, void *stream) {
     const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
                       (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, (uint16_t *)out,
-                      nullptr, nullptr, nullptr, nullptr, 0, 0, false};
+                      nullptr, nullptr, nullptr, nullptr, 0, 0};
     return fg_gemm(g, FG_STORE, stream);
 }
 
@@ -724,7 +766,7 @@ extern "C" int nc_fp8_matmul_relu2(const void *a, const void *a_scale, long long
                                    void *scale, long long scale_stride, void *stream) {
     const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
                       (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, nullptr,
-                      (unsigned char *)codes, (unsigned char *)scale, nullptr, nullptr, scale_stride, 0, false};
+                      (unsigned char *)codes, (unsigned char *)scale, nullptr, nullptr, scale_stride, 0};
     return fg_gemm(g, FG_RELU2, stream);
 }
 
@@ -735,6 +777,6 @@ extern "C" int nc_fp8_matmul_relu2_bwd(const void *a, const void *a_scale, long 
     const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
                       (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, (uint16_t *)out,
                       (unsigned char *)codes, (unsigned char *)scale, (const unsigned char *)act,
-                      (const unsigned char *)act_scale, scale_stride, act_scale_stride, false};
+                      (const unsigned char *)act_scale, scale_stride, act_scale_stride};
     return fg_gemm(g, FG_RELU2_BWD, stream);
 }

@@ -97,6 +97,11 @@ template <int STEP> __device__ __forceinline__ void f8_dma16(uint32_t base, uint
     asm volatile("s_add_u32 m0, %1, %2\n\tv_add_u32 %0, %4, %3\n\tbuffer_load_dwordx4 %0, %5, 0 offen lds"
                  : "=&v"(at) : "s"(base), "i"(STEP), "v"(off), "s"(more), "s"(r) : "memory", "scc");
 }
+/* f8_dma16 to base + STEP, from off, which then moves on. */
+template <int STEP> __device__ __forceinline__ void f8_dma16_on(uint32_t base, uint32_t &off, uint32_t on, const f8_u32x4 &r) {
+    asm volatile("s_add_u32 m0, %1, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %3, 0 offen lds\n\tv_add_u32 %0, %4, %0"
+                 : "+v"(off) : "s"(base), "i"(STEP), "s"(r), "s"(on) : "memory", "scc");
+}
 __device__ __forceinline__ uint32_t f8_lds(const void *p) {
     return (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)p);
 }

@@ -16,7 +16,7 @@ import pytest
 from nanochat_amd import native
 from tests.test_prefill_gemm_isa import blocks, loop_lines, regs, wait_states_before_agpr_reads, writer_kind
 
-ASM = {"gemm": ("fp8_gemm.hip", r"_ZN2nc12_GLOBAL__N_115fp8_gemm_kernelINS0_6FgTileILi8ELi2ELi2ELi2EEELi([012])EEEvNS0_6F8GemmE"),
+ASM = {"gemm": ("fp8_gemm.hip", r"_ZN2nc12_GLOBAL__N_115fp8_gemm_kernelINS0_6FgTileILi8ELi2ELi2ELi2EEELi([012])EEEvNS0_6F8GemmEi"),
        "grad": ("fp8_grad.hip", r"_ZN2nc12_GLOBAL__N_115fp8_grad_kernelILi([0123])EEEvNS0_7F8GradsE")}
 KERNELS = [("gemm", e) for e in range(3)] + [("grad", m) for m in range(4)]
 
@@ -80,6 +80,14 @@ def test_every_kernel_is_built(kernels):
         assert counts and all(int(c) == 0 for c in counts)
 
 
+@pytest.mark.parametrize("epi,wide,narrow", [(0, 32, 0), (1, 16, 8)])
+def test_a_tiles_stores_are_as_many_as_its_successor_counts(kernels, epi, wide, narrow):
+    """The wait for a tile's first stage lets that many newer stores of the last tile's be on their way."""
+    count = lambda mn: sum(line.strip().startswith(mn) for line in kernels[0][("gemm", epi)])   # noqa: E731
+    assert count("global_store_dwordx4") == wide and count("global_store_byte") == narrow
+    assert count("buffer_store") == count("flat_store") == 0
+
+
 @pytest.mark.parametrize("which", KERNELS)
 def test_operands_are_not_written_right_before(kernels, which):
     # 2 are needed; both kernels read their operands a phase or a stage ahead
@@ -89,9 +97,11 @@ def test_operands_are_not_written_right_before(kernels, which):
 
 @pytest.mark.parametrize("which", KERNELS)
 def test_accumulators_stay_in_place(kernels, which):
-    walk = [line for line in loop_lines(kernels[0][which])]
-    assert any("v_mfma" in line for line in walk)
-    assert not [line for line in walk if "v_accvgpr" in line]
+    walk = [body for _, body, _ in blocks(kernels[0][which]) if any(mn.startswith("v_mfma") for mn, _ in body)]
+    assert walk and any("v_mfma" in line for line in loop_lines(kernels[0][which]))
+    for body in walk:   # what a tile's results read stands behind the last product, in a block of its own or at the end of one
+        last = max(i for i, (mn, _) in enumerate(body) if mn.startswith("v_mfma"))
+        assert not [i for i, (mn, _) in enumerate(body) if mn.startswith("v_accvgpr") and i < last and mn != "v_accvgpr_write_b32"]
 
 
 @pytest.mark.parametrize("which", KERNELS)
