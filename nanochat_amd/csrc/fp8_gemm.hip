@@ -14,9 +14,9 @@
  *
  * Full tiles, 256 x 256 (two stages in LDS, one workgroup a CU): four waves, one a SIMD, of 128 x 128 results each (all 256 AGPRs of a
  * lane), which take their next operands from LDS between this stage's products. Bound by the matrix core: a stage takes 1.4 us (3,100
- * TFLOP/s over 256 CUs; a library product of 8,192^3 reaches 3,040), a tile about 5 more for its first operands and its results:
- * 8,192^3 371 to 385 us (2,960 to 2,860 TFLOP/s); 65,536 x 4,992 x 1,664 459 to 476 (2,370 to 2,290); 65,536 x 1,664 x 6,656 533 to
- * 548 (2,720 to 2,650); the ReLU^2 form of 65,536 x 6,656 x 1,664 612; its backward, which moves 1.7 GB besides, 843. Eight waves of
+ * TFLOP/s over 256 CUs; a library product of 8,192^3 reaches 3,040), a tile about 4 more for its results, beside which the next
+ * tile's first stage is fetched: 8,192^3 375 to 380 us (2,930 to 2,890 TFLOP/s); 65,536 x 4,992 x 1,664 454 to 465 (2,400 to 2,340);
+ * 65,536 x 1,664 x 6,656 531 (2,734); the ReLU^2 form of 65,536 x 6,656 x 1,664 594; its backward, which moves 1.7 GB besides, 842. Eight waves of
  * 64 x 128 that took turns at the core read half as much again from LDS and took 417, 508, 611 and 642 us for the first four (and
  * 822 for the backward, whose results two waves a SIMD make in less time than one). Half tiles, 128 x 128, two workgroups a CU, and
  * small ones, 64 x 128, three stages in LDS: for results that make fewer tiles. Bound by LDS, 0.5 to 0.65 and 0.35 to 0.42 us a

@@ -50,45 +50,45 @@ def _new_scale(like: Tensor, rows: int, cols: int) -> Tensor:
     return torch.empty(rows, -(-blocks // 4) * 4, dtype=SCALE, device=like.device)[:, :blocks]
 
 
-def _check_codes(codes: Tensor, name: str, device: torch.device) -> None:
+def _check_codes(codes: Tensor, name: str, device: torch.device, part: str = "") -> None:
     if codes.dtype != CODES:
-        raise TypeError(f"{name} must be {CODES}, got {codes.dtype}")
-    if not codes.is_cuda or codes.device != device:
-        raise ValueError(f"{name} must be a device tensor on {device}, got {codes.device}")
+        raise TypeError(f"{name}{part} must be {CODES}, got {codes.dtype}")
+    if codes.device != device or not codes.is_cuda:
+        raise ValueError(f"{name}{part} must be a device tensor on {device}, got {codes.device}")
     if codes.dim() != 2 or not codes.is_contiguous() or codes.data_ptr() % 16:
-        raise ValueError(f"{name} must be a contiguous, 16-byte aligned matrix")
+        raise ValueError(f"{name}{part} must be a contiguous, 16-byte aligned matrix")
     if codes.size(1) % 16:
-        raise ValueError(f"{name} must have a multiple of 16 columns, got {codes.size(1)}")
+        raise ValueError(f"{name}{part} must have a multiple of 16 columns, got {codes.size(1)}")
 
 
-def _check_scale(scale: Tensor, name: str, rows: int, cols: int, device: torch.device) -> int:
+def _check_scale(scale: Tensor, name: str, rows: int, cols: int, device: torch.device, part: str = "") -> int:
     """A scale tensor's row stride in bytes."""
     if scale.dtype != SCALE:
-        raise TypeError(f"{name} must be {SCALE}, got {scale.dtype}")
-    blocks = _blocks(cols)
+        raise TypeError(f"{name}{part} must be {SCALE}, got {scale.dtype}")
+    blocks = -(-cols // BLOCK)
     if scale.dim() != 2 or scale.shape != (rows, blocks) or scale.device != device:
-        raise ValueError(f"{name} must be [{rows}, {blocks}] on {device}, got {tuple(scale.shape)} on {scale.device}")
+        raise ValueError(f"{name}{part} must be [{rows}, {blocks}] on {device}, got {tuple(scale.shape)} on {scale.device}")
     pitch, step = scale.stride()
     if ((blocks > 1 and step != 1) or pitch % 4 or pitch < blocks or pitch > cols or scale.data_ptr() % 4
             or scale.storage_offset() + (rows - 1) * pitch + -(-blocks // 4) * 4 > scale.untyped_storage().nbytes()):
-        raise ValueError(f"{name} must have 4-byte aligned rows of adjacent scales, padded to a multiple of 4 bytes")
+        raise ValueError(f"{name}{part} must have 4-byte aligned rows of adjacent scales, padded to a multiple of 4 bytes")
     return pitch
 
 
 def _check_weight(w: Fp8Weight, name: str, device: torch.device, transposed: bool = False) -> tuple[int, int]:
     """(pitch of the scales, of the transpose's or 0) of a weight in the 8-bit form."""
     codes, scale, codes_t, scale_t = w
-    _check_codes(codes, f"{name}.codes", device)
+    _check_codes(codes, name, device, ".codes")
     n, k = codes.shape
-    pitch = _check_scale(scale, f"{name}.scale", _blocks(n), k, device)
+    pitch = _check_scale(scale, name, -(-n // BLOCK), k, device, ".scale")
     if not transposed:
         return pitch, 0
     if codes_t is None or scale_t is None:
         raise ValueError(f"{name} needs its transpose for training: quantize_weight(w, transpose=True)")
-    _check_codes(codes_t, f"{name}.codes_t", device)
+    _check_codes(codes_t, name, device, ".codes_t")
     if codes_t.shape != (k, n):
         raise ValueError(f"{name}.codes_t must be {(k, n)}, got {tuple(codes_t.shape)}")
-    return pitch, _check_scale(scale_t, f"{name}.scale_t", _blocks(k), n, device)
+    return pitch, _check_scale(scale_t, name, -(-k // BLOCK), n, device, ".scale_t")
 
 
 def _as_rows(x: Tensor, name: str, dtypes: tuple, of: int = 16) -> Tensor:
@@ -181,6 +181,9 @@ def _serving_input(x: Tensor, weight: Fp8Weight, name: str) -> Tensor:
     return rows
 
 
+FEW = 16   # rows that one launch of the few-row kernel takes
+
+
 def _workspace(x: Tensor, need: int) -> Tensor:
     return torch.empty(max(need, 16), dtype=torch.uint8, device=x.device)   # an unsupported size: refused by the call
 
@@ -193,12 +196,14 @@ def fp8_linear(x: Tensor, weight: Fp8Weight) -> Tensor:
     (m, k), n = rows.shape, weight.codes.size(0)
     _outputs(n, "weight")
     with device_guard(x):
-        lib = hip_library()
-        out, at, stride = torch.empty(m, n, dtype=BF16, device=x.device), rows.data_ptr(), rows.stride(0)
-        need = lib.nc_fp8_linear_workspace_bytes(at, 0, stride, m, n, k)
-        ws = _workspace(x, need) if need else None
-        check(lib.nc_fp8_linear(at, 0, stride, weight.codes.data_ptr(), weight.scale.data_ptr(), pitch, m, n, k, out.data_ptr(),
-                                ws.data_ptr() if need else None, need, stream()))
+        call, at, stride = hip_library().nc_fp8_linear, rows.data_ptr(), rows.stride(0)
+        out = torch.empty(m, n, dtype=BF16, device=x.device)
+        args = (at, 0, stride, weight.codes.data_ptr(), weight.scale.data_ptr(), pitch, m, n, k, out.data_ptr())
+        # a few rows need no workspace as a rule: asked for only where the call refuses to go without
+        if m > FEW or call(*args, None, 0, stream()) != 0:
+            need = hip_library().nc_fp8_linear_workspace_bytes(at, 0, stride, m, n, k)
+            ws = _workspace(x, need)
+            check(call(*args, ws.data_ptr(), need, stream()))
     return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 
