@@ -372,7 +372,8 @@ int nc_fp8_quantize_weight(const void *w, int is_f32, long long row_stride, int 
  * nc_fp8_matmul_relu2_bwd  out = bf16(sum * 2 sqrt(act)), act [rows][n] in the 8-bit form (as nc_fp8_matmul_relu2 leaves it), and
  *                       the 8-bit form of out: the gradient before a ReLU^2 whose result act is, from the one behind it
  * Sums are fp32, but for the eight products of adjacent k that the matrix cores add at a time: of those, bits below 2^-13 of
- * the largest are dropped (at most 2^-10 of the sum of magnitudes, and 1e-5 to 3e-5 of a result as a rule). The outputs may not overlap the inputs. */
+ * the largest are dropped (at most 2^-10 of the sum of magnitudes, and 1e-5 to 3e-5 of a result as a rule). The outputs may not
+ * overlap the inputs. */
 int nc_fp8_matmul(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
                   int w_scale_stride, long long rows, int n, int k, void *out, void *stream);
 int nc_fp8_matmul_relu2(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
@@ -386,10 +387,10 @@ int nc_fp8_matmul_relu2_bwd(const void *a, const void *a_scale, long long a_scal
 /* A layer, out = x8 w^T, and a ReLU^2 MLP, out = a8 proj^T with a = relu(x8 fc^T)^2, for serving: x8, a8 the 8-bit forms of x's
  * rows (bf16, or fp32 for a layer with is_f32; [rows][k] at row_stride elements, any alignment of its type) and of the squares of the
  * fp32 sums, w [n][k], fc [hidden][c] and proj [n][hidden] held in 8 bits, out bf16 [rows][n], all widths multiples of 16 up to 2^20.
- * A few rows are bound by reading the weights once; up to 16 that can be read 16 bytes at a time, on few enough outputs, are one
- * launch a product. workspace: nc_fp8_*_workspace_bytes (-1 for unsupported sizes; of a layer, for the x and row_stride of the call,
- * and 0 where none is read: it may then be NULL), 16-byte aligned, need not be cleared. A call's workspace is its own until it has
- * run. */
+ * A few rows are bound by reading the weights once; up to 64 that can be read 16 bytes at a time, where they are short and the
+ * outputs few enough, are one launch a product. workspace: nc_fp8_*_workspace_bytes (-1 for unsupported sizes; of a layer, for the x
+ * and row_stride of the call, and 0 where none is read: it may then be NULL), 16-byte aligned, need not be cleared. A call's workspace
+ * is its own until it has run. */
 long long nc_fp8_linear_workspace_bytes(const void *x, int is_f32, long long row_stride, long long rows, int n, int k);
 int nc_fp8_linear(const void *x, int is_f32, long long row_stride, const void *w, const void *w_scale, int w_scale_stride,
                   long long rows, int n, int k, void *out, void *workspace, long long workspace_bytes, void *stream);

@@ -3,9 +3,9 @@
  * 8-bit form of x's rows: a decoding step, draft tokens. Then a layer and an MLP for serving as one call each. Bound by reading w once,
  * and below about 8 MB of it by latency: a launch, a row's way through k, the sums.
  *
- * Up to 16 rows, x as it is (fp8_few_kernel): a workgroup holds 16 rows of w and x's 16, its eight waves take every eighth block of 128
+ * Up to 64 rows, x as it is (fp8_few_kernel): a workgroup holds 16 rows of w and all of x's, its eight waves take every eighth block of 128
  * k, both operands from memory straight into registers: lane (g = lane / 16, i = lane % 16) takes bytes 16 g .. + 15 and 64 + 16 g ..
- * + 15 of row i's block, so that a load instruction reads 64 adjacent bytes a row. Which k stands where in a product does not matter
+ * + 15 of row i's block (w's, and each 16 rows' of x), so that a load instruction reads 64 adjacent bytes a row. Which k stands where in a product does not matter
  * as long as both operands agree. x comes in bf16 or fp32: a row's block lies in four lanes, which find its largest magnitude together
  * and make the codes that nc_fp8_quantize_rows makes. One row: 4,992 x 1,664 5.0 us, 16,384 x 1,664 8.7 us (3.1 TB/s of weights).
  *
@@ -127,28 +127,33 @@ template <bool RELU2> __device__ __forceinline__ void sk_product(f32x4 &acc, con
                                                                (int)x.byte);
     }
 }
-template <int XT, bool RELU2>
-__global__ void __launch_bounds__(SK_WAVES *WAVE, 4) fp8_few_kernel(Skinny p) {
-    __shared__ __align__(16) f32x4 part[SK_WAVES][WAVE];
+/* 16 MT rows of x. */
+template <int XT, int MT, bool RELU2>
+__global__ void __launch_bounds__(SK_WAVES *WAVE, MT == 1 ? 4 : 2) fp8_few_kernel(Skinny p) {
+    __shared__ __align__(16) f32x4 part[SK_WAVES][MT][WAVE];
     const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, i16 = lane & 15;
     const int n0 = blockIdx.x * 16;
     const Rsrc rw = f8_rsrc(p.w + (long long)n0 * p.K, 16LL * p.K);
     const Rsrc rx = f8_rsrc(p.x, p.M * p.row_bytes);
     const unsigned char *ws = p.ws + (long long)(n0 / F8_BLOCK) * p.ws_stride;   /* 16 rows lie in one block */
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int AHEAD = 3;   /* blocks of w on their way beside the present one; one of x */
+    f32x4 acc[MT];
+#pragma unroll
+    for (int u = 0; u < MT; u++) acc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int AHEAD = 3;   /* blocks of w on their way beside the present one; one of x, but for 64 rows */
     Raw<SK_CODES> w[AHEAD + 1];
-    Raw<XT> x, next;
+    Raw<XT> x[MT], next[MT];
     const auto fetch = [&](int slot, int kb) {
         if (kb >= p.blocks) return;
         w[slot].load(rw, (unsigned)(i16 * p.K), kb, g, p.K);
         w[slot].byte = ws[kb];
     };
-    const auto fetch_x = [&](int kb) {
-        if (kb < p.blocks) next.load(rx, (unsigned)(i16 * p.row_bytes), kb, g, p.K);
+    const auto fetch_x = [&](Raw<XT> (&to)[MT], int kb) {
+        if (kb >= p.blocks) return;
+#pragma unroll
+        for (int u = 0; u < MT; u++) to[u].load(rx, (unsigned)((16 * u + i16) * p.row_bytes), kb, g, p.K);
     };
-    fetch_x(wave);
+    if (MT < 4) fetch_x(next, wave);
 #pragma unroll
     for (int a = 0; a < AHEAD; a++) fetch(a, wave + SK_WAVES * a);
     for (int kb0 = wave; kb0 < p.blocks; kb0 += SK_WAVES * (AHEAD + 1)) {
@@ -156,23 +161,32 @@ __global__ void __launch_bounds__(SK_WAVES *WAVE, 4) fp8_few_kernel(Skinny p) {
         for (int a = 0; a <= AHEAD; a++) {
             const int kb = kb0 + SK_WAVES * a;
             if (kb >= p.blocks) break;
-            x = next;
-            fetch_x(kb + SK_WAVES);
+            if constexpr (MT < 4) {
+#pragma unroll
+                for (int u = 0; u < MT; u++) x[u] = next[u];
+                fetch_x(next, kb + SK_WAVES);
+            } else {
+                fetch_x(x, kb);
+            }
             fetch((a + AHEAD) % (AHEAD + 1), kb + SK_WAVES * AHEAD);
-            sk_product<RELU2>(acc, w[a].codes(), x.codes());
+            const Codes32 cw = w[a].codes();
+#pragma unroll
+            for (int u = 0; u < MT; u++) sk_product<RELU2>(acc[u], cw, x[u].codes());
         }
     }
-    part[wave][lane] = acc;
+#pragma unroll
+    for (int u = 0; u < MT; u++) part[wave][u][lane] = acc[u];
     __syncthreads();
-    if (wave > 0 || i16 >= p.M) return;
-    f32x4 v = part[0][lane];   /* columns 4 g .. 4 g + 3 of row i16 */
+    const int row = 16 * wave + i16;
+    if (wave >= MT || row >= p.M) return;
+    f32x4 v = part[0][wave][lane];   /* columns 4 g .. 4 g + 3 of the row */
 #pragma unroll
     for (int s = 1; s < SK_WAVES; s++) {
-        const f32x4 o = part[s][lane];
+        const f32x4 o = part[s][wave][lane];
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = v[e] + o[e];
     }
-    const long long at = (long long)i16 * p.N + n0 + 4 * g;
+    const long long at = (long long)row * p.N + n0 + 4 * g;
     if constexpr (RELU2) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -308,21 +322,28 @@ template <int RW, int S> int some_go(const Skinny &p, hipStream_t stream) {
     return (int)hipGetLastError();
 }
 
-/* x bf16 or fp32 taken as it is: rows must be readable 16 bytes at a time. Every workgroup reads x, which tells with many of them and
- * many rows; else it is two launches to put x in 8 bits first. Microseconds for 1, 4, 8 and 16 rows, against the two launches:
+/* x bf16 or fp32 taken as it is: rows must be readable 16 bytes at a time. Every workgroup reads x and puts it in 8 bits, which tells
+ * with many of them, many rows and long ones; else it is two launches to do that first. Microseconds for 1, 4, 8 and 16 rows, against
+ * the two launches:
  *    1,280 x 1,280   3.2   3.3   3.5   3.8 (6.8 to 7.4)     16,384 x 1,664    8.8   9.4  10.5  11.8 (10.0 to 10.4)
  *    4,992 x 1,664   5.0   5.4   5.7   6.7 (8.2 to 9.1)     65,536 x 1,664   25.4  25.9  27.7  31.4 (24.8 to 25.7)
- * and from an MLP's squares in fp32, all of it, 6,656 wide: 14.0  16.4  19.0 (18.0 and more). */
-bool few_takes(const void *x, bool f32, long long row_stride, long long rows, int n) {
+ * and from an MLP's squares in fp32, all of it, 6,656 wide: 14.0  16.4  19.0 (18.0 and more). For 17, 32, 37 and 64 rows:
+ *    1,280 x 1,280   4.5   5.5   6.2   7.5 (7.4 to 7.8)      1,664 x 1,664    5.3   6.6   7.8   9.4 (7.5 to 7.9)
+ *    4,992 x 1,664   9.2  11.7  14.6  17.7 (9.0 to 10.2)     1,280 x 5,120   10.8  14.0  17.4  22.9 (10.1 to 11.1) */
+bool few_takes(const void *x, bool f32, long long row_stride, long long rows, int n, int k) {
     const long long size = f32 ? 4 : 2, tiles = n / 16, cus = device_cus();
-    return rows <= (f32 ? 4 : 16) && tiles <= 4 * cus && rows * tiles <= 32 * cus && !((uintptr_t)x & 15) &&
+    const bool few = f32 ? rows <= 4 : rows <= 16 || (rows <= 64 && tiles <= cus && rows * k <= 640 * F8_BLOCK);
+    return few && tiles <= 4 * cus && (rows > 16 || rows * tiles <= 32 * cus) && !((uintptr_t)x & 15) &&
            (rows == 1 || (row_stride * size % 16 == 0 && row_stride <= 1 << 22));
 }
 int few(const void *x, bool f32, long long row_stride, const void *w, const void *ws, int ws_stride, int rows, int n, int k,
         bool relu2, void *out, hipStream_t stream) {
     const Skinny p = {x, (rows > 1 ? row_stride : k) * (f32 ? 4 : 2), nullptr, 0, ws_stride, (const unsigned char *)w,
                       (const unsigned char *)ws, rows, n, k, (k + F8_BLOCK - 1) / F8_BLOCK, out};
-    const auto kernel = relu2 ? fp8_few_kernel<SK_BF16, true> : f32 ? fp8_few_kernel<SK_F32, false> : fp8_few_kernel<SK_BF16, false>;
+    const auto kernel = relu2        ? fp8_few_kernel<SK_BF16, 1, true>
+                        : f32        ? fp8_few_kernel<SK_F32, 1, false>
+                        : rows <= 16 ? fp8_few_kernel<SK_BF16, 1, false>
+                        : rows <= 32 ? fp8_few_kernel<SK_BF16, 2, false> : fp8_few_kernel<SK_BF16, 4, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(n / 16)), dim3(SK_WAVES * WAVE), 0, stream, p);
     return (int)hipGetLastError();
 }
@@ -336,7 +357,7 @@ bool weight_pitch(int stride, int k) { return stride >= (k + F8_BLOCK - 1) / F8_
 
 int linear(const void *x, int is_f32, long long row_stride, const void *w, const void *ws, int ws_stride, long long rows, int n,
            int k, void *out, void *workspace, hipStream_t stream) {
-    if (few_takes(x, is_f32, row_stride, rows, n))
+    if (few_takes(x, is_f32, row_stride, rows, n, k))
         return few(x, is_f32, row_stride, w, ws, ws_stride, (int)rows, n, k, false, out, stream);
     const F8Form f(workspace, rows, k);
     const int status = nc_fp8_quantize_rows(x, is_f32, row_stride, rows, k, f.codes, f.scale, f.pitch, stream);
@@ -365,7 +386,7 @@ using namespace nc;
 
 extern "C" long long nc_fp8_linear_workspace_bytes(const void *x, int is_f32, long long row_stride, long long rows, int n, int k) {
     if (!serve_sizes(rows, n, k)) return -1;
-    return rows == 0 || few_takes(x, is_f32, row_stride, rows, n) ? 0 : f8_form_bytes(rows, k);
+    return rows == 0 || few_takes(x, is_f32, row_stride, rows, n, k) ? 0 : f8_form_bytes(rows, k);
 }
 
 extern "C" int nc_fp8_linear(const void *x, int is_f32, long long row_stride, const void *w, const void *w_scale,
@@ -403,7 +424,7 @@ extern "C" int nc_fp8_mlp(const void *x, long long row_stride, const void *fc, c
     if (misaligned(workspace, 16) || workspace_bytes < nc_fp8_mlp_workspace_bytes(rows, c, hidden)) return NC_ERR_WORKSPACE;
     const hipStream_t s = (hipStream_t)stream;
     const F8Form f(workspace, rows, c), a(f.codes + f.bytes, rows, hidden);
-    if (few_takes(x, false, row_stride, rows, hidden)) {
+    if (rows <= 16 && few_takes(x, false, row_stride, rows, hidden, c)) {
         float *const act = (float *)(a.codes + a.bytes);
         const int status = few(x, false, row_stride, fc, fc_scale, fc_scale_stride, (int)rows, hidden, c, true, act, s);
         return status ? status : linear(act, 1, hidden, proj, proj_scale, proj_scale_stride, rows, n, hidden, out, a.codes, s);

@@ -181,7 +181,7 @@ def _serving_input(x: Tensor, weight: Fp8Weight, name: str) -> Tensor:
     return rows
 
 
-FEW = 16   # rows that one launch of the few-row kernel takes
+FEW = 64   # rows that one launch of the few-row kernel takes
 
 
 def _workspace(x: Tensor, need: int) -> Tensor:

@@ -122,7 +122,7 @@ def test_products_refuse(lib):
 
 
 def linear_args(**over):
-    return list((dict(x=DUMMY, f32=0, stride=256, w=DUMMY, w_scale=DUMMY, w_pitch=4, rows=40, n=32, k=256, out=DUMMY, ws=DUMMY,
+    return list((dict(x=DUMMY, f32=0, stride=256, w=DUMMY, w_scale=DUMMY, w_pitch=4, rows=80, n=32, k=256, out=DUMMY, ws=DUMMY,
                       bytes=2 ** 20, stream=None) | over).values())
 
 
@@ -139,15 +139,17 @@ def test_serving_refuses(lib):
                  dict(rows=2 ** 30), dict(stride=255), dict(w_pitch=1), dict(w_pitch=6), dict(w=odd), dict(out=odd),
                  dict(x=ctypes.c_void_p(0x1001)), dict(x=ctypes.c_void_p(0x1002), f32=1)):
         assert lib.nc_fp8_linear(*linear_args(**over)) == -2, over
-    need = lib.nc_fp8_linear_workspace_bytes(DUMMY, 0, 256, 40, 32, 256)
-    assert need >= 40 * 256 + 40 * 2 and lib.nc_fp8_linear(*linear_args(bytes=need - 1)) == -3
+    need = lib.nc_fp8_linear_workspace_bytes(DUMMY, 0, 256, 80, 32, 256)
+    assert need >= 80 * 256 + 80 * 2 and lib.nc_fp8_linear(*linear_args(bytes=need - 1)) == -3
     assert lib.nc_fp8_linear(*linear_args(ws=odd)) == -3 and lib.nc_fp8_linear(*linear_args(rows=0)) == 0
     for few in (dict(x=odd, ws=None), dict(rows=16, stride=257, ws=None), dict(rows=9, f32=1, ws=None),
-                dict(n=2 ** 20, ws=None)):   # these need it
+                dict(n=2 ** 20, ws=None),
+                dict(rows=65, ws=None), dict(rows=64, k=1296, stride=1296, w_pitch=12, ws=None)):   # these need it
         assert lib.nc_fp8_linear(*linear_args(**(dict(rows=2) | few))) == -1, few
     assert lib.nc_fp8_linear_workspace_bytes(DUMMY, 0, 24, 1, 16, 24) == -1
     assert lib.nc_fp8_linear_workspace_bytes(DUMMY, 0, 16, -1, 16, 16) == -1
     assert lib.nc_fp8_linear_workspace_bytes(DUMMY, 0, 256, 16, 32, 256) == 0
+    assert lib.nc_fp8_linear_workspace_bytes(DUMMY, 0, 1280, 64, 32, 1280) == 0
     for name in ("x", "fc", "fc_scale", "proj", "proj_scale", "out", "ws"):
         assert lib.nc_fp8_mlp(*mlp_args(**{name: None})) == -1, name
     for over in (dict(rows=-1), dict(c=0), dict(c=40), dict(hidden=500), dict(n=20), dict(hidden=2 ** 20 + 16), dict(stride=255),

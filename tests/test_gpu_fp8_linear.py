@@ -259,7 +259,8 @@ def test_serving_layers(device, rows):
 # by the number of rows, of outputs, and of (16 outputs) x (32 rows) against the CUs (256)
 FEW = [(rows, 400, 2064) for rows in (1, 2, 8, 9, 15, 16, 17, 31, 32, 33, 100, 127, 128)]
 FEW += [(1, 16, 20000), (16, 33024, 144), (3, 4992, 400), (20, 48, 16400), (20, 4800, 272), (32, 33024, 144), (40, 4816, 144),
-        (64, 2064, 1296), (97, 9616, 144), (128, 33040, 272), (128, 16, 16384), (77, 16, 16)]
+        (64, 2064, 1296), (97, 9616, 144), (128, 33040, 272), (128, 16, 16384), (77, 16, 16),
+        (37, 1280, 1280), (49, 4096, 16), (64, 144, 1280), (64, 784, 400)]
 
 
 @pytest.mark.parametrize("rows,n,k", FEW)
