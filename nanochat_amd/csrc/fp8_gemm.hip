@@ -531,8 +531,8 @@ __device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, lo
                 for (int h = 0; h < 4; h++)
                     c[h] = *(const u32x2 *)(codes + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1));
             }
-            const float s = f8_scale(act_byte[u]);
-            uint32_t m = 0u;
+            const float s = 4.0f * f8_scale(act_byte[u]);   /* 2 sqrt(a) = sqrt(4 a); a finite a's byte is at most 247 */
+            float m = 0.0f;   /* the largest before its rounding, which keeps the order */
 #pragma unroll
             for (int h = 0; h < 4; h++)
 #pragma unroll
@@ -540,12 +540,12 @@ __device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, lo
                     const auto a = (k & 1) ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[h][k >> 1], s, true)
                                            : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c[h][k >> 1], s, false);
                     /* v_sqrt_f32 is within an ulp; the result is rounded to bf16 right away */
-                    const float x = v[8 * h + 2 * k] * (2.0f * __builtin_amdgcn_sqrtf(a[0]));
-                    const float y = v[8 * h + 2 * k + 1] * (2.0f * __builtin_amdgcn_sqrtf(a[1]));
+                    const float x = v[8 * h + 2 * k] * __builtin_amdgcn_sqrtf(a[0]);
+                    const float y = v[8 * h + 2 * k + 1] * __builtin_amdgcn_sqrtf(a[1]);
                     o[4 * h + k] = bf16_pair(x, y);
-                    m = pair_amax(m, o[4 * h + k]);
+                    m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(__builtin_fabsf(x), __builtin_fabsf(y)), m);
                 }
-            const uint32_t byte = f8_scale_byte(group_max(pair_top(m)));
+            const uint32_t byte = f8_scale_byte(group_max((bf16_pair(m, m) & 0x7FFFu) << 16));
             const float qs = f8_scale(byte);
 #pragma unroll
             for (int h = 0; h < 4; h++)
