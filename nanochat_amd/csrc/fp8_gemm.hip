@@ -15,14 +15,15 @@
  * Full tiles, 256 x 256 (two stages in LDS, one workgroup a CU): four waves, one a SIMD, of 128 x 128 results each (all 256 AGPRs of a
  * lane), which take their next operands from LDS between this stage's products. Bound by the matrix core: a stage takes 1.4 us (3,100
  * TFLOP/s over 256 CUs; a library product of 8,192^3 reaches 3,040), a tile about 4 more for its results, beside which the next
- * tile's first stage is fetched: 8,192^3 375 to 380 us (2,930 to 2,890 TFLOP/s); 65,536 x 4,992 x 1,664 454 to 465 (2,400 to 2,340);
- * 65,536 x 1,664 x 6,656 531 (2,734); the ReLU^2 form of 65,536 x 6,656 x 1,664 594; its backward, which moves 1.7 GB besides, 842. Eight waves of
- * 64 x 128 that took turns at the core read half as much again from LDS and took 417, 508, 611 and 642 us for the first four (and
- * 822 for the backward, whose results two waves a SIMD make in less time than one). Half tiles, 128 x 128, two workgroups a CU, and
- * small ones, 64 x 128, three stages in LDS: for results that make fewer tiles. Bound by LDS, 0.5 to 0.65 and 0.35 to 0.42 us a
- * stage: 1,001 x 5,120 x 1,280 11 us; 128 x 65,536 x 1,664 26 us (4.2 TB/s of weights); 128 x 4,992 x 1,664 7.6. Rings of six stages
- * in small tiles and of four in half tiles leave room for one workgroup a CU: 256 x 4,992 x 1,664 7.7 -> 8.8 us, 1,001 x 4,992 13.4
- * -> 19.9.
+ * tile's first stage is fetched: 8,192^3 375 to 378 us (2,930 to 2,910 TFLOP/s); 65,536 x 4,992 x 1,664 441 to 447 (2,470 to 2,435);
+ * 65,536 x 1,664 x 6,656 531 (2,734); the ReLU^2 form of 65,536 x 6,656 x 1,664 583 to 602; its backward, which moves 1.7 GB besides,
+ * 811 to 827. Eight waves of 64 x 128 that took turns at the core read half as much again from LDS and took 417, 508, 611, 642 and
+ * 822 us. Results leave by buffer stores, whose range takes the place of masks and 64-bit addresses (the five took 376, 453, 534, 594
+ * and 852 us with those).
+ * Half tiles, 128 x 128, two workgroups a CU, and small ones, 64 x 128, three stages in LDS: for results that make fewer tiles.
+ * Bound by LDS, 0.5 to 0.65 and 0.35 to 0.42 us a stage: 1,001 x 5,120 x 1,280 11 us; 128 x 65,536 x 1,664 26 us (4.2 TB/s of
+ * weights); 128 x 4,992 x 1,664 7.6. Rings of six stages in small tiles and of four in half tiles leave room for one workgroup a CU:
+ * 256 x 4,992 x 1,664 7.7 -> 8.8 us, 1,001 x 4,992 13.4 -> 19.9.
  *
  * Rows past M and N and columns past K read zeros (offsets past the buffer resource), and are not stored.
  *
@@ -46,6 +47,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int FG_ROWB = F8_BLOCK;        /* bytes of a row of a stage: one block */
 constexpr int FG_PAST = 0x7FFF0000;      /* a byte offset past every operand's range */
+constexpr int FG_NT = 2;                 /* a store past the caches */
 
 enum { FG_STORE, FG_RELU2, FG_RELU2_BWD };
 
@@ -443,6 +445,9 @@ __device__ __forceinline__ void fg_wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+/* An offset moves on, here and now: the compiler would keep every sum of them in a register of its own. */
+__device__ __forceinline__ void fg_on(uint32_t &at, uint32_t by) { asm volatile("v_add_u32 %0, %1, %0" : "+v"(at) : "s"(by)); }
+
 /* A wave's results. turns: the workgroup's part of LDS for them; acts, act_bytes: ACT_STAGE's codes of a, in LDS, and the scale bytes
  * of the wave's rows `lane` and 64 on. */
 template <class P, int EPI>
@@ -478,6 +483,26 @@ __device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, lo
             act_byte[u] = r < rows_left ? g.acts[(first + r) * g.act_stride + nb] : 127u;
         }
     }
+    /* Stores by way of a buffer's range: rows past the last fall behind it, columns past the last have offsets behind it. So each is an
+     * addition and a store, without masks, and all of them are issued. */
+    const auto rsrc = [&](void *base, long long row_bytes) {
+        return f8_rsrc((unsigned char *)base + m0 * row_bytes, rows * row_bytes);
+    };
+    const uint32_t top = (uint32_t)(16 * P::NU * p.wm);   /* the wave's first row */
+    __amdgpu_buffer_rsrc_t r_out, r_q, r_qs;
+    uint32_t out_at = 0, q_at = 0, qs_at = 0;
+    if constexpr (EPI != FG_RELU2) {
+        r_out = rsrc(g.out, 2LL * g.N);
+        const int c = col + 8 * (lane & 15);
+        out_at = c < cols ? ((top + (lane >> 4)) * (uint32_t)g.N + n0 + c) * 2u : (uint32_t)FG_PAST;
+    }
+    if constexpr (EPI != FG_STORE) {
+        r_q = rsrc(g.q, g.N);
+        r_qs = rsrc(g.qs, g.qs_stride);
+        const int c = col + 16 * (lane & 7);
+        q_at = c < cols ? (top + (lane >> 3)) * (uint32_t)g.N + n0 + c : (uint32_t)FG_PAST;
+        qs_at = grp == 0 ? (top + r16) * (uint32_t)g.qs_stride + nb : (uint32_t)FG_PAST;
+    }
     /* Rows 16 u + r16: this lane's results, columns 32 h + 8 grp + 0 .. 7, into the wave's turn buffer u % 2 */
     u32x2 c_next[4];   /* ACT_STAGE: a's codes of the rows after next */
     const auto read_act = [&](int u) {
@@ -487,7 +512,6 @@ __device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, lo
     };
     if constexpr (ACT_STAGE) read_act(0);
     const auto make = [&](int u) {
-        const int row = 16 * u + r16;
         unsigned char *const turn = mine + u % 2 * P::WAVES * FG_TURN, *const codes = turn + 16 * 256;
         float v[32];
 #pragma unroll
@@ -514,7 +538,8 @@ __device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, lo
                     const int z = 8 * h + 4 * k;
                     q[h][k] = byte == F8_NAN_BYTE ? F8_NAN_CODES : f8_codes(v[z], v[z + 1], v[z + 2], v[z + 3], s);
                 }
-            if (row < rows_left && grp == 0) g.qs[(first + row) * g.qs_stride + nb] = (unsigned char)byte;
+            __builtin_amdgcn_raw_buffer_store_b8((unsigned char)byte, r_qs, qs_at, 0, 0);
+            fg_on(qs_at, 16u * (uint32_t)g.qs_stride);
         } else if constexpr (EPI == FG_RELU2_BWD) {
             /* dh = da 2 sqrt(a) */
             u32x2 c[4];
@@ -551,7 +576,8 @@ __device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, lo
             for (int h = 0; h < 4; h++)
                 q[h] = byte == F8_NAN_BYTE ? u32x2{F8_NAN_CODES, F8_NAN_CODES}
                                            : u32x2{f8_codes(o[4 * h], o[4 * h + 1], qs), f8_codes(o[4 * h + 2], o[4 * h + 3], qs)};
-            if (row < rows_left && grp == 0) g.qs[(first + row) * g.qs_stride + nb] = (unsigned char)byte;
+            __builtin_amdgcn_raw_buffer_store_b8((unsigned char)byte, r_qs, qs_at, 0, 0);
+            fg_on(qs_at, 16u * (uint32_t)g.qs_stride);
         } else {
 #pragma unroll
             for (int k = 0; k < 16; k++) o[k] = bf16_pair(v[2 * k], v[2 * k + 1]);
@@ -577,8 +603,8 @@ __device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, lo
             for (int k = 0; k < 4; k++) {   /* four rows an instruction, past the caches: larger than they are, and read much later */
                 const int r = 4 * k + (lane >> 4), c = lane & 15;
                 const u32x4 d = *(const u32x4 *)(turn + r * 256 + ((c ^ r) << 4));
-                if (16 * u + r < rows_left && col + 8 * c < cols)
-                    __builtin_nontemporal_store(d, (u32x4 *)(g.out + (first + 16 * u + r) * g.N + n0 + col + 8 * c));
+                __builtin_amdgcn_raw_buffer_store_b128(d, r_out, out_at, 0, FG_NT);
+                fg_on(out_at, 8u * g.N);   /* four rows */
             }
         }
         if constexpr (EPI != FG_STORE) {
@@ -588,8 +614,8 @@ __device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, lo
                 const u32x4 d = *(const u32x4 *)(codes + fg_code_place(r, c));
                 /* through the caches: the next product reads them (an MLP of 9,995 x 1,280/5,120 170 us past them, 157; the training of
                  * 65,536 x 1,664/6,656, whose 436 MB do not fit, 5,108 and 5,170) */
-                if (16 * u + r < rows_left && col + 16 * c < cols)
-                    *(u32x4 *)(g.q + (first + 16 * u + r) * g.N + n0 + col + 16 * c) = d;
+                __builtin_amdgcn_raw_buffer_store_b128(d, r_q, q_at, 0, 0);
+                fg_on(q_at, 8u * g.N);
             }
         }
     };
@@ -623,6 +649,16 @@ template <class P, int EPI> __device__ __forceinline__ void fg_run(const F8Gemm 
     fg_walk_ring<P, P::NU == 1 && EPI == FG_RELU2>(g, p, m0, t.x * P::TN, lds, acc);
     const uint32_t none[2] = {0u, 0u};
     fg_results<P, EPI>(g, p, m0, t.x * P::TN, acc, lds, lds, none);
+}
+
+/* The kernel's arguments with the codes' places read anew: kept over the walk they are four scalar registers too many. */
+__device__ __forceinline__ F8Gemm fg_again(F8Gemm g) {
+    typedef __attribute__((address_space(4))) const F8Gemm Args;
+    Args *at = (Args *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    g.q = at->q;
+    g.qs = at->qs;
+    return g;
 }
 
 /* Full tiles: a workgroup a CU takes every gridDim.x-th of them, and the first stage of the next is fetched while the last one's results
@@ -660,9 +696,9 @@ template <int EPI> __device__ __forceinline__ void fg_run_full(const F8Gemm &g, 
             dma = FgDma(g, p, (long long)t.y * P::TM, t.x * P::TN, lds, flip);
             dma.fetch(0);
         }
-        fg_results<P, EPI>(g, done, m0, n0, acc, lds + (flip ^ 1) * P::STAGE, lds + flip * P::STAGE, act_bytes);
+        fg_results<P, EPI>(fg_again(g), done, m0, n0, acc, lds + (flip ^ 1) * P::STAGE, lds + flip * P::STAGE, act_bytes);
         if (!more) return;
-        stores = done.rows == P::TM && done.cols == P::TN;   /* all were issued */
+        stores = done.some;   /* then all were issued */
         __builtin_amdgcn_s_waitcnt(0xC07F);   /* the LDS reads */
         fg_barrier();
     }

@@ -84,8 +84,8 @@ def test_every_kernel_is_built(kernels):
 def test_a_tiles_stores_are_as_many_as_its_successor_counts(kernels, epi, wide, narrow):
     """The wait for a tile's first stage lets that many newer stores of the last tile's be on their way."""
     count = lambda mn: sum(line.strip().startswith(mn) for line in kernels[0][("gemm", epi)])   # noqa: E731
-    assert count("global_store_dwordx4") == wide and count("global_store_byte") == narrow
-    assert count("buffer_store") == count("flat_store") == 0
+    assert count("buffer_store_dwordx4") == wide and count("buffer_store_byte") == narrow
+    assert count("global_store") == count("flat_store") == 0
 
 
 @pytest.mark.parametrize("which", KERNELS)
