@@ -212,6 +212,45 @@ def test_product_relu2_backward(device, rows, n, k):
     assert same_form(q, q_s, codes_of(dh), 1)
 
 
+@pytest.mark.parametrize("rows,n,k", [(65, 1280, 128), (600, 4112, 128), (3000, 4112, 128), (9000, 2064, 272)])
+def test_products_write_their_results_and_nothing_else(device, rows, n, k):
+    """Results of small, half, full and both tiles in the middle of larger buffers: 300 rows before and behind them, and the scales'
+    other columns, stay."""
+    gen = torch.Generator().manual_seed(rows)
+    codes, scale, _ = form(gen, device, rows, k)
+    w, _ = weight(gen, device, n, k)
+    a8, a_s = product_relu2(codes, scale, w)
+    dh, q, q_s = product_relu2_bwd(codes, scale, w, a8, a_s)
+    y, blocks, pitch, guard = fl.fp8_matmul(codes, scale, w), a_s.size(1), 4 * ((n + 127) // 128 // 4 + 2), 300
+
+    def around(width):
+        whole = torch.full((rows + 2 * guard, width), 0xA5, dtype=torch.uint8, device=device)
+        return whole, whole[guard:].data_ptr()
+
+    def check(whole, want):
+        inside = whole[guard:guard + rows, :want.size(1)]
+        assert torch.equal(inside, want)
+        inside.fill_(0xA5)
+        assert bool((whole == 0xA5).all())
+
+    head = (codes.data_ptr(), scale.data_ptr(), scale.stride(0), w.codes.data_ptr(), w.scale.data_ptr(), w.scale.stride(0), rows, n, k)
+    raw = lambda v: v.contiguous().view(torch.uint8)   # noqa: E731
+    lib = hip_library()
+    out, out_at = around(2 * n)
+    native.check(lib.nc_fp8_matmul(*head, out_at, stream()))
+    check(out, raw(y))
+    form_, form_at = around(n)
+    exps, exps_at = around(pitch)
+    native.check(lib.nc_fp8_matmul_relu2(*head, form_at, exps_at, pitch, stream()))
+    check(form_, raw(a8))
+    check(exps, raw(a_s)[:, :blocks])
+    native.check(lib.nc_fp8_matmul_relu2_bwd(*head, a8.data_ptr(), a_s.data_ptr(), a_s.stride(0), out_at, form_at, exps_at, pitch,
+                                             stream()))
+    check(out, raw(dh))
+    check(form_, raw(q))
+    check(exps, raw(q_s)[:, :blocks])
+
+
 def test_product_of_everyone_elses_scales(device):
     """Scales of other tensors than quantize_rows makes: a wider pitch, and exponents far apart in one row."""
     gen = torch.Generator().manual_seed(3)
