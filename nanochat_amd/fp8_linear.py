@@ -61,12 +61,14 @@ def _check_codes(codes: Tensor, name: str, device: torch.device, part: str = "")
         raise ValueError(f"{name}{part} must have a multiple of 16 columns, got {codes.size(1)}")
 
 
-def _check_scale(scale: Tensor, name: str, rows: int, cols: int, device: torch.device, part: str = "") -> int:
-    """A scale tensor's row stride in bytes."""
+def _check_scale(scale: Tensor, name: str, rows: int, cols: int, device: torch.device, part: str = "",
+                 padded: bool = False) -> int:
+    """A scale tensor's row stride in bytes. padded: it may have its rows' padding in its shape, as an op returns it."""
     if scale.dtype != SCALE:
         raise TypeError(f"{name}{part} must be {SCALE}, got {scale.dtype}")
     blocks = -(-cols // BLOCK)
-    if scale.dim() != 2 or scale.shape != (rows, blocks) or scale.device != device:
+    if (scale.dim() != 2 or scale.device != device
+            or (scale.shape != (rows, blocks) and not (padded and scale.shape == (rows, -(-blocks // 4) * 4)))):
         raise ValueError(f"{name}{part} must be [{rows}, {blocks}] on {device}, got {tuple(scale.shape)} on {scale.device}")
     pitch, step = scale.stride()
     if ((blocks > 1 and step != 1) or pitch % 4 or pitch < blocks or pitch > cols or scale.data_ptr() % 4
@@ -89,6 +91,14 @@ def _check_weight(w: Fp8Weight, name: str, device: torch.device, transposed: boo
     if codes_t.shape != (k, n):
         raise ValueError(f"{name}.codes_t must be {(k, n)}, got {tuple(codes_t.shape)}")
     return pitch, _check_scale(scale_t, name, -(-k // BLOCK), n, device, ".scale_t")
+
+
+def _check_kept(codes: Tensor, scale: Tensor, names: tuple[str, str], rows: int, cols: int, of: int, device: torch.device) -> None:
+    """An 8-bit form as a backward op is given it: codes [rows, cols] with a scale for each `of` rows."""
+    _check_codes(codes, names[0], device)
+    if codes.shape != (rows, cols):
+        raise ValueError(f"{names[0]} must be {(rows, cols)}, got {tuple(codes.shape)}")
+    _check_scale(scale, names[1], -(-rows // of), cols, device, padded=True)
 
 
 def _as_rows(x: Tensor, name: str, dtypes: tuple, of: int = 16) -> Tensor:
@@ -382,7 +392,10 @@ def _run_linear_bwd(dy: Tensor, x8: Tensor, xs: Tensor, codes_t: Tensor, scale_t
     rows, lib = _as_rows(dy, "dy", (BF16,)), hip_library()
     if need_w:
         rows = _dense(rows)
-    (m, n), k = rows.shape, x8.size(1)
+    (m, n), k = rows.shape, x8.size(-1)
+    _check_kept(x8, xs, ("x8", "xs"), m, k, 1, dy.device)
+    if need_x:
+        _check_kept(codes_t, scale_t, ("codes_t", "scale_t"), k, n, BLOCK, dy.device)
     with device_guard(dy):
         dx = torch.empty(m, k, dtype=BF16, device=dy.device) if need_x else dy.new_empty(0)
         dw, mode, into = _layer_grad(n, k, grad, need_w, wide, dy)
@@ -487,7 +500,13 @@ def _run_mlp_bwd(dy: Tensor, x8: Tensor, xs: Tensor, a8: Tensor, a_s: Tensor, fc
     rows, lib = _as_rows(dy, "dy", (BF16,)), hip_library()
     if need_proj:
         rows = _dense(rows)
-    (m, n), c, hidden = rows.shape, x8.size(1), a8.size(1)
+    (m, n), c, hidden = rows.shape, x8.size(-1), a8.size(-1)
+    _check_kept(x8, xs, ("x8", "xs"), m, c, 1, dy.device)
+    _check_kept(a8, a_s, ("a8", "a_s"), m, hidden, 1, dy.device)
+    if need_x:
+        _check_kept(fc_codes_t, fc_scale_t, ("fc_codes_t", "fc_scale_t"), c, hidden, BLOCK, dy.device)
+    if need_x or need_fc:
+        _check_kept(proj_codes_t, proj_scale_t, ("proj_codes_t", "proj_scale_t"), hidden, n, BLOCK, dy.device)
     with device_guard(dy):
         dx = torch.empty(m, c, dtype=BF16, device=dy.device) if need_x else dy.new_empty(0)
         dfc, fc_mode, fc_into = _layer_grad(hidden, c, fc_grad, need_fc, fc_wide, dy)

@@ -1,0 +1,131 @@
+"""What the 8-bit layers hand to the library, without a GPU: host tensors that say they lie on a device, and a library that
+records its calls. Operands that do not belong together have to be refused before any of them."""
+import contextlib
+
+import pytest
+import torch
+
+from nanochat_amd import fp8_linear as fl, native
+
+CODES, SCALE, BF16, F32 = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.bfloat16, torch.float32
+
+
+class OnDevice(torch.Tensor):
+    is_cuda = True
+
+
+class Recorder:
+    """The library's functions by name: calls of theirs are kept, and answered from `answers` (else 0)."""
+
+    def __init__(self):
+        self.calls, self.answers = [], {}
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return self.answers.get(name, 0)
+        return call
+
+    def named(self, name):
+        return [args for n, args in self.calls if n == name]
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    r = Recorder()
+    monkeypatch.setattr(fl, "hip_library", lambda: r)
+    monkeypatch.setattr(native, "hip_library", lambda: native_strings)
+    monkeypatch.setattr(fl, "device_guard", lambda t: contextlib.nullcontext())
+    monkeypatch.setattr(fl, "stream", lambda: 0)
+    return r
+
+
+class native_strings:
+    @staticmethod
+    def nc_status_string(status):
+        return b"a status"
+
+
+def new(*shape, dtype=BF16):
+    return torch.zeros(*shape, dtype=torch.uint8).view(dtype).as_subclass(OnDevice) if dtype in (CODES, SCALE) else \
+        torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+
+
+def up4(n):
+    return -(-n // 4) * 4
+
+
+def form(rows, cols, of=1, whole=True):
+    blocks = -(-cols // 128)
+    scale = new(-(-rows // of), up4(blocks), dtype=SCALE)
+    return new(rows, cols, dtype=CODES), scale if whole else scale[:, :blocks]
+
+
+# --- the backward ops, given operands that do not belong together
+
+M, N, K, F = 10, 528, 656, 560   # of more blocks than one dword of scales holds
+
+
+def linear_bwd(**over):
+    x8, xs = form(M, K)
+    codes_t, scale_t = form(K, N, 128)
+    a = dict(dy=new(M, N), x8=x8, xs=xs, codes_t=codes_t, scale_t=scale_t, grad=None, need_x=True, need_w=True, wide=True) | over
+    return fl._run_linear_bwd(**a)
+
+
+def mlp_bwd(**over):
+    """x [M, K], fc [F, K], proj [N, F]"""
+    x8, xs = form(M, K)
+    a8, a_s = form(M, F)
+    f, fs = form(K, F, 128)
+    p, ps = form(F, N, 128)
+    a = dict(dy=new(M, N), x8=x8, xs=xs, a8=a8, a_s=a_s, fc_codes_t=f, fc_scale_t=fs, proj_codes_t=p, proj_scale_t=ps, fc_grad=None,
+             proj_grad=None, need_x=True, need_fc=True, need_proj=True, fc_wide=True, proj_wide=True) | over
+    return fl._run_mlp_bwd(**a)
+
+
+WRONG_FORMS = {"fewer rows": lambda r, c, of: form(r - of, c, of), "more rows": lambda r, c, of: form(r + of, c, of),
+               "fewer columns": lambda r, c, of: form(r, 16, of), "no tensor of the op": lambda r, c, of: form(0, 16, of)}
+LINEAR_FORMS = {"x8": ("xs", M, K, 1), "codes_t": ("scale_t", K, N, 128)}
+MLP_FORMS = {"x8": ("xs", M, K, 1), "a8": ("a_s", M, F, 1), "fc_codes_t": ("fc_scale_t", K, F, 128),
+             "proj_codes_t": ("proj_scale_t", F, N, 128)}
+BOTH = [(linear_bwd, name, *v) for name, v in LINEAR_FORMS.items()] + [(mlp_bwd, name, *v) for name, v in MLP_FORMS.items()]
+
+
+@pytest.mark.parametrize("call,codes,scale,rows,cols,of", BOTH)
+@pytest.mark.parametrize("wrong", WRONG_FORMS)
+def test_backward_ops_refuse_forms_of_other_sizes(recorder, call, codes, scale, rows, cols, of, wrong):
+    c, s = WRONG_FORMS[wrong](rows, cols, of)
+    right_c, right_s = form(rows, cols, of)
+    for over in ({codes: c, scale: s}, {codes: right_c, scale: s}, {codes: c, scale: right_s}):
+        with pytest.raises(ValueError):
+            call(**over)
+    assert not recorder.calls
+
+
+@pytest.mark.parametrize("call,codes,scale,rows,cols,of", BOTH)
+def test_backward_ops_refuse_forms_of_other_types_and_places(recorder, call, codes, scale, rows, cols, of):
+    c, s = form(rows, cols, of)
+    for over in ({codes: c.float()}, {codes: c.view(torch.uint8)}, {scale: s.view(torch.uint8)}, {scale: s.float()}):
+        with pytest.raises(TypeError):
+            call(**over)
+    for over in ({codes: c.as_subclass(torch.Tensor)}, {codes: c.as_subclass(torch.Tensor).to("meta")},
+                 {scale: s.as_subclass(torch.Tensor).to("meta")}, {codes: form(cols, rows // 16 * 16 + 16, of)[0].t()[:rows]},
+                 {scale: s.repeat(1, 3)[:, :s.size(1)][:, ::1].t().contiguous().t()}):
+        with pytest.raises(ValueError):
+            call(**over)
+    assert not recorder.calls
+
+
+def test_backward_ops_take_forms_with_and_without_padding(recorder):
+    """As the forward ops return them, and as quantize_weight does; what a call does not read it does not check."""
+    for whole in (True, False):
+        linear_bwd(**dict(zip(("x8", "xs"), form(M, K, whole=whole))), **dict(zip(("codes_t", "scale_t"), form(K, N, 128, whole))))
+        mlp_bwd(**dict(zip(("a8", "a_s"), form(M, F, whole=whole))),
+                **dict(zip(("proj_codes_t", "proj_scale_t"), form(F, N, 128, whole))))
+    empty = new(0, dtype=CODES), new(0, dtype=SCALE)
+    linear_bwd(codes_t=empty[0], scale_t=empty[1], need_x=False)
+    mlp_bwd(fc_codes_t=empty[0], fc_scale_t=empty[1], need_x=False)
+    mlp_bwd(fc_codes_t=empty[0], fc_scale_t=empty[1], proj_codes_t=empty[0], proj_scale_t=empty[1], need_x=False, need_fc=False)
+    assert len(recorder.named("nc_fp8_linear_bwd")) == 3 and len(recorder.named("nc_fp8_mlp_bwd")) == 4
+    assert all(args[8:11] == (M, N, K) for args in recorder.named("nc_fp8_linear_bwd"))
