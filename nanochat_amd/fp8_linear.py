@@ -322,12 +322,14 @@ def _whole_scale(like: Tensor, rows: int, cols: int) -> Tensor:
     return torch.empty(rows, -(-_blocks(cols) // 4) * 4, dtype=SCALE, device=like.device)
 
 
-def _layer_grad(weight: int, k: int, grad: Tensor | None, wanted: bool, wide: bool, like: Tensor) -> tuple[Tensor, int, Tensor]:
+def _layer_grad(weight: int, k: int, grad: Tensor | None, wanted: bool, wide: bool, like: Tensor,
+                name: str) -> tuple[Tensor, int, Tensor]:
     """A layer's weight gradient [weight, k] as its op returns it (new, or empty where it goes into grad or is not wanted), the
-    mode that makes it, and where it goes."""
+    mode that makes it, and where it goes. grad is checked here, where it is written: since the forward it may have changed."""
     if not wanted:
         return like.new_empty(0), _GRAD_NONE, None
     if grad is not None:
+        _check_grad(grad, (weight, k), like.device, name)
         torch.autograd.graph.increment_version(grad)
         return like.new_empty(0), _GRAD_ADD, grad
     out = torch.empty(weight, k, dtype=F32 if wide else BF16, device=like.device)
@@ -398,7 +400,7 @@ def _run_linear_bwd(dy: Tensor, x8: Tensor, xs: Tensor, codes_t: Tensor, scale_t
         _check_kept(codes_t, scale_t, ("codes_t", "scale_t"), k, n, BLOCK, dy.device)
     with device_guard(dy):
         dx = torch.empty(m, k, dtype=BF16, device=dy.device) if need_x else dy.new_empty(0)
-        dw, mode, into = _layer_grad(n, k, grad, need_w, wide, dy)
+        dw, mode, into = _layer_grad(n, k, grad, need_w, wide, dy, "grad")
         if m == 0:
             return dx, dw.zero_()
         need = lib.nc_fp8_linear_bwd_workspace_bytes(m, n, k, need_x, mode)
@@ -509,8 +511,8 @@ def _run_mlp_bwd(dy: Tensor, x8: Tensor, xs: Tensor, a8: Tensor, a_s: Tensor, fc
         _check_kept(proj_codes_t, proj_scale_t, ("proj_codes_t", "proj_scale_t"), hidden, n, BLOCK, dy.device)
     with device_guard(dy):
         dx = torch.empty(m, c, dtype=BF16, device=dy.device) if need_x else dy.new_empty(0)
-        dfc, fc_mode, fc_into = _layer_grad(hidden, c, fc_grad, need_fc, fc_wide, dy)
-        dproj, proj_mode, proj_into = _layer_grad(n, hidden, proj_grad, need_proj, proj_wide, dy)
+        dfc, fc_mode, fc_into = _layer_grad(hidden, c, fc_grad, need_fc, fc_wide, dy, "fc_grad")
+        dproj, proj_mode, proj_into = _layer_grad(n, hidden, proj_grad, need_proj, proj_wide, dy, "proj_grad")
         if m == 0:
             return dx, dfc.zero_(), dproj.zero_()
         need = lib.nc_fp8_mlp_bwd_workspace_bytes(m, c, hidden, n, need_x, fc_mode, proj_mode)

@@ -129,3 +129,43 @@ def test_backward_ops_take_forms_with_and_without_padding(recorder):
     mlp_bwd(fc_codes_t=empty[0], fc_scale_t=empty[1], proj_codes_t=empty[0], proj_scale_t=empty[1], need_x=False, need_fc=False)
     assert len(recorder.named("nc_fp8_linear_bwd")) == 3 and len(recorder.named("nc_fp8_mlp_bwd")) == 4
     assert all(args[8:11] == (M, N, K) for args in recorder.named("nc_fp8_linear_bwd"))
+
+
+# --- gradient buffers, where they are written
+
+def bad_buffers(n, k):
+    return [new(n, k, dtype=torch.float64), new(n, k), new(16, 16, dtype=F32), new(k, n, dtype=F32), new(n * k, dtype=F32),
+            new(k, n, dtype=F32).t(), new(n, 2 * k, dtype=F32)[:, :k], new(n * k + 1, dtype=F32)[1:].view(n, k),
+            torch.zeros(n, k, device="meta")]
+
+
+def test_backward_ops_refuse_buffers_that_do_not_fit(recorder):
+    for call, name, n, k in ((linear_bwd, "grad", N, K), (mlp_bwd, "fc_grad", F, K), (mlp_bwd, "proj_grad", N, F)):
+        for bad in bad_buffers(n, k):
+            with pytest.raises(ValueError, match=name):
+                call(**{name: bad})
+        assert not recorder.calls
+        call(**{name: new(n, k, dtype=F32)})
+        assert len(recorder.named("nc_fp8_linear_bwd") + recorder.named("nc_fp8_mlp_bwd")) == 1
+        recorder.calls.clear()
+
+
+@pytest.mark.parametrize("other", [dict(dtype=torch.float64), dict(shape=(16, 16)), dict(dtype=BF16)])
+def test_a_buffer_exchanged_before_the_backward_is_refused(recorder, monkeypatch, other):
+    """The forward has checked it; what counts is what it is when it is added to."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)   # of what the calls make themselves too
+    monkeypatch.setattr(fl, "_linear", fl._run_linear)
+    monkeypatch.setattr(fl, "_linear_bwd", fl._run_linear_bwd)
+    monkeypatch.setattr(fl, "_mlp", fl._run_mlp)
+    monkeypatch.setattr(fl, "_mlp_bwd", fl._run_mlp_bwd)
+    x = new(M, K).requires_grad_()
+    for layer, shape in ((lambda b: fl.checkpointed_linear(x, new(N, K), grad=b), (N, K)),
+                         (lambda b: fl.checkpointed_mlp(x, new(F, K), new(N, F), fc_grad=b), (F, K)),
+                         (lambda b: fl.checkpointed_mlp(x, new(F, K), new(N, F), proj_grad=b), (N, F))):
+        buffer = new(*shape, dtype=F32)
+        y = layer(buffer)
+        recorder.calls.clear()
+        buffer.data = torch.zeros(other.get("shape", shape), dtype=other.get("dtype", F32))
+        with pytest.raises(ValueError, match="grad must be"):
+            y.backward(new(M, y.size(-1)))
+        assert not recorder.calls
