@@ -351,7 +351,8 @@ int nc_debug_sample_tokens(const void *logits, int is_bf16, long long row_stride
  * gradients, 128 x 128 for weights (the last of a row or column may be shorter). The scale is the least power of two s with
  * max |x| <= 448 s, at least 2^-126 (1 for a block of zeros); a code is x / s rounded to nearest even and stands for code * s. A
  * block that holds an infinity or a NaN becomes NaN (byte 255, codes 0x7F). Columns are a multiple of 16. Codes are dense and
- * 16-byte aligned; scales have rows at a stride in bytes that is a multiple of 4, readable to its end, 4-byte aligned.
+ * 16-byte aligned; scales have rows at a stride in bytes that is a multiple of 4, 4-byte aligned, each row's readable up to a multiple
+ * of 4 (the last row's too, but not to the end of its stride).
  */
 
 /* The 8-bit form of rows of activations: x bf16 or fp32 (is_f32) [rows][cols] at row_stride elements (any alignment of its

@@ -183,8 +183,9 @@ __device__ __forceinline__ void fg_walk_ring(const F8Gemm &g, const FgPlace &p, 
                                              f32x4 (&acc)[8][P::NU]) {
     const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK, K = g.K;
     const u32x4 ra = f8_words(g.a + m0 * K, (long long)p.rows * K), rw = f8_words(g.w + (long long)n0 * K, (long long)p.cols * K);
-    const u32x4 rsa = f8_words(g.as + m0 * g.as_stride, p.rows * g.as_stride);
-    const u32x4 rsw = f8_words(g.ws + (long long)p.nb * g.ws_stride, g.ws_stride);
+    /* stages past the last ask for dwords behind their rows' scales: zeros, or the next row's */
+    const u32x4 rsa = f8_words(g.as + m0 * g.as_stride, f8_scale_range(p.rows, g.as_stride, stages));
+    const u32x4 rsw = f8_words(g.ws + (long long)p.nb * g.ws_stride, f8_scale_range(1, g.ws_stride, stages));
     const uint32_t base = f8_lds(lds) + p.wave * 1024;
     unsigned char *const scales = lds + P::RING * P::STAGE + p.wave * 2 * FG_OWN;
     const uint32_t scale_to = f8_lds(scales);
@@ -264,8 +265,9 @@ struct FgDma {
         : flip(flip) {
         ra = f8_words(g.a + m0 * g.K, (long long)p.rows * g.K);
         rw = f8_words(g.w + (long long)n0 * g.K, (long long)p.cols * g.K);
-        rsa = f8_words(g.as + m0 * g.as_stride, p.rows * g.as_stride);
-        rsw = f8_words(g.ws + (long long)(p.some ? p.nb : 0) * g.ws_stride, g.ws_stride);
+        const int stages = (g.K + F8_BLOCK - 1) / F8_BLOCK;
+        rsa = f8_words(g.as + m0 * g.as_stride, f8_scale_range(p.rows, g.as_stride, stages));
+        rsw = f8_words(g.ws + (long long)(p.some ? p.nb : 0) * g.ws_stride, f8_scale_range(1, g.ws_stride, stages));
         scale_at = (128 * p.wm + p.lane) * (int)g.as_stride;
         more = 64 * (int)g.as_stride;
         lds = f8_lds(b0) + p.wave * 1024;

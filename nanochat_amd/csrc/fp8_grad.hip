@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(GR_WAVES *WAVE, 1) fp8_grad_kernel(F8Grads bot
     GrDma dma;
     dma.ra = f8_words(p.dy + m0 * p.N1, (long long)rows * p.N1 * 2);
     dma.rx = f8_words(p.x + m0 * p.N2, (long long)rows * p.N2);
-    dma.rs = f8_words(p.xs + m0 * p.xs_stride, rows * p.xs_stride);
+    dma.rs = f8_words(p.xs + m0 * p.xs_stride, f8_scale_range(rows, p.xs_stride, (p.N2 + F8_BLOCK - 1) / F8_BLOCK));
     dma.lds = f8_lds(lds);
     dma.wave = wave;
     dma.s_row = (uint32_t)p.xs_stride;

@@ -73,6 +73,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t f8_rsrc(const void *p, long lo
                                              __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
 }
 
+/* Bytes of the scales of some rows of `blocks` blocks, from the first row's on, that a kernel may read: whole rows to their end, the
+ * last one to its own scales' padding to a dword. A tensor may end there, also where its rows lie further apart. */
+__host__ __device__ static inline long long f8_scale_range(long long rows, long long stride, int blocks) {
+    return (rows - 1) * stride + (blocks + 3) / 4 * 4;
+}
+
 /* DMA from memory to LDS of 16 or 4 bytes a lane (lane l's to `to` + 16 l or 4 l), as inline assembly: the compiler makes every
  * LDS read that follows its own form wait for it. The kernels that use it load and store nothing else meanwhile, and keep its
  * waits themselves. An offset past the resource's range reads zeros without an access. */
