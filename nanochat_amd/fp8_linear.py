@@ -191,7 +191,8 @@ def _serving_input(x: Tensor, weight: Fp8Weight, name: str) -> Tensor:
     return rows
 
 
-FEW = 64   # rows that one launch of the few-row kernel takes
+FEW = 64          # rows that one launch of the few-row kernel takes
+NO_POINTER = -1   # a call's status where a pointer that it needs is missing (NC_ERR_NULL)
 
 
 def _workspace(x: Tensor, need: int) -> Tensor:
@@ -210,10 +211,12 @@ def fp8_linear(x: Tensor, weight: Fp8Weight) -> Tensor:
         out = torch.empty(m, n, dtype=BF16, device=x.device)
         args = (at, 0, stride, weight.codes.data_ptr(), weight.scale.data_ptr(), pitch, m, n, k, out.data_ptr())
         # a few rows need no workspace as a rule: asked for only where the call refuses to go without
-        if m > FEW or call(*args, None, 0, stream()) != 0:
+        status = call(*args, None, 0, stream()) if m <= FEW else NO_POINTER
+        if status == NO_POINTER:
             need = hip_library().nc_fp8_linear_workspace_bytes(at, 0, stride, m, n, k)
             ws = _workspace(x, need)
-            check(call(*args, ws.data_ptr(), need, stream()))
+            status = call(*args, ws.data_ptr(), need, stream())
+        check(status)
     return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 

@@ -169,3 +169,33 @@ def test_a_buffer_exchanged_before_the_backward_is_refused(recorder, monkeypatch
         with pytest.raises(ValueError, match="grad must be"):
             y.backward(new(M, y.size(-1)))
         assert not recorder.calls
+
+
+# --- statuses
+
+@pytest.mark.parametrize("rows", [1, 40, 64])
+@pytest.mark.parametrize("status", [-2, -3, 1, 98, 719])
+def test_a_failed_launch_of_a_few_rows_is_reported(recorder, rows, status):
+    """Only a missing workspace's status has the call made again with one: a failure's would be lost behind a second call that
+    returns 0."""
+    w8 = fl.Fp8Weight(*form(N, K, 128, whole=False))
+    answers = iter([status])
+    recorder.nc_fp8_linear = lambda *args: (recorder.calls.append(("nc_fp8_linear", args)), next(answers, 0))[1]
+    with pytest.raises(native.NativeError, match=str(status)):
+        fl.fp8_linear(new(rows, K), w8)
+    assert len(recorder.named("nc_fp8_linear")) == 1
+
+
+@pytest.mark.parametrize("second", [0, 98])
+def test_a_missing_workspace_is_brought(recorder, second):
+    w8 = fl.Fp8Weight(*form(N, K, 128, whole=False))
+    answers = iter([-1, second])
+    recorder.answers["nc_fp8_linear_workspace_bytes"] = 4096
+    recorder.nc_fp8_linear = lambda *args: (recorder.calls.append(("nc_fp8_linear", args)), next(answers))[1]
+    if second:
+        with pytest.raises(native.NativeError, match="98"):
+            fl.fp8_linear(new(40, K), w8)
+    else:
+        assert fl.fp8_linear(new(40, K), w8).shape == (40, N)
+    without, given = recorder.named("nc_fp8_linear")
+    assert without[10:12] == (None, 0) and given[10] is not None and given[11] == 4096
