@@ -270,6 +270,12 @@ def _check_grad(grad: Tensor, shape: tuple, device: torch.device, name: str) -> 
         raise ValueError(f"{name} must be a contiguous, 16-byte aligned {tuple(shape)}, got {tuple(grad.shape)}")
 
 
+def _written(t: Tensor) -> None:
+    """t is added to in place: autograd may hold it for a backward of its own, which has to notice."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def checkpoint_weight_grad(dy: Tensor, codes: Tensor, scale: Tensor, out: Tensor | None = None,
                            dtype: torch.dtype = F32) -> Tensor:
     """The gradient dy^T x of a weight [N, K], dy bf16 [..., N] (N a multiple of 8) the gradient behind the layer and x [M, K] the 8-bit
@@ -283,6 +289,7 @@ def checkpoint_weight_grad(dy: Tensor, codes: Tensor, scale: Tensor, out: Tensor
     shape = (dy.size(1), codes.size(1))
     if out is not None:
         _check_grad(out, shape, dy.device, "out")
+        _written(out)
     elif dtype not in (F32, BF16):
         raise TypeError(f"dtype must be {F32} or {BF16}, got {dtype}")
     with device_guard(dy):
@@ -333,7 +340,7 @@ def _layer_grad(weight: int, k: int, grad: Tensor | None, wanted: bool, wide: bo
         return like.new_empty(0), _GRAD_NONE, None
     if grad is not None:
         _check_grad(grad, (weight, k), like.device, name)
-        torch.autograd.graph.increment_version(grad)
+        _written(grad)
         return like.new_empty(0), _GRAD_ADD, grad
     out = torch.empty(weight, k, dtype=F32 if wide else BF16, device=like.device)
     return out, _GRAD_F32 if wide else _GRAD_BF16, out

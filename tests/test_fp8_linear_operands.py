@@ -199,3 +199,18 @@ def test_a_missing_workspace_is_brought(recorder, second):
         assert fl.fp8_linear(new(40, K), w8).shape == (40, N)
     without, given = recorder.named("nc_fp8_linear")
     assert without[10:12] == (None, 0) and given[10] is not None and given[11] == 4096
+
+
+# --- autograd's bookkeeping
+
+def test_a_weight_gradient_added_in_place_is_noticed(recorder):
+    """A backward that needs the buffer as it was refuses to run on what it has become."""
+    codes, scale = form(M, K, whole=False)
+    out, factor = new(N, K, dtype=F32).as_subclass(torch.Tensor), torch.ones(N, K, requires_grad=True)
+    y = (factor * out).sum()
+    fl.checkpoint_weight_grad(new(M, N), codes, scale, out=out.as_subclass(OnDevice))
+    assert len(recorder.named("nc_fp8_weight_grad")) == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():   # such tensors have no versions
+        fl.checkpoint_weight_grad(new(M, N), codes, scale, out=new(N, K, dtype=F32))
