@@ -459,6 +459,14 @@ class _Linear(torch.autograd.Function):
 _NOT_HELD = (None, None, None, None)
 
 
+def _asking(weight: Tensor, grad: Tensor | None, *others: Tensor) -> Tensor:
+    """weight, or, where a buffer is given for its gradient and nothing else would have the call recorded, an alias that requires
+    a gradient (and gets none: it goes into the buffer)."""
+    if grad is None or weight.requires_grad or not torch.is_grad_enabled() or any(t.requires_grad for t in others):
+        return weight
+    return weight.detach().requires_grad_()
+
+
 def checkpointed_linear(x: Tensor, weight: Tensor, weight8: Fp8Weight | None = None, grad: Tensor | None = None) -> Tensor:
     """x bf16 [..., K] through a linear layer in 8-bit products, bf16 [..., N], differentiable in x and weight (bf16 or fp32
     [N, K], N and K multiples of 16 up to 65,536). Kept for the backward is x's 8-bit form alone, not x. With x8, dy8, w8 the 8-bit forms:
@@ -467,7 +475,10 @@ def checkpointed_linear(x: Tensor, weight: Tensor, weight8: Fp8Weight | None = N
 
     weight8: quantize_weight(weight, transpose=True), which a program that uses a weight more than once a step keeps; made in
     the call when absent. grad: None (dw is returned to autograd, in the weight's type), or an fp32 [N, K] buffer that dw is
-    added to in the backward, autograd then getting none for the weight. The gradients themselves cannot be differentiated."""
+    added to in the backward, autograd then getting none for the weight; with a buffer the call is recorded (unless under
+    torch.no_grad()) and dw made whether or not x or weight requires a gradient. The gradients themselves cannot be
+    differentiated."""
+    weight = _asking(weight, grad, x)
     return _Linear.apply(x, weight, *(weight8 or _NOT_HELD), grad)
 
 
@@ -590,4 +601,6 @@ def checkpointed_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc8: Fp8Weight | None 
 
     The derivative of the square is read from the checkpoint itself: 2 relu(h) = 2 sqrt(a). fc8, proj8, fc_grad and proj_grad
     as checkpointed_linear's weight8 and grad."""
+    fc = _asking(fc, fc_grad, x, proj)
+    proj = _asking(proj, proj_grad, x, fc)
     return _Mlp.apply(x, fc, proj, *(fc8 or _NOT_HELD), fc_grad, *(proj8 or _NOT_HELD), proj_grad)

@@ -214,3 +214,40 @@ def test_a_weight_gradient_added_in_place_is_noticed(recorder):
         y.backward()
     with torch.inference_mode():   # such tensors have no versions
         fl.checkpoint_weight_grad(new(M, N), codes, scale, out=new(N, K, dtype=F32))
+
+
+@pytest.fixture
+def eager(recorder, monkeypatch):
+    """The ops' own functions in place of the dispatcher, which has none for host tensors."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", True)
+    for name in ("linear", "linear_bwd", "mlp", "mlp_bwd"):
+        monkeypatch.setattr(fl, f"_{name}", getattr(fl, f"_run_{name}"))
+    return recorder
+
+
+def test_a_buffer_is_added_to_whatever_requires_a_gradient(eager):
+    """Frozen weights, or such as are no parameters, on inputs without a gradient: the first layer of a model that keeps its
+    gradients in buffers."""
+    x, w, f, p = new(M, K), new(N, K), new(F, K), new(N, F)
+    buffer = lambda t: new(*t.shape, dtype=F32)   # noqa: E731
+    for layer, name, modes in ((lambda: fl.checkpointed_linear(x, w, grad=buffer(w)), "linear", {13: 1}),
+                               (lambda: fl.checkpointed_mlp(x, f, p, fc_grad=buffer(f)), "mlp", {20: 1, 22: -1}),
+                               (lambda: fl.checkpointed_mlp(x, f, p, proj_grad=buffer(p)), "mlp", {20: -1, 22: 1}),
+                               (lambda: fl.checkpointed_mlp(x, f, p, fc_grad=buffer(f), proj_grad=buffer(p)), "mlp", {20: 1, 22: 1})):
+        y = layer()
+        assert y.requires_grad
+        y.backward(new(M, N))
+        call, = eager.named(f"nc_fp8_{name}_bwd")
+        assert {i: call[i] for i in modes} == modes and all(t.grad is None and not t.requires_grad for t in (x, w, f, p))
+        eager.calls.clear()
+        with torch.no_grad():
+            assert not layer().requires_grad
+    assert not fl.checkpointed_linear(x, w).requires_grad and not fl.checkpointed_mlp(x, f, p).requires_grad
+
+
+def test_a_buffer_of_a_layer_that_is_recorded_anyway(eager):
+    for x, w in ((new(M, K).requires_grad_(), new(N, K)), (new(M, K), new(N, K).requires_grad_())):
+        y = fl.checkpointed_linear(x, w, grad=new(N, K, dtype=F32))
+        y.backward(new(M, N))
+        assert w.grad is None and (x.grad is not None) == x.requires_grad
+    assert [args[13] for args in eager.named("nc_fp8_linear_bwd")] == [1, 1]

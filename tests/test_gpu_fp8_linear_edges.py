@@ -29,3 +29,18 @@ def test_scales_that_end_with_their_storage(device, rows, n, k):
         assert torch.equal(fl.fp8_matmul(codes, at_the_end(scale, wider), fl.Fp8Weight(w.codes, at_the_end(w.scale, wider))), want)
     dy = bf(gen, rows, 144).to(device)
     assert torch.equal(fl.checkpoint_weight_grad(dy, codes, at_the_end(scale, 48)), fl.checkpoint_weight_grad(dy, codes, scale))
+
+
+def test_buffers_of_layers_without_a_gradient(device):
+    """Neither the input nor the weights require one: what the buffers are given is what a parameter would get."""
+    gen = torch.Generator().manual_seed(20)
+    x, dy = bf(gen, 70, 256).to(device), bf(gen, 70, 144).to(device)
+    w, fc, proj = (torch.randn(*s, generator=gen).to(device) / 16 for s in ((144, 256), (640, 256), (144, 640)))
+    buffers = [torch.zeros_like(t) for t in (w, fc, proj)]
+    fl.checkpointed_linear(x, w, grad=buffers[0]).backward(dy)
+    fl.checkpointed_mlp(x, fc, proj, fc_grad=buffers[1], proj_grad=buffers[2]).backward(dy)
+    asked = [t.clone().requires_grad_() for t in (w, fc, proj)]
+    fl.checkpointed_linear(x, asked[0]).backward(dy)
+    fl.checkpointed_mlp(x, *asked[1:]).backward(dy)
+    # the same sums, added to zeros
+    assert all(torch.equal(b, t.grad) for b, t in zip(buffers, asked)) and all(t.grad is None for t in (w, fc, proj))
