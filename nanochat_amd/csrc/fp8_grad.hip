@@ -422,11 +422,12 @@ bool grad_fits(long long M, int N1, int N2) {
 /* Sizes first, then pointers, then their alignment. A slice's scales take no more bytes than its codes. */
 int grad_check(const GradOf &g, long long rows, const void *workspace) {
     if (!grad_fits(rows, g.n1, g.n2) || g.mode < 0 || g.mode > 2 || g.scale_stride < (g.n2 + F8_BLOCK - 1) / F8_BLOCK ||
-        g.scale_stride > g.n2)
+        g.scale_stride > g.n2 || g.scale_stride % 4)
         return NC_ERR_SHAPE;
     if (rows == 0) return NC_OK;
     if (!g.dy || !g.codes || !g.scale || !g.out || !workspace) return NC_ERR_NULL;
-    return ((uintptr_t)g.dy | (uintptr_t)g.codes | (uintptr_t)g.out | (uintptr_t)workspace) & 15 ? NC_ERR_SHAPE : NC_OK;
+    return ((uintptr_t)g.dy | (uintptr_t)g.codes | (uintptr_t)g.out | (uintptr_t)workspace) & 15 || (uintptr_t)g.scale & 3
+               ? NC_ERR_SHAPE : NC_OK;
 }
 
 int grad_launch(const GradOf *g, int results, const GrPlan &plan, long long rows, void *workspace, hipStream_t s) {
