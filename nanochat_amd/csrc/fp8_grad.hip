@@ -419,15 +419,10 @@ bool grad_fits(long long M, int N1, int N2) {
     return M >= 0 && M < (1LL << 31) && N1 > 0 && N2 > 0 && N1 % 8 == 0 && N2 % 16 == 0 && N1 <= 65536 && N2 <= 65536;
 }
 
-/* Sizes first, then pointers, then their alignment. A slice's scales take no more bytes than its codes. */
 int grad_check(const GradOf &g, long long rows, const void *workspace) {
-    if (!grad_fits(rows, g.n1, g.n2) || g.mode < 0 || g.mode > 2 || g.scale_stride < (g.n2 + F8_BLOCK - 1) / F8_BLOCK ||
-        g.scale_stride > g.n2 || g.scale_stride % 4)
-        return NC_ERR_SHAPE;
+    if (const int e = fp8_weight_grad_refuses(g, rows)) return e;
     if (rows == 0) return NC_OK;
-    if (!g.dy || !g.codes || !g.scale || !g.out || !workspace) return NC_ERR_NULL;
-    return ((uintptr_t)g.dy | (uintptr_t)g.codes | (uintptr_t)g.out | (uintptr_t)workspace) & 15 || (uintptr_t)g.scale & 3
-               ? NC_ERR_SHAPE : NC_OK;
+    return !workspace ? NC_ERR_NULL : (uintptr_t)workspace & 15 ? NC_ERR_SHAPE : NC_OK;
 }
 
 int grad_launch(const GradOf *g, int results, const GrPlan &plan, long long rows, void *workspace, hipStream_t s) {
@@ -465,6 +460,16 @@ GrPlan grad_shared(long long rows, const int (&n1)[2], const int (&n2)[2], int m
 }
 
 }  // namespace
+
+/* Sizes first, then pointers, then their alignment. A slice's scales take no more bytes than its codes. */
+int fp8_weight_grad_refuses(const GradOf &g, long long rows) {
+    if (!grad_fits(rows, g.n1, g.n2) || g.mode < 0 || g.mode > 2 || g.scale_stride < (g.n2 + F8_BLOCK - 1) / F8_BLOCK ||
+        g.scale_stride > g.n2 || g.scale_stride % 4)
+        return NC_ERR_SHAPE;
+    if (rows == 0) return NC_OK;
+    if (!g.dy || !g.codes || !g.scale || !g.out) return NC_ERR_NULL;
+    return ((uintptr_t)g.dy | (uintptr_t)g.codes | (uintptr_t)g.out) & 15 || (uintptr_t)g.scale & 3 ? NC_ERR_SHAPE : NC_OK;
+}
 
 long long fp8_weight_grads_bytes(long long rows, int n1, int n2, int mode, int m1, int m2, int other) {
     if (!grad_fits(rows, n1, n2) || !grad_fits(rows, m1, m2)) return -1;

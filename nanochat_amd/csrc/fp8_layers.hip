@@ -17,6 +17,14 @@ bool layer_sizes(long long rows, int n, int k) {
            rows <= (1LL << 31) / ((k + F8_BLOCK - 1) / F8_BLOCK) - 32;
 }
 bool misaligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) != 0; }
+/* What the calls below hand on is checked before the first of them launches: a call that is refused has written nothing. */
+bool bad_form(const void *codes, const void *scale, long long stride, int cols) {
+    return misaligned(codes, 16) || misaligned(scale, 4) || stride % 4 || stride < (cols + F8_BLOCK - 1) / F8_BLOCK ||
+           stride > 1 << 14;
+}
+bool bad_rows(const void *x, long long stride, long long rows, int cols) {
+    return misaligned(x, 2) || (rows > 1 && stride < cols) || stride > (1LL << 40);
+}
 long long up16(long long n) { return (n + 15) / 16 * 16; }
 long long grad_need(long long rows, int n1, int n2, int mode) {
     return mode == NONE ? 0 : nc_fp8_weight_grad_workspace_bytes(rows, n1, n2);
@@ -31,8 +39,11 @@ extern "C" int nc_fp8_linear_fwd(const void *x, long long row_stride, const void
                                  long long rows, int n, int k, void *codes, void *scale, long long scale_stride, void *out,
                                  void *stream) {
     if (!layer_sizes(rows, n, k)) return NC_ERR_SHAPE;
-    if (rows && (!w || !w_scale || !out)) return NC_ERR_NULL;
-    if (misaligned(w, 16) || misaligned(w_scale, 4) || misaligned(out, 16)) return NC_ERR_SHAPE;
+    if (rows == 0) return NC_OK;
+    if (!x || !w || !w_scale || !codes || !scale || !out) return NC_ERR_NULL;
+    if (bad_rows(x, row_stride, rows, k) || bad_form(w, w_scale, w_scale_stride, k) || bad_form(codes, scale, scale_stride, k) ||
+        misaligned(out, 16))
+        return NC_ERR_SHAPE;
     const int status = nc_fp8_quantize_rows(x, 0, row_stride, rows, k, codes, scale, scale_stride, stream);
     return status ? status : nc_fp8_matmul(codes, scale, scale_stride, w, w_scale, w_scale_stride, rows, n, k, out, stream);
 }
@@ -51,7 +62,11 @@ extern "C" int nc_fp8_linear_bwd(const void *dy, long long row_stride, const voi
     if (need < 0 || (mode != NONE && rows > 1 && row_stride != n)) return NC_ERR_SHAPE;
     if (rows == 0) return NC_OK;
     if (!dy || !workspace || (dx && (!codes_t || !scale_t)) || (mode != NONE && (!codes || !scale || !dw))) return NC_ERR_NULL;
+    if (bad_rows(dy, row_stride, rows, n) || (dx && (bad_form(codes_t, scale_t, scale_t_stride, n) || misaligned(dx, 16))))
+        return NC_ERR_SHAPE;
     if (misaligned(workspace, 16) || workspace_bytes < need) return NC_ERR_WORKSPACE;
+    if (mode != NONE)
+        if (const int e = fp8_weight_grad_refuses({dy, codes, scale, scale_stride, n, k, mode, dw}, rows)) return e;
     int status = NC_OK;
     char *rest = (char *)workspace;
     if (dx) {
@@ -72,9 +87,11 @@ extern "C" int nc_fp8_mlp_fwd(const void *x, long long row_stride, const void *f
                               int n, void *codes, void *scale, long long scale_stride, void *act, void *act_scale,
                               long long act_scale_stride, void *out, void *stream) {
     if (!layer_sizes(rows, hidden, c) || !layer_sizes(rows, n, hidden)) return NC_ERR_SHAPE;
-    if (rows && (!fc || !fc_scale || !proj || !proj_scale || !act || !act_scale || !out)) return NC_ERR_NULL;
-    if (misaligned(fc, 16) || misaligned(fc_scale, 4) || misaligned(proj, 16) || misaligned(proj_scale, 4) ||
-        misaligned(act, 16) || misaligned(act_scale, 4) || misaligned(out, 16))
+    if (rows == 0) return NC_OK;
+    if (!x || !fc || !fc_scale || !proj || !proj_scale || !codes || !scale || !act || !act_scale || !out) return NC_ERR_NULL;
+    if (bad_rows(x, row_stride, rows, c) || bad_form(fc, fc_scale, fc_scale_stride, c) ||
+        bad_form(proj, proj_scale, proj_scale_stride, hidden) || bad_form(codes, scale, scale_stride, c) ||
+        bad_form(act, act_scale, act_scale_stride, hidden) || misaligned(out, 16))
         return NC_ERR_SHAPE;
     int status = nc_fp8_quantize_rows(x, 0, row_stride, rows, c, codes, scale, scale_stride, stream);
     if (!status)
@@ -109,7 +126,17 @@ extern "C" int nc_fp8_mlp_bwd(const void *dy, long long row_stride, const void *
     if (!dy || !act || !act_scale || !workspace || (inner && (!proj_codes_t || !proj_scale_t)) ||
         (dx && (!fc_codes_t || !fc_scale_t)) || (fc_mode != NONE && (!codes || !scale || !dfc)) || (proj_mode != NONE && !dproj))
         return NC_ERR_NULL;
+    if (bad_rows(dy, row_stride, rows, n) ||
+        ((inner || proj_mode != NONE) && bad_form(act, act_scale, act_scale_stride, hidden)) ||
+        (inner && bad_form(proj_codes_t, proj_scale_t, proj_scale_t_stride, n)) ||
+        (dx && (bad_form(fc_codes_t, fc_scale_t, fc_scale_t_stride, hidden) || misaligned(dx, 16))))
+        return NC_ERR_SHAPE;
     if (misaligned(workspace, 16) || workspace_bytes < need) return NC_ERR_WORKSPACE;
+    GradOf g[2] = {{workspace, codes, scale, scale_stride, hidden, c, fc_mode, dfc},   /* its dy is dh, in the workspace: below */
+                   {dy, act, act_scale, act_scale_stride, n, hidden, proj_mode, dproj}};
+    for (const GradOf &of : g)
+        if (of.mode != NONE)
+            if (const int e = fp8_weight_grad_refuses(of, rows)) return e;
     int status = NC_OK;
     unsigned char *rest = (unsigned char *)workspace, *dh = nullptr;
     if (inner) {
@@ -126,11 +153,8 @@ extern "C" int nc_fp8_mlp_bwd(const void *dy, long long row_stride, const void *
                                    stream);
     }
     const long long left = need - (rest - (unsigned char *)workspace);
-    if (!status && fc_mode != NONE && proj_mode != NONE) {
-        const GradOf g[2] = {{dh, codes, scale, scale_stride, hidden, c, fc_mode, dfc},
-                             {dy, act, act_scale, act_scale_stride, n, hidden, proj_mode, dproj}};
-        return fp8_weight_grads(g, rows, rest, left, (hipStream_t)stream);
-    }
+    g[0].dy = dh;
+    if (!status && fc_mode != NONE && proj_mode != NONE) return fp8_weight_grads(g, rows, rest, left, (hipStream_t)stream);
     if (!status && fc_mode != NONE)
         status = nc_fp8_weight_grad(dh, codes, scale, scale_stride, rows, hidden, c, fc_mode, dfc, rest, left, stream);
     if (!status && proj_mode != NONE)

@@ -66,6 +66,7 @@ struct GradOf {
     void *out;
 };
 long long fp8_weight_grads_bytes(long long rows, int n1, int n2, int mode, int m1, int m2, int other);
+int fp8_weight_grad_refuses(const GradOf &g, long long rows);   /* the status of a refused one, but for its workspace */
 int fp8_weight_grads(const GradOf (&g)[2], long long rows, void *workspace, long long workspace_bytes, hipStream_t stream);
 
 /* The decode step's GEMM operands: out[n][r] = epilogue(sum_k x[n][k] w[r][k]), bf16 operands, fp32 sums,
