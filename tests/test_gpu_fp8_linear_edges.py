@@ -1,10 +1,12 @@
 """More of the 8-bit linear layers on the GPU: calls that the documentation allows at the edges of what tests/test_gpu_fp8_linear.py
 runs. Bounds as there."""
+import numpy as np
 import pytest
 import torch
 
 from nanochat_amd import fp8_linear as fl
-from tests.test_gpu_fp8_linear import bf, form, weight
+from oracle import fp8_block as fb
+from tests.test_gpu_fp8_linear import EPS, bf, close, codes_of, exps_of, form, held, product_relu2, product_relu2_bwd, same_form, weight
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +46,80 @@ def test_buffers_of_layers_without_a_gradient(device):
     fl.checkpointed_mlp(x, *asked[1:]).backward(dy)
     # the same sums, added to zeros
     assert all(torch.equal(b, t.grad) for b, t in zip(buffers, asked)) and all(t.grad is None for t in (w, fc, proj))
+
+
+# --- long walks, and workgroups that take several tiles (256 CUs; stages of 128 columns)
+
+# rows, outputs, columns: what the product's rule makes of them
+LONG = [(65, 1280, 1168),       # small tiles before a ReLU^2, 10 stages
+        (130, 8208, 1168),      # small tiles, 195
+        (600, 4112, 1168),      # half tiles, 165, 10 stages
+        (2500, 1680, 2000),     # half tiles, 16 stages
+        (9300, 2064, 1168),     # full tiles, 252, and half ones; a last column of 16
+        (6100, 5520, 640),      # 506 full tiles, two a workgroup, 5 stages; the last column of 144
+        (12000, 2832, 1152),    # 504, 9 stages; the last column of 16: two of a tile's four waves have nothing
+        (8400, 4112, 1664),     # 510, 13 stages; the same
+        (8190, 4352, 768),      # 510, 6 stages
+        (8190, 6144, 528),      # 768, three a workgroup, 5 stages, the last of 16 columns
+        (8190, 6144, 256),      # 768 of 2 stages
+        (8190, 6144, 128)]      # 768 of one
+
+
+def uneven(gen, device, rows, cols, of):
+    """Values whose blocks (of `of` rows and 128 columns) lie up to 2^6 apart, so that a wrong block's scale shows anywhere."""
+    x = torch.randn(rows, cols, generator=gen)
+    e = torch.randint(-3, 4, (-(-rows // of), -(-cols // 128)), generator=gen).float()
+    return x * torch.exp2(e).repeat_interleave(of, 0)[:rows].repeat_interleave(128, 1)[:, :cols]
+
+
+def sampled(rows):
+    """Rows of every tile, at its waves' borders and at places of their own."""
+    return [r for r in range(rows) if r % 64 in (0, 15, 16, 63) or r == rows - 1 or r % 61 == 7]
+
+
+def operands(device, rows, n, k):
+    gen = torch.Generator().manual_seed(rows + n + k)
+    codes, scale = fl.quantize_rows(uneven(gen, device, rows, k, 1).to(torch.bfloat16).to(device))
+    w = fl.quantize_weight((uneven(gen, device, n, k, 128) * k ** -0.5).to(device))
+    at = sampled(rows)
+    there = torch.tensor(at, device=device)
+    x = fb.values(codes_of(codes[there].contiguous()), exps_of(scale[there]), 1)
+    wv = fb.values(codes_of(w.codes), exps_of(w.scale), 128)
+    return gen, codes, scale, w, there, x @ wv.T, (2.0 ** -10 + k * EPS) * (np.abs(x) @ np.abs(wv).T)
+
+
+@pytest.mark.parametrize("rows,n,k", LONG)
+def test_long_product(device, rows, n, k):
+    _, codes, scale, w, there, want, off = operands(device, rows, n, k)
+    y = fl.fp8_matmul(codes, scale, w)
+    assert torch.equal(fl.fp8_matmul(codes, scale, w), y)
+    got = codes_of(y[there])
+    close(got, want, 2.0 ** -8 * np.abs(want) + off)
+    assert np.linalg.norm(got - want) <= 2.0 ** -8 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("rows,n,k", LONG)
+def test_long_product_relu2(device, rows, n, k):
+    _, codes, scale, w, there, h, off = operands(device, rows, n, k)
+    a8, a_s = product_relu2(codes, scale, w)
+    want = np.maximum(h, 0.0) ** 2
+    slack = 2 * np.maximum(h, 0.0) * off + off * off + 4 * EPS * want
+    s = held(a_s[there])
+    got = fb.values(codes_of(a8[there].contiguous()), exps_of(a_s[there]), 1)
+    close(got, want, slack + np.maximum(2.0 ** -4 * (want + slack), 2.0 ** -10 * np.repeat(s, 128, 1)[:, :n]))
+    pad = lambda t: np.pad(t, ((0, 0), (0, -n % 128))).reshape(len(h), -1, 128).max(-1)   # noqa: E731
+    most, worst = pad(want), pad(slack)
+    assert bool((most - worst <= 448 * s).all()) and bool(((most + worst > 224 * s) | (most == 0)).all())
+
+
+@pytest.mark.parametrize("rows,n,k", LONG)
+def test_long_product_relu2_backward(device, rows, n, k):
+    gen, codes, scale, w, there, h, off = operands(device, rows, n, k)
+    a8, a_s = fl.quantize_rows((uneven(gen, device, rows, n, 1).clamp(min=0) ** 2).to(device))
+    root = 2 * np.sqrt(fb.values(codes_of(a8[there].contiguous()), exps_of(a_s[there]), 1))
+    dh, q, q_s = product_relu2_bwd(codes, scale, w, a8, a_s)
+    want = h * root
+    got = codes_of(dh[there])
+    close(got, want, 2.0 ** -8 * np.abs(want) + off * root + 4 * EPS * np.abs(want))
+    some = there[::7]
+    assert same_form(q[some], q_s[some], codes_of(dh[some]), 1)
