@@ -123,3 +123,80 @@ def test_long_product_relu2_backward(device, rows, n, k):
     close(got, want, 2.0 ** -8 * np.abs(want) + off * root + 4 * EPS * np.abs(want))
     some = there[::7]
     assert same_form(q[some], q_s[some], codes_of(dh[some]), 1)
+
+
+# --- gradients against differences, where nothing is rounded
+
+def whole_numbers(gen, rows, cols, of):
+    """0, +-1, +-2 and +-3."""
+    return torch.randint(-3, 4, (rows, cols), generator=gen).float()
+
+
+def one_a_row(gen, rows, cols):
+    """One number of 1 and 2 in each row, of either sign, anywhere."""
+    t = torch.zeros(rows, cols)
+    t[torch.arange(rows), torch.randint(0, cols, (rows,), generator=gen)] = (
+        torch.randint(1, 3, (rows,), generator=gen) * (2 * torch.randint(0, 2, (rows,), generator=gen) - 1)).float()
+    return t
+
+
+def directions(gen, shape):
+    """Single entries, then one row, one column, and a few entries over all of it."""
+    rows, cols = shape
+    entries = [(int(torch.randint(0, rows, (1,), generator=gen)), int(torch.randint(0, cols, (1,), generator=gen)))
+               for _ in range(12)] + [(0, 0), (rows - 1, cols - 1)]
+    for i, j in entries:
+        v = torch.zeros(shape, dtype=torch.float64)
+        v[i, j] = 1.0
+        yield v
+    for at in (np.s_[rows // 2, :], np.s_[:, cols // 3]):
+        v = torch.zeros(shape, dtype=torch.float64)
+        v[at] = 1.0
+        yield v
+    yield (torch.rand(shape, generator=gen) < 0.02).double()
+
+
+STEP = 2.0 ** -20
+
+
+def compare(gen, loss, inputs, grads, kink):
+    """<gradient, v> against (L(+v) - L(-v)) / 2 in float64 for directions of few entries. L is a square of what relu lets through at
+    most, so the difference is the derivative but at relu's border, where it adds at most STEP / 2 kink for an entry of v, and for
+    float64's own rounding of L. Half and twice the gradient have to fail where there is one."""
+    told = 0
+    for i, g in enumerate(grads):
+        g = g.detach().double().cpu()
+        slack = 2.0 ** -8 if inputs[i].dtype == torch.bfloat16 else EPS
+        at = [t.double() for t in inputs]
+        for v in directions(gen, tuple(g.shape)):
+            plus, minus = (loss(*(t + s * STEP * v if j == i else t for j, t in enumerate(at))) for s in (1, -1))
+            want, size = (plus - minus) / (2 * STEP), float((g.abs() * v).sum())
+            off = size * slack + float(v.sum()) ** 2 * kink * STEP / 2 + 2.0 ** -50 * (abs(plus) + abs(minus) + 1) / STEP
+            got = float((g * v).sum())
+            assert abs(got - want) <= off, (i, got, want, off)
+            if abs(want) > 8 * off:
+                told += 1
+                assert abs(got / 2 - want) > off and abs(2 * got - want) > off
+    assert told >= 6 * len(grads)
+
+
+@pytest.mark.parametrize("m,c,f,n", [(500, 144, 384, 80), (700, 272, 1040, 160)])
+def test_gradients_of_whole_numbers_by_differences(device, m, c, f, n):
+    """Inputs whose 8-bit forms, sums, squares and gradients before the square are all exact: x and dy have one number a row, so a
+    sum before the square is one of 0, 1, 2, 3, 4 and 6, its square has four bits at most, as has dh = da 2 sqrt(a) (1, 3 or 9
+    times a power of two). What is left is dx's rounding to bf16."""
+    gen = torch.Generator().manual_seed(30)
+    x, dy = one_a_row(gen, m, c).to(torch.bfloat16), one_a_row(gen, m, n).to(torch.bfloat16)
+    fc, proj, w = whole_numbers(gen, f, c, 128), whole_numbers(gen, n, f, 128), whole_numbers(gen, n, c, 128)
+    asked = lambda *ts: [t.to(device).requires_grad_() for t in ts]   # noqa: E731
+    given = asked(x, fc, proj)
+    got = torch.autograd.grad(fl.checkpointed_mlp(*given), given, dy.to(device))
+
+    def mlp(x, fc, proj):
+        return float(((x @ fc.t()).clamp(min=0).square() @ proj.t() * dy.double()).sum())
+
+    # an entry's border: at most 3 rows (of fc) or numbers (of x) squared times a da of 6, for each row or output that it reaches
+    compare(gen, mlp, (x, fc, proj), got, 9 * 6 * max(m, f))
+    given = asked(x, w)
+    got = torch.autograd.grad(fl.checkpointed_linear(*given), given, dy.to(device))
+    compare(gen, lambda x, w: float(((x @ w.t()) * dy.double()).sum()), (x, w), got, 0)
