@@ -558,7 +558,15 @@ __device__ __forceinline__ void fg_results(const F8Gemm &g, const FgPlace &p, lo
                 for (int h = 0; h < 4; h++)
                     c[h] = *(const u32x2 *)(codes + fg_code_place(r16, 2 * h + (grp >> 1)) + 8 * (grp & 1));
             }
-            const float s = 4.0f * f8_scale(act_byte[u]);   /* 2 sqrt(a) = sqrt(4 a); a finite a's byte is at most 247 */
+            /* 2 sqrt(a) = sqrt(4 a). Where 4 a may leave fp32's normal range (which v_sqrt_f32 takes for 0, or is infinite) it is
+             * taken times 2^32 or 2^-32, and the sum times the inverse of the root of that. */
+            const bool low = act_byte[u] < 16u, high = act_byte[u] >= 240u;
+            const float s = 4.0f * (f8_scale(act_byte[u]) * (low ? 0x1p32f : high ? 0x1p-32f : 1.0f));
+            if (__any(low || high)) {
+                const float p = low ? 0x1p-16f : high ? 0x1p16f : 1.0f;
+#pragma unroll
+                for (int k = 0; k < 32; k++) v[k] = v[k] * p;
+            }
             float m = 0.0f;   /* the largest before its rounding, which keeps the order */
 #pragma unroll
             for (int h = 0; h < 4; h++)

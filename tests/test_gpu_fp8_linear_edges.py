@@ -125,6 +125,26 @@ def test_long_product_relu2_backward(device, rows, n, k):
     assert same_form(q[some], q_s[some], codes_of(dh[some]), 1)
 
 
+@pytest.mark.parametrize("rows,n,k", [(33, 272, 144), (600, 4112, 128), (3000, 4112, 128)])
+@pytest.mark.parametrize("least,most", [(1, 8), (8, 24), (120, 134), (232, 247)])
+def test_square_roots_at_the_ends_of_the_range(device, rows, n, k, least, most):
+    """Squared activations from fp32's smallest numbers, and below, to its largest: twice their roots lie far inside its range.
+    Small, half and full tiles."""
+    gen = torch.Generator().manual_seed(rows + least)
+    codes, scale, x = form(gen, device, rows, k)
+    w, wv = weight(gen, device, n, k)
+    blocks = -(-n // 128)
+    a8 = torch.randint(0, 0x78, (rows, n), generator=gen, dtype=torch.uint8).to(device).view(fl.CODES)   # 0 to 240
+    e = torch.randint(least, most + 1, (rows, -(-blocks // 4) * 4), generator=gen, dtype=torch.uint8)
+    e[torch.rand(e.shape, generator=gen) < 0.3] = 127   # beside ordinary ones
+    a_s = e.to(device).view(fl.SCALE)[:, :blocks]
+    root = 2 * np.sqrt(fb.values(codes_of(a8), exps_of(a_s), 1))
+    dh, q, q_s = product_relu2_bwd(codes, scale, w, a8, a_s)
+    want, off = (x @ wv.T) * root, (2.0 ** -10 + k * EPS) * (np.abs(x) @ np.abs(wv).T) * root
+    close(codes_of(dh), want, 2.0 ** -8 * np.abs(want) + off + 4 * EPS * np.abs(want))
+    assert same_form(q[:40], q_s[:40], codes_of(dh[:40]), 1)
+
+
 # --- gradients against differences, where nothing is rounded
 
 def whole_numbers(gen, rows, cols, of):
