@@ -31,8 +31,9 @@
  * 2^16, 2^3 is kept and 2^2 is not, of either sign; products of other eights keep theirs) and everything else in fp32: 1.5e-5
  * relative error for normal values, 3e-5 with a few channels far above the others, against the 2e-3 of a bf16 result. Before a
  * ReLU^2, whose result is rounded to 8 bits next, such an error lands on another code now and then: an MLP's result was 0.0029 off
- * float64's in place of 0.0017. The small tiles, which have the time, take those products exactly, from the values in bf16; the
- * others would take twice as long.
+ * float64's in place of 0.0017. The small tiles, which have the time, take those products exactly, from the values in bf16. So do the
+ * others where the caller asks for it, all in half tiles, in twice the time: 65,536 x 6,656 x 1,664 595 -> 1,231 us (1,180 TFLOP/s),
+ * 9,995 x 5,120 x 1,280 70 -> 124, 1,001 x 5,120 x 1,280 12 -> 20.
  */
 #include "nanochat_amd.h"
 #include "nc_fp8.h"
@@ -49,7 +50,7 @@ constexpr int FG_ROWB = F8_BLOCK;        /* bytes of a row of a stage: one block
 constexpr int FG_PAST = 0x7FFF0000;      /* a byte offset past every operand's range */
 constexpr int FG_NT = 2;                 /* a store past the caches */
 
-enum { FG_STORE, FG_RELU2, FG_RELU2_BWD };
+enum { FG_STORE, FG_RELU2, FG_RELU2_BWD, FG_RELU2_EXACT };
 
 struct F8Gemm {
     const unsigned char *a, *as;         /* [M][K] codes, [M] scale bytes at as_stride */
@@ -127,15 +128,20 @@ __device__ __forceinline__ void fg_compute(const unsigned char *buf, f32x4 (&acc
 #pragma unroll
     for (int u = 0; u < P::NU; u++) fb[u] = fg_operand(buf, a_at + u * 16 * FG_ROWB, (a_at ^ 16) + u * 16 * FG_ROWB);
     if constexpr (EXACT) {
-        static_assert(P::NU == 1, "one operand of a");
-        const float s = fg_scale<BYTE>(sa[0]), t_s = fg_scale<BYTE>(sw);
-        bf16x8 b[4];
-        fg_unroll<4>([&](auto q) { b[decltype(q)::value] = fg_values<decltype(q)::value>(fb[0], s); });
+        const float t_s = fg_scale<BYTE>(sw);
+        bf16x8 b[P::NU][4];
+        fg_unroll<P::NU>([&](auto u) {
+            constexpr int U = decltype(u)::value;
+            const float s = fg_scale<BYTE>(sa[U]);
+            fg_unroll<4>([&](auto q) { b[U][decltype(q)::value] = fg_values<decltype(q)::value>(fb[U], s); });
+        });
 #pragma unroll
         for (int t = 0; t < 8; t++) {
             const i32x8 fa = fg_operand(buf, w_at + fg_column(t, 0) * FG_ROWB, (w_at ^ 16) + fg_column(t, 0) * FG_ROWB);
             fg_unroll<4>([&](auto q) {
-                acc[t][0] = mfma16x16x32(fg_values<decltype(q)::value>(fa, t_s), b[decltype(q)::value], acc[t][0]);
+                const bf16x8 v = fg_values<decltype(q)::value>(fa, t_s);
+#pragma unroll
+                for (int u = 0; u < P::NU; u++) acc[t][u] = mfma16x16x32(v, b[u][decltype(q)::value], acc[t][u]);
             });
         }
     } else {
@@ -656,9 +662,9 @@ template <class P, int EPI> __device__ __forceinline__ void fg_run(const F8Gemm 
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int u = 0; u < P::NU; u++) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    fg_walk_ring<P, P::NU == 1 && EPI == FG_RELU2>(g, p, m0, t.x * P::TN, lds, acc);
+    fg_walk_ring<P, EPI == FG_RELU2_EXACT || (P::NU == 1 && EPI == FG_RELU2)>(g, p, m0, t.x * P::TN, lds, acc);
     const uint32_t none[2] = {0u, 0u};
-    fg_results<P, EPI>(g, p, m0, t.x * P::TN, acc, lds, lds, none);
+    fg_results<P, EPI == FG_RELU2_EXACT ? FG_RELU2 : EPI>(g, p, m0, t.x * P::TN, acc, lds, lds, none);
 }
 
 /* The kernel's arguments with the codes' places read anew: kept over the walk they are four scalar registers too many. */
@@ -725,8 +731,10 @@ template <class P>
 int fg_launch(const F8Gemm &g, int epi, hipStream_t stream) {
     const long long tiles = (g.M + P::TM - 1) / P::TM * ((g.N + P::TN - 1) / P::TN);
     if (tiles >= (1LL << 31)) return NC_ERR_SHAPE;
-    const auto kernel = epi == FG_STORE ? fp8_gemm_kernel<P, FG_STORE>
-                        : epi == FG_RELU2 ? fp8_gemm_kernel<P, FG_RELU2> : fp8_gemm_kernel<P, FG_RELU2_BWD>;
+    auto kernel = epi == FG_STORE ? fp8_gemm_kernel<P, FG_STORE>
+                  : epi == FG_RELU2 ? fp8_gemm_kernel<P, FG_RELU2> : fp8_gemm_kernel<P, FG_RELU2_BWD>;
+    if constexpr (P::NU == 2)
+        if (epi == FG_RELU2_EXACT) kernel = fp8_gemm_kernel<P, FG_RELU2_EXACT>;
     const long long cus = device_cus(), grid = P::FULL && epi != FG_RELU2_BWD && tiles > cus ? cus : tiles;
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(P::WAVES * WAVE), 0, stream, g, (int)tiles);
     return (int)hipGetLastError();
@@ -739,6 +747,7 @@ bool bad_scales(const void *p, long long stride, int cols) {
 
 /* Sizes first, then pointers, then their alignment. */
 int fg_check(const F8Gemm &g, int epi) {
+    if (epi == FG_RELU2_EXACT) epi = FG_RELU2;
     if (g.M < 0 || g.M > (1LL << 31) || g.N <= 0 || g.K <= 0 || g.N % 16 || g.K % 16 || g.N > (1 << 20) || g.K > (1 << 20))
         return NC_ERR_SHAPE;
     if (g.M == 0) return NC_OK;
@@ -781,7 +790,8 @@ int fg_gemm(const F8Gemm &g, int epi, void *stream) {
     const long long small = (g.M + 63) / 64 * half_nx;
     if (epi == FG_STORE && fp8_some_takes(g.M, g.N, g.K, cus))
         return fp8_some(g.a, g.as, g.as_stride, g.w, g.ws, g.ws_stride, (int)g.M, g.N, g.K, g.out, s);
-    if (small <= cus) return fg_launch<FgSmall>(g, epi, s);
+    if (small <= cus) return fg_launch<FgSmall>(g, epi == FG_RELU2_EXACT ? FG_RELU2 : epi, s);
+    if (epi == FG_RELU2_EXACT) return fg_launch<FgHalf>(g, epi, s);
     const long long full_time = 8 * ((full + cus - 1) / cus), half_time = fg_half_time((g.M + 127) / 128 * half_nx, cus);
     const long long rounds = full / cus, top = rounds * cus / nx * 256;   /* rows of whole rounds: less than M, or all are whole */
     if (top > 0 && top < g.M) {
@@ -814,6 +824,15 @@ extern "C" int nc_fp8_matmul_relu2(const void *a, const void *a_scale, long long
                       (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, nullptr,
                       (unsigned char *)codes, (unsigned char *)scale, nullptr, nullptr, scale_stride, 0};
     return fg_gemm(g, FG_RELU2, stream);
+}
+
+extern "C" int nc_fp8_matmul_relu2_exact(const void *a, const void *a_scale, long long a_scale_stride, const void *w,
+                                         const void *w_scale, int w_scale_stride, long long rows, int n, int k, void *codes,
+                                         void *scale, long long scale_stride, void *stream) {
+    const F8Gemm g = {(const unsigned char *)a, (const unsigned char *)a_scale, (const unsigned char *)w,
+                      (const unsigned char *)w_scale, a_scale_stride, w_scale_stride, rows, n, k, nullptr,
+                      (unsigned char *)codes, (unsigned char *)scale, nullptr, nullptr, scale_stride, 0};
+    return fg_gemm(g, FG_RELU2_EXACT, stream);
 }
 
 extern "C" int nc_fp8_matmul_relu2_bwd(const void *a, const void *a_scale, long long a_scale_stride, const void *w,

@@ -20,6 +20,7 @@ from tests.test_prefill_gemm_isa import blocks
 # stages in LDS, 16-byte DMA of a stage and wave
 KERNELS = {("fp8_gemm.hip", f"15fp8_gemm_kernelINS0_6FgTileI{tile}EELi{epi}EEEv"): sizes
            for tile, sizes in (("Li2ELi1ELi4ELi2E", (2, 8)), ("Li1ELi1ELi4ELi3E", (3, 6))) for epi in range(3)}
+KERNELS |= {("fp8_gemm.hip", "15fp8_gemm_kernelINS0_6FgTileILi2ELi1ELi4ELi2EEELi3EEEv"): (2, 8)}   # exact products before a ReLU^2
 KERNELS |= {("fp8_skinny.hip", "15fp8_some_kernelILi1ELi8EEEv"): (3, 4), ("fp8_skinny.hip", "15fp8_some_kernelILi2ELi4EEEv"): (4, 2)}
 LANDED = 1 << 20
 VMEM = ("buffer_", "global_", "flat_", "scratch_")

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from nanochat_amd import fp8_linear as fl
+from nanochat_amd import fp8_linear as fl, native
+from nanochat_amd.native import hip_library, stream
 from oracle import fp8_block as fb
 from tests.test_gpu_fp8_linear import EPS, bf, close, codes_of, exps_of, form, held, product_relu2, product_relu2_bwd, same_form, weight
 
@@ -143,6 +144,100 @@ def test_square_roots_at_the_ends_of_the_range(device, rows, n, k, least, most):
     want, off = (x @ wv.T) * root, (2.0 ** -10 + k * EPS) * (np.abs(x) @ np.abs(wv).T) * root
     close(codes_of(dh), want, 2.0 ** -8 * np.abs(want) + off + 4 * EPS * np.abs(want))
     assert same_form(q[:40], q_s[:40], codes_of(dh[:40]), 1)
+
+
+# --- how exact the squares are
+
+def relu2_exact(codes, scale, w):
+    rows, k = codes.shape
+    n = w.codes.size(0)
+    out, out_scale = torch.empty(rows, n, dtype=fl.CODES, device=codes.device), fl._new_scale(codes, rows, n)
+    native.check(hip_library().nc_fp8_matmul_relu2_exact(codes.data_ptr(), scale.data_ptr(), scale.stride(0), w.codes.data_ptr(),
+                                                         w.scale.data_ptr(), w.scale.stride(0), rows, n, k, out.data_ptr(),
+                                                         out_scale.data_ptr(), out_scale.stride(0), stream()))
+    return out, out_scale
+
+
+def dropped(x, w):
+    """What the matrix cores may drop of x w^T: of each eight adjacent products seven times 2^-13 of the largest."""
+    rows, k = x.shape
+    x, w = np.abs(x).reshape(rows, 1, k // 8, 8), np.abs(w).reshape(1, -1, k // 8, 8)
+    return 7 * 2.0 ** -13 * np.stack([(x[i] * w[0]).max(-1).sum(-1) for i in range(rows)])
+
+
+def between(got, scale, h, off):
+    """Whether 8-bit squares are those of sums within off of h, each rounded once: code for code, and the scales."""
+    n = h.shape[1]
+    lo, hi = np.maximum(h - off, 0.0) ** 2 * (1 - EPS), np.maximum(h + off, 0.0) ** 2 * (1 + EPS)
+    top = lambda t: np.pad(t, ((0, 0), (0, -n % 128))).reshape(len(h), -1, 128).max(-1)   # noqa: E731
+    least, most = fb.exponents(top(lo)), fb.exponents(top(hi))
+    assert bool(((exps_of(scale) >= least) & (exps_of(scale) <= most)).all())
+    s = np.repeat(held(scale), 128, 1)[:, :n]
+    codes = codes_of(got.contiguous())
+    low, high = fb.e4m3_round(np.minimum(lo / s, 448)), fb.e4m3_round(np.minimum(hi / s, 448))
+    assert bool(((codes >= low) & (codes <= high)).all())
+
+
+def others(codes, scale, h):
+    """The share of 8-bit squares that are not float64's."""
+    return (fb.values(codes_of(codes.contiguous()), exps_of(scale), 1) != fb.through(np.maximum(h, 0.0) ** 2, 1)).mean()
+
+
+# few rows, small, half and full tiles, several tiles a workgroup
+SQUARES = [(40, 272, 400), (65, 1280, 1168), (600, 4112, 1168), (3000, 4112, 128), (9300, 2064, 1168), (8190, 4352, 768)]
+
+
+@pytest.mark.parametrize("rows,n,k", SQUARES)
+def test_squares_of_exact_products(device, rows, n, k):
+    """fp32 sums of exact products: a code may be another than float64's where the square lies that near to the border of two.
+    How many do: a square is off by twice its sum's relative error d, codes lie 2^-4 to 2^-3 of a value apart, 0.09 in the mean: a
+    share of 2 d / 0.09. k / 8 roundings of 2^-24 / sqrt(3), all of a result's own size, make d 4e-7 at k = 1,168: 1e-5; a tenfold of it
+    is allowed, where the products by eights with their d of 1e-5 to 3e-5 give 2e-4 to 7e-4."""
+    _, codes, scale, w, there, h, _ = operands(device, rows, n, k)
+    x, wv = fb.values(codes_of(codes[there].contiguous()), exps_of(scale[there]), 1), fb.values(codes_of(w.codes), exps_of(w.scale), 128)
+    a8, a_s = relu2_exact(codes, scale, w)
+    between(a8[there], a_s[there], h, k * EPS * (np.abs(x) @ np.abs(wv).T))
+    assert others(a8[there], a_s[there], h) <= 1e-4
+    again = relu2_exact(codes, scale, w)
+    assert torch.equal(again[0].view(torch.uint8), a8.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows,n,k", SQUARES)
+def test_squares_of_products_by_eights(device, rows, n, k):
+    """The larger tiles' products drop bits, by eights of columns: where, and no more than that."""
+    _, codes, scale, w, there, h, _ = operands(device, rows, n, k)
+    some = np.arange(0, len(h), max(1, len(h) // 24))
+    there, h = there[torch.from_numpy(some).to(device)], h[some]
+    x, wv = fb.values(codes_of(codes[there].contiguous()), exps_of(scale[there]), 1), fb.values(codes_of(w.codes), exps_of(w.scale), 128)
+    a8, a_s = product_relu2(codes, scale, w)
+    between(a8[there], a_s[there], h, dropped(x, wv) + k * EPS * (np.abs(x) @ np.abs(wv).T))
+    assert others(a8[there], a_s[there], h) <= 1e-3
+
+
+@pytest.mark.parametrize("rows", [1, 40, 700, 9000])
+def test_exact_mlp(device, rows):
+    """An MLP's result is off by its own rounding alone, in any batch; in training, too, and its gradients are of those squares."""
+    gen = torch.Generator().manual_seed(rows)
+    x = bf(gen, rows, 400).to(device)
+    fc_w, proj_w = (torch.randn(*s, generator=gen).to(device) * s[1] ** -0.5 for s in ((2064, 400), (144, 2064)))
+    fc, proj = fl.quantize_weight(fc_w, True), fl.quantize_weight(proj_w, True)
+    fcv, pv = (fb.values(codes_of(t.codes), exps_of(t.scale), 128) for t in (fc, proj))
+    at = torch.arange(0, rows, max(1, rows // 200))
+    want = fb.through(np.maximum(fb.through(x[at].double().cpu().numpy(), 1) @ fcv.T, 0.0) ** 2, 1) @ pv.T
+    z = fl.fp8_mlp(x, fc, proj, exact=True)
+    assert np.linalg.norm(codes_of(z[at]) - want) <= 2.0 ** -8 * np.linalg.norm(want)
+    given = [t.clone().requires_grad_() for t in (x, fc_w, proj_w)]
+    y = fl.checkpointed_mlp(*given, exact=True)
+    codes, scale = fl.quantize_rows(x)
+    act = relu2_exact(codes, scale, fc)
+    assert torch.equal(y, fl.fp8_matmul(*act, proj)) and (rows <= 16 or torch.equal(y, z))
+    dy = bf(gen, rows, 144).to(device)
+    dx, dfc, dproj = torch.autograd.grad(y, given, dy)
+    dh, q, q_s = product_relu2_bwd(*fl.quantize_rows(dy), fl.Fp8Weight(proj.codes_t, proj.scale_t), *act)
+    assert torch.equal(dx, fl.fp8_matmul(q, q_s, fl.Fp8Weight(fc.codes_t, fc.scale_t)))
+    for got, left, right, depth in ((dfc, dh, (codes, scale), rows), (dproj, dy, act, rows)):
+        a, b = left.double().cpu().numpy(), fb.values(codes_of(right[0]), exps_of(right[1]), 1)
+        close(codes_of(got), a.T @ b, (depth + 300) * EPS * (np.abs(a).T @ np.abs(b)))
 
 
 # --- gradients against differences, where nothing is rounded
