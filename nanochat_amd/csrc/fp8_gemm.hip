@@ -42,10 +42,6 @@
 namespace nc {
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
 constexpr int FG_ROWB = F8_BLOCK;        /* bytes of a row of a stage: one block */
 constexpr int FG_PAST = 0x7FFF0000;      /* a byte offset past every operand's range */
 constexpr int FG_NT = 2;                 /* a store past the caches */
@@ -75,14 +71,8 @@ typedef FgTile<8, 2, 2, 2> FgFull;   /* 256 x 256, 4 waves of 128 x 128, two sta
 typedef FgTile<2, 1, 4, 2> FgHalf;   /* 128 x 128, 4 waves */
 typedef FgTile<1, 1, 4, 3> FgSmall;  /* 64 x 128, 4 waves */
 
-/* A 16-byte LDS read serves lanes 0-3, 12-15, 20-23 and 24-27 together, then 4-11, 16-19 and 28-31, and so the upper half. Two
- * rows lie side by side over the 64 banks, so 8 rows of one parity, four of one 16-byte piece b and four of b ^ 2, need 8
- * places. Activation rows i: i / 2 in {0, 1, 6, 7} gives places 0 to 3 (closed under ^ 2), the others 4 to 7. A weight row that
- * stands for i = 4 q + c has the same by q (0, 3 or 1, 2) and c / 2, whichever operand t it belongs to. */
-__device__ __forceinline__ int fg_swizzle_a(int row) {
-    const int k = (row >> 1) & 7;
-    return (k & 3) | (((k + 2) & 4));
-}
+/* Activation rows lie in LDS by f8_swizzle. A weight row that stands for row i = 4 q + c of an operand has the same by q (0, 3 or 1, 2)
+ * and c / 2, whichever operand t it belongs to. */
 /* The column (0 .. 127 of a wave's block) of row 4 q of operand t, rows on being columns on. */
 __host__ __device__ constexpr int fg_column(int t, int q) { return 32 * (t / 2) + 8 * q + 4 * (t % 2); }
 __device__ __forceinline__ int fg_swizzle_w(int row) {
@@ -113,13 +103,7 @@ __device__ __forceinline__ i32x8 fg_operand(const unsigned char *buf, int lo, in
  * place of one (codes 8 Q .. + 7 of each lane's 32 in instruction Q). */
 template <int BYTE> __device__ __forceinline__ float fg_scale(uint32_t s) { return f8_scale((s >> (8 * BYTE)) & 0xFFu); }
 template <int Q> __device__ __forceinline__ bf16x8 fg_values(const i32x8 &c, float s) {
-    u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[2 * Q + i], s, false));
-        o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[2 * Q + i], s, true));
-    }
-    return __builtin_bit_cast(bf16x8, o);
+    return f8_values((uint32_t)c[2 * Q], (uint32_t)c[2 * Q + 1], s);
 }
 template <class P, int BYTE, bool EXACT>
 __device__ __forceinline__ void fg_compute(const unsigned char *buf, f32x4 (&acc)[8][P::NU], const uint32_t (&sa)[P::NU],
@@ -196,7 +180,7 @@ __device__ __forceinline__ void fg_walk_ring(const F8Gemm &g, const FgPlace &p, 
     unsigned char *const scales = lds + P::RING * P::STAGE + p.wave * 2 * FG_OWN;
     const uint32_t scale_to = f8_lds(scales);
     const int row = 8 * p.wave + (p.lane >> 3), first = row * K;   /* rows 32 on have the same pieces */
-    const int ca = ((p.lane & 7) ^ fg_swizzle_a(row)) << 4, cw = ((p.lane & 7) ^ fg_swizzle_w(row)) << 4;
+    const int ca = ((p.lane & 7) ^ f8_swizzle(row)) << 4, cw = ((p.lane & 7) ^ fg_swizzle_w(row)) << 4;
     const int scale_at = p.lane < 16 * P::NU ? (16 * P::NU * p.wm + p.lane) * (int)g.as_stride : FG_PAST;
     const auto fetch = [&](int j, int slot) {   /* a stage past the last: zeros, without an access */
         const int k = j * FG_ROWB;
@@ -213,7 +197,7 @@ __device__ __forceinline__ void fg_walk_ring(const F8Gemm &g, const FgPlace &p, 
     };
 #pragma unroll
     for (int j = 0; j < P::RING - 1; j++) fetch(j, j);
-    const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
+    const int a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ f8_swizzle(p.row0)) << 4);
     const int w_row = fg_column(0, p.i >> 2) + (p.i & 3);
     const int w_at = (P::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
     uint32_t sa[P::NU], sw = 0;
@@ -281,7 +265,7 @@ struct FgDma {
         K = g.K;
         const int row = 8 * p.wave + (p.lane >> 3), pos = p.lane & 7;
         first = row * K;
-        ca = (pos ^ fg_swizzle_a(row)) << 4;
+        ca = (pos ^ f8_swizzle(row)) << 4;
         cw = (pos ^ fg_swizzle_w(row)) << 4;   /* rows 32 on have the same */
     }
     /* Stage j's offsets, and its scales' DMA where it is the first of four. Past K they lie past the range, also with 224 K added. */
@@ -416,7 +400,7 @@ __device__ __forceinline__ void fg_walk_full(const F8Gemm &g, const FgPlace &p, 
     k.own = lds + 2 * FgFull::STAGE + p.wave * 2 * FG_SCALES;
     k.i = p.i;
     k.flip = dma.flip;
-    k.a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_a(p.row0)) << 4);
+    k.a_at = p.row0 * FG_ROWB + (((2 * p.grp) ^ f8_swizzle(p.row0)) << 4);
     const int w_row = F8_BLOCK * p.wn + fg_column(0, p.i >> 2) + (p.i & 3);
     k.w_at = (FgFull::TM + w_row) * FG_ROWB + (((2 * p.grp) ^ fg_swizzle_w(w_row)) << 4);
     if (newer) fg_wait<16 + NEWER>();
@@ -740,11 +724,6 @@ int fg_launch(const F8Gemm &g, int epi, hipStream_t stream) {
     return (int)hipGetLastError();
 }
 
-bool misaligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) != 0; }
-bool bad_scales(const void *p, long long stride, int cols) {
-    return misaligned(p, 4) || stride % 4 || stride < (cols + F8_BLOCK - 1) / F8_BLOCK || stride > (1 << 14);
-}
-
 /* Sizes first, then pointers, then their alignment. */
 int fg_check(const F8Gemm &g, int epi) {
     if (epi == FG_RELU2_EXACT) epi = FG_RELU2;
@@ -754,10 +733,10 @@ int fg_check(const F8Gemm &g, int epi) {
     if (!g.a || !g.as || !g.w || !g.ws || (epi != FG_RELU2 && !g.out) || (epi != FG_STORE && (!g.q || !g.qs)) ||
         (epi == FG_RELU2_BWD && (!g.act || !g.acts)))
         return NC_ERR_NULL;
-    if (misaligned(g.a, 16) || misaligned(g.w, 16) || misaligned(g.out, 16) || misaligned(g.q, 16) || misaligned(g.act, 16) ||
-        bad_scales(g.as, g.as_stride, g.K) || bad_scales(g.ws, g.ws_stride, g.K) ||
-        (epi != FG_STORE && bad_scales(g.qs, g.qs_stride, g.N)) ||
-        (epi == FG_RELU2_BWD && bad_scales(g.acts, g.act_stride, g.N)))
+    if (f8_misaligned(g.a, 16) || f8_misaligned(g.w, 16) || f8_misaligned(g.out, 16) || f8_misaligned(g.q, 16) || f8_misaligned(g.act, 16) ||
+        f8_bad_scales(g.as, g.as_stride, g.K) || f8_bad_scales(g.ws, g.ws_stride, g.K) ||
+        (epi != FG_STORE && f8_bad_scales(g.qs, g.qs_stride, g.N)) ||
+        (epi == FG_RELU2_BWD && f8_bad_scales(g.acts, g.act_stride, g.N)))
         return NC_ERR_SHAPE;
     return NC_OK;
 }

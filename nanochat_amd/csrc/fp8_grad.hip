@@ -27,7 +27,6 @@
 namespace nc {
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 typedef __attribute__((address_space(3))) void LdsPtr;
 typedef short v4i16 __attribute__((ext_vector_type(4)));
@@ -64,7 +63,7 @@ constexpr int GR_X = 4 * GR_OPB, GR_XC = GR_X + 2 * GR_OPB, GR_XS = GR_XC + 4 * 
  * piece (l % 32) / 2, half l % 2. x's codes: rows 4 q .. + 3, lane l row 4 q + l / 16, columns 16 (l % 16) .. + 15, q = wave + 4 s.
  * Scales: every wave asks for all 64 tokens' dwords of two stages, lane l token l, so that each waits for its own. */
 struct GrDma {
-    f8_u32x4 ra, rx, rs;
+    u32x4 ra, rx, rs;
     uint32_t lds;                 /* the workgroup's LDS */
     uint32_t a, x, s;             /* this lane's offsets of instruction 0 in stage 0 (GR_PAST: a column past the result's) */
     uint32_t s_row;               /* bytes of a token's scales */

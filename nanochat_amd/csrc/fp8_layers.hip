@@ -16,14 +16,12 @@ bool layer_sizes(long long rows, int n, int k) {
     return rows >= 0 && n > 0 && k > 0 && n % 16 == 0 && k % 16 == 0 && n <= 1 << 20 && k <= 1 << 20 &&
            rows <= (1LL << 31) / ((k + F8_BLOCK - 1) / F8_BLOCK) - 32;
 }
-bool misaligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) != 0; }
 /* What the calls below hand on is checked before the first of them launches: a call that is refused has written nothing. */
 bool bad_form(const void *codes, const void *scale, long long stride, int cols) {
-    return misaligned(codes, 16) || misaligned(scale, 4) || stride % 4 || stride < (cols + F8_BLOCK - 1) / F8_BLOCK ||
-           stride > 1 << 14;
+    return f8_misaligned(codes, 16) || f8_bad_scales(scale, stride, cols);
 }
 bool bad_rows(const void *x, long long stride, long long rows, int cols) {
-    return misaligned(x, 2) || (rows > 1 && stride < cols) || stride > (1LL << 40);
+    return f8_misaligned(x, 2) || (rows > 1 && stride < cols) || stride > (1LL << 40);
 }
 long long up16(long long n) { return (n + 15) / 16 * 16; }
 long long grad_need(long long rows, int n1, int n2, int mode) {
@@ -42,7 +40,7 @@ extern "C" int nc_fp8_linear_fwd(const void *x, long long row_stride, const void
     if (rows == 0) return NC_OK;
     if (!x || !w || !w_scale || !codes || !scale || !out) return NC_ERR_NULL;
     if (bad_rows(x, row_stride, rows, k) || bad_form(w, w_scale, w_scale_stride, k) || bad_form(codes, scale, scale_stride, k) ||
-        misaligned(out, 16))
+        f8_misaligned(out, 16))
         return NC_ERR_SHAPE;
     const int status = nc_fp8_quantize_rows(x, 0, row_stride, rows, k, codes, scale, scale_stride, stream);
     return status ? status : nc_fp8_matmul(codes, scale, scale_stride, w, w_scale, w_scale_stride, rows, n, k, out, stream);
@@ -62,9 +60,9 @@ extern "C" int nc_fp8_linear_bwd(const void *dy, long long row_stride, const voi
     if (need < 0 || (mode != NONE && rows > 1 && row_stride != n)) return NC_ERR_SHAPE;
     if (rows == 0) return NC_OK;
     if (!dy || !workspace || (dx && (!codes_t || !scale_t)) || (mode != NONE && (!codes || !scale || !dw))) return NC_ERR_NULL;
-    if (bad_rows(dy, row_stride, rows, n) || (dx && (bad_form(codes_t, scale_t, scale_t_stride, n) || misaligned(dx, 16))))
+    if (bad_rows(dy, row_stride, rows, n) || (dx && (bad_form(codes_t, scale_t, scale_t_stride, n) || f8_misaligned(dx, 16))))
         return NC_ERR_SHAPE;
-    if (misaligned(workspace, 16) || workspace_bytes < need) return NC_ERR_WORKSPACE;
+    if (f8_misaligned(workspace, 16) || workspace_bytes < need) return NC_ERR_WORKSPACE;
     if (mode != NONE)
         if (const int e = fp8_weight_grad_refuses({dy, codes, scale, scale_stride, n, k, mode, dw}, rows)) return e;
     int status = NC_OK;
@@ -91,7 +89,7 @@ static int mlp_fwd(bool exact, const void *x, long long row_stride, const void *
     if (!x || !fc || !fc_scale || !proj || !proj_scale || !codes || !scale || !act || !act_scale || !out) return NC_ERR_NULL;
     if (bad_rows(x, row_stride, rows, c) || bad_form(fc, fc_scale, fc_scale_stride, c) ||
         bad_form(proj, proj_scale, proj_scale_stride, hidden) || bad_form(codes, scale, scale_stride, c) ||
-        bad_form(act, act_scale, act_scale_stride, hidden) || misaligned(out, 16))
+        bad_form(act, act_scale, act_scale_stride, hidden) || f8_misaligned(out, 16))
         return NC_ERR_SHAPE;
     int status = nc_fp8_quantize_rows(x, 0, row_stride, rows, c, codes, scale, scale_stride, stream);
     if (!status)
@@ -145,9 +143,9 @@ extern "C" int nc_fp8_mlp_bwd(const void *dy, long long row_stride, const void *
     if (bad_rows(dy, row_stride, rows, n) ||
         ((inner || proj_mode != NONE) && bad_form(act, act_scale, act_scale_stride, hidden)) ||
         (inner && bad_form(proj_codes_t, proj_scale_t, proj_scale_t_stride, n)) ||
-        (dx && (bad_form(fc_codes_t, fc_scale_t, fc_scale_t_stride, hidden) || misaligned(dx, 16))))
+        (dx && (bad_form(fc_codes_t, fc_scale_t, fc_scale_t_stride, hidden) || f8_misaligned(dx, 16))))
         return NC_ERR_SHAPE;
-    if (misaligned(workspace, 16) || workspace_bytes < need) return NC_ERR_WORKSPACE;
+    if (f8_misaligned(workspace, 16) || workspace_bytes < need) return NC_ERR_WORKSPACE;
     GradOf g[2] = {{workspace, codes, scale, scale_stride, hidden, c, fc_mode, dfc},   /* its dy is dh, in the workspace: below */
                    {dy, act, act_scale, act_scale_stride, n, hidden, proj_mode, dproj}};
     for (const GradOf &of : g)

@@ -15,8 +15,6 @@
 namespace nc {
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 /* 16 adjacent values of a row as they come: 8 dwords of bf16 pairs, or 16 of fp32. ALIGNED: by 16-byte loads. */
 template <bool F32, bool ALIGNED> struct Sixteen {
     uint32_t w[F32 ? 16 : 8];
@@ -157,8 +155,6 @@ __global__ void __launch_bounds__(256) fp8_weight_kernel(Weight p) {
     }
 }
 
-bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
-
 }  // namespace
 }  // namespace nc
 
@@ -173,11 +169,11 @@ extern "C" int nc_fp8_quantize_rows(const void *x, int is_f32, long long row_str
     if (rows == 0) return NC_OK;
     if (!x || !codes || !scale) return NC_ERR_NULL;
     const int size = is_f32 ? 4 : 2;
-    if (!aligned16(codes) || ((uintptr_t)scale & 3) || ((uintptr_t)x & (size - 1))) return NC_ERR_SHAPE;
+    if (f8_misaligned(codes, 16) || f8_misaligned(scale, 4) || f8_misaligned(x, size)) return NC_ERR_SHAPE;
     const Rows p = {(const unsigned char *)x, row_stride * size, cols, blocks, rows * blocks, (unsigned char *)codes,
                     (unsigned char *)scale, scale_stride};
     const dim3 grid((unsigned)((p.items + 31) / 32)), block(256);
-    const bool fast = aligned16(x) && p.row_bytes % 16 == 0;
+    const bool fast = !f8_misaligned(x, 16) && p.row_bytes % 16 == 0;
     const auto kernel = is_f32 ? fast ? fp8_rows_kernel<true, true> : fp8_rows_kernel<true, false>
                                : fast ? fp8_rows_kernel<false, true> : fp8_rows_kernel<false, false>;
     hipLaunchKernelGGL(kernel, grid, block, 0, (hipStream_t)stream, p);
@@ -193,13 +189,13 @@ extern "C" int nc_fp8_quantize_weight(const void *w, int is_f32, long long row_s
         return NC_ERR_SHAPE;
     if (!w || !codes || !scale || (codes_t && !scale_t)) return NC_ERR_NULL;
     const int size = is_f32 ? 4 : 2;
-    if (!aligned16(codes) || !aligned16(codes_t) || ((uintptr_t)scale & 3) || ((uintptr_t)scale_t & 3) ||
-        ((uintptr_t)w & (size - 1)))
+    if (f8_misaligned(codes, 16) || f8_misaligned(codes_t, 16) || f8_misaligned(scale, 4) || f8_misaligned(scale_t, 4) ||
+        f8_misaligned(w, size))
         return NC_ERR_SHAPE;
     const Weight p = {(const unsigned char *)w, row_stride * size, n, k, (unsigned char *)codes, (unsigned char *)scale,
                       (unsigned char *)codes_t, (unsigned char *)scale_t, scale_stride, scale_t_stride};
     const dim3 grid((unsigned)kb, (unsigned)nb), block(256);   /* at most 8,192 x 8,192 */
-    const bool fast = aligned16(w) && p.row_bytes % 16 == 0;
+    const bool fast = !f8_misaligned(w, 16) && p.row_bytes % 16 == 0;
     const auto kernel = is_f32 ? fast ? fp8_weight_kernel<true, true> : fp8_weight_kernel<true, false>
                                : fast ? fp8_weight_kernel<false, true> : fp8_weight_kernel<false, false>;
     hipLaunchKernelGGL(kernel, grid, block, 0, (hipStream_t)stream, p);

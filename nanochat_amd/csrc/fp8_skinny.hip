@@ -26,9 +26,6 @@
 namespace nc {
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 
 constexpr int SK_WAVES = 8;
@@ -57,13 +54,7 @@ __device__ __forceinline__ i32x8 sk_operand(const Codes32 &f) {
 /* Codes 8 Q .. + 7 of a lane as bf16. */
 template <int Q> __device__ __forceinline__ bf16x8 sk_exact(const Codes32 &f) {
     const float s = f8_scale(f.byte < 1u ? 1u : f.byte);   /* a row past the last has byte 0, and zeros */
-    u32x4 o;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)f.c[2 * Q + i], s, false));
-        o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)f.c[2 * Q + i], s, true));
-    }
-    return __builtin_bit_cast(bf16x8, o);
+    return f8_values(f.c[2 * Q], f.c[2 * Q + 1], s);
 }
 
 /* A lane's part of a block as it comes from memory: 16 values from 16 g and 16 from 64 + 16 g. */
@@ -199,13 +190,6 @@ __global__ void __launch_bounds__(SK_WAVES *WAVE, MT == 1 ? 4 : 2) fp8_few_kerne
     }
 }
 
-/* As the large tiles' activation rows (fp8_gemm.hip): rows' 16-byte pieces b at place b ^ this, so that the 16 lanes that an LDS
- * read serves (rows 0-3 and 12-15 of one piece, 4-11 of the next) meet in different banks. */
-__device__ __forceinline__ int sk_swizzle(int row) {
-    const int k = (row >> 1) & 7;
-    return (k & 3) | ((k + 2) & 4);
-}
-
 /* Step j: blocks j S + s of k. RW, S 1, 8 and 2, 4, us: 64 x 1,280 x 1,280 4.8, 5.3; 128 x 1,280 x 1,280 8.4, 5.4; 64 x 1,664 x 6,656
  * 9.6, 12.3; 128 x 1,664 x 6,656 17.4, 12.4; 17 x 4,992 x 1,664 8.9, 6.4. */
 constexpr int SK_BLOCKS = 128;   /* of a row at most: their scales are kept in LDS */
@@ -227,7 +211,7 @@ __global__ void __launch_bounds__(SK_WAVES *WAVE, S == 8 ? 2 : 4) fp8_some_kerne
     const int m0 = id % parts * 16 * MT, n0 = id / parts * COLS;
     const int rows = min(p.M - m0, 16 * MT), cols = min(p.N - n0, COLS);
     const Rsrc rsw = f8_rsrc(p.w + (long long)n0 * p.K, (long long)cols * p.K);
-    const f8_u32x4 rx = f8_words((const unsigned char *)p.x + (long long)m0 * p.K, (long long)rows * p.K);
+    const u32x4 rx = f8_words((const unsigned char *)p.x + (long long)m0 * p.K, (long long)rows * p.K);
     const unsigned char *ws = p.ws + (long long)(n0 / F8_BLOCK) * p.ws_stride;   /* COLS rows lie in one block */
     const unsigned w_row = (unsigned)((16 * rw + i16) * p.K);
     const int steps = (p.blocks + S - 1) / S;
@@ -237,7 +221,7 @@ __global__ void __launch_bounds__(SK_WAVES *WAVE, S == 8 ? 2 : 4) fp8_some_kerne
 #pragma unroll
         for (int d = 0; d < DMAS; d++) {
             const int q = wave * DMAS + d, row = 8 * (q % (2 * MT)) + (lane >> 3);
-            const int k = (j * S + q / (2 * MT)) * F8_BLOCK + (((lane & 7) ^ sk_swizzle(row)) << 4);
+            const int k = (j * S + q / (2 * MT)) * F8_BLOCK + (((lane & 7) ^ f8_swizzle(row)) << 4);
             f8_dma16(base + j % RING * STEP + q * 1024, k < p.K ? (unsigned)(row * p.K + k) : SK_PAST, rx);
         }
     };
@@ -284,7 +268,7 @@ __global__ void __launch_bounds__(SK_WAVES *WAVE, S == 8 ? 2 : 4) fp8_some_kerne
                 Codes32 cx;
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const u32x4 v = *(const u32x4 *)(xb + row * F8_BLOCK + (((4 * h + g) ^ sk_swizzle(row)) << 4));
+                    const u32x4 v = *(const u32x4 *)(xb + row * F8_BLOCK + (((4 * h + g) ^ f8_swizzle(row)) << 4));
 #pragma unroll
                     for (int e = 0; e < 4; e++) cx.c[4 * h + e] = v[e];
                 }
@@ -352,7 +336,6 @@ bool serve_sizes(long long rows, int n, int k) {
     return rows >= 0 && n > 0 && k > 0 && n % 16 == 0 && k % 16 == 0 && n <= 1 << 20 && k <= 1 << 20 &&
            rows <= (1LL << 31) / ((k + F8_BLOCK - 1) / F8_BLOCK) - 32;
 }
-bool misaligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) != 0; }
 bool weight_pitch(int stride, int k) { return stride >= (k + F8_BLOCK - 1) / F8_BLOCK && stride % 4 == 0 && stride <= 1 << 14; }
 
 int linear(const void *x, int is_f32, long long row_stride, const void *w, const void *ws, int ws_stride, long long rows, int n,
@@ -397,10 +380,10 @@ extern "C" int nc_fp8_linear(const void *x, int is_f32, long long row_stride, co
         return NC_ERR_SHAPE;
     if (rows == 0) return NC_OK;
     if (!x || !w || !w_scale || !out) return NC_ERR_NULL;
-    if (misaligned(x, is_f32 ? 4 : 2) || misaligned(w, 16) || misaligned(w_scale, 4) || misaligned(out, 16)) return NC_ERR_SHAPE;
+    if (f8_misaligned(x, is_f32 ? 4 : 2) || f8_misaligned(w, 16) || f8_misaligned(w_scale, 4) || f8_misaligned(out, 16)) return NC_ERR_SHAPE;
     const long long need = nc_fp8_linear_workspace_bytes(x, is_f32, row_stride, rows, n, k);
     if (need > 0 && !workspace) return NC_ERR_NULL;
-    if (need > 0 && (misaligned(workspace, 16) || workspace_bytes < need)) return NC_ERR_WORKSPACE;
+    if (need > 0 && (f8_misaligned(workspace, 16) || workspace_bytes < need)) return NC_ERR_WORKSPACE;
     return linear(x, is_f32, row_stride, w, w_scale, w_scale_stride, rows, n, k, out, workspace, (hipStream_t)stream);
 }
 
@@ -418,10 +401,10 @@ static int mlp(bool exact, const void *x, long long row_stride, const void *fc, 
         return NC_ERR_SHAPE;
     if (rows == 0) return NC_OK;
     if (!x || !fc || !fc_scale || !proj || !proj_scale || !out || !workspace) return NC_ERR_NULL;
-    if (misaligned(x, 2) || misaligned(fc, 16) || misaligned(fc_scale, 4) || misaligned(proj, 16) || misaligned(proj_scale, 4) ||
-        misaligned(out, 16))
+    if (f8_misaligned(x, 2) || f8_misaligned(fc, 16) || f8_misaligned(fc_scale, 4) || f8_misaligned(proj, 16) || f8_misaligned(proj_scale, 4) ||
+        f8_misaligned(out, 16))
         return NC_ERR_SHAPE;
-    if (misaligned(workspace, 16) || workspace_bytes < nc_fp8_mlp_workspace_bytes(rows, c, hidden)) return NC_ERR_WORKSPACE;
+    if (f8_misaligned(workspace, 16) || workspace_bytes < nc_fp8_mlp_workspace_bytes(rows, c, hidden)) return NC_ERR_WORKSPACE;
     const hipStream_t s = (hipStream_t)stream;
     const F8Form f(workspace, rows, c), a(f.codes + f.bytes, rows, hidden);
     if (rows <= 16 && few_takes(x, false, row_stride, rows, hidden, c)) {

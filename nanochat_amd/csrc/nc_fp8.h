@@ -21,6 +21,9 @@ constexpr uint32_t F8_NAN_BYTE = 255, F8_NAN_CODES = 0x7F7F7F7Fu;
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 /* The scale byte for a block's largest magnitude, given as the bits of |x| in fp32 (at or past 0x7F800000: an infinity or a
  * NaN is in the block). At least 1: 2^-126, so that both the scale and its inverse are normal numbers. */
@@ -45,6 +48,15 @@ __device__ __forceinline__ uint32_t f8_codes(float a, float b, float c, float d,
     r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, s, false);
     r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, s, true);
     return __builtin_bit_cast(uint32_t, r);
+}
+
+/* The values of eight codes at a scale, as bf16. */
+__device__ __forceinline__ bf16x8 f8_values(uint32_t a, uint32_t b, float s) {
+    return __builtin_bit_cast(bf16x8, u32x4{
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)a, s, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)a, s, true)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)b, s, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)b, s, true))});
 }
 
 /* Two fp32 -> a bf16 pair (to nearest even; NaN stays NaN). */
@@ -82,29 +94,28 @@ __host__ __device__ static inline long long f8_scale_range(long long rows, long 
 /* DMA from memory to LDS of 16 or 4 bytes a lane (lane l's to `to` + 16 l or 4 l), as inline assembly: the compiler makes every
  * LDS read that follows its own form wait for it. The kernels that use it load and store nothing else meanwhile, and keep its
  * waits themselves. An offset past the resource's range reads zeros without an access. */
-typedef uint32_t f8_u32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ f8_u32x4 f8_words(const void *p, long long bytes) {
+__device__ __forceinline__ u32x4 f8_words(const void *p, long long bytes) {
     const uint64_t at = (uint64_t)p;
-    return f8_u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
                     (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) & 0xFFFFu,
                     (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 }
-__device__ __forceinline__ void f8_dma16(uint32_t to, uint32_t off, const f8_u32x4 &r) {
+__device__ __forceinline__ void f8_dma16(uint32_t to, uint32_t off, const u32x4 &r) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(to), "v"(off), "s"(r)
                  : "memory");
 }
-__device__ __forceinline__ void f8_dma4(uint32_t to, uint32_t off, const f8_u32x4 &r) {
+__device__ __forceinline__ void f8_dma4(uint32_t to, uint32_t off, const u32x4 &r) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(to), "v"(off), "s"(r)
                  : "memory");
 }
 /* f8_dma16 to base + STEP, from off + more, in three instructions. */
-template <int STEP> __device__ __forceinline__ void f8_dma16(uint32_t base, uint32_t off, uint32_t more, const f8_u32x4 &r) {
+template <int STEP> __device__ __forceinline__ void f8_dma16(uint32_t base, uint32_t off, uint32_t more, const u32x4 &r) {
     uint32_t at;
     asm volatile("s_add_u32 m0, %1, %2\n\tv_add_u32 %0, %4, %3\n\tbuffer_load_dwordx4 %0, %5, 0 offen lds"
                  : "=&v"(at) : "s"(base), "i"(STEP), "v"(off), "s"(more), "s"(r) : "memory", "scc");
 }
 /* f8_dma16 to base + STEP, from off, which then moves on. */
-template <int STEP> __device__ __forceinline__ void f8_dma16_on(uint32_t base, uint32_t &off, uint32_t on, const f8_u32x4 &r) {
+template <int STEP> __device__ __forceinline__ void f8_dma16_on(uint32_t base, uint32_t &off, uint32_t on, const u32x4 &r) {
     asm volatile("s_add_u32 m0, %1, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %3, 0 offen lds\n\tv_add_u32 %0, %4, %0"
                  : "+v"(off) : "s"(base), "i"(STEP), "s"(r), "s"(on) : "memory", "scc");
 }
@@ -122,6 +133,21 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
     v = a[0] > a[1] ? a[0] : a[1];
     const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return b[0] > b[1] ? b[0] : b[1];
+}
+
+/* Rows of activations in LDS, 128 bytes each: a row keeps its 16-byte piece b at place b ^ f8_swizzle(row). A 16-byte LDS read serves
+ * lanes 0-3, 12-15, 20-23 and 24-27 together, then 4-11, 16-19 and 28-31, and so the upper half. Two rows lie side by side over the 64
+ * banks, so 8 rows of one parity, four of one 16-byte piece b and four of b ^ 2, need 8 places. Rows i: i / 2 in {0, 1, 6, 7} gives
+ * places 0 to 3 (closed under ^ 2), the others 4 to 7. */
+__device__ __forceinline__ int f8_swizzle(int row) {
+    const int k = (row >> 1) & 7;
+    return (k & 3) | ((k + 2) & 4);
+}
+
+/* What the entry points check. */
+static inline bool f8_misaligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) != 0; }
+static inline bool f8_bad_scales(const void *p, long long stride, int cols) {
+    return f8_misaligned(p, 4) || stride % 4 || stride < (cols + F8_BLOCK - 1) / F8_BLOCK || stride > 1 << 14;
 }
 
 /* Rows in the 8-bit form in a workspace: their codes, then their scales at a padded stride. */
