@@ -370,18 +370,19 @@ int nc_fp8_quantize_weight(const void *w, int is_f32, long long row_stride, int 
 /* out[m][n] = sum_k a[m][k] w[n][k], a [rows][k] and w [n][k] in the 8-bit form, n and k multiples of 16:
  * nc_fp8_matmul         out bf16 [rows][n]
  * nc_fp8_matmul_relu2   relu(out)^2 of the fp32 sums in the 8-bit form: codes [rows][n], scale at scale_stride
- * nc_fp8_matmul_relu2_exact  the same, no bits of a product dropped (see below), in twice the time
+ * nc_fp8_matmul_relu2_fast  the same from sums that drop bits where the rows are many, in 0.55 to 0.6 of the time there
  * nc_fp8_matmul_relu2_bwd  out = bf16(sum * 2 sqrt(act)), act [rows][n] in the 8-bit form (as nc_fp8_matmul_relu2 leaves it), and
  *                       the 8-bit form of out: the gradient before a ReLU^2 whose result act is, from the one behind it
- * Sums are fp32, but for the eight products of adjacent k that the matrix cores add at a time: of those, bits below 2^-13 of
- * the largest are dropped (at most 2^-10 of the sum of magnitudes, and 1e-5 to 3e-5 of a result as a rule); nc_fp8_matmul_relu2 drops
- * none where ceil(rows / 64) ceil(n / 128) is at most the device's number of CUs. The outputs may not overlap the inputs. */
+ * Sums are fp32, of exact products in nc_fp8_matmul_relu2. In the others they are so but for the eight products of adjacent k that
+ * the matrix cores add at a time: of those, bits below 2^-13 of the largest are dropped (at most 2^-10 of the sum of magnitudes, and
+ * 1e-5 to 3e-5 of a result as a rule); nc_fp8_matmul_relu2_fast drops none where ceil(rows / 64) ceil(n / 128) is at most the device's
+ * number of CUs. The outputs may not overlap the inputs. */
 int nc_fp8_matmul(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
                   int w_scale_stride, long long rows, int n, int k, void *out, void *stream);
 int nc_fp8_matmul_relu2(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
                         int w_scale_stride, long long rows, int n, int k, void *codes, void *scale, long long scale_stride,
                         void *stream);
-int nc_fp8_matmul_relu2_exact(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
+int nc_fp8_matmul_relu2_fast(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
                               int w_scale_stride, long long rows, int n, int k, void *codes, void *scale, long long scale_stride,
                               void *stream);
 int nc_fp8_matmul_relu2_bwd(const void *a, const void *a_scale, long long a_scale_stride, const void *w, const void *w_scale,
@@ -395,7 +396,7 @@ int nc_fp8_matmul_relu2_bwd(const void *a, const void *a_scale, long long a_scal
  * A few rows are bound by reading the weights once; up to 64 that can be read 16 bytes at a time, where they are short and the
  * outputs few enough, are one launch a product. workspace: nc_fp8_*_workspace_bytes (-1 for unsupported sizes; of a layer, for the x
  * and row_stride of the call, and 0 where none is read: it may then be NULL), 16-byte aligned, need not be cleared. A call's workspace
- * is its own until it has run. nc_fp8_mlp_exact is nc_fp8_mlp by way of nc_fp8_matmul_relu2_exact. */
+ * is its own until it has run. nc_fp8_mlp_fast is nc_fp8_mlp by way of nc_fp8_matmul_relu2_fast. */
 long long nc_fp8_linear_workspace_bytes(const void *x, int is_f32, long long row_stride, long long rows, int n, int k);
 int nc_fp8_linear(const void *x, int is_f32, long long row_stride, const void *w, const void *w_scale, int w_scale_stride,
                   long long rows, int n, int k, void *out, void *workspace, long long workspace_bytes, void *stream);
@@ -403,7 +404,7 @@ long long nc_fp8_mlp_workspace_bytes(long long rows, int c, int hidden);
 int nc_fp8_mlp(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride, const void *proj,
                const void *proj_scale, int proj_scale_stride, long long rows, int c, int hidden, int n, void *out,
                void *workspace, long long workspace_bytes, void *stream);
-int nc_fp8_mlp_exact(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride, const void *proj,
+int nc_fp8_mlp_fast(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride, const void *proj,
                      const void *proj_scale, int proj_scale_stride, long long rows, int c, int hidden, int n, void *out,
                      void *workspace, long long workspace_bytes, void *stream);
 
@@ -420,7 +421,7 @@ int nc_fp8_weight_grad(const void *dy, const void *codes, const void *scale, lon
  * The training of a layer and of a ReLU^2 MLP, a direction a call, from the parts above. All in the 8-bit form are at strides as
  * there; rows bf16 at row_stride elements; all widths are multiples of 16.
  *   forward   codes, scale = x in the 8-bit form: the checkpoint; linear: out = it w^T; mlp: act, act_scale = relu(it fc^T)^2 in the
- *             8-bit form, the second checkpoint, and out = it proj^T (_exact: by way of nc_fp8_matmul_relu2_exact)
+ *             8-bit form, the second checkpoint, and out = it proj^T (_fast: by way of nc_fp8_matmul_relu2_fast)
  *   backward  dy bf16 [rows][n] (dense, 16-byte aligned, where a weight gradient reads it) -> dx bf16 [rows][k] (not wanted where
  *             NULL), from the weights' transposes in the 8-bit form, and dw in nc_fp8_weight_grad's mode, or -1 where it is not wanted:
  *             dx = dy8 w8, dw = dy^T x8; dh = bf16((dy8 p8) 2 sqrt(a8)), dx = dh8 f8, dfc = dh^T x8, dproj = dy^T a8. rows = 0
@@ -437,7 +438,7 @@ int nc_fp8_mlp_fwd(const void *x, long long row_stride, const void *fc, const vo
                    const void *proj, const void *proj_scale, int proj_scale_stride, long long rows, int c, int hidden, int n,
                    void *codes, void *scale, long long scale_stride, void *act, void *act_scale, long long act_scale_stride,
                    void *out, void *stream);
-int nc_fp8_mlp_fwd_exact(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
+int nc_fp8_mlp_fwd_fast(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
                          const void *proj, const void *proj_scale, int proj_scale_stride, long long rows, int c, int hidden, int n,
                          void *codes, void *scale, long long scale_stride, void *act, void *act_scale, long long act_scale_stride,
                          void *out, void *stream);

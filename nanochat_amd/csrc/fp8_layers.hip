@@ -80,7 +80,7 @@ extern "C" int nc_fp8_linear_bwd(const void *dy, long long row_stride, const voi
     return status;
 }
 
-static int mlp_fwd(bool exact, const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
+static int mlp_fwd(bool fast, const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
                    const void *proj, const void *proj_scale, int proj_scale_stride, long long rows, int c, int hidden, int n,
                    void *codes, void *scale, long long scale_stride, void *act, void *act_scale, long long act_scale_stride,
                    void *out, void *stream) {
@@ -93,7 +93,7 @@ static int mlp_fwd(bool exact, const void *x, long long row_stride, const void *
         return NC_ERR_SHAPE;
     int status = nc_fp8_quantize_rows(x, 0, row_stride, rows, c, codes, scale, scale_stride, stream);
     if (!status)
-        status = (exact ? nc_fp8_matmul_relu2_exact : nc_fp8_matmul_relu2)(codes, scale, scale_stride, fc, fc_scale, fc_scale_stride,
+        status = (fast ? nc_fp8_matmul_relu2_fast : nc_fp8_matmul_relu2)(codes, scale, scale_stride, fc, fc_scale, fc_scale_stride,
                                                                            rows, hidden, c, act, act_scale, act_scale_stride, stream);
     return status ? status : nc_fp8_matmul(act, act_scale, act_scale_stride, proj, proj_scale, proj_scale_stride, rows, n,
                                            hidden, out, stream);
@@ -107,7 +107,7 @@ extern "C" int nc_fp8_mlp_fwd(const void *x, long long row_stride, const void *f
                    scale, scale_stride, act, act_scale, act_scale_stride, out, stream);
 }
 
-extern "C" int nc_fp8_mlp_fwd_exact(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
+extern "C" int nc_fp8_mlp_fwd_fast(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
                                     const void *proj, const void *proj_scale, int proj_scale_stride, long long rows, int c, int hidden,
                                     int n, void *codes, void *scale, long long scale_stride, void *act, void *act_scale,
                                     long long act_scale_stride, void *out, void *stream) {

@@ -393,7 +393,7 @@ extern "C" long long nc_fp8_mlp_workspace_bytes(long long rows, int c, int hidde
     return f8_form_bytes(rows, c) + f8_form_bytes(rows, hidden) + (rows <= 16 ? 4 * rows * hidden : 0);
 }
 
-static int mlp(bool exact, const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
+static int mlp(bool fast, const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
                const void *proj, const void *proj_scale, int proj_scale_stride, long long rows, int c, int hidden, int n, void *out,
                void *workspace, long long workspace_bytes, void *stream) {
     if (!serve_sizes(rows, hidden, c) || !serve_sizes(rows, n, hidden) || (rows > 1 && row_stride < c) ||
@@ -414,7 +414,7 @@ static int mlp(bool exact, const void *x, long long row_stride, const void *fc, 
     }
     int status = nc_fp8_quantize_rows(x, 0, row_stride, rows, c, f.codes, f.scale, f.pitch, stream);
     if (!status)
-        status = (exact ? nc_fp8_matmul_relu2_exact : nc_fp8_matmul_relu2)(f.codes, f.scale, f.pitch, fc, fc_scale, fc_scale_stride,
+        status = (fast ? nc_fp8_matmul_relu2_fast : nc_fp8_matmul_relu2)(f.codes, f.scale, f.pitch, fc, fc_scale, fc_scale_stride,
                                                                            rows, hidden, c, a.codes, a.scale, a.pitch, stream);
     return status ? status : nc_fp8_matmul(a.codes, a.scale, a.pitch, proj, proj_scale, proj_scale_stride, rows, n, hidden, out,
                                            stream);
@@ -427,7 +427,7 @@ extern "C" int nc_fp8_mlp(const void *x, long long row_stride, const void *fc, c
                workspace, workspace_bytes, stream);
 }
 
-extern "C" int nc_fp8_mlp_exact(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
+extern "C" int nc_fp8_mlp_fast(const void *x, long long row_stride, const void *fc, const void *fc_scale, int fc_scale_stride,
                                 const void *proj, const void *proj_scale, int proj_scale_stride, long long rows, int c, int hidden,
                                 int n, void *out, void *workspace, long long workspace_bytes, void *stream) {
     return mlp(true, x, row_stride, fc, fc_scale, fc_scale_stride, proj, proj_scale, proj_scale_stride, rows, c, hidden, n, out,

@@ -225,13 +225,13 @@ def fp8_linear(x: Tensor, weight: Fp8Weight) -> Tensor:
     return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
 
 
-def fp8_mlp(x: Tensor, fc: Fp8Weight, proj: Fp8Weight, exact: bool = False) -> Tensor:
+def fp8_mlp(x: Tensor, fc: Fp8Weight, proj: Fp8Weight, fast: bool = False) -> Tensor:
     """x bf16 [..., C] through proj(relu(fc(x))^2), fc [F, C] and proj [N, F] held in 8 bits: bf16 [..., N]. The squared
-    activations are taken in their 8-bit form from fp32 sums, of products that drop bits as fp8_matmul's do where there are many
-    rows (ceil(rows / 64) ceil(F / 128) above the number of CUs): some 5 of 10,000 squares, which lie on the border of two codes, then get the other one, and a result lies 0.0024 to 0.0029
-    (relative norm) from what float64 makes of the same operands, where a bf16 rounding alone is 0.0017 (the 8-bit form itself puts it
-    0.057 off the MLP without it). exact: no bits are dropped before the square, as for few rows anyway; that product then
-    takes twice as long. For serving: no gradient (checkpointed_mlp has one)."""
+    activations are taken in their 8-bit form from fp32 sums of exact products. fast: for many rows (ceil(rows / 64) ceil(F / 128)
+    above the number of CUs) that product takes 0.55 to 0.6 of the time, and drops bits as fp8_matmul's does: some 5 of 10,000 squares, which
+    lie on the border of two codes, then get the other one, and a result lies 0.0024 to 0.0037 (relative norm) from what float64
+    makes of the same operands, in place of the 0.0017 that its own rounding to bf16 makes (the 8-bit form itself puts it 0.057 off the
+    MLP without it). For serving: no gradient (checkpointed_mlp has one)."""
     rows = _serving_input(x, fc, "fp8_mlp")
     fc_pitch, _ = _check_weight(fc, "fc", x.device)
     proj_pitch, _ = _check_weight(proj, "proj", x.device)
@@ -243,7 +243,7 @@ def fp8_mlp(x: Tensor, fc: Fp8Weight, proj: Fp8Weight, exact: bool = False) -> T
         lib = hip_library()
         need = lib.nc_fp8_mlp_workspace_bytes(m, c, hidden)
         out, ws = torch.empty(m, n, dtype=BF16, device=x.device), _workspace(x, need)
-        call = lib.nc_fp8_mlp_exact if exact else lib.nc_fp8_mlp
+        call = lib.nc_fp8_mlp_fast if fast else lib.nc_fp8_mlp
         check(call(rows.data_ptr(), rows.stride(0), fc.codes.data_ptr(), fc.scale.data_ptr(), fc_pitch, proj.codes.data_ptr(),
                    proj.scale.data_ptr(), proj_pitch, m, c, hidden, n, out.data_ptr(), ws.data_ptr(), need, stream()))
     return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
@@ -494,7 +494,7 @@ def checkpointed_linear(x: Tensor, weight: Tensor, weight8: Fp8Weight | None = N
 def _run_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc_codes: Tensor | None, fc_scale: Tensor | None, fc_codes_t: Tensor | None,
              fc_scale_t: Tensor | None, fc_grad: Tensor | None, proj_codes: Tensor | None, proj_scale: Tensor | None,
              proj_codes_t: Tensor | None, proj_scale_t: Tensor | None, proj_grad: Tensor | None,
-             exact: bool = False) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+             fast: bool = False) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
     """-> y, then what the backward reads: the codes and scales of x, of the hidden activations, and of both transposes."""
     rows, device = _as_rows(x, "x", (BF16,)), x.device
     if fc.dim() == proj.dim() == 2 and (rows.size(1) != fc.size(1) or proj.size(1) != fc.size(0)):
@@ -506,7 +506,7 @@ def _run_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc_codes: Tensor | None, fc_sc
         x8, xs = torch.empty(m, c, dtype=CODES, device=device), _whole_scale(x, m, c)
         a8, a_s = torch.empty(m, hidden, dtype=CODES, device=device), _whole_scale(x, m, hidden)
         y = torch.empty(*x.shape[:-1], n, dtype=BF16, device=device)
-        call = hip_library().nc_fp8_mlp_fwd_exact if exact else hip_library().nc_fp8_mlp_fwd
+        call = hip_library().nc_fp8_mlp_fwd_fast if fast else hip_library().nc_fp8_mlp_fwd
         check(call(rows.data_ptr(), rows.stride(0), f.data_ptr(), fs.data_ptr(), f_pitch, p.data_ptr(), ps.data_ptr(), p_pitch, m, c,
                    hidden, n, x8.data_ptr(), xs.data_ptr(), xs.size(1), a8.data_ptr(), a_s.data_ptr(), a_s.size(1), y.data_ptr(),
                    stream()))
@@ -514,7 +514,7 @@ def _run_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc_codes: Tensor | None, fc_sc
 
 
 def _fake_mlp(x, fc, proj, fc_codes, fc_scale, fc_codes_t, fc_scale_t, fc_grad, proj_codes, proj_scale, proj_codes_t,
-              proj_scale_t, proj_grad, exact=False):
+              proj_scale_t, proj_grad, fast=False):
     rows, (hidden, k), n = _rows_of(x), fc.shape, proj.size(0)
 
     def kept(made, rows_t, cols_t):
@@ -569,7 +569,7 @@ _mlp_bwd = _op("checkpointed_mlp_bwd", "(Tensor dy, Tensor x8, Tensor xs, Tensor
                "bool need_x, bool need_fc, bool need_proj, bool fc_wide, bool proj_wide) -> (Tensor, Tensor, Tensor)",
                _run_mlp_bwd, _fake_mlp_bwd)
 _mlp = _op("checkpointed_mlp", f"(Tensor x, Tensor fc, Tensor proj, {_HELD.format('fc_')}, {_HELD.format('proj_')}, "
-           f"bool exact=False) -> ({', '.join(['Tensor'] * 9)})", _run_mlp, _fake_mlp)
+           f"bool fast=False) -> ({', '.join(['Tensor'] * 9)})", _run_mlp, _fake_mlp)
 
 
 class _Mlp(torch.autograd.Function):
@@ -600,7 +600,7 @@ class _Mlp(torch.autograd.Function):
 
 
 def checkpointed_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc8: Fp8Weight | None = None, proj8: Fp8Weight | None = None,
-                     fc_grad: Tensor | None = None, proj_grad: Tensor | None = None, exact: bool = False) -> Tensor:
+                     fc_grad: Tensor | None = None, proj_grad: Tensor | None = None, fast: bool = False) -> Tensor:
     """x bf16 [..., C] through proj(relu(fc(x))^2) in 8-bit products, bf16 [..., N], differentiable in x, fc [F, C] and proj
     [N, F] (bf16 or fp32, all sizes multiples of 16 up to 65,536). Kept for the backward are the 8-bit forms of x and of the squared
     activations a, C + F bytes a token where bf16 keeps x, the sums before the square and the squares in 2 C + 4 F. With x8
@@ -610,8 +610,7 @@ def checkpointed_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc8: Fp8Weight | None 
         dx = dh8 f8      dfc = dh^T x8      dproj = dy^T a8
 
     The derivative of the square is read from the checkpoint itself: 2 relu(h) = 2 sqrt(a). fc8, proj8, fc_grad and proj_grad
-    as checkpointed_linear's weight8 and grad. exact: as fp8_mlp's, of x8 f8^T; what it says of the result holds for the
-    gradients that are made from a8, too."""
+    as checkpointed_linear's weight8 and grad. fast: as fp8_mlp's, of x8 f8^T; what it says of the result holds for dproj, too."""
     fc = _asking(fc, fc_grad, x, proj)
     proj = _asking(proj, proj_grad, x, fc)
-    return _Mlp.apply(x, fc, proj, *(fc8 or _NOT_HELD), fc_grad, *(proj8 or _NOT_HELD), proj_grad, exact)
+    return _Mlp.apply(x, fc, proj, *(fc8 or _NOT_HELD), fc_grad, *(proj8 or _NOT_HELD), proj_grad, fast)

@@ -163,7 +163,7 @@ SIGNATURES = {
                         c_int, c_void_p, c_longlong, c_void_p], c_int),
     "nc_pages_trim": ([c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p], c_int),
 }
-SIGNATURES |= {f"{name}_exact": SIGNATURES[name] for name in ("nc_fp8_matmul_relu2", "nc_fp8_mlp", "nc_fp8_mlp_fwd")}
+SIGNATURES |= {f"{name}_fast": SIGNATURES[name] for name in ("nc_fp8_matmul_relu2", "nc_fp8_mlp", "nc_fp8_mlp_fwd")}
 
 
 # argtypes of every entry point of include/nanochat_decode.h (the reference's binding: decoder.py:132-148)

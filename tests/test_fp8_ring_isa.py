@@ -1,4 +1,4 @@
-"""The smaller tiles of the 8-bit products (fp8_gemm.hip: half and small tiles; fp8_skinny.hip: fp8_some_kernel) read stages from LDS
+"""All but the full tiles of the 8-bit products (fp8_gemm.hip: wide, half and small ones; fp8_skinny.hip: fp8_some_kernel) read stages from LDS
 that DMA issued as inline assembly brings, and wait for them by a number of newer memory instructions: that number has to be on
 its way behind a stage's DMA on every path, or a wait for it lets the stage itself be late. What the compiler moves of its own loads and
 stores could change it. This checks on the compiler's gfx950 assembly, for every such kernel:
@@ -20,7 +20,8 @@ from tests.test_prefill_gemm_isa import blocks
 # stages in LDS, 16-byte DMA of a stage and wave
 KERNELS = {("fp8_gemm.hip", f"15fp8_gemm_kernelINS0_6FgTileI{tile}EELi{epi}EEEv"): sizes
            for tile, sizes in (("Li2ELi1ELi4ELi2E", (2, 8)), ("Li1ELi1ELi4ELi3E", (3, 6))) for epi in range(3)}
-KERNELS |= {("fp8_gemm.hip", "15fp8_gemm_kernelINS0_6FgTileILi2ELi1ELi4ELi2EEELi3EEEv"): (2, 8)}   # exact products before a ReLU^2
+KERNELS |= {("fp8_gemm.hip", f"15fp8_gemm_kernelINS0_6FgTileI{tile}EELi3EEEv"): (2, 8)   # exact products before a ReLU^2
+            for tile in ("Li2ELi1ELi4ELi2E", "Li4ELi2ELi4ELi2E")}
 KERNELS |= {("fp8_skinny.hip", "15fp8_some_kernelILi1ELi8EEEv"): (3, 4), ("fp8_skinny.hip", "15fp8_some_kernelILi2ELi4EEEv"): (4, 2)}
 LANDED = 1 << 20
 VMEM = ("buffer_", "global_", "flat_", "scratch_")

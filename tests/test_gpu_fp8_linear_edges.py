@@ -7,7 +7,7 @@ import torch
 from nanochat_amd import fp8_linear as fl, native
 from nanochat_amd.native import hip_library, stream
 from oracle import fp8_block as fb
-from tests.test_gpu_fp8_linear import EPS, bf, close, codes_of, exps_of, form, held, product_relu2, product_relu2_bwd, same_form, weight
+from tests.test_gpu_fp8_linear import EPS, SIZES, bf, close, codes_of, exps_of, form, held, product_relu2, product_relu2_bwd, same_form, weight
 
 pytestmark = pytest.mark.gpu
 
@@ -47,6 +47,17 @@ def test_buffers_of_layers_without_a_gradient(device):
     fl.checkpointed_mlp(x, *asked[1:]).backward(dy)
     # the same sums, added to zeros
     assert all(torch.equal(b, t.grad) for b, t in zip(buffers, asked)) and all(t.grad is None for t in (w, fc, proj))
+
+
+def relu2_fast(codes, scale, w):
+    """product_relu2 by the products that drop bits in half and full tiles."""
+    rows, k = codes.shape
+    n = w.codes.size(0)
+    out, out_scale = torch.empty(rows, n, dtype=fl.CODES, device=codes.device), fl._new_scale(codes, rows, n)
+    native.check(hip_library().nc_fp8_matmul_relu2_fast(codes.data_ptr(), scale.data_ptr(), scale.stride(0), w.codes.data_ptr(),
+                                                         w.scale.data_ptr(), w.scale.stride(0), rows, n, k, out.data_ptr(),
+                                                         out_scale.data_ptr(), out_scale.stride(0), stream()))
+    return out, out_scale
 
 
 # --- long walks, and workgroups that take several tiles (256 CUs; stages of 128 columns)
@@ -99,10 +110,11 @@ def test_long_product(device, rows, n, k):
     assert np.linalg.norm(got - want) <= 2.0 ** -8 * np.linalg.norm(want)
 
 
-@pytest.mark.parametrize("rows,n,k", LONG)
-def test_long_product_relu2(device, rows, n, k):
+@pytest.mark.parametrize("squares", [product_relu2, relu2_fast])
+@pytest.mark.parametrize("rows,n,k", LONG + SIZES[-5:])
+def test_long_product_relu2(device, rows, n, k, squares):
     _, codes, scale, w, there, h, off = operands(device, rows, n, k)
-    a8, a_s = product_relu2(codes, scale, w)
+    a8, a_s = squares(codes, scale, w)
     want = np.maximum(h, 0.0) ** 2
     slack = 2 * np.maximum(h, 0.0) * off + off * off + 4 * EPS * want
     s = held(a_s[there])
@@ -148,16 +160,6 @@ def test_square_roots_at_the_ends_of_the_range(device, rows, n, k, least, most):
 
 # --- how exact the squares are
 
-def relu2_exact(codes, scale, w):
-    rows, k = codes.shape
-    n = w.codes.size(0)
-    out, out_scale = torch.empty(rows, n, dtype=fl.CODES, device=codes.device), fl._new_scale(codes, rows, n)
-    native.check(hip_library().nc_fp8_matmul_relu2_exact(codes.data_ptr(), scale.data_ptr(), scale.stride(0), w.codes.data_ptr(),
-                                                         w.scale.data_ptr(), w.scale.stride(0), rows, n, k, out.data_ptr(),
-                                                         out_scale.data_ptr(), out_scale.stride(0), stream()))
-    return out, out_scale
-
-
 def dropped(x, w):
     """What the matrix cores may drop of x w^T: of each eight adjacent products seven times 2^-13 of the largest."""
     rows, k = x.shape
@@ -195,49 +197,53 @@ def test_squares_of_exact_products(device, rows, n, k):
     is allowed, where the products by eights with their d of 1e-5 to 3e-5 give 2e-4 to 7e-4."""
     _, codes, scale, w, there, h, _ = operands(device, rows, n, k)
     x, wv = fb.values(codes_of(codes[there].contiguous()), exps_of(scale[there]), 1), fb.values(codes_of(w.codes), exps_of(w.scale), 128)
-    a8, a_s = relu2_exact(codes, scale, w)
+    a8, a_s = product_relu2(codes, scale, w)
     between(a8[there], a_s[there], h, k * EPS * (np.abs(x) @ np.abs(wv).T))
     assert others(a8[there], a_s[there], h) <= 1e-4
-    again = relu2_exact(codes, scale, w)
+    again = product_relu2(codes, scale, w)
     assert torch.equal(again[0].view(torch.uint8), a8.view(torch.uint8))
 
 
 @pytest.mark.parametrize("rows,n,k", SQUARES)
 def test_squares_of_products_by_eights(device, rows, n, k):
-    """The larger tiles' products drop bits, by eights of columns: where, and no more than that."""
+    """The fast form's products drop bits in the larger tiles, by eights of columns, and no more than that."""
     _, codes, scale, w, there, h, _ = operands(device, rows, n, k)
     some = np.arange(0, len(h), max(1, len(h) // 24))
     there, h = there[torch.from_numpy(some).to(device)], h[some]
     x, wv = fb.values(codes_of(codes[there].contiguous()), exps_of(scale[there]), 1), fb.values(codes_of(w.codes), exps_of(w.scale), 128)
-    a8, a_s = product_relu2(codes, scale, w)
+    a8, a_s = relu2_fast(codes, scale, w)
     between(a8[there], a_s[there], h, dropped(x, wv) + k * EPS * (np.abs(x) @ np.abs(wv).T))
     assert others(a8[there], a_s[there], h) <= 1e-3
 
 
+@pytest.mark.parametrize("fast", [False, True])
 @pytest.mark.parametrize("rows", [1, 40, 700, 9000])
-def test_exact_mlp(device, rows):
-    """An MLP's result is off by its own rounding alone, in any batch; in training, too, and its gradients are of those squares."""
+def test_mlp_is_as_exact_as_its_squares(device, rows, fast):
+    """An MLP's result is off by its own rounding alone, in any batch, but for the squares that the fast form takes otherwise; in
+    training, too, whose gradients are of those squares."""
     gen = torch.Generator().manual_seed(rows)
     x = bf(gen, rows, 400).to(device)
     fc_w, proj_w = (torch.randn(*s, generator=gen).to(device) * s[1] ** -0.5 for s in ((2064, 400), (144, 2064)))
     fc, proj = fl.quantize_weight(fc_w, True), fl.quantize_weight(proj_w, True)
-    fcv, pv = (fb.values(codes_of(t.codes), exps_of(t.scale), 128) for t in (fc, proj))
-    at = torch.arange(0, rows, max(1, rows // 200))
-    want = fb.through(np.maximum(fb.through(x[at].double().cpu().numpy(), 1) @ fcv.T, 0.0) ** 2, 1) @ pv.T
-    z = fl.fp8_mlp(x, fc, proj, exact=True)
-    assert np.linalg.norm(codes_of(z[at]) - want) <= 2.0 ** -8 * np.linalg.norm(want)
+    z = fl.fp8_mlp(x, fc, proj, fast=fast)
+    if not fast:
+        fcv, pv = (fb.values(codes_of(t.codes), exps_of(t.scale), 128) for t in (fc, proj))
+        at = torch.arange(0, rows, max(1, rows // 200))
+        want = fb.through(np.maximum(fb.through(x[at].double().cpu().numpy(), 1) @ fcv.T, 0.0) ** 2, 1) @ pv.T
+        assert np.linalg.norm(codes_of(z[at]) - want) <= 2.0 ** -8 * np.linalg.norm(want)
+        assert torch.equal(fl.fp8_mlp(x, fc, proj), z)
     given = [t.clone().requires_grad_() for t in (x, fc_w, proj_w)]
-    y = fl.checkpointed_mlp(*given, exact=True)
+    y = fl.checkpointed_mlp(*given, fast=fast)
     codes, scale = fl.quantize_rows(x)
-    act = relu2_exact(codes, scale, fc)
+    act = (relu2_fast if fast else product_relu2)(codes, scale, fc)
     assert torch.equal(y, fl.fp8_matmul(*act, proj)) and (rows <= 16 or torch.equal(y, z))
     dy = bf(gen, rows, 144).to(device)
     dx, dfc, dproj = torch.autograd.grad(y, given, dy)
     dh, q, q_s = product_relu2_bwd(*fl.quantize_rows(dy), fl.Fp8Weight(proj.codes_t, proj.scale_t), *act)
     assert torch.equal(dx, fl.fp8_matmul(q, q_s, fl.Fp8Weight(fc.codes_t, fc.scale_t)))
-    for got, left, right, depth in ((dfc, dh, (codes, scale), rows), (dproj, dy, act, rows)):
+    for got, left, right in ((dfc, dh, (codes, scale)), (dproj, dy, act)):
         a, b = left.double().cpu().numpy(), fb.values(codes_of(right[0]), exps_of(right[1]), 1)
-        close(codes_of(got), a.T @ b, (depth + 300) * EPS * (np.abs(a).T @ np.abs(b)))
+        close(codes_of(got), a.T @ b, (rows + 300) * EPS * (np.abs(a).T @ np.abs(b)))
 
 
 # --- gradients against differences, where nothing is rounded
