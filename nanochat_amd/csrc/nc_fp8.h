@@ -6,7 +6,8 @@
  * The scale is the least power of two s with amax <= 448 s: amax = m 2^e with m in [1, 2) gives 2^(e - 8), doubled where m >
  * 1.75 (448 = 1.75 2^8). A block of zeros has scale 1. A power of two keeps the codes' relative error at half a step (2^-4)
  * whatever it is, down to amax 2^-15 / 1.75 or less where e4m3 becomes subnormal; it makes x / s exact, so a code is one
- * rounding of x, and code * s exact in bf16 (from s = 2^-124 on), which the matrix cores multiply as it is.
+ * rounding of x, and code * s exact in bf16, which the matrix cores multiply as it is (but at either end of the range: under s = 2^-124
+ * a code's lowest bits fall below bf16's least number, and one that rounds a magnitude above 2^128 (1 - 2^-5) up stands for 2^128).
  * A block with an infinity or a NaN becomes NaN whole (byte 255, every code 0x7F): what is made from it is NaN too.
  */
 #pragma once

@@ -446,7 +446,7 @@ _linear = _op("checkpointed_linear", f"(Tensor x, Tensor weight, {_HELD.format('
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx: FunctionCtx, *inputs: Tensor | None) -> Tensor:
-        x, weight, codes, _, codes_t, scale_t, grad = inputs
+        x, weight, codes, _, codes_t, scale_t, grad = inputs = inputs[:7]   # without _asking's
         y, x8, xs, made_t, made_ts = _linear(*inputs)
         ctx.x_shape, ctx.wide, ctx.grad = x.shape, weight.dtype == F32, grad   # grad not saved: it may change until it is added to
         ctx.set_materialize_grads(False)
@@ -457,23 +457,26 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx: FunctionCtx, dy: Tensor | None) -> tuple:
         if dy is None:
-            return (None,) * 7
+            return (None,) * 8
         grad, need_x = ctx.grad, ctx.needs_input_grad[0]
         need_w = ctx.needs_input_grad[1] or grad is not None
         dx, dw = _linear_bwd(dy, *ctx.saved_tensors, grad, need_x, need_w, ctx.wide)
-        return (dx.view(ctx.x_shape) if need_x else None, dw if need_w and grad is None else None, *(None,) * 5)
+        return (dx.view(ctx.x_shape) if need_x else None, dw if need_w and grad is None else None, *(None,) * 6)
 
 
 
 _NOT_HELD = (None, None, None, None)
 
 
-def _asking(weight: Tensor, grad: Tensor | None, *others: Tensor) -> Tensor:
-    """weight, or, where a buffer is given for its gradient and nothing else would have the call recorded, an alias that requires
-    a gradient (and gets none: it goes into the buffer)."""
-    if grad is None or weight.requires_grad or not torch.is_grad_enabled() or any(t.requires_grad for t in others):
-        return weight
-    return weight.detach().requires_grad_()
+with torch.inference_mode(False):
+    _ASKS = torch.zeros((), device="cpu", requires_grad=True)   # has a call recorded whose other inputs do not; gets no gradient
+
+
+def _asking(grads: tuple, inputs: tuple) -> Tensor | None:
+    """The input that has a call with gradient buffers recorded where nothing else would."""
+    if not torch.is_grad_enabled() or all(g is None for g in grads) or any(t.requires_grad for t in inputs):
+        return None
+    return _ASKS
 
 
 def checkpointed_linear(x: Tensor, weight: Tensor, weight8: Fp8Weight | None = None, grad: Tensor | None = None) -> Tensor:
@@ -487,8 +490,7 @@ def checkpointed_linear(x: Tensor, weight: Tensor, weight8: Fp8Weight | None = N
     added to in the backward, autograd then getting none for the weight; with a buffer the call is recorded (unless under
     torch.no_grad()) and dw made whether or not x or weight requires a gradient. The gradients themselves cannot be
     differentiated."""
-    weight = _asking(weight, grad, x)
-    return _Linear.apply(x, weight, *(weight8 or _NOT_HELD), grad)
+    return _Linear.apply(x, weight, *(weight8 or _NOT_HELD), grad, _asking((grad,), (x, weight)))
 
 
 def _run_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc_codes: Tensor | None, fc_scale: Tensor | None, fc_codes_t: Tensor | None,
@@ -577,7 +579,7 @@ class _Mlp(torch.autograd.Function):
     def forward(ctx: FunctionCtx, *inputs: Tensor | bool | None) -> Tensor:
         x, fc, proj = inputs[:3]
         f, p = inputs[3:8], inputs[8:13]
-        y, x8, xs, a8, a_s, f_t, f_ts, p_t, p_ts = _mlp(*inputs)
+        y, x8, xs, a8, a_s, f_t, f_ts, p_t, p_ts = _mlp(*inputs[:14])   # without _asking's
         ctx.x_shape, ctx.fc_wide, ctx.proj_wide = x.shape, fc.dtype == F32, proj.dtype == F32
         ctx.fc_grad, ctx.proj_grad = f[4], p[4]
         ctx.set_materialize_grads(False)
@@ -589,13 +591,13 @@ class _Mlp(torch.autograd.Function):
     @once_differentiable
     def backward(ctx: FunctionCtx, dy: Tensor | None) -> tuple:
         if dy is None:
-            return (None,) * 14
+            return (None,) * 15
         fc_grad, proj_grad, need_x = ctx.fc_grad, ctx.proj_grad, ctx.needs_input_grad[0]
         need_fc, need_proj = ctx.needs_input_grad[1] or fc_grad is not None, ctx.needs_input_grad[2] or proj_grad is not None
         dx, dfc, dproj = _mlp_bwd(dy, *ctx.saved_tensors, fc_grad, proj_grad, need_x, need_fc, need_proj, ctx.fc_wide,
                                   ctx.proj_wide)
         return (dx.view(ctx.x_shape) if need_x else None, dfc if need_fc and fc_grad is None else None,
-                dproj if need_proj and proj_grad is None else None, *(None,) * 11)
+                dproj if need_proj and proj_grad is None else None, *(None,) * 12)
 
 
 
@@ -611,6 +613,5 @@ def checkpointed_mlp(x: Tensor, fc: Tensor, proj: Tensor, fc8: Fp8Weight | None 
 
     The derivative of the square is read from the checkpoint itself: 2 relu(h) = 2 sqrt(a). fc8, proj8, fc_grad and proj_grad
     as checkpointed_linear's weight8 and grad. fast: as fp8_mlp's, of x8 f8^T; what it says of the result holds for dproj, too."""
-    fc = _asking(fc, fc_grad, x, proj)
-    proj = _asking(proj, proj_grad, x, fc)
-    return _Mlp.apply(x, fc, proj, *(fc8 or _NOT_HELD), fc_grad, *(proj8 or _NOT_HELD), proj_grad, fast)
+    return _Mlp.apply(x, fc, proj, *(fc8 or _NOT_HELD), fc_grad, *(proj8 or _NOT_HELD), proj_grad, fast,
+                      _asking((fc_grad, proj_grad), (x, fc, proj)))

@@ -251,3 +251,17 @@ def test_a_buffer_of_a_layer_that_is_recorded_anyway(eager):
         y.backward(new(M, N))
         assert w.grad is None and (x.grad is not None) == x.requires_grad
     assert [args[13] for args in eager.named("nc_fp8_linear_bwd")] == [1, 1]
+
+
+@pytest.mark.parametrize("asked", ["x", "weight", "nothing"])
+def test_layers_trace_without_a_break(asked):
+    """With a buffer, whatever requires a gradient (on meta tensors, through the ops' fakes)."""
+    x = torch.empty(4, 256, dtype=BF16, device="meta", requires_grad=asked == "x")
+    w, p = (torch.empty(*s, device="meta", requires_grad=asked == "weight") for s in ((128, 256), (256, 128)))
+
+    def layers(x, buffer):
+        return fl.checkpointed_mlp(x, w, p, fc_grad=buffer) + fl.checkpointed_mlp(x, w, p, proj_grad=buffer.t().contiguous(), fast=True)
+
+    torch._dynamo.reset()
+    y = torch.compile(layers, fullgraph=True, backend="aot_eager")(x, torch.empty(128, 256, device="meta"))
+    assert y.requires_grad and y.shape == x.shape

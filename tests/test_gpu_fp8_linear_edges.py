@@ -47,6 +47,32 @@ def test_buffers_of_layers_without_a_gradient(device):
     fl.checkpointed_mlp(x, *asked[1:]).backward(dy)
     # the same sums, added to zeros
     assert all(torch.equal(b, t.grad) for b, t in zip(buffers, asked)) and all(t.grad is None for t in (w, fc, proj))
+    # captured, beside an eager call that has not been differentiated yet
+    waiting = fl.checkpointed_linear(x, w, grad=torch.zeros_like(w))
+    into, held_x, held_dy = [torch.zeros_like(t) for t in (w, fc, proj)], x.clone(), dy.clone()
+
+    def step():
+        for t in into:
+            t.zero_()
+        fl.checkpointed_linear(held_x, w, grad=into[0]).backward(held_dy)
+        fl.checkpointed_mlp(held_x, fc, proj, fc_grad=into[1], proj_grad=into[2]).backward(held_dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(3):
+        held_x.copy_(bf(gen, 70, 256).to(device))
+        graph.replay()
+        held_x.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(into, buffers))
+    waiting.backward(dy)
 
 
 def relu2_fast(codes, scale, w):
