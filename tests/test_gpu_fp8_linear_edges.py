@@ -7,6 +7,7 @@ import torch
 from nanochat_amd import fp8_linear as fl, native
 from nanochat_amd.native import hip_library, stream
 from oracle import fp8_block as fb
+from tests import test_gpu_fp8_linear as whole
 from tests.test_gpu_fp8_linear import EPS, SIZES, bf, close, codes_of, exps_of, form, held, product_relu2, product_relu2_bwd, same_form, weight
 
 pytestmark = pytest.mark.gpu
@@ -73,6 +74,22 @@ def test_buffers_of_layers_without_a_gradient(device):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(into, buffers))
     waiting.backward(dy)
+
+
+@pytest.mark.parametrize("rows,n,k", [(8190, 4352, 768), (12000, 2832, 1152)])
+def test_several_tiles_a_workgroup_write_nothing_else(device, rows, n, k):
+    whole.test_products_write_their_results_and_nothing_else(device, rows, n, k)
+    gen = torch.Generator().manual_seed(rows)
+    codes, scale, _ = form(gen, device, rows, k)
+    w, _ = weight(gen, device, n, k)
+    a8, a_s = relu2_fast(codes, scale, w)
+    out, exps = torch.full((rows + 600, n), 0xA5, dtype=torch.uint8, device=device), fl._new_scale(codes, rows, n)
+    native.check(hip_library().nc_fp8_matmul_relu2_fast(codes.data_ptr(), scale.data_ptr(), scale.stride(0), w.codes.data_ptr(),
+                                                        w.scale.data_ptr(), w.scale.stride(0), rows, n, k, out[300:].data_ptr(),
+                                                        exps.data_ptr(), exps.stride(0), stream()))
+    assert torch.equal(out[300:300 + rows], a8.view(torch.uint8))
+    out[300:300 + rows] = 0xA5
+    assert bool((out == 0xA5).all())
 
 
 def relu2_fast(codes, scale, w):
