@@ -359,6 +359,14 @@ def _address(t: Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _laid_out(scale: Tensor) -> Tensor:
+    """Saved scales of a weight held by the caller, whose rows' padding hooks on saved tensors may have left out."""
+    if scale.stride(0) % 4 == 0:
+        return scale
+    padded = torch.empty(scale.size(0), -(-scale.size(1) // 4) * 4, dtype=SCALE, device=scale.device)[:, :scale.size(1)]
+    return padded.copy_(scale)
+
+
 def _rows_of(x: Tensor) -> int:
     n = 1
     for d in x.shape[:-1]:
@@ -460,7 +468,8 @@ class _Linear(torch.autograd.Function):
             return (None,) * 8
         grad, need_x = ctx.grad, ctx.needs_input_grad[0]
         need_w = ctx.needs_input_grad[1] or grad is not None
-        dx, dw = _linear_bwd(dy, *ctx.saved_tensors, grad, need_x, need_w, ctx.wide)
+        x8, xs, codes_t, scale_t = ctx.saved_tensors
+        dx, dw = _linear_bwd(dy, x8, xs, codes_t, _laid_out(scale_t), grad, need_x, need_w, ctx.wide)
         return (dx.view(ctx.x_shape) if need_x else None, dw if need_w and grad is None else None, *(None,) * 6)
 
 
@@ -594,8 +603,9 @@ class _Mlp(torch.autograd.Function):
             return (None,) * 15
         fc_grad, proj_grad, need_x = ctx.fc_grad, ctx.proj_grad, ctx.needs_input_grad[0]
         need_fc, need_proj = ctx.needs_input_grad[1] or fc_grad is not None, ctx.needs_input_grad[2] or proj_grad is not None
-        dx, dfc, dproj = _mlp_bwd(dy, *ctx.saved_tensors, fc_grad, proj_grad, need_x, need_fc, need_proj, ctx.fc_wide,
-                                  ctx.proj_wide)
+        x8, xs, a8, a_s, f_t, f_ts, p_t, p_ts = ctx.saved_tensors
+        dx, dfc, dproj = _mlp_bwd(dy, x8, xs, a8, a_s, f_t, _laid_out(f_ts), p_t, _laid_out(p_ts), fc_grad, proj_grad, need_x,
+                                  need_fc, need_proj, ctx.fc_wide, ctx.proj_wide)
         return (dx.view(ctx.x_shape) if need_x else None, dfc if need_fc and fc_grad is None else None,
                 dproj if need_proj and proj_grad is None else None, *(None,) * 12)
 

@@ -265,3 +265,19 @@ def test_layers_trace_without_a_break(asked):
     torch._dynamo.reset()
     y = torch.compile(layers, fullgraph=True, backend="aot_eager")(x, torch.empty(128, 256, device="meta"))
     assert y.requires_grad and y.shape == x.shape
+
+
+def test_saved_tensors_that_hooks_lay_out_anew(eager):
+    """Tensors kept for the backward may come back contiguous, as from host memory: the scales of a weight held by the caller, views
+    of wider rows, then lack their padding."""
+    def held(n, k):
+        return fl.Fp8Weight(*form(n, k, 128, whole=False), *form(k, n, 128, whole=False))
+
+    x = new(M, K).requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t):
+        y = fl.checkpointed_linear(x, new(N, K), held(N, K)), fl.checkpointed_mlp(x, new(F, K), new(N, F), held(F, K), held(N, F))
+    for t in y:
+        t.backward(new(M, N))
+    linear, = eager.named("nc_fp8_linear_bwd")
+    mlp, = eager.named("nc_fp8_mlp_bwd")
+    assert linear[7] == 8 and (mlp[10], mlp[13]) == (8, 8)   # the pitches of 5 blocks

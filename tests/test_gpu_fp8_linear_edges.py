@@ -201,6 +201,23 @@ def test_square_roots_at_the_ends_of_the_range(device, rows, n, k, least, most):
     assert same_form(q[:40], q_s[:40], codes_of(dh[:40]), 1)
 
 
+def test_what_is_kept_may_wait_in_host_memory(device):
+    """Saved tensors that go to the host and come back, weights held by the caller among them."""
+    gen = torch.Generator().manual_seed(21)
+    x, dy = bf(gen, 70, 256).to(device).requires_grad_(), bf(gen, 70, 144).to(device)
+    w, fc, proj = ((torch.randn(*s, generator=gen) / 16).to(device).requires_grad_() for s in ((144, 256), (640, 256), (144, 640)))
+    held_w, held_fc, held_proj = (fl.quantize_weight(t.detach(), True) for t in (w, fc, proj))
+
+    def step():
+        y = fl.checkpointed_linear(x, w, held_w) + fl.checkpointed_mlp(x, fc, proj, held_fc, held_proj)
+        return y, (x, w, fc, proj)
+
+    want = torch.autograd.grad(*step(), dy)
+    with torch.autograd.graph.save_on_cpu():
+        out = step()
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(*out, dy)))
+
+
 # --- how exact the squares are
 
 def dropped(x, w):
